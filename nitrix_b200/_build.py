@@ -39,6 +39,10 @@ LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompil
 HOST_SOURCE = CSRC / "host" / "torch_ops.cpp"
 HOST_MODULE = "_torch_ops"
 HOST_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
+# The C++ library that torch itself runs on, whatever the compiler would link by itself: a copy of its own inside the module (a
+# toolchain without the shared library links the archive) shares locales with torch's, and printing a number into an error's
+# text then crashes.
+HOST_RUNTIME = ["-nostdlib++", "-l:libstdc++.so.6"]
 
 
 def sources() -> list[pathlib.Path]:
@@ -92,7 +96,7 @@ def host_module_runtime() -> str:
 
 
 def _host_digest() -> str:
-    h = hashlib.sha256(" ".join([*HOST_FLAGS, host_runtime()]).encode())
+    h = hashlib.sha256(" ".join([*HOST_FLAGS, *HOST_RUNTIME, host_runtime()]).encode())
     for f in [HOST_SOURCE, *sorted(INCLUDE.glob("*.h"))]:
         h.update(f.read_bytes())
     return h.hexdigest()
@@ -117,7 +121,7 @@ def _compile_host() -> None:
     tmp = LIBDIR / (HOST_MODULE + ".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), *HOST_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-I{d}" for d in includes), str(HOST_SOURCE), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda",
-           "-ltorch_cpu", "-ltorch_python"]
+           "-ltorch_cpu", "-ltorch_python", *HOST_RUNTIME]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("host compiler failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)

@@ -534,3 +534,12 @@ def test_the_library_is_linked_where_the_host_module_does_not_compile(monkeypatc
     with pytest.raises(RuntimeError, match="host compiler failed"):
         _build.build()
     assert C.CDLL(str(_build.lib_path())).one() == 1
+
+
+def test_the_host_module_has_no_cxx_library_of_its_own():
+    """A second copy of it made numbers in error texts crash: the module must name the shared one and define none of it."""
+    from nitrix_b200 import _build
+
+    image = _build.host_module_path().read_bytes()
+    assert b"libstdc++.so.6\0" in image
+    assert b"St12codecvt_byname" not in image
