@@ -115,6 +115,17 @@ EXPORTS = (
     "nb200_selective_scan_workspace_bytes",
     "nb200_selective_scan_workspace_least_bytes",
     "nb200_selective_scan_checkpoint_bytes",
+    "nb200_rotary",
+    "nb200_cache_append",
+    "nb200_cache_fork",
+    "nb200_cache_compact",
+    "nb200_cache_workspace_bytes",
+    "nb200_decode",
+    "nb200_decode_workspace_bytes",
+    "nb200_packed_fwd",
+    "nb200_packed_bwd",
+    "nb200_packed_workspace_bytes",
+    "nb200_packed_plan",
 )
 
 

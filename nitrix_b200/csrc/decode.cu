@@ -1,0 +1,656 @@
+// Attention of one new token per sequence over the paged cache, split over the sequences' lengths and joined.
+//
+//   s_t = scale q . k_t,  p = softmax(s),  out = sum_t p_t v_t       for every query head, t < length of its sequence
+//
+// Bound by HBM: every kept key and value is read once, by the CTA that serves all query heads of its key head, and with G
+// query heads per key head a byte of the cache takes G multiply-adds.  The lengths are known on the device only, and the grid
+// is the same whatever they are: the tokens of all (sequence, key head) items, in units, are dealt in equal contiguous shares
+// to as many CTAs as the GPU holds, so that one long sequence, many short ones and any mix end together.  A CTA's share is a
+// run of pieces of items; a piece that is a whole item is finished on the spot, one that is not leaves its maximum, sum and
+// unnormalised output (fp32) in the workspace: at most two per CTA, the share's first and last.  decode_join_kernel adds up
+// those pieces, in order.
+//
+// Two inner loops:
+//  * 16-bit operands, head dim 64 or 128: warp-level MMAs on operands that go from global memory straight into registers, no
+//    shared memory and no barrier in the loop.  Keys are the M side (S^T = K Q^T, O^T = V^T P^T), so that up to 8 query heads
+//    are one N = 8 tile and nothing is wasted on padding to 16.  The order of the head dim inside a product is free, so a
+//    lane's 16-byte words of K serve as the fragments of two steps; V's fragments pair two keys of one element, which is one
+//    byte permutation of words loaded from the two keys' rows.  P^T goes from accumulator to operand layout by movmatrix.
+//  * anything else: fp32 multiply-adds, lanes along the head dim, a reduce-scatter of the query heads' sums.
+#include <math.h>
+
+#include "nitrix_b200_cache.h"
+#include "sdpa_tc_common.cuh"
+
+namespace nb200 {
+namespace {
+
+using tc::ex2;
+using tc::pack2;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+
+struct DecodeArgs {
+  const void* k;
+  const void* v;
+  int64_t ks[3], vs[3];      // elements, over (page, head, slot)
+  int pages, kv_heads, page_size, page_shift;   // page_shift: log2 of page_size, or -1
+  int D;
+  const int* table;
+  const int* lengths;
+  int rows, width;
+  const void* q;
+  int64_t qs[2];
+  void* out;
+  int q_heads, group;        // query heads, and those of one key head
+  int chunks;                // runs of query heads that a key head's group is taken in
+  float mul;                 // scale * log2 e
+  int unit;                  // tokens per unit of work
+  float* part;               // pieces: [2 * CTAs][heads of a chunk][D + 2]: output, maximum (base 2), sum
+  int workers;               // most CTAs of the main kernel that get work
+};
+
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int row) {
+  return int(min(int64_t(max(a.lengths[row], 0)), int64_t(a.width) * a.page_size));
+}
+__device__ __forceinline__ int units_of(const DecodeArgs& a, int row) { return (length_of(a, row) + a.unit - 1) / a.unit; }
+
+// Work position: units of all rows times (key head, chunk), row-major.  All lanes of a warp hold the same values.
+struct Share {
+  int64_t total;             // units of work
+  int workers;               // with a unit at least
+  __device__ __forceinline__ Share(const DecodeArgs& a, int64_t units) : total(units), workers(int(min(int64_t(a.workers), units))) {}
+  __device__ __forceinline__ int64_t begin(int worker) const { return total * worker / workers; }
+  // the worker whose share holds position u < total
+  __device__ __forceinline__ int worker_of(int64_t u) const {
+    int w = int(u * workers / total);
+    while (begin(w + 1) <= u) ++w;        // (begin rounds down, so that the estimate may be one short)
+    return w;
+  }
+};
+
+__device__ __forceinline__ Share share_of(const DecodeArgs& a, int lane) {
+  int64_t units = 0;
+  for (int i = lane; i < a.rows; i += 32) units += units_of(a, i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+  return Share(a, units * a.kv_heads * a.chunks);
+}
+
+// the row that position u < total lies in, and the position of its first unit
+__device__ __forceinline__ void find_row(const DecodeArgs& a, int lane, int64_t u, int* row, int64_t* row_begin) {
+  const int per = a.kv_heads * a.chunks;
+  int64_t before = 0;
+  for (int row0 = 0; row0 < a.rows; row0 += 32) {
+    int64_t upto = row0 + lane < a.rows ? int64_t(units_of(a, row0 + lane)) * per : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    const unsigned above = __ballot_sync(0xffffffffu, before + upto > u);
+    if (above) {
+      const int j = __ffs(above) - 1;
+      const int64_t prev = __shfl_sync(0xffffffffu, upto, j > 0 ? j - 1 : 0);
+      *row = row0 + j;
+      *row_begin = before + (j > 0 ? prev : 0);
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  *row = a.rows;
+  *row_begin = before;
+}
+
+// Element offsets of a token's row, of a head at `head_off`; the page is checked.
+__device__ __forceinline__ int page_of(const DecodeArgs& a, const int* row_table, int token, int* slot) {
+  const int column = a.page_shift >= 0 ? token >> a.page_shift : token / a.page_size;
+  *slot = token - (a.page_shift >= 0 ? column << a.page_shift : column * a.page_size);
+  const int page = __ldg(row_table + column);
+  return min(max(page, 0), a.pages - 1);
+}
+
+// ---- warp-level MMA ------------------------------------------------------------------------------------------------------
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// One warp's part of a piece: blocks of 16 tokens `warp`, `warp + kWarps`, ... of [t0, t1) of a sequence.
+template <int D, int kTiles, bool kBf16>
+struct MmaLoop {
+  static constexpr int kHeads = 8 * kTiles;      // query heads of a chunk
+  static constexpr int kBlock = 16;              // tokens
+  static constexpr int kSlots = kWarps;          // partial results of a CTA
+  static constexpr int kMinCtas = kTiles == 1 ? 4 : 2;
+  float o[kTiles][D / 16][4];                    // O^T: lane (g, t): head 2t (+1), see store
+  float m[kTiles][2], l[kTiles][2];              // of heads 2t, 2t + 1; l: this lane's keys
+
+  __device__ __forceinline__ void run(const DecodeArgs& a, const int* row_table, int kv_head, const void* q_row, int heads,
+                                      int t0, int t1) {
+    const uint16_t* q = static_cast<const uint16_t*>(q_row);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + kv_head * a.ks[1];
+    const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + kv_head * a.vs[1];
+    uint4 qf[kTiles][D / 32];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        qf[n][i] = n * 8 + g < heads ? *reinterpret_cast<const uint4*>(q + (n * 8 + g) * a.qs[1] + (i * 4 + t) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    const int last = t1 - 1;
+    uint4 kf[2][D / 32], vf[4][D / 64];
+    auto load_k = [&](int b0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        int slot;
+        const int64_t page = page_of(a, row_table, min(b0 + g + 8 * r, last), &slot);
+        const uint16_t* row = kbase + page * a.ks[0] + slot * a.ks[2];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) kf[r][i] = sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(row + (i * 4 + t) * 8));
+      }
+    };
+    auto load_v = [&](int b0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        int slot;
+        const int64_t page = page_of(a, row_table, min(b0 + 2 * t + (r & 1) + (r >> 1) * 8, last), &slot);
+        const uint16_t* row = vbase + page * a.vs[0] + slot * a.vs[2];
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) vf[r][i] = sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(row + i * 64 + g * 8));
+      }
+    };
+    int b0 = t0 + warp * kBlock;
+    if (b0 >= t1) return;
+    load_k(b0);
+    load_v(b0);
+    const float thr = a.mul > 0.f ? 8.f / a.mul : INFINITY;
+    for (; b0 < t1; b0 += kWarps * kBlock) {
+      const int next = b0 + kWarps * kBlock;
+      float s[kTiles][4];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          mma16816<kBf16>(s[n], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[n][i].x, qf[n][i].y);
+          mma16816<kBf16>(s[n], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[n][i].z, qf[n][i].w);
+        }
+      if (next < t1) load_k(next);      // (the keys are used: their registers take the next block's)
+      uint32_t pt[kTiles][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        if (b0 + g >= t1) s[n][0] = s[n][1] = -INFINITY;
+        if (b0 + g + 8 >= t1) s[n][2] = s[n][3] = -INFINITY;
+        // The reference maximum moves only when a score passes it by more than 2^8 (p <= 256; sums and outputs are fp32).
+        const float mx0 = fmaxf(s[n][0], s[n][2]), mx1 = fmaxf(s[n][1], s[n][3]);
+        if (__any_sync(0xffffffffu, mx0 > m[n][0] + thr || mx1 > m[n][1] + thr)) {
+          float x0 = mx0, x1 = mx1;
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+          }
+          x0 = fmaxf(x0, m[n][0]);
+          x1 = fmaxf(x1, m[n][1]);
+          const float c0 = x0 > m[n][0] ? ex2((m[n][0] - x0) * a.mul) : 1.f, c1 = x1 > m[n][1] ? ex2((m[n][1] - x1) * a.mul) : 1.f;
+          m[n][0] = x0;
+          m[n][1] = x1;
+          l[n][0] *= c0;
+          l[n][1] *= c1;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][0] *= c0; o[n][i][1] *= c1; o[n][i][2] *= c0; o[n][i][3] *= c1;
+          }
+        }
+        const float n0 = m[n][0] == -INFINITY ? 0.f : -m[n][0] * a.mul, n1 = m[n][1] == -INFINITY ? 0.f : -m[n][1] * a.mul;
+        const float p0 = ex2(fmaf(s[n][0], a.mul, n0)), p1 = ex2(fmaf(s[n][1], a.mul, n1));
+        const float p2 = ex2(fmaf(s[n][2], a.mul, n0)), p3 = ex2(fmaf(s[n][3], a.mul, n1));
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+        pt[n][0] = transpose8x8(pack2<kBf16>(p0, p1));
+        pt[n][1] = transpose8x8(pack2<kBf16>(p2, p3));
+      }
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const uint32_t* w[4] = {&vf[0][i].x, &vf[1][i].x, &vf[2][i].x, &vf[3][i].x};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {      // elements i * 64 + g * 8 + 2 e, + 1
+          const uint32_t a0 = __byte_perm(w[0][e], w[1][e], 0x5410), a1 = __byte_perm(w[0][e], w[1][e], 0x7632);
+          const uint32_t a2 = __byte_perm(w[2][e], w[3][e], 0x5410), a3 = __byte_perm(w[2][e], w[3][e], 0x7632);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) mma16816<kBf16>(o[n][i * 4 + e], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+        }
+      }
+      if (next < t1) load_v(next);
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
+        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
+      }
+  }
+
+  // output, maximum (base 2) and sum of this warp's part: [head][D + 2] floats
+  __device__ __forceinline__ void store(const DecodeArgs& a, float* dst) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float* slot = dst + (threadIdx.x >> 5) * kHeads * (D + 2);
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float* row = slot + (n * 8 + 2 * t + hh) * (D + 2);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          *reinterpret_cast<float2*>(row + (i / 4) * 64 + g * 8 + 2 * (i & 3)) = make_float2(o[n][i][hh], o[n][i][2 + hh]);
+        if (g == 0) {
+          row[D] = m[n][hh] == -INFINITY ? -INFINITY : m[n][hh] * a.mul;
+          row[D + 1] = l[n][hh];
+        }
+      }
+  }
+};
+
+// ---- fp32 multiply-adds ----------------------------------------------------------------------------------------------------
+// kLanes lanes share a token's row, kPer 16-byte words each; 8 query heads.  A warp's 32 / kLanes groups take tokens of their own.
+template <typename T, int kLanes, int kPer>
+struct FmaLoop {
+  static constexpr int kHeads = 8;
+  static constexpr int kVec = 16 / int(sizeof(T));
+  static constexpr int kGroups = kThreads / kLanes;
+  static constexpr int kSlots = kGroups;
+  static constexpr int kAhead = 2;
+  static constexpr int kMinCtas = 2;
+  float o[kHeads][kPer][kVec];
+  float m, l;             // of the head that the reduce-scatter leaves in this lane
+
+  __device__ __forceinline__ static int my_head(int c) {   // bits of the lane, high to low: the reduce-scatter's choices
+    return ((c & (kLanes / 2)) ? 4 : 0) + ((c & (kLanes / 4)) ? 2 : 0) + ((c & (kLanes / 8)) ? 1 : 0);
+  }
+  // the lane (of a group) that holds head h
+  __device__ __forceinline__ static int lane_of(int h) {
+    return ((h & 4) ? kLanes / 2 : 0) + ((h & 2) ? kLanes / 4 : 0) + ((h & 1) ? kLanes / 8 : 0);
+  }
+
+  __device__ __forceinline__ void run(const DecodeArgs& a, const int* row_table, int kv_head, const T* q, int heads, int t0, int t1) {
+    const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes, lane = threadIdx.x & 31;
+    const int words = a.D / kVec;
+    float qf[kHeads][kPer][kVec];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const bool in = h < heads && c + p * kLanes < words;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          qf[h][p][e] = in ? to_f32<T>(q[h * a.qs[1] + (c + p * kLanes) * kVec + e]) : 0.f;
+          o[h][p][e] = 0.f;
+        }
+      }
+    m = -INFINITY;
+    l = 0.f;
+    const T* kbase = static_cast<const T*>(a.k) + kv_head * a.ks[1];
+    const T* vbase = static_cast<const T*>(a.v) + kv_head * a.vs[1];
+    const int last = t1 - 1;
+    // (every group of a warp makes as many turns as its first, which has the most: the shuffles below are warp-wide)
+    const int first_group = group - (group % (32 / kLanes));
+    for (int b = t0; b + first_group < t1; b += kGroups * kAhead) {
+      uint4 kw[kAhead][kPer], vw[kAhead][kPer];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        int slot;
+        const int64_t page = page_of(a, row_table, min(b + group + j * kGroups, last), &slot);
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) {
+          const bool in = c + p * kLanes < words;
+          kw[j][p] = in ? sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(kbase + page * a.ks[0] + slot * a.ks[2]) + c + p * kLanes) : make_uint4(0, 0, 0, 0);
+          vw[j][p] = in ? sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(vbase + page * a.vs[0] + slot * a.vs[2]) + c + p * kLanes) : make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        float s[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          s[h] = 0.f;
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) {
+            const T* e = reinterpret_cast<const T*>(&kw[j][p]);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) s[h] = fmaf(qf[h][p][i], to_f32<T>(e[i]), s[h]);
+          }
+        }
+        // reduce-scatter: every step halves the heads that a lane still sums
+#pragma unroll
+        for (int step = 0; step < 3; ++step) {
+          const int off = kLanes >> (step + 1), n = 4 >> step;
+          const bool upper = (c & off) != 0;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            if (h >= n) continue;
+            const float keep = upper ? s[h + n] : s[h], send = upper ? s[h] : s[h + n];
+            s[h] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+          }
+        }
+#pragma unroll
+        for (int off = kLanes / 16; off > 0; off >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+        float x = s[0] * a.mul;
+        if (b + group + j * kGroups >= t1) x = -INFINITY;
+        const float m_new = fmaxf(m, x);
+        const float shift = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = ex2(m - shift), pr = ex2(x - shift);
+        l = l * alpha + pr;
+        const bool moved = __any_sync(0xffffffffu, m_new > m);
+        m = m_new;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const int from = (lane & ~(kLanes - 1)) + lane_of(h);
+          const float ph = __shfl_sync(0xffffffffu, pr, from);
+          if (moved) {
+            const float ah = __shfl_sync(0xffffffffu, alpha, from);
+#pragma unroll
+            for (int p = 0; p < kPer; ++p)
+#pragma unroll
+              for (int i = 0; i < kVec; ++i) o[h][p][i] *= ah;
+          }
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) {
+            const T* e = reinterpret_cast<const T*>(&vw[j][p]);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) o[h][p][i] = fmaf(ph, to_f32<T>(e[i]), o[h][p][i]);
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const DecodeArgs& a, float* dst) const {
+    const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    float* slot = dst + group * kHeads * (a.D + 2);
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p)
+        if (c + p * kLanes < a.D / kVec)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) slot[h * (a.D + 2) + (c + p * kLanes) * kVec + e] = o[h][p][e];
+    if ((c & (kLanes / 8 - 1)) == 0) {
+      float* row = slot + my_head(c) * (a.D + 2);
+      row[a.D] = m;
+      row[a.D + 1] = l;
+    }
+  }
+};
+
+template <typename T, typename Loop>
+__global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const DecodeArgs a) {
+  extern __shared__ float merge[];      // [slot][head][D + 2]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const Share share = share_of(a, lane);
+  if (int(blockIdx.x) >= share.workers) return;
+  int64_t u = share.begin(blockIdx.x);
+  const int64_t u_end = share.begin(blockIdx.x + 1);
+  const int per = a.kv_heads * a.chunks;
+  int row;
+  int64_t row_begin;
+  find_row(a, lane, u, &row, &row_begin);
+  while (u < u_end) {
+    const int length = length_of(a, row);
+    const int units = (length + a.unit - 1) / a.unit;
+    if (units == 0) { ++row; continue; }
+    const int item = int((u - row_begin) / units);
+    const int64_t item_begin = row_begin + int64_t(item) * units;
+    const int kv_head = item / a.chunks, chunk = item - kv_head * a.chunks;
+    const int ub = int(u - item_begin), ue = int(min(int64_t(units), u_end - item_begin));
+    const int head0 = kv_head * a.group + chunk * Loop::kHeads;
+    const int heads = min(Loop::kHeads, a.group - chunk * Loop::kHeads);
+    const bool whole = ub == 0 && ue == units;
+    {
+      Loop loop;
+      const int t0 = ub * a.unit, t1 = min(length, ue * a.unit);
+      const T* q = static_cast<const T*>(a.q) + row * a.qs[0] + head0 * a.qs[1];
+      loop.run(a, a.table + int64_t(row) * a.width, kv_head, q, heads, t0, t1);
+      loop.store(a, merge);
+    }
+    __syncthreads();
+    // the CTA's result: sums over the slots, relative to their largest maximum
+    float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * Loop::kHeads * (a.D + 2);
+    for (int i = threadIdx.x; i < heads * a.D; i += kThreads) {
+      const int h = i / a.D, d = i - h * a.D;
+      const float* col = merge + h * (a.D + 2);
+      const int step = Loop::kHeads * (a.D + 2);
+      float mx = -INFINITY;
+      for (int s = 0; s < Loop::kSlots; ++s) mx = fmaxf(mx, col[s * step + a.D]);
+      const float shift = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f, acc = 0.f;
+      for (int s = 0; s < Loop::kSlots; ++s) {
+        const float w = ex2(col[s * step + a.D] - shift);
+        sum = fmaf(w, col[s * step + a.D + 1], sum);
+        acc = fmaf(w, col[s * step + d], acc);
+      }
+      if (whole) {
+        static_cast<T*>(a.out)[(int64_t(row) * a.q_heads + head0 + h) * a.D + d] = from_f32<T>(acc / sum);
+      } else {
+        part[h * (a.D + 2) + d] = acc;
+        if (d == 0) {
+          part[h * (a.D + 2) + a.D] = mx;
+          part[h * (a.D + 2) + a.D + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    u += ue - ub;
+    if (u == row_begin + int64_t(units) * per) { row_begin = u; ++row; }
+  }
+}
+
+// One CTA per (row, query head): the pieces of its item, in order; zeros for a sequence without a token.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a, int heads_per_chunk) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.y, head = blockIdx.x;
+  T* out = static_cast<T*>(a.out) + (int64_t(row) * a.q_heads + head) * a.D;
+  const int units = units_of(a, row);
+  if (units == 0) {
+    for (int d = threadIdx.x; d < a.D; d += kThreads) out[d] = from_f32<T>(0.f);
+    return;
+  }
+  const int per = a.kv_heads * a.chunks;
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < a.rows; i += 32) {
+    const int64_t n = int64_t(units_of(a, i)) * per;
+    total += n;
+    if (i < row) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const Share share(a, total);
+  const int kv_head = head / a.group, in_group = head - kv_head * a.group;
+  const int chunk = in_group / heads_per_chunk, h = in_group - chunk * heads_per_chunk;
+  const int64_t begin = before + int64_t(kv_head * a.chunks + chunk) * units;
+  const int w0 = share.worker_of(begin), w1 = share.worker_of(begin + units - 1);
+  if (w0 == w1) return;                  // finished by the CTA that had all of it
+  const int64_t step = int64_t(heads_per_chunk) * (a.D + 2);
+  // the first piece begins the item (slot 1 of its worker); the others begin inside it (slot 0)
+  auto piece = [&](int w) { return a.part + (2 * int64_t(w) + (w == w0 ? 1 : 0)) * step + h * (a.D + 2); };
+  float mx = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, piece(w)[a.D]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float shift = mx == -INFINITY ? 0.f : mx;
+  for (int d = threadIdx.x; d < a.D; d += kThreads) {
+    float sum = 0.f, acc = 0.f;
+    for (int w = w0; w <= w1; ++w) {
+      const float* p = piece(w);
+      const float f = ex2(p[a.D] - shift);
+      sum = fmaf(f, p[a.D + 1], sum);
+      acc = fmaf(f, p[d], acc);
+    }
+    out[d] = from_f32<T>(acc / sum);
+  }
+}
+
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// What a call runs as, which the size of its workspace depends on.
+struct Plan {
+  bool mma;
+  int heads;       // query heads of a chunk
+  int unit, workers;
+  size_t bytes;
+};
+
+int check(const nb200_decode_params* p, const char* what) {
+  if (!p || p->struct_size != sizeof(nb200_decode_params)) { set_error("%s: NULL params or wrong struct_size", what); return NB200_ERR_INVALID; }
+  const nb200_cache_pages& c = p->pages;
+  if (c.dtype != NB200_F32 && c.dtype != NB200_BF16 && c.dtype != NB200_F16) { set_error("%s: bad dtype", what); return NB200_ERR_INVALID; }
+  if (c.pages < 0 || c.heads <= 0 || c.page_size <= 0 || c.head_dim <= 0 || p->rows < 0 || p->width < 0 || p->q_heads <= 0) {
+    set_error("%s: bad extents", what);
+    return NB200_ERR_INVALID;
+  }
+  if (p->q_heads % c.heads) { set_error("%s: %d query heads are no multiple of %d key heads", what, p->q_heads, c.heads); return NB200_ERR_INVALID; }
+  const int vec = c.dtype == NB200_F32 ? 4 : 8;
+  if (c.head_dim % vec || c.head_dim > 256) {
+    set_error("%s: head dim %d must be a multiple of %d and at most 256", what, c.head_dim, vec);
+    return NB200_ERR_UNSUPPORTED;
+  }
+  if (p->rows > 65535) { set_error("%s: %d sequences, at most 65535", what, p->rows); return NB200_ERR_UNSUPPORTED; }
+  return NB200_OK;
+}
+
+Plan plan(const nb200_decode_params* p) {
+  const nb200_cache_pages& c = p->pages;
+  Plan pl{};
+  const int group = p->q_heads / c.heads;
+  bool q_words = aligned16(p->q);
+  for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
+  pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words && p->scale > 0.f;
+  pl.heads = pl.mma && group > 8 ? 16 : 8;
+  pl.unit = 64;
+  const int ctas = pl.mma && pl.heads == 8 ? 4 : 2;      // resident per SM (the kernels' launch bounds)
+  const int chunks = (group + pl.heads - 1) / pl.heads;
+  const int64_t units = (int64_t(p->width) * c.page_size + pl.unit - 1) / pl.unit * p->rows * c.heads * chunks;
+  const int64_t most = int64_t(tc::sm_count()) * ctas;
+  pl.workers = int(units < most ? (units > 0 ? units : 1) : most);
+  pl.bytes = size_t(pl.workers) * 2 * pl.heads * (c.head_dim + 2) * sizeof(float);
+  return pl;
+}
+
+template <typename T, typename Loop>
+int launch(const DecodeArgs& a, cudaStream_t st) {
+  const size_t smem = size_t(Loop::kSlots) * Loop::kHeads * (a.D + 2) * sizeof(float);
+  decode_kernel<T, Loop><<<unsigned(a.workers), kThreads, smem, st>>>(a);
+  count_launch();
+  if (int rc = check_launch("decode_kernel")) return rc;
+  // the joining CTAs may be set up while the main kernel runs; they wait for its end before they read anything it wrote
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(a.q_heads), unsigned(a.rows));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, decode_join_kernel<T>, a, int(Loop::kHeads)) != cudaSuccess) return check_launch("decode_join_kernel");
+  count_launch();
+  return check_launch("decode_join_kernel");
+}
+
+template <typename T>
+int launch_fma(const DecodeArgs& a, cudaStream_t st) {
+  const int words = a.D / (16 / int(sizeof(T)));
+  if (words <= 8) return launch<T, FmaLoop<T, 8, 1>>(a, st);
+  if (words <= 16) return launch<T, FmaLoop<T, 16, 1>>(a, st);
+  if constexpr (sizeof(T) == 4) {
+    if (words > 32) return launch<T, FmaLoop<T, 32, 2>>(a, st);
+  }
+  return launch<T, FmaLoop<T, 32, 1>>(a, st);      // (16-bit heads of 256 are 32 words)
+}
+
+template <typename T, bool kBf16>
+int launch_mma(const DecodeArgs& a, int heads, cudaStream_t st) {
+  if (a.D == 64) return heads == 8 ? launch<T, MmaLoop<64, 1, kBf16>>(a, st) : launch<T, MmaLoop<64, 2, kBf16>>(a, st);
+  return heads == 8 ? launch<T, MmaLoop<128, 1, kBf16>>(a, st) : launch<T, MmaLoop<128, 2, kBf16>>(a, st);
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" NB200_API int nb200_decode_workspace_bytes(const nb200_decode_params* p, size_t* bytes) {
+  if (!bytes) { set_error("bytes out-pointer is NULL"); return NB200_ERR_INVALID; }
+  if (int rc = check(p, "decode_workspace_bytes")) return rc;
+  *bytes = plan(p).bytes;
+  return NB200_OK;
+}
+
+extern "C" NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_stream) {
+  if (int rc = check(p, "decode")) return rc;
+  if (p->rows == 0) return NB200_OK;
+  const nb200_cache_pages& c = p->pages;
+  if (!p->q || !p->out || !p->lengths || (p->width && !p->table) || (c.pages && (!c.k || !c.v))) { set_error("decode: NULL operand"); return NB200_ERR_INVALID; }
+  const int vec = c.dtype == NB200_F32 ? 4 : 8;
+  bool ok = aligned16(c.k) && aligned16(c.v);
+  for (int i = 0; i < 3; ++i) ok = ok && c.k_stride[i] % vec == 0 && c.v_stride[i] % vec == 0;
+  if (!ok) { set_error("decode: the rows of the pages must begin on 16-byte boundaries"); return NB200_ERR_ALIGNMENT; }
+  const Plan pl = plan(p);
+  if (!p->workspace || p->workspace_bytes < pl.bytes) {
+    set_error("decode: workspace of %zu bytes needed (nb200_decode_workspace_bytes), %zu given", pl.bytes, p->workspace_bytes);
+    return NB200_ERR_WORKSPACE;
+  }
+  DecodeArgs a{};
+  a.k = c.k; a.v = c.v;
+  for (int i = 0; i < 3; ++i) { a.ks[i] = c.k_stride[i]; a.vs[i] = c.v_stride[i]; }
+  a.pages = c.pages; a.kv_heads = c.heads; a.page_size = c.page_size; a.D = c.head_dim;
+  a.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (c.page_size == 1 << s) a.page_shift = s;
+  a.table = p->table; a.lengths = p->lengths; a.rows = p->rows;
+  a.width = c.pages ? p->width : 0;      // (without pages every sequence is empty)
+  a.q = p->q; a.qs[0] = p->q_stride[0]; a.qs[1] = p->q_stride[1];
+  a.out = p->out;
+  a.q_heads = p->q_heads; a.group = p->q_heads / c.heads;
+  a.chunks = (a.group + pl.heads - 1) / pl.heads;
+  a.mul = p->scale * kLog2e;
+  a.unit = pl.unit;
+  a.part = static_cast<float*>(p->workspace);
+  a.workers = pl.workers;
+  cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+  prof_call_begin(st);
+  if (c.dtype == NB200_F32) return launch_fma<float>(a, st);
+  if (c.dtype == NB200_BF16) return pl.mma ? launch_mma<__nv_bfloat16, true>(a, pl.heads, st) : launch_fma<__nv_bfloat16>(a, st);
+  return pl.mma ? launch_mma<__half, false>(a, pl.heads, st) : launch_fma<__half>(a, st);
+}

@@ -16,7 +16,10 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "nitrix_b200_attention.h"
+#include "nitrix_b200_cache.h"
 #include "nitrix_b200_norm.h"
+#include "nitrix_b200_packed.h"
+#include "nitrix_b200_rotary.h"
 #include "nitrix_b200_scan.h"
 
 namespace {
@@ -31,7 +34,9 @@ using MaybeTensor = std::optional<Tensor>;
   X(nb200_sdpa_fwd) X(nb200_sdpa_bwd) X(nb200_mask_pack_bytes) X(nb200_mask_pack) X(nb200_qk_rms_norm)                     \
   X(nb200_qk_rms_norm_grad) X(nb200_layer_norm_fwd) X(nb200_layer_norm_bwd) X(nb200_layer_norm_workspace_bytes)            \
   X(nb200_selective_scan_fwd) X(nb200_selective_scan_bwd) X(nb200_selective_scan_checkpoint_bytes)                         \
-  X(nb200_selective_scan_workspace_bytes)
+  X(nb200_selective_scan_workspace_bytes) X(nb200_rotary) X(nb200_cache_append) X(nb200_cache_fork) X(nb200_cache_compact)  \
+  X(nb200_cache_workspace_bytes) X(nb200_decode) X(nb200_decode_workspace_bytes) X(nb200_packed_plan) X(nb200_packed_fwd)  \
+  X(nb200_packed_bwd) X(nb200_packed_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -550,6 +555,419 @@ Tensor selective_scan(const Tensor& x, const Tensor& delta, const Tensor& A, con
   return ScanRule::apply(x, delta, A, B, C, D, differentiate);
 }
 
+// ---- checks that the operators of a decoder layer share --------------------------------------------------------------------
+void check_float(const char* what, const char* name, const Tensor& t) {
+  TORCH_CHECK_TYPE(t.is_cuda() && dtype_code(t.scalar_type()) >= 0, what, ": ", name, " must be a CUDA tensor of float32, bfloat16 or float16; got ",
+                   t.scalar_type(), " on ", t.device());
+}
+void check_ints(const char* what, const char* name, const Tensor& t, const Tensor& like, int64_t dims) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt && t.device() == like.device(), what, ": ", name, " must be int32 on ", like.device(), "; got ",
+                   t.scalar_type(), " on ", t.device());
+  TORCH_CHECK_VALUE(t.dim() == dims, what, ": ", name, " must have ", dims, " axes; got shape ", t.sizes());
+}
+// rows along the last axis that begin on 16-byte boundaries, none of them shared
+Tensor aligned_rows(const Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && !has_expanded_axis(t);
+  for (int64_t a = 0; a + 1 < t.dim(); ++a) ok = ok && t.stride(a) * int64_t(t.element_size()) % 16 == 0;
+  if (ok) return t;
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+// ---- rotary positions -------------------------------------------------------------------------------------------------------
+// x (..., heads, D) as (B, S, heads, D); the result is dense
+void rotary_operand(nb200_rotary_tensor& t, const Tensor& x4, const Tensor& y) {
+  t.x = x4.data_ptr();
+  t.y = y.data_ptr();
+  for (int a = 0; a < 3; ++a) t.x_stride[a] = x4.stride(a);
+  t.heads = int32_t(x4.size(2));
+}
+Tensor two_leading_axes(const Tensor& x) {
+  const Tensor r = x.stride(-1) == 1 ? x : x.contiguous();
+  if (r.dim() == 4) return r;
+  if (r.dim() == 3) return r.unsqueeze(0);
+  return r.reshape({1, -1, r.size(-2), r.size(-1)});
+}
+
+tensor_list rotate(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& frequencies, at::IntArrayRef sections,
+                   bool interleaved, bool inverse) {
+  const Tensor& any = q.defined() ? q : k;
+  nb200_rotary_params p{};
+  p.struct_size = sizeof(p);
+  tensor_list out(2);
+  Tensor held[2];
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& x = i ? k : q;
+    if (!x.defined()) continue;
+    out[i] = at::empty(x.sizes(), x.options());
+    held[i] = two_leading_axes(x);
+    rotary_operand(i ? p.k : p.q, held[i], out[i]);
+    p.batch = int32_t(held[i].size(0));
+    p.length = int32_t(held[i].size(1));
+  }
+  if (p.batch == 0 || p.length == 0) return out;
+  p.positions = positions.data_ptr();
+  p.frequencies = frequencies.data_ptr<float>();
+  p.head_dim = int32_t(any.size(-1));
+  p.axes = int32_t(sections.size());
+  for (size_t a = 0; a < sections.size(); ++a) p.sections[a] = int32_t(sections[a]);
+  p.position_dtype = positions.scalar_type() == at::kInt ? NB200_POS_I32 : positions.scalar_type() == at::kLong ? NB200_POS_I64 : NB200_POS_F32;
+  p.dtype = dtype_code(any.scalar_type());
+  p.interleaved = interleaved;
+  p.inverse = inverse;
+  check(lib.nb200_rotary(&p, stream_of(any)), "nb200_rotary");
+  return out;
+}
+
+// Saves the positions and frequencies; the gradient turns back.
+struct RotaryRule : torch::autograd::Function<RotaryRule> {
+  static tensor_list forward(AutogradContext* ctx, const Tensor& q, const MaybeTensor& k, const Tensor& positions, const Tensor& frequencies,
+                             std::vector<int64_t> sections, bool interleaved) {
+    tensor_list out = rotate(q, k.value_or(Tensor()), positions, frequencies, sections, interleaved, false);
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->set_materialize_grads(false);
+    if (!k) out.pop_back();
+    return out;
+  }
+  static tensor_list backward(AutogradContext* ctx, const tensor_list& grads) {
+    const Tensor gq = grads[0], gk = grads.size() > 1 ? grads[1] : Tensor();
+    tensor_list d(6);
+    if (!gq.defined() && !gk.defined()) return d;
+    const auto s = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    const tensor_list r = rotate(gq, gk, s[0], s[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
+    d[0] = r[0];
+    d[1] = r[1];
+    return d;
+  }
+};
+
+std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, const Tensor& positions, const Tensor& frequencies,
+                                       std::vector<int64_t> sections, bool interleaved) {
+  const char* what = "rotary_embedding";
+  check_float(what, "q", q);
+  TORCH_CHECK_VALUE(q.dim() >= 3, what, ": q must be (..., heads, head_dim); got shape ", q.sizes());
+  const c10::cuda::CUDAGuard guard(q.device());
+  if (sections.empty()) sections.push_back(frequencies.numel());
+  TORCH_CHECK_VALUE(sections.size() <= NB200_ROTARY_MAX_AXES, what, ": at most ", NB200_ROTARY_MAX_AXES, " axes; got ", sections.size());
+  int64_t pairs = 0;
+  for (int64_t n : sections) {
+    TORCH_CHECK_VALUE(n >= 0, what, ": a section has ", n, " pairs");
+    pairs += n;
+  }
+  const int64_t D = q.size(-1), axes = int64_t(sections.size());
+  TORCH_CHECK_VALUE(2 * pairs <= D, what, ": ", pairs, " pairs do not fit head dim ", D);
+  TORCH_CHECK_TYPE(frequencies.scalar_type() == at::kFloat && frequencies.device() == q.device(), what, ": frequencies must be float32 on ",
+                   q.device(), "; got ", frequencies.scalar_type(), " on ", frequencies.device());
+  TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.size(0) == pairs, what, ": frequencies must have shape (", pairs, ",); got ", frequencies.sizes());
+  const auto pt = positions.scalar_type();
+  TORCH_CHECK_TYPE((pt == at::kInt || pt == at::kLong || pt == at::kFloat) && positions.device() == q.device(), what,
+                   ": positions must be int32, int64 or float32 on ", q.device(), "; got ", pt, " on ", positions.device());
+  const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 2);
+  const bool with_axis = positions.dim() == int64_t(lead.size()) + 1 && positions.size(-1) == axes && positions.sizes().slice(0, lead.size()) == lead;
+  TORCH_CHECK_VALUE(with_axis || (axes == 1 && positions.sizes() == lead), what, ": positions must have shape ", lead, " + (", axes, ",); got ", positions.sizes());
+  if (k) {
+    check_float(what, "k", *k);
+    TORCH_CHECK_TYPE(k->scalar_type() == q.scalar_type() && k->device() == q.device(), what, ": k must be ", q.scalar_type(), " on ", q.device());
+    TORCH_CHECK_VALUE(k->dim() == q.dim() && k->size(-1) == D && k->sizes().slice(0, lead.size()) == lead, what, ": k must be ", lead,
+                      " + (heads, ", D, "); got ", k->sizes());
+  }
+  TORCH_CHECK_VALUE(!positions.requires_grad() && !frequencies.requires_grad(), what, ": positions and frequencies are not differentiable");
+  const Tensor pos = positions.contiguous(), freq = frequencies.contiguous();
+  if (c10::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
+    refuse_tangents(what, q, k);
+    const tensor_list r = RotaryRule::apply(q, k, pos, freq, sections, interleaved);
+    return {r[0], k ? MaybeTensor(r[1]) : std::nullopt};
+  }
+  const tensor_list r = rotate(q, k.value_or(Tensor()), pos, freq, sections, interleaved, false);
+  return {r[0], k ? MaybeTensor(r[1]) : std::nullopt};
+}
+
+// ---- paged cache --------------------------------------------------------------------------------------------------------------
+nb200_cache_pages cache_pages(const char* what, const Tensor& k_pages, const Tensor& v_pages) {
+  check_float(what, "k_pages", k_pages);
+  TORCH_CHECK_TYPE(v_pages.scalar_type() == k_pages.scalar_type() && v_pages.device() == k_pages.device(), what, ": v_pages must be like k_pages");
+  TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), what,
+                    ": k_pages and v_pages must have one shape (pages, heads, page size, head dim); got ", k_pages.sizes(), " and ", v_pages.sizes());
+  nb200_cache_pages c{};
+  const Tensor* t[2] = {&k_pages, &v_pages};
+  for (int i = 0; i < 2; ++i) {
+    // (written in place: a copy in another layout would not do)
+    TORCH_CHECK_VALUE(t[i]->stride(3) == 1 && !has_expanded_axis(*t[i]), what, ": pages must have unit stride along the head dim and no expanded axis");
+    for (int a = 0; a < 3; ++a) (i ? c.v_stride : c.k_stride)[a] = t[i]->stride(a);
+  }
+  c.k = k_pages.data_ptr();
+  c.v = v_pages.data_ptr();
+  c.pages = int32_t(k_pages.size(0)); c.heads = int32_t(k_pages.size(1));
+  c.page_size = int32_t(k_pages.size(2)); c.head_dim = int32_t(k_pages.size(3));
+  c.dtype = dtype_code(k_pages.scalar_type());
+  return c;
+}
+
+struct CacheCall {
+  nb200_cache_params p{};
+  Tensor lengths, free_pages, free_range;
+  const char* what;
+
+  CacheCall(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths_in,
+            const Tensor& free_pages_in, const Tensor& free_range_in)
+      : what(name) {
+    p.struct_size = sizeof(p);
+    p.pages = cache_pages(what, k_pages, v_pages);
+    check_ints(what, "table", table, k_pages, 2);
+    check_ints(what, "lengths", lengths_in, k_pages, 1);
+    check_ints(what, "free_pages", free_pages_in, k_pages, 1);
+    check_ints(what, "free_range", free_range_in, k_pages, 1);
+    TORCH_CHECK_VALUE(table.is_contiguous(), what, ": table must be contiguous");
+    TORCH_CHECK_VALUE(lengths_in.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths_in.sizes());
+    TORCH_CHECK_VALUE(table.size(1) > 0, what, ": the table's rows must hold a page at least");
+    TORCH_CHECK_VALUE(free_pages_in.size(0) == k_pages.size(0) && free_range_in.size(0) == 2, what, ": free_pages must have shape (", k_pages.size(0),
+                      ",) and free_range (2,)");
+    lengths = lengths_in.contiguous();
+    free_pages = free_pages_in.contiguous();
+    free_range = free_range_in.contiguous();
+    p.table = table.data_ptr<int32_t>();
+    p.lengths = lengths.data_ptr<int32_t>();
+    p.free_pages = free_pages.data_ptr<int32_t>();
+    p.free_range = free_range.data_ptr<int32_t>();
+    p.rows = int32_t(table.size(0));
+    p.width = int32_t(table.size(1));
+  }
+  Tensor ints(int64_t n) const { return at::empty({n}, lengths.options()); }
+  Tensor workspace() {
+    size_t need = 0;
+    check(lib.nb200_cache_workspace_bytes(&p, &need), "nb200_cache_workspace_bytes");
+    Tensor ws = scratch(need, lengths);
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = need;
+    return ws;
+  }
+};
+
+// (lengths, free_range, shortfall)
+std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                                                const Tensor& free_pages, const Tensor& free_range, const Tensor& k, const Tensor& v,
+                                                const Tensor& offsets) {
+  const char* what = "cache_append";
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
+  for (const Tensor* t : {&k, &v}) {
+    TORCH_CHECK_TYPE(t->scalar_type() == k_pages.scalar_type() && t->device() == k_pages.device(), what, ": k and v must be ", k_pages.scalar_type(), " on ",
+                     k_pages.device());
+    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) == k.size(0) && t->size(1) == k_pages.size(1) && t->size(2) == k_pages.size(3), what,
+                      ": k and v must be (tokens, ", k_pages.size(1), ", ", k_pages.size(3), "); got ", t->sizes());
+  }
+  check_ints(what, "offsets", offsets, k_pages, 1);
+  TORCH_CHECK_VALUE(table.size(0) > 0 && offsets.size(0) == table.size(0) + 1, what, ": ", table.size(0), " rows, but offsets of shape ", offsets.sizes());
+  const Tensor kr = aligned_rows(k), vr = aligned_rows(v), off = offsets.contiguous();
+  const Tensor new_lengths = c.ints(table.size(0)), new_range = c.ints(2), shortfall = c.ints(1);
+  c.p.new_k = kr.data_ptr();
+  c.p.new_v = vr.data_ptr();
+  for (int a = 0; a < 2; ++a) { c.p.new_k_stride[a] = kr.stride(a); c.p.new_v_stride[a] = vr.stride(a); }
+  c.p.offsets = off.data_ptr<int32_t>();
+  c.p.tokens = k.size(0);
+  c.p.new_lengths = new_lengths.data_ptr<int32_t>();
+  c.p.new_free_range = new_range.data_ptr<int32_t>();
+  c.p.shortfall = shortfall.data_ptr<int32_t>();
+  check(lib.nb200_cache_append(&c.p, stream_of(k_pages)), "nb200_cache_append");
+  return {new_lengths, new_range, shortfall};
+}
+
+// (table, lengths, free_pages, free_range, shortfall); `rows`: parents (int32), or which rows are finished (bool)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                                                              const Tensor& free_pages, const Tensor& free_range, const Tensor& rows, bool finished) {
+  const char* what = finished ? "cache_free" : "cache_fork";
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
+  const Tensor r = rows.contiguous();
+  if (finished) {
+    TORCH_CHECK_TYPE(r.scalar_type() == at::kBool && r.device() == k_pages.device(), what, ": finished must be bool on ", k_pages.device());
+    TORCH_CHECK_VALUE(r.dim() == 1 && r.size(0) == table.size(0), what, ": finished must have shape (", table.size(0), ",); got ", r.sizes());
+    c.p.finished = static_cast<const uint8_t*>(r.data_ptr());
+  } else {
+    check_ints(what, "parents", r, k_pages, 1);
+    c.p.parents = r.data_ptr<int32_t>();
+  }
+  const int64_t n = r.size(0);
+  c.p.new_rows = int32_t(n);
+  const Tensor new_table = at::empty({n, table.size(1)}, table.options()), new_lengths = c.ints(n), new_free = c.ints(k_pages.size(0)),
+               new_range = c.ints(2), shortfall = c.ints(1);
+  c.p.new_table = new_table.data_ptr<int32_t>();
+  c.p.new_lengths = new_lengths.data_ptr<int32_t>();
+  c.p.new_free_pages = new_free.data_ptr<int32_t>();
+  c.p.new_free_range = new_range.data_ptr<int32_t>();
+  c.p.shortfall = shortfall.data_ptr<int32_t>();
+  const Tensor ws = c.workspace();
+  check(lib.nb200_cache_fork(&c.p, stream_of(k_pages)), "nb200_cache_fork");
+  return {new_table, new_lengths, new_free, new_range, shortfall};
+}
+
+// (table, free_pages, free_range, shortfall)
+std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                                                         const Tensor& free_pages, const Tensor& free_range) {
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  CacheCall c("cache_compact", k_pages, v_pages, table, lengths, free_pages, free_range);
+  const Tensor new_table = at::empty(table.sizes(), table.options()), new_free = c.ints(k_pages.size(0)), new_range = c.ints(2),
+               shortfall = c.ints(1);
+  c.p.new_table = new_table.data_ptr<int32_t>();
+  c.p.new_free_pages = new_free.data_ptr<int32_t>();
+  c.p.new_free_range = new_range.data_ptr<int32_t>();
+  c.p.shortfall = shortfall.data_ptr<int32_t>();
+  const Tensor ws = c.workspace();
+  check(lib.nb200_cache_compact(&c.p, stream_of(k_pages)), "nb200_cache_compact");
+  return {new_table, new_free, new_range, shortfall};
+}
+
+Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, double scale) {
+  const char* what = "decode_attention";
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  nb200_decode_params p{};
+  p.struct_size = sizeof(p);
+  p.pages = cache_pages(what, k_pages, v_pages);
+  TORCH_CHECK_TYPE(q.scalar_type() == k_pages.scalar_type() && q.device() == k_pages.device(), what, ": q must be ", k_pages.scalar_type(), " on ", k_pages.device());
+  TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == table.size(0) && q.size(2) == k_pages.size(3) && q.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, what,
+                    ": q must be (", table.size(0), ", a multiple of ", k_pages.size(1), ", ", k_pages.size(3), "); got ", q.sizes());
+  check_ints(what, "table", table, k_pages, 2);
+  check_ints(what, "lengths", lengths, k_pages, 1);
+  TORCH_CHECK_VALUE(lengths.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths.sizes());
+  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad())), what,
+                              " is not differentiable; packed_attention is");
+  const Tensor qr = aligned_rows(q), tab = table.contiguous(), len = lengths.contiguous();
+  const Tensor out = at::empty(q.sizes(), q.options());
+  p.table = tab.data_ptr<int32_t>();
+  p.lengths = len.data_ptr<int32_t>();
+  p.rows = int32_t(q.size(0));
+  p.width = int32_t(table.size(1));
+  p.q = qr.data_ptr();
+  p.out = out.data_ptr();
+  p.q_stride[0] = qr.stride(0);
+  p.q_stride[1] = qr.stride(1);
+  p.q_heads = int32_t(q.size(1));
+  p.scale = float(scale);
+  if (p.rows == 0) return out;
+  check(lib.nb200_decode_workspace_bytes(&p, &p.workspace_bytes), "nb200_decode_workspace_bytes");
+  const Tensor ws = scratch(p.workspace_bytes, q);
+  p.workspace = ws.data_ptr();
+  check(lib.nb200_decode(&p, stream_of(q)), "nb200_decode");
+  return out;
+}
+
+// ---- packed sequences ------------------------------------------------------------------------------------------------------
+struct Packed {
+  Tensor q, k, v, offsets_q, offsets_k;
+  double scale;
+  bool causal;
+  int kernel;
+
+  nb200_packed_params params() const {
+    nb200_packed_params p{};
+    p.struct_size = sizeof(p);
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr();
+    p.offsets_q = offsets_q.data_ptr<int32_t>();
+    p.offsets_k = offsets_k.data_ptr<int32_t>();
+    for (int a = 0; a < 2; ++a) { p.q_stride[a] = q.stride(a); p.k_stride[a] = k.stride(a); p.v_stride[a] = v.stride(a); }
+    p.tokens_q = int32_t(q.size(0)); p.tokens_k = int32_t(k.size(0));
+    p.sequences = int32_t(offsets_q.size(0) - 1);
+    p.heads = int32_t(q.size(1)); p.kv_heads = int32_t(k.size(1)); p.head_dim = int32_t(q.size(2));
+    p.dtype = dtype_code(q.scalar_type());
+    p.causal = causal;
+    p.scale = float(scale);
+    p.kernel = kernel;
+    return p;
+  }
+  int plan(int pass) const {
+    const nb200_packed_params p = params();
+    int chosen = 0;
+    check(lib.nb200_packed_plan(&p, pass, &chosen), "nb200_packed_plan");
+    return chosen;
+  }
+  Tensor workspace(nb200_packed_params& p, int pass) const {
+    check(lib.nb200_packed_workspace_bytes(&p, pass, &p.workspace_bytes), "nb200_packed_workspace_bytes");
+    Tensor ws;
+    if (p.workspace_bytes) {
+      ws = scratch(p.workspace_bytes, q);
+      p.workspace = ws.data_ptr();
+    }
+    return ws;
+  }
+  std::pair<Tensor, Tensor> forward() const {
+    const Tensor out = at::empty(q.sizes(), q.options());
+    const Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    nb200_packed_params p = params();
+    p.out = out.data_ptr();
+    p.lse = lse.data_ptr<float>();
+    const Tensor ws = workspace(p, NB200_PASS_FWD);
+    check(lib.nb200_packed_fwd(&p, stream_of(q)), "nb200_packed_fwd");
+    return {out, lse};
+  }
+  tensor_list backward(const Tensor& out, const Tensor& lse, const Tensor& grad) const {
+    const Tensor dout = aligned_rows(grad);
+    const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+    nb200_packed_params p = params();
+    p.out = out.data_ptr();
+    p.lse = lse.data_ptr<float>();
+    p.dout = dout.data_ptr(); p.dq = dq.data_ptr(); p.dk = dk.data_ptr(); p.dv = dv.data_ptr();
+    for (int a = 0; a < 2; ++a) p.dout_stride[a] = dout.stride(a);
+    const Tensor ws = workspace(p, NB200_PASS_BWD);
+    check(lib.nb200_packed_bwd(&p, stream_of(q)), "nb200_packed_bwd");
+    return {dq, dk, dv};
+  }
+};
+
+// Saves (q, k, v, offsets, out, lse), returns (dq, dk, dv).
+struct PackedRule : torch::autograd::Function<PackedRule> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets_q, const Tensor& offsets_k,
+                        double scale, bool causal, int64_t kernel) {
+    auto [out, lse] = Packed{q, k, v, offsets_q, offsets_k, scale, causal, int(kernel)}.forward();
+    ctx->save_for_backward({q, k, v, offsets_q, offsets_k, out, lse});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["flags"] = (kernel << 1) | int64_t(causal);
+    return out;
+  }
+  static tensor_list backward(AutogradContext* ctx, const tensor_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    // (a saved-tensor hook may hand the operands back in another layout)
+    const Packed a{aligned_rows(s[0]), aligned_rows(s[1]), aligned_rows(s[2]), s[3].contiguous(), s[4].contiguous(),
+                   ctx->saved_data["scale"].toDouble(), (flags & 1) != 0, int(flags >> 1)};
+    tensor_list g = a.backward(s[5].contiguous(), s[6].contiguous(), grads[0].to(s[0].scalar_type()));
+    g.resize(8);
+    return g;
+  }
+};
+
+// Nothing where the problem leaves the tensor-core family and the caller has not allowed that.
+MaybeTensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const MaybeTensor& offsets_k, double scale,
+                             bool causal, int64_t kernel, bool any_family) {
+  const char* what = "packed_attention";
+  check_float(what, "q", q);
+  const c10::cuda::CUDAGuard guard(q.device());
+  for (const Tensor* t : {&k, &v})
+    TORCH_CHECK_TYPE(t->scalar_type() == q.scalar_type() && t->device() == q.device(), what, ": k and v must be ", q.scalar_type(), " on ", q.device());
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(2) == k.size(2), what,
+                    ": q must be (tokens, heads, head dim), k and v (tokens, key heads, head dim); got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(q.size(1) > 0 && k.size(1) > 0 && q.size(1) % k.size(1) == 0, what, ": ", q.size(1), " query heads are no multiple of ", k.size(1), " key heads");
+  check_ints(what, "offsets", offsets, q, 1);
+  TORCH_CHECK_VALUE(offsets.size(0) >= 1, what, ": offsets must hold the number of sequences + 1 elements");
+  if (offsets_k) {
+    check_ints(what, "offsets_k", *offsets_k, q, 1);
+    TORCH_CHECK_VALUE(offsets_k->sizes() == offsets.sizes(), what, ": offsets_k must have shape ", offsets.sizes(), "; got ", offsets_k->sizes());
+  } else {
+    TORCH_CHECK_VALUE(k.size(0) == q.size(0), what, ": ", q.size(0), " queries and ", k.size(0), " keys need offsets_k");
+  }
+  const Tensor oq = offsets.contiguous(), ok = offsets_k ? offsets_k->contiguous() : oq;
+  const Packed a{aligned_rows(q), aligned_rows(k), aligned_rows(v), oq, ok, scale, causal, int(kernel)};
+  if (kernel == NB200_KERNEL_AUTO && !any_family && a.plan(NB200_PASS_FWD) != NB200_KERNEL_TCGEN05) return std::nullopt;
+  if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    refuse_tangents(what, q, k, v);
+    return PackedRule::apply(a.q, a.k, a.v, oq, ok, scale, causal, kernel);
+  }
+  return a.forward().first;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -562,4 +980,10 @@ PYBIND11_MODULE(_torch_ops, m) {
   m.def("layer_norm", torch::wrap_pybind_function_no_gil(layer_norm));
   m.def("set_scan_allocator", [](py::object allocator) { scan_allocator = allocator.release().ptr(); });   // (for good)
   m.def("selective_scan", torch::wrap_pybind_function_no_gil(selective_scan));
+  m.def("rotary", torch::wrap_pybind_function_no_gil(rotary));
+  m.def("cache_append", torch::wrap_pybind_function_no_gil(cache_append));
+  m.def("cache_fork", torch::wrap_pybind_function_no_gil(cache_fork));
+  m.def("cache_compact", torch::wrap_pybind_function_no_gil(cache_compact));
+  m.def("decode_attention", torch::wrap_pybind_function_no_gil(decode_attention));
+  m.def("packed_attention", torch::wrap_pybind_function_no_gil(packed_attention));
 }

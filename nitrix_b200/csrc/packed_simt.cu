@@ -1,0 +1,466 @@
+// Attention over packed sequences on the fp32 units: every type, head dim up to 256, group size and stride, forward and
+// backward, each sum in one order (no atomics).  The tensor-core kernels take what they cover; this is the rest.
+//
+// The query heads of one key head are rows of the same matrix: row r of a sequence is query r / G, head r % G, so that a tile
+// of rows reads its keys once for the whole group whatever G is, and dK and dV sum over the group by themselves.
+//   forward   a tile of kT rows walks over key tiles with the running maximum and sum of a softmax
+//   dq        the same walk with P = exp2(S - lse), dS = P (dO V^T - delta), dQ += dS K
+//   dk, dv    a tile of kT keys walks over row tiles, dV += P^T dO, dK += dS^T Q
+// Bound by the fp32 units: 256 threads as 16 x 16, each with a (kT / 16)-square piece of the scores and kT / 16 rows of the
+// outputs in registers, operands in shared memory as fp32 with rows padded by four words (16-byte reads of 8 rows meet no bank
+// twice).  Tiles are 64 rows up to head dim 128, and 32 above, where four operands of 64 rows would not fit.
+#include <math.h>
+
+#include "packed.cuh"
+
+namespace nb200 {
+namespace packed {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int kD>
+struct Tile {
+  static constexpr int kT = kD > 128 ? 32 : 64;
+  static constexpr int kM = kT / 16;            // rows and score columns of a thread
+  static constexpr int kStride = kD + 4;
+  static constexpr int kCols = kD / 64;         // 16-byte pieces of an output row of a thread
+  static constexpr int kPStride = kT + 1;
+  static constexpr int kOperand = kT * kStride;
+  static constexpr int kScores = kT * kPStride;
+};
+
+// The tile this CTA works on: tile `index` over all sequences' `count(i)` rows.
+struct Place {
+  int sequence;
+  int tile;          // within the sequence; -1: none
+};
+template <int kT, typename Count>
+__device__ __forceinline__ Place find_tile(int index, int sequences, Count count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < sequences; s0 += 32) {
+    int upto = s0 + lane < sequences ? int((count(s0 + lane) + kT - 1) / kT) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    const unsigned above = __ballot_sync(0xffffffffu, before + upto > index);
+    if (above) {
+      const int j = __ffs(above) - 1;
+      const int prev = __shfl_sync(0xffffffffu, upto, j > 0 ? j - 1 : 0);
+      return Place{s0 + j, index - before - (j > 0 ? prev : 0)};
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Place{0, -1};
+}
+
+// rows 0 .. n - 1 of a tile from `offset(row)` elements on; zeros elsewhere
+template <typename T, int kD, typename Offset>
+__device__ __forceinline__ void load_tile(float* dst, const void* base, int n, int D, Offset offset) {
+  using L = Tile<kD>;
+  for (int i = threadIdx.x; i < L::kT * kD; i += kThreads) {
+    const int r = i / kD, d = i - r * kD;
+    dst[r * L::kStride + d] = r < n && d < D ? to_f32<T>(static_cast<const T*>(base)[offset(r) + d]) : 0.f;
+  }
+}
+
+// s[i][j] = A row (ty * kM + i) . B row (tx + 16 j)
+template <int kD>
+__device__ __forceinline__ void products(float (&s)[Tile<kD>::kM][Tile<kD>::kM], const float* A, const float* B) {
+  using L = Tile<kD>;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i)
+#pragma unroll
+    for (int j = 0; j < L::kM; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < kD; d += 4) {
+    float4 a[L::kM], b[L::kM];
+#pragma unroll
+    for (int i = 0; i < L::kM; ++i) {
+      a[i] = *reinterpret_cast<const float4*>(A + (ty * L::kM + i) * L::kStride + d);
+      b[i] = *reinterpret_cast<const float4*>(B + (tx + 16 * i) * L::kStride + d);
+    }
+#pragma unroll
+    for (int i = 0; i < L::kM; ++i)
+#pragma unroll
+      for (int j = 0; j < L::kM; ++j)
+        s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+  }
+}
+
+// acc[i] += sum_c W(row ty * kM + i, c) B row c; W is kT x kT in shared memory, read along rows or (transposed) columns.
+// Columns of a thread: tx * 4 + 64 j.
+template <int kD, bool kTransposed>
+__device__ __forceinline__ void accumulate(float4 (&acc)[Tile<kD>::kM][Tile<kD>::kCols], const float* W, const float* B) {
+  using L = Tile<kD>;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll 4
+  for (int c = 0; c < L::kT; ++c) {
+    float w[L::kM];
+#pragma unroll
+    for (int i = 0; i < L::kM; ++i) w[i] = kTransposed ? W[c * L::kPStride + ty * L::kM + i] : W[(ty * L::kM + i) * L::kPStride + c];
+#pragma unroll
+    for (int j = 0; j < L::kCols; ++j) {
+      const float4 b = *reinterpret_cast<const float4*>(B + c * L::kStride + tx * 4 + 64 * j);
+#pragma unroll
+      for (int i = 0; i < L::kM; ++i) {
+        acc[i][j].x = fmaf(w[i], b.x, acc[i][j].x);
+        acc[i][j].y = fmaf(w[i], b.y, acc[i][j].y);
+        acc[i][j].z = fmaf(w[i], b.z, acc[i][j].z);
+        acc[i][j].w = fmaf(w[i], b.w, acc[i][j].w);
+      }
+    }
+  }
+}
+
+template <int kD>
+__device__ __forceinline__ void clear(float4 (&acc)[Tile<kD>::kM][Tile<kD>::kCols]) {
+#pragma unroll
+  for (int i = 0; i < Tile<kD>::kM; ++i)
+#pragma unroll
+    for (int j = 0; j < Tile<kD>::kCols; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+template <typename T, int kD>
+__device__ __forceinline__ void store_row(T* dst, const float4 (&row)[Tile<kD>::kCols], float mul, int D) {
+  const int tx = threadIdx.x & 15;
+#pragma unroll
+  for (int j = 0; j < Tile<kD>::kCols; ++j) {
+    const float v[4] = {row[j].x, row[j].y, row[j].z, row[j].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = tx * 4 + 64 * j + e;
+      if (d < D) dst[d] = from_f32<T>(v[e] * mul);
+    }
+  }
+}
+
+// Rows of a sequence of one key head: query r / G, head r % G.
+struct Rows {
+  int2 q, k;           // first token, tokens
+  int kv_head, group, heads;
+  int64_t n;           // rows
+  __device__ __forceinline__ Rows(const PackedArgs& a, int sequence, int kv)
+      : q(sequence_span(a.offsets_q, sequence, a.tokens_q)), k(sequence_span(a.offsets_k, sequence, a.tokens_k)), kv_head(kv),
+        group(a.group), heads(a.heads), n(int64_t(q.y) * a.group) {}
+  __device__ __forceinline__ int token(int64_t r) const { return q.x + int(r / group); }
+  __device__ __forceinline__ int head(int64_t r) const { return kv_head * group + int(r % group); }
+  __device__ __forceinline__ int64_t at(int64_t r, const int64_t (&stride)[2]) const { return token(r) * stride[0] + head(r) * stride[1]; }
+  // (token, head) index of a dense array
+  __device__ __forceinline__ int64_t flat(int64_t r) const { return int64_t(token(r)) * heads + head(r); }
+  // keys that row r sees: the first `seen` of the sequence
+  __device__ __forceinline__ int seen(int64_t r, int causal) const {
+    return causal ? min(k.y, max(int(r / group) + 1 + k.y - q.y, 0)) : k.y;
+  }
+};
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads) packed_fwd_simt_kernel(const PackedArgs a) {
+  using L = Tile<kD>;
+  extern __shared__ __align__(16) float smem[];
+  float *sq = smem, *sk = sq + L::kOperand, *sv = sk + L::kOperand, *sp = sv + L::kOperand;
+  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group; });
+  if (place.tile < 0) return;
+  const Rows rows(a, place.sequence, blockIdx.y);
+  const int64_t r0 = int64_t(place.tile) * L::kT;
+  const int n = int(min(int64_t(L::kT), rows.n - r0));
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const float mul = a.scale * kLog2e;
+  load_tile<T, kD>(sq, a.q, n, a.D, [&](int r) { return rows.at(r0 + r, a.qs); });
+  float m[L::kM], l[L::kM];
+  int seen[L::kM];
+  float4 acc[L::kM][L::kCols];
+  clear<kD>(acc);
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    seen[i] = ty * L::kM + i < n ? rows.seen(r0 + ty * L::kM + i, a.causal) : 0;
+  }
+  const int keys = rows.seen(r0 + n - 1, a.causal);     // the tile's last row sees the most
+  for (int k0 = 0; k0 < keys; k0 += L::kT) {
+    const int nk = min(L::kT, rows.k.y - k0);
+    __syncthreads();
+    load_tile<T, kD>(sk, a.k, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.ks[0] + rows.kv_head * a.ks[1]; });
+    load_tile<T, kD>(sv, a.v, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.vs[0] + rows.kv_head * a.vs[1]; });
+    __syncthreads();
+    float s[L::kM][L::kM];
+    products<kD>(s, sq, sk);
+#pragma unroll
+    for (int i = 0; i < L::kM; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int j = 0; j < L::kM; ++j) {
+        s[i][j] = k0 + tx + 16 * j < seen[i] ? s[i][j] * mul : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float shift = mx == -INFINITY ? 0.f : mx, alpha = exp2f(m[i] - shift);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < L::kM; ++j) {
+        const float p = exp2f(s[i][j] - shift);
+        sum += p;
+        sp[(ty * L::kM + i) * L::kPStride + tx + 16 * j] = p;
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l[i] = l[i] * alpha + sum;
+      m[i] = mx;
+#pragma unroll
+      for (int j = 0; j < L::kCols; ++j) {
+        acc[i][j].x *= alpha; acc[i][j].y *= alpha; acc[i][j].z *= alpha; acc[i][j].w *= alpha;
+      }
+    }
+    __syncthreads();
+    accumulate<kD, false>(acc, sp, sv);
+  }
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i) {
+    const int r = ty * L::kM + i;
+    if (r >= n) continue;
+    const int64_t at = rows.flat(r0 + r);
+    const bool empty = seen[i] == 0;
+    store_row<T, kD>(static_cast<T*>(a.out) + at * a.D, acc[i], empty ? 0.f : 1.f / l[i], a.D);
+    if (tx == 0) a.lse[at] = empty ? -INFINITY : m[i] + log2f(l[i]);
+  }
+}
+
+// P and dS of a (row tile, key tile) pair into shared memory; row statistics in `stat` (lse, delta per row)
+template <int kD>
+__device__ __forceinline__ void score_gradients(const float* sq, const float* sdo, const float* sk, const float* sv, float* sp,
+                                                float* sds, const float* stat, const int* seen, int k0, float mul) {
+  using L = Tile<kD>;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float s[L::kM][L::kM], dp[L::kM][L::kM];
+  products<kD>(s, sq, sk);
+  products<kD>(dp, sdo, sv);
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i)
+#pragma unroll
+    for (int j = 0; j < L::kM; ++j) {
+      const int r = ty * L::kM + i, c = tx + 16 * j;
+      const bool in = k0 + c < seen[r];
+      const float p = in ? exp2f(s[i][j] * mul - stat[2 * r]) : 0.f;
+      if (sp) sp[r * L::kPStride + c] = p;
+      sds[r * L::kPStride + c] = in ? p * (dp[i][j] - stat[2 * r + 1]) : 0.f;
+    }
+}
+
+template <int kT>
+__device__ __forceinline__ void load_stats(const PackedArgs& a, const Rows& rows, int64_t r0, int n, float* stat, int* seen) {
+  if (threadIdx.x < kT) {
+    const int r = threadIdx.x;
+    const int64_t at = r < n ? rows.flat(r0 + r) : 0;
+    stat[2 * r] = r < n ? a.lse[at] : 0.f;
+    stat[2 * r + 1] = r < n ? a.delta[at] : 0.f;
+    seen[r] = r < n ? rows.seen(r0 + r, a.causal) : 0;
+  }
+}
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads) packed_dq_simt_kernel(const PackedArgs a) {
+  using L = Tile<kD>;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ float stat[2 * L::kT];
+  __shared__ int seen[L::kT];
+  float *sq = smem, *sdo = sq + L::kOperand, *sk = sdo + L::kOperand, *sv = sk + L::kOperand, *sds = sv + L::kOperand;
+  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group; });
+  if (place.tile < 0) return;
+  const Rows rows(a, place.sequence, blockIdx.y);
+  const int64_t r0 = int64_t(place.tile) * L::kT;
+  const int n = int(min(int64_t(L::kT), rows.n - r0));
+  const int ty = threadIdx.x >> 4;
+  load_tile<T, kD>(sq, a.q, n, a.D, [&](int r) { return rows.at(r0 + r, a.qs); });
+  load_tile<T, kD>(sdo, a.dout, n, a.D, [&](int r) { return rows.at(r0 + r, a.dos); });
+  load_stats<L::kT>(a, rows, r0, n, stat, seen);
+  float4 acc[L::kM][L::kCols];
+  clear<kD>(acc);
+  const int keys = rows.seen(r0 + n - 1, a.causal);
+  for (int k0 = 0; k0 < keys; k0 += L::kT) {
+    const int nk = min(L::kT, rows.k.y - k0);
+    __syncthreads();
+    load_tile<T, kD>(sk, a.k, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.ks[0] + rows.kv_head * a.ks[1]; });
+    load_tile<T, kD>(sv, a.v, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.vs[0] + rows.kv_head * a.vs[1]; });
+    __syncthreads();
+    score_gradients<kD>(sq, sdo, sk, sv, nullptr, sds, stat, seen, k0, a.scale * kLog2e);
+    __syncthreads();
+    accumulate<kD, false>(acc, sds, sk);
+  }
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i) {
+    const int r = ty * L::kM + i;
+    if (r < n) store_row<T, kD>(static_cast<T*>(a.dq) + rows.flat(r0 + r) * a.D, acc[i], a.scale, a.D);
+  }
+}
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads) packed_dkv_simt_kernel(const PackedArgs a) {
+  using L = Tile<kD>;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ float stat[2 * L::kT];
+  __shared__ int seen[L::kT];
+  float *sq = smem, *sdo = sq + L::kOperand, *sk = sdo + L::kOperand, *sv = sk + L::kOperand, *sp = sv + L::kOperand,
+        *sds = sp + L::kScores;
+  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_k, i, a.tokens_k).y); });
+  if (place.tile < 0) return;
+  const Rows rows(a, place.sequence, blockIdx.y);
+  const int k0 = place.tile * L::kT, nk = min(L::kT, rows.k.y - k0);
+  const int ty = threadIdx.x >> 4;
+  load_tile<T, kD>(sk, a.k, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.ks[0] + rows.kv_head * a.ks[1]; });
+  load_tile<T, kD>(sv, a.v, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.vs[0] + rows.kv_head * a.vs[1]; });
+  float4 dk[L::kM][L::kCols], dv[L::kM][L::kCols];
+  clear<kD>(dk);
+  clear<kD>(dv);
+  // the first query that sees this tile's first key
+  const int64_t first = a.causal ? int64_t(max(k0 - (rows.k.y - rows.q.y), 0)) * a.group : 0;
+  for (int64_t r0 = first / L::kT * L::kT; r0 < rows.n; r0 += L::kT) {
+    const int n = int(min(int64_t(L::kT), rows.n - r0));
+    __syncthreads();
+    load_tile<T, kD>(sq, a.q, n, a.D, [&](int r) { return rows.at(r0 + r, a.qs); });
+    load_tile<T, kD>(sdo, a.dout, n, a.D, [&](int r) { return rows.at(r0 + r, a.dos); });
+    load_stats<L::kT>(a, rows, r0, n, stat, seen);
+    __syncthreads();
+    score_gradients<kD>(sq, sdo, sk, sv, sp, sds, stat, seen, k0, a.scale * kLog2e);
+    __syncthreads();
+    accumulate<kD, true>(dv, sp, sdo);
+    accumulate<kD, true>(dk, sds, sq);
+  }
+#pragma unroll
+  for (int i = 0; i < L::kM; ++i) {
+    const int r = ty * L::kM + i;
+    if (r >= nk) continue;
+    const int64_t at = (int64_t(rows.k.x) + k0 + r) * a.kv_heads + rows.kv_head;
+    store_row<T, kD>(static_cast<T*>(a.dk) + at * a.D, dk[i], a.scale, a.D);
+    store_row<T, kD>(static_cast<T*>(a.dv) + at * a.D, dv[i], 1.f, a.D);
+  }
+}
+
+// delta[token][head] = sum_d out dout: a warp per row
+template <typename T>
+__global__ void __launch_bounds__(kThreads) packed_delta_kernel(const PackedArgs a) {
+  const int64_t row = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (row >= int64_t(a.tokens_q) * a.heads) return;
+  const int64_t token = row / a.heads;
+  const int head = int(row - token * a.heads);
+  const T* o = static_cast<const T*>(a.out) + row * a.D;
+  const T* g = static_cast<const T*>(a.dout) + token * a.dos[0] + head * a.dos[1];
+  float sum = 0.f;
+  for (int d = lane; d < a.D; d += 32) sum = fmaf(to_f32<T>(o[d]), to_f32<T>(g[d]), sum);
+#pragma unroll
+  for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+  if (lane == 0) a.delta[row] = sum;
+}
+
+// The tokens behind the last sequence.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) packed_clear_kernel(const PackedArgs a, bool backward) {
+  const int64_t step = int64_t(gridDim.x) * kThreads, start = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k);
+  T* rows_q = static_cast<T*>(backward ? a.dq : a.out);
+  for (int64_t i = q0 * a.heads * a.D + start; i < int64_t(a.tokens_q) * a.heads * a.D; i += step) rows_q[i] = from_f32<T>(0.f);
+  if (!backward) {
+    for (int64_t i = q0 * a.heads + start; i < int64_t(a.tokens_q) * a.heads; i += step) a.lse[i] = -INFINITY;
+    return;
+  }
+  for (int64_t i = k0 * a.kv_heads * a.D + start; i < int64_t(a.tokens_k) * a.kv_heads * a.D; i += step) {
+    static_cast<T*>(a.dk)[i] = from_f32<T>(0.f);
+    static_cast<T*>(a.dv)[i] = from_f32<T>(0.f);
+  }
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == NB200_F32) return f(float());
+  if (dtype == NB200_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+template <int kN>
+struct Int {
+  static constexpr int value = kN;
+};
+template <typename F>
+int by_head_dim(int D, F f) {
+  if (D <= 64) return f(Int<64>());
+  if (D <= 128) return f(Int<128>());
+  return f(Int<256>());
+}
+
+template <typename Kernel>
+int configure(Kernel kernel, size_t smem, const char* what) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return check_launch(what);
+  return NB200_OK;
+}
+
+// most tiles that sequences of `tokens` tokens together can have
+unsigned most_tiles(int64_t rows, int sequences, int tile) { return unsigned(rows / tile + sequences); }
+
+}  // namespace
+
+int launch_clear_uncovered(const PackedArgs& a, int dtype, bool backward, cudaStream_t st) {
+  return by_type(dtype, [&](auto t) {
+    packed_clear_kernel<decltype(t)><<<32, kThreads, 0, st>>>(a, backward);
+    count_launch();
+    return check_launch("packed_clear_kernel");
+  });
+}
+
+int launch_packed_delta(const PackedArgs& a, int dtype, cudaStream_t st) {
+  return by_type(dtype, [&](auto t) {
+    const int64_t rows = int64_t(a.tokens_q) * a.heads;
+    packed_delta_kernel<decltype(t)><<<unsigned((rows + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
+    count_launch();
+    return check_launch("packed_delta_kernel");
+  });
+}
+
+int simt_packed_fwd(const PackedArgs& a, int dtype, cudaStream_t st) {
+  return by_type(dtype, [&](auto t) {
+    return by_head_dim(a.D, [&](auto d) {
+      constexpr int kD = decltype(d)::value;
+      using L = Tile<kD>;
+      auto kernel = packed_fwd_simt_kernel<decltype(t), kD>;
+      constexpr size_t smem = sizeof(float) * (3 * L::kOperand + L::kScores);
+      static_assert(smem <= 232448, "shared memory of a CTA");
+      if (int rc = configure(kernel, smem, "packed_fwd_simt_kernel")) return rc;
+      kernel<<<dim3(most_tiles(int64_t(a.tokens_q) * a.group, a.sequences, L::kT), unsigned(a.kv_heads)), kThreads, smem, st>>>(a);
+      count_launch();
+      return check_launch("packed_fwd_simt_kernel");
+    });
+  });
+}
+
+int simt_packed_bwd(const PackedArgs& a, int dtype, cudaStream_t st) {
+  return by_type(dtype, [&](auto t) {
+    return by_head_dim(a.D, [&](auto d) {
+      constexpr int kD = decltype(d)::value;
+      using L = Tile<kD>;
+      constexpr size_t smem_dq = sizeof(float) * (4 * L::kOperand + L::kScores), smem_dkv = smem_dq + sizeof(float) * L::kScores;
+      static_assert(smem_dkv + 1024 <= 232448, "shared memory of a CTA");
+      if (a.tokens_q > 0) {
+        auto kernel = packed_dq_simt_kernel<decltype(t), kD>;
+        if (int rc = configure(kernel, smem_dq, "packed_dq_simt_kernel")) return rc;
+        kernel<<<dim3(most_tiles(int64_t(a.tokens_q) * a.group, a.sequences, L::kT), unsigned(a.kv_heads)), kThreads, smem_dq, st>>>(a);
+        count_launch();
+        if (int rc = check_launch("packed_dq_simt_kernel")) return rc;
+      }
+      if (a.tokens_k > 0) {
+        auto kernel = packed_dkv_simt_kernel<decltype(t), kD>;
+        if (int rc = configure(kernel, smem_dkv, "packed_dkv_simt_kernel")) return rc;
+        kernel<<<dim3(most_tiles(a.tokens_k, a.sequences, L::kT), unsigned(a.kv_heads)), kThreads, smem_dkv, st>>>(a);
+        count_launch();
+        return check_launch("packed_dkv_simt_kernel");
+      }
+      return int(NB200_OK);
+    });
+  });
+}
+
+}  // namespace packed
+}  // namespace nb200

@@ -1,0 +1,39 @@
+"""Attention over packed sequences of unequal length with grouped heads (``include/nitrix_b200_packed.h``)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import _cabi
+from ..backend import fallback, resolve_backend
+from .attention import default_scale
+
+__all__ = ["packed_attention"]
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, *,
+                     offsets_k: Optional[torch.Tensor] = None, scale: Optional[float] = None, causal: bool = True,
+                     backend: str = "auto") -> torch.Tensor:
+    """Softmax attention within each of several sequences that lie one after the other.
+
+    ``q`` is ``(tokens, heads, head_dim)``, ``k`` and ``v`` are ``(tokens, key heads, head_dim)``; query head ``h`` reads key
+    head ``h // (heads // key heads)``.  Sequence ``i`` has the tokens ``offsets[i] .. offsets[i + 1]`` (int32, on the device);
+    ``offsets_k`` where its keys are not as many as its queries.  With ``causal`` the last query of a sequence sees all its
+    keys, each one before it one less.  A query that sees no key gives zeros and has no gradient; so do tokens behind the last
+    offset.  Differentiable in ``q``, ``k`` and ``v``.
+
+    bf16 and fp16 with head dim 64 or 128 run on the tensor cores; what they do not take runs on the fp32 units, with one
+    ``NitrixBackendFallback`` warning.  That family sums everything in a fixed order and is what reproducibility mode uses.
+    """
+    resolved = resolve_backend(backend)
+    kernel = _cabi.KERNEL_SIMT if resolved == "cuda-simt" else _cabi.KERNEL_AUTO
+    factor = default_scale(q.shape[-1]) if scale is None else float(scale)
+    out = _cabi.torch_ops().packed_attention(q, k, v, offsets, offsets_k, factor, bool(causal), kernel, False)
+    if out is None:
+        fallback(function="packed_attention", requested=resolved, resolved="cuda-simt",
+                 reason="the fused tcgen05 kernels take bf16/fp16 with head dim 64 or 128, up to 64 query heads per key head "
+                        "and a positive scale",
+                 shapes=(tuple(q.shape), tuple(k.shape)), dtype=q.dtype)
+        out = _cabi.torch_ops().packed_attention(q, k, v, offsets, offsets_k, factor, bool(causal), kernel, True)
+    return out

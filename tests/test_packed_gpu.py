@@ -1,0 +1,262 @@
+"""Attention over packed sequences on the GPU against 64 bits, forward and gradients.
+
+16-bit operands: probabilities, their gradients and the results are each rounded once to the operand type, the row sums of the
+backward come from a rounded output, all else is fp32.  The oracle returns with every value the sum that such a relative error
+multiplies, so the bound is u times that sum, u half an ulp, doubled for the fp32 parts (and exponentials good to 1e-4 relative,
+which 16-bit forwards may use: below a tenth of an fp16 ulp's half).  fp32: 1e-5 of the same sums.
+"""
+import random
+
+import pytest
+import torch
+
+from oracle import decoder_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+U = {t: torch.finfo(t).eps for t in (torch.bfloat16, torch.float16)} | {torch.float32: 1e-5}
+
+
+def _offsets(lengths):
+    return torch.tensor([0, *lengths]).cumsum(0).int().cuda()
+
+
+def _inputs(lengths_q, lengths_k, H, Hk, D, dtype, seed=0, extra=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    tq, tk = sum(lengths_q) + extra, sum(lengths_k) + extra
+    q, k, v, dout = (torch.randn(t, h, D, generator=g, device="cuda").to(dtype) for t, h in ((tq, H), (tk, Hk), (tk, Hk), (tq, H)))
+    return q, k, v, dout
+
+
+def _check(q, k, v, dout, lengths_q, lengths_k, causal=True, scale=None, backend="auto", offsets=None):
+    from nitrix_b200 import _cabi
+    from nitrix_b200.nn import packed_attention
+
+    dtype = q.dtype
+    oq = _offsets(lengths_q)
+    ok = None if lengths_k is lengths_q else _offsets(lengths_k)
+    with torch.no_grad():
+        plain = packed_attention(q, k, v, oq, offsets_k=ok, causal=causal, scale=scale, backend=backend)
+    leaves = [t.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) if t.is_contiguous() else t.detach().requires_grad_(True)
+              for t in (q, k, v)]
+    out = packed_attention(*leaves, oq, offsets_k=ok, causal=causal, scale=scale, backend=backend)
+    grads = torch.autograd.grad(out, leaves, dout)
+    torch.cuda.synchronize()
+    assert _cabi.lib().nb200_device_status(0) == 0
+    assert torch.equal(plain, out.detach())
+    want = O.packed(q, k, v, lengths_q, lengths_k, q.shape[-1] ** -0.5 if scale is None else scale, causal, dout)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)):
+        value, bound = want[name]
+        assert got.dtype == dtype and got.shape == value.shape
+        err = (got.double() - value).abs() - U[dtype] * bound
+        assert bool((err <= 1e-6).all()), (name, float(err.max()))
+    return out.detach(), grads
+
+
+SHAPES = {
+    "one token": [1],
+    "tile edges": [63, 64, 65, 127, 128, 129],
+    "empty ones": [0, 5, 0, 0, 200, 1, 0],
+    "one longer": [700],
+    "many short": [3, 1, 17, 9, 2, 31, 16, 8, 40, 5, 1, 1, 12],
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 40, 256])
+@pytest.mark.parametrize("Hk,G", [(1, 1), (2, 4), (1, 3), (2, 8), (1, 16)])
+@pytest.mark.parametrize("name", SHAPES)
+def test_causal(dtype, D, Hk, G, name, monkeypatch):
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths = SHAPES[name]
+    _check(*_inputs(lengths, lengths, Hk * G, Hk, D, dtype, seed=D + G), lengths, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths_q,lengths_k", [
+    ([5, 100, 64], [300, 100, 0]), ([200, 1, 33], [7, 129, 256]), ([0, 40, 130], [50, 0, 129]), ([300], [128]), ([1, 1, 1], [257, 1, 64])])
+def test_keys_of_other_lengths(dtype, D, causal, lengths_q, lengths_k, monkeypatch):
+    """Fewer keys than queries leave the first queries without any under causal: zeros, and no gradient."""
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    out, grads = _check(*_inputs(lengths_q, lengths_k, 8, 2, D, dtype), lengths_q, lengths_k, causal)
+    at = 0
+    for lq, lk in zip(lengths_q, lengths_k):
+        blind = lq if lk == 0 else (max(lq - lk, 0) if causal else 0)
+        assert not bool(out[at:at + blind].any()) and not bool(grads[0][at:at + blind].any())
+        at += lq
+
+
+@pytest.mark.parametrize("D,Hk,G", [(64, 1, 5), (128, 1, 7), (64, 2, 32), (128, 1, 64), (64, 1, 65), (128, 3, 2), (64, 1, 128)])
+def test_group_sizes(D, Hk, G, monkeypatch):
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths = [70, 3, 141]
+    _check(*_inputs(lengths, lengths, Hk * G, Hk, D, torch.bfloat16), lengths, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.5, 0.0, -0.3])
+def test_scales(dtype, scale, monkeypatch):
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths = [150, 20]
+    _check(*_inputs(lengths, lengths, 4, 2, 64, dtype), lengths, lengths, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_sequence_does_not_see_its_neighbours(dtype, D, monkeypatch):
+    """NaN and infinities in every other sequence, and in the tokens behind the last, stay there -- in the gradients too."""
+    from nitrix_b200.nn import packed_attention
+
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths = [37, 130, 64, 200, 1, 90]
+    q, k, v, dout = _inputs(lengths, lengths, 6, 2, D, dtype, extra=11)
+    spans, at = [], 0
+    for n in lengths:
+        spans.append(slice(at, at + n))
+        at += n
+    clean = [i for i in range(len(lengths)) if i % 2 == 0]
+
+    def run(*operands):
+        leaves = [t.clone().requires_grad_(True) for t in operands[:3]]
+        out = packed_attention(*leaves, _offsets(lengths))
+        return [out.detach(), *torch.autograd.grad(out, leaves, operands[3])]
+    want = run(q, k, v, dout)
+    for bad in (float("nan"), float("inf")):
+        dirty = [t.clone() for t in (q, k, v, dout)]
+        for t in dirty:
+            for i, s in enumerate(spans):
+                if i not in clean:
+                    t[s] = bad
+            t[at:] = bad
+        got = run(*dirty)
+        for a, b in zip(got, want):
+            for i in clean:
+                # (the sums of dq are made in no fixed order)
+                assert bool(torch.isfinite(a[spans[i]]).all())
+                assert float((a[spans[i]].double() - b[spans[i]].double()).abs().max()) <= 2 * U[dtype] * float(b[spans[i]].double().abs().max())
+            assert not bool(a[at:].any())
+
+
+def test_views_of_one_projection_and_expanded_cotangents():
+    lengths = [100, 29, 300]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.randn(429, 12, 64, generator=g, device="cuda").bfloat16()
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    dout = torch.randn(429, 8, 64, generator=g, device="cuda").bfloat16()
+    _check(q, k, v, dout, lengths, lengths)
+    _check(q, k, v, torch.ones((), device="cuda", dtype=torch.bfloat16).expand(429, 8, 64), lengths, lengths)
+    odd = torch.randn(429 * 8 * 64 + 1, generator=g, device="cuda").bfloat16()[1:].view(429, 8, 64)
+    _check(odd, k, v, dout, lengths, lengths)
+
+
+def test_gradients_against_differences():
+    """fp32, central differences along random directions: truncation is O(h^2) of third derivatives of order one; with h = 1e-2
+    the fp32 noise of a sum of 23 040 outputs over 2 h stays below 2e-2, as does h^2."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [33, 60, 27]
+    q, k, v, dout = _inputs(lengths, lengths, 3, 1, 64, torch.float32)
+    off = _offsets(lengths)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, off, backend="cuda-simt"), leaves, dout)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for i in range(3):
+        e = torch.randn(leaves[i].shape, generator=g, device="cuda")
+        e /= e.norm()
+        h = 1e-2
+
+        def f(sign):
+            ops = [q, k, v]
+            ops[i] = ops[i] + sign * h * e
+            return (packed_attention(*ops, off, backend="cuda-simt").double() * dout.double()).sum()
+        assert abs(float((f(1) - f(-1)) / (2 * h) - (grads[i].double() * e.double()).sum())) < 2e-2
+
+
+def test_families_and_reproducibility(monkeypatch):
+    import nitrix_b200
+    from nitrix_b200.backend import NitrixBackendError, NitrixBackendFallback, reset_fallback_state
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [90, 40]
+    q, k, v, dout = _inputs(lengths, lengths, 4, 2, 64, torch.bfloat16)
+    off = _offsets(lengths)
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = packed_attention(*leaves, off)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    with nitrix_b200.reproducible():
+        first = run()
+        for _ in range(3):
+            for a, b in zip(run(), first):
+                assert torch.equal(a, b)
+    reset_fallback_state()
+    with pytest.warns(NitrixBackendFallback, match="packed_attention"):
+        packed_attention(q.float(), k.float(), v.float(), off)
+    monkeypatch.setenv("NITRIX_STRICT_BACKEND", "1")
+    with pytest.raises(NitrixBackendError):
+        packed_attention(q.float(), k.float(), v.float(), off)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_random_batches(dtype):
+    rng = random.Random(5)
+    for _ in range(25):
+        D, Hk, G = rng.choice([64, 128]), rng.choice([1, 2, 3]), rng.choice([1, 2, 3, 4, 5, 8, 12])
+        n = rng.randint(1, 9)
+        lq = [rng.choice([0, 1, rng.randint(1, 30), rng.randint(1, 400)]) for _ in range(n)]
+        lk = lq if rng.random() < 0.5 else [rng.choice([0, 1, rng.randint(1, 30), rng.randint(1, 400)]) for _ in range(n)]
+        _check(*_inputs(lq, lk, Hk * G, Hk, D, dtype, seed=n), lq, lk, rng.random() < 0.7)
+
+
+def test_streams_and_graphs():
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [130, 20, 55]
+    q, k, v, _ = _inputs(lengths, lengths, 4, 2, 128, torch.bfloat16)
+    off = _offsets(lengths)
+    want = packed_attention(q, k, v, off)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = packed_attention(q, k, v, off)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = packed_attention(q, k, v, off)
+    other = [20, 130, 55]
+    off.copy_(_offsets(other))        # other lengths, the same graph
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, packed_attention(q, k, v, _offsets(other)))
+
+
+def test_refusals():
+    from nitrix_b200.nn import packed_attention
+
+    q, k, v, _ = _inputs([10], [10], 4, 2, 64, torch.bfloat16)
+    off = _offsets([10])
+    with pytest.raises(TypeError, match="CUDA tensor"):
+        packed_attention(q.cpu(), k, v, off)
+    with pytest.raises(TypeError, match="k and v"):
+        packed_attention(q, k.half(), v, off)
+    with pytest.raises(ValueError, match="head dim"):
+        packed_attention(q, k, v[:, :1], off)
+    with pytest.raises(ValueError, match="multiple"):
+        packed_attention(q[:, :3], k, v, off)
+    with pytest.raises(TypeError, match="offsets"):
+        packed_attention(q, k, v, off.long())
+    with pytest.raises(ValueError, match="offsets"):
+        packed_attention(q, k, v, off[None])
+    with pytest.raises(ValueError, match="offsets_k"):
+        packed_attention(q[:9], k, v, off)
+    with pytest.raises(ValueError, match="offsets_k"):
+        packed_attention(q, k, v, off, offsets_k=_offsets([5, 5]))
+    with pytest.raises(RuntimeError, match="at most 256"):
+        packed_attention(*(t.repeat(1, 1, 5) for t in (q, k, v)), off, backend="cuda-simt")
+    empty = packed_attention(q[:0], k[:0], v[:0], _offsets([0, 0]))
+    assert empty.shape == (0, 4, 64)
+    assert not bool(packed_attention(q, k, v, _offsets([]), backend="cuda-simt").any())
