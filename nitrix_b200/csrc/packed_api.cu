@@ -1,5 +1,5 @@
 // Entry points of attention over packed sequences: checks, choice of the kernel family, scratch.
-#include "packed.cuh"
+#include "packed_tc.cuh"
 
 namespace nb200 {
 namespace packed {
@@ -36,7 +36,23 @@ PackedArgs lower(const nb200_packed_params* p) {
 
 size_t delta_bytes(const nb200_packed_params* p) { return (size_t(p->tokens_q) * size_t(p->heads) * sizeof(float) + 255) / 256 * 256; }
 
-size_t workspace(const nb200_packed_params* p, int pass) { return pass == NB200_PASS_BWD ? delta_bytes(p) : 0; }
+bool tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
+  return pass == NB200_PASS_FWD && p->kernel == NB200_KERNEL_AUTO && tc_packed_supported(a, p->dtype);
+}
+
+size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
+  if (pass == NB200_PASS_BWD) return delta_bytes(p);
+  return tensor_cores(p, a, pass) ? tc_packed_fwd_bytes(a) : 0;
+}
+
+int check_workspace(const nb200_packed_params* p, const PackedArgs& a, int pass, const char* what) {
+  const size_t need = workspace(p, a, pass);
+  if (need && (!p->workspace || p->workspace_bytes < need)) {
+    set_error("%s: workspace of %zu bytes needed (nb200_packed_workspace_bytes), %zu given", what, need, p->workspace_bytes);
+    return NB200_ERR_WORKSPACE;
+  }
+  return NB200_OK;
+}
 
 int check_operands(const nb200_packed_params* p, const char* what, bool backward) {
   const bool q = p->tokens_q > 0, k = p->tokens_k > 0;
@@ -56,14 +72,14 @@ using namespace nb200::packed;
 extern "C" NB200_API int nb200_packed_plan(const nb200_packed_params* p, int pass, int* kernel) {
   if (int rc = check(p, "packed_plan")) return rc;
   if (!kernel || (pass != NB200_PASS_FWD && pass != NB200_PASS_BWD)) { set_error("packed_plan: NULL result or bad pass"); return NB200_ERR_INVALID; }
-  *kernel = NB200_KERNEL_SIMT;
+  *kernel = tensor_cores(p, lower(p), pass) ? NB200_KERNEL_TCGEN05 : NB200_KERNEL_SIMT;
   return NB200_OK;
 }
 
 extern "C" NB200_API int nb200_packed_workspace_bytes(const nb200_packed_params* p, int pass, size_t* bytes) {
   if (int rc = check(p, "packed_workspace_bytes")) return rc;
   if (!bytes || (pass != NB200_PASS_FWD && pass != NB200_PASS_BWD)) { set_error("packed_workspace_bytes: NULL result or bad pass"); return NB200_ERR_INVALID; }
-  *bytes = workspace(p, pass);
+  *bytes = workspace(p, lower(p), pass);
   return NB200_OK;
 }
 
@@ -71,9 +87,11 @@ extern "C" NB200_API int nb200_packed_fwd(const nb200_packed_params* p, void* cu
   if (int rc = check(p, "packed_fwd")) return rc;
   if (p->tokens_q == 0) return NB200_OK;
   if (int rc = check_operands(p, "packed_fwd", false)) return rc;
+  const PackedArgs a = lower(p);
+  if (int rc = check_workspace(p, a, NB200_PASS_FWD, "packed_fwd")) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  const PackedArgs a = lower(p);
+  if (tensor_cores(p, a, NB200_PASS_FWD)) return tc_packed_fwd(a, p->dtype, p->workspace, st);
   if (int rc = launch_clear_uncovered(a, p->dtype, false, st)) return rc;
   if (p->sequences == 0) return NB200_OK;
   return simt_packed_fwd(a, p->dtype, st);
@@ -83,14 +101,10 @@ extern "C" NB200_API int nb200_packed_bwd(const nb200_packed_params* p, void* cu
   if (int rc = check(p, "packed_bwd")) return rc;
   if (p->tokens_q == 0 && p->tokens_k == 0) return NB200_OK;
   if (int rc = check_operands(p, "packed_bwd", true)) return rc;
-  const size_t need = workspace(p, NB200_PASS_BWD);
-  if (need && (!p->workspace || p->workspace_bytes < need)) {
-    set_error("packed_bwd: workspace of %zu bytes needed (nb200_packed_workspace_bytes), %zu given", need, p->workspace_bytes);
-    return NB200_ERR_WORKSPACE;
-  }
+  PackedArgs a = lower(p);
+  if (int rc = check_workspace(p, a, NB200_PASS_BWD, "packed_bwd")) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  PackedArgs a = lower(p);
   a.delta = static_cast<float*>(p->workspace);
   if (int rc = launch_clear_uncovered(a, p->dtype, true, st)) return rc;
   if (p->sequences == 0) return NB200_OK;

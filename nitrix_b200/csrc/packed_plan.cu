@@ -1,0 +1,135 @@
+// Work lists of the tensor-core kernels of attention over packed sequences.
+//
+// The lengths are in device memory, so the blocks of all sequences are listed there: one CTA counts them by their length in
+// tiles (longest first, so that the short ones even out the end) and writes them in that order; blocks of one length come in
+// any order, which changes no result.  The other CTAs clear the outputs of tokens that belong to no sequence.
+#include "packed_tc.cuh"
+
+namespace nb200 {
+namespace packed {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kClearCtas = 31;
+constexpr int kBuckets = 1024;
+
+struct PlanArgs {
+  PackedArgs a;
+  int backward;
+  int block, step_tokens;
+  int shift;             // lengths in tiles are counted in units of 2^shift
+  int* count;
+  WorkItem* items;
+};
+
+template <typename Visit>
+__device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
+  const PackedArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int steps_before = 0;      // backward: 64-row steps of the sequences before, every warp for itself
+  int at = 0;
+  for (int s = warp; s < a.sequences; s += kPlanThreads / 32) {
+    const int2 q = sequence_span(a.offsets_q, s, a.tokens_q), k = sequence_span(a.offsets_k, s, a.tokens_k);
+    if (p.backward) {
+      int more = 0;
+      for (int i = at + lane; i < s; i += 32) more += (sequence_span(a.offsets_q, i, a.tokens_q).y + p.step_tokens - 1) / p.step_tokens;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+      steps_before += more;
+      at = s;
+    }
+    const int2 own = p.backward ? k : q, other = p.backward ? q : k;
+    const int shift = k.y - q.y;       // query i sees keys up to i + shift
+    for (int b = lane; int64_t(b) * p.block < own.y; b += 32) {
+      WorkItem w;
+      const int first = b * p.block;
+      w.begin = own.x + first;
+      w.n = min(p.block, own.y - first);
+      w.other = other.x;
+      w.other_n = other.y;
+      w.steps = steps_before;
+      w.pad[0] = w.pad[1] = 0;
+      int length;        // tokens of the other side
+      if (p.backward) {
+        w.seen = a.causal ? min(max(first - shift, 0), other.y) : 0;
+        length = other.y - w.seen;
+      } else {
+        w.seen = a.causal ? first + 1 + shift : other.y;
+        length = a.causal ? min(max(w.seen + w.n - 1, 0), other.y) : other.y;
+      }
+      visit(w, min((length / 128) >> p.shift, kBuckets - 1));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void clear_tail(T* base, int64_t first, int64_t end, T value) {
+  for (int64_t i = first + int64_t(blockIdx.x - 1) * kPlanThreads + threadIdx.x; i < end; i += int64_t(kClearCtas) * kPlanThreads) base[i] = value;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArgs p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const PackedArgs& a = p.a;
+  if (blockIdx.x > 0) {
+    const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D;
+    uint16_t* out = static_cast<uint16_t*>(p.backward ? a.dq : a.out);
+    clear_tail<uint16_t>(out, q0 * row, a.tokens_q * row, 0);      // (16-bit operands: zero has no bits)
+    if (!p.backward) {
+      clear_tail<float>(a.lse, q0 * a.heads, int64_t(a.tokens_q) * a.heads, -INFINITY);
+    } else {
+      const int64_t k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k), krow = int64_t(a.kv_heads) * a.D;
+      clear_tail<uint16_t>(static_cast<uint16_t*>(a.dk), k0 * krow, a.tokens_k * krow, 0);
+      clear_tail<uint16_t>(static_cast<uint16_t*>(a.dv), k0 * krow, a.tokens_k * krow, 0);
+    }
+    return;
+  }
+  __shared__ int buckets[kBuckets];      // blocks of each length, then the place of the next one
+  __shared__ int sums[32];
+  for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) buckets[i] = 0;
+  __syncthreads();
+  for_each_block(p, [&](const WorkItem&, int bucket) { atomicAdd(&buckets[bucket], 1); });
+  __syncthreads();
+  // places, longest first: thread t holds bucket kBuckets - 1 - t
+  static_assert(kBuckets == kPlanThreads, "a bucket per thread");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int own = buckets[kBuckets - 1 - threadIdx.x];
+  int upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += sums[w];
+  buckets[kBuckets - 1 - threadIdx.x] = upto - own;
+  if (threadIdx.x == kPlanThreads - 1) *p.count = upto;
+  __syncthreads();
+  for_each_block(p, [&](const WorkItem& w, int bucket) {
+    const int place = atomicAdd(&buckets[bucket], 1);
+    int4* dst = reinterpret_cast<int4*>(p.items + place);
+    dst[0] = make_int4(w.begin, w.n, w.other, w.other_n);
+    dst[1] = make_int4(w.seen, w.steps, 0, 0);
+  });
+}
+
+}  // namespace
+
+int launch_plan(const PackedArgs& a, int dtype, bool backward, int block, int step_tokens, void* list, cudaStream_t st) {
+  (void)dtype;
+  PlanArgs p{};
+  p.a = a;
+  p.backward = backward;
+  p.block = block;
+  p.step_tokens = step_tokens;
+  const int64_t most = (backward ? a.tokens_q : a.tokens_k) / 128;
+  while ((most >> p.shift) >= kBuckets) ++p.shift;
+  p.count = static_cast<int*>(list);
+  p.items = reinterpret_cast<WorkItem*>(static_cast<char*>(list) + 16);
+  packed_plan_kernel<<<1 + kClearCtas, kPlanThreads, 0, st>>>(p);
+  count_launch();
+  return check_launch("packed_plan_kernel");
+}
+
+}  // namespace packed
+}  // namespace nb200

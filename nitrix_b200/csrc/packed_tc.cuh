@@ -1,0 +1,62 @@
+// The tensor-core kernels of attention over packed sequences: work lists and launches.
+#pragma once
+
+#include "packed.cuh"
+#include "sdpa_tc_common.cuh"
+
+namespace nb200 {
+namespace packed {
+
+// One entry of a work list: a block of one sequence, for every key head.
+//   forward   queries q0 .. q0 + n of the packed tensor, of which the first sees the sequence's first `seen` keys (causal)
+//   backward  keys q0 .. q0 + n, of which the first is seen by the queries from `seen` on (counted within the sequence)
+struct __align__(16) WorkItem {
+  int begin;        // first token of the block
+  int n;            // tokens of the block
+  int other;        // first token of the sequence on the other side: its keys (forward), its queries (backward)
+  int other_n;      // tokens there
+  int seen;         // see above; all of them without causal
+  int steps;        // backward: first 64-row step of the sequence's rows in the gradient sums of dq
+  int pad[2];
+};
+static_assert(sizeof(WorkItem) == 32, "two 16-byte loads");
+
+// List in device memory: 16 bytes of header (the number of entries), then the entries, longest first.
+struct WorkList {
+  const int* count;
+  const WorkItem* items;
+};
+inline size_t work_list_bytes(int64_t most) { return (16 + size_t(most) * sizeof(WorkItem) + 255) / 256 * 256; }
+// most blocks of `block` tokens that sequences of `tokens` tokens together have
+inline int64_t most_blocks(int64_t tokens, int sequences, int block) { return tokens / block + sequences; }
+
+// Fills the list (and clears the outputs of tokens that no sequence covers, which would be a launch of its own).
+// `block`: queries (forward) or keys (backward) of a block; `step_tokens` (backward): queries of a 64-row step.
+int launch_plan(const PackedArgs& a, int dtype, bool backward, int block, int step_tokens, void* list, cudaStream_t st);
+
+// Rows of a query tile are, token after token, the query heads of one key head: this many tokens fit.
+__host__ __device__ inline int tile_tokens(int rows, int group) { return rows / group; }
+
+bool tc_packed_supported(const PackedArgs& a, int dtype);
+size_t tc_packed_fwd_bytes(const PackedArgs& a);
+int tc_packed_fwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ WorkItem load_item(const WorkItem* p) {
+  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
+  WorkItem w;
+  w.begin = a.x; w.n = a.y; w.other = a.z; w.other_n = a.w; w.seen = b.x; w.steps = b.y;
+  return w;
+}
+// Position of a CTA's `round`-th piece of work among `total` that are sorted by length and dealt in rows of gridDim.x that
+// alternate direction, so that nobody gets the longest of every row.  -1: none.
+__device__ __forceinline__ int dealt_position(int round, int total) {
+  const int G = int(gridDim.x), first = round * G;
+  if (first + int(blockIdx.x) >= total) return -1;
+  const bool full = first + G <= total;
+  return first + ((round & 1) && full ? G - 1 - int(blockIdx.x) : int(blockIdx.x));
+}
+#endif
+
+}  // namespace packed
+}  // namespace nb200

@@ -30,6 +30,11 @@ enum BiasMode : int {
 bool make_tile_map(CUtensorMap* map, const void* base, int rows, int cols, int H, int B, int64_t row_stride,
                    int64_t h_stride, int64_t b_stride, int box_rows, const char** why);
 
+// 4-D map (D, heads, tokens, 1) over 16-bit (tokens, heads, D) with unit stride on D: box = 64 columns x `box_heads` x
+// `box_tokens`, whose rows are, token after token, the heads of the token; otherwise as above.  Coordinates (column, head, token, 0).
+bool make_token_map(CUtensorMap* map, const void* base, int tokens, int heads, int D, int64_t token_stride, int64_t head_stride,
+                    int box_tokens, int box_heads);
+
 // 1 / scale as hi + lo, both exactly representable in the 16-bit operand type (lo = 0 for a power-of-two scale).
 // False when the scale is zero / not finite or 1 / scale overflows the type.
 bool split_inv_scale(float scale, bool bf16, float* hi, float* lo);

@@ -77,6 +77,21 @@ bool make_tile_map(CUtensorMap* map, const void* base, int rows, int cols, int H
   return true;
 }
 
+bool make_token_map(CUtensorMap* map, const void* base, int tokens, int heads, int D, int64_t token_stride, int64_t head_stride,
+                    int box_tokens, int box_heads) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  // (the stride of an axis of one element says nothing, and need not be one that the map can hold)
+  const int64_t hs = heads > 1 ? head_stride : D, ts = tokens > 1 ? token_stride : int64_t(heads) * D;
+  cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(tokens), 1};
+  cuuint64_t strides[3] = {cuuint64_t(hs) * 2, cuuint64_t(ts) * 2, cuuint64_t(ts) * 2};
+  cuuint32_t box[4] = {cuuint32_t(kSlotCols), cuuint32_t(box_heads), cuuint32_t(box_tokens), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // ---- mask packing -------------------------------------------------------------
 namespace {
 
