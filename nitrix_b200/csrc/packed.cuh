@@ -37,6 +37,33 @@ __device__ __forceinline__ int2 sequence_span(const int* offsets, int i, int tok
 __device__ __forceinline__ int covered_tokens(const int* offsets, int sequences, int tokens) {
   return sequences > 0 ? min(max(offsets[sequences], 0), tokens) : 0;
 }
+
+// The sequence that piece `index` of all sequences' `count(i)` pieces belongs to, and its number there (-1: there is no such
+// piece).  For a whole warp.
+struct Place {
+  int sequence, index;
+};
+template <typename Count>
+__device__ __forceinline__ Place find_place(int index, int sequences, Count count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < sequences; s0 += 32) {
+    int upto = s0 + lane < sequences ? count(s0 + lane) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    const unsigned above = __ballot_sync(0xffffffffu, before + upto > index);
+    if (above) {
+      const int j = __ffs(above) - 1;
+      const int prev = __shfl_sync(0xffffffffu, upto, j > 0 ? j - 1 : 0);
+      return Place{s0 + j, index - before - (j > 0 ? prev : 0)};
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Place{0, -1};
+}
 #endif
 
 // out = zeros for the tokens behind the last sequence (and lse = -inf, where `lse` is given): part of every pass

@@ -37,12 +37,13 @@ PackedArgs lower(const nb200_packed_params* p) {
 size_t delta_bytes(const nb200_packed_params* p) { return (size_t(p->tokens_q) * size_t(p->heads) * sizeof(float) + 255) / 256 * 256; }
 
 bool tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
-  return pass == NB200_PASS_FWD && p->kernel == NB200_KERNEL_AUTO && tc_packed_supported(a, p->dtype);
+  if (p->kernel != NB200_KERNEL_AUTO) return false;
+  return pass == NB200_PASS_FWD ? tc_packed_supported(a, p->dtype) : tc_packed_bwd_supported(a, p->dtype);
 }
 
 size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
-  if (pass == NB200_PASS_BWD) return delta_bytes(p);
-  return tensor_cores(p, a, pass) ? tc_packed_fwd_bytes(a) : 0;
+  if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a);
+  return pass == NB200_PASS_FWD ? 0 : delta_bytes(p);
 }
 
 int check_workspace(const nb200_packed_params* p, const PackedArgs& a, int pass, const char* what) {
@@ -105,6 +106,7 @@ extern "C" NB200_API int nb200_packed_bwd(const nb200_packed_params* p, void* cu
   if (int rc = check_workspace(p, a, NB200_PASS_BWD, "packed_bwd")) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
+  if (tensor_cores(p, a, NB200_PASS_BWD)) return tc_packed_bwd(a, p->dtype, p->workspace, st);
   a.delta = static_cast<float*>(p->workspace);
   if (int rc = launch_clear_uncovered(a, p->dtype, true, st)) return rc;
   if (p->sequences == 0) return NB200_OK;

@@ -18,6 +18,10 @@ struct PlanArgs {
   int backward;
   int block, step_tokens;
   int shift;             // lengths in tiles are counted in units of 2^shift
+  // Entries and (backward) steps that there is room for: as many as sequences that follow one another have.  Offsets that run
+  // backwards describe sequences that overlap, of which those that do not fit are left out.
+  int most;
+  int64_t most_steps;
   int* count;
   WorkItem* items;
 };
@@ -26,18 +30,19 @@ template <typename Visit>
 __device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
   const PackedArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int steps_before = 0;      // backward: 64-row steps of the sequences before, every warp for itself
+  int64_t steps_before = 0;  // backward: 64-row steps of the sequences before, every warp for itself
   int at = 0;
   for (int s = warp; s < a.sequences; s += kPlanThreads / 32) {
     const int2 q = sequence_span(a.offsets_q, s, a.tokens_q), k = sequence_span(a.offsets_k, s, a.tokens_k);
     if (p.backward) {
-      int more = 0;
+      int64_t more = 0;
       for (int i = at + lane; i < s; i += 32) more += (sequence_span(a.offsets_q, i, a.tokens_q).y + p.step_tokens - 1) / p.step_tokens;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
       steps_before += more;
       at = s;
     }
+    if (p.backward && steps_before + (q.y + p.step_tokens - 1) / p.step_tokens > p.most_steps) break;
     const int2 own = p.backward ? k : q, other = p.backward ? q : k;
     const int shift = k.y - q.y;       // query i sees keys up to i + shift
     for (int b = lane; int64_t(b) * p.block < own.y; b += 32) {
@@ -47,14 +52,14 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
       w.n = min(p.block, own.y - first);
       w.other = other.x;
       w.other_n = other.y;
-      w.steps = steps_before;
+      w.steps = int(steps_before);
       w.pad[0] = w.pad[1] = 0;
       int length;        // tokens of the other side
       if (p.backward) {
-        w.seen = a.causal ? min(max(first - shift, 0), other.y) : 0;
-        length = other.y - w.seen;
+        w.seen = first - shift;
+        length = other.y - (a.causal ? min(max(w.seen, 0), other.y) : 0);
       } else {
-        w.seen = a.causal ? first + 1 + shift : other.y;
+        w.seen = first + 1 + shift;
         length = a.causal ? min(max(w.seen + w.n - 1, 0), other.y) : other.y;
       }
       visit(w, min((length / 128) >> p.shift, kBuckets - 1));
@@ -103,10 +108,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
   __syncthreads();
   for (int w = 0; w < warp; ++w) upto += sums[w];
   buckets[kBuckets - 1 - threadIdx.x] = upto - own;
-  if (threadIdx.x == kPlanThreads - 1) *p.count = upto;
+  if (threadIdx.x == kPlanThreads - 1) *p.count = min(upto, p.most);
   __syncthreads();
   for_each_block(p, [&](const WorkItem& w, int bucket) {
     const int place = atomicAdd(&buckets[bucket], 1);
+    if (place >= p.most) return;
     int4* dst = reinterpret_cast<int4*>(p.items + place);
     dst[0] = make_int4(w.begin, w.n, w.other, w.other_n);
     dst[1] = make_int4(w.seen, w.steps, 0, 0);
@@ -115,15 +121,16 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
 
 }  // namespace
 
-int launch_plan(const PackedArgs& a, int dtype, bool backward, int block, int step_tokens, void* list, cudaStream_t st) {
-  (void)dtype;
+int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st) {
   PlanArgs p{};
   p.a = a;
   p.backward = backward;
   p.block = block;
   p.step_tokens = step_tokens;
-  const int64_t most = (backward ? a.tokens_q : a.tokens_k) / 128;
-  while ((most >> p.shift) >= kBuckets) ++p.shift;
+  const int64_t tiles = (backward ? a.tokens_q : a.tokens_k) / 128;
+  while ((tiles >> p.shift) >= kBuckets) ++p.shift;
+  p.most = int(most_blocks(backward ? a.tokens_k : a.tokens_q, a.sequences, block));
+  p.most_steps = most_blocks(a.tokens_q, a.sequences, step_tokens);
   p.count = static_cast<int*>(list);
   p.items = reinterpret_cast<WorkItem*>(static_cast<char*>(list) + 16);
   packed_plan_kernel<<<1 + kClearCtas, kPlanThreads, 0, st>>>(p);

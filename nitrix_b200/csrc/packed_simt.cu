@@ -30,33 +30,6 @@ struct Tile {
   static constexpr int kScores = kT * kPStride;
 };
 
-// The tile this CTA works on: tile `index` over all sequences' `count(i)` rows.
-struct Place {
-  int sequence;
-  int tile;          // within the sequence; -1: none
-};
-template <int kT, typename Count>
-__device__ __forceinline__ Place find_tile(int index, int sequences, Count count) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int s0 = 0; s0 < sequences; s0 += 32) {
-    int upto = s0 + lane < sequences ? int((count(s0 + lane) + kT - 1) / kT) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
-    }
-    const unsigned above = __ballot_sync(0xffffffffu, before + upto > index);
-    if (above) {
-      const int j = __ffs(above) - 1;
-      const int prev = __shfl_sync(0xffffffffu, upto, j > 0 ? j - 1 : 0);
-      return Place{s0 + j, index - before - (j > 0 ? prev : 0)};
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return Place{0, -1};
-}
-
 // rows 0 .. n - 1 of a tile from `offset(row)` elements on; zeros elsewhere
 template <typename T, int kD, typename Offset>
 __device__ __forceinline__ void load_tile(float* dst, const void* base, int n, int D, Offset offset) {
@@ -163,10 +136,10 @@ __global__ void __launch_bounds__(kThreads) packed_fwd_simt_kernel(const PackedA
   using L = Tile<kD>;
   extern __shared__ __align__(16) float smem[];
   float *sq = smem, *sk = sq + L::kOperand, *sv = sk + L::kOperand, *sp = sv + L::kOperand;
-  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group; });
-  if (place.tile < 0) return;
+  const Place place = find_place(blockIdx.x, a.sequences, [&](int i) { return int((int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group + L::kT - 1) / L::kT); });
+  if (place.index < 0) return;
   const Rows rows(a, place.sequence, blockIdx.y);
-  const int64_t r0 = int64_t(place.tile) * L::kT;
+  const int64_t r0 = int64_t(place.index) * L::kT;
   const int n = int(min(int64_t(L::kT), rows.n - r0));
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float mul = a.scale * kLog2e;
@@ -270,10 +243,10 @@ __global__ void __launch_bounds__(kThreads) packed_dq_simt_kernel(const PackedAr
   __shared__ float stat[2 * L::kT];
   __shared__ int seen[L::kT];
   float *sq = smem, *sdo = sq + L::kOperand, *sk = sdo + L::kOperand, *sv = sk + L::kOperand, *sds = sv + L::kOperand;
-  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group; });
-  if (place.tile < 0) return;
+  const Place place = find_place(blockIdx.x, a.sequences, [&](int i) { return int((int64_t(sequence_span(a.offsets_q, i, a.tokens_q).y) * a.group + L::kT - 1) / L::kT); });
+  if (place.index < 0) return;
   const Rows rows(a, place.sequence, blockIdx.y);
-  const int64_t r0 = int64_t(place.tile) * L::kT;
+  const int64_t r0 = int64_t(place.index) * L::kT;
   const int n = int(min(int64_t(L::kT), rows.n - r0));
   const int ty = threadIdx.x >> 4;
   load_tile<T, kD>(sq, a.q, n, a.D, [&](int r) { return rows.at(r0 + r, a.qs); });
@@ -307,10 +280,10 @@ __global__ void __launch_bounds__(kThreads) packed_dkv_simt_kernel(const PackedA
   __shared__ int seen[L::kT];
   float *sq = smem, *sdo = sq + L::kOperand, *sk = sdo + L::kOperand, *sv = sk + L::kOperand, *sp = sv + L::kOperand,
         *sds = sp + L::kScores;
-  const Place place = find_tile<L::kT>(blockIdx.x, a.sequences, [&](int i) { return int64_t(sequence_span(a.offsets_k, i, a.tokens_k).y); });
-  if (place.tile < 0) return;
+  const Place place = find_place(blockIdx.x, a.sequences, [&](int i) { return int((int64_t(sequence_span(a.offsets_k, i, a.tokens_k).y) + L::kT - 1) / L::kT); });
+  if (place.index < 0) return;
   const Rows rows(a, place.sequence, blockIdx.y);
-  const int k0 = place.tile * L::kT, nk = min(L::kT, rows.k.y - k0);
+  const int k0 = place.index * L::kT, nk = min(L::kT, rows.k.y - k0);
   const int ty = threadIdx.x >> 4;
   load_tile<T, kD>(sk, a.k, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.ks[0] + rows.kv_head * a.ks[1]; });
   load_tile<T, kD>(sv, a.v, nk, a.D, [&](int r) { return (int64_t(rows.k.x) + k0 + r) * a.vs[0] + rows.kv_head * a.vs[1]; });

@@ -8,14 +8,15 @@ namespace nb200 {
 namespace packed {
 
 // One entry of a work list: a block of one sequence, for every key head.
-//   forward   queries q0 .. q0 + n of the packed tensor, of which the first sees the sequence's first `seen` keys (causal)
-//   backward  keys q0 .. q0 + n, of which the first is seen by the queries from `seen` on (counted within the sequence)
+//   forward   queries begin .. begin + n of the packed tensor, of which the first sees the sequence's first `seen` keys (causal)
+//   backward  keys begin .. begin + n, of which the first is seen by the queries from `seen` on (counted within the sequence)
+// Under causal `seen` may lie outside the sequence; it means nothing otherwise.
 struct __align__(16) WorkItem {
   int begin;        // first token of the block
   int n;            // tokens of the block
   int other;        // first token of the sequence on the other side: its keys (forward), its queries (backward)
   int other_n;      // tokens there
-  int seen;         // see above; all of them without causal
+  int seen;         // see above
   int steps;        // backward: first 64-row step of the sequence's rows in the gradient sums of dq
   int pad[2];
 };
@@ -32,7 +33,7 @@ inline int64_t most_blocks(int64_t tokens, int sequences, int block) { return to
 
 // Fills the list (and clears the outputs of tokens that no sequence covers, which would be a launch of its own).
 // `block`: queries (forward) or keys (backward) of a block; `step_tokens` (backward): queries of a 64-row step.
-int launch_plan(const PackedArgs& a, int dtype, bool backward, int block, int step_tokens, void* list, cudaStream_t st);
+int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st);
 
 // Rows of a query tile are, token after token, the query heads of one key head: this many tokens fit.
 __host__ __device__ inline int tile_tokens(int rows, int group) { return rows / group; }
@@ -40,6 +41,9 @@ __host__ __device__ inline int tile_tokens(int rows, int group) { return rows / 
 bool tc_packed_supported(const PackedArgs& a, int dtype);
 size_t tc_packed_fwd_bytes(const PackedArgs& a);
 int tc_packed_fwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
+bool tc_packed_bwd_supported(const PackedArgs& a, int dtype);
+size_t tc_packed_bwd_bytes(const PackedArgs& a);
+int tc_packed_bwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ WorkItem load_item(const WorkItem* p) {

@@ -592,6 +592,10 @@ bool tc_packed_supported(const PackedArgs& a, int dtype) {
          strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads);
 }
 
+bool tc_packed_bwd_supported(const PackedArgs& a, int dtype) {
+  return tc_packed_supported(a, dtype) && strides_fit(a.dout, a.dos, a.tokens_q, a.heads);
+}
+
 size_t tc_packed_fwd_bytes(const PackedArgs& a) {
   return work_list_bytes(most_blocks(a.tokens_q, a.sequences, 2 * tile_tokens(kTile, a.group)));
 }
@@ -599,7 +603,7 @@ size_t tc_packed_fwd_bytes(const PackedArgs& a) {
 int tc_packed_fwd(const PackedArgs& p, int dtype, void* ws, cudaStream_t st) {
   FwdArgs a{};
   a.tokens = tile_tokens(kTile, p.group);
-  if (int rc = launch_plan(p, dtype, false, 2 * a.tokens, 1, ws, st)) return rc;
+  if (int rc = launch_plan(p, false, 2 * a.tokens, 1, ws, st)) return rc;
   CUtensorMap tq, tk, tv;
   if (!make_token_map(&tq, p.q, p.tokens_q, p.heads, p.D, p.qs[0], p.qs[1], a.tokens, p.group) ||
       !make_token_map(&tk, p.k, p.tokens_k, p.kv_heads, p.D, p.ks[0], p.ks[1], kTile, 1) ||

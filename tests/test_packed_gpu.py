@@ -234,6 +234,21 @@ def test_streams_and_graphs():
     assert torch.equal(again, packed_attention(q, k, v, _offsets(other)))
 
 
+def test_offsets_that_make_no_sense_stay_in_bounds():
+    """Offsets that run backwards, overlap or leave the tensors: no access outside, no hang; what comes out means nothing."""
+    from nitrix_b200 import _cabi
+    from nitrix_b200.nn import packed_attention
+
+    q, k, v, dout = _inputs([300], [300], 6, 2, 64, torch.bfloat16)
+    for bad in ([0, 300] * 40, [0, 900, -5, 20, 7, 300], [300, 0, 300, 0, 300], [-(1 << 30), 1 << 30, 0, 1 << 30], [50, 60]):
+        off = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        for backend in ("auto", "cuda-simt"):
+            leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+            torch.autograd.grad(packed_attention(*leaves, off, backend=backend), leaves, dout)
+    torch.cuda.synchronize()
+    assert _cabi.lib().nb200_device_status(0) == 0
+
+
 def test_refusals():
     from nitrix_b200.nn import packed_attention
 
