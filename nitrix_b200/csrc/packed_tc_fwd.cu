@@ -13,7 +13,7 @@
 // behind the end are masked by selection, and rows of Q behind the end stay in rows that nobody stores); 2 and 3 issue the
 // MMAs of query tile 0 and 1; the others are the softmax, one thread per row at head dim 128, two at 64.  The scheme of the
 // tiles -- halves of 64 keys whose P overwrites S at head dim 128, separate P at 64, a reference maximum that moves only past
-// 2^8, every fourth pair of exponentials on the FMA units at head dim 128 -- is that of sdpa_tc_fwd.cu, which has the reasons.
+// 2^8, every third pair of exponentials on the FMA units at head dim 128 -- is that of sdpa_tc_fwd.cu, which has the reasons.
 // Bound by the exponentials and the packing of P as that kernel is.
 // All waits on mbarriers are bounded (sdpa_tc_common.cuh).
 #include <type_traits>
@@ -52,7 +52,9 @@ struct Split {
   static_assert((kLaunchRegs - kProducerRegs) * 128 >= (kSoftmaxRegs - kLaunchRegs) * 256 * kHalves,
                 "softmax warps would wait forever for registers the producer warps never release");
 };
-constexpr int kPolyPeriod = 4;
+// D = 128: one pair of exponentials in this many on the FMA units (every second 491 us, fourth 477, third 471 and 240 causal: 8192
+// tokens, 16 heads on 4).  None at 64, where every fourth or eighth changes nothing and every sixteenth costs 8 %.
+constexpr int kPolyPeriod = 3;
 
 template <int D>
 struct FwdSmem {
@@ -161,8 +163,8 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   //   tc_g tiles query tile g has processed     -> phase of s_full / p_ready / s_free / pv_done
   //   oc_g blocks in which query tile g had any -> phase of q_full / q_empty / o_done / o_free
   //   clear: bit s is the phase of v_clear[s], which sees the tails only
-  Item it;
   if (warp < 4) {
+  Item it;
   reg_dealloc<Split<D>::kProducerRegs>();
   if (warp == 0) {
     // ---------------- Q / K / V ----------------
@@ -374,11 +376,17 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 
     // A warp that gives up (`ok` false) waits no more and stores nothing, but walks on through its passes: its partner waits
     // for it at the pair's barrier, which has no time limit of its own.
-    for (int round = 0; decode_item(a, round, count, &it); ++round) {
-      const int my_nt = it.nt(g);
-      const bool live = token < it.tokens(g);
-      const int local = g * a.tokens + token;            // query of the block
-      const int seen = a.causal ? min(it.seen + local, it.lk) : it.lk;
+    for (int round = 0;; ++round) {
+      // of the block only what the passes and the epilogue need: a spilled register costs more than anything here (head dim 64)
+      int my_nt, seen, row;
+      {
+        Item it;
+        if (!decode_item(a, round, count, &it)) break;
+        const int local = g * a.tokens + token;            // query of the block
+        my_nt = it.nt(g);
+        seen = a.causal ? min(it.seen + local, it.lk) : it.lk;
+        row = token < it.tokens(g) ? (it.q0 + local) * a.heads + it.head * a.group + in_group : -1;   // of out; -1: none
+      }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < my_nt; ++j) {
         const int gt = tc + j;
@@ -472,7 +480,8 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
       }
 
-      // ---------------- epilogue: out = O / l, lse = m mul + log2 l; zeros where no key was seen ----------------
+      // ---------------- epilogue: out = O / l, lse = m mul + log2 l ----------------
+      uint8_t* const orow = static_cast<uint8_t*>(a.out) + 2 * (int64_t(row) * D + half * kOutCols);
       if (my_nt > 0) {
         if constexpr (kHalves == 2) {
           if (half == 0) *xrow = l;
@@ -482,17 +491,12 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (half == 0) l = *xrow;
         }
         ok = ok && wait_or_abort(bar(O_DONE + g), oc & 1, abort_flag, a.status, 410);
-      }
-      if (ok && it.tokens(g) > 0) {
-        tc_fence_after_sync();
-        const bool empty = seen <= 0;
-        const float inv = 1.f / l;
-        const int64_t row = (int64_t(it.q0) + local) * a.heads + it.head * a.group + in_group;
-        uint8_t* orow = static_cast<uint8_t*>(a.out) + 2 * (row * D + half * kOutCols);
+        if (ok) {
+          tc_fence_after_sync();
+          const float inv = 1.f / l;
 #pragma unroll
-        for (int c = 0; c < kOutCols / 32; ++c) {
-          uint32_t o[32];
-          if (my_nt > 0) {
+          for (int c = 0; c < kOutCols / 32; ++c) {
+            uint32_t o[32];
             tmem_ld32(tO + c * 32, o);
             tmem_wait_ld();
             if (c == kOutCols / 32 - 1) {
@@ -500,28 +504,31 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
               __syncwarp();
               if (lane == 0) mbar_arrive(bar(O_FREE + g));
             }
-          }
-          if (live) {
-            uint4 w[4];
+            if (row >= 0) {
+              uint4 w[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4& x = w[i >> 3];
-              x.x = pack2<kBf16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-              x.y = pack2<kBf16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-              x.z = pack2<kBf16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-              x.w = pack2<kBf16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-              if (empty) x = make_uint4(0, 0, 0, 0);
-            }
-            if (a.out_v8) {
-              st_global_v8(orow + c * 64, w[0], w[1]);
-              st_global_v8(orow + c * 64 + 32, w[2], w[3]);
-            } else {
+              for (int i = 0; i < 32; i += 8) {
+                uint4& x = w[i >> 3];
+                x.x = pack2<kBf16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                x.y = pack2<kBf16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                x.z = pack2<kBf16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                x.w = pack2<kBf16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+              }
+              if (a.out_v8) {
+                st_global_v8(orow + c * 64, w[0], w[1]);
+                st_global_v8(orow + c * 64 + 32, w[2], w[3]);
+              } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(orow + c * 64 + i * 16) = w[i];
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(orow + c * 64 + i * 16) = w[i];
+              }
             }
           }
+          if (half == 0 && row >= 0) a.lse[row] = m * mul + log2f(l);
         }
-        if (half == 0 && live) a.lse[row] = empty ? -INFINITY : m * mul + log2f(l);
+      }
+      if (ok && seen <= 0 && row >= 0) {      // no key: zeros
+        for (int i = 0; i < kOutCols / 8; ++i) reinterpret_cast<uint4*>(orow)[i] = make_uint4(0, 0, 0, 0);
+        if (half == 0) a.lse[row] = -INFINITY;
       }
       tc += my_nt;
       oc += my_nt > 0 ? 1 : 0;
@@ -588,7 +595,7 @@ bool strides_fit(const void* base, const int64_t (&s)[2], int tokens, int heads)
 // A group's heads of one token have to fit a tile (64 rows in the backward).
 bool tc_packed_supported(const PackedArgs& a, int dtype) {
   return dtype != NB200_F32 && (a.D == 64 || a.D == 128) && a.group <= 64 && a.scale > 0.f && a.scale < 1e30f &&
-         a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
+         int64_t(a.tokens_q) * a.heads <= 0x7fffffff && a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
          strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads);
 }
 
