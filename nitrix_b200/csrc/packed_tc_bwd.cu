@@ -530,29 +530,40 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   }
 }
 
-// delta[token][head] = sum_d out dout in fp32: D / 8 lanes per row, 16 bytes each
+// delta[token][head] = sum_d out dout in fp32.  Bound by HBM: D / 8 lanes per row with 16 bytes of each tensor, four rows per
+// lane whose loads are in flight together.
+constexpr int kDeltaThreads = 256, kDeltaRows = 4;
+
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(256) packed_delta_tc_kernel(const PackedArgs a) {
-  constexpr int kLanes = D / 8;
-  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int c = threadIdx.x % kLanes;
-  const bool in = row < int64_t(a.tokens_q) * a.heads;
-  float sum = 0.f;
-  if (in) {
-    const int64_t token = row / a.heads;
-    const int head = int(row - token * a.heads);
-    const uint4 o = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + row * D) + c);
-    const uint4 g = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + token * a.dos[0] + head * a.dos[1]) + c);
-    const uint32_t ow[4] = {o.x, o.y, o.z, o.w}, gw[4] = {g.x, g.y, g.z, g.w};
+__global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const PackedArgs a) {
+  constexpr int kLanes = D / 8, kGroups = kDeltaThreads / kLanes;
+  const int rows = a.tokens_q * a.heads;      // (below 2^31: checked on the host)
+  const int row0 = blockIdx.x * (kGroups * kDeltaRows) + int(threadIdx.x) / kLanes, c = threadIdx.x % kLanes;
+  uint4 o[kDeltaRows], g[kDeltaRows];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = unpack2<kBf16>(ow[i]), y = unpack2<kBf16>(gw[i]);
-      sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const int row = row0 + i * kGroups;
+    o[i] = g[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
+      const int token = row / a.heads, head = row - token * a.heads;
+      o[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + int64_t(row) * D) + c);
+      g[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + token * a.dos[0] + head * a.dos[1]) + c);
     }
   }
 #pragma unroll
-  for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (in && c == 0) a.delta[row] = sum;
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = unpack2<kBf16>(ow[j]), y = unpack2<kBf16>(gw[j]);
+      sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+    }
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const int row = row0 + i * kGroups;
+    if (row < rows && c == 0) a.delta[row] = sum;
+  }
 }
 
 // dq = scale * (fp32 sums) in the operand type: one CTA per step and key head; a thread takes four rows x eight d (eight
@@ -560,14 +571,14 @@ __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const PackedArgs a
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kStep / 4 * (D / 8)) packed_dq_finish_kernel(const PackedArgs a, const float* __restrict__ acc,
                                                                                 int64_t all_steps, int tokens) {
+  const int head = blockIdx.y, dchunk = threadIdx.x % (D / 8), rg = threadIdx.x / (D / 8);
+  const float* src = acc + (int64_t(head) * all_steps + blockIdx.x) * (kStep * D) + rg * (D * 4) + dchunk * 32;
+  float4 v[8];      // in flight while the step's sequence is looked for
+#pragma unroll
+  for (int d = 0; d < 8; ++d) v[d] = __ldcs(reinterpret_cast<const float4*>(src) + d);
   const Place place = find_place(int(blockIdx.x), a.sequences, [&](int i) { return (sequence_span(a.offsets_q, i, a.tokens_q).y + tokens - 1) / tokens; });
   if (place.index < 0) return;
   const int2 q = sequence_span(a.offsets_q, place.sequence, a.tokens_q);
-  const int head = blockIdx.y, dchunk = threadIdx.x % (D / 8), rg = threadIdx.x / (D / 8);
-  const float* src = acc + (int64_t(head) * all_steps + blockIdx.x) * (kStep * D) + rg * (D * 4) + dchunk * 32;
-  float4 v[8];
-#pragma unroll
-  for (int d = 0; d < 8; ++d) v[d] = __ldg(reinterpret_cast<const float4*>(src) + d);
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
     const int row = rg * 4 + rr, t = row / a.group, token = place.index * tokens + t;
@@ -619,9 +630,10 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   float* acc = reinterpret_cast<float*>(base + delta_bytes(p) + list_bytes(p));
   BwdArgs a{};
   a.tokens = tile_tokens(kStep, p.group);
-  const int64_t delta_rows = int64_t(p.tokens_q) * p.heads, delta_grid = (delta_rows * (D / 8) + 255) / 256;
+  constexpr int kDeltaCta = kDeltaThreads / (D / 8) * kDeltaRows;      // rows
+  const int64_t delta_grid = (int64_t(p.tokens_q) * p.heads + kDeltaCta - 1) / kDeltaCta;
   if (cudaMemsetAsync(acc, 0, acc_bytes(p), st) != cudaSuccess) return check_launch("packed_bwd: clearing the sums of dq");
-  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid), 256, 0, st>>>(p);
+  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid), kDeltaThreads, 0, st>>>(p);
   count_launch();
   if (int rc = check_launch("packed_delta_tc_kernel")) return rc;
   if (int rc = launch_plan(p, true, kTile, a.tokens, list, st)) return rc;
