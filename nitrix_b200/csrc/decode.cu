@@ -47,7 +47,7 @@ struct DecodeArgs {
   int chunks;                // runs of query heads that a key head's group is taken in
   float mul;                 // scale * log2 e
   int unit;                  // tokens per unit of work
-  float* part;               // pieces: [2 * CTAs][heads of a chunk][D + 2]: output, maximum (base 2), sum
+  float* part;               // pieces: [2 * CTAs][heads of a chunk][D + 4]: output, maximum (base 2), sum
   int workers;               // most CTAs of the main kernel that get work
 };
 
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
     }
     __syncthreads();
     // the CTA's result: sums over the slots, relative to their largest maximum
-    float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * Loop::kHeads * (a.D + 2);
+    float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * Loop::kHeads * (a.D + 4);
     for (int i = threadIdx.x; i < heads * a.D; i += kThreads) {
       const int h = i / a.D, d = i - h * a.D;
       const float* col = merge + h * (a.D + 2);
@@ -457,11 +457,8 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
       if (whole) {
         static_cast<T*>(a.out)[(int64_t(row) * a.q_heads + head0 + h) * a.D + d] = from_f32<T>(acc / sum);
       } else {
-        part[h * (a.D + 2) + d] = acc;
-        if (d == 0) {
-          part[h * (a.D + 2) + a.D] = mx;
-          part[h * (a.D + 2) + a.D + 1] = sum;
-        }
+        part[h * (a.D + 4) + d] = acc;
+        if (d == 0) *reinterpret_cast<float2*>(part + h * (a.D + 4) + a.D) = make_float2(mx, sum);
       }
     }
     __syncthreads();
@@ -470,15 +467,19 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
   }
 }
 
-// One CTA per (row, query head): the pieces of its item, in order; zeros for a sequence without a token.
+// One CTA per (row, query head): the pieces of its item, zeros for a sequence without a token.  A warp takes every fourth
+// piece, a lane 16-byte words of it; the warps' sums are added in their order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a, int heads_per_chunk) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
+  constexpr int kMaxWords = 64;             // 16-byte words of a head of 256
+  __shared__ float4 outs[kWarps][kMaxWords];
+  __shared__ float sums[kWarps], tops[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.y, head = blockIdx.x;
   T* out = static_cast<T*>(a.out) + (int64_t(row) * a.q_heads + head) * a.D;
   const int units = units_of(a, row);
   if (units == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int d = threadIdx.x; d < a.D; d += kThreads) out[d] = from_f32<T>(0.f);
     return;
   }
@@ -499,27 +500,75 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
   const int chunk = in_group / heads_per_chunk, h = in_group - chunk * heads_per_chunk;
   const int64_t begin = before + int64_t(kv_head * a.chunks + chunk) * units;
   const int w0 = share.worker_of(begin), w1 = share.worker_of(begin + units - 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // (the lengths are the caller's: what is above needs no wait)
   if (w0 == w1) return;                  // finished by the CTA that had all of it
-  const int64_t step = int64_t(heads_per_chunk) * (a.D + 2);
+  const int64_t step = int64_t(heads_per_chunk) * (a.D + 4);
   // the first piece begins the item (slot 1 of its worker); the others begin inside it (slot 0)
-  auto piece = [&](int w) { return a.part + (2 * int64_t(w) + (w == w0 ? 1 : 0)) * step + h * (a.D + 2); };
-  float mx = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) mx = fmaxf(mx, piece(w)[a.D]);
+  auto piece = [&](int w) { return a.part + (2 * int64_t(w) + (w == w0 ? 1 : 0)) * step + h * (a.D + 4); };
+  const int words = a.D / 4;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  constexpr int kAhead = 4;
+  for (int w = w0 + warp; w <= w1; w += kWarps * kAhead) {
+    float2 st[kAhead];
+    float4 v[kAhead][2];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float shift = mx == -INFINITY ? 0.f : mx;
-  for (int d = threadIdx.x; d < a.D; d += kThreads) {
-    float sum = 0.f, acc = 0.f;
-    for (int w = w0; w <= w1; ++w) {
-      const float* p = piece(w);
-      const float f = ex2(p[a.D] - shift);
-      sum = fmaf(f, p[a.D + 1], sum);
-      acc = fmaf(f, p[d], acc);
+    for (int j = 0; j < kAhead; ++j) {
+      const int wj = w + j * kWarps;
+      st[j] = make_float2(-INFINITY, 0.f);
+      if (wj > w1) continue;
+      const float* p = piece(wj);
+      st[j] = *reinterpret_cast<const float2*>(p + a.D);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + 32 * i < words) v[j][i] = reinterpret_cast<const float4*>(p)[lane + 32 * i];
     }
-    out[d] = from_f32<T>(acc / sum);
+    float next = top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) next = fmaxf(next, st[j].x);
+    const float shift = next == -INFINITY ? 0.f : next, old = ex2(top - shift);
+    sum *= old;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { acc[i].x *= old; acc[i].y *= old; acc[i].z *= old; acc[i].w *= old; }
+    top = next;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (w + j * kWarps > w1) continue;
+      const float f = ex2(st[j].x - shift);
+      sum = fmaf(f, st[j].y, sum);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (lane + 32 * i >= words) continue;
+        acc[i].x = fmaf(f, v[j][i].x, acc[i].x); acc[i].y = fmaf(f, v[j][i].y, acc[i].y);
+        acc[i].z = fmaf(f, v[j][i].z, acc[i].z); acc[i].w = fmaf(f, v[j][i].w, acc[i].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 32 * i < words) outs[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) {
+    sums[warp] = sum;
+    tops[warp] = top;
+  }
+  __syncthreads();
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) most = fmaxf(most, tops[i]);
+  const float shift = most == -INFINITY ? 0.f : most;
+  float f[kWarps], all = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    f[i] = ex2(tops[i] - shift);
+    all = fmaf(f[i], sums[i], all);
+  }
+  for (int d = threadIdx.x; d < a.D; d += kThreads) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) x = fmaf(f[i], reinterpret_cast<const float*>(outs[i])[d], x);
+    out[d] = from_f32<T>(x / all);
   }
 }
-
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -563,7 +612,7 @@ Plan plan(const nb200_decode_params* p) {
   const int64_t units = (int64_t(p->width) * c.page_size + pl.unit - 1) / pl.unit * p->rows * c.heads * chunks;
   const int64_t most = int64_t(tc::sm_count()) * ctas;
   pl.workers = int(units < most ? (units > 0 ? units : 1) : most);
-  pl.bytes = size_t(pl.workers) * 2 * pl.heads * (c.head_dim + 2) * sizeof(float);
+  pl.bytes = size_t(pl.workers) * 2 * pl.heads * (c.head_dim + 4) * sizeof(float);
   return pl;
 }
 

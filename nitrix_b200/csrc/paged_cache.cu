@@ -183,11 +183,11 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
 }
 
 // ---- fork and compact -----------------------------------------------------------------------------------------------------
-// Workspace: [0] dropped tokens, [1 .. 4) unused, then one bit per page (live), then (compact) the live pages before each
-// word of bits, then the free pages in ascending order.
+// Workspace: [0] dropped tokens, [1] pages to move, [2 .. 4) unused, then one bit per page (live), then (compact) the live pages
+// before each word of bits, the free pages in ascending order, the live pages that move in ascending order.
 struct Layout {
-  int words;                         // of 32 pages
-  size_t bits, before, holes, total; // offsets in ints
+  int words;                                  // of 32 pages
+  size_t bits, before, holes, moves, total;   // offsets in ints
 };
 Layout layout(int pages) {
   Layout l{};
@@ -195,7 +195,8 @@ Layout layout(int pages) {
   l.bits = 4;
   l.before = l.bits + size_t(l.words);
   l.holes = l.before + size_t(l.words);
-  l.total = l.holes + size_t(pages);
+  l.moves = l.holes + size_t(pages);
+  l.total = l.moves + size_t(pages);
   return l;
 }
 
@@ -217,6 +218,8 @@ struct MoveArgs {
   unsigned* bits;
   int* before;
   int* holes;
+  int* moves;
+  int* n_moves;
 };
 
 __device__ __forceinline__ int parent_of(const MoveArgs& a, int row) {
@@ -328,12 +331,14 @@ __global__ void __launch_bounds__(kThreads) cache_mark_kernel(const MoveArgs a) 
 constexpr int kListWords = 64;      // words of bits per CTA of the listing kernel
 
 // The pages without a bit, ascending, -1 behind them.  Every CTA counts the bits before its own anew, which costs a reading of
-// the bits (32 KB for 256 K pages) and saves a launch.
-__global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, int words, int* list, int* range, int* before) {
-  __shared__ int sums[2];
+// the bits (32 KB for 256 K pages) and saves a launch.  For compact: also the live pages before each word, and the live pages
+// that have to move, which are those at or behind the number of live ones.
+template <bool kCompact>
+__global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, int words, int* list, int* range) {
+  __shared__ int sums[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w0 = blockIdx.x * kListWords;
-  if (threadIdx.x < 2) sums[threadIdx.x] = 0;
+  if (threadIdx.x < 3) sums[threadIdx.x] = 0;
   __syncthreads();
   int earlier = 0, all = 0;
   for (int w = threadIdx.x; w < words; w += kThreads) {
@@ -352,15 +357,25 @@ __global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, 
   }
   __syncthreads();
   const int live = sums[1], n_free = a.p.pages - live;
+  int stay = 0;             // live pages in front of the live-th
+  if constexpr (kCompact) {
+    for (int w = threadIdx.x; w <= live >> 5 && w < words; w += kThreads) stay += __popc(a.bits[w] & (w < live >> 5 ? ~0u : (1u << (live & 31)) - 1u));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) stay += __shfl_xor_sync(0xffffffffu, stay, o);
+    if (lane == 0) atomicAdd(&sums[2], stay);
+    __syncthreads();
+    stay = sums[2];
+  }
   int base = sums[0];       // live pages before word w0; then before word w
   for (int w = w0; w < min(w0 + kListWords, words); ++w) {
     const unsigned word = a.bits[w];
     if (((w - w0) & (kThreads / 32 - 1)) == warp) {
       const int page = w * 32 + lane;
-      if (before && lane == 0) before[w] = base;
+      if (kCompact && lane == 0) a.before[w] = base;
       if (page < a.p.pages) {
-        const int rank = page - base - __popc(word & ((1u << lane) - 1u));    // free pages before this one
-        if (!((word >> lane) & 1u)) list[rank] = page;
+        const int rank = base + __popc(word & ((1u << lane) - 1u));      // live pages before this one
+        if (!((word >> lane) & 1u)) list[page - rank] = page;
+        else if (kCompact && page >= live) a.moves[rank - stay] = page;
         if (page >= n_free) list[page] = -1;
       }
     }
@@ -370,15 +385,15 @@ __global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, 
     range[0] = 0;
     range[1] = n_free;
     *a.shortfall = *a.dropped;
+    if (kCompact) *a.n_moves = live - stay;
   }
 }
 
 // Live pages at or behind the number of live pages go to the lowest free ones, in order: free pages are the only ones
 // written, live ones the only ones read, so that moves cannot meet.
-__global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a) {
-  const int n_free = a.new_free_range[1], live = a.p.pages - n_free;
+__global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a, int parts) {
+  const int n_free = a.new_free_range[1], live = a.p.pages - n_free, kept = live - *a.n_moves;      // kept: live pages that stay
   auto live_before = [&](int page) { return a.before[page >> 5] + __popc(a.bits[page >> 5] & ((1u << (page & 31)) - 1u)); };
-  const int kept = live < a.p.pages ? live_before(live) : live;       // live pages that stay
   auto moved_to = [&](int page) { return page < live ? page : a.holes[live_before(page) - kept]; };
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int pages = int((held_by(a, row) + a.p.page_size - 1) / a.p.page_size);
@@ -387,8 +402,9 @@ __global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a) 
       a.new_table[int64_t(row) * a.width + c] = page >= 0 && page < a.p.pages ? moved_to(page) : page;
     }
   }
-  for (int page = live + int(blockIdx.x); page < a.p.pages; page += gridDim.x)
-    if ((a.bits[page >> 5] >> (page & 31)) & 1u) copy_page(a.p, page, moved_to(page), a.p.page_size, 0, 1);
+  // a page in `parts` parts, all parts of all pages dealt to the CTAs in turn
+  const int n = *a.n_moves * parts;
+  for (int i = blockIdx.x; i < n; i += gridDim.x) copy_page(a.p, a.moves[i / parts], a.holes[i / parts], a.p.page_size, i % parts, parts);
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.p.pages; i += gridDim.x * kThreads)
     a.new_free_pages[i] = i < n_free ? live + i : -1;
 }
@@ -444,8 +460,16 @@ int move_args(const nb200_cache_params* p, const char* what, const Pages& pages,
   a->bits = reinterpret_cast<unsigned*>(ws + l->bits);
   a->before = ws + l->before;
   a->holes = ws + l->holes;
+  a->moves = ws + l->moves;
+  a->n_moves = ws + 1;
   if (cudaMemsetAsync(ws, 0, (l->bits + size_t(l->words)) * sizeof(int), st) != cudaSuccess) return check_launch("cache: clearing the workspace");
   return NB200_OK;
+}
+
+// parts that a page is copied in: 32 KB of keys and values, which eight words in flight per thread cover in one turn
+int page_parts(const Pages& p) {
+  const int64_t bytes = int64_t(p.heads) * p.page_size * p.words * 32;
+  return int(bytes <= 32768 ? 1 : bytes >= 16 * 32768 ? 16 : (bytes + 32767) / 32768);
 }
 
 unsigned list_grid(const Layout& l) { return l.words ? unsigned((l.words + kListWords - 1) / kListWords) : 1u; }
@@ -512,14 +536,11 @@ extern "C" NB200_API int nb200_cache_fork(const nb200_cache_params* p, void* cud
   if (int rc = move_args(p, "cache_fork", pages, &a, &l, st)) return rc;
   a.parents = p->parents; a.finished = p->finished; a.shortfall = p->shortfall;
   if (p->new_rows > 0) {
-    // a part of a page copy: 32 KB of keys and values, which eight words in flight per thread cover in one turn
-    const int64_t bytes = int64_t(pages.heads) * pages.page_size * pages.words * 32;
-    const unsigned parts = unsigned(bytes <= 32768 ? 1 : bytes >= 16 * 32768 ? 16 : (bytes + 32767) / 32768);
-    cache_fork_rows_kernel<<<dim3(unsigned(p->new_rows), parts), kThreads, size_t((p->rows + 31) / 32) * sizeof(unsigned), st>>>(a);
+    cache_fork_rows_kernel<<<dim3(unsigned(p->new_rows), unsigned(page_parts(pages))), kThreads, size_t((p->rows + 31) / 32) * sizeof(unsigned), st>>>(a);
     count_launch();
     if (int rc = check_launch("cache_fork_rows_kernel")) return rc;
   }
-  cache_list_kernel<<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.new_free_pages, a.new_free_range, nullptr);
+  cache_list_kernel<false><<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.new_free_pages, a.new_free_range);
   count_launch();
   return check_launch("cache_list_kernel");
 }
@@ -539,11 +560,12 @@ extern "C" NB200_API int nb200_cache_compact(const nb200_cache_params* p, void* 
     count_launch();
     if (int rc = check_launch("cache_mark_kernel")) return rc;
   }
-  cache_list_kernel<<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.holes, a.new_free_range, a.before);
+  cache_list_kernel<true><<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.holes, a.new_free_range);
   count_launch();
   if (int rc = check_launch("cache_list_kernel")) return rc;
-  const int most = pages.pages > p->rows ? pages.pages : p->rows;
-  cache_move_kernel<<<unsigned(most < 1 ? 1 : most < 148 * 8 ? most : 148 * 8), kThreads, 0, st>>>(a);
+  const int parts = page_parts(pages);
+  const int64_t most = int64_t(pages.pages) * parts > p->rows ? int64_t(pages.pages) * parts : p->rows;
+  cache_move_kernel<<<unsigned(most < 1 ? 1 : most < 148 * 8 ? most : 148 * 8), kThreads, 0, st>>>(a, parts);
   count_launch();
   return check_launch("cache_move_kernel");
 }
