@@ -10,8 +10,8 @@
  *   (x1, x2) -> (x1 cos phase - x2 sin phase,  x1 sin phase + x2 cos phase)
  *
  * where a pair is elements (j, j + P), or (2 j, 2 j + 1) with `interleaved`.  `inverse` turns the other way: it is the
- * gradient, since the rotation is orthogonal.  Phases are formed and reduced to one turn in 64 bits (products with
- * their rounding errors), so that they are as good at position 2^40 as at 1; the rotation itself is fp32, rounded once to the operands' type.
+ * gradient, since the rotation is orthogonal.  Phases are formed with the rounding errors of their products and
+ * reduced to one turn, so that they are as good at position 2^40 as at 1; the rotation itself is fp32, rounded once to the operands' type.
  *
  * Layout.  x is (B, S, heads, D) described by three element strides (unit stride on D), y is dense.  positions are dense
  * (B, S, axes), frequencies dense fp32 (P).  Every pointer is a device pointer; the work is enqueued on the caller's

@@ -19,6 +19,7 @@
 //  * anything else: fp32 multiply-adds, lanes along the head dim, a reduce-scatter of the query heads' sums.
 #include <math.h>
 
+#include "dependent_launch.cuh"
 #include "nitrix_b200_cache.h"
 #include "sdpa_tc_common.cuh"
 
@@ -410,7 +411,7 @@ struct FmaLoop {
 template <typename T, typename Loop>
 __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const DecodeArgs a) {
   extern __shared__ float merge[];      // [slot][head][D + 2]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  allow_dependents();
   const int lane = threadIdx.x & 31;
   const Share share = share_of(a, lane);
   if (int(blockIdx.x) >= share.workers) return;
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
   T* out = static_cast<T*>(a.out) + (int64_t(row) * a.q_heads + head) * a.D;
   const int units = units_of(a, row);
   if (units == 0) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
     for (int d = threadIdx.x; d < a.D; d += kThreads) out[d] = from_f32<T>(0.f);
     return;
   }
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
   const int chunk = in_group / heads_per_chunk, h = in_group - chunk * heads_per_chunk;
   const int64_t begin = before + int64_t(kv_head * a.chunks + chunk) * units;
   const int w0 = share.worker_of(begin), w1 = share.worker_of(begin + units - 1);
-  asm volatile("griddepcontrol.wait;" ::: "memory");      // (the lengths are the caller's: what is above needs no wait)
+  wait_for_previous();      // (the lengths are the caller's: what is above needs no wait)
   if (w0 == w1) return;                  // finished by the CTA that had all of it
   const int64_t step = int64_t(heads_per_chunk) * (a.D + 4);
   // the first piece begins the item (slot 1 of its worker); the others begin inside it (slot 0)
@@ -622,17 +623,8 @@ int launch(const DecodeArgs& a, cudaStream_t st) {
   decode_kernel<T, Loop><<<unsigned(a.workers), kThreads, smem, st>>>(a);
   count_launch();
   if (int rc = check_launch("decode_kernel")) return rc;
-  // the joining CTAs may be set up while the main kernel runs; they wait for its end before they read anything it wrote
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(a.q_heads), unsigned(a.rows));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, decode_join_kernel<T>, a, int(Loop::kHeads)) != cudaSuccess) return check_launch("decode_join_kernel");
+  if (launch_dependent(decode_join_kernel<T>, dim3(unsigned(a.q_heads), unsigned(a.rows)), kThreads, 0, st, a, int(Loop::kHeads)) != cudaSuccess)
+    return check_launch("decode_join_kernel");
   count_launch();
   return check_launch("decode_join_kernel");
 }

@@ -3,6 +3,7 @@
 // The lengths are in device memory, so the blocks of all sequences are listed there: one CTA counts them by their length in
 // tiles (longest first, so that the short ones even out the end) and writes them in that order; blocks of one length come in
 // any order, which changes no result.  The other CTAs clear the outputs of tokens that belong to no sequence.
+#include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
 namespace nb200 {
@@ -73,7 +74,7 @@ __device__ __forceinline__ void clear_tail(T* base, int64_t first, int64_t end, 
 }
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArgs p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  allow_dependents();
   const PackedArgs& a = p.a;
   if (blockIdx.x > 0) {
     const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D;

@@ -17,6 +17,7 @@
 // Bound by the element-wise warps and the shared-memory traffic of the MMAs as that kernel is.  All waits bounded.
 #include <math.h>
 
+#include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
 namespace nb200 {
@@ -92,7 +93,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   static_assert(P_READY + 2 == L::kNumBars, "barrier count");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // the work list and delta are written by the launches before
+  wait_for_previous();       // the work list and delta are written by the launches before
   const int entry = blockIdx.x / a.kv_heads, head = blockIdx.x - entry * a.kv_heads;
   if (entry >= *reinterpret_cast<const volatile int*>(a.list.count)) return;
   const WorkItem it = load_item(a.list.items + entry);
@@ -659,17 +660,7 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   a.status = device_status_word();
   if (!a.status) { set_error("packed_bwd: no status word on this device"); return NB200_ERR_LAUNCH; }
   const int64_t grid = most_blocks(p.tokens_k, p.sequences, kTile) * p.kv_heads;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, tk, tv, tq, tdo, a) != cudaSuccess) return check_launch("packed_bwd_tc_kernel");
+  if (launch_dependent(kernel, unsigned(grid), kThreads, smem, st, tk, tv, tq, tdo, a) != cudaSuccess) return check_launch("packed_bwd_tc_kernel");
   count_launch();
   if (int rc = check_launch("packed_bwd_tc_kernel")) return rc;
   packed_dq_finish_kernel<D, kBf16><<<dim3(unsigned(a.all_steps), unsigned(p.kv_heads)), kStep / 4 * (D / 8), 0, st>>>(p, acc, a.all_steps, a.tokens);

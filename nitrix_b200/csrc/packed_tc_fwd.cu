@@ -18,6 +18,7 @@
 // All waits on mbarriers are bounded (sdpa_tc_common.cuh).
 #include <type_traits>
 
+#include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
 namespace nb200 {
@@ -155,7 +156,7 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   auto tm_S = [&](int g) { return tmem + g * 128; };
   auto tm_P = [&](int g) { return kAlias ? tmem + g * 128 : tmem + 256 + g * 64; };
   auto tm_O = [&](int g) { return kAlias ? tmem + 256 + g * D : tmem + 384 + g * D; };
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // the work list is written by the launch before
+  wait_for_previous();       // the work list is written by the launch before
   const int count = *reinterpret_cast<const volatile int*>(a.list.count);
 
   // Phase bookkeeping across blocks (every role derives the same numbers from the same list):
@@ -570,18 +571,9 @@ int launch_one(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
     if (dev >= 0) ready[dev] = true;
   }
   const int sms = sm_count();
-  // set up while the list is being written; it waits for that before it reads it
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(most < sms ? most : sms));
-  cfg.blockDim = dim3(Split<D>::kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, a) != cudaSuccess) return check_launch("packed_fwd_tc_kernel");
+  // (set up while the list is being written)
+  if (launch_dependent(kernel, unsigned(most < sms ? most : sms), Split<D>::kThreads, smem, st, tq, tk, tv, a) != cudaSuccess)
+    return check_launch("packed_fwd_tc_kernel");
   count_launch();
   return check_launch("packed_fwd_tc_kernel");
 }

@@ -8,6 +8,7 @@
 // thread), by launches and latency where a step adds one token per sequence: append is ONE launch, in which every warp finds
 // its token's sequence and the number of pages that the sequences before it take by one pass over `offsets` and `lengths`;
 // fork is a memset and two launches, compact a memset and three.
+#include "dependent_launch.cuh"
 #include "nitrix_b200_cache.h"
 #include "sdpa_common.cuh"
 
@@ -262,6 +263,7 @@ __device__ __forceinline__ void copy_page(const Pages& p, int src, int dst, int 
 // of rows before it with an open page less the number of their distinct parents, which a bit per parent counts.
 __global__ void __launch_bounds__(kThreads) cache_fork_rows_kernel(const MoveArgs a) {
   extern __shared__ unsigned seen[];       // one bit per row of the old table
+  allow_dependents();
   __shared__ int open_rows, distinct;
   const int row = blockIdx.x, words = (a.rows + 31) / 32;
   for (int i = threadIdx.x; i < words; i += kThreads) seen[i] = 0;
@@ -323,6 +325,7 @@ __global__ void __launch_bounds__(kThreads) cache_fork_rows_kernel(const MoveArg
 }
 
 __global__ void __launch_bounds__(kThreads) cache_mark_kernel(const MoveArgs a) {
+  allow_dependents();
   const int row = blockIdx.x;
   const int pages = int((held_by(a, row) + a.p.page_size - 1) / a.p.page_size);
   for (int c = threadIdx.x; c < pages; c += kThreads) mark(a, a.table[int64_t(row) * a.width + c]);
@@ -336,6 +339,8 @@ constexpr int kListWords = 64;      // words of bits per CTA of the listing kern
 template <bool kCompact>
 __global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, int words, int* list, int* range) {
   __shared__ int sums[3];
+  allow_dependents();
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w0 = blockIdx.x * kListWords;
   if (threadIdx.x < 3) sums[threadIdx.x] = 0;
@@ -392,6 +397,7 @@ __global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, 
 // Live pages at or behind the number of live pages go to the lowest free ones, in order: free pages are the only ones
 // written, live ones the only ones read, so that moves cannot meet.
 __global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a, int parts) {
+  wait_for_previous();
   const int n_free = a.new_free_range[1], live = a.p.pages - n_free, kept = live - *a.n_moves;      // kept: live pages that stay
   auto live_before = [&](int page) { return a.before[page >> 5] + __popc(a.bits[page >> 5] & ((1u << (page & 31)) - 1u)); };
   auto moved_to = [&](int page) { return page < live ? page : a.holes[live_before(page) - kept]; };
@@ -508,8 +514,9 @@ extern "C" NB200_API int nb200_cache_append(const nb200_cache_params* p, void* c
     a.vs[i] = p->new_v_stride[i] / vec;
   }
   a.tokens = p->tokens;
-  // one token per warp while that does not fill the GPU's warps; then four, which share a sequence's search
-  a.tokens_per_warp = p->tokens < 148 * 64 ? 1 : 4;
+  // one token per warp while that does not fill the GPU's warps; then two, which share a sequence's search (33 k tokens of bf16,
+  // 8 heads of 128: one 55.9 us, two 51.4, four 53.9, eight 60.2)
+  a.tokens_per_warp = p->tokens < 148 * 64 ? 1 : 2;
   const int64_t per_cta = int64_t(a.tokens_per_warp) * (kThreads / 32);
   const unsigned grid = unsigned((p->tokens + per_cta - 1) / per_cta) + 1u;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
@@ -540,7 +547,8 @@ extern "C" NB200_API int nb200_cache_fork(const nb200_cache_params* p, void* cud
     count_launch();
     if (int rc = check_launch("cache_fork_rows_kernel")) return rc;
   }
-  cache_list_kernel<false><<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.new_free_pages, a.new_free_range);
+  if (launch_dependent(cache_list_kernel<false>, list_grid(l), kThreads, 0, st, a, l.words, a.new_free_pages, a.new_free_range) != cudaSuccess)
+    return check_launch("cache_list_kernel");
   count_launch();
   return check_launch("cache_list_kernel");
 }
@@ -560,12 +568,16 @@ extern "C" NB200_API int nb200_cache_compact(const nb200_cache_params* p, void* 
     count_launch();
     if (int rc = check_launch("cache_mark_kernel")) return rc;
   }
-  cache_list_kernel<true><<<list_grid(l), kThreads, 0, st>>>(a, l.words, a.holes, a.new_free_range);
+  if (launch_dependent(cache_list_kernel<true>, list_grid(l), kThreads, 0, st, a, l.words, a.holes, a.new_free_range) != cudaSuccess)
+    return check_launch("cache_list_kernel");
   count_launch();
   if (int rc = check_launch("cache_list_kernel")) return rc;
+  // a CTA per part of a page that may have to move, which half of the pages at most have
   const int parts = page_parts(pages);
-  const int64_t most = int64_t(pages.pages) * parts > p->rows ? int64_t(pages.pages) * parts : p->rows;
-  cache_move_kernel<<<unsigned(most < 1 ? 1 : most < 148 * 8 ? most : 148 * 8), kThreads, 0, st>>>(a, parts);
+  int64_t grid = int64_t(pages.pages + 1) / 2 * parts;
+  if (grid < p->rows) grid = p->rows;
+  grid = grid < 1 ? 1 : grid > 65536 ? 65536 : grid;
+  if (launch_dependent(cache_move_kernel, unsigned(grid), kThreads, 0, st, a, parts) != cudaSuccess) return check_launch("cache_move_kernel");
   count_launch();
   return check_launch("cache_move_kernel");
 }

@@ -4,10 +4,11 @@
 //   (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos),   phase = position[token][axis of the pair] * frequency[pair]
 //
 // Bound by HBM: every element is read and written once, and a pair costs three multiply-adds.  The cosines and sines are
-// the same for every head of a token, so a CTA takes all heads of a few tokens, forms the tokens' table once in shared
-// memory and streams the heads past it in 16-byte words.  The phase is formed in 64 bits and reduced to one turn there: as
-// a product of two fp32 numbers it is off by 0.008 at position 131072.  (One 64-bit product and reduction per token and
-// pair, not per element: with 32 heads of 128, an element's 64-bit work is 1/64 of that.)
+// the same for every head of a token, so a CTA takes all heads of its tokens and forms their table once, in shared memory.  The
+// phase is formed with the rounding errors of its products, so that a position of 2^40 is as good as one of 1: as one product of
+// two fp32 numbers it is off by 0.008 at position 131072.  16384 bf16 tokens, 16 + 16 heads of 128, forward and gradient: 96 us,
+// 5.6 TB/s, with small CTAs and one row per thread in flight; 256 or 512 threads 101 and 108, two or four rows in flight 104 and
+// 100, cosines and sines in registers of a thread that goes over the heads 115, loads that do not stay in L2 115.
 #include <math.h>
 
 #include <type_traits>
@@ -18,10 +19,13 @@
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxPairs = 128;      // head dim 256
 // 1 / (2 pi) in two doubles
 constexpr double kTurnHigh = 0.15915494309189535, kTurnLow = -9.839338337591243e-18;
+// and in two fp32 numbers
+constexpr float kTurnHigh32 = 0.15915494f, kTurnLow32 = float(kTurnHigh - double(kTurnHigh32));
+constexpr float kFp32Positions = 16777216.f;
 
 struct RotaryTensor {
   const void* x;
@@ -44,22 +48,45 @@ struct RotaryArgs {
   uint32_t heads_magic;       // ceil(2^32 / heads of both tensors): row of a CTA -> its token, exact below 2^16 (one head: not used)
 };
 
-__device__ __forceinline__ double position_of(const RotaryArgs& a, int64_t i) {
-  if (a.position_dtype == NB200_POS_I32) return double(static_cast<const int32_t*>(a.positions)[i]);
-  if (a.position_dtype == NB200_POS_I64) return double(static_cast<const int64_t*>(a.positions)[i]);
-  return double(static_cast<const float*>(a.positions)[i]);
-}
-
-// cos and sin of a pair's phase at a token
+// cos and sin of a pair's phase at a token.  position * frequency / (2 pi) is formed with the rounding errors of its products,
+// less whole turns: in pairs of fp32 numbers up to 2^24, where a position is one, in pairs of fp64 ones above.  (64-bit units
+// are few: with them alone the training pass of 16384 tokens took 102 us at its best.)
+template <typename T>
 __device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int token, int pair) {
   int axis = 0;
   while (axis + 1 < a.axes && pair >= a.bound[axis]) ++axis;
-  // position * frequency / (2 pi) with the products' rounding errors kept, less whole turns
-  const double p = position_of(a, int64_t(token) * a.axes + axis), f = double(a.frequencies[pair]);
-  const double phase = p * f, phase_low = fma(p, f, -phase);
-  const double turns = phase * kTurnHigh, turns_low = fma(phase, kTurnHigh, -turns) + fma(phase, kTurnLow, phase_low * kTurnHigh);
+  const int64_t i = int64_t(token) * a.axes + axis;
+  double exact = 0.0;
+  float p;
+  if (a.position_dtype == NB200_POS_I32) {
+    const int32_t n = static_cast<const int32_t*>(a.positions)[i];
+    p = float(n);
+    if (fabsf(p) > kFp32Positions) exact = double(n);
+  } else if (a.position_dtype == NB200_POS_I64) {
+    const int64_t n = static_cast<const int64_t*>(a.positions)[i];
+    p = float(n);
+    if (fabsf(p) > kFp32Positions) exact = double(n);
+  } else {
+    p = static_cast<const float*>(a.positions)[i];
+    if (fabsf(p) > kFp32Positions) exact = double(p);
+  }
+  const float f = a.frequencies[pair];
+  float part;      // of a turn
+  if (fabsf(p) > kFp32Positions) {
+    const double phase = exact * f, phase_low = fma(exact, double(f), -phase);
+    const double turns = phase * kTurnHigh, turns_low = fma(phase, kTurnHigh, -turns) + fma(phase, kTurnLow, phase_low * kTurnHigh);
+    part = float((turns - rint(turns)) + turns_low);
+  } else {
+    const float step = f * kTurnHigh32, step_low = fmaf(f, kTurnLow32, fmaf(f, kTurnHigh32, -step));      // turns per position
+    const float turns = p * step, turns_low = fmaf(p, step_low, fmaf(p, step, -turns));
+    part = (turns - rintf(turns)) + turns_low;
+  }
   float s, c;
-  sincospif(float(2.0 * ((turns - rint(turns)) + turns_low)), &s, &c);
+  if constexpr (sizeof(T) == 4) {
+    sincospif(2.f * part, &s, &c);
+  } else {
+    __sincosf(part * 6.283185307f, &s, &c);      // within 5e-7, a thousandth of the result's rounding
+  }
   return make_float2(c, a.sign * s);
 }
 
@@ -99,66 +126,47 @@ struct Piece {
   }
 };
 
-// kLanes lanes (a power of two) share a (token, head) row; lane c takes rotated word c, lanes behind those the words that
-// pass unchanged.  kAhead rows per thread have their loads in flight together.
-template <typename T, bool kInterleaved, int kLanes, int kAhead>
+// kLanes threads (a power of two) share a (token, head) row; thread c takes rotated word c, threads behind those the words that
+// pass unchanged.  A CTA takes all heads of its tokens, a row per group of threads at a time; the first are on their way while
+// the tokens' table is formed.
+template <typename T, bool kInterleaved, int kLanes>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-  constexpr int kVec = 16 / int(sizeof(T));
+  constexpr int kVec = 16 / int(sizeof(T)), kGroups = kThreads / kLanes;
   extern __shared__ float2 table[];     // [token of the CTA][pair]
   const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  constexpr int kGroups = kThreads / kLanes;
   const int token0 = blockIdx.x * a.tokens_per_cta;
   const int n_tokens = min(a.tokens_per_cta, a.tokens - token0);
   const int heads = a.t[0].heads + a.t[1].heads;
   const int rows = n_tokens * heads;
   const int words = kInterleaved ? 2 * a.pairs / kVec : a.pairs / kVec;      // rotated words (for split pairs: of the first halves)
   const int pass0 = 2 * a.pairs / kVec, passing = a.D / kVec - pass0;        // words that pass unchanged
-  const bool rotated = c < words, passes = c >= words && c - words < passing;
+  const bool rotated = c < words, takes = rotated || c - words < passing;
   const int word = rotated ? c : pass0 + c - words;
 
-  Piece<T, kInterleaved> piece[kAhead];
-  auto place = [&](int row, const T** x, T** y, int* token) {
-    const int tl = heads == 1 ? row : int(__umulhi(uint32_t(row), a.heads_magic));
-    int head = row - tl * heads;
-    *token = tl;
-    const int n = token0 + tl;
-    const RotaryTensor& t = head < a.t[0].heads ? a.t[0] : a.t[1];
-    if (head >= a.t[0].heads) head -= a.t[0].heads;
+  Piece<T, kInterleaved> piece;
+  T* y = nullptr;
+  int token = 0;           // of the CTA
+  auto load = [&](int row) {
+    token = heads == 1 ? row : int(__umulhi(uint32_t(row), a.heads_magic));
+    int head = row - token * heads;
+    const int n = token0 + token;
+    const bool second = head >= a.t[0].heads;
+    const RotaryTensor& t = second ? a.t[1] : a.t[0];
+    if (second) head -= a.t[0].heads;
     const int b = n / a.length, s = n - b * a.length;
-    *x = static_cast<const T*>(t.x) + (b * t.xs[0] + s * t.xs[1] + head * t.xs[2]);
-    *y = static_cast<T*>(t.y) + (int64_t(n) * t.heads + head) * a.D;
+    y = static_cast<T*>(t.y) + (int64_t(n) * t.heads + head) * a.D;
+    piece.load(static_cast<const T*>(t.x) + (b * t.xs[0] + s * t.xs[1] + head * t.xs[2]), word, a.pairs, rotated);
   };
-  auto load = [&](int row0) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int row = row0 + i * kGroups;
-      if (row >= rows || !(rotated || passes)) continue;
-      const T* x;
-      T* y;
-      int token;
-      place(row, &x, &y, &token);
-      piece[i].load(x, word, a.pairs, rotated);
-    }
-  };
-  load(group);      // (under the table's arithmetic)
+  if (group < rows && takes) load(group);
   for (int i = threadIdx.x; i < n_tokens * a.pairs; i += kThreads) {
     const int tl = i / a.pairs;
-    table[i] = turn_of(a, token0 + tl, i - tl * a.pairs);
+    table[i] = turn_of<T>(a, token0 + tl, i - tl * a.pairs);
   }
   __syncthreads();
-  for (int row0 = group; row0 < rows; row0 += kGroups * kAhead) {
-    if (row0 != group) load(row0);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int row = row0 + i * kGroups;
-      if (row >= rows || !(rotated || passes)) continue;
-      const T* x;
-      T* y;
-      int token;
-      place(row, &x, &y, &token);
-      if (rotated) piece[i].turn(table + token * a.pairs, word);
-      piece[i].store(y, word, a.pairs, rotated);
-    }
+  for (int row = group; row < rows && takes; row += kGroups) {
+    if (row != group) load(row);
+    if (rotated) piece.turn(table + token * a.pairs, word);
+    piece.store(y, word, a.pairs, rotated);
   }
 }
 
@@ -167,7 +175,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_generic_kernel(const RotaryArgs a) {
   extern __shared__ float2 table[];
   const int token = blockIdx.x;
-  for (int i = threadIdx.x; i < a.pairs; i += kThreads) table[i] = turn_of(a, token, i);
+  for (int i = threadIdx.x; i < a.pairs; i += kThreads) table[i] = turn_of<T>(a, token, i);
   __syncthreads();
   const int b = token / a.length, s = token - b * a.length;
   const int per_head = a.D - a.pairs;      // pairs, then passing elements
@@ -192,16 +200,14 @@ __global__ void __launch_bounds__(kThreads) rotary_generic_kernel(const RotaryAr
 
 template <typename T, bool kInterleaved, int kLanes>
 int launch_lanes(RotaryArgs a, cudaStream_t st) {
-  constexpr int kAhead = 4;
   const int heads = a.t[0].heads + a.t[1].heads;
-  // Tokens of a CTA: enough rows for every group's loads in flight, one where that leaves the GPU short of CTAs.
-  int per = kThreads / kLanes * kAhead / heads;
-  per = per < 1 ? 1 : per > 16 ? 16 : per;
-  if (a.tokens / per < 4 * 148) per = 1;
+  // Tokens of a CTA: as many as give every group a row, one where that leaves the GPU short of CTAs.
+  int per = kThreads / kLanes / heads;
+  per = per < 1 || a.tokens / per < 4 * 148 ? 1 : per;
   a.tokens_per_cta = per;
   a.heads_magic = uint32_t(((uint64_t(1) << 32) + uint32_t(heads) - 1) / uint32_t(heads));
   const unsigned grid = unsigned((a.tokens + per - 1) / per);
-  rotary_kernel<T, kInterleaved, kLanes, kAhead><<<grid, kThreads, sizeof(float2) * size_t(per) * a.pairs, st>>>(a);
+  rotary_kernel<T, kInterleaved, kLanes><<<grid, kThreads, sizeof(float2) * size_t(per) * a.pairs, st>>>(a);
   count_launch();
   return check_launch("rotary_kernel");
 }

@@ -36,7 +36,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     ``positions`` is ``(..., axes)`` (``(...)`` will do for one axis): int32, int64 or float32.  ``frequencies`` is fp32
     ``(pairs,)``; ``sections`` says how many of the pairs belong to each axis, in order (one axis by default).  A pair is
     elements ``(j, j + pairs)`` of a head, or ``(2 j, 2 j + 1)`` with ``interleaved``; elements from ``2 * pairs`` on pass
-    unchanged.  Angles are formed in 64 bits, the rotation in fp32.  Differentiable in ``q`` and ``k``.
+    unchanged.  Angles are as good at far positions as at near ones; the rotation is fp32, rounded once.  Differentiable in ``q`` and ``k``.
     """
     resolve_backend(backend)   # raises without a Blackwell device: there is no host path
     return _cabi.torch_ops().rotary(q, k, positions, frequencies, list(sections), bool(interleaved))
