@@ -1,8 +1,12 @@
 // Work lists of the tensor-core kernels of attention over packed sequences.
 //
-// The lengths are in device memory, so the blocks of all sequences are listed there: one CTA counts them by their length in
-// tiles (longest first, so that the short ones even out the end) and writes them in that order; blocks of one length come in
-// any order, which changes no result.  The other CTAs clear the outputs of tokens that belong to no sequence.
+// The lengths are in device memory, so the blocks of all sequences are listed there, by one CTA.  Two things decide their
+// order.  CTAs that work on one sequence side by side share its keys in L2 (forward), or its queries and the sums of dq, which
+// every key block adds to (backward: with all sequences' blocks sorted by length alone, 16 documents of up to 4096 tokens, the
+// sums alone are 284 MB and the kernel takes 1252 us for 1120).  And the longest blocks of what is left should come first, so that
+// short ones even out the end.  So the sequences, longest first, are cut into groups of at least two blocks per SM, and within a
+// group the blocks are sorted by their length in tiles; blocks of one length come in any order, which changes no result.
+// The other CTAs clear the outputs of tokens that belong to no sequence.
 #include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
@@ -12,13 +16,18 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kClearCtas = 31;
-constexpr int kBuckets = 1024;
+constexpr int kBuckets = 1024;         // group, then length
+constexpr int kLengths = 64;           // of them per group, longest first
+constexpr int kGroups = kBuckets / kLengths;
+constexpr int kGroupItems = 2 * 148;   // (block, key head) pairs that a group has at least
 
 struct PlanArgs {
   PackedArgs a;
   int backward;
   int block, step_tokens;
   int shift;             // lengths in tiles are counted in units of 2^shift
+  int kv_heads;
+  int grouped;           // more than one group is possible
   // Entries and (backward) steps that there is room for: as many as sequences that follow one another have.  Offsets that run
   // backwards describe sequences that overlap, of which those that do not fit are left out.
   int most;
@@ -27,8 +36,48 @@ struct PlanArgs {
   WorkItem* items;
 };
 
+// Blocks of a sequence.
+__device__ __forceinline__ int blocks_of(const PlanArgs& p, int s) {
+  const int n = p.backward ? sequence_span(p.a.offsets_k, s, p.a.tokens_k).y : sequence_span(p.a.offsets_q, s, p.a.tokens_q).y;
+  return (n + p.block - 1) / p.block;
+}
+
+// Group of every sequence into `group`; up to kPlanThreads sequences (more of them are one group).
+__device__ __forceinline__ void form_groups(const PlanArgs& p, uint8_t* group, int* blocks, int* sorted) {
+  const int n = p.a.sequences, i = threadIdx.x, lane = i & 31, warp = i >> 5;
+  __shared__ int sums[kPlanThreads / 32];
+  if (i < n) blocks[i] = blocks_of(p, i);
+  sorted[i] = 0;
+  __syncthreads();
+  int rank = 0;
+  if (i < n) {
+    const int mine = blocks[i];
+    for (int j = 0; j < n; ++j) rank += blocks[j] > mine || (blocks[j] == mine && j < i) ? 1 : 0;
+    sorted[rank] = mine;
+  }
+  __syncthreads();
+  const int own = sorted[i];
+  int64_t upto = own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 31) sums[warp] = int(upto);
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
+  const int64_t items = max(int64_t(kGroupItems), (total * p.kv_heads + kGroups - 1) / kGroups);
+  sorted[i] = int(min((upto - own) * p.kv_heads / items, int64_t(kGroups - 1)));      // the group of rank i
+  __syncthreads();
+  if (i < n) group[i] = uint8_t(sorted[rank]);
+  __syncthreads();
+}
+
 template <typename Visit>
-__device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
+__device__ __forceinline__ void for_each_block(const PlanArgs& p, const uint8_t* group, Visit visit) {
   const PackedArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t steps_before = 0;  // backward: 64-row steps of the sequences before, every warp for itself
@@ -54,7 +103,7 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
       w.other = other.x;
       w.other_n = other.y;
       w.steps = int(steps_before);
-      w.pad[0] = w.pad[1] = 0;
+      w.index = b;
       int length;        // tokens of the other side
       if (p.backward) {
         w.seen = first - shift;
@@ -63,7 +112,7 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, Visit visit) {
         w.seen = first + 1 + shift;
         length = a.causal ? min(max(w.seen + w.n - 1, 0), other.y) : other.y;
       }
-      visit(w, min((length / 128) >> p.shift, kBuckets - 1));
+      visit(w, (group ? group[s] : 0) * kLengths + kLengths - 1 - min((length / 128) >> p.shift, kLengths - 1));
     }
   }
 }
@@ -89,16 +138,20 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
     }
     return;
   }
-  __shared__ int buckets[kBuckets];      // blocks of each length, then the place of the next one
+  __shared__ int buckets[kBuckets];      // blocks of each group and length, then the place of the next one
   __shared__ int sums[32];
+  __shared__ uint8_t groups[kPlanThreads];
+  __shared__ int scratch[kPlanThreads];
+  if (p.grouped) form_groups(p, groups, buckets, scratch);
+  const uint8_t* group = p.grouped ? groups : nullptr;
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) buckets[i] = 0;
   __syncthreads();
-  for_each_block(p, [&](const WorkItem&, int bucket) { atomicAdd(&buckets[bucket], 1); });
+  for_each_block(p, group, [&](const WorkItem&, int bucket) { atomicAdd(&buckets[bucket], 1); });
   __syncthreads();
-  // places, longest first: thread t holds bucket kBuckets - 1 - t
+  // places
   static_assert(kBuckets == kPlanThreads, "a bucket per thread");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int own = buckets[kBuckets - 1 - threadIdx.x];
+  const int own = buckets[threadIdx.x];
   int upto = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -108,15 +161,18 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
   if (lane == 31) sums[warp] = upto;
   __syncthreads();
   for (int w = 0; w < warp; ++w) upto += sums[w];
-  buckets[kBuckets - 1 - threadIdx.x] = upto - own;
-  if (threadIdx.x == kPlanThreads - 1) *p.count = min(upto, p.most);
+  buckets[threadIdx.x] = upto - own;
+  if (threadIdx.x == kPlanThreads - 1) {
+    p.count[0] = min(upto, p.most);
+    p.count[1] = 0;
+  }
   __syncthreads();
-  for_each_block(p, [&](const WorkItem& w, int bucket) {
+  for_each_block(p, group, [&](const WorkItem& w, int bucket) {
     const int place = atomicAdd(&buckets[bucket], 1);
     if (place >= p.most) return;
     int4* dst = reinterpret_cast<int4*>(p.items + place);
     dst[0] = make_int4(w.begin, w.n, w.other, w.other_n);
-    dst[1] = make_int4(w.seen, w.steps, 0, 0);
+    dst[1] = make_int4(w.seen, w.steps, w.index, 0);
   });
 }
 
@@ -127,9 +183,11 @@ int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, 
   p.a = a;
   p.backward = backward;
   p.block = block;
+  p.kv_heads = a.kv_heads;
+  p.grouped = a.sequences > 1 && a.sequences <= kPlanThreads && most_blocks(backward ? a.tokens_k : a.tokens_q, a.sequences, block) * a.kv_heads > kGroupItems;
   p.step_tokens = step_tokens;
   const int64_t tiles = (backward ? a.tokens_q : a.tokens_k) / 128;
-  while ((tiles >> p.shift) >= kBuckets) ++p.shift;
+  while ((tiles >> p.shift) >= kLengths) ++p.shift;
   p.most = int(most_blocks(backward ? a.tokens_k : a.tokens_q, a.sequences, block));
   p.most_steps = most_blocks(a.tokens_q, a.sequences, step_tokens);
   p.count = static_cast<int*>(list);

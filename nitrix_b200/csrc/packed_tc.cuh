@@ -18,13 +18,16 @@ struct __align__(16) WorkItem {
   int other_n;      // tokens there
   int seen;         // see above
   int steps;        // backward: first 64-row step of the sequence's rows in the gradient sums of dq
-  int pad[2];
+  int index;        // number of the block in its sequence
+  int pad;
 };
 static_assert(sizeof(WorkItem) == 32, "two 16-byte loads");
 
-// List in device memory: 16 bytes of header (the number of entries), then the entries, longest first.
+// List in device memory: 16 bytes of header (the number of entries; the pieces of work taken so far, zero to begin with), then
+// the entries (packed_plan.cu: their order).
 struct WorkList {
   const int* count;
+  int* taken;
   const WorkItem* items;
 };
 inline size_t work_list_bytes(int64_t most) { return (16 + size_t(most) * sizeof(WorkItem) + 255) / 256 * 256; }
@@ -49,16 +52,8 @@ int tc_packed_bwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
 __device__ __forceinline__ WorkItem load_item(const WorkItem* p) {
   const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
   WorkItem w;
-  w.begin = a.x; w.n = a.y; w.other = a.z; w.other_n = a.w; w.seen = b.x; w.steps = b.y;
+  w.begin = a.x; w.n = a.y; w.other = a.z; w.other_n = a.w; w.seen = b.x; w.steps = b.y; w.index = b.z;
   return w;
-}
-// Position of a CTA's `round`-th piece of work among `total` that are sorted by length and dealt in rows of gridDim.x that
-// alternate direction, so that nobody gets the longest of every row.  -1: none.
-__device__ __forceinline__ int dealt_position(int round, int total) {
-  const int G = int(gridDim.x), first = round * G;
-  if (first + int(blockIdx.x) >= total) return -1;
-  const bool full = first + G <= total;
-  return first + ((round & 1) && full ? G - 1 - int(blockIdx.x) : int(blockIdx.x));
 }
 #endif
 

@@ -7,7 +7,8 @@
 // stay unused where G is no divisor), one TMA box brings them in that order, and a short sequence fills a tile G times as far
 // as it would head by head; the keys are read once for the group.
 //
-// PERSISTENT: one CTA per SM walks a list of blocks (packed_plan.cu), longest first, dealt in rows of alternating direction;
+// PERSISTENT: one CTA per SM takes blocks from a list (packed_plan.cu), the next one whenever it has loaded all of the last (the
+// warp that loads takes it and hands its number on through a ring in shared memory);
 // a block is two query tiles of one key head, for which the key tiles are streamed once.  Warps: 0 loads Q, K and V; 1 clears
 // the rows of a sequence's last V tile that belong to its neighbour (their probabilities are zeros, but 0 * NaN is NaN; keys
 // behind the end are masked by selection, and rows of Q behind the end stay in rows that nobody stores); 2 and 3 issue the
@@ -65,11 +66,13 @@ struct FwdSmem {
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kBars = kV + kStages * kTileBytes;
+  static constexpr int kItems = 4;                        // numbers of blocks on their way to the other warps
   // q_full[2] q_empty[2] k_full[S] k_empty[S] v_full[S] v_empty[S] v_clear[S] s_full[4] p_ready[4] o_done[2] o_free[2] s_free[2]
-  // pv_done[2]
-  static constexpr int kNumBars = 4 + 5 * kStages + 16;
+  // pv_done[2] i_full[I] i_empty[I]
+  static constexpr int kNumBars = 4 + 5 * kStages + 16 + 2 * kItems;
   static constexpr int kMisc = kBars + 8 * kNumBars;
-  static constexpr int kExchange = kMisc + 16;            // one fp32 per query row of both tiles
+  static constexpr int kItemRing = kMisc + 16;
+  static constexpr int kExchange = kItemRing + 4 * kItems;   // one fp32 per query row of both tiles
   static constexpr int kTotal = kExchange + 2 * kTile * 4;
 };
 
@@ -86,10 +89,8 @@ struct Item {
   __device__ __forceinline__ int tokens(int g) const { return g ? n1 : n0; }
 };
 
-// A CTA's `round`-th block; false: there is none.
-__device__ __forceinline__ bool decode_item(const FwdArgs& a, int round, int count, Item* it) {
-  const int pos = dealt_position(round, count * a.kv_heads);
-  if (pos < 0) return false;
+// Piece of work `pos`: a block for one key head.
+__device__ __forceinline__ void decode_item(const FwdArgs& a, int pos, Item* it) {
   const int entry = pos / a.kv_heads;
   const WorkItem w = load_item(a.list.items + entry);
   it->head = pos - entry * a.kv_heads;
@@ -104,7 +105,6 @@ __device__ __forceinline__ bool decode_item(const FwdArgs& a, int round, int cou
   it->nt1 = it->n1 > 0 ? tiles(w.n) : 0;
   it->nt_max = max(it->nt0, it->nt1);
   it->tail = it->nt_max * kTile > w.other_n;
-  return true;
 }
 
 template <int D, bool kBf16>
@@ -126,8 +126,9 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   auto bar = [&](int i) { return smem_u32(bars + i); };
   constexpr int Q_FULL = 0, Q_EMPTY = 2, K_FULL = 4, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages,
                 V_EMPTY = V_FULL + kStages, V_CLEAR = V_EMPTY + kStages, S_FULL = V_CLEAR + kStages, P_READY = S_FULL + 4,
-                O_DONE = P_READY + 4, O_FREE = O_DONE + 2, S_FREE = O_FREE + 2, PV_DONE = S_FREE + 2;
-  static_assert(PV_DONE + 2 == L::kNumBars, "barrier count");
+                O_DONE = P_READY + 4, O_FREE = O_DONE + 2, S_FREE = O_FREE + 2, PV_DONE = S_FREE + 2, I_FULL = PV_DONE + 2,
+                I_EMPTY = I_FULL + L::kItems;
+  static_assert(I_EMPTY + L::kItems == L::kNumBars, "barrier count");
   constexpr bool kAlias = D == 128;      // P over S, key tiles in halves
   constexpr int kPoly = kAlias ? kPolyPeriod : 0;
 
@@ -140,6 +141,7 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if (i >= V_EMPTY && i < V_EMPTY + kStages) count = 3;                     // and one of the warp that clears tails
       if (i >= O_FREE && i < O_FREE + 2) count = 4 * kHalves;
       if (i >= S_FREE && i < S_FREE + 2) count = 4 * kHalves;
+      if (i >= I_EMPTY && i < I_EMPTY + L::kItems) count = 3 + 8 * kHalves;      // warp 1, two issuers, the softmax warps
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -157,9 +159,17 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   auto tm_P = [&](int g) { return kAlias ? tmem + g * 128 : tmem + 256 + g * 64; };
   auto tm_O = [&](int g) { return kAlias ? tmem + 256 + g * D : tmem + 384 + g * D; };
   wait_for_previous();       // the work list is written by the launch before
-  const int count = *reinterpret_cast<const volatile int*>(a.list.count);
+  volatile int* const items = reinterpret_cast<volatile int*>(smem + L::kItemRing);
+  // The `n`-th piece of work of this CTA, for every warp but the one that takes them: waits for its number (-1: no more, -2: the
+  // wait was given up); give_back() once it has been read.
+  auto next_item = [&](int n) {
+    if (!wait_or_abort(bar(I_FULL + n % L::kItems), (n / L::kItems) & 1, abort_flag, a.status, 416)) return -2;
+    return items[n % L::kItems];
+  };
+  auto give_back = [&](int n) { mbar_arrive(bar(I_EMPTY + n % L::kItems)); };
 
   // Phase bookkeeping across blocks (every role derives the same numbers from the same list):
+  //   n    blocks that this CTA has taken so far
   //   kv   key tiles streamed so far            -> ring stage kv % kStages, phase (kv / kStages) & 1
   //   tc_g tiles query tile g has processed     -> phase of s_full / p_ready / s_free / pv_done
   //   oc_g blocks in which query tile g had any -> phase of q_full / q_empty / o_done / o_free
@@ -175,7 +185,16 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tma_prefetch_desc(&tm_v);
       int kv = 0, oc[2] = {0, 0};
       bool ok = true;
-      for (int round = 0; ok && decode_item(a, round, count, &it); ++round) {
+      const int total = *reinterpret_cast<const volatile int*>(a.list.count) * a.kv_heads;
+      int pos = int(blockIdx.x) < total ? int(blockIdx.x) : -1;
+      for (int n = 0;; ++n) {
+        if (n >= L::kItems) ok = ok && wait_or_abort(bar(I_EMPTY + n % L::kItems), (n / L::kItems - 1) & 1, abort_flag, a.status, 417);
+        if (!ok) break;
+        items[n % L::kItems] = pos;
+        mbar_arrive(bar(I_FULL + n % L::kItems));
+        if (pos < 0) break;
+        const int next = int(gridDim.x) + atomicAdd(a.list.taken, 1);      // (its latency runs under this block's loads)
+        decode_item(a, pos, &it);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if (it.nt(g) == 0) continue;
@@ -202,6 +221,7 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           for (int x = 0; x < D / 64; ++x)
             tma_load_4d(sbase + L::kV + st * L::kTileBytes + x * kBoxBytes, &tm_v, bar(V_FULL + st), x * 64, it.head, it.k0 + j * kTile, 0);
         }
+        pos = next < total ? next : -1;
       }
     }
   } else if (warp == 1) {
@@ -210,7 +230,11 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     // of the same parity for its own, and one that holds nothing back could fall behind by two.)
     int kv = 0;
     bool ok = true;
-    for (int round = 0; ok && decode_item(a, round, count, &it); ++round) {
+    for (int n = 0; ok; ++n) {
+      const int pos = next_item(n);
+      if (!__all_sync(0xffffffffu, pos >= 0)) break;
+      if (lane == 0) give_back(n);
+      decode_item(a, pos, &it);
       for (int j = 0; j < it.nt_max; ++j, ++kv) {
         const int st = kv % kStages;
         ok = __all_sync(0xffffffffu, wait_or_abort(bar(V_FULL + st), (kv / kStages) & 1, abort_flag, a.status, 403));
@@ -242,7 +266,11 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       bool ok = true;
       int kv = 0, tc = 0, oc = 0;
       uint32_t clear = 0;
-      for (int round = 0; ok && decode_item(a, round, count, &it); ++round) {
+      for (int n = 0; ok; ++n) {
+        const int pos = next_item(n);
+        if (pos < 0) break;
+        give_back(n);
+        decode_item(a, pos, &it);
         const int nt = it.nt(g);
         // V of tile j is in shared memory, its tail cleared; of a tail that this query tile skips only the phase is noted
         auto wait_v = [&](int j) {
@@ -377,12 +405,17 @@ packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 
     // A warp that gives up (`ok` false) waits no more and stores nothing, but walks on through its passes: its partner waits
     // for it at the pair's barrier, which has no time limit of its own.
-    for (int round = 0;; ++round) {
+    for (int n = 0;; ++n) {
+      const int pos = ok ? next_item(n) : -2;
+      // (two warps that share rows end together: one that has given up takes its partner along)
+      const bool last = kHalves == 1 ? !__all_sync(0xffffffffu, pos >= 0) : named_barrier_or(pair_bar, 64, pos < 0);
+      if (last) break;
+      if (lane == 0) give_back(n);
       // of the block only what the passes and the epilogue need: a spilled register costs more than anything here (head dim 64)
       int my_nt, seen, row;
       {
         Item it;
-        if (!decode_item(a, round, count, &it)) break;
+        decode_item(a, pos, &it);
         const int local = g * a.tokens + token;            // query of the block
         my_nt = it.nt(g);
         seen = a.causal ? min(it.seen + local, it.lk) : it.lk;
@@ -611,6 +644,7 @@ int tc_packed_fwd(const PackedArgs& p, int dtype, void* ws, cudaStream_t st) {
     return NB200_ERR_LAUNCH;
   }
   a.list.count = static_cast<const int*>(ws);
+  a.list.taken = static_cast<int*>(ws) + 1;
   a.list.items = reinterpret_cast<const WorkItem*>(static_cast<const char*>(ws) + 16);
   a.kv_heads = p.kv_heads; a.group = p.group; a.heads = p.heads;
   a.group_magic = uint32_t((65536 + p.group - 1) / p.group);
