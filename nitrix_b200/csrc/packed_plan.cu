@@ -3,8 +3,8 @@
 // The lengths are in device memory, so the blocks of all sequences are listed there, by one CTA.  Two things decide their
 // order.  CTAs that work on one sequence side by side share its keys in L2 (forward), or its queries and the sums of dq, which
 // every key block adds to (backward: with all sequences' blocks sorted by length alone, 16 documents of up to 4096 tokens, the
-// sums alone are 284 MB and the kernel takes 1252 us for 1120).  And the longest blocks of what is left should come first, so that
-// short ones even out the end.  So the sequences, longest first, are cut into groups of at least two blocks per SM, and within a
+// sums alone are 284 MB and the kernel takes 1252 us for 1054).  And the longest blocks of what is left should come first, so that
+// short ones even out the end.  So the sequences, longest first, are cut into groups of at least one block per SM (two: 1078 us, three: 1089), and within a
 // group the blocks are sorted by their length in tiles; blocks of one length come in any order, which changes no result.
 // The other CTAs clear the outputs of tokens that belong to no sequence.
 #include "dependent_launch.cuh"
@@ -19,7 +19,7 @@ constexpr int kClearCtas = 31;
 constexpr int kBuckets = 1024;         // group, then length
 constexpr int kLengths = 64;           // of them per group, longest first
 constexpr int kGroups = kBuckets / kLengths;
-constexpr int kGroupItems = 2 * 148;   // (block, key head) pairs that a group has at least
+constexpr int kGroupItems = 148;       // (block, key head) pairs that a group has at least
 
 struct PlanArgs {
   PackedArgs a;

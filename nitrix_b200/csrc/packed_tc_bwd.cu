@@ -101,9 +101,9 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   const int s_begin = a.causal ? min(max(it.seen, 0), it.other_n) / a.tokens : 0, s_end = (it.other_n + a.tokens - 1) / a.tokens;
   const int n_steps = max(s_end - s_begin, 0);
   // The CTAs of one sequence and key head read the same rows and add into the same sums.  They walk from the sequence's end to
-  // its front (and wrap around), each two steps behind its neighbour: near enough to find the rows in L2, and not on the same
+  // its front (and wrap around), each one step behind its neighbour: near enough to find the rows in L2, and not on the same
   // lines at the same moment.
-  const int rot = n_steps > 0 ? int((uint32_t(it.index) * 2u) % uint32_t(n_steps)) : 0;
+  const int rot = n_steps > 0 ? int((uint32_t(it.index)) % uint32_t(n_steps)) : 0;
   auto step_of = [&](int n) {   // the n-th step this CTA visits, counted within the sequence
     int j = n + rot;
     if (j >= n_steps) j -= n_steps;
