@@ -26,6 +26,7 @@ struct PackedArgs {
   int causal;
   float scale;
   float* delta;              // (tokens_q, heads): rowsum(out * dout)
+  float* parts;              // fp32 units: parts of dk and dv, [part][dk, dv][token][key head][D]
 };
 
 #ifdef __CUDACC__
@@ -70,6 +71,7 @@ __device__ __forceinline__ Place find_place(int index, int sequences, Count coun
 int launch_clear_uncovered(const PackedArgs& a, int dtype, bool backward, cudaStream_t st);
 int launch_packed_delta(const PackedArgs& a, int dtype, cudaStream_t st);
 int simt_packed_fwd(const PackedArgs& a, int dtype, cudaStream_t st);
+size_t simt_packed_bwd_bytes(const PackedArgs& a);
 int simt_packed_bwd(const PackedArgs& a, int dtype, cudaStream_t st);
 
 }  // namespace packed

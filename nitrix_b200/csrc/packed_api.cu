@@ -43,7 +43,7 @@ bool tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
 
 size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
   if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a);
-  return pass == NB200_PASS_FWD ? 0 : delta_bytes(p);
+  return pass == NB200_PASS_FWD ? 0 : delta_bytes(p) + simt_packed_bwd_bytes(a);
 }
 
 int check_workspace(const nb200_packed_params* p, const PackedArgs& a, int pass, const char* what) {
@@ -108,6 +108,7 @@ extern "C" NB200_API int nb200_packed_bwd(const nb200_packed_params* p, void* cu
   prof_call_begin(st);
   if (tensor_cores(p, a, NB200_PASS_BWD)) return tc_packed_bwd(a, p->dtype, p->workspace, st);
   a.delta = static_cast<float*>(p->workspace);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + delta_bytes(p));
   if (int rc = launch_clear_uncovered(a, p->dtype, true, st)) return rc;
   if (p->sequences == 0) return NB200_OK;
   if (p->tokens_q > 0) {
