@@ -46,7 +46,7 @@ typedef struct nb200_packed_params {
   int32_t causal;
   float scale;
   int32_t kernel;            /* nb200_kernel: AUTO or SIMT */
-  void* workspace;           /* nb200_packed_workspace_bytes of the pass */
+  void* workspace;           /* nb200_packed_workspace_bytes of the pass, asked for with the same operands; 256-byte aligned */
   size_t workspace_bytes;
 } nb200_packed_params;
 

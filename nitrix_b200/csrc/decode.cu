@@ -672,6 +672,7 @@ extern "C" NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_s
     set_error("decode: workspace of %zu bytes needed (nb200_decode_workspace_bytes), %zu given", pl.bytes, p->workspace_bytes);
     return NB200_ERR_WORKSPACE;
   }
+  if (!aligned16(p->workspace)) { set_error("decode: the workspace must begin on a 16-byte boundary"); return NB200_ERR_ALIGNMENT; }
   DecodeArgs a{};
   a.k = c.k; a.v = c.v;
   for (int i = 0; i < 3; ++i) { a.ks[i] = c.k_stride[i]; a.vs[i] = c.v_stride[i]; }

@@ -637,7 +637,7 @@ struct RotaryRule : torch::autograd::Function<RotaryRule> {
     if (!gq.defined() && !gk.defined()) return d;
     const auto s = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(s[0].device());
-    const tensor_list r = rotate(gq, gk, s[0], s[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
+    const tensor_list r = rotate(gq, gk, s[0].contiguous(), s[1].contiguous(), ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
     d[0] = r[0];
     d[1] = r[1];
     return d;

@@ -52,6 +52,7 @@ int check_workspace(const nb200_packed_params* p, const PackedArgs& a, int pass,
     set_error("%s: workspace of %zu bytes needed (nb200_packed_workspace_bytes), %zu given", what, need, p->workspace_bytes);
     return NB200_ERR_WORKSPACE;
   }
+  if (need && reinterpret_cast<uintptr_t>(p->workspace) % 256) { set_error("%s: the workspace must begin on a 256-byte boundary", what); return NB200_ERR_ALIGNMENT; }
   return NB200_OK;
 }
 

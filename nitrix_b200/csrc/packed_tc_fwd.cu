@@ -611,8 +611,10 @@ int launch_one(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
   return check_launch("packed_fwd_tc_kernel");
 }
 
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 bool strides_fit(const void* base, const int64_t (&s)[2], int tokens, int heads) {
-  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (tokens <= 1 || (s[0] > 0 && s[0] % 8 == 0)) && (heads <= 1 || (s[1] > 0 && s[1] % 8 == 0));
+  return aligned16(base) && (tokens <= 1 || (s[0] > 0 && s[0] % 8 == 0)) && (heads <= 1 || (s[1] > 0 && s[1] % 8 == 0));
 }
 
 }  // namespace
@@ -621,11 +623,12 @@ bool strides_fit(const void* base, const int64_t (&s)[2], int tokens, int heads)
 bool tc_packed_supported(const PackedArgs& a, int dtype) {
   return dtype != NB200_F32 && (a.D == 64 || a.D == 128) && a.group <= 64 && a.scale > 0.f && a.scale < 1e30f &&
          int64_t(a.tokens_q) * a.heads <= 0x7fffffff && a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
-         strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads);
+         strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads) && aligned16(a.out);
 }
 
 bool tc_packed_bwd_supported(const PackedArgs& a, int dtype) {
-  return tc_packed_supported(a, dtype) && strides_fit(a.dout, a.dos, a.tokens_q, a.heads);
+  return tc_packed_supported(a, dtype) && strides_fit(a.dout, a.dos, a.tokens_q, a.heads) && aligned16(a.dq) && aligned16(a.dk) &&
+         aligned16(a.dv);
 }
 
 size_t tc_packed_fwd_bytes(const PackedArgs& a) {

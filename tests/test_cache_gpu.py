@@ -278,6 +278,36 @@ def test_decode_offsets_beyond_32_bits():
     _check_decode(torch.randn(1, 8, D, device="cuda").bfloat16(), cache, [35 * page - 3])
 
 
+def test_pages_beyond_32_bits():
+    """Append, fork and compact in a pool of more than 2^31 elements, at its end."""
+    from nitrix_b200.nn import PagedCache, cache_append, cache_compact, cache_fork
+
+    page, Hk, D = 16, 2, 64
+    pool = (1 << 31) // (page * Hk * D) + 100
+    k_pages = torch.zeros(pool, Hk, page, D, dtype=torch.float16, device="cuda")
+    ints = dict(dtype=torch.int32, device="cuda")
+    order = torch.arange(pool - 1, -1, -1, **ints)
+    cache = PagedCache(k_pages, torch.zeros_like(k_pages), torch.full((2, 8), -1, **ints), torch.zeros(2, **ints), order,
+                       torch.tensor([0, pool], **ints), torch.zeros(1, **ints))
+    k = torch.randn(70, Hk, D, device="cuda").half()
+    cache = cache_append(cache, k, -k, torch.tensor([0, 37, 70], **ints))
+    assert cache.table[:, :3].tolist() == [[pool - 1, pool - 2, pool - 3], [pool - 4, pool - 5, pool - 6]]
+
+    def held(c, row, n):
+        t = torch.arange(n, device="cuda")
+        where = c.table[row].long()[t // page], slice(None), t % page
+        return c.k_pages[where], c.v_pages[where]
+    for c in (cache, cache_fork(cache, torch.tensor([1, 1, 0], **ints))):
+        parents = [0, 1] if c.lengths.shape[0] == 2 else [1, 1, 0]
+        packed = cache_compact(c)
+        assert int(packed.table.max()) < 10
+        for row, parent in enumerate(parents):
+            want = k[:37] if parent == 0 else k[37:]
+            for state in (c, packed):
+                got = held(state, row, want.shape[0])
+                assert torch.equal(got[0], want) and torch.equal(got[1], -want)
+
+
 def test_decode_is_the_same_every_time():
     from nitrix_b200.nn import decode_attention
 
