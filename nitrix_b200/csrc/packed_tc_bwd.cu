@@ -8,13 +8,17 @@
 // over the rows, so that the sum over a group's heads costs nothing; dQ of a step goes to fp32 sums in global memory by
 // 16-byte reductions, which is the one place where the order of a sum is not fixed.  The scheme of a step -- two issuing
 // warps, two element-wise groups on alternate steps, lse and delta added by a K = 16 MMA step, dQ^T with d on the TMEM lanes --
-// is that of sdpa_tc_bwd_d128.cu, which has the reasons and the measurements.  At head dim 64 the tile of dQ^T has 128 lanes as
+// is that of sdpa_tc_bwd_d128.cu, which has the reasons and the measurements.  One thing is different: dS goes to TMEM as well,
+// as the A operand of dK, which takes an eighth off what the MMAs read from shared memory (8192 tokens, 16 heads on 4, causal,
+// head dim 128: 710 -> 682 us).  At head dim 64 the tile of dQ^T has 128 lanes as
 // well, of which the upper 64 (V in place of K: the tiles lie one after the other) are not read.
 //
 // What belongs to a neighbouring sequence must not get into a sum, not even as 0 * NaN: keys behind the end have P and dS
 // selected to zero and their rows of K cleared in shared memory, queries behind the end have P and dS selected to zero and
 // their rows of Q and dO cleared.  Warp 3, which forms the addends of every step before its products may run, does that.
-// Bound by the element-wise warps and the shared-memory traffic of the MMAs as that kernel is.  All waits bounded.
+// Head dim 128: bound by the operands that the MMAs read from shared memory (about 1900 of a step's 2700 cycles) and by the sums
+// of dq in L2 (without them, for timing: 744 -> 551 us when it was 744).  Head dim 64: by the chain of a step; two steps' products
+// in TMEM 522 -> 508 us, two dS tiles as well 551.  All waits bounded.
 #include <math.h>
 
 #include "dependent_launch.cuh"
@@ -171,8 +175,11 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tm_dv = tmem, tm_dk = tmem + 128, tm_p1 = tmem + 256, tm_p2 = tmem + 320, tm_e = tmem + 384,
-                 tm_dq = tmem + 448;
+  // TMEM: dV, dK, the products P1 and P2 (at head dim 64 there is room for those of two steps), p and ds, dQ^T
+  constexpr int kProds = D == 64 ? 2 : 1;
+  const uint32_t tm_dv = tmem, tm_dk = tmem + D, tm_e = tmem + 384, tm_dq = tmem + 448;
+  auto tm_p1 = [&](int n) { return tmem + 2 * D + (n & (kProds - 1)) * 64; };
+  auto tm_p2 = [&](int n) { return tmem + 2 * D + kProds * 64 + (n & (kProds - 1)) * 64; };
 
   if (warp < 4) {
   reg_dealloc<kProducerRegs>();
@@ -195,8 +202,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       for (int n = 0; n < n_steps && ok; ++n) {
         const int st = n % NY, s = n & 1;
         ok = wait_or_abort(bar(Y_FULL + st), (n / NY) & 1, abort_flag, a.status, 504);
-        // a product may be overwritten once the warps of step n - 1 hold it in registers
-        if (ok && n >= 1) ok = wait_or_abort(bar(P_FREE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_flag, a.status, 509);
+        // a product may be overwritten once the warps of the step before on its columns hold it in registers
+        if (ok && n >= kProds) ok = wait_or_abort(bar(P_FREE + ((n - kProds) & 1)), ((n - kProds) >> 1) & 1, abort_flag, a.status, 509);
         if (ok) ok = wait_or_abort(bar(AUG_FULL + s), (n >> 1) & 1, abort_flag, a.status, 512);
         if (!ok) break;
         tc_fence_after_sync();
@@ -207,22 +214,22 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint64_t xo = uint64_t(((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4);
           const uint64_t yo = uint64_t(((kk / 4) * kYBoxBytes + (kk % 4) * 32) >> 4);
-          mma_ss(tm_p1, kdesc + xo, qdesc + yo, idesc_prod, kk > 0 ? 1u : 0u);
+          mma_ss(tm_p1(n), kdesc + xo, qdesc + yo, idesc_prod, kk > 0 ? 1u : 0u);
         }
         // P1 += W C1^T (C1: -lse / (scale log2e))
-        mma_ss(tm_p1, wdesc, make_smem_desc_noswizzle(aslot, 128, 256), idesc_prod, 1u);
+        mma_ss(tm_p1(n), wdesc, make_smem_desc_noswizzle(aslot, 128, 256), idesc_prod, 1u);
         mma_commit(bar(PROD_FULL + s));
-        if (n >= 1) ok = wait_or_abort(bar(P_FREE + 2 + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_flag, a.status, 519);
+        if (n >= kProds) ok = wait_or_abort(bar(P_FREE + 2 + ((n - kProds) & 1)), ((n - kProds) >> 1) & 1, abort_flag, a.status, 519);
         if (!ok) break;
         tc_fence_after_sync();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint64_t xo = uint64_t(((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4);
           const uint64_t yo = uint64_t(((kk / 4) * kYBoxBytes + (kk % 4) * 32) >> 4);
-          mma_ss(tm_p2, vdesc + xo, gdesc + yo, idesc_prod, kk > 0 ? 1u : 0u);
+          mma_ss(tm_p2(n), vdesc + xo, gdesc + yo, idesc_prod, kk > 0 ? 1u : 0u);
         }
         // P2 += W C2^T (C2: -delta)
-        mma_ss(tm_p2, wdesc, make_smem_desc_noswizzle(aslot + L::kAugTileBytes, 128, 256), idesc_prod, 1u);
+        mma_ss(tm_p2(n), wdesc, make_smem_desc_noswizzle(aslot + L::kAugTileBytes, 128, 256), idesc_prod, 1u);
         mma_commit(bar(AUG_FREE + s));
         mma_commit(bar(PROD_FULL + 2 + s));
       }
@@ -230,19 +237,18 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   } else if (warp == 0) {
     // ---------------- MMA issuer 2: dV, dK and dQ^T of every step ----------------
     if (elect_one() && n_steps > 0) {
-      constexpr uint32_t idesc_acc = make_idesc(kBf16, kTile, D, false, true);      // dV: A from TMEM, B = dO MN-major
-      constexpr uint32_t idesc_dk = make_idesc(kBf16, kTile, D, false, true);       // dK: A = ds K-major, B = Q MN-major
+      constexpr uint32_t idesc_acc = make_idesc(kBf16, kTile, D, false, true);      // dV, dK: A (p, ds) from TMEM, B (dO, Q) MN-major
       constexpr uint32_t idesc_dq = make_idesc(kBf16, kTile, kStep, true, true);    // dQ^T: A = K MN-major, B = ds MN-major
       bool ok = wait_or_abort(bar(X_FULL), 0, abort_flag, a.status, 503);
       const uint64_t kmn = make_smem_desc(sbase + L::kX, kBoxBytes, 1024);          // K as [d x key], d contiguous
       const uint32_t dsbuf = sbase + L::kDs;
-      const uint64_t ds_a = make_smem_desc(dsbuf, 16, 1024), ds_b = make_smem_desc(dsbuf, kBoxBytes, 1024);
+      const uint64_t ds_b = make_smem_desc(dsbuf, kBoxBytes, 1024);
       for (int m = 0; m < n_steps && ok; ++m) {
         const int st = m % NY, s = m & 1;
         const uint32_t ybase = sbase + L::kY + st * L::kYStageBytes;
         const uint64_t qmn = make_smem_desc(ybase, kYBoxBytes, 1024);                    // Q as [query x d], d contiguous
         const uint64_t gmn = make_smem_desc(ybase + L::kYBytes, kYBoxBytes, 1024);      // dO likewise
-        const uint32_t e1 = tm_e + s * 32;
+        const uint32_t e1 = tm_e, e2 = tm_e + 32;      // p, ds
         // dV += p^T dO as soon as p is there: it runs while the warps still form ds
         ok = wait_or_abort(bar(P_READY + s), (m >> 1) & 1, abort_flag, a.status, 519);
         if (!ok) break;
@@ -257,7 +263,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         tc_fence_after_sync();
 #pragma unroll
         for (int kk = 0; kk < kStep / 16; ++kk)
-          mma_ss(tm_dk, ds_a + uint64_t((kk * 32) >> 4), qmn + uint64_t((kk * 2048) >> 4), idesc_dk, (m > 0 || kk > 0) ? 1u : 0u);
+          mma_ts(tm_dk, e2 + kk * 8, qmn + uint64_t((kk * 2048) >> 4), idesc_acc, (m > 0 || kk > 0) ? 1u : 0u);
         mma_commit(bar(Y_EMPTY + st));           // the last readers of this Q / dO stage
         // dQ^T[d, row] = sum_key K[key, d] ds[key, row]; the previous tile must have been drained
         if (m >= 1) {
@@ -419,8 +425,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       float2 t[kStep / 2];
       {
         uint32_t raw[kStep];
-        tmem_ld32(tm_p1 + lane_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-        tmem_ld32(tm_p1 + lane_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+        tmem_ld32(tm_p1(n) + lane_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+        tmem_ld32(tm_p1(n) + lane_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
         tmem_wait_ld();
         tc_fence_before_sync();
         __syncwarp();
@@ -439,13 +445,13 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         t[c] = make_float2(ex2(x.x), ex2(x.y));
         e1[c] = pack2<kBf16>(t[c].x, t[c].y);
       }
-      // p of this stage is still being read by dV of step n - 2
-      if (n >= 2) {
-        ok = wait_or_abort(bar(E_FREE + s), ((n - 2) >> 1) & 1, abort_flag, a.status, 510);
+      // p is still being read by dV of step n - 1
+      if (n >= 1) {
+        ok = wait_or_abort(bar(E_FREE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_flag, a.status, 510);
         if (!ok) break;
         tc_fence_after_sync();
       }
-      tmem_st32(tm_e + s * 32 + lane_addr, e1);
+      tmem_st32(tm_e + lane_addr, e1);
       // ds = p dP (dP arrives with -delta already added)
       ok = wait_or_abort(bar(PROD_FULL + 2 + s), (n >> 1) & 1, abort_flag, a.status, 518);
       if (!ok) break;
@@ -457,8 +463,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       tc_fence_after_sync();
       {
         uint32_t raw[kStep];
-        tmem_ld32(tm_p2 + lane_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-        tmem_ld32(tm_p2 + lane_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+        tmem_ld32(tm_p2(n) + lane_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+        tmem_ld32(tm_p2(n) + lane_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
         tmem_wait_ld();
         tc_fence_before_sync();
         __syncwarp();
@@ -475,15 +481,18 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           e2[c] = pack2<kBf16>(ds.x, ds.y);
         }
       }
-      // the ds buffer was last read by the MMAs of step n - 1
+      // ds, in TMEM for dK and in shared memory for dQ, was last read by the MMAs of step n - 1
       if (n >= 1) {
         ok = wait_or_abort(bar(DS_FREE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_flag, a.status, 517);
         if (!ok) break;
+        tc_fence_after_sync();
       }
+      tmem_st32(tm_e + 32 + lane_addr, e2);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         st_shared_v4(ds_thread ^ (uint32_t(i) << 4), make_uint4(e2[4 * i], e2[4 * i + 1], e2[4 * i + 2], e2[4 * i + 3]));
       fence_proxy_async_smem();
+      tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(E_READY + s));
