@@ -33,9 +33,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 
 struct DecodeArgs {
-  const void* k;
-  const void* v;
-  int64_t ks[3], vs[3];      // elements, over (page, head, slot)
+  const uint4* k;
+  const uint4* v;
+  int ks[3], vs[3];          // 16-byte words, over (page, head, slot): 32 bits, so that an offset is one wide multiply-add each
   int pages, kv_heads, page_size, page_shift;   // page_shift: log2 of page_size, or -1
   int D;
   const int* table;
@@ -45,7 +45,7 @@ struct DecodeArgs {
   int64_t qs[2];
   void* out;
   int q_heads, group;        // query heads, and those of one key head
-  int chunks;                // runs of query heads that a key head's group is taken in
+  int chunks;                // times that a key head's group is taken, kSide chunks of query heads side by side each
   float mul;                 // scale * log2 e
   int unit;                  // tokens per unit of work
   float* part;               // pieces: [2 * CTAs][heads of a chunk][D + 4]: output, maximum (base 2), sum
@@ -104,12 +104,19 @@ __device__ __forceinline__ void find_row(const DecodeArgs& a, int lane, int64_t 
   *row_begin = before;
 }
 
-// Element offsets of a token's row, of a head at `head_off`; the page is checked.
-__device__ __forceinline__ int page_of(const DecodeArgs& a, const int* row_table, int token, int* slot) {
+// Where a token's row lies: its page (cut to the pool) and slot.
+struct Where {
+  int page, slot;
+};
+__device__ __forceinline__ int page_at(const DecodeArgs& a, const int* row_table, int column) {
+  return min(max(__ldg(row_table + column), 0), a.pages - 1);
+}
+__device__ __forceinline__ Where where(const DecodeArgs& a, const int* row_table, int token) {
   const int column = a.page_shift >= 0 ? token >> a.page_shift : token / a.page_size;
-  *slot = token - (a.page_shift >= 0 ? column << a.page_shift : column * a.page_size);
-  const int page = __ldg(row_table + column);
-  return min(max(page, 0), a.pages - 1);
+  return Where{page_at(a, row_table, column), token - (a.page_shift >= 0 ? column << a.page_shift : column * a.page_size)};
+}
+__device__ __forceinline__ const uint4* row_of(const uint4* base, const int (&stride)[3], Where w) {
+  return base + int64_t(w.page) * stride[0] + int64_t(w.slot) * stride[2];
 }
 
 // ---- warp-level MMA ------------------------------------------------------------------------------------------------------
@@ -131,22 +138,22 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// One warp's part of a piece: blocks of 16 tokens `warp`, `warp + kWarps`, ... of [t0, t1) of a sequence.
+// Part `wi` of `wn` of a piece, for one warp: blocks of 16 tokens wi, wi + wn, ... of [t0, t1) of a sequence.
 template <int D, int kTiles, bool kBf16>
 struct MmaLoop {
   static constexpr int kHeads = 8 * kTiles;      // query heads of a chunk
   static constexpr int kBlock = 16;              // tokens
-  static constexpr int kSlots = kWarps;          // partial results of a CTA
-  static constexpr int kMinCtas = kTiles == 1 ? 4 : 2;
+  static constexpr int kSlots = 1;               // partial results of a warp
+  static constexpr int kMinCtas = kTiles == 1 ? 4 : D == 64 ? 3 : 2;
   float o[kTiles][D / 16][4];                    // O^T: lane (g, t): head 2t (+1), see store
   float m[kTiles][2], l[kTiles][2];              // of heads 2t, 2t + 1; l: this lane's keys
 
   __device__ __forceinline__ void run(const DecodeArgs& a, const int* row_table, int kv_head, const void* q_row, int heads,
-                                      int t0, int t1) {
+                                      int t0, int t1, int wi, int wn) {
     const uint16_t* q = static_cast<const uint16_t*>(q_row);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + kv_head * a.ks[1];
-    const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + kv_head * a.vs[1];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
+    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
     uint4 qf[kTiles][D / 32];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -162,33 +169,40 @@ struct MmaLoop {
     }
     const int last = t1 - 1;
     uint4 kf[2][D / 32], vf[4][D / 64];
-    auto load_k = [&](int b0) {
+    // Blocks begin at multiples of 16 tokens, so that a block lies in one page where pages are of 16, 32, ... slots: the page is
+    // looked up once, a turn ahead.
+    const bool one_page = a.page_shift >= 4;
+    auto page_of_block = [&](int b) { return one_page && b < t1 ? page_at(a, row_table, b >> a.page_shift) : 0; };
+    auto place = [&](int b, int page, int token) {
+      token = min(token, last);
+      if (one_page) return Where{page, (b & (a.page_size - 1)) + token - b};
+      return where(a, row_table, token);
+    };
+    auto load_k = [&](int b, int page) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        int slot;
-        const int64_t page = page_of(a, row_table, min(b0 + g + 8 * r, last), &slot);
-        const uint16_t* row = kbase + page * a.ks[0] + slot * a.ks[2];
+        const uint4* row = row_of(kbase, a.ks, place(b, page, b + g + 8 * r));
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) kf[r][i] = sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(row + (i * 4 + t) * 8));
+        for (int i = 0; i < D / 32; ++i) kf[r][i] = sm100::ldg_no_allocate(row + i * 4 + t);
       }
     };
-    auto load_v = [&](int b0) {
+    auto load_v = [&](int b, int page) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        int slot;
-        const int64_t page = page_of(a, row_table, min(b0 + 2 * t + (r & 1) + (r >> 1) * 8, last), &slot);
-        const uint16_t* row = vbase + page * a.vs[0] + slot * a.vs[2];
+        const uint4* row = row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8));
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) vf[r][i] = sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(row + i * 64 + g * 8));
+        for (int i = 0; i < D / 64; ++i) vf[r][i] = sm100::ldg_no_allocate(row + i * 8 + g);
       }
     };
-    int b0 = t0 + warp * kBlock;
+    int b0 = t0 + wi * kBlock;
     if (b0 >= t1) return;
-    load_k(b0);
-    load_v(b0);
+    int next_page = page_of_block(b0);
+    load_k(b0, next_page);
+    load_v(b0, next_page);
+    next_page = page_of_block(b0 + wn * kBlock);
     const float thr = a.mul > 0.f ? 8.f / a.mul : INFINITY;
-    for (; b0 < t1; b0 += kWarps * kBlock) {
-      const int next = b0 + kWarps * kBlock;
+    for (; b0 < t1; b0 += wn * kBlock) {
+      const int next = b0 + wn * kBlock;
       float s[kTiles][4];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
@@ -201,7 +215,7 @@ struct MmaLoop {
           mma16816<kBf16>(s[n], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[n][i].x, qf[n][i].y);
           mma16816<kBf16>(s[n], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[n][i].z, qf[n][i].w);
         }
-      if (next < t1) load_k(next);      // (the keys are used: their registers take the next block's)
+      if (next < t1) load_k(next, next_page);      // (the keys are used: their registers take the next block's)
       uint32_t pt[kTiles][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
@@ -247,7 +261,8 @@ struct MmaLoop {
           for (int n = 0; n < kTiles; ++n) mma16816<kBf16>(o[n][i * 4 + e], a0, a1, a2, a3, pt[n][0], pt[n][1]);
         }
       }
-      if (next < t1) load_v(next);
+      if (next < t1) load_v(next, next_page);
+      next_page = page_of_block(next + wn * kBlock);
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
@@ -279,115 +294,155 @@ struct MmaLoop {
 };
 
 // ---- fp32 multiply-adds ----------------------------------------------------------------------------------------------------
-// kLanes lanes share a token's row, kPer 16-byte words each; 8 query heads.  A warp's 32 / kLanes groups take tokens of their own.
-template <typename T, int kLanes, int kPer>
+// kLanes lanes share a token's row, kPer 16-byte words each.  A warp's 32 / kLanes groups take tokens of their own, kAhead at a
+// time: the next ones' keys are on their way from the scores on, their values from the end of the output sums on.
+template <typename T, int kLanes, int kPer, int kNumHeads>
 struct FmaLoop {
-  static constexpr int kHeads = 8;
+  static constexpr int kHeads = kNumHeads;
   static constexpr int kVec = 16 / int(sizeof(T));
-  static constexpr int kGroups = kThreads / kLanes;
-  static constexpr int kSlots = kGroups;
-  static constexpr int kAhead = 2;
-  static constexpr int kMinCtas = 2;
-  float o[kHeads][kPer][kVec];
+  static constexpr int kSlots = 32 / kLanes;
+  static constexpr int kAhead = sizeof(T) == 4 && kPer == 1 ? 4 : 2;
+  static constexpr int kMinCtas = sizeof(T) == 4 && kPer == 1 ? 4 : 2;
+  static constexpr int kSteps = kHeads == 8 ? 3 : kHeads == 4 ? 2 : kHeads == 2 ? 1 : 0;   // of the reduce-scatter
+  float2 o[kHeads][kPer][kVec / 2];      // (pairs: two multiply-adds per instruction)
   float m, l;             // of the head that the reduce-scatter leaves in this lane
 
-  __device__ __forceinline__ static int my_head(int c) {   // bits of the lane, high to low: the reduce-scatter's choices
-    return ((c & (kLanes / 2)) ? 4 : 0) + ((c & (kLanes / 4)) ? 2 : 0) + ((c & (kLanes / 8)) ? 1 : 0);
+  __device__ __forceinline__ static int my_head(int c) {   // the reduce-scatter's choices, high to low
+    int h = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) h = 2 * h + ((c & (kLanes >> (s + 1))) ? 1 : 0);
+    return h;
   }
-  // the lane (of a group) that holds head h
+  // the first lane (of a group) that holds head h
   __device__ __forceinline__ static int lane_of(int h) {
-    return ((h & 4) ? kLanes / 2 : 0) + ((h & 2) ? kLanes / 4 : 0) + ((h & 1) ? kLanes / 8 : 0);
+    int c = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      if (h & (kHeads >> (s + 1))) c += kLanes >> (s + 1);
+    return c;
   }
 
-  __device__ __forceinline__ void run(const DecodeArgs& a, const int* row_table, int kv_head, const T* q, int heads, int t0, int t1) {
-    const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes, lane = threadIdx.x & 31;
+  __device__ __forceinline__ void run(const DecodeArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0,
+                                      int t1, int wi, int wn) {
+    const T* q = static_cast<const T*>(q_row);
+    const int c = threadIdx.x % kLanes, lane = threadIdx.x & 31;
+    const int first = wi * kSlots, group = first + lane / kLanes, groups = wn * kSlots;
     const int words = a.D / kVec;
-    float qf[kHeads][kPer][kVec];
+    float2 qf[kHeads][kPer][kVec / 2];
 #pragma unroll
     for (int h = 0; h < kHeads; ++h)
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
         const bool in = h < heads && c + p * kLanes < words;
+        const T* e = q + h * a.qs[1] + (c + p * kLanes) * kVec;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          qf[h][p][e] = in ? to_f32<T>(q[h * a.qs[1] + (c + p * kLanes) * kVec + e]) : 0.f;
-          o[h][p][e] = 0.f;
+        for (int i = 0; i < kVec / 2; ++i) {
+          qf[h][p][i] = in ? make_float2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1])) : make_float2(0.f, 0.f);
+          o[h][p][i] = make_float2(0.f, 0.f);
         }
       }
     m = -INFINITY;
     l = 0.f;
-    const T* kbase = static_cast<const T*>(a.k) + kv_head * a.ks[1];
-    const T* vbase = static_cast<const T*>(a.v) + kv_head * a.vs[1];
+    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
+    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
     const int last = t1 - 1;
-    // (every group of a warp makes as many turns as its first, which has the most: the shuffles below are warp-wide)
-    const int first_group = group - (group % (32 / kLanes));
-    for (int b = t0; b + first_group < t1; b += kGroups * kAhead) {
-      uint4 kw[kAhead][kPer], vw[kAhead][kPer];
+    uint4 kw[kAhead][kPer], vw[kAhead][kPer];
+    Where at[kAhead];       // of the tokens whose keys were asked for last
+    auto load = [&](uint4 (&w)[kAhead][kPer], const uint4* base, const int (&stride)[3]) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        int slot;
-        const int64_t page = page_of(a, row_table, min(b + group + j * kGroups, last), &slot);
+        const uint4* row = row_of(base, stride, at[j]);
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) w[j][p] = c + p * kLanes < words ? __ldg(row + c + p * kLanes) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto load_k = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) at[j] = where(a, row_table, min(b + group + j * groups, last));
+      load(kw, kbase, a.ks);
+    };
+    // (every group of a warp makes as many turns as its first, which has the most: the shuffles below are warp-wide)
+    int b = t0;
+    if (b + first >= t1) return;
+    load_k(b);
+    load(vw, vbase, a.vs);
+    for (; b + first < t1; b += groups * kAhead) {
+      const int next = b + groups * kAhead;
+      float x[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        float2 s2[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) s2[h] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int p = 0; p < kPer; ++p) {
-          const bool in = c + p * kLanes < words;
-          kw[j][p] = in ? sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(kbase + page * a.ks[0] + slot * a.ks[2]) + c + p * kLanes) : make_uint4(0, 0, 0, 0);
-          vw[j][p] = in ? sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(vbase + page * a.vs[0] + slot * a.vs[2]) + c + p * kLanes) : make_uint4(0, 0, 0, 0);
-        }
-      }
+          const T* e = reinterpret_cast<const T*>(&kw[j][p]);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        float s[kHeads];
+          for (int i = 0; i < kVec / 2; ++i) {
+            const float2 x2 = make_float2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1]));
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          s[h] = 0.f;
-#pragma unroll
-          for (int p = 0; p < kPer; ++p) {
-            const T* e = reinterpret_cast<const T*>(&kw[j][p]);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) s[h] = fmaf(qf[h][p][i], to_f32<T>(e[i]), s[h]);
+            for (int h = 0; h < kHeads; ++h) s2[h] = __ffma2_rn(qf[h][p][i], x2, s2[h]);
           }
         }
-        // reduce-scatter: every step halves the heads that a lane still sums
+        float s[kHeads];
 #pragma unroll
-        for (int step = 0; step < 3; ++step) {
-          const int off = kLanes >> (step + 1), n = 4 >> step;
+        for (int h = 0; h < kHeads; ++h) s[h] = s2[h].x + s2[h].y;
+        // reduce-scatter: every step halves the heads that a lane still sums; then what is left of the lanes
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          const int off = kLanes >> (step + 1), n = kHeads >> (step + 1);
           const bool upper = (c & off) != 0;
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
+          for (int h = 0; h < kHeads / 2; ++h) {
             if (h >= n) continue;
             const float keep = upper ? s[h + n] : s[h], send = upper ? s[h] : s[h + n];
             s[h] = keep + __shfl_xor_sync(0xffffffffu, send, off);
           }
         }
 #pragma unroll
-        for (int off = kLanes / 16; off > 0; off >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
-        float x = s[0] * a.mul;
-        if (b + group + j * kGroups >= t1) x = -INFINITY;
-        const float m_new = fmaxf(m, x);
-        const float shift = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = ex2(m - shift), pr = ex2(x - shift);
-        l = l * alpha + pr;
-        const bool moved = __any_sync(0xffffffffu, m_new > m);
-        m = m_new;
+        for (int off = kLanes >> (kSteps + 1); off > 0; off >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+        x[j] = b + group + j * groups < t1 ? s[0] * a.mul : -INFINITY;
+      }
+      if (next + first < t1) load_k(next);
+      float m_new = m;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) m_new = fmaxf(m_new, x[j]);
+      const float shift = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = ex2(m - shift);
+      if (__any_sync(0xffffffffu, m_new > m)) {
+        l *= alpha;
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
-          const int from = (lane & ~(kLanes - 1)) + lane_of(h);
-          const float ph = __shfl_sync(0xffffffffu, pr, from);
-          if (moved) {
-            const float ah = __shfl_sync(0xffffffffu, alpha, from);
+          const float ah = __shfl_sync(0xffffffffu, alpha, (lane & ~(kLanes - 1)) + lane_of(h));
 #pragma unroll
-            for (int p = 0; p < kPer; ++p)
+          for (int p = 0; p < kPer; ++p)
 #pragma unroll
-              for (int i = 0; i < kVec; ++i) o[h][p][i] *= ah;
-          }
+            for (int i = 0; i < kVec / 2; ++i) o[h][p][i] = __fmul2_rn(o[h][p][i], make_float2(ah, ah));
+        }
+      }
+      m = m_new;
 #pragma unroll
-          for (int p = 0; p < kPer; ++p) {
-            const T* e = reinterpret_cast<const T*>(&vw[j][p]);
+      for (int j = 0; j < kAhead; ++j) {
+        const float pr = ex2(x[j] - shift);
+        l += pr;
+        float2 ph[kHeads];
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) o[h][p][i] = fmaf(ph, to_f32<T>(e[i]), o[h][p][i]);
+        for (int h = 0; h < kHeads; ++h) {
+          ph[h].x = __shfl_sync(0xffffffffu, pr, (lane & ~(kLanes - 1)) + lane_of(h));
+          ph[h].y = ph[h].x;
+        }
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) {
+          const T* e = reinterpret_cast<const T*>(&vw[j][p]);
+#pragma unroll
+          for (int i = 0; i < kVec / 2; ++i) {
+            const float2 x2 = make_float2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1]));
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) o[h][p][i] = __ffma2_rn(ph[h], x2, o[h][p][i]);
           }
         }
       }
+      if (next + first < t1) load(vw, vbase, a.vs);
     }
   }
   __device__ __forceinline__ void store(const DecodeArgs& a, float* dst) const {
@@ -399,8 +454,8 @@ struct FmaLoop {
       for (int p = 0; p < kPer; ++p)
         if (c + p * kLanes < a.D / kVec)
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) slot[h * (a.D + 2) + (c + p * kLanes) * kVec + e] = o[h][p][e];
-    if ((c & (kLanes / 8 - 1)) == 0) {
+          for (int i = 0; i < kVec / 2; ++i) *reinterpret_cast<float2*>(slot + h * (a.D + 2) + (c + p * kLanes) * kVec + 2 * i) = o[h][p][i];
+    if ((c & ((kLanes >> kSteps) - 1)) == 0) {
       float* row = slot + my_head(c) * (a.D + 2);
       row[a.D] = m;
       row[a.D + 1] = l;
@@ -408,7 +463,8 @@ struct FmaLoop {
   }
 };
 
-template <typename T, typename Loop>
+// kSide chunks of query heads are taken by the warps of a CTA side by side.
+template <typename T, typename Loop, int kSide>
 __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const DecodeArgs a) {
   extern __shared__ float merge[];      // [slot][head][D + 2]
   allow_dependents();
@@ -429,28 +485,34 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
     const int64_t item_begin = row_begin + int64_t(item) * units;
     const int kv_head = item / a.chunks, chunk = item - kv_head * a.chunks;
     const int ub = int(u - item_begin), ue = int(min(int64_t(units), u_end - item_begin));
-    const int head0 = kv_head * a.group + chunk * Loop::kHeads;
-    const int heads = min(Loop::kHeads, a.group - chunk * Loop::kHeads);
+    const int in_group = chunk * kSide * Loop::kHeads;                 // the first query head within its group
+    const int heads = min(kSide * Loop::kHeads, a.group - in_group);   // of all chunks that are taken side by side
+    const int head0 = kv_head * a.group + in_group;
     const bool whole = ub == 0 && ue == units;
-    {
+    constexpr int wn = kWarps / kSide;                                  // warps of a chunk
+    const int own = (threadIdx.x >> 5) / wn;                            // this warp's chunk
+    if (own * Loop::kHeads < heads) {
       Loop loop;
       const int t0 = ub * a.unit, t1 = min(length, ue * a.unit);
-      const T* q = static_cast<const T*>(a.q) + row * a.qs[0] + head0 * a.qs[1];
-      loop.run(a, a.table + int64_t(row) * a.width, kv_head, q, heads, t0, t1);
+      const T* q = static_cast<const T*>(a.q) + row * a.qs[0] + (head0 + own * Loop::kHeads) * a.qs[1];
+      loop.run(a, a.table + int64_t(row) * a.width, kv_head, q, min(Loop::kHeads, heads - own * Loop::kHeads), t0, t1, (threadIdx.x >> 5) % wn, wn);
       loop.store(a, merge);
     }
     __syncthreads();
-    // the CTA's result: sums over the slots, relative to their largest maximum
-    float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * Loop::kHeads * (a.D + 4);
+    // the CTA's result: sums over the slots of a head's warps, relative to their largest maximum
+    float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * kSide * Loop::kHeads * (a.D + 4);
+    constexpr int slots = wn * Loop::kSlots;
+    const int step = Loop::kHeads * (a.D + 2);
     for (int i = threadIdx.x; i < heads * a.D; i += kThreads) {
-      const int h = i / a.D, d = i - h * a.D;
-      const float* col = merge + h * (a.D + 2);
-      const int step = Loop::kHeads * (a.D + 2);
+      const int h = i / a.D, d = i - h * a.D, of = h / Loop::kHeads;
+      const float* col = merge + of * slots * step + (h - of * Loop::kHeads) * (a.D + 2);
       float mx = -INFINITY;
-      for (int s = 0; s < Loop::kSlots; ++s) mx = fmaxf(mx, col[s * step + a.D]);
+#pragma unroll
+      for (int s = 0; s < slots; ++s) mx = fmaxf(mx, col[s * step + a.D]);
       const float shift = mx == -INFINITY ? 0.f : mx;
       float sum = 0.f, acc = 0.f;
-      for (int s = 0; s < Loop::kSlots; ++s) {
+#pragma unroll
+      for (int s = 0; s < slots; ++s) {
         const float w = ex2(col[s * step + a.D] - shift);
         sum = fmaf(w, col[s * step + a.D + 1], sum);
         acc = fmaf(w, col[s * step + d], acc);
@@ -468,20 +530,83 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
   }
 }
 
-// One CTA per (row, query head): the pieces of its item, zeros for a sequence without a token.  A warp takes every fourth
-// piece, a lane 16-byte words of it; the warps' sums are added in their order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a, int heads_per_chunk) {
+// Sums of pieces w, w + stride, ... up to w1 of one query head, a lane's 16-byte words of them.
+struct Joined {
+  float top, sum;
+  float4 acc[2];
+};
+template <typename Piece>
+__device__ __forceinline__ Joined join_pieces(int w, int w1, int stride, int D, Piece piece) {
+  constexpr int kAhead = 4;
+  const int lane = threadIdx.x & 31, words = D / 4;
+  Joined r{-INFINITY, 0.f, {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)}};
+  for (; w <= w1; w += stride * kAhead) {
+    float2 st[kAhead];
+    float4 v[kAhead][2];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int wj = w + j * stride;
+      st[j] = make_float2(-INFINITY, 0.f);
+      if (wj > w1) continue;
+      const float* p = piece(wj);
+      st[j] = *reinterpret_cast<const float2*>(p + D);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + 32 * i < words) v[j][i] = reinterpret_cast<const float4*>(p)[lane + 32 * i];
+    }
+    float next = r.top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) next = fmaxf(next, st[j].x);
+    const float shift = next == -INFINITY ? 0.f : next, old = ex2(r.top - shift);
+    r.sum *= old;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { r.acc[i].x *= old; r.acc[i].y *= old; r.acc[i].z *= old; r.acc[i].w *= old; }
+    r.top = next;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (w + j * stride > w1) continue;
+      const float f = ex2(st[j].x - shift);
+      r.sum = fmaf(f, st[j].y, r.sum);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (lane + 32 * i >= words) continue;
+        r.acc[i].x = fmaf(f, v[j][i].x, r.acc[i].x); r.acc[i].y = fmaf(f, v[j][i].y, r.acc[i].y);
+        r.acc[i].z = fmaf(f, v[j][i].z, r.acc[i].z); r.acc[i].w = fmaf(f, v[j][i].w, r.acc[i].w);
+      }
+    }
+  }
+  return r;
+}
+
+// The pieces of items that no CTA had the whole of; zeros for a sequence without a token.
+//  kByItem: a CTA per (row, key head and chunk), a warp per query head: where there are items for every SM, they have few pieces
+//  otherwise a CTA per (row, query head), whose warps take every fourth piece
+template <typename T, bool kByItem>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a, int heads_per_item) {
   constexpr int kMaxWords = 64;             // 16-byte words of a head of 256
   __shared__ float4 outs[kWarps][kMaxWords];
   __shared__ float sums[kWarps], tops[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.y, head = blockIdx.x;
-  T* out = static_cast<T*>(a.out) + (int64_t(row) * a.q_heads + head) * a.D;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = a.D / 4;
+  const int row = blockIdx.y;
+  int item, h0, heads, head0;               // within the row's items; query heads of this CTA in the item; its first query head
+  if constexpr (kByItem) {
+    item = blockIdx.x;
+    const int kv_head = item / a.chunks, in_group = (item - kv_head * a.chunks) * heads_per_item;
+    h0 = 0;
+    heads = min(heads_per_item, a.group - in_group);
+    head0 = kv_head * a.group + in_group;
+  } else {
+    head0 = blockIdx.x;
+    const int kv_head = head0 / a.group, in_group = head0 - kv_head * a.group, chunk = in_group / heads_per_item;
+    item = kv_head * a.chunks + chunk;
+    h0 = in_group - chunk * heads_per_item;
+    heads = 1;
+  }
+  T* out = static_cast<T*>(a.out) + (int64_t(row) * a.q_heads + head0) * a.D;
   const int units = units_of(a, row);
   if (units == 0) {
     wait_for_previous();
-    for (int d = threadIdx.x; d < a.D; d += kThreads) out[d] = from_f32<T>(0.f);
+    for (int i = threadIdx.x; i < heads * a.D; i += kThreads) out[i] = from_f32<T>(0.f);
     return;
   }
   const int per = a.kv_heads * a.chunks;
@@ -497,77 +622,53 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
   const Share share(a, total);
-  const int kv_head = head / a.group, in_group = head - kv_head * a.group;
-  const int chunk = in_group / heads_per_chunk, h = in_group - chunk * heads_per_chunk;
-  const int64_t begin = before + int64_t(kv_head * a.chunks + chunk) * units;
+  const int64_t begin = before + int64_t(item) * units;
   const int w0 = share.worker_of(begin), w1 = share.worker_of(begin + units - 1);
   wait_for_previous();      // (the lengths are the caller's: what is above needs no wait)
-  if (w0 == w1) return;                  // finished by the CTA that had all of it
-  const int64_t step = int64_t(heads_per_chunk) * (a.D + 4);
+  if (w0 == w1) return;     // finished by the CTA that had all of it
+  const int64_t step = int64_t(heads_per_item) * (a.D + 4);
   // the first piece begins the item (slot 1 of its worker); the others begin inside it (slot 0)
-  auto piece = [&](int w) { return a.part + (2 * int64_t(w) + (w == w0 ? 1 : 0)) * step + h * (a.D + 4); };
-  const int words = a.D / 4;
-  float top = -INFINITY, sum = 0.f;
-  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  constexpr int kAhead = 4;
-  for (int w = w0 + warp; w <= w1; w += kWarps * kAhead) {
-    float2 st[kAhead];
-    float4 v[kAhead][2];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int wj = w + j * kWarps;
-      st[j] = make_float2(-INFINITY, 0.f);
-      if (wj > w1) continue;
-      const float* p = piece(wj);
-      st[j] = *reinterpret_cast<const float2*>(p + a.D);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane + 32 * i < words) v[j][i] = reinterpret_cast<const float4*>(p)[lane + 32 * i];
-    }
-    float next = top;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) next = fmaxf(next, st[j].x);
-    const float shift = next == -INFINITY ? 0.f : next, old = ex2(top - shift);
-    sum *= old;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) { acc[i].x *= old; acc[i].y *= old; acc[i].z *= old; acc[i].w *= old; }
-    top = next;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (w + j * kWarps > w1) continue;
-      const float f = ex2(st[j].x - shift);
-      sum = fmaf(f, st[j].y, sum);
+  auto piece_of = [&](int h) {
+    return [&, h](int w) { return a.part + (2 * int64_t(w) + (w == w0 ? 1 : 0)) * step + h * (a.D + 4); };
+  };
+  if constexpr (kByItem) {
+    for (int h = warp; h < heads; h += kWarps) {
+      const Joined r = join_pieces(w0, w1, 1, a.D, piece_of(h));
+      const float inv = 1.f / r.sum;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (lane + 32 * i >= words) continue;
-        acc[i].x = fmaf(f, v[j][i].x, acc[i].x); acc[i].y = fmaf(f, v[j][i].y, acc[i].y);
-        acc[i].z = fmaf(f, v[j][i].z, acc[i].z); acc[i].w = fmaf(f, v[j][i].w, acc[i].w);
+        T* to = out + h * a.D + (lane + 32 * i) * 4;
+        to[0] = from_f32<T>(r.acc[i].x * inv); to[1] = from_f32<T>(r.acc[i].y * inv);
+        to[2] = from_f32<T>(r.acc[i].z * inv); to[3] = from_f32<T>(r.acc[i].w * inv);
       }
     }
-  }
+  } else {
+    const Joined r = join_pieces(w0 + warp, w1, kWarps, a.D, piece_of(h0));
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 32 * i < words) outs[warp][lane + 32 * i] = acc[i];
-  if (lane == 0) {
-    sums[warp] = sum;
-    tops[warp] = top;
-  }
-  __syncthreads();
-  float most = -INFINITY;
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i < words) outs[warp][lane + 32 * i] = r.acc[i];
+    if (lane == 0) {
+      sums[warp] = r.sum;
+      tops[warp] = r.top;
+    }
+    __syncthreads();
+    float most = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) most = fmaxf(most, tops[i]);
-  const float shift = most == -INFINITY ? 0.f : most;
-  float f[kWarps], all = 0.f;
+    for (int i = 0; i < kWarps; ++i) most = fmaxf(most, tops[i]);
+    const float shift = most == -INFINITY ? 0.f : most;
+    float f[kWarps], all = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    f[i] = ex2(tops[i] - shift);
-    all = fmaf(f[i], sums[i], all);
-  }
-  for (int d = threadIdx.x; d < a.D; d += kThreads) {
-    float x = 0.f;
+    for (int i = 0; i < kWarps; ++i) {
+      f[i] = ex2(tops[i] - shift);
+      all = fmaf(f[i], sums[i], all);
+    }
+    for (int d = threadIdx.x; d < a.D; d += kThreads) {
+      float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) x = fmaf(f[i], reinterpret_cast<const float*>(outs[i])[d], x);
-    out[d] = from_f32<T>(x / all);
+      for (int i = 0; i < kWarps; ++i) x = fmaf(f[i], reinterpret_cast<const float*>(outs[i])[d], x);
+      out[d] = from_f32<T>(x / all);
+    }
   }
 }
 
@@ -577,6 +678,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct Plan {
   bool mma;
   int heads;       // query heads of a chunk
+  int side, chunks;
   int unit, workers;
   size_t bytes;
 };
@@ -606,44 +708,79 @@ Plan plan(const nb200_decode_params* p) {
   bool q_words = aligned16(p->q);
   for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
   pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words && p->scale > 0.f;
-  pl.heads = pl.mma && group > 8 ? 16 : 8;
-  pl.unit = 64;
-  const int ctas = pl.mma && pl.heads == 8 ? 4 : 2;      // resident per SM (the kernels' launch bounds)
+  int ctas;      // resident per SM (the kernels' launch bounds)
+  if (pl.mma) {
+    pl.heads = group > 8 ? 16 : 8;
+    ctas = pl.heads == 8 ? 4 : c.head_dim == 64 ? 3 : 2;
+  } else if (c.dtype == NB200_F32) {
+    pl.heads = group == 1 ? 1 : group == 2 ? 2 : group <= 4 ? 4 : 8;
+    ctas = c.head_dim <= 128 ? 4 : 2;
+  } else {
+    pl.heads = 8;
+    ctas = 2;
+  }
+  // A group of several chunks: warps side by side take them over the same tokens, which come from HBM once.
   const int chunks = (group + pl.heads - 1) / pl.heads;
-  const int64_t units = (int64_t(p->width) * c.page_size + pl.unit - 1) / pl.unit * p->rows * c.heads * chunks;
+  pl.side = chunks == 1 ? 1 : chunks == 2 ? 2 : 4;
+  pl.chunks = (chunks + pl.side - 1) / pl.side;
+  pl.unit = 64;
+  const int64_t units = (int64_t(p->width) * c.page_size + pl.unit - 1) / pl.unit * p->rows * c.heads * pl.chunks;
   const int64_t most = int64_t(tc::sm_count()) * ctas;
   pl.workers = int(units < most ? (units > 0 ? units : 1) : most);
-  pl.bytes = size_t(pl.workers) * 2 * pl.heads * (c.head_dim + 4) * sizeof(float);
+  pl.bytes = size_t(pl.workers) * 2 * pl.side * pl.heads * (c.head_dim + 4) * sizeof(float);
   return pl;
 }
 
-template <typename T, typename Loop>
-int launch(const DecodeArgs& a, cudaStream_t st) {
-  const size_t smem = size_t(Loop::kSlots) * Loop::kHeads * (a.D + 2) * sizeof(float);
-  decode_kernel<T, Loop><<<unsigned(a.workers), kThreads, smem, st>>>(a);
+template <typename T, typename Loop, int kSide>
+int launch_side(const DecodeArgs& a, cudaStream_t st) {
+  const size_t smem = size_t(kWarps) * Loop::kSlots * Loop::kHeads * (a.D + 2) * sizeof(float);
+  decode_kernel<T, Loop, kSide><<<unsigned(a.workers), kThreads, smem, st>>>(a);
   count_launch();
   if (int rc = check_launch("decode_kernel")) return rc;
-  if (launch_dependent(decode_join_kernel<T>, dim3(unsigned(a.q_heads), unsigned(a.rows)), kThreads, 0, st, a, int(Loop::kHeads)) != cudaSuccess)
+  const int items = a.kv_heads * a.chunks;      // of a row
+  const bool by_item = int64_t(items) * a.rows >= tc::sm_count();
+  if (launch_dependent(by_item ? decode_join_kernel<T, true> : decode_join_kernel<T, false>, dim3(unsigned(by_item ? items : a.q_heads), unsigned(a.rows)),
+                       kThreads, 0, st, a, kSide * Loop::kHeads) != cudaSuccess)
     return check_launch("decode_join_kernel");
   count_launch();
   return check_launch("decode_join_kernel");
 }
 
-template <typename T>
-int launch_fma(const DecodeArgs& a, cudaStream_t st) {
-  const int words = a.D / (16 / int(sizeof(T)));
-  if (words <= 8) return launch<T, FmaLoop<T, 8, 1>>(a, st);
-  if (words <= 16) return launch<T, FmaLoop<T, 16, 1>>(a, st);
-  if constexpr (sizeof(T) == 4) {
-    if (words > 32) return launch<T, FmaLoop<T, 32, 2>>(a, st);
+// (loops of few query heads take the whole of a group that small)
+template <typename T, typename Loop, bool kWholeGroup>
+int launch(const DecodeArgs& a, int side, cudaStream_t st) {
+  if constexpr (!kWholeGroup) {
+    if (side == 2) return launch_side<T, Loop, 2>(a, st);
+    if (side == 4) return launch_side<T, Loop, 4>(a, st);
   }
-  return launch<T, FmaLoop<T, 32, 1>>(a, st);      // (16-bit heads of 256 are 32 words)
+  return launch_side<T, Loop, 1>(a, st);
+}
+
+template <typename T, int kHeads>
+int launch_fma(const DecodeArgs& a, int side, cudaStream_t st) {
+  constexpr bool kWhole = kHeads < 8;
+  const int words = a.D / (16 / int(sizeof(T)));
+  if (words <= 8) return launch<T, FmaLoop<T, 8, 1, kHeads>, kWhole>(a, side, st);
+  if (words <= 16) return launch<T, FmaLoop<T, 16, 1, kHeads>, kWhole>(a, side, st);
+  if constexpr (sizeof(T) == 4) {
+    if (words > 32) return launch<T, FmaLoop<T, 32, 2, kHeads>, kWhole>(a, side, st);
+  }
+  return launch<T, FmaLoop<T, 32, 1, kHeads>, kWhole>(a, side, st);      // (16-bit heads of 256 are 32 words)
+}
+
+int launch_f32(const DecodeArgs& a, int heads, int side, cudaStream_t st) {
+  switch (heads) {
+    case 1: return launch_fma<float, 1>(a, side, st);
+    case 2: return launch_fma<float, 2>(a, side, st);
+    case 4: return launch_fma<float, 4>(a, side, st);
+    default: return launch_fma<float, 8>(a, side, st);
+  }
 }
 
 template <typename T, bool kBf16>
-int launch_mma(const DecodeArgs& a, int heads, cudaStream_t st) {
-  if (a.D == 64) return heads == 8 ? launch<T, MmaLoop<64, 1, kBf16>>(a, st) : launch<T, MmaLoop<64, 2, kBf16>>(a, st);
-  return heads == 8 ? launch<T, MmaLoop<128, 1, kBf16>>(a, st) : launch<T, MmaLoop<128, 2, kBf16>>(a, st);
+int launch_mma(const DecodeArgs& a, int heads, int side, cudaStream_t st) {
+  if (a.D == 64) return heads == 8 ? launch<T, MmaLoop<64, 1, kBf16>, true>(a, side, st) : launch<T, MmaLoop<64, 2, kBf16>, false>(a, side, st);
+  return heads == 8 ? launch<T, MmaLoop<128, 1, kBf16>, true>(a, side, st) : launch<T, MmaLoop<128, 2, kBf16>, false>(a, side, st);
 }
 
 }  // namespace
@@ -664,9 +801,15 @@ extern "C" NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_s
   const nb200_cache_pages& c = p->pages;
   if (!p->q || !p->out || !p->lengths || (p->width && !p->table) || (c.pages && (!c.k || !c.v))) { set_error("decode: NULL operand"); return NB200_ERR_INVALID; }
   const int vec = c.dtype == NB200_F32 ? 4 : 8;
-  bool ok = aligned16(c.k) && aligned16(c.v);
-  for (int i = 0; i < 3; ++i) ok = ok && c.k_stride[i] % vec == 0 && c.v_stride[i] % vec == 0;
+  bool ok = aligned16(c.k) && aligned16(c.v), near = true;
+  for (int i = 0; i < 3; ++i) {
+    for (const int64_t stride : {c.k_stride[i], c.v_stride[i]}) {
+      ok = ok && stride % vec == 0;
+      near = near && stride / vec <= 0x7fffffff && stride / vec >= -0x7fffffff;
+    }
+  }
   if (!ok) { set_error("decode: the rows of the pages must begin on 16-byte boundaries"); return NB200_ERR_ALIGNMENT; }
+  if (!near) { set_error("decode: a stride of the pages is 2^31 words of 16 bytes or more"); return NB200_ERR_UNSUPPORTED; }
   const Plan pl = plan(p);
   if (!p->workspace || p->workspace_bytes < pl.bytes) {
     set_error("decode: workspace of %zu bytes needed (nb200_decode_workspace_bytes), %zu given", pl.bytes, p->workspace_bytes);
@@ -674,8 +817,9 @@ extern "C" NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_s
   }
   if (!aligned16(p->workspace)) { set_error("decode: the workspace must begin on a 16-byte boundary"); return NB200_ERR_ALIGNMENT; }
   DecodeArgs a{};
-  a.k = c.k; a.v = c.v;
-  for (int i = 0; i < 3; ++i) { a.ks[i] = c.k_stride[i]; a.vs[i] = c.v_stride[i]; }
+  a.k = static_cast<const uint4*>(c.k);
+  a.v = static_cast<const uint4*>(c.v);
+  for (int i = 0; i < 3; ++i) { a.ks[i] = int(c.k_stride[i] / vec); a.vs[i] = int(c.v_stride[i] / vec); }
   a.pages = c.pages; a.kv_heads = c.heads; a.page_size = c.page_size; a.D = c.head_dim;
   a.page_shift = -1;
   for (int s = 0; s < 31; ++s)
@@ -685,14 +829,15 @@ extern "C" NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_s
   a.q = p->q; a.qs[0] = p->q_stride[0]; a.qs[1] = p->q_stride[1];
   a.out = p->out;
   a.q_heads = p->q_heads; a.group = p->q_heads / c.heads;
-  a.chunks = (a.group + pl.heads - 1) / pl.heads;
+  a.chunks = pl.chunks;
   a.mul = p->scale * kLog2e;
   a.unit = pl.unit;
   a.part = static_cast<float*>(p->workspace);
   a.workers = pl.workers;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  if (c.dtype == NB200_F32) return launch_fma<float>(a, st);
-  if (c.dtype == NB200_BF16) return pl.mma ? launch_mma<__nv_bfloat16, true>(a, pl.heads, st) : launch_fma<__nv_bfloat16>(a, st);
-  return pl.mma ? launch_mma<__half, false>(a, pl.heads, st) : launch_fma<__half>(a, st);
+  if (c.dtype == NB200_F32) return launch_f32(a, pl.heads, pl.side, st);
+  if (c.dtype == NB200_BF16)
+    return pl.mma ? launch_mma<__nv_bfloat16, true>(a, pl.heads, pl.side, st) : launch_fma<__nv_bfloat16, 8>(a, pl.side, st);
+  return pl.mma ? launch_mma<__half, false>(a, pl.heads, pl.side, st) : launch_fma<__half, 8>(a, pl.side, st);
 }
