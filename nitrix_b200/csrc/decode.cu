@@ -144,7 +144,8 @@ struct MmaLoop {
   static constexpr int kHeads = 8 * kTiles;      // query heads of a chunk
   static constexpr int kBlock = 16;              // tokens
   static constexpr int kSlots = 1;               // partial results of a warp
-  static constexpr int kMinCtas = kTiles == 1 ? 4 : D == 64 ? 3 : 2;
+  // (head dim 128, one tile: four CTAs per SM spill, 5280 GB/s of cache, three 5675; 64: four 5510, five 5616)
+  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : 3) : D == 64 ? 3 : 2;
   float o[kTiles][D / 16][4];                    // O^T: lane (g, t): head 2t (+1), see store
   float m[kTiles][2], l[kTiles][2];              // of heads 2t, 2t + 1; l: this lane's keys
 
@@ -302,7 +303,8 @@ struct FmaLoop {
   static constexpr int kVec = 16 / int(sizeof(T));
   static constexpr int kSlots = 32 / kLanes;
   static constexpr int kAhead = sizeof(T) == 4 && kPer == 1 ? 4 : 2;
-  static constexpr int kMinCtas = sizeof(T) == 4 && kPer == 1 ? 4 : 2;
+  // (eight heads: two, three, four, five CTAs per SM 2730, 3330, 3030, 2470 GB/s)
+  static constexpr int kMinCtas = sizeof(T) == 4 && kPer == 1 ? (kNumHeads == 8 ? 3 : 4) : 2;
   static constexpr int kSteps = kHeads == 8 ? 3 : kHeads == 4 ? 2 : kHeads == 2 ? 1 : 0;   // of the reduce-scatter
   float2 o[kHeads][kPer][kVec / 2];      // (pairs: two multiply-adds per instruction)
   float m, l;             // of the head that the reduce-scatter leaves in this lane
@@ -708,13 +710,13 @@ Plan plan(const nb200_decode_params* p) {
   bool q_words = aligned16(p->q);
   for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
   pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words && p->scale > 0.f;
-  int ctas;      // resident per SM (the kernels' launch bounds)
+  int ctas;      // resident per SM: the loops' kMinCtas
   if (pl.mma) {
     pl.heads = group > 8 ? 16 : 8;
-    ctas = pl.heads == 8 ? 4 : c.head_dim == 64 ? 3 : 2;
+    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 5 : 3) : c.head_dim == 64 ? 3 : 2;
   } else if (c.dtype == NB200_F32) {
     pl.heads = group == 1 ? 1 : group == 2 ? 2 : group <= 4 ? 4 : 8;
-    ctas = c.head_dim <= 128 ? 4 : 2;
+    ctas = c.head_dim <= 128 ? (pl.heads == 8 ? 3 : 4) : 2;
   } else {
     pl.heads = 8;
     ctas = 2;
