@@ -8,7 +8,9 @@
 //   dk, dv    a tile of kT keys walks over row tiles, dV += P^T dO, dK += dS^T Q
 // Bound by the fp32 units: 256 threads as 16 x 16, each with a (kT / 16)-square piece of the scores and kT / 16 rows of the
 // outputs in registers, operands in shared memory as fp32 with rows padded by four words (16-byte reads of 8 rows meet no bank
-// twice).  Tiles are 64 rows up to head dim 128, and 32 above, where four operands of 64 rows would not fit.
+// twice), two multiply-adds per instruction.  Tiles are 64 rows up to head dim 128, and 32 above, where four operands of 64 rows
+// would not fit.  fp32 rows of whole words are copied while the tile before is worked on.  f32, 2048 tokens, 16 heads on 4, head dim
+// 128, causal: forward 513 us (33 TFLOP/s), dq 726, dk and dv 1051; both directions 2.3 ms.
 #include <math.h>
 
 #include <type_traits>

@@ -13,6 +13,8 @@
 // head dim 128: 710 -> 682 us).  At head dim 64 the tile of dQ^T has 128 lanes as
 // well, of which the upper 64 (V in place of K: the tiles lie one after the other) are not read.
 //
+// P and dS are rounded to the operand type where they become operands (dS from the unrounded P); sums, lse and delta are fp32.
+//
 // What belongs to a neighbouring sequence must not get into a sum, not even as 0 * NaN: keys behind the end have P and dS
 // selected to zero and their rows of K cleared in shared memory, queries behind the end have P and dS selected to zero and
 // their rows of Q and dO cleared.  Warp 3, which forms the addends of every step before its products may run, does that.
@@ -51,10 +53,23 @@ struct BwdArgs {
   const float* delta;
   float* dq_acc;             // [key head][step][row / 4][d][row % 4]
   int64_t all_steps;         // steps that the accumulator has room for, per key head
+  const float* largest;      // fp16: the largest squared norms of a row of dout and of v
   void* dk;                  // dense (tokens_k, kv_heads, D)
   void* dv;
   int* status;
 };
+
+// fp16 has few exponents: with thousands of keys P and dS lie where it loses its digits.  P is taken times 2^10 (at most 1024), dS
+// times the power of two that its bound allows: |dS| <= |dout row| |v row| + |delta| <= 2 max |dout row| max |v row|, since a row of
+// out is a mean of rows of v.  Both factors leave with the results.  (Relative error of dq and dk over sequences of thousands of
+// tokens: 4.1e-4 without, 3.1e-4 with them; the rounding of dS and that of the results are 2.1e-4 each.)
+constexpr int kPShift = 10;
+__device__ __forceinline__ int ds_shift(const float* largest) {
+  const float bound = 2.f * sqrtf(largest[0]) * sqrtf(largest[1]);
+  if (!(bound < INFINITY)) return 0;
+  const float room = floorf(log2f(60000.f / fmaxf(bound, 1e-30f)));
+  return int(fminf(fmaxf(room, -14.f), 14.f));
+}
 
 template <int D>
 struct Smem {
@@ -305,7 +320,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const bool keyless = next[e][0] == -INFINITY;
-        c[e][0] = keyless ? 0.f : -next[e][0] * inv_mul;
+        c[e][0] = keyless ? 0.f : -(next[e][0] - (kBf16 ? 0.f : float(kPShift))) * inv_mul;
         c[e][1] = keyless ? 0.f : -next[e][1];
       }
       if (n + 1 < n_steps) fetch(n + 1);
@@ -372,6 +387,9 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     bool ok = true;
     const float mul = a.scale * kLog2e;
     const float2 mul2 = make_float2(mul, mul);
+    const int shift = kBf16 ? 0 : ds_shift(a.largest);
+    const float ds_mul = kBf16 ? 1.f : exp2f(float(shift - kPShift));      // (P is 2^10 times itself)
+    const float2 ds_mul2 = make_float2(ds_mul, ds_mul);
     const bool dropped = r >= it.n;
     const int first_query = it.seen + r;      // that sees this key, counted within the sequence (causal)
     // The ds tile (16 KB, 128-byte swizzle) is [128 keys x 64 rows]: a thread writes its own 128-byte row as eight 16-byte
@@ -477,7 +495,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         }
 #pragma unroll
         for (int c = 0; c < kStep / 2; ++c) {
-          const float2 ds = __fmul2_rn(t[c], make_float2(__uint_as_float(raw[2 * c]), __uint_as_float(raw[2 * c + 1])));
+          float2 ds = __fmul2_rn(t[c], make_float2(__uint_as_float(raw[2 * c]), __uint_as_float(raw[2 * c + 1])));
+          if constexpr (!kBf16) ds = __fmul2_rn(ds, ds_mul2);
           e2[c] = pack2<kBf16>(ds.x, ds.y);
         }
       }
@@ -507,7 +526,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     if (ok) {
       tc_fence_after_sync();
       const uint32_t tacc = (grp == 0 ? tm_dv : tm_dk) + lane_addr;
-      const float omul = grp == 0 ? 1.f : a.scale;
+      const float omul = kBf16 ? (grp == 0 ? 1.f : a.scale) : grp == 0 ? exp2f(-float(kPShift)) : a.scale * exp2f(-float(shift));
       uint8_t* orow = static_cast<uint8_t*>(grp == 0 ? a.dv : a.dk) + 2 * ((int64_t(it.begin) + r) * a.kv_heads + head) * D;
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -543,38 +562,56 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 }
 
 // delta[token][head] = sum_d out dout in fp32.  Bound by HBM: D / 8 lanes per row with 16 bytes of each tensor, four rows per
-// lane whose loads are in flight together.
+// lane whose loads are in flight together.  fp16: also the largest squared norm of a row of dout, and, by the CTAs behind
+// `delta_ctas`, of a row of v.
 constexpr int kDeltaThreads = 256, kDeltaRows = 4;
 
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const PackedArgs a, int delta_ctas, unsigned* largest) {
   constexpr int kLanes = D / 8, kGroups = kDeltaThreads / kLanes;
-  const int rows = a.tokens_q * a.heads;      // (below 2^31: checked on the host)
-  const int row0 = blockIdx.x * (kGroups * kDeltaRows) + int(threadIdx.x) / kLanes, c = threadIdx.x % kLanes;
+  const bool values = !kBf16 && int(blockIdx.x) >= delta_ctas;
+  const int heads = values ? a.kv_heads : a.heads, rows = values ? a.tokens_k * a.kv_heads : a.tokens_q * a.heads;      // (below 2^31: checked on the host)
+  const int row0 = (int(blockIdx.x) - (values ? delta_ctas : 0)) * (kGroups * kDeltaRows) + int(threadIdx.x) / kLanes, c = threadIdx.x % kLanes;
   uint4 o[kDeltaRows], g[kDeltaRows];
 #pragma unroll
   for (int i = 0; i < kDeltaRows; ++i) {
     const int row = row0 + i * kGroups;
     o[i] = g[i] = make_uint4(0, 0, 0, 0);
     if (row < rows) {
-      const int token = row / a.heads, head = row - token * a.heads;
-      o[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + int64_t(row) * D) + c);
-      g[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + token * a.dos[0] + head * a.dos[1]) + c);
+      const int token = row / heads, head = row - token * heads;
+      const int64_t at = values ? token * a.vs[0] + head * a.vs[1] : token * a.dos[0] + head * a.dos[1];
+      if (!values) o[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + int64_t(row) * D) + c);
+      g[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(values ? a.v : a.dout) + at) + c);
     }
   }
+  float norm = 0.f;
 #pragma unroll
   for (int i = 0; i < kDeltaRows; ++i) {
     const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-    float sum = 0.f;
+    float sum = 0.f, squares = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 x = unpack2<kBf16>(ow[j]), y = unpack2<kBf16>(gw[j]);
       sum = fmaf(x.x, y.x, fmaf(x.y, y.y, sum));
+      if constexpr (!kBf16) squares = fmaf(y.x, y.x, fmaf(y.y, y.y, squares));
     }
 #pragma unroll
-    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (int off = kLanes / 2; off > 0; off >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if constexpr (!kBf16) squares += __shfl_xor_sync(0xffffffffu, squares, off);
+    }
     const int row = row0 + i * kGroups;
-    if (row < rows && c == 0) a.delta[row] = sum;
+    if (!values && row < rows && c == 0) a.delta[row] = sum;
+    norm = squares <= norm ? norm : squares < INFINITY ? squares : INFINITY;      // (a NaN counts as infinite)
+  }
+  if constexpr (!kBf16) {
+    __shared__ unsigned most;
+    if (threadIdx.x == 0) most = 0;
+    __syncthreads();
+    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));      // (of numbers >= 0, in their order)
+    if ((threadIdx.x & 31) == 0) atomicMax(&most, bits);
+    __syncthreads();
+    if (threadIdx.x == 0 && most > *reinterpret_cast<volatile unsigned*>(largest + (values ? 1 : 0))) atomicMax(largest + (values ? 1 : 0), most);
   }
 }
 
@@ -582,7 +619,7 @@ __global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const Pa
 // 16-byte loads, four 16-byte stores).
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kStep / 4 * (D / 8)) packed_dq_finish_kernel(const PackedArgs a, const float* __restrict__ acc,
-                                                                                int64_t all_steps, int tokens) {
+                                                                                int64_t all_steps, int tokens, const float* largest) {
   const int head = blockIdx.y, dchunk = threadIdx.x % (D / 8), rg = threadIdx.x / (D / 8);
   const float* src = acc + (int64_t(head) * all_steps + blockIdx.x) * (kStep * D) + rg * (D * 4) + dchunk * 32;
   float4 v[8];      // in flight while the step's sequence is looked for
@@ -591,13 +628,14 @@ __global__ void __launch_bounds__(kStep / 4 * (D / 8)) packed_dq_finish_kernel(c
   const Place place = find_place(int(blockIdx.x), a.sequences, [&](int i) { return (sequence_span(a.offsets_q, i, a.tokens_q).y + tokens - 1) / tokens; });
   if (place.index < 0) return;
   const int2 q = sequence_span(a.offsets_q, place.sequence, a.tokens_q);
+  const float scale = kBf16 ? a.scale : a.scale * exp2f(-float(ds_shift(largest)));
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
     const int row = rg * 4 + rr, t = row / a.group, token = place.index * tokens + t;
     if (t >= tokens || token >= q.y) break;
     float x[8];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) x[d] = (rr == 0 ? v[d].x : rr == 1 ? v[d].y : rr == 2 ? v[d].z : v[d].w) * a.scale;
+    for (int d = 0; d < 8; ++d) x[d] = (rr == 0 ? v[d].x : rr == 1 ? v[d].y : rr == 2 ? v[d].z : v[d].w) * scale;
     uint4 w;
     w.x = pack2<kBf16>(x[0], x[1]);
     w.y = pack2<kBf16>(x[2], x[3]);
@@ -612,6 +650,7 @@ int64_t most_steps(const PackedArgs& a) { return most_blocks(a.tokens_q, a.seque
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 size_t delta_bytes(const PackedArgs& a) { return up256(size_t(a.tokens_q) * a.heads * sizeof(float)); }
 size_t list_bytes(const PackedArgs& a) { return work_list_bytes(most_blocks(a.tokens_k, a.sequences, kTile)); }
+constexpr size_t kLargestBytes = 256;      // in front of the sums, cleared with them
 size_t acc_bytes(const PackedArgs& a) { return size_t(a.kv_heads) * size_t(most_steps(a)) * kStep * a.D * sizeof(float); }
 
 template <int D, bool kBf16>
@@ -639,13 +678,15 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   char* base = static_cast<char*>(ws);
   p.delta = reinterpret_cast<float*>(base);
   void* list = base + delta_bytes(p);
-  float* acc = reinterpret_cast<float*>(base + delta_bytes(p) + list_bytes(p));
+  unsigned* largest = reinterpret_cast<unsigned*>(base + delta_bytes(p) + list_bytes(p));
+  float* acc = reinterpret_cast<float*>(base + delta_bytes(p) + list_bytes(p) + kLargestBytes);
   BwdArgs a{};
   a.tokens = tile_tokens(kStep, p.group);
   constexpr int kDeltaCta = kDeltaThreads / (D / 8) * kDeltaRows;      // rows
   const int64_t delta_grid = (int64_t(p.tokens_q) * p.heads + kDeltaCta - 1) / kDeltaCta;
-  if (cudaMemsetAsync(acc, 0, acc_bytes(p), st) != cudaSuccess) return check_launch("packed_bwd: clearing the sums of dq");
-  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid), kDeltaThreads, 0, st>>>(p);
+  const int64_t value_grid = kBf16 ? 0 : (int64_t(p.tokens_k) * p.kv_heads + kDeltaCta - 1) / kDeltaCta;
+  if (cudaMemsetAsync(largest, 0, kLargestBytes + acc_bytes(p), st) != cudaSuccess) return check_launch("packed_bwd: clearing the sums of dq");
+  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid + value_grid), kDeltaThreads, 0, st>>>(p, int(delta_grid), largest);
   count_launch();
   if (int rc = check_launch("packed_delta_tc_kernel")) return rc;
   if (int rc = launch_plan(p, true, kTile, a.tokens, list, st)) return rc;
@@ -665,6 +706,7 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   a.lse = p.lse;
   a.delta = p.delta;
   a.dq_acc = acc;
+  a.largest = reinterpret_cast<const float*>(largest);
   a.all_steps = most_steps(p);
   a.dk = p.dk;
   a.dv = p.dv;
@@ -674,14 +716,14 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   if (launch_dependent(kernel, unsigned(grid), kThreads, smem, st, tk, tv, tq, tdo, a) != cudaSuccess) return check_launch("packed_bwd_tc_kernel");
   count_launch();
   if (int rc = check_launch("packed_bwd_tc_kernel")) return rc;
-  packed_dq_finish_kernel<D, kBf16><<<dim3(unsigned(a.all_steps), unsigned(p.kv_heads)), kStep / 4 * (D / 8), 0, st>>>(p, acc, a.all_steps, a.tokens);
+  packed_dq_finish_kernel<D, kBf16><<<dim3(unsigned(a.all_steps), unsigned(p.kv_heads)), kStep / 4 * (D / 8), 0, st>>>(p, acc, a.all_steps, a.tokens, a.largest);
   count_launch();
   return check_launch("packed_dq_finish_kernel");
 }
 
 }  // namespace
 
-size_t tc_packed_bwd_bytes(const PackedArgs& a) { return delta_bytes(a) + list_bytes(a) + acc_bytes(a); }
+size_t tc_packed_bwd_bytes(const PackedArgs& a) { return delta_bytes(a) + list_bytes(a) + kLargestBytes + acc_bytes(a); }
 
 int tc_packed_bwd(const PackedArgs& p, int dtype, void* ws, cudaStream_t st) {
   const bool bf16 = dtype == NB200_BF16;

@@ -1,5 +1,5 @@
 // Forward attention over packed sequences for sm_100a: TMA -> shared memory -> tcgen05.mma with TMEM accumulators, fp32 online
-// softmax in registers; bf16 and fp16, head dim 64 and 128, any group of up to 128 query heads per key head.
+// softmax in registers; bf16 and fp16, head dim 64 and 128, any group of up to 64 query heads per key head.
 //
 //   S = Q K^T, P = exp2(S scale log2 e - m), O = P V / sum P,  query i of a sequence sees keys up to i + lk - lq (causal)
 //
@@ -15,7 +15,10 @@
 // MMAs of query tile 0 and 1; the others are the softmax, one thread per row at head dim 128, two at 64.  The scheme of the
 // tiles -- halves of 64 keys whose P overwrites S at head dim 128, separate P at 64, a reference maximum that moves only past
 // 2^8, every third pair of exponentials on the FMA units at head dim 128 -- is that of sdpa_tc_fwd.cu, which has the reasons.
-// Bound by the exponentials and the packing of P as that kernel is.
+// Head dim 128: bound by the tensor pipe with its operand fetch (busy 82 % of the time, 63 % of it multiplying: the MMAs of a half
+// read 6 KB of operands for 32 cycles of products) at the clock that the power cap leaves; 8192 tokens, 16 heads on 4, 469 us (1170
+// TFLOP/s), causal 232 (1180).  Key tiles taken whole, with N = 128 and the query tiles in turn, 606 -> 730 us.  Head dim 64: by the
+// exponentials, 398 and 207 us (690 and 660 TFLOP/s).
 // All waits on mbarriers are bounded (sdpa_tc_common.cuh).
 #include <type_traits>
 
@@ -622,7 +625,7 @@ bool strides_fit(const void* base, const int64_t (&s)[2], int tokens, int heads)
 // A group's heads of one token have to fit a tile (64 rows in the backward).
 bool tc_packed_supported(const PackedArgs& a, int dtype) {
   return dtype != NB200_F32 && (a.D == 64 || a.D == 128) && a.group <= 64 && a.scale > 0.f && a.scale < 1e30f &&
-         int64_t(a.tokens_q) * a.heads <= 0x7fffffff && a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
+         int64_t(a.tokens_q) * a.heads <= 0x7fffffff && int64_t(a.tokens_k) * a.kv_heads <= 0x7fffffff && a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
          strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads) && aligned16(a.out);
 }
 

@@ -174,6 +174,30 @@ def test_gradients_against_differences():
         assert abs(float((f(1) - f(-1)) / (2 * h) - (grads[i].double() * e.double()).sum())) < 2e-2
 
 
+def test_fp16_gradients_of_long_sequences():
+    """Thousands of keys: P and dS are small, where fp16 has fewer digits.  The roundings of dS and of the results are 2^-11 at
+    most, 2.1e-4 in the root mean square of values spread over a binade, and independent; a third one of that size stands for
+    delta's and P's: sqrt(3) * 2.1e-4 in the 2-norm."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [6000]
+    q, k, v, dout = _inputs(lengths, lengths, 2, 1, 64, torch.float16)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, _offsets(lengths)), leaves, dout)
+    want = O.packed(q, k, v, lengths, lengths, 0.125, True, dout)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        value = want[name][0]
+        assert float((got.double() - value).norm() / value.norm()) < 3.7e-4, name
+
+
+def test_fp16_gradients_whose_products_leave_fp16():
+    """dout and v so large that dS itself would overflow; the gradients do not."""
+    lengths = [300, 40]
+    q, k, v, dout = _inputs(lengths, lengths, 4, 2, 128, torch.float16)
+    _check(q * 0.01, k * 0.01, v * 30, dout * 1000, lengths, lengths)
+    _check(q * 0.01, k * 0.01, v * 0, dout * 0, lengths, lengths)
+
+
 def test_families_and_reproducibility(monkeypatch):
     import nitrix_b200
     from nitrix_b200.backend import NitrixBackendError, NitrixBackendFallback, reset_fallback_state
