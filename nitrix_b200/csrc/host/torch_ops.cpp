@@ -7,6 +7,8 @@
 // Nothing is kept between calls: every call asks the library for its plan and its scratch anew (about a microsecond).
 //
 // The library is the one ctypes has loaded: bind() receives the addresses of its entry points.
+#include <limits>
+
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -560,10 +562,15 @@ void check_float(const char* what, const char* name, const Tensor& t) {
   TORCH_CHECK_TYPE(t.is_cuda() && dtype_code(t.scalar_type()) >= 0, what, ": ", name, " must be a CUDA tensor of float32, bfloat16 or float16; got ",
                    t.scalar_type(), " on ", t.device());
 }
+// extents that the library takes as 32-bit numbers
+void check_extents(const char* what, const Tensor& t) {
+  for (int64_t n : t.sizes()) TORCH_CHECK_VALUE(n <= std::numeric_limits<int32_t>::max(), what, ": an axis of ", n, " elements does not fit 32 bits");
+}
 void check_ints(const char* what, const char* name, const Tensor& t, const Tensor& like, int64_t dims) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt && t.device() == like.device(), what, ": ", name, " must be int32 on ", like.device(), "; got ",
                    t.scalar_type(), " on ", t.device());
   TORCH_CHECK_VALUE(t.dim() == dims, what, ": ", name, " must have ", dims, " axes; got shape ", t.sizes());
+  check_extents(what, t);
 }
 // rows along the last axis that begin on 16-byte boundaries, none of them shared
 Tensor aligned_rows(const Tensor& t) {
@@ -599,8 +606,9 @@ tensor_list rotate(const Tensor& q, const Tensor& k, const Tensor& positions, co
   for (int i = 0; i < 2; ++i) {
     const Tensor& x = i ? k : q;
     if (!x.defined()) continue;
-    out[i] = at::empty(x.sizes(), x.options());
     held[i] = two_leading_axes(x);
+    check_extents("rotary_embedding", held[i]);
+    out[i] = at::empty(x.sizes(), x.options());
     rotary_operand(i ? p.k : p.q, held[i], out[i]);
     p.batch = int32_t(held[i].size(0));
     p.length = int32_t(held[i].size(1));
@@ -649,6 +657,7 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
   const char* what = "rotary_embedding";
   check_float(what, "q", q);
   TORCH_CHECK_VALUE(q.dim() >= 3, what, ": q must be (..., heads, head_dim); got shape ", q.sizes());
+  check_extents(what, q);
   const c10::cuda::CUDAGuard guard(q.device());
   if (sections.empty()) sections.push_back(frequencies.numel());
   TORCH_CHECK_VALUE(sections.size() <= NB200_ROTARY_MAX_AXES, what, ": at most ", NB200_ROTARY_MAX_AXES, " axes; got ", sections.size());
@@ -687,10 +696,11 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
 
 // ---- paged cache --------------------------------------------------------------------------------------------------------------
 nb200_cache_pages cache_pages(const char* what, const Tensor& k_pages, const Tensor& v_pages) {
-  check_float(what, "k_pages", k_pages);
   TORCH_CHECK_TYPE(v_pages.scalar_type() == k_pages.scalar_type() && v_pages.device() == k_pages.device(), what, ": v_pages must be like k_pages");
   TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), what,
                     ": k_pages and v_pages must have one shape (pages, heads, page size, head dim); got ", k_pages.sizes(), " and ", v_pages.sizes());
+  TORCH_CHECK_VALUE(k_pages.size(1) > 0 && k_pages.size(2) > 0 && k_pages.size(3) > 0, what, ": a page must hold a token at least; got shape ", k_pages.sizes());
+  check_extents(what, k_pages);
   nb200_cache_pages c{};
   const Tensor* t[2] = {&k_pages, &v_pages};
   for (int i = 0; i < 2; ++i) {
@@ -751,6 +761,7 @@ std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Ten
                                                 const Tensor& free_pages, const Tensor& free_range, const Tensor& k, const Tensor& v,
                                                 const Tensor& offsets) {
   const char* what = "cache_append";
+  check_float(what, "k_pages", k_pages);
   const c10::cuda::CUDAGuard guard(k_pages.device());
   CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
   for (const Tensor* t : {&k, &v}) {
@@ -779,6 +790,7 @@ std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Ten
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
                                                               const Tensor& free_pages, const Tensor& free_range, const Tensor& rows, bool finished) {
   const char* what = finished ? "cache_free" : "cache_fork";
+  check_float(what, "k_pages", k_pages);
   const c10::cuda::CUDAGuard guard(k_pages.device());
   CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
   const Tensor r = rows.contiguous();
@@ -807,6 +819,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pa
 // (table, free_pages, free_range, shortfall)
 std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
                                                          const Tensor& free_pages, const Tensor& free_range) {
+  check_float("cache_compact", "k_pages", k_pages);
   const c10::cuda::CUDAGuard guard(k_pages.device());
   CacheCall c("cache_compact", k_pages, v_pages, table, lengths, free_pages, free_range);
   const Tensor new_table = at::empty(table.sizes(), table.options()), new_free = c.ints(k_pages.size(0)), new_range = c.ints(2),
@@ -822,6 +835,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, 
 
 Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, double scale) {
   const char* what = "decode_attention";
+  check_float(what, "k_pages", k_pages);
   const c10::cuda::CUDAGuard guard(k_pages.device());
   nb200_decode_params p{};
   p.struct_size = sizeof(p);
@@ -829,6 +843,7 @@ Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
   TORCH_CHECK_TYPE(q.scalar_type() == k_pages.scalar_type() && q.device() == k_pages.device(), what, ": q must be ", k_pages.scalar_type(), " on ", k_pages.device());
   TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == table.size(0) && q.size(2) == k_pages.size(3) && q.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, what,
                     ": q must be (", table.size(0), ", a multiple of ", k_pages.size(1), ", ", k_pages.size(3), "); got ", q.sizes());
+  check_extents(what, q);
   check_ints(what, "table", table, k_pages, 2);
   check_ints(what, "lengths", lengths, k_pages, 1);
   TORCH_CHECK_VALUE(lengths.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths.sizes());
@@ -950,6 +965,8 @@ MaybeTensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, 
   TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(2) == k.size(2), what,
                     ": q must be (tokens, heads, head dim), k and v (tokens, key heads, head dim); got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
   TORCH_CHECK_VALUE(q.size(1) > 0 && k.size(1) > 0 && q.size(1) % k.size(1) == 0, what, ": ", q.size(1), " query heads are no multiple of ", k.size(1), " key heads");
+  check_extents(what, q);
+  check_extents(what, k);
   check_ints(what, "offsets", offsets, q, 1);
   TORCH_CHECK_VALUE(offsets.size(0) >= 1, what, ": offsets must hold the number of sequences + 1 elements");
   if (offsets_k) {

@@ -402,3 +402,23 @@ def test_refusals():
         wide = paged_cache(2, 4, 1, 264, sequences=1, max_length=4)
         decode_attention(torch.zeros(1, 1, 264, device="cuda", dtype=torch.bfloat16), wide)
     assert cache_fork(cache, torch.zeros(0, dtype=torch.int32, device="cuda")).lengths.shape == (0,)
+
+
+def test_refusals_of_pages():
+    """Pools that no kernel may see: on the host, pages without a head or a slot."""
+    from nitrix_b200.nn import PagedCache, cache_append, cache_compact, cache_fork, decode_attention, paged_cache
+
+    cache = paged_cache(8, 4, 2, 64, sequences=3, max_length=16)
+    k = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    offsets = torch.arange(4, device="cuda").int()
+    q = torch.zeros(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    calls = [lambda c, k=k: cache_append(c, k, k, offsets), lambda c: cache_fork(c, offsets[:3]), cache_compact,
+             lambda c: decode_attention(q, c)]
+    host = PagedCache(*(t.cpu() for t in cache))
+    for call in calls:
+        with pytest.raises(TypeError, match="CUDA tensor"):
+            call(host)
+    for empty in (cache.k_pages[:, :0], cache.k_pages[:, :, :0]):
+        for call in (lambda c: cache_append(c, k[:, :empty.shape[1]], k[:, :empty.shape[1]], offsets), *calls[1:]):
+            with pytest.raises(ValueError, match="a token at least"):
+                call(cache._replace(k_pages=empty, v_pages=empty))

@@ -299,3 +299,12 @@ def test_refusals():
     empty = packed_attention(q[:0], k[:0], v[:0], _offsets([0, 0]))
     assert empty.shape == (0, 4, 64)
     assert not bool(packed_attention(q, k, v, _offsets([]), backend="cuda-simt").any())
+
+
+def test_more_tokens_than_32_bits_count():
+    from nitrix_b200.nn import packed_attention
+
+    q = torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    many = q.expand(2 ** 32 + 1, 1, 64)
+    with pytest.raises(ValueError, match="32 bits"):
+        packed_attention(many, many, many, _offsets([1]))

@@ -163,3 +163,12 @@ def test_refusals():
         rotary_embedding(wide, None, pos, freq)
     with pytest.raises(ValueError):
         rotary_frequencies(())
+
+
+def test_more_tokens_than_32_bits_count():
+    from nitrix_b200.nn import rotary_embedding
+
+    q = torch.zeros(1, 1, 8, device="cuda", dtype=torch.bfloat16).expand(2 ** 32 + 1, 1, 8)
+    positions = torch.zeros(1, dtype=torch.int32, device="cuda").expand(2 ** 32 + 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        rotary_embedding(q, None, positions, torch.ones(4, device="cuda"))
