@@ -41,7 +41,13 @@ bool tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
   return pass == NB200_PASS_FWD ? tc_packed_supported(a, p->dtype) : tc_packed_bwd_supported(a, p->dtype);
 }
 
+// fp32 forwards on the tensor cores
+bool fp32_tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
+  return p->kernel == NB200_KERNEL_AUTO && pass == NB200_PASS_FWD && fp32_packed_supported(a, p->dtype);
+}
+
 size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
+  if (fp32_tensor_cores(p, a, pass)) return fp32_packed_fwd_bytes(a);
   if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a);
   return pass == NB200_PASS_FWD ? 0 : delta_bytes(p) + simt_packed_bwd_bytes(a);
 }
@@ -74,7 +80,8 @@ using namespace nb200::packed;
 extern "C" NB200_API int nb200_packed_plan(const nb200_packed_params* p, int pass, int* kernel) {
   if (int rc = check(p, "packed_plan")) return rc;
   if (!kernel || (pass != NB200_PASS_FWD && pass != NB200_PASS_BWD)) { set_error("packed_plan: NULL result or bad pass"); return NB200_ERR_INVALID; }
-  *kernel = tensor_cores(p, lower(p), pass) ? NB200_KERNEL_TCGEN05 : NB200_KERNEL_SIMT;
+  const PackedArgs a = lower(p);
+  *kernel = tensor_cores(p, a, pass) || fp32_tensor_cores(p, a, pass) ? NB200_KERNEL_TCGEN05 : NB200_KERNEL_SIMT;
   return NB200_OK;
 }
 
@@ -94,6 +101,7 @@ extern "C" NB200_API int nb200_packed_fwd(const nb200_packed_params* p, void* cu
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   if (tensor_cores(p, a, NB200_PASS_FWD)) return tc_packed_fwd(a, p->dtype, p->workspace, st);
+  if (fp32_tensor_cores(p, a, NB200_PASS_FWD)) return fp32_packed_fwd(a, p->workspace, st);
   if (int rc = launch_clear_uncovered(a, p->dtype, false, st)) return rc;
   if (p->sequences == 0) return NB200_OK;
   return simt_packed_fwd(a, p->dtype, st);

@@ -24,6 +24,7 @@ constexpr int kGroupItems = 148;       // (block, key head) pairs that a group h
 struct PlanArgs {
   PackedArgs a;
   int backward;
+  int halves;            // of an element of the outputs, 16 bits each
   int block, step_tokens;
   int shift;             // lengths in tiles are counted in units of 2^shift
   int kv_heads;
@@ -104,6 +105,7 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, const uint8_t*
       w.other_n = other.y;
       w.steps = int(steps_before);
       w.index = b;
+      w.sequence = s;
       int length;        // tokens of the other side
       if (p.backward) {
         w.seen = first - shift;
@@ -126,13 +128,13 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
   allow_dependents();
   const PackedArgs& a = p.a;
   if (blockIdx.x > 0) {
-    const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D;
+    const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D * p.halves;
     uint16_t* out = static_cast<uint16_t*>(p.backward ? a.dq : a.out);
-    clear_tail<uint16_t>(out, q0 * row, a.tokens_q * row, 0);      // (16-bit operands: zero has no bits)
+    clear_tail<uint16_t>(out, q0 * row, a.tokens_q * row, 0);      // (a zero has no bits)
     if (!p.backward) {
       clear_tail<float>(a.lse, q0 * a.heads, int64_t(a.tokens_q) * a.heads, -INFINITY);
     } else {
-      const int64_t k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k), krow = int64_t(a.kv_heads) * a.D;
+      const int64_t k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k), krow = int64_t(a.kv_heads) * a.D * p.halves;
       clear_tail<uint16_t>(static_cast<uint16_t*>(a.dk), k0 * krow, a.tokens_k * krow, 0);
       clear_tail<uint16_t>(static_cast<uint16_t*>(a.dv), k0 * krow, a.tokens_k * krow, 0);
     }
@@ -172,16 +174,17 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
     if (place >= p.most) return;
     int4* dst = reinterpret_cast<int4*>(p.items + place);
     dst[0] = make_int4(w.begin, w.n, w.other, w.other_n);
-    dst[1] = make_int4(w.seen, w.steps, w.index, 0);
+    dst[1] = make_int4(w.seen, w.steps, w.index, w.sequence);
   });
 }
 
 }  // namespace
 
-int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st) {
+int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st, int element) {
   PlanArgs p{};
   p.a = a;
   p.backward = backward;
+  p.halves = element / 2;
   p.block = block;
   p.kv_heads = a.kv_heads;
   p.grouped = a.sequences > 1 && a.sequences <= kPlanThreads && most_blocks(backward ? a.tokens_k : a.tokens_q, a.sequences, block) * a.kv_heads > kGroupItems;

@@ -19,7 +19,7 @@ struct __align__(16) WorkItem {
   int seen;         // see above
   int steps;        // backward: first 64-row step of the sequence's rows in the gradient sums of dq
   int index;        // number of the block in its sequence
-  int pad;
+  int sequence;
 };
 static_assert(sizeof(WorkItem) == 32, "two 16-byte loads");
 
@@ -35,8 +35,9 @@ inline size_t work_list_bytes(int64_t most) { return (16 + size_t(most) * sizeof
 inline int64_t most_blocks(int64_t tokens, int sequences, int block) { return tokens / block + sequences; }
 
 // Fills the list (and clears the outputs of tokens that no sequence covers, which would be a launch of its own).
+// `element`: bytes of an element of the outputs.
 // `block`: queries (forward) or keys (backward) of a block; `step_tokens` (backward): queries of a 64-row step.
-int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st);
+int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st, int element = 2);
 
 // Rows of a query tile are, token after token, the query heads of one key head: this many tokens fit.
 __host__ __device__ inline int tile_tokens(int rows, int group) { return rows / group; }
@@ -48,11 +49,16 @@ bool tc_packed_bwd_supported(const PackedArgs& a, int dtype);
 size_t tc_packed_bwd_bytes(const PackedArgs& a);
 int tc_packed_bwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
 
+// fp32 operands as three bf16 planes (packed_fp32_tc.cu): forward
+bool fp32_packed_supported(const PackedArgs& a, int dtype);
+size_t fp32_packed_fwd_bytes(const PackedArgs& a);
+int fp32_packed_fwd(const PackedArgs& a, void* ws, cudaStream_t st);
+
 #ifdef __CUDACC__
 __device__ __forceinline__ WorkItem load_item(const WorkItem* p) {
   const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
   WorkItem w;
-  w.begin = a.x; w.n = a.y; w.other = a.z; w.other_n = a.w; w.seen = b.x; w.steps = b.y; w.index = b.z;
+  w.begin = a.x; w.n = a.y; w.other = a.z; w.other_n = a.w; w.seen = b.x; w.steps = b.y; w.index = b.z; w.sequence = b.w;
   return w;
 }
 #endif

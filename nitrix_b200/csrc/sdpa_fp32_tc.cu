@@ -14,6 +14,7 @@
 // them with plain bulk copies, whatever the strides and the length of the operand were: rows past the end are zeros.
 #include <math.h>
 
+#include "fp32_planes.cuh"
 #include "sdpa_tc_common.cuh"
 
 namespace nb200 {
@@ -36,23 +37,6 @@ struct SplitArgs {
   SplitOperand op[4];
   int H, bh_begin, D;
 };
-
-// eight fp32 as three words of eight bf16 each (see the file's comment)
-__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&w)[3]) {
-  uint32_t r[8], o[4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[i]);
-#pragma unroll
-  for (int p = 0; p < 3; ++p) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __byte_perm(r[2 * i], r[2 * i + 1], 0x7632);
-    w[p] = make_uint4(o[0], o[1], o[2], o[3]);
-    if (p < 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) - __uint_as_float(r[i] & 0xffff0000u));
-    }
-  }
-}
 
 // Grid (tiles, bh, operands); kCols = the head dim padded to whole 64-column chunks.  Bound by memory traffic (4 bytes in,
 // 6 out per element).
@@ -98,11 +82,6 @@ struct FwdArgs {
   int bias_dtype;
   int* status;
 };
-
-// the six products, small ones first: (plane of the left operand, plane of the right one)
-constexpr int kProducts = 6;
-__device__ __forceinline__ constexpr int left_plane(int i) { return i == 0 ? 2 : (i == 1 ? 0 : (i == 2 ? 1 : (i == 3 ? 1 : 0))); }
-__device__ __forceinline__ constexpr int right_plane(int i) { return i == 0 ? 0 : (i == 1 ? 2 : (i == 2 ? 1 : (i == 3 ? 0 : (i == 4 ? 1 : 0)))); }
 
 // the addend of a key that the mask drops: a NaN that no arithmetic produces (an -inf bias is a value like any other)
 constexpr uint32_t kDropped = 0x7fc0deadu;

@@ -23,8 +23,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     keys, each one before it one less.  A query that sees no key gives zeros and has no gradient; so do tokens behind the last
     offset.  Differentiable in ``q``, ``k`` and ``v``.
 
-    bf16 and fp16 with head dim 64 or 128 run on the tensor cores; what they do not take runs on the fp32 units, with one
-    ``NitrixBackendFallback`` warning.  That family sums everything in a fixed order and is what reproducibility mode uses.
+    bf16 and fp16 with head dim 64 or 128 run on the tensor cores, as does the forward pass of fp32 operands of 128 keys per
+    sequence or more on average (three bf16 numbers each, good to 2^-20 of a product; an infinity makes its rows NaN); what
+    they do not take runs on the fp32 units, with one ``NitrixBackendFallback`` warning.  That family sums everything in a
+    fixed order and is what reproducibility mode uses.
     """
     resolved = resolve_backend(backend)
     kernel = _cabi.KERNEL_SIMT if resolved == "cuda-simt" else _cabi.KERNEL_AUTO
@@ -32,8 +34,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     out = _cabi.torch_ops().packed_attention(q, k, v, offsets, offsets_k, factor, bool(causal), kernel, False)
     if out is None:
         fallback(function="packed_attention", requested=resolved, resolved="cuda-simt",
-                 reason="the fused tcgen05 kernels take bf16/fp16 with head dim 64 or 128, up to 64 query heads per key head "
-                        "and a positive scale",
+                 reason="the fused tcgen05 kernels take head dim 64 or 128: bf16/fp16 with up to 64 query heads per key head and a "
+                        "positive scale, fp32 with up to 128 and 128 keys per sequence on average",
                  shapes=(tuple(q.shape), tuple(k.shape)), dtype=q.dtype)
         out = _cabi.torch_ops().packed_attention(q, k, v, offsets, offsets_k, factor, bool(causal), kernel, True)
     return out

@@ -308,3 +308,79 @@ def test_more_tokens_than_32_bits_count():
     many = q.expand(2 ** 32 + 1, 1, 64)
     with pytest.raises(ValueError, match="32 bits"):
         packed_attention(many, many, many, _offsets([1]))
+
+
+LONG = {
+    "one": [300],
+    "edges": [128, 127, 129, 256],
+    "empty and short ones": [0, 700, 1, 64, 65, 0, 500],
+    "two tiles and a row": [257, 130],
+}
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hk,G", [(1, 1), (2, 3), (1, 4), (1, 16), (1, 128), (3, 1)])
+@pytest.mark.parametrize("name", LONG)
+def test_fp32_on_the_tensor_cores(D, Hk, G, name):
+    """Three bf16 numbers per operand: what is left out of a product is below 2^-20 of it, and the accumulators, emptied every
+    other step, truncate 48 times by 2^-24: 4e-6 of the sums of either product, within the 1e-5 of fp32."""
+    from nitrix_b200 import _cabi
+
+    lengths = LONG[name]
+    before = _cabi.lib().nb200_launch_count()
+    _check(*_inputs(lengths, lengths, Hk * G, Hk, D, torch.float32, seed=D + G), lengths, lengths)
+    assert _cabi.lib().nb200_launch_count() > before
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths_q,lengths_k", [
+    ([5, 100, 64], [300, 500, 0]), ([200, 1, 33], [137, 129, 256]), ([400, 300], [300, 5]), ([1, 90], [777, 64]), ([64], [4000])])
+def test_fp32_keys_of_other_lengths(D, causal, lengths_q, lengths_k):
+    out, grads = _check(*_inputs(lengths_q, lengths_k, 8, 2, D, torch.float32), lengths_q, lengths_k, causal)
+    at = 0
+    for lq, lk in zip(lengths_q, lengths_k):
+        blind = lq if lk == 0 else (max(lq - lk, 0) if causal else 0)
+        assert not bool(out[at:at + blind].any()) and not bool(grads[0][at:at + blind].any())
+        at += lq
+
+
+def test_fp32_more_blocks_than_a_wave_and_strides():
+    """Two query tiles per CTA; views of one projection, operands that are not 16-byte aligned, tokens behind the last offset."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [1000, 30, 900, 0, 300, 129]
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = sum(lengths)
+    qkv = torch.randn(n, 24, 64, generator=g, device="cuda")
+    q, k, v = qkv[:, :16], qkv[:, 16:20], qkv[:, 20:]
+    dout = torch.randn(n, 16, 64, generator=g, device="cuda")
+    _check(q, k, v, dout, lengths, lengths)
+    _check(q, k, v, dout, lengths, lengths, scale=-0.2)
+    odd = torch.randn(n * 16 * 64 + 1, generator=g, device="cuda")[1:].view(n, 16, 64)
+    _check(odd, k, v, dout, lengths, lengths, causal=False)
+    with torch.no_grad():
+        more = [torch.cat([t, torch.full((700, *t.shape[1:]), float("nan"), device="cuda")]) for t in (q, k, v)]
+        out = packed_attention(*more, _offsets(lengths))
+        assert torch.equal(out[:n], packed_attention(q, k, v, _offsets(lengths)))
+        assert not bool(out[n:].any())
+
+
+def test_fp32_neighbours_and_magnitudes():
+    """NaN and infinities of a neighbour stay there; operands of 1e-18 and 1e18 keep their digits."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [200, 131, 300, 77]
+    q, k, v, dout = _inputs(lengths, lengths, 4, 2, 128, torch.float32)
+    off = _offsets(lengths)
+    with torch.no_grad():
+        want = packed_attention(q, k, v, off)
+        for bad in (float("nan"), float("inf")):
+            dirty = [t.clone() for t in (q, k, v)]
+            for t in dirty:
+                t[200:331] = bad
+                t[631:] = bad
+            got = packed_attention(*dirty, off)
+            assert torch.equal(got[:200], want[:200]) and torch.equal(got[331:631], want[331:631])
+        big = packed_attention(q * 2.0 ** 60, k * 2.0 ** -60, v * 2.0 ** -60, off)
+        assert torch.equal(big, want * 2.0 ** -60)
