@@ -41,13 +41,14 @@ bool tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
   return pass == NB200_PASS_FWD ? tc_packed_supported(a, p->dtype) : tc_packed_bwd_supported(a, p->dtype);
 }
 
-// fp32 forwards on the tensor cores
+// fp32 on the tensor cores
 bool fp32_tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pass) {
-  return p->kernel == NB200_KERNEL_AUTO && pass == NB200_PASS_FWD && fp32_packed_supported(a, p->dtype);
+  if (p->kernel != NB200_KERNEL_AUTO) return false;
+  return pass == NB200_PASS_FWD ? fp32_packed_supported(a, p->dtype) : fp32_packed_bwd_supported(a, p->dtype);
 }
 
 size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
-  if (fp32_tensor_cores(p, a, pass)) return fp32_packed_fwd_bytes(a);
+  if (fp32_tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? fp32_packed_fwd_bytes(a) : delta_bytes(p) + fp32_packed_bwd_bytes(a);
   if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a);
   return pass == NB200_PASS_FWD ? 0 : delta_bytes(p) + simt_packed_bwd_bytes(a);
 }
@@ -117,6 +118,10 @@ extern "C" NB200_API int nb200_packed_bwd(const nb200_packed_params* p, void* cu
   prof_call_begin(st);
   if (tensor_cores(p, a, NB200_PASS_BWD)) return tc_packed_bwd(a, p->dtype, p->workspace, st);
   a.delta = static_cast<float*>(p->workspace);
+  if (fp32_tensor_cores(p, a, NB200_PASS_BWD)) {
+    if (int rc = launch_packed_delta(a, p->dtype, st)) return rc;
+    return fp32_packed_bwd(a, static_cast<char*>(p->workspace) + delta_bytes(p), st);
+  }
   a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + delta_bytes(p));
   if (int rc = launch_clear_uncovered(a, p->dtype, true, st)) return rc;
   if (p->sequences == 0) return NB200_OK;

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
   allow_dependents();
   const PackedArgs& a = p.a;
   if (blockIdx.x > 0) {
+    if (p.halves == 0) return;
     const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D * p.halves;
     uint16_t* out = static_cast<uint16_t*>(p.backward ? a.dq : a.out);
     clear_tail<uint16_t>(out, q0 * row, a.tokens_q * row, 0);      // (a zero has no bits)
