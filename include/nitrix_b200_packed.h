@@ -54,7 +54,7 @@ NB200_API int nb200_packed_fwd(const nb200_packed_params* p, void* cuda_stream);
 NB200_API int nb200_packed_bwd(const nb200_packed_params* p, void* cuda_stream);
 /* pass: nb200_pass */
 NB200_API int nb200_packed_workspace_bytes(const nb200_packed_params* p, int pass, size_t* bytes);
-/* The family that runs the pass: NB200_KERNEL_TCGEN05 (fp32 forwards among them, as three bf16 planes) or NB200_KERNEL_SIMT. */
+/* The family that runs the pass: NB200_KERNEL_TCGEN05 (fp32 as three bf16 planes among it) or NB200_KERNEL_SIMT. */
 NB200_API int nb200_packed_plan(const nb200_packed_params* p, int pass, int* kernel);
 
 #ifdef __cplusplus

@@ -1,18 +1,22 @@
-// Forward attention over packed sequences with fp32 operands on the tcgen05 tensor cores: every fp32 number is three bf16
-// numbers and every product the six bf16 products that matter (sdpa_fp32_tc.cu has the error bounds and the scheme of a tile).
+// Attention over packed sequences with fp32 operands on the tcgen05 tensor cores, forward at head dim 64 and 128, backward at
+// head dim 64 (at 128 the planes of an owner's two operands alone are 192 KB of shared memory): every fp32 number is three
+// bf16 numbers and every product the six bf16 products that matter (sdpa_fp32_tc.cu has the error bounds and the scheme of a
+// tile).
 //
-// packed_planes_kernel writes the planes of q, k and v into the workspace as the tiles that the MMAs read, a sequence and key
-// head at a time: 128 rows of queries (token after token, the query heads of the key head), 64 keys.  Rows behind the end of
-// a sequence are zeros there, so nothing of a neighbouring sequence gets near a sum.  The tiles of sequence i begin at tile
-// begin / tokens per tile + i: sequences that follow one another never share one, and nobody has to add up the lengths.
-// packed_fwd_fp32_kernel then fetches whole tiles by untiled bulk copies; its blocks come from the list of packed_plan.cu.
+// packed_planes_kernel writes the planes of q, k, v and dout into the workspace as the tiles that the MMAs read, a sequence and
+// key head at a time: 128 rows of queries, or 64 (token after token, the query heads of the key head), 64 keys.  Rows behind
+// the end of a sequence are zeros there, so nothing of a neighbouring sequence gets near a sum.  The tiles of sequence i begin
+// at tile begin / tokens per tile + i: sequences that follow one another never share one, and nobody has to add up the lengths.
+// The other kernels fetch whole tiles by untiled bulk copies; their blocks come from the lists of packed_plan.cu.
 //
 // An infinity in a sequence's own operands becomes a NaN in its planes (x - x0), so that its scores are NaN where the fp32
 // units may still give a number.
 //
-// Where these kernels run and where the fp32 units do: the rule and both sides are beside fp32_packed_supported.  Bound by the
-// chain of a step (scores, soft-max, P V of a tile follow one another; two tiles per CTA at head dim 64, one at 128, where the
-// planes of one fill the shared memory): 84 % and 64 % of the 275 TFLOP/s that six products at the bf16 rate leave, long sequences.
+// Where these kernels run and where the fp32 units do: the rules and both sides are beside fp32_packed_supported and
+// fp32_packed_bwd_supported.  Forward: bound by the chain of a step (scores, soft-max, P V of a tile follow one another; two
+// tiles per CTA at head dim 64, one at 128, where the planes of one fill the shared memory): 84 % and 64 % of the 275 TFLOP/s
+// that six products at the bf16 rate leave, long sequences.  Backward: one step of a CTA at a time, 1.5 us each by keys, 45 % of
+// that rate.
 #include <math.h>
 
 #include "dependent_launch.cuh"
@@ -861,8 +865,16 @@ size_t fp32_packed_fwd_bytes(const PackedArgs& a) { return list_bytes(a) + query
 
 int fp32_packed_fwd(const PackedArgs& p, void* ws, cudaStream_t st) { return p.D == 64 ? launch<64>(p, ws, st) : launch<128>(p, ws, st); }
 
+// Backward, us, here / there: a CTA of the key-major kernel walks over all rows of its 128 keys, G tokens' worth of the walk for
+// a token, while the fp32 units cut the walk into parts where there are few keys.  Blocks of 128 keys, all key heads:
+//  G 1 to 3: 1 block 22 / 39 (G 1), 29 / 39 (G 2); 8 blocks 39 / 39 (G 3)
+//  G 4: 8 blocks 42 / 40, 109 / 106  <  the line  <  16 blocks 44 / 53, 203 / 364
+//  G 8 to 64: 16 blocks 768 / 673, 70 / 90 (G 8), 1517 / 1308 (G 16), 950 / 888 (G 64)  <  the line  <  32 blocks 94 / 143, 1575 /
+//   2165 (G 8), 1109 / 1572 (G 64)
+//  4 x 2048 tokens, 4 x 4 heads 885 / 4122; 1 x 8192, 8 x 8 11084 / 58688
 bool fp32_packed_bwd_supported(const PackedArgs& a, int dtype) {
   if (!fp32_packed_supported(a, dtype) || a.D != 64 || a.group > kKeys) return false;
+  if (a.group > 3 && a.tokens_k / kRows * int64_t(a.kv_heads) < (a.group < 8 ? 16 : 32)) return false;
   if (reinterpret_cast<uintptr_t>(a.dq) % 16 || reinterpret_cast<uintptr_t>(a.dk) % 16 || reinterpret_cast<uintptr_t>(a.dv) % 16) return false;
   if (step_tiles(a) > 0x7fffffff || most_blocks(a.tokens_k, a.sequences, kRows) * a.kv_heads > 0x7fffffff) return false;
   return fp32_packed_bwd_bytes(a) <= (size_t(8) << 30);

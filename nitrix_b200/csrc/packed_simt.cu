@@ -1,6 +1,6 @@
 // Attention over packed sequences on the fp32 units: every type, head dim up to 256, group size and stride, forward and
 // backward, each sum in one order (no atomics).  The tensor-core kernels take what they cover; this is the rest,
-// the backward of fp32 operands among it.
+// short fp32 sequences and the backward of fp32 operands of head dim 128 among it.
 //
 // The query heads of one key head are rows of the same matrix: row r of a sequence is query r / G, head r % G, so that a tile
 // of rows reads its keys once for the whole group whatever G is, and dK and dV sum over the group by themselves.

@@ -23,10 +23,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     keys, each one before it one less.  A query that sees no key gives zeros and has no gradient; so do tokens behind the last
     offset.  Differentiable in ``q``, ``k`` and ``v``.
 
-    bf16 and fp16 with head dim 64 or 128 run on the tensor cores, as does the forward pass of fp32 operands of 128 keys per
-    sequence or more on average (three bf16 numbers each, good to 2^-20 of a product; an infinity makes its rows NaN); what
-    they do not take runs on the fp32 units, with one ``NitrixBackendFallback`` warning.  That family sums everything in a
-    fixed order and is what reproducibility mode uses.
+    bf16 and fp16 with head dim 64 or 128 run on the tensor cores, as do fp32 operands (three bf16 numbers each, good to 2^-20
+    of a product; an infinity makes its rows NaN) of 128 keys per sequence or more on average: their forward pass, and their
+    gradients at head dim 64.  A forward pass that the tensor cores do not take runs on the fp32 units, with one
+    ``NitrixBackendFallback`` warning.  That family sums everything in a fixed order and is what reproducibility mode uses.
     """
     resolved = resolve_backend(backend)
     kernel = _cabi.KERNEL_SIMT if resolved == "cuda-simt" else _cabi.KERNEL_AUTO

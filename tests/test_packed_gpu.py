@@ -384,3 +384,34 @@ def test_fp32_neighbours_and_magnitudes():
             assert torch.equal(got[:200], want[:200]) and torch.equal(got[331:631], want[331:631])
         big = packed_attention(q * 2.0 ** 60, k * 2.0 ** -60, v * 2.0 ** -60, off)
         assert torch.equal(big, want * 2.0 ** -60)
+
+
+@pytest.mark.parametrize("Hk,G,lengths", [(4, 16, [600, 0, 300, 200]), (8, 64, [300, 257]), (3, 5, [700, 31, 129]), (16, 4, [1, 270])])
+def test_fp32_gradients_of_groups(Hk, G, lengths):
+    """Groups whose rows fill the tiles and groups that leave some unused; the same bits every time."""
+    operands = _inputs(lengths, lengths, Hk * G, Hk, 64, torch.float32, seed=G)
+    out, grads = _check(*operands, lengths, lengths)
+    again, more = _check(*operands, lengths, lengths)
+    assert torch.equal(out, again) and all(torch.equal(a, b) for a, b in zip(grads, more))
+
+
+def test_fp32_gradients_on_the_tensor_cores_against_differences():
+    """As above; 55 680 outputs that are good to 2^-20 each leave 2^-20 sqrt(55 680) / (2 h) = 1e-2 at most."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [140, 150]
+    q, k, v, dout = _inputs(lengths, lengths, 3, 1, 64, torch.float32)
+    off = _offsets(lengths)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, off), leaves, dout)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for i in range(3):
+        e = torch.randn(leaves[i].shape, generator=g, device="cuda")
+        e /= e.norm()
+        h = 1e-2
+
+        def f(sign):
+            ops = [q, k, v]
+            ops[i] = ops[i] + sign * h * e
+            return (packed_attention(*ops, off).double() * dout.double()).sum()
+        assert abs(float((f(1) - f(-1)) / (2 * h) - (grads[i].double() * e.double()).sum())) < 2e-2
