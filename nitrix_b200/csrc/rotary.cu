@@ -49,8 +49,8 @@ struct RotaryArgs {
 };
 
 // cos and sin of a pair's phase at a token.  position * frequency / (2 pi) is formed with the rounding errors of its products,
-// less whole turns: in pairs of fp32 numbers up to 2^24, where a position is one, in pairs of fp64 ones above.  (64-bit units
-// are few: with them alone the training pass of 16384 tokens took 102 us at its best.)
+// less whole turns: in pairs of fp32 numbers below 2^24, where a position is one, in pairs of fp64 ones from there on (2^24 + 1
+// rounds to 2^24).  (64-bit units are few: with them alone the training pass of 16384 tokens took 102 us at its best.)
 template <typename T>
 __device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int token, int pair) {
   int axis = 0;
@@ -61,18 +61,18 @@ __device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int token, int pa
   if (a.position_dtype == NB200_POS_I32) {
     const int32_t n = static_cast<const int32_t*>(a.positions)[i];
     p = float(n);
-    if (fabsf(p) > kFp32Positions) exact = double(n);
+    if (fabsf(p) >= kFp32Positions) exact = double(n);
   } else if (a.position_dtype == NB200_POS_I64) {
     const int64_t n = static_cast<const int64_t*>(a.positions)[i];
     p = float(n);
-    if (fabsf(p) > kFp32Positions) exact = double(n);
+    if (fabsf(p) >= kFp32Positions) exact = double(n);
   } else {
     p = static_cast<const float*>(a.positions)[i];
-    if (fabsf(p) > kFp32Positions) exact = double(p);
+    if (fabsf(p) >= kFp32Positions) exact = double(p);
   }
   const float f = a.frequencies[pair];
   float part;      // of a turn
-  if (fabsf(p) > kFp32Positions) {
+  if (fabsf(p) >= kFp32Positions) {
     const double phase = exact * f, phase_low = fma(exact, double(f), -phase);
     const double turns = phase * kTurnHigh, turns_low = fma(phase, kTurnHigh, -turns) + fma(phase, kTurnLow, phase_low * kTurnHigh);
     part = float((turns - rint(turns)) + turns_low);

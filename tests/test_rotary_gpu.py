@@ -172,3 +172,19 @@ def test_more_tokens_than_32_bits_count():
     positions = torch.zeros(1, dtype=torch.int32, device="cuda").expand(2 ** 32 + 1)
     with pytest.raises(ValueError, match="32 bits"):
         rotary_embedding(q, None, positions, torch.ones(4, device="cuda"))
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_positions_around_the_first_that_fp32_does_not_hold(kind):
+    """2^24 + 1 as an fp32 number is 2^24: one radian away at frequency 1."""
+    from nitrix_b200.nn import rotary_embedding, rotary_frequencies
+
+    n = 1 << 24
+    pos = torch.tensor([n - 1, n, n + 1, n + 2, n + 3, -n - 1, -n, 1 - n], device="cuda").to(kind)
+    x, ct = (torch.randn(8, 2, 64, device="cuda") for _ in range(2))
+    freq = rotary_frequencies((32,), device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    y, _ = rotary_embedding(leaf, None, pos, freq)
+    _close(y.detach(), x, O.rotary(x, pos[:, None], freq, (32,)), torch.float32, 32)
+    grad, = torch.autograd.grad(y, leaf, ct)
+    _close(grad, ct, O.rotary(ct, pos[:, None], freq, (32,), inverse=True), torch.float32, 32)
