@@ -9,8 +9,8 @@
  * offsets_q[i + 1) and the keys offsets_k[i] .. offsets_k[i + 1), lq and lk of them.  q is (tokens_q, heads, D), k and v are
  * (tokens_k, kv_heads, D); query head h reads key head h / (heads / kv_heads).  With `causal`, query i of a sequence sees its
  * keys up to i + lk - lq: the last query sees all of them.  A query that sees no key gives zeros, lse = -inf and zero
- * gradients.  Tokens behind offsets[sequences] belong to no sequence; their rows of every output are zeros.  lse is
- * (tokens_q, heads) fp32, the base-2 log-sum-exp of the scaled scores.
+ * gradients.  Tokens before offsets[0] and behind offsets[sequences] belong to no sequence; their rows of every output are
+ * zeros.  lse is (tokens_q, heads) fp32, the base-2 log-sum-exp of the scaled scores.
  *
  * q, k, v and dout are described by two element strides (token, head; unit stride on D); out, dq, dk and dv are dense.  The
  * offsets are device memory: nothing is read on the host.  Every pointer is a device pointer; all work is enqueued on the

@@ -35,8 +35,19 @@ __device__ __forceinline__ int2 sequence_span(const int* offsets, int i, int tok
   const int begin = min(max(offsets[i], 0), tokens), end = min(max(offsets[i + 1], begin), tokens);
   return make_int2(begin, end - begin);
 }
+// Tokens before the first sequence, and up to the end of the last one: those outside belong to no sequence.
+__device__ __forceinline__ int tokens_before(const int* offsets, int sequences, int tokens) {
+  return sequences > 0 ? min(max(offsets[0], 0), tokens) : 0;
+}
 __device__ __forceinline__ int covered_tokens(const int* offsets, int sequences, int tokens) {
   return sequences > 0 ? min(max(offsets[sequences], 0), tokens) : 0;
+}
+
+// Elements of the rows, `row` elements each, that lie outside [first, last); every `step`-th of them from `at` on.
+template <typename T>
+__device__ __forceinline__ void clear_outside(T* base, int64_t row, int first, int last, int rows, T value, int64_t at, int64_t step) {
+  for (int64_t i = at; i < first * row; i += step) base[i] = value;
+  for (int64_t i = last * row + at; i < rows * row; i += step) base[i] = value;
 }
 
 // The sequence that piece `index` of all sequences' `count(i)` pieces belongs to, and its number there (-1: there is no such
@@ -67,7 +78,7 @@ __device__ __forceinline__ Place find_place(int index, int sequences, Count coun
 }
 #endif
 
-// out = zeros for the tokens behind the last sequence (and lse = -inf, where `lse` is given): part of every pass
+// out = zeros for the tokens of no sequence (and lse = -inf), or zero gradients: part of every pass
 int launch_clear_uncovered(const PackedArgs& a, int dtype, bool backward, cudaStream_t st);
 int launch_packed_delta(const PackedArgs& a, int dtype, cudaStream_t st);
 int simt_packed_fwd(const PackedArgs& a, int dtype, cudaStream_t st);

@@ -119,25 +119,22 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, const uint8_t*
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void clear_tail(T* base, int64_t first, int64_t end, T value) {
-  for (int64_t i = first + int64_t(blockIdx.x - 1) * kPlanThreads + threadIdx.x; i < end; i += int64_t(kClearCtas) * kPlanThreads) base[i] = value;
-}
-
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArgs p) {
   allow_dependents();
   const PackedArgs& a = p.a;
   if (blockIdx.x > 0) {
     if (p.halves == 0) return;
-    const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), row = int64_t(a.heads) * a.D * p.halves;
-    uint16_t* out = static_cast<uint16_t*>(p.backward ? a.dq : a.out);
-    clear_tail<uint16_t>(out, q0 * row, a.tokens_q * row, 0);      // (a zero has no bits)
+    const int q0 = tokens_before(a.offsets_q, a.sequences, a.tokens_q), q1 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q);
+    const int64_t row = int64_t(a.heads) * a.D * p.halves;
+    const int64_t at = int64_t(blockIdx.x - 1) * kPlanThreads + threadIdx.x, step = int64_t(kClearCtas) * kPlanThreads;
+    clear_outside<uint16_t>(static_cast<uint16_t*>(p.backward ? a.dq : a.out), row, q0, q1, a.tokens_q, 0, at, step);      // (a zero has no bits)
     if (!p.backward) {
-      clear_tail<float>(a.lse, q0 * a.heads, int64_t(a.tokens_q) * a.heads, -INFINITY);
+      clear_outside<float>(a.lse, a.heads, q0, q1, a.tokens_q, -INFINITY, at, step);
     } else {
-      const int64_t k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k), krow = int64_t(a.kv_heads) * a.D * p.halves;
-      clear_tail<uint16_t>(static_cast<uint16_t*>(a.dk), k0 * krow, a.tokens_k * krow, 0);
-      clear_tail<uint16_t>(static_cast<uint16_t*>(a.dv), k0 * krow, a.tokens_k * krow, 0);
+      const int k0 = tokens_before(a.offsets_k, a.sequences, a.tokens_k), k1 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k);
+      const int64_t krow = int64_t(a.kv_heads) * a.D * p.halves;
+      clear_outside<uint16_t>(static_cast<uint16_t*>(a.dk), krow, k0, k1, a.tokens_k, 0, at, step);
+      clear_outside<uint16_t>(static_cast<uint16_t*>(a.dv), krow, k0, k1, a.tokens_k, 0, at, step);
     }
     return;
   }

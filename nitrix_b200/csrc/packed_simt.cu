@@ -451,8 +451,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkv_simt_kernel(const Pack
 // dk and dv as the sums of their parts, in order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) packed_dkv_sum_kernel(const PackedArgs a, int parts) {
-  const int64_t covered = int64_t(covered_tokens(a.offsets_k, a.sequences, a.tokens_k)) * a.kv_heads * a.D, all = int64_t(a.tokens_k) * a.kv_heads * a.D;
-  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < covered; i += int64_t(gridDim.x) * kThreads) {
+  const int64_t row = int64_t(a.kv_heads) * a.D, all = a.tokens_k * row;
+  const int64_t first = tokens_before(a.offsets_k, a.sequences, a.tokens_k) * row, end = covered_tokens(a.offsets_k, a.sequences, a.tokens_k) * row;
+  for (int64_t i = first + int64_t(blockIdx.x) * kThreads + threadIdx.x; i < end; i += int64_t(gridDim.x) * kThreads) {
     float dk = 0.f, dv = 0.f;
     for (int p = 0; p < parts; ++p) {
       dk += a.parts[2 * p * all + i];
@@ -480,21 +481,19 @@ __global__ void __launch_bounds__(kThreads) packed_delta_kernel(const PackedArgs
   if (lane == 0) a.delta[row] = sum;
 }
 
-// The tokens behind the last sequence.
+// The tokens of no sequence: before the first and behind the last.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) packed_clear_kernel(const PackedArgs a, bool backward) {
-  const int64_t step = int64_t(gridDim.x) * kThreads, start = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t q0 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q), k0 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k);
-  T* rows_q = static_cast<T*>(backward ? a.dq : a.out);
-  for (int64_t i = q0 * a.heads * a.D + start; i < int64_t(a.tokens_q) * a.heads * a.D; i += step) rows_q[i] = from_f32<T>(0.f);
+  const int64_t step = int64_t(gridDim.x) * kThreads, at = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int q0 = tokens_before(a.offsets_q, a.sequences, a.tokens_q), q1 = covered_tokens(a.offsets_q, a.sequences, a.tokens_q);
+  clear_outside(static_cast<T*>(backward ? a.dq : a.out), int64_t(a.heads) * a.D, q0, q1, a.tokens_q, from_f32<T>(0.f), at, step);
   if (!backward) {
-    for (int64_t i = q0 * a.heads + start; i < int64_t(a.tokens_q) * a.heads; i += step) a.lse[i] = -INFINITY;
+    clear_outside(a.lse, a.heads, q0, q1, a.tokens_q, -INFINITY, at, step);
     return;
   }
-  for (int64_t i = k0 * a.kv_heads * a.D + start; i < int64_t(a.tokens_k) * a.kv_heads * a.D; i += step) {
-    static_cast<T*>(a.dk)[i] = from_f32<T>(0.f);
-    static_cast<T*>(a.dv)[i] = from_f32<T>(0.f);
-  }
+  const int k0 = tokens_before(a.offsets_k, a.sequences, a.tokens_k), k1 = covered_tokens(a.offsets_k, a.sequences, a.tokens_k);
+  clear_outside(static_cast<T*>(a.dk), int64_t(a.kv_heads) * a.D, k0, k1, a.tokens_k, from_f32<T>(0.f), at, step);
+  clear_outside(static_cast<T*>(a.dv), int64_t(a.kv_heads) * a.D, k0, k1, a.tokens_k, from_f32<T>(0.f), at, step);
 }
 
 template <typename F>

@@ -20,8 +20,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     ``q`` is ``(tokens, heads, head_dim)``, ``k`` and ``v`` are ``(tokens, key heads, head_dim)``; query head ``h`` reads key
     head ``h // (heads // key heads)``.  Sequence ``i`` has the tokens ``offsets[i] .. offsets[i + 1]`` (int32, on the device);
     ``offsets_k`` where its keys are not as many as its queries.  With ``causal`` the last query of a sequence sees all its
-    keys, each one before it one less.  A query that sees no key gives zeros and has no gradient; so do tokens behind the last
-    offset.  Differentiable in ``q``, ``k`` and ``v``.
+    keys, each one before it one less.  A query that sees no key gives zeros and has no gradient; so do tokens before the
+    first offset and behind the last.  Differentiable in ``q``, ``k`` and ``v``.
 
     bf16 and fp16 with head dim 64 or 128 run on the tensor cores, as do fp32 operands (three bf16 numbers each, good to 2^-20
     of a product; an infinity makes its rows NaN) of 128 keys per sequence or more on average: their forward pass, and their

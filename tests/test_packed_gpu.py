@@ -415,3 +415,34 @@ def test_fp32_gradients_on_the_tensor_cores_against_differences():
             ops[i] = ops[i] + sign * h * e
             return (packed_attention(*ops, off).double() * dout.double()).sum()
         assert abs(float((f(1) - f(-1)) / (2 * h) - (grads[i].double() * e.double()).sum())) < 2e-2
+
+
+@pytest.mark.parametrize("dtype,D,backend", [
+    (torch.bfloat16, 64, "auto"), (torch.float16, 128, "auto"), (torch.float32, 64, "auto"), (torch.float32, 128, "auto"),
+    (torch.bfloat16, 64, "cuda-simt"), (torch.float32, 40, "cuda-simt"), (torch.float16, 256, "cuda-simt")])
+@pytest.mark.parametrize("lead_q,lead_k", [(37, 37), (5, 130), (200, 0)])
+def test_tokens_before_the_first_offset(dtype, D, backend, lead_q, lead_k, monkeypatch):
+    """Sequences cut out of a longer batch: what lies before the first offset belongs to none of them, as what lies behind the
+    last: zeros, in the gradients too, whatever its operands hold."""
+    from nitrix_b200.nn import packed_attention
+
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths_q, lengths_k = [300, 0, 140], [260, 31, 190]
+    nq, nk = sum(lengths_q), sum(lengths_k)
+    q, k, v, dout = _inputs([lead_q + nq + 21], [lead_k + nk + 21], 4, 2, D, dtype)
+    rows, keys = slice(lead_q, lead_q + nq), slice(lead_k, lead_k + nk)
+    for t, s in ((q, rows), (k, keys), (v, keys), (dout, rows)):
+        t[:s.start] = float("nan")
+        t[s.stop:] = float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    stale = [torch.full_like(t, float("nan")) for t in (q, q, k, v) for _ in range(3)]      # what the results are given to write on
+    del stale
+    out = packed_attention(*leaves, _offsets(lengths_q) + lead_q, offsets_k=_offsets(lengths_k) + lead_k, backend=backend)
+    stale = [torch.full_like(t, float("nan")) for t in (q, k, v) for _ in range(3)]
+    del stale
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = O.packed(q[rows], k[keys], v[keys], lengths_q, lengths_k, D ** -0.5, True, dout[rows])
+    for name, got, s in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), (rows, rows, keys, keys)):
+        assert not bool(got[:s.start].any()) and not bool(got[s.stop:].any()), name
+        value, bound = want[name]
+        assert float(((got[s].double() - value).abs() - U[dtype] * bound).max()) <= 1e-6, name
