@@ -49,7 +49,7 @@ bool fp32_tensor_cores(const nb200_packed_params* p, const PackedArgs& a, int pa
 
 size_t workspace(const nb200_packed_params* p, const PackedArgs& a, int pass) {
   if (fp32_tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? fp32_packed_fwd_bytes(a) : delta_bytes(p) + fp32_packed_bwd_bytes(a);
-  if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a);
+  if (tensor_cores(p, a, pass)) return pass == NB200_PASS_FWD ? tc_packed_fwd_bytes(a) : tc_packed_bwd_bytes(a, p->dtype);
   return pass == NB200_PASS_FWD ? 0 : delta_bytes(p) + simt_packed_bwd_bytes(a);
 }
 

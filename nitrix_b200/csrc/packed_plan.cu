@@ -6,7 +6,7 @@
 // sums alone are 284 MB and the kernel takes 1252 us for 1054).  And the longest blocks of what is left should come first, so that
 // short ones even out the end.  So the sequences, longest first, are cut into groups of at least one block per SM (two: 1078 us, three: 1089), and within a
 // group the blocks are sorted by their length in tiles; blocks of one length come in any order, which changes no result.
-// The other CTAs clear the outputs of tokens that belong to no sequence.
+// The other CTAs clear the outputs of tokens that belong to no sequence, and reduce what the fp16 backward wants the maxima of.
 #include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
@@ -119,6 +119,39 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, const uint8_t*
   }
 }
 
+// The largest of value(row) >= 0 over every sequence's rows, `heads` a token, into to[2 * sequence].  The tokens are dealt to the
+// warps in contiguous shares, so that nobody looks a row's sequence up by itself.
+template <typename Value>
+__device__ __forceinline__ void raise_largest(const int* offsets, int sequences, int tokens, int heads, unsigned* to, Value value) {
+  const int lane = threadIdx.x & 31, warps = kClearCtas * (kPlanThreads / 32);
+  const int share = (tokens + warps - 1) / warps;
+  const int64_t t0 = (int64_t(blockIdx.x - 1) * (kPlanThreads / 32) + (threadIdx.x >> 5)) * share;
+  const int64_t t1 = min(t0 + share, int64_t(tokens));
+  if (t0 >= t1) return;
+  int s0 = 0, n = sequences;      // the last sequence that begins at t0 or before it is one of s0 .. s0 + n - 1
+  while (n > 1) {
+    const int step = (n + 31) / 32, i = lane * step;
+    const int skip = max(__popc(__ballot_sync(0xffffffffu, i < n && offsets[s0 + i] <= t0)) - 1, 0) * step;
+    s0 += skip;
+    n = min(step, n - skip);
+  }
+  for (; s0 < sequences; s0 += 32) {
+    const int2 span = s0 + lane < sequences ? sequence_span(offsets, s0 + lane, tokens) : make_int2(tokens, 0);
+    unsigned some = __ballot_sync(0xffffffffu, span.y > 0 && span.x < t1 && int64_t(span.x) + span.y > t0);
+    for (; some; some &= some - 1) {
+      const int j = __ffs(some) - 1, first = __shfl_sync(0xffffffffu, span.x, j), length = __shfl_sync(0xffffffffu, span.y, j);
+      const int64_t end = min(t1, int64_t(first) + length) * heads;
+      float most = 0.f;
+#pragma unroll 4
+      for (int64_t row = max(t0, int64_t(first)) * heads + lane; row < end; row += 32) most = fmaxf(most, value(row));
+      const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));      // (numbers >= 0 have the order of their bits)
+      unsigned* at = to + 2 * int64_t(s0 + j);
+      if (lane == 0 && bits > *reinterpret_cast<volatile unsigned*>(at)) atomicMax(at, bits);
+    }
+    if (__any_sync(0xffffffffu, span.x >= t1)) break;
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArgs p) {
   allow_dependents();
   const PackedArgs& a = p.a;
@@ -135,6 +168,14 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
       const int64_t krow = int64_t(a.kv_heads) * a.D * p.halves;
       clear_outside<uint16_t>(static_cast<uint16_t*>(a.dk), krow, k0, k1, a.tokens_k, 0, at, step);
       clear_outside<uint16_t>(static_cast<uint16_t*>(a.dv), krow, k0, k1, a.tokens_k, 0, at, step);
+      if (a.largest) {
+        // (a NaN counts as infinite; a query without a key has no gradient)
+        auto size = [](float squares) { return squares < INFINITY ? squares : INFINITY; };
+        raise_largest(a.offsets_q, a.sequences, a.tokens_q, a.heads, a.largest,
+                      [&](int64_t row) { return a.lse[row] == -INFINITY ? 0.f : size(a.squares[row]); });
+        const float* values = a.squares + int64_t(a.tokens_q) * a.heads;
+        raise_largest(a.offsets_k, a.sequences, a.tokens_k, a.kv_heads, a.largest + 1, [&](int64_t row) { return size(values[row]); });
+      }
     }
     return;
   }

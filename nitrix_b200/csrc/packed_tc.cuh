@@ -34,7 +34,8 @@ inline size_t work_list_bytes(int64_t most) { return (16 + size_t(most) * sizeof
 // most blocks of `block` tokens that sequences of `tokens` tokens together have
 inline int64_t most_blocks(int64_t tokens, int sequences, int block) { return tokens / block + sequences; }
 
-// Fills the list (and clears the outputs of tokens that no sequence covers, which would be a launch of its own).
+// Fills the list (and clears the outputs of tokens that no sequence covers, and takes the maxima that the fp16 backward asks for,
+// which would be launches of their own).
 // `element`: bytes of an element of the outputs; 0: they are left alone.
 // `block`: queries (forward) or keys (backward) of a block; `step_tokens` (backward): queries of a 64-row step.
 int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st, int element = 2);
@@ -46,7 +47,7 @@ bool tc_packed_supported(const PackedArgs& a, int dtype);
 size_t tc_packed_fwd_bytes(const PackedArgs& a);
 int tc_packed_fwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
 bool tc_packed_bwd_supported(const PackedArgs& a, int dtype);
-size_t tc_packed_bwd_bytes(const PackedArgs& a);
+size_t tc_packed_bwd_bytes(const PackedArgs& a, int dtype);
 int tc_packed_bwd(const PackedArgs& a, int dtype, void* ws, cudaStream_t st);
 
 // fp32 operands as three bf16 planes (packed_fp32_tc.cu)

@@ -53,7 +53,7 @@ struct BwdArgs {
   const float* delta;
   float* dq_acc;             // [key head][step][row / 4][d][row % 4]
   int64_t all_steps;         // steps that the accumulator has room for, per key head
-  const float* largest;      // fp16: the largest squared norms of a row of dout and of v
+  const float* largest;      // fp16: for every sequence the largest squared norms of a row of dout and of v
   void* dk;                  // dense (tokens_k, kv_heads, D)
   void* dv;
   int* status;
@@ -62,10 +62,11 @@ struct BwdArgs {
 // fp16 has few exponents: with thousands of keys P and dS lie where it loses its digits.  P is taken times 2^10 (at most 1024), dS
 // times the power of two that its bound allows: |dS| <= |dout row| |v row| + |delta| <= 2 max |dout row| max |v row|, since a row of
 // out is a mean of rows of v.  Both factors leave with the results.  (Relative error of dq and dk over sequences of thousands of
-// tokens: 4.1e-4 without, 3.1e-4 with them; the rounding of dS and that of the results are 2.1e-4 each.)
+// tokens: 4.1e-4 without, 3.1e-4 with them; the rounding of dS and that of the results are 2.1e-4 each.)  The bound is taken for each
+// sequence by itself, over its queries that see a key: what stands elsewhere must not cost its gradients their digits.
 constexpr int kPShift = 10;
-__device__ __forceinline__ int ds_shift(const float* largest) {
-  const float bound = 2.f * sqrtf(largest[0]) * sqrtf(largest[1]);
+__device__ __forceinline__ int ds_shift(const float* largest, int sequence) {
+  const float bound = 2.f * sqrtf(largest[2 * sequence]) * sqrtf(largest[2 * sequence + 1]);
   if (!(bound < INFINITY)) return 0;
   const float room = floorf(log2f(60000.f / fmaxf(bound, 1e-30f)));
   return int(fminf(fmaxf(room, -14.f), 14.f));
@@ -387,7 +388,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     bool ok = true;
     const float mul = a.scale * kLog2e;
     const float2 mul2 = make_float2(mul, mul);
-    const int shift = kBf16 ? 0 : ds_shift(a.largest);
+    const int shift = kBf16 ? 0 : ds_shift(a.largest, it.sequence);
     const float ds_mul = kBf16 ? 1.f : exp2f(float(shift - kPShift));      // (P is 2^10 times itself)
     const float2 ds_mul2 = make_float2(ds_mul, ds_mul);
     const bool dropped = r >= it.n;
@@ -562,12 +563,12 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 }
 
 // delta[token][head] = sum_d out dout in fp32.  Bound by HBM: D / 8 lanes per row with 16 bytes of each tensor, four rows per
-// lane whose loads are in flight together.  fp16: also the largest squared norm of a row of dout, and, by the CTAs behind
-// `delta_ctas`, of a row of v.
+// lane whose loads are in flight together.  fp16: also the squared norms of the rows of dout, and, by the CTAs behind `delta_ctas`,
+// of those of v; the launch that lists the blocks has their maxima.
 constexpr int kDeltaThreads = 256, kDeltaRows = 4;
 
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const PackedArgs a, int delta_ctas, unsigned* largest) {
+__global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const PackedArgs a, int delta_ctas) {
   constexpr int kLanes = D / 8, kGroups = kDeltaThreads / kLanes;
   const bool values = !kBf16 && int(blockIdx.x) >= delta_ctas;
   const int heads = values ? a.kv_heads : a.heads, rows = values ? a.tokens_k * a.kv_heads : a.tokens_q * a.heads;      // (below 2^31: checked on the host)
@@ -584,7 +585,6 @@ __global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const Pa
       g[i] = ldg_no_allocate(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(values ? a.v : a.dout) + at) + c);
     }
   }
-  float norm = 0.f;
 #pragma unroll
   for (int i = 0; i < kDeltaRows; ++i) {
     const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
@@ -602,16 +602,7 @@ __global__ void __launch_bounds__(kDeltaThreads) packed_delta_tc_kernel(const Pa
     }
     const int row = row0 + i * kGroups;
     if (!values && row < rows && c == 0) a.delta[row] = sum;
-    norm = squares <= norm ? norm : squares < INFINITY ? squares : INFINITY;      // (a NaN counts as infinite)
-  }
-  if constexpr (!kBf16) {
-    __shared__ unsigned most;
-    if (threadIdx.x == 0) most = 0;
-    __syncthreads();
-    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(norm));      // (of numbers >= 0, in their order)
-    if ((threadIdx.x & 31) == 0) atomicMax(&most, bits);
-    __syncthreads();
-    if (threadIdx.x == 0 && most > *reinterpret_cast<volatile unsigned*>(largest + (values ? 1 : 0))) atomicMax(largest + (values ? 1 : 0), most);
+    if (!kBf16 && row < rows && c == 0) a.squares[(values ? int64_t(a.tokens_q) * a.heads : 0) + row] = squares;
   }
 }
 
@@ -628,7 +619,7 @@ __global__ void __launch_bounds__(kStep / 4 * (D / 8)) packed_dq_finish_kernel(c
   const Place place = find_place(int(blockIdx.x), a.sequences, [&](int i) { return (sequence_span(a.offsets_q, i, a.tokens_q).y + tokens - 1) / tokens; });
   if (place.index < 0) return;
   const int2 q = sequence_span(a.offsets_q, place.sequence, a.tokens_q);
-  const float scale = kBf16 ? a.scale : a.scale * exp2f(-float(ds_shift(largest)));
+  const float scale = kBf16 ? a.scale : a.scale * exp2f(-float(ds_shift(largest, place.sequence)));
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
     const int row = rg * 4 + rr, t = row / a.group, token = place.index * tokens + t;
@@ -649,8 +640,11 @@ __global__ void __launch_bounds__(kStep / 4 * (D / 8)) packed_dq_finish_kernel(c
 int64_t most_steps(const PackedArgs& a) { return most_blocks(a.tokens_q, a.sequences, tile_tokens(kStep, a.group)); }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 size_t delta_bytes(const PackedArgs& a) { return up256(size_t(a.tokens_q) * a.heads * sizeof(float)); }
+size_t squares_bytes(const PackedArgs& a, bool bf16) {
+  return bf16 ? 0 : up256((size_t(a.tokens_q) * a.heads + size_t(a.tokens_k) * a.kv_heads) * sizeof(float));
+}
 size_t list_bytes(const PackedArgs& a) { return work_list_bytes(most_blocks(a.tokens_k, a.sequences, kTile)); }
-constexpr size_t kLargestBytes = 256;      // in front of the sums, cleared with them
+size_t largest_bytes(const PackedArgs& a, bool bf16) { return bf16 ? 0 : up256(size_t(a.sequences) * 2 * sizeof(float)); }      // in front of the sums, cleared with them
 size_t acc_bytes(const PackedArgs& a) { return size_t(a.kv_heads) * size_t(most_steps(a)) * kStep * a.D * sizeof(float); }
 
 template <int D, bool kBf16>
@@ -678,15 +672,18 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   char* base = static_cast<char*>(ws);
   p.delta = reinterpret_cast<float*>(base);
   void* list = base + delta_bytes(p);
-  unsigned* largest = reinterpret_cast<unsigned*>(base + delta_bytes(p) + list_bytes(p));
-  float* acc = reinterpret_cast<float*>(base + delta_bytes(p) + list_bytes(p) + kLargestBytes);
+  char* rest = base + delta_bytes(p) + list_bytes(p);
+  if (!kBf16) p.squares = reinterpret_cast<float*>(rest);
+  rest += squares_bytes(p, kBf16);
+  if (!kBf16) p.largest = reinterpret_cast<unsigned*>(rest);
+  float* acc = reinterpret_cast<float*>(rest + largest_bytes(p, kBf16));
   BwdArgs a{};
   a.tokens = tile_tokens(kStep, p.group);
   constexpr int kDeltaCta = kDeltaThreads / (D / 8) * kDeltaRows;      // rows
   const int64_t delta_grid = (int64_t(p.tokens_q) * p.heads + kDeltaCta - 1) / kDeltaCta;
   const int64_t value_grid = kBf16 ? 0 : (int64_t(p.tokens_k) * p.kv_heads + kDeltaCta - 1) / kDeltaCta;
-  if (cudaMemsetAsync(largest, 0, kLargestBytes + acc_bytes(p), st) != cudaSuccess) return check_launch("packed_bwd: clearing the sums of dq");
-  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid + value_grid), kDeltaThreads, 0, st>>>(p, int(delta_grid), largest);
+  if (cudaMemsetAsync(rest, 0, largest_bytes(p, kBf16) + acc_bytes(p), st) != cudaSuccess) return check_launch("packed_bwd: clearing the sums of dq");
+  packed_delta_tc_kernel<D, kBf16><<<unsigned(delta_grid + value_grid), kDeltaThreads, 0, st>>>(p, int(delta_grid));
   count_launch();
   if (int rc = check_launch("packed_delta_tc_kernel")) return rc;
   if (int rc = launch_plan(p, true, kTile, a.tokens, list, st)) return rc;
@@ -706,7 +703,7 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
   a.lse = p.lse;
   a.delta = p.delta;
   a.dq_acc = acc;
-  a.largest = reinterpret_cast<const float*>(largest);
+  a.largest = reinterpret_cast<const float*>(p.largest);
   a.all_steps = most_steps(p);
   a.dk = p.dk;
   a.dv = p.dv;
@@ -723,7 +720,10 @@ int launch_all(PackedArgs p, void* ws, cudaStream_t st) {
 
 }  // namespace
 
-size_t tc_packed_bwd_bytes(const PackedArgs& a) { return delta_bytes(a) + list_bytes(a) + kLargestBytes + acc_bytes(a); }
+size_t tc_packed_bwd_bytes(const PackedArgs& a, int dtype) {
+  const bool bf16 = dtype == NB200_BF16;
+  return delta_bytes(a) + list_bytes(a) + squares_bytes(a, bf16) + largest_bytes(a, bf16) + acc_bytes(a);
+}
 
 int tc_packed_bwd(const PackedArgs& p, int dtype, void* ws, cudaStream_t st) {
   const bool bf16 = dtype == NB200_BF16;

@@ -446,3 +446,31 @@ def test_tokens_before_the_first_offset(dtype, D, backend, lead_q, lead_k, monke
         assert not bool(got[:s.start].any()) and not bool(got[s.stop:].any()), name
         value, bound = want[name]
         assert float(((got[s].double() - value).abs() - U[dtype] * bound).max()) <= 1e-6, name
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [3e2, 6e4])
+def test_fp16_gradients_beside_large_numbers(D, size):
+    """Numbers of any size in neighbouring sequences, and in rows of no sequence, take no digits from the gradients of the others."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths, lead, tail = [200, 150, 33, 1, 100], 19, 70
+    n = lead + sum(lengths)
+    q, k, v, dout = _inputs([n + tail], [n + tail], 6, 2, D, torch.float16)
+    dout *= 1e-3
+    spans, at = [], lead
+    for length in lengths:
+        spans.append(slice(at, at + length))
+        at += length
+    dirty = [slice(0, lead), spans[1], spans[3], slice(n, n + tail)]
+    for s in dirty:
+        v[s] = size
+        dout[s] = -size
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, _offsets(lengths) + lead), leaves, dout)
+    for i in (0, 2, 4):
+        s = spans[i]
+        want = O.packed(q[s], k[s], v[s], [lengths[i]], [lengths[i]], D ** -0.5, True, dout[s])
+        for name, got in zip(("dq", "dk", "dv"), grads):
+            value, bound = want[name]
+            assert float(((got[s].double() - value).abs() - U[torch.float16] * bound).max()) <= 1e-6, (i, name)
