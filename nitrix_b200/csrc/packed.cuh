@@ -27,7 +27,7 @@ struct PackedArgs {
   float scale;
   float* delta;              // (tokens_q, heads): rowsum(out * dout)
   float* squares;            // fp16 on the tensor cores: squared norms of the rows of dout (tokens_q, heads), then of v
-  unsigned* largest;         // and the largest of each sequence, [sequence][dout, v], as the bits of fp32 numbers
+  unsigned* largest;         // and maxima over each sequence (SequenceMost), as the bits of fp32 numbers
   float* parts;              // fp32 units: parts of dk and dv, [part][dk, dv][token][key head][D]
 };
 

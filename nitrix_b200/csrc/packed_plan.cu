@@ -119,7 +119,7 @@ __device__ __forceinline__ void for_each_block(const PlanArgs& p, const uint8_t*
   }
 }
 
-// The largest of value(row) >= 0 over every sequence's rows, `heads` a token, into to[2 * sequence].  The tokens are dealt to the
+// The largest of value(row) >= 0 over every sequence's rows, `heads` a token, into to[kMosts * sequence].  The tokens are dealt to the
 // warps in contiguous shares, so that nobody looks a row's sequence up by itself.
 template <typename Value>
 __device__ __forceinline__ void raise_largest(const int* offsets, int sequences, int tokens, int heads, unsigned* to, Value value) {
@@ -145,7 +145,7 @@ __device__ __forceinline__ void raise_largest(const int* offsets, int sequences,
 #pragma unroll 4
       for (int64_t row = max(t0, int64_t(first)) * heads + lane; row < end; row += 32) most = fmaxf(most, value(row));
       const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));      // (numbers >= 0 have the order of their bits)
-      unsigned* at = to + 2 * int64_t(s0 + j);
+      unsigned* at = to + kMosts * int64_t(s0 + j);
       if (lane == 0 && bits > *reinterpret_cast<volatile unsigned*>(at)) atomicMax(at, bits);
     }
     if (__any_sync(0xffffffffu, span.x >= t1)) break;
@@ -170,11 +170,16 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PlanArg
       clear_outside<uint16_t>(static_cast<uint16_t*>(a.dv), krow, k0, k1, a.tokens_k, 0, at, step);
       if (a.largest) {
         // (a NaN counts as infinite; a query without a key has no gradient)
-        auto size = [](float squares) { return squares < INFINITY ? squares : INFINITY; };
-        raise_largest(a.offsets_q, a.sequences, a.tokens_q, a.heads, a.largest,
+        auto size = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : INFINITY; };
+        const float inv_mul = 1.f / (a.scale * kLog2e);
+        raise_largest(a.offsets_q, a.sequences, a.tokens_q, a.heads, a.largest + kMostDout,
                       [&](int64_t row) { return a.lse[row] == -INFINITY ? 0.f : size(a.squares[row]); });
+        raise_largest(a.offsets_q, a.sequences, a.tokens_q, a.heads, a.largest + kMostOfAddends, [&](int64_t row) {
+          const float lse = a.lse[row];
+          return lse == -INFINITY ? 0.f : fmaxf(size((lse - float(kPShift)) * inv_mul), size(a.delta[row]));
+        });
         const float* values = a.squares + int64_t(a.tokens_q) * a.heads;
-        raise_largest(a.offsets_k, a.sequences, a.tokens_k, a.kv_heads, a.largest + 1, [&](int64_t row) { return size(values[row]); });
+        raise_largest(a.offsets_k, a.sequences, a.tokens_k, a.kv_heads, a.largest + kMostV, [&](int64_t row) { return size(values[row]); });
       }
     }
     return;

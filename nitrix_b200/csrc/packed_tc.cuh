@@ -40,6 +40,11 @@ inline int64_t most_blocks(int64_t tokens, int sequences, int block) { return to
 // `block`: queries (forward) or keys (backward) of a block; `step_tokens` (backward): queries of a 64-row step.
 int launch_plan(const PackedArgs& a, bool backward, int block, int step_tokens, void* list, cudaStream_t st, int element = 2);
 
+// fp16 backward: a power of two on P, and what is known of each sequence (over its queries that see a key): the largest squared
+// norm of a row of dout and of v, the largest size of what is added to a product (lse - kPShift over scale log2 e, and delta).
+constexpr int kPShift = 10;
+enum SequenceMost { kMostDout = 0, kMostV = 1, kMostOfAddends = 2, kMosts = 4 };
+
 // Rows of a query tile are, token after token, the query heads of one key head: this many tokens fit.
 __host__ __device__ inline int tile_tokens(int rows, int group) { return rows / group; }
 

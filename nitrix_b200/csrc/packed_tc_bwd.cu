@@ -23,6 +23,8 @@
 // in TMEM 522 -> 508 us, two dS tiles as well 551.  All waits bounded.
 #include <math.h>
 
+#include <type_traits>
+
 #include "dependent_launch.cuh"
 #include "packed_tc.cuh"
 
@@ -53,7 +55,7 @@ struct BwdArgs {
   const float* delta;
   float* dq_acc;             // [key head][step][row / 4][d][row % 4]
   int64_t all_steps;         // steps that the accumulator has room for, per key head
-  const float* largest;      // fp16: for every sequence the largest squared norms of a row of dout and of v
+  const float* largest;      // fp16: what SequenceMost says, for every sequence
   void* dk;                  // dense (tokens_k, kv_heads, D)
   void* dv;
   int* status;
@@ -64,13 +66,16 @@ struct BwdArgs {
 // out is a mean of rows of v.  Both factors leave with the results.  (Relative error of dq and dk over sequences of thousands of
 // tokens: 4.1e-4 without, 3.1e-4 with them; the rounding of dS and that of the results are 2.1e-4 each.)  The bound is taken for each
 // sequence by itself, over its queries that see a key: what stands elsewhere must not cost its gradients their digits.
-constexpr int kPShift = 10;
 __device__ __forceinline__ int ds_shift(const float* largest, int sequence) {
-  const float bound = 2.f * sqrtf(largest[2 * sequence]) * sqrtf(largest[2 * sequence + 1]);
+  const float bound = 2.f * sqrtf(largest[kMosts * sequence + kMostDout]) * sqrtf(largest[kMosts * sequence + kMostV]);
   if (!(bound < INFINITY)) return 0;
   const float room = floorf(log2f(60000.f / fmaxf(bound, 1e-30f)));
   return int(fminf(fmaxf(room, -14.f), 14.f));
 }
+// Three fp16 numbers under the weights 2^8, 1 and 2^-8 hold an addend of up to 1.67e7.  In a sequence with a larger one (scores or
+// sums of out * dout of that size before the scale, or a scale below about 1e-6) the addends of the MMA are zeros, and the
+// element-wise warps take lse and delta off in fp32.
+constexpr float kMostAddend = 1.6e7f;
 
 template <int D>
 struct Smem {
@@ -120,6 +125,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   const int live_rows = a.tokens * a.group;                // rows of a step that hold a token
   const int s_begin = a.causal ? min(max(it.seen, 0), it.other_n) / a.tokens : 0, s_end = (it.other_n + a.tokens - 1) / a.tokens;
   const int n_steps = max(s_end - s_begin, 0);
+  const bool wide = !kBf16 && !(a.largest[kMosts * it.sequence + kMostOfAddends] < kMostAddend);
   // The CTAs of one sequence and key head read the same rows and add into the same sums.  They walk from the sequence's end to
   // its front (and wrap around), each one step behind its neighbour: near enough to find the rows in L2, and not on the same
   // lines at the same moment.
@@ -321,8 +327,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const bool keyless = next[e][0] == -INFINITY;
-        c[e][0] = keyless ? 0.f : -(next[e][0] - (kBf16 ? 0.f : float(kPShift))) * inv_mul;
-        c[e][1] = keyless ? 0.f : -next[e][1];
+        c[e][0] = keyless || wide ? 0.f : -(next[e][0] - (kBf16 ? 0.f : float(kPShift))) * inv_mul;
+        c[e][1] = keyless || wide ? 0.f : -next[e][1];
       }
       if (n + 1 < n_steps) fetch(n + 1);
       ok = wait_or_abort(bar(Y_FULL + st), (n / NY) & 1, abort_flag, a.status, 513);
@@ -398,6 +404,16 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     const uint32_t ds_thread = sbase + L::kDs + uint32_t(r) * 128 + (uint32_t(r & 7) << 4);
     float* const acc = a.dq_acc + (int64_t(head) * a.all_steps + it.steps) * (kStep * D) + r * 4;
 
+    // wide: lse or delta of rows lane and lane + 32 of a step
+    auto statistic = [&](const float* x, int n, float (&own)[2]) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = lane + 32 * e, t = row / a.group, token = step_of(n) * a.tokens + t;
+        const bool in = row < live_rows && token < it.other_n;
+        own[e] = in ? x[(int64_t(it.other) + token) * a.heads + head * a.group + (row - t * a.group)] : 0.f;
+      }
+    };
+
     // dQ^T of step j to the sums: [row / 4][d][row % 4] floats, so that a warp's reduction of four rows covers 512 bytes
     auto drain = [&](int j) -> bool {
       if (!wait_or_abort(bar(DQ_FULL + (j & 1)), (j >> 1) & 1, abort_flag, a.status, 516)) return false;
@@ -419,6 +435,9 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       return true;
     };
 
+    // (a loop of its own for `wide`: as conditions inside one they cost the usual case 5 %)
+    auto walk = [&](auto is_wide) {
+    constexpr bool kWide = decltype(is_wide)::value;
     for (int n = grp; n < n_steps && ok; n += 2) {
       const int s = n & 1;
       // keep bits over the step's rows: row c needs a token of the sequence and (causal) one that sees the key
@@ -453,10 +472,21 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
         for (int i = 0; i < kStep / 2; ++i) t[i] = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
       }
+      if constexpr (kWide) {
+        // (p is 1 at most, where lse is so large that its own rounding would say otherwise)
+        float lse[2];
+        statistic(a.lse, n, lse);
+        auto exponent = [&](float x, int row) {
+          const float y = fmaf(x, mul, float(kPShift) - __shfl_sync(0xffffffffu, lse[row >> 5], row & 31));
+          return y > float(kPShift) ? float(kPShift) : y;
+        };
+#pragma unroll
+        for (int i = 0; i < kStep / 2; ++i) t[i] = make_float2(exponent(t[i].x, 2 * i), exponent(t[i].y, 2 * i + 1));
+      }
       uint32_t e1[kStep / 2], e2[kStep / 2];
 #pragma unroll
       for (int c = 0; c < kStep / 2; ++c) {
-        float2 x = __fmul2_rn(t[c], mul2);
+        float2 x = kWide ? t[c] : __fmul2_rn(t[c], mul2);
         if (need_mask) {
           if (!((keep[c >> 4] >> ((2 * c) & 31)) & 1u)) x.x = -INFINITY;
           if (!((keep[c >> 4] >> ((2 * c + 1) & 31)) & 1u)) x.y = -INFINITY;
@@ -488,6 +518,12 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(P_FREE + 2 + s));
+        if constexpr (kWide) {
+          float delta[2];
+          statistic(a.delta, n, delta);
+#pragma unroll
+          for (int c = 0; c < kStep; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) - __shfl_sync(0xffffffffu, delta[c >> 5], c & 31));
+        }
         if (need_mask) {
           // (a dropped key's row of V, or a masked score's dP, may be anything)
 #pragma unroll
@@ -518,6 +554,13 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       if (lane == 0) mbar_arrive(bar(E_READY + s));
       // dQ^T of the previous step (the other group's) is complete by now: add it to the sums
       if (n >= 1) ok = drain(n - 1);
+    }
+    };
+    if constexpr (kBf16) {
+      walk(std::false_type());
+    } else {
+      if (wide) walk(std::true_type());
+      else walk(std::false_type());
     }
     // the last step's dQ^T is drained by the group that did not produce it
     if (ok && n_steps > 0 && grp == (n_steps & 1)) ok = drain(n_steps - 1);
@@ -644,7 +687,7 @@ size_t squares_bytes(const PackedArgs& a, bool bf16) {
   return bf16 ? 0 : up256((size_t(a.tokens_q) * a.heads + size_t(a.tokens_k) * a.kv_heads) * sizeof(float));
 }
 size_t list_bytes(const PackedArgs& a) { return work_list_bytes(most_blocks(a.tokens_k, a.sequences, kTile)); }
-size_t largest_bytes(const PackedArgs& a, bool bf16) { return bf16 ? 0 : up256(size_t(a.sequences) * 2 * sizeof(float)); }      // in front of the sums, cleared with them
+size_t largest_bytes(const PackedArgs& a, bool bf16) { return bf16 ? 0 : up256(size_t(a.sequences) * kMosts * sizeof(float)); }      // in front of the sums, cleared with them
 size_t acc_bytes(const PackedArgs& a) { return size_t(a.kv_heads) * size_t(most_steps(a)) * kStep * a.D * sizeof(float); }
 
 template <int D, bool kBf16>

@@ -622,9 +622,10 @@ bool strides_fit(const void* base, const int64_t (&s)[2], int tokens, int heads)
 
 }  // namespace
 
-// A group's heads of one token have to fit a tile (64 rows in the backward).
+// A group's heads of one token have to fit a tile (64 rows in the backward).  With a scale below 1e-30, 8 / scale (the forward's
+// threshold) and lse / scale (the backward's addend) come near the end of fp32.
 bool tc_packed_supported(const PackedArgs& a, int dtype) {
-  return dtype != NB200_F32 && (a.D == 64 || a.D == 128) && a.group <= 64 && a.scale > 0.f && a.scale < 1e30f &&
+  return dtype != NB200_F32 && (a.D == 64 || a.D == 128) && a.group <= 64 && a.scale > 1e-30f && a.scale < 1e30f &&
          int64_t(a.tokens_q) * a.heads <= 0x7fffffff && int64_t(a.tokens_k) * a.kv_heads <= 0x7fffffff && a.tokens_q > 0 && a.tokens_k > 0 && a.sequences > 0 && strides_fit(a.q, a.qs, a.tokens_q, a.heads) &&
          strides_fit(a.k, a.ks, a.tokens_k, a.kv_heads) && strides_fit(a.v, a.vs, a.tokens_k, a.kv_heads) && aligned16(a.out);
 }

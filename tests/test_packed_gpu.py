@@ -474,3 +474,42 @@ def test_fp16_gradients_beside_large_numbers(D, size):
         for name, got in zip(("dq", "dk", "dv"), grads):
             value, bound = want[name]
             assert float(((got[s].double() - value).abs() - U[torch.float16] * bound).max()) <= 1e-6, (i, name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_where_the_row_statistics_leave_fp16(D):
+    """Scores, sums of out * dout and 1 / scale so large that no few fp16 numbers hold a row's lse / scale or delta: the gradients
+    are as good as elsewhere."""
+    lengths = [150, 20, 300]
+    q, k, v, dout = _inputs(lengths, lengths, 4, 2, D, torch.float16)
+    _check(q, k, v * 0 + 200, dout * 0 + 1000, lengths, lengths)         # delta: 1.3e7 and 2.6e7
+    for scale in (1e-5, 1e-7, 1e-9):
+        _check(q, k, v, dout, lengths, lengths, scale=scale)
+    _check(q * 5000, k * 5000, v, dout, lengths, lengths, scale=1e-8)    # scores of 1e9 before the scale, of 10 after it
+    _check(q * 5000, k * 5000, v, dout, lengths, lengths, scale=1e-8, causal=False)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_equal_scores_of_millions(D):
+    """All scores 2e7 before the scale (1e7 at head dim 64): lse is 1.3e6 to 2.6e6, where fp32 steps by 1/8 and 1/4.  Two roundings
+    of it are a factor of 2^(1/4) in a row's probabilities at most, 0.19 of them."""
+    from nitrix_b200.nn import packed_attention
+
+    lengths = [150, 40]
+    q, k, v, dout = _inputs(lengths, lengths, 4, 2, D, torch.float16)
+    q, k = q * 0 + 400, k * 0 + 400
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed_attention(*leaves, _offsets(lengths))
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = O.packed(q, k, v, lengths, lengths, D ** -0.5, True, dout)
+    for name, got, u in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), (0.0, 0.19, 0.19, 0.19)):
+        value, bound = want[name]
+        assert float(((got.double() - value).abs() - (u + U[torch.float16]) * bound).max()) <= 1e-6, name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_near_the_end_of_fp32(dtype, monkeypatch):
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths = [150, 20]
+    for scale in (1e-25, 1e-34, 2e-38, 1e-38):
+        _check(*_inputs(lengths, lengths, 4, 2, 64, dtype), lengths, lengths, scale=scale)
