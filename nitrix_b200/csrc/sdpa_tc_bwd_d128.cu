@@ -445,11 +445,12 @@ sdpa_bwd_tc_d128_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const float mul = fold_scale ? a.scale * kLog2e : kLog2e;
     const float2 mul2 = make_float2(mul, mul), scale2 = make_float2(a.scale, a.scale);
     const uint32_t* mbits = nullptr;
-    bool key_dropped = false;
+    // (keys past the end: their rows of K and V are zeros, but P is not, and where a row's scores are far below zero it has no bound)
+    bool key_dropped = key >= a.T;
     if (a.mask.rows) {
       if (a.mask_key_only) {
         const uint32_t* krow = a.mask.rows + b * a.mask.b_stride + h * a.mask.h_stride;
-        key_dropped = key >= a.T || !((krow[key >> 5] >> (key & 31)) & 1u);
+        key_dropped = key_dropped || !((krow[key >> 5] >> (key & 31)) & 1u);
       } else {
         mbits = a.mask.cols + b * a.mask.tb_stride + h * a.mask.th_stride + int64_t(min(key, a.T - 1)) * a.mask.tkey_stride;
       }

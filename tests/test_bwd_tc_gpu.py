@@ -45,3 +45,38 @@ def test_gradients_against_fp64(D, dtype, S, T, kind):
     tol = 2e-2 if dtype == torch.bfloat16 else 4e-3
     for name, a, b in zip(("dq", "dk", "dv", "dbias"), got, want):
         assert float((a.double() - b).abs().max()) <= tol * max(1.0, float(b.abs().max())), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,S,T", [(64, 256, 200), (64, 200, 200), (128, 200, 200), (128, 64, 72)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_scores_far_below_zero_beside_padded_keys(dtype, D, S, T, masked):
+    """Every score is about -200, exp2(-lse) beyond fp32: the keys that fill the last tile up must not take part with it.
+
+    P, dS and the results are rounded to the operand type, delta comes from a rounded output: u times the sums that such relative errors
+    multiply, u an ulp's half, doubled for the fp32 parts."""
+    from nitrix_b200.nn import scaled_dot_product_attention
+
+    g = torch.Generator(device="cuda").manual_seed(D)
+    size = (200 / D ** 0.5) ** 0.5
+    q, k = (sign * size + 0.1 * torch.randn(2, 3, n, D, generator=g, device="cuda") for sign, n in ((1, S), (-1, T)))
+    v, dout = (torch.randn(2, 3, n, D, generator=g, device="cuda") for n in (T, S))
+    q, k, v, dout = (t.to(dtype) for t in (q, k, v, dout))
+    mask = None
+    if masked:
+        mask = torch.rand(2, 1, S, T, device="cuda", generator=g) > 0.3
+        mask[..., 0] = True
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = scaled_dot_product_attention(*leaves, mask=mask)
+    got = torch.autograd.grad(out, leaves, dout)
+    qd, kd, vd, dd = (t.double() for t in (q, k, v, dout))
+    s = qd @ kd.transpose(-1, -2) * D ** -0.5
+    assert float(s.max()) < -150
+    p = torch.softmax(s if mask is None else s.masked_fill(~mask, float("-inf")), -1)
+    o = p @ vd
+    ds = p * (dd @ vd.transpose(-1, -2) - (dd * o).sum(-1, keepdim=True)) * D ** -0.5
+    err = ds.abs() + p * (dd * o).abs().sum(-1, keepdim=True) * D ** -0.5
+    want = ds @ kd, ds.transpose(-1, -2) @ qd, p.transpose(-1, -2) @ dd
+    sums = err @ kd.abs(), err.transpose(-1, -2) @ qd.abs(), p.transpose(-1, -2) @ dd.abs()
+    for name, a, b, c in zip(("dq", "dk", "dv"), got, want, sums):
+        assert float(((a.double() - b).abs() - torch.finfo(dtype).eps * (c + b.abs())).max()) <= 1e-6, name
