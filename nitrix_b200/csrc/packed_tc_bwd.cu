@@ -72,10 +72,8 @@ __device__ __forceinline__ int ds_shift(const float* largest, int sequence) {
   const float room = floorf(log2f(60000.f / fmaxf(bound, 1e-30f)));
   return int(fminf(fmaxf(room, -14.f), 14.f));
 }
-// Three fp16 numbers under the weights 2^8, 1 and 2^-8 hold an addend of up to 1.67e7.  In a sequence with a larger one (scores or
-// sums of out * dout of that size before the scale, or a scale below about 1e-6) the addends of the MMA are zeros, and the
-// element-wise warps take lse and delta off in fp32.
-constexpr float kMostAddend = 1.6e7f;
+// In a sequence with an addend that its fp16 numbers do not hold (scores or sums of out * dout of kRowAddendMost before the scale, or a
+// scale below 1e-8) the addends of the MMA are zeros, and the element-wise warps take lse and delta off in fp32.
 
 template <int D>
 struct Smem {
@@ -125,7 +123,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   const int live_rows = a.tokens * a.group;                // rows of a step that hold a token
   const int s_begin = a.causal ? min(max(it.seen, 0), it.other_n) / a.tokens : 0, s_end = (it.other_n + a.tokens - 1) / a.tokens;
   const int n_steps = max(s_end - s_begin, 0);
-  const bool wide = !kBf16 && !(a.largest[kMosts * it.sequence + kMostOfAddends] < kMostAddend);
+  const bool wide = !kBf16 && !(a.largest[kMosts * it.sequence + kMostOfAddends] < kRowAddendMost);
   // The CTAs of one sequence and key head read the same rows and add into the same sums.  They walk from the sequence's end to
   // its front (and wrap around), each one step behind its neighbour: near enough to find the rows in L2, and not on the same
   // lines at the same moment.
@@ -172,13 +170,9 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     for (int n = 0; n < min(n_steps, NY); ++n) load_step(n);
   }
   {
-    // weight rows (w0, w1, w2, 0, ...): a query's addend is sum_j w_j c_j with c_j 16-bit; bf16 has fp32's range, so
-    // three unit weights give 24 bits; fp16 spreads the terms over 2^8, 1, 2^-8
     uint4* wt = reinterpret_cast<uint4*>(smem + L::kWeights);
-    const uint32_t w01 = kBf16 ? 0x3F803F80u : 0x3C005C00u;
-    const uint32_t w2 = kBf16 ? 0x00003F80u : 0x00001C00u;
     for (int idx = threadIdx.x; idx < L::kWeightBytes / 16; idx += kThreads)
-      wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(w01, w2, 0, 0);
+      wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : row_addend_weights<kBf16>();
     uint4* aug = reinterpret_cast<uint4*>(smem + L::kAug);
     for (int idx = threadIdx.x; idx < 2 * L::kAugSlotBytes / 16; idx += kThreads) aug[idx] = make_uint4(0, 0, 0, 0);
     // rows of the ring that no load fills (the group is no divisor of 64)
@@ -357,26 +351,7 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         const int q = lane + 32 * e;
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
-          float rem = c[e][tile];
-          uint32_t hh[3];
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            const float w = kBf16 ? 1.f : (j == 0 ? 256.f : (j == 1 ? 1.f : 0.00390625f));
-            const float v = rem * (1.f / w);
-            float back;
-            if constexpr (kBf16) {
-              const __nv_bfloat16 hv = __float2bfloat16_rn(v);
-              hh[j] = __bfloat16_as_ushort(hv);
-              back = __bfloat162float(hv);
-            } else {
-              const __half hv = __float2half_rn(v);
-              hh[j] = __half_as_ushort(hv);
-              back = __half2float(hv);
-            }
-            rem = fmaf(-back, w, rem);
-          }
-          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) =
-              make_uint4(hh[0] | (hh[1] << 16), hh[2], 0u, 0u);
+          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) = row_addend<kBf16>(c[e][tile]);
         }
       }
       fence_proxy_async_smem();

@@ -209,13 +209,12 @@ sdpa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_const
   }
   if (kKeyMajor || a.key_aug) {
     {
-      // weight rows (w0, w1, w2, 0, ...): a query's addend is sum_j w_j c_j with c_j 16-bit; bf16 has fp32's range,
-      // so three unit weights give 24 bits; fp16 spreads the terms over 2^8, 1, 2^-8 to cover magnitudes up to 1.6e7
+      // weight rows (w0, w1, w2, 0, ...) of the addends: of queries (row_addend) in the key-major kernel; of keys, the biases,
+      // in the query-major one: sum_j w_j c_j as well, where fp16 spreads the terms over 2^8, 1, 2^-8
       uint4* wt = reinterpret_cast<uint4*>(smem + L::kWeights);
-      const uint32_t w01 = kBf16 ? 0x3F803F80u : 0x3C005C00u;   // (w0, w1): bf16 (1, 1); fp16 (256, 1)
-      const uint32_t w2 = kBf16 ? 0x00003F80u : 0x00001C00u;    // (w2, 0):  bf16 1; fp16 2^-8
+      const uint4 w = kKeyMajor || kBf16 ? row_addend_weights<kBf16>() : make_uint4(0x3C005C00u, 0x00001C00u, 0, 0);
       for (int idx = threadIdx.x; idx < L::kWeightBytes / 16; idx += kThreads)
-        wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(w01, w2, 0, 0);
+        wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : w;
       uint4* aug = reinterpret_cast<uint4*>(smem + L::kAug);
       for (int idx = threadIdx.x; idx < kAugSlots * L::kAugSlotBytes / 16; idx += kThreads) aug[idx] = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
@@ -526,27 +525,7 @@ sdpa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_const
         const float c[2] = {live ? -ld[q] * inv_mul : 0.f, live ? -ld[kStep + q] : 0.f};
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
-          // c = w0 c0 + w1 c1 + w2 c2 with the remainder carried in fp32
-          float rem = c[tile];
-          uint32_t h[3];
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            const float w = kBf16 ? 1.f : (j == 0 ? 256.f : (j == 1 ? 1.f : 0.00390625f));
-            const float v = rem * (1.f / w);
-            float back;
-            if constexpr (kBf16) {
-              const __nv_bfloat16 hv = __float2bfloat16_rn(v);
-              h[j] = __bfloat16_as_ushort(hv);
-              back = __bfloat162float(hv);
-            } else {
-              const __half hv = __float2half_rn(v);
-              h[j] = __half_as_ushort(hv);
-              back = __half2float(hv);
-            }
-            rem = fmaf(-back, w, rem);
-          }
-          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) =
-              make_uint4(h[0] | (h[1] << 16), h[2], 0u, 0u);
+          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) = row_addend<kBf16>(c[tile]);
         }
       }
       fence_proxy_async_smem();
@@ -1002,6 +981,11 @@ bool bwd_supported(const Problem& pr, int dtype, int bias_dtype, const char** wh
   // forward coverage (dtype, head dims, lengths, q/k/v/bias layout) was checked by the caller
   if (pr.scale == 0.f || !isfinite(1.f / pr.scale) || !isfinite(pr.scale)) {
     *why = "scale is zero or not finite";   // the key-major kernel divides lse by scale
+    return false;
+  }
+  // (lse is log2 of the number of keys at least, 31 at most; the end of fp32 is as near for bf16 at 1e-30)
+  if (fabsf(pr.scale) < (dtype == NB200_F16 ? 2e-8f : 1e-30f)) {
+    *why = "lse over a scale this small has no place in the addends of the tensor cores";
     return false;
   }
   if (pr.mask_packed == 1 && !mask_key_only(pr)) {

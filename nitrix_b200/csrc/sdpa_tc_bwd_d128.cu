@@ -161,13 +161,9 @@ sdpa_bwd_tc_d128_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     }
   }
   {
-    // weight rows (w0, w1, w2, 0, ...): a query's addend is sum_j w_j c_j with c_j 16-bit; bf16 has fp32's range, so
-    // three unit weights give 24 bits; fp16 spreads the terms over 2^8, 1, 2^-8
     uint4* wt = reinterpret_cast<uint4*>(smem + L::kWeights);
-    const uint32_t w01 = kBf16 ? 0x3F803F80u : 0x3C005C00u;
-    const uint32_t w2 = kBf16 ? 0x00003F80u : 0x00001C00u;
     for (int idx = threadIdx.x; idx < L::kWeightBytes / 16; idx += kThreads)
-      wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(w01, w2, 0, 0);
+      wt[idx] = (idx & 8) ? make_uint4(0, 0, 0, 0) : row_addend_weights<kBf16>();
     uint4* aug = reinterpret_cast<uint4*>(smem + L::kAug);
     for (int idx = threadIdx.x; idx < 2 * L::kAugSlotBytes / 16; idx += kThreads) aug[idx] = make_uint4(0, 0, 0, 0);
     if (kTileBias) {
@@ -404,26 +400,7 @@ sdpa_bwd_tc_d128_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const float c[2] = {live ? -ld[q] * inv_mul : 0.f, live ? -ld[kStep + q] : 0.f};
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
-          float rem = c[tile];
-          uint32_t hh[3];
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            const float w = kBf16 ? 1.f : (j == 0 ? 256.f : (j == 1 ? 1.f : 0.00390625f));
-            const float v = rem * (1.f / w);
-            float back;
-            if constexpr (kBf16) {
-              const __nv_bfloat16 hv = __float2bfloat16_rn(v);
-              hh[j] = __bfloat16_as_ushort(hv);
-              back = __bfloat162float(hv);
-            } else {
-              const __half hv = __float2half_rn(v);
-              hh[j] = __half_as_ushort(hv);
-              back = __half2float(hv);
-            }
-            rem = fmaf(-back, w, rem);
-          }
-          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) =
-              make_uint4(hh[0] | (hh[1] << 16), hh[2], 0u, 0u);
+          *reinterpret_cast<uint4*>(slot + tile * L::kAugTileBytes + (q >> 3) * 256 + (q & 7) * 16) = row_addend<kBf16>(c[tile]);
         }
       }
       fence_proxy_async_smem();

@@ -114,6 +114,36 @@ int stage_out(const Problem& pr, const Problem& staged, const Staging& sg, cudaS
 // ---- device helpers -----------------------------------------------------------
 #ifdef __CUDACC__
 
+// A row statistic (lse over scale log2 e, or delta) is added to a product by one K = 16 MMA step as w0 c0 + w1 c1 + w2 c2 with 16-bit
+// c_j.  bf16 has fp32's range, so that three unit weights give 24 bits; fp16 has the weights 2^15, 2^4 and 2^-7, eleven bits apart:
+// whatever its size up to kRowAddendMost, the sum is within 2^-24 of it or 2^-31.
+constexpr float kRowAddendMost = 2.1e9f;      // fp16: 65504 * 2^15 is 2.15e9
+template <bool kBf16>
+__device__ __forceinline__ uint4 row_addend_weights() {
+  return kBf16 ? make_uint4(0x3F803F80u, 0x00003F80u, 0, 0) : make_uint4(0x4C007800u, 0x00002000u, 0, 0);
+}
+template <bool kBf16>
+__device__ __forceinline__ uint4 row_addend(float c) {
+  uint32_t h[3];
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    const float w = kBf16 ? 1.f : (j == 0 ? 32768.f : (j == 1 ? 16.f : 0.0078125f));
+    const float v = c * (1.f / w);
+    float back;
+    if constexpr (kBf16) {
+      const __nv_bfloat16 hv = __float2bfloat16_rn(v);
+      h[j] = __bfloat16_as_ushort(hv);
+      back = __bfloat162float(hv);
+    } else {
+      const __half hv = __float2half_rn(v);
+      h[j] = __half_as_ushort(hv);
+      back = __half2float(hv);
+    }
+    c = fmaf(-back, w, c);
+  }
+  return make_uint4(h[0] | (h[1] << 16), h[2], 0u, 0u);
+}
+
 constexpr uint32_t kWaitHintNs = 16384;         // a waiting thread may sleep this long per try_wait before it re-checks
 constexpr long long kWaitCycles = 400000000LL;  // ~0.2 s of SM clock: far beyond any real wait (microseconds)
 
