@@ -193,12 +193,23 @@ struct MmaLoop {
         for (int i = 0; i < D / 32; ++i) kf[r][i] = sm100::ldg_no_allocate(row + i * 4 + t);
       }
     };
+    // (zeros behind the last token: another's value there would be multiplied by a probability of zero, which an infinity survives)
     auto load_v = [&](int b, int page) {
+      if (b + kBlock <= t1) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint4* row = row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8));
+        for (int r = 0; r < 4; ++r) {
+          const uint4* row = row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8));
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) vf[r][i] = sm100::ldg_no_allocate(row + i * 8 + g);
+          for (int i = 0; i < D / 64; ++i) vf[r][i] = sm100::ldg_no_allocate(row + i * 8 + g);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int token = b + 2 * t + (r & 1) + (r >> 1) * 8;
+          const uint4* row = row_of(vbase, a.vs, place(b, page, token));
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) vf[r][i] = token <= last ? sm100::ldg_no_allocate(row + i * 8 + g) : make_uint4(0, 0, 0, 0);
+        }
       }
     };
     int b0 = t0 + wi * kBlock;
@@ -356,24 +367,28 @@ struct FmaLoop {
     const int last = t1 - 1;
     uint4 kw[kAhead][kPer], vw[kAhead][kPer];
     Where at[kAhead];       // of the tokens whose keys were asked for last
-    auto load = [&](uint4 (&w)[kAhead][kPer], const uint4* base, const int (&stride)[3]) {
+    auto load = [&](uint4 (&w)[kAhead][kPer], const uint4* base, const int (&stride)[3], auto wanted) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const uint4* row = row_of(base, stride, at[j]);
 #pragma unroll
-        for (int p = 0; p < kPer; ++p) w[j][p] = c + p * kLanes < words ? __ldg(row + c + p * kLanes) : make_uint4(0, 0, 0, 0);
+        for (int p = 0; p < kPer; ++p) w[j][p] = c + p * kLanes < words && wanted(j) ? __ldg(row + c + p * kLanes) : make_uint4(0, 0, 0, 0);
       }
     };
     auto load_k = [&](int b) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) at[j] = where(a, row_table, min(b + group + j * groups, last));
-      load(kw, kbase, a.ks);
+      load(kw, kbase, a.ks, [](int) { return true; });
+    };
+    // (zeros behind the last token: another's value there would be multiplied by a probability of zero, which an infinity survives)
+    auto load_v = [&](int b) {
+      load(vw, vbase, a.vs, [&](int j) { return b + group + j * groups <= last; });
     };
     // (every group of a warp makes as many turns as its first, which has the most: the shuffles below are warp-wide)
     int b = t0;
     if (b + first >= t1) return;
     load_k(b);
-    load(vw, vbase, a.vs);
+    load_v(b);
     for (; b + first < t1; b += groups * kAhead) {
       const int next = b + groups * kAhead;
       float x[kAhead];
@@ -450,7 +465,7 @@ struct FmaLoop {
           }
         }
       }
-      if (next + first < t1) load(vw, vbase, a.vs);
+      if (next + first < t1) load_v(next);
     }
   }
   __device__ __forceinline__ void store(const DecodeArgs& a, float* dst) const {

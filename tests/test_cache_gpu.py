@@ -422,3 +422,24 @@ def test_refusals_of_pages():
         for call in (lambda c: cache_append(c, k[:, :empty.shape[1]], k[:, :empty.shape[1]], offsets), *calls[1:]):
             with pytest.raises(ValueError, match="a token at least"):
                 call(cache._replace(k_pages=empty, v_pages=empty))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 80, 256])
+@pytest.mark.parametrize("G", [1, 4, 16])
+def test_decode_an_infinity_in_the_last_value(dtype, D, G):
+    """It reaches the element it stands in, as an infinity, and no other."""
+    from nitrix_b200.nn import decode_attention
+
+    lengths = [1, 5, 16, 33, 100, 700]
+    cache = _cache_of(lengths, 16, 2, D, dtype, seed=D + G)
+    q = torch.randn(len(lengths), 2 * G, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    want, bound = O.decode(q, cache.k_pages, cache.v_pages, cache.table, lengths, D ** -0.5)
+    for i, n in enumerate(lengths):
+        page, slot = cache.table[i, (n - 1) // 16].long(), (n - 1) % 16
+        cache.v_pages[page, :, slot, 3] = float("inf")
+        cache.v_pages[page, :, slot, 17] = -float("inf")
+    got = decode_attention(q, cache).double()
+    assert bool((got[..., 3] == float("inf")).all()) and bool((got[..., 17] == -float("inf")).all())
+    rest = [d for d in range(D) if d not in (3, 17)]
+    assert float(((got - want).abs() - U[dtype] * bound)[..., rest].max()) <= 1e-7
