@@ -19,7 +19,8 @@
  * those in use.  Pages are written in place, but only slots that are free in the state that the call is given; the old
  * arrays therefore describe a valid cache until the next call that writes pages.  Where pages run out (or a row of `table`
  * is full), tokens are dropped from the end of the sequences that got none, lengths say what is stored, and `shortfall`
- * counts the dropped tokens: nothing is reported on the host, which does not wait.
+ * counts the dropped tokens: nothing is reported on the host, which does not wait.  Offsets that leave the new tokens are cut
+ * to them, and what a sequence misses by that counts as dropped; offsets that descend store nothing, and all tokens count.
  *
  * Every pointer is a device pointer; all work is enqueued on the caller's stream; nothing is allocated.
  */

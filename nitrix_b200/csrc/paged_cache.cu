@@ -47,12 +47,15 @@ struct AppendArgs {
 };
 
 struct RowPlan {
-  int held, want, have, need;   // tokens held and asked for, pages held and asked for
+  int held, want, have, need;   // tokens held and to be held, pages held and asked for
 };
+
+// Offsets that leave the tokens are cut to them.
+__device__ __forceinline__ int first_of(const AppendArgs& a, int row) { return int(min(int64_t(max(a.offsets[row], 0)), a.tokens)); }
 
 __device__ __forceinline__ RowPlan plan_row(const AppendArgs& a, int row) {
   RowPlan r;
-  const int lo = a.offsets[row], hi = a.offsets[row + 1];
+  const int lo = first_of(a, row), hi = first_of(a, row + 1);
   r.held = int(min(int64_t(max(a.lengths[row], 0)), int64_t(a.width) * a.p.page_size));
   r.want = int(min(int64_t(r.held) + max(hi - lo, 0), int64_t(0x7fffffff)));
   r.have = int((int64_t(r.held) + a.p.page_size - 1) / a.p.page_size);
@@ -84,11 +87,16 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
     __shared__ int64_t part[kThreads / 32];
     __shared__ unsigned long long dropped;
     if (threadIdx.x == 0) dropped = 0;
+    // (offsets that descend name no row's tokens: every row keeps what it holds, as the other CTAs store nothing)
+    bool descend = false;
+    for (int row = threadIdx.x; row < a.rows; row += kThreads) descend = descend || a.offsets[row] > a.offsets[row + 1];
+    descend = __syncthreads_or(descend);
     int64_t before = 0;
     for (int row0 = 0; row0 < a.rows; row0 += kThreads) {
       const int row = row0 + threadIdx.x;
       RowPlan r{0, 0, 0, 0};
       if (row < a.rows) r = plan_row(a, row);
+      if (descend) r = RowPlan{r.held, r.held, r.have, 0};
       int64_t upto = r.need;      // inclusive sum over the warp, then over the warps before
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -106,7 +114,8 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
       if (row < a.rows) {
         const int kept = tokens_kept(r, pages_got(r, avail, before + upto - r.need), a.p.page_size);
         a.new_lengths[row] = kept;
-        if (r.want > kept) atomicAdd(&dropped, static_cast<unsigned long long>(r.want - kept));
+        const int64_t asked = descend ? 0 : int64_t(a.offsets[row + 1]) - a.offsets[row], stored = max(kept - r.held, 0);
+        if (asked > stored) atomicAdd(&dropped, static_cast<unsigned long long>(asked - stored));
       }
       before += total;
     }
@@ -114,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
     if (threadIdx.x == 0) {
       a.new_free_range[0] = begin + int(min(before, avail));
       a.new_free_range[1] = end;
-      *a.shortfall = int(min(dropped, 0x7fffffffull));
+      *a.shortfall = int(min(descend ? static_cast<unsigned long long>(a.tokens) : dropped, 0x7fffffffull));
     }
     return;
   }
@@ -127,7 +136,9 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
       // the token's sequence, and the pages that those before it take
       int count = 0;
       int64_t need = 0;
+      bool descend = false;
       for (int i = lane; i < a.rows; i += 32) {
+        descend = descend || a.offsets[i] > a.offsets[i + 1];
         if (int64_t(a.offsets[i + 1]) <= t) {
           ++count;
           need += plan_row(a, i).need;
@@ -139,9 +150,9 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
         need += __shfl_xor_sync(0xffffffffu, need, o);
       }
       row = count;
-      if (row >= a.rows) return;     // (tokens behind the last offset)
+      if (row >= a.rows || __any_sync(0xffffffffu, descend)) return;     // (tokens behind the last offset)
       r = plan_row(a, row);
-      first = a.offsets[row];
+      first = first_of(a, row);
       next = a.offsets[row + 1];
       got = pages_got(r, avail, need);
       before = int(min(need, avail));

@@ -48,8 +48,9 @@ def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, seq
 def cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, *, backend: str = "auto") -> PagedCache:
     """The cache with tokens ``offsets[i] .. offsets[i + 1]`` of ``k`` and ``v`` ``(tokens, key heads, head dim)`` behind those
     of sequence ``i``; ``offsets`` is int32 ``(sequences + 1,)``.  New pages go to the sequences in order.  Tokens for which
-    there is no page (or no room in the table) are dropped from the end of a sequence and counted in ``shortfall``.  The cache
-    holds values: no gradient flows back through it."""
+    there is no page (or no room in the table) are dropped from the end of a sequence and counted in ``shortfall``, as are those
+    that offsets name beyond ``k`` and ``v``; offsets that descend store nothing.  The cache holds values: no gradient flows back
+    through it."""
     resolve_backend(backend)
     lengths, free_range, shortfall = _cabi.torch_ops().cache_append(*cache[:6], k, v, offsets)
     return cache._replace(lengths=lengths, free_range=free_range, shortfall=shortfall)

@@ -443,3 +443,30 @@ def test_decode_an_infinity_in_the_last_value(dtype, D, G):
     assert bool((got[..., 3] == float("inf")).all()) and bool((got[..., 17] == -float("inf")).all())
     rest = [d for d in range(D) if d not in (3, 17)]
     assert float(((got - want).abs() - U[dtype] * bound)[..., rest].max()) <= 1e-7
+
+
+def test_offsets_that_leave_the_new_tokens():
+    """Offsets that end behind ``k`` and ``v``, begin before them or descend: lengths and pages are those of what was stored."""
+    from nitrix_b200.nn import cache_append
+
+    def start():
+        pair = Pair(20, 4, 3, 4)
+        pair.append([5, 6, 7])
+        return pair
+
+    tokens = [100, 101, 102, 103, 104, 105]
+    k = torch.tensor(tokens, dtype=torch.float32, device="cuda")[:, None, None].expand(6, 2, 8) + 0
+    for offsets, stored, missing in (([0, 2, 4, 9], [tokens[:2], tokens[2:4], tokens[4:]], 3),
+                                     ([0, 2, 40, 50], [tokens[:2], tokens[2:], []], 44),
+                                     ([-4, 1, 2, 3], [tokens[:1], tokens[1:2], tokens[2:3]], 4),
+                                     ([7, 8, 9, 2 ** 31 - 1], [[], [], []], 2 ** 31 - 8),
+                                     ([0, 9, 2, 6], [[], [], []], 6),
+                                     ([3, 2, 2, 1], [[], [], []], 6)):
+        pair = start()
+        pages = pair.cache.k_pages.clone()
+        pair.cache = cache_append(pair.cache, k, -k, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+        pair.model.append(stored)
+        pair.model.shortfall += missing
+        pair.check()
+        if not any(stored):
+            assert torch.equal(pair.cache.k_pages.nan_to_num(-1.0), pages.nan_to_num(-1.0))
