@@ -33,6 +33,9 @@
 extern "C" {
 #endif
 
+/* Tokens that a sequence counts at most: places a few blocks behind its end still fit 32 bits. */
+#define NB200_CACHE_MOST_TOKENS 0x7fffff00
+
 typedef struct nb200_cache_pages {
   void* k;
   void* v;

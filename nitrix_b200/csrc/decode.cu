@@ -59,7 +59,7 @@ struct DecodeArgs {
 };
 
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int row) {
-  return int(min(int64_t(max(a.lengths[row], 0)), int64_t(a.width) * a.page_size));
+  return int(min(int64_t(min(max(a.lengths[row], 0), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.page_size));
 }
 __device__ __forceinline__ int units_of(const DecodeArgs& a, int row) { return (length_of(a, row) + a.unit - 1) / a.unit; }
 

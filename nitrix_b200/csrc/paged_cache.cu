@@ -56,8 +56,8 @@ __device__ __forceinline__ int first_of(const AppendArgs& a, int row) { return i
 __device__ __forceinline__ RowPlan plan_row(const AppendArgs& a, int row) {
   RowPlan r;
   const int lo = first_of(a, row), hi = first_of(a, row + 1);
-  r.held = int(min(int64_t(max(a.lengths[row], 0)), int64_t(a.width) * a.p.page_size));
-  r.want = int(min(int64_t(r.held) + max(hi - lo, 0), int64_t(0x7fffffff)));
+  r.held = int(min(int64_t(min(max(a.lengths[row], 0), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.p.page_size));
+  r.want = int(min(int64_t(r.held) + max(hi - lo, 0), int64_t(NB200_CACHE_MOST_TOKENS)));
   r.have = int((int64_t(r.held) + a.p.page_size - 1) / a.p.page_size);
   const int pages = int((int64_t(r.want) + a.p.page_size - 1) / a.p.page_size);
   r.need = max(min(pages, a.width) - r.have, 0);

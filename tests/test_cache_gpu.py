@@ -470,3 +470,23 @@ def test_offsets_that_leave_the_new_tokens():
         pair.check()
         if not any(stored):
             assert torch.equal(pair.cache.k_pages.nan_to_num(-1.0), pages.nan_to_num(-1.0))
+
+
+def test_lengths_at_the_end_of_32_bits():
+    """A table of one page many times over: 2^31 tokens and more.  A sequence counts 2^31 - 256 of them at most."""
+    from nitrix_b200.nn import PagedCache, cache_append, decode_attention
+
+    page, most = 1 << 16, 2 ** 31 - 256
+    ints = dict(dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, (1 << 15) + 4, **ints)
+    z = torch.zeros(1, **ints)
+    for dtype, D in ((torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 80)):
+        k = torch.zeros(1, 1, page, D, dtype=dtype, device="cuda")
+        v = torch.full_like(k, 3.0)
+        for n in (2 ** 31 - 1, most, most - 63):
+            cache = PagedCache(k, v, table, torch.tensor([n], **ints), z, torch.zeros(2, **ints), z)
+            out = decode_attention(torch.ones(1, 1, D, dtype=dtype, device="cuda"), cache)
+            assert bool(((out - 3).abs() < 0.02).all())
+    more = torch.zeros(4, 1, 80, dtype=torch.bfloat16, device="cuda")
+    cache = cache_append(cache._replace(lengths=torch.tensor([most - 3], **ints)), more, more, torch.tensor([0, 4], **ints))
+    assert cache.lengths.tolist() == [most] and cache.shortfall.tolist() == [1]
