@@ -306,6 +306,7 @@ bool operands_fit(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe
 using AttentionResult = std::tuple<MaybeTensor, MaybeTensor, bool>;
 AttentionResult attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& bias, const MaybeTensor& mask,
                           double scale, bool causal, int64_t kernel, bool any_family) {
+  refuse_tangents("scaled_dot_product_attention", q, k, v, bias);
   if (!operands_fit(q, k, v, bias, mask)) return {std::nullopt, std::nullopt, false};
   const c10::cuda::CUDAGuard guard(q.device());
   const Attention a{q, k, v, bias.value_or(Tensor()), mask.value_or(Tensor()), Tensor(), scale, causal, int(kernel), {}};
@@ -316,7 +317,6 @@ AttentionResult attention(const Tensor& q, const Tensor& k, const Tensor& v, con
   }
   if (c10::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || v.requires_grad() || (bias && bias->requires_grad()))) {
-    refuse_tangents("scaled_dot_product_attention", q, k, v, bias);
     tensor_list r = AttentionRule::apply(q, k, v, bias, mask, scale, causal, kernel, family == NB200_KERNEL_TCGEN05);
     return {r[0], r[1], true};
   }
@@ -684,9 +684,9 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
                       " + (heads, ", D, "); got ", k->sizes());
   }
   TORCH_CHECK_VALUE(!positions.requires_grad() && !frequencies.requires_grad(), what, ": positions and frequencies are not differentiable");
+  refuse_tangents(what, q, k, positions, frequencies);
   const Tensor pos = positions.contiguous(), freq = frequencies.contiguous();
   if (c10::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
-    refuse_tangents(what, q, k);
     const tensor_list r = RotaryRule::apply(q, k, pos, freq, sections, interleaved);
     return {r[0], k ? MaybeTensor(r[1]) : std::nullopt};
   }
@@ -772,6 +772,7 @@ std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Ten
   }
   check_ints(what, "offsets", offsets, k_pages, 1);
   TORCH_CHECK_VALUE(table.size(0) > 0 && offsets.size(0) == table.size(0) + 1, what, ": ", table.size(0), " rows, but offsets of shape ", offsets.sizes());
+  refuse_tangents(what, k, v, k_pages, v_pages);
   const Tensor kr = aligned_rows(k), vr = aligned_rows(v), off = offsets.contiguous();
   const Tensor new_lengths = c.ints(table.size(0)), new_range = c.ints(2), shortfall = c.ints(1);
   c.p.new_k = kr.data_ptr();
@@ -849,6 +850,7 @@ Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
   TORCH_CHECK_VALUE(lengths.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths.sizes());
   TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad())), what,
                               " is not differentiable; packed_attention is");
+  refuse_tangents(what, q, k_pages, v_pages);
   const Tensor qr = aligned_rows(q), tab = table.contiguous(), len = lengths.contiguous();
   const Tensor out = at::empty(q.sizes(), q.options());
   p.table = tab.data_ptr<int32_t>();
@@ -975,11 +977,11 @@ MaybeTensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, 
   } else {
     TORCH_CHECK_VALUE(k.size(0) == q.size(0), what, ": ", q.size(0), " queries and ", k.size(0), " keys need offsets_k");
   }
+  refuse_tangents(what, q, k, v);
   const Tensor oq = offsets.contiguous(), ok = offsets_k ? offsets_k->contiguous() : oq;
   const Packed a{aligned_rows(q), aligned_rows(k), aligned_rows(v), oq, ok, scale, causal, int(kernel)};
   if (kernel == NB200_KERNEL_AUTO && !any_family && a.plan(NB200_PASS_FWD) != NB200_KERNEL_TCGEN05) return std::nullopt;
   if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
-    refuse_tangents(what, q, k, v);
     return PackedRule::apply(a.q, a.k, a.v, oq, ok, scale, causal, kernel);
   }
   return a.forward().first;
