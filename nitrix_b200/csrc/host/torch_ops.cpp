@@ -716,6 +716,14 @@ nb200_cache_pages cache_pages(const char* what, const Tensor& k_pages, const Ten
   return c;
 }
 
+// Raises the version of what a call has written in place, by which autograd notices that a saved tensor is no longer what it was.
+// (Inference tensors have none.)
+template <typename... T>
+void written(const T&... tensors) {
+  for (const Tensor* t : {&tensors...})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 struct CacheCall {
   nb200_cache_params p{};
   Tensor lengths, free_pages, free_range;
@@ -784,6 +792,7 @@ std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Ten
   c.p.new_free_range = new_range.data_ptr<int32_t>();
   c.p.shortfall = shortfall.data_ptr<int32_t>();
   check(lib.nb200_cache_append(&c.p, stream_of(k_pages)), "nb200_cache_append");
+  if (k.size(0) > 0) written(k_pages, v_pages, table);
   return {new_lengths, new_range, shortfall};
 }
 
@@ -814,6 +823,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pa
   c.p.shortfall = shortfall.data_ptr<int32_t>();
   const Tensor ws = c.workspace();
   check(lib.nb200_cache_fork(&c.p, stream_of(k_pages)), "nb200_cache_fork");
+  if (!finished) written(k_pages, v_pages);      // (rows that stay, or become empty, copy nothing)
   return {new_table, new_lengths, new_free, new_range, shortfall};
 }
 
@@ -831,6 +841,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, 
   c.p.shortfall = shortfall.data_ptr<int32_t>();
   const Tensor ws = c.workspace();
   check(lib.nb200_cache_compact(&c.p, stream_of(k_pages)), "nb200_cache_compact");
+  written(k_pages, v_pages);
   return {new_table, new_free, new_range, shortfall};
 }
 

@@ -490,3 +490,32 @@ def test_lengths_at_the_end_of_32_bits():
     more = torch.zeros(4, 1, 80, dtype=torch.bfloat16, device="cuda")
     cache = cache_append(cache._replace(lengths=torch.tensor([most - 3], **ints)), more, more, torch.tensor([0, 4], **ints))
     assert cache.lengths.tolist() == [most] and cache.shortfall.tolist() == [1]
+
+
+def test_autograd_notices_that_pages_are_written():
+    """The calls write their pools in place: a graph that has saved one is told so, as by torch's own in-place operations."""
+    from nitrix_b200.nn import cache_append, cache_compact, cache_fork, cache_free, paged_cache
+
+    cache = paged_cache(16, 4, 2, 64, sequences=3, max_length=16, dtype=torch.float32)
+    k = torch.randn(6, 2, 64, device="cuda")
+    offsets = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda")
+    calls = {"append": lambda c: cache_append(c, k, k, offsets),
+             "fork": lambda c: cache_fork(c, torch.tensor([0, 0, 2], dtype=torch.int32, device="cuda")),
+             "free": lambda c: cache_free(c, torch.tensor([True, False, False], device="cuda")), "compact": cache_compact}
+    for name, call in calls.items():
+        before = cache.k_pages._version, cache.v_pages._version, cache.table._version
+        w = torch.ones((), device="cuda", requires_grad=True)
+        y = (cache.k_pages * w).sum()
+        after = call(cache)
+        if name == "free":      # (which writes no page)
+            y.backward()
+        else:
+            assert cache.k_pages._version > before[0] and cache.v_pages._version > before[1]
+            assert (cache.table._version > before[2]) == (name == "append")
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward()
+        cache = after
+    with torch.inference_mode():
+        inside = paged_cache(16, 4, 2, 64, sequences=3, max_length=16, dtype=torch.float32)
+        inside = cache_append(inside, k, k, offsets)
+    assert cache_append(inside, k, k, offsets).lengths.tolist() == [4, 4, 4]      # (such tensors have no version)
