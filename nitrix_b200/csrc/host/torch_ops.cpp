@@ -906,7 +906,9 @@ struct Packed {
     return p;
   }
   int plan(int pass) const {
-    const nb200_packed_params p = params();
+    nb200_packed_params p = params();
+    p.dout_stride[0] = q.size(1) * q.size(2);      // (a cotangent is brought into rows that fit)
+    p.dout_stride[1] = q.size(2);
     int chosen = 0;
     check(lib.nb200_packed_plan(&p, pass, &chosen), "nb200_packed_plan");
     return chosen;
@@ -967,8 +969,9 @@ struct PackedRule : torch::autograd::Function<PackedRule> {
   }
 };
 
-// Nothing where the problem leaves the tensor-core family and the caller has not allowed that.
-MaybeTensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const MaybeTensor& offsets_k, double scale,
+// Without a tensor where the problem leaves the tensor-core family and the caller has not allowed that; whether it does so with its
+// gradients only.
+std::tuple<MaybeTensor, bool> packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const MaybeTensor& offsets_k, double scale,
                              bool causal, int64_t kernel, bool any_family) {
   const char* what = "packed_attention";
   check_float(what, "q", q);
@@ -991,11 +994,14 @@ MaybeTensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, 
   refuse_tangents(what, q, k, v);
   const Tensor oq = offsets.contiguous(), ok = offsets_k ? offsets_k->contiguous() : oq;
   const Packed a{aligned_rows(q), aligned_rows(k), aligned_rows(v), oq, ok, scale, causal, int(kernel)};
-  if (kernel == NB200_KERNEL_AUTO && !any_family && a.plan(NB200_PASS_FWD) != NB200_KERNEL_TCGEN05) return std::nullopt;
-  if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
-    return PackedRule::apply(a.q, a.k, a.v, oq, ok, scale, causal, kernel);
+  const bool differentiate = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  // (a batch without a query, a key or a sequence has nothing to compute in any family)
+  if (kernel == NB200_KERNEL_AUTO && !any_family && q.size(0) > 0 && k.size(0) > 0 && offsets.size(0) > 1) {
+    if (a.plan(NB200_PASS_FWD) != NB200_KERNEL_TCGEN05) return {std::nullopt, false};
+    if (differentiate && a.plan(NB200_PASS_BWD) != NB200_KERNEL_TCGEN05) return {std::nullopt, true};
   }
-  return a.forward().first;
+  if (differentiate) return {PackedRule::apply(a.q, a.k, a.v, oq, ok, scale, causal, kernel), false};
+  return {a.forward().first, false};
 }
 
 }  // namespace

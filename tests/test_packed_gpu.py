@@ -513,3 +513,54 @@ def test_scales_near_the_end_of_fp32(dtype, monkeypatch):
     lengths = [150, 20]
     for scale in (1e-25, 1e-34, 2e-38, 1e-38):
         _check(*_inputs(lengths, lengths, 4, 2, 64, dtype), lengths, lengths, scale=scale)
+
+
+def test_what_falls_back_is_told_once_per_head_layout(monkeypatch):
+    """Batches differ in their number of tokens every time: that is no new problem to tell of, nor to remember."""
+    from nitrix_b200 import backend
+    from nitrix_b200.nn import packed_attention
+
+    backend.reset_fallback_state()
+    with pytest.warns(backend.NitrixBackendFallback, match="head dim 64 or 128"):
+        for n in (20, 21, 22, 40):
+            packed_attention(*_inputs([n], [n], 4, 2, 64, torch.float32)[:3], _offsets([n]))
+    assert len(backend._warned_keys) == 1
+    packed_attention(*_inputs([20], [20], 8, 2, 64, torch.float32)[:3], _offsets([20]))
+    assert len(backend._warned_keys) == 2
+    backend.reset_fallback_state()
+
+
+def test_empty_batches_fall_back_to_nothing(monkeypatch):
+    from nitrix_b200.nn import packed_attention
+
+    monkeypatch.setenv("NITRIX_STRICT_BACKEND", "1")
+    q, k, v, dout = _inputs([10], [10], 4, 2, 64, torch.bfloat16)
+    assert packed_attention(q[:0], k[:0], v[:0], _offsets([0, 0])).shape == (0, 4, 64)
+    assert packed_attention(q[:0], k, v, _offsets([0]), offsets_k=_offsets([10])).shape == (0, 4, 64)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k[:0], v[:0])]
+    out = packed_attention(*leaves, _offsets([4, 6]), offsets_k=_offsets([0, 0]))
+    assert not bool(out.any())
+    assert not bool(torch.autograd.grad(out, leaves, dout)[0].any())
+    assert not bool(packed_attention(q, k, v, _offsets([])).any())
+
+
+def test_a_gradient_that_leaves_the_tensor_cores_is_told(monkeypatch):
+    """fp32 of head dim 128: the forward pass stays on them, its gradient does not."""
+    from nitrix_b200 import backend
+    from nitrix_b200.nn import packed_attention
+
+    q, k, v, dout = _inputs([300], [300], 4, 2, 128, torch.float32)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    off = _offsets([300])
+    backend.reset_fallback_state()
+    with pytest.warns(backend.NitrixBackendFallback, match="gradients"):
+        packed_attention(*leaves, off)
+    monkeypatch.setenv("NITRIX_STRICT_BACKEND", "1")
+    with pytest.raises(backend.NitrixBackendError, match="gradients"):
+        packed_attention(*leaves, off)
+    packed_attention(q, k, v, off)                                       # no gradient is asked for
+    with torch.no_grad():
+        packed_attention(*leaves, off)
+    for dtype, D in ((torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)):
+        packed_attention(*(t[..., :D].to(dtype).detach().requires_grad_(True) for t in leaves), off)
+    backend.reset_fallback_state()
