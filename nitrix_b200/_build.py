@@ -41,8 +41,8 @@ HOST_MODULE = "_torch_ops"
 HOST_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
 # The C++ library that torch itself runs on, whatever the compiler would link by itself: a copy of its own inside the module (a
 # toolchain without the shared library links the archive) shares locales with torch's, and printing a number into an error's
-# text then crashes.
-HOST_RUNTIME = ["-nostdlib++", "-l:libstdc++.so.6"]
+# text then crashes.  (All default libraries are named: -nostdlib++, which leaves out the one, came with GCC 13.)
+HOST_RUNTIME = ["-nodefaultlibs", "-l:libstdc++.so.6", "-lm", "-lc", "-lgcc_s", "-lgcc"]
 
 
 def sources() -> list[pathlib.Path]:

@@ -543,3 +543,29 @@ def test_the_host_module_has_no_cxx_library_of_its_own():
     image = _build.host_module_path().read_bytes()
     assert b"libstdc++.so.6\0" in image
     assert b"St12codecvt_byname" not in image
+
+
+def test_the_host_module_links_with_compilers_older_than_gcc_13(monkeypatch, tmp_path):
+    """They know no -nostdlib++.  What is linked throws, catches and prints a number with the shared C++ library."""
+    import shutil
+
+    from nitrix_b200 import _build
+
+    old = tmp_path / "older-g++"
+    old.write_text('#!/bin/sh\nfor a in "$@"; do\n  case "$a" in -nostdlib++) echo "unrecognized command-line option $a" >&2; exit 1;; esac\ndone\n'
+                   f'exec {shutil.which("g++")} "$@"\n')
+    old.chmod(0o755)
+    (tmp_path / "host.cpp").write_text(
+        '#include <cmath>\n#include <sstream>\n#include <stdexcept>\n'
+        'extern "C" __attribute__((visibility("default"))) int seven(double x) {\n'
+        '  try { std::ostringstream s; s << std::round(x); throw std::runtime_error(s.str()); }\n'
+        '  catch (const std::exception& e) { return std::stoi(e.what()); }\n}\n')
+    monkeypatch.setenv("CXX", str(old))
+    monkeypatch.setattr(_build, "LIBDIR", tmp_path)
+    monkeypatch.setattr(_build, "HOST_SOURCE", tmp_path / "host.cpp")
+    _build._compile_host()
+    module = C.CDLL(str(_build.host_module_path()))
+    module.seven.argtypes = [C.c_double]
+    assert module.seven(7.2) == 7
+    image = _build.host_module_path().read_bytes()
+    assert b"libstdc++.so.6\0" in image and b"St12codecvt_byname" not in image
