@@ -519,3 +519,48 @@ def test_autograd_notices_that_pages_are_written():
         inside = paged_cache(16, 4, 2, 64, sequences=3, max_length=16, dtype=torch.float32)
         inside = cache_append(inside, k, k, offsets)
     assert cache_append(inside, k, k, offsets).lengths.tolist() == [4, 4, 4]      # (such tensors have no version)
+
+
+def test_forks_frees_and_compactions_in_a_graph():
+    """Captured once each, replayed with other parents, other finished rows and other lengths."""
+    from nitrix_b200.nn import cache_compact, cache_fork, cache_free
+
+    rng = random.Random(2)
+    pair = Pair(64, 4, 6, 8, Hk=2, D=64, dtype=torch.float32)
+    state = [t.clone() for t in pair.cache]      # what the graphs read; the pools are shared
+    state[0], state[1] = pair.cache.k_pages, pair.cache.v_pages
+    parents = torch.arange(6, dtype=torch.int32, device="cuda")
+    finished = torch.zeros(6, dtype=torch.bool, device="cuda")
+    held = type(pair.cache)(*state)
+    calls = {"fork": lambda: cache_fork(held, parents), "free": lambda: cache_free(held, finished), "compact": lambda: cache_compact(held)}
+    graphs = {}
+    side = torch.cuda.Stream()
+    for name, call in calls.items():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            result = call()
+        graphs[name] = graph, result
+    for _ in range(20):
+        pair.append([rng.choice([0, 1, 3, 5]) for _ in range(6)])
+        what = rng.choice(list(calls))
+        if what == "fork":
+            chosen = [rng.randint(-1, 5) for _ in range(6)]
+            parents.copy_(torch.tensor(chosen))
+            pair.model.fork(chosen)
+        elif what == "free":
+            flags = [rng.random() < 0.4 for _ in range(6)]
+            finished.copy_(torch.tensor(flags))
+            pair.model.fork([-1 if f else i for i, f in enumerate(flags)])
+        else:
+            pair.model.compact()
+        for to, now in zip(state[2:], pair.cache[2:]):
+            to.copy_(now)
+        graph, result = graphs[what]
+        graph.replay()
+        pair.cache = type(pair.cache)(pair.cache.k_pages, pair.cache.v_pages, *(t.clone() for t in result[2:]))
+        torch.cuda.synchronize()
+        pair.check()
