@@ -5,7 +5,8 @@
 //
 // packed_planes_kernel writes the planes of q, k, v and dout into the workspace as the tiles that the MMAs read, a sequence and
 // key head at a time: 128 rows of queries, or 64 (token after token, the query heads of the key head), 64 keys.  Rows behind
-// the end of a sequence are zeros there, so nothing of a neighbouring sequence gets near a sum.  The tiles of sequence i begin
+// the end of a sequence are zeros there, so nothing of a neighbouring sequence gets near a sum; so are, for the sums over queries,
+// those of queries that see no key.  The tiles of sequence i begin
 // at tile begin / tokens per tile + i: sequences that follow one another never share one, and nobody has to add up the lengths.
 // The other kernels fetch whole tiles by untiled bulk copies; their blocks come from the lists of packed_plan.cu.
 //
@@ -46,6 +47,8 @@ struct PlaneOperand {
   int heads;            // rows per token
   uint32_t heads_magic; // ceil(2^16 / heads)
   int64_t tiles;        // that there is room for
+  const int* keys;      // offsets of the keys, where the first queries of a sequence with fewer keys are to be zeros
+  int total_keys;
 };
 struct PlaneArgs {
   PlaneOperand op[4];
@@ -73,6 +76,7 @@ __global__ void __launch_bounds__(128) packed_planes_kernel(const PlaneArgs a) {
   const int64_t index = tile - first_tile(span.x, op.tokens, lo);
   if (tile < op.tiles && index >= 0 && index * op.tokens < span.y) {
     const int first = span.x + int(index) * op.tokens, n = min(op.tokens, span.x + span.y - first);
+    const int blind = op.keys ? span.y - sequence_span(op.keys, lo, op.total_keys).y - int(index) * op.tokens : 0;      // tokens left out
     const float* x = op.x + int64_t(first) * op.xs[0] + int64_t(blockIdx.y) * op.heads * op.xs[1];
     const int chunk = op.rows * kRowBytes;
     uint8_t* dst_tile = op.planes + (tile * a.kv_heads + blockIdx.y) * (3 * kChunks * chunk);
@@ -83,7 +87,7 @@ __global__ void __launch_bounds__(128) packed_planes_kernel(const PlaneArgs a) {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      if (token < n) {
+      if (token >= blind && token < n) {
         const float* src = x + token * op.xs[0] + (r - token * op.heads) * op.xs[1] + c * 8;
         if (vec) {
           *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
@@ -792,7 +796,7 @@ int launch_bwd(const Fp32BwdArgs& a, int64_t blocks, cudaStream_t st) {
 
 PlaneOperand plane_operand(const void* x, uint8_t* planes, const int* offsets, const int64_t (&xs)[2], int total, int rows, int heads, int64_t tiles) {
   return PlaneOperand{static_cast<const float*>(x), planes, offsets, {xs[0], xs[1]}, total, tile_tokens(rows, heads), rows, heads,
-                      uint32_t((65536 + heads - 1) / heads), tiles};
+                      uint32_t((65536 + heads - 1) / heads), tiles, nullptr, 0};
 }
 int launch_planes(const PlaneArgs& pa, int D, int operands, int64_t tiles, cudaStream_t st) {
   const dim3 grid(unsigned(tiles), unsigned(pa.kv_heads), unsigned(operands));
@@ -900,6 +904,9 @@ int fp32_packed_bwd(const PackedArgs& p, void* ws, cudaStream_t st) {
   pa.kv_heads = p.kv_heads;
   pa.op[0] = plane_operand(p.q, planes[0], p.offsets_q, p.qs, p.tokens_q, kKeys, p.group, step_tiles(p));
   pa.op[1] = plane_operand(p.dout, planes[1], p.offsets_q, p.dos, p.tokens_q, kKeys, p.group, step_tiles(p));
+  if (p.causal) {
+    for (int i = 0; i < 2; ++i) { pa.op[i].keys = p.offsets_k; pa.op[i].total_keys = p.tokens_k; }
+  }
   pa.op[2] = plane_operand(p.k, planes[2], p.offsets_k, p.ks, p.tokens_k, kKeys, 1, key_tiles(p));
   pa.op[3] = plane_operand(p.v, planes[3], p.offsets_k, p.vs, p.tokens_k, kKeys, 1, key_tiles(p));
   if (int rc = launch_planes(pa, p.D, 4, step_tiles(p) > key_tiles(p) ? step_tiles(p) : key_tiles(p), st)) return rc;

@@ -42,9 +42,9 @@ __device__ __forceinline__ void row_offsets(int64_t* dst, int n, Offset offset) 
   if (threadIdx.x < kT) dst[threadIdx.x] = int(threadIdx.x) < n ? offset(threadIdx.x) : 0;
 }
 
-// Rows 0 .. n - 1 of a tile from `offset(row)` elements on; zeros elsewhere.  kWords: rows of whole 16-byte words.
+// Rows `first` .. n - 1 of a tile from `offset(row)` elements on; zeros elsewhere.  kWords: rows of whole 16-byte words.
 template <typename T, int kD, bool kWords, typename Offset>
-__device__ __forceinline__ void load_tile(float* dst, const void* base, int n, int D, Offset offset) {
+__device__ __forceinline__ void load_tile(float* dst, const void* base, int n, int D, Offset offset, int first = 0) {
   using L = Tile<kD>;
   const T* x = static_cast<const T*>(base);
   if constexpr (kWords) {
@@ -53,7 +53,7 @@ __device__ __forceinline__ void load_tile(float* dst, const void* base, int n, i
     for (int i = threadIdx.x; i < L::kT * kRow; i += kThreads) {
       const int r = i / kRow, d = (i - r * kRow) * kVec;
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (r < n && d < D) w = *reinterpret_cast<const uint4*>(x + offset(r) + d);
+      if (r >= first && r < n && d < D) w = *reinterpret_cast<const uint4*>(x + offset(r) + d);
       const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
       for (int j = 0; j < kVec; j += 4)
@@ -62,21 +62,21 @@ __device__ __forceinline__ void load_tile(float* dst, const void* base, int n, i
   } else {
     for (int i = threadIdx.x; i < L::kT * kD; i += kThreads) {
       const int r = i / kD, d = i - r * kD;
-      dst[r * L::kStride + d] = r < n && d < D ? to_f32<T>(x[offset(r) + d]) : 0.f;
+      dst[r * L::kStride + d] = r >= first && r < n && d < D ? to_f32<T>(x[offset(r) + d]) : 0.f;
     }
   }
 }
 
 // The same for fp32 rows of whole words, by copies that this thread waits for later.
 template <int kD, typename Offset>
-__device__ __forceinline__ void copy_tile(float* dst, const void* base, int n, int D, Offset offset) {
+__device__ __forceinline__ void copy_tile(float* dst, const void* base, int n, int D, Offset offset, int first = 0) {
   using L = Tile<kD>;
   constexpr int kRow = kD / 4;
 #pragma unroll
   for (int i = threadIdx.x; i < L::kT * kRow; i += kThreads) {
     const int r = i / kRow, d = (i - r * kRow) * 4;
     float* to = dst + r * L::kStride + d;
-    if (r < n && d < D) sm100::cp_async16(sm100::smem_u32(to), static_cast<const float*>(base) + offset(r) + d);
+    if (r >= first && r < n && d < D) sm100::cp_async16(sm100::smem_u32(to), static_cast<const float*>(base) + offset(r) + d);
     else *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
@@ -86,9 +86,9 @@ __device__ __forceinline__ void wait_copies_but_one() { asm volatile("cp.async.w
 
 // A key or value tile: copied (fp32 words; what follows has to wait) or loaded.
 template <typename T, int kD, bool kWords, typename Offset>
-__device__ __forceinline__ void fetch_tile(float* dst, const void* base, int n, int D, Offset offset) {
-  if constexpr (kWords && sizeof(T) == 4) copy_tile<kD>(dst, base, n, D, offset);
-  else load_tile<T, kD, kWords>(dst, base, n, D, offset);
+__device__ __forceinline__ void fetch_tile(float* dst, const void* base, int n, int D, Offset offset, int first = 0) {
+  if constexpr (kWords && sizeof(T) == 4) copy_tile<kD>(dst, base, n, D, offset, first);
+  else load_tile<T, kD, kWords>(dst, base, n, D, offset, first);
   commit_copies();
 }
 
@@ -411,8 +411,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkv_simt_kernel(const Pack
     row_offsets<L::kT>(at_do[buf], n, [&](int r) { return rows.at(r0 + r, a.dos); });
     if (n > 0) load_stats<L::kT>(a, rows, r0, n, stat[buf], seen[buf]);
   };
+  // (rows of queries that see no key are left out: a probability of zero makes a NaN of what is not a number in them)
+  const int64_t blind = a.causal ? int64_t(max(rows.q.y - rows.k.y, 0)) * a.group : 0;
   auto fetch = [&](float* dst, const void* base, const int64_t* at, int64_t r0) {
-    if (r0 < rows.n) fetch_tile<T, kD, kWords>(dst, base, count(r0), a.D, [&](int r) { return at[r]; });
+    if (r0 < rows.n)
+      fetch_tile<T, kD, kWords>(dst, base, count(r0), a.D, [&](int r) { return at[r]; }, int(min(max(blind - r0, int64_t(0)), int64_t(L::kT))));
   };
   place_rows(0, begin);
   __syncthreads();

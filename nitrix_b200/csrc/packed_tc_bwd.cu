@@ -17,7 +17,8 @@
 //
 // What belongs to a neighbouring sequence must not get into a sum, not even as 0 * NaN: keys behind the end have P and dS
 // selected to zero and their rows of K cleared in shared memory, queries behind the end have P and dS selected to zero and
-// their rows of Q and dO cleared.  Warp 3, which forms the addends of every step before its products may run, does that.
+// their rows of Q and dO cleared, as have queries that see no key.  Warp 3, which forms the addends of every step before its
+// products may run, does that.
 // Head dim 128: bound by the operands that the MMAs read from shared memory (about 1900 of a step's 2700 cycles) and by the sums
 // of dq in L2 (without them, for timing: 744 -> 551 us when it was 744).  Head dim 64: by the chain of a step; two steps' products
 // in TMEM 522 -> 508 us, two dS tiles as well 551.  All waits bounded.
@@ -298,6 +299,8 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   } else {
     // ---------------- warp 3: the addends of every row as MMA operands, rows of other sequences cleared ----------------
     const float inv_mul = 1.f / (a.scale * kLog2e);
+    // the sequence's first queries, which see no key; only its first block of keys comes near them
+    const int blind = a.causal && it.index == 0 ? max(it.seen, 0) : 0;
     bool ok = true;
     // lse and delta of rows lane and lane + 32 of a step, fetched a step ahead; rows without a token or a key: zeros (P and
     // dS are selected there, the addends have to be finite)
@@ -337,12 +340,15 @@ packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           st_shared_v4(sbase + L::kX + box * kBoxBytes + it.n * 128 + rem * 16, make_uint4(0, 0, 0, 0));
         }
       }
-      const int rows = min(it.other_n - step_of(n) * a.tokens, a.tokens) * a.group;      // rows of this sequence
-      if (rows < live_rows) {
-        const int words = (live_rows - rows) * 8;      // of a box of Q or dO
-        for (int i = lane; i < words * (2 * (D / 64)); i += 32) {
-          const int box = i / words, rem = i - box * words;
-          st_shared_v4(sbase + L::kY + st * L::kYStageBytes + box * kYBoxBytes + rows * 128 + rem * 16, make_uint4(0, 0, 0, 0));
+      // rows [first, end) take part: of this sequence, of queries that see a key
+      const int token0 = step_of(n) * a.tokens, end = min(it.other_n - token0, a.tokens) * a.group;
+      if (end < live_rows || token0 < blind) {
+        const int first = min(max(blind - token0, 0), a.tokens) * a.group;
+#pragma unroll 1
+        for (int i = lane; i < live_rows * 8 * (2 * (D / 64)); i += 32) {
+          const int box = i / (live_rows * 8), rem = i - box * (live_rows * 8);
+          if (rem < first * 8 || rem >= end * 8)
+            st_shared_v4(sbase + L::kY + st * L::kYStageBytes + box * kYBoxBytes + rem * 16, make_uint4(0, 0, 0, 0));
         }
       }
       uint8_t* slot = smem + L::kAug + s * L::kAugSlotBytes;

@@ -564,3 +564,31 @@ def test_a_gradient_that_leaves_the_tensor_cores_is_told(monkeypatch):
     for dtype, D in ((torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)):
         packed_attention(*(t[..., :D].to(dtype).detach().requires_grad_(True) for t in leaves), off)
     backend.reset_fallback_state()
+
+
+@pytest.mark.parametrize("dtype,D,backend", [
+    (torch.bfloat16, 64, "auto"), (torch.float16, 64, "auto"), (torch.bfloat16, 128, "auto"), (torch.float16, 128, "auto"),
+    (torch.float32, 64, "auto"), (torch.float32, 128, "auto"), (torch.bfloat16, 64, "cuda-simt"), (torch.float32, 40, "cuda-simt"),
+    (torch.float16, 256, "cuda-simt")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_a_query_without_keys_holds_reaches_no_gradient(dtype, D, backend, bad, monkeypatch):
+    """More queries than keys under causal: the first see none, and neither their row of q nor that of dout takes part."""
+    from nitrix_b200.nn import packed_attention
+
+    monkeypatch.setenv("NITRIX_SILENCE_FALLBACK", "1")
+    lengths_q, lengths_k = [300, 33, 0, 140, 200], [260, 190, 20, 11, 199]
+    q, k, v, dout = _inputs(lengths_q, lengths_k, 6, 2, D, dtype)
+    at = 0
+    clean = [t.clone() for t in (q, dout)]
+    for lq, lk in zip(lengths_q, lengths_k):
+        blind = slice(at, at + max(lq - lk, 0))
+        q[blind], dout[blind] = bad, bad
+        clean[0][blind], clean[1][blind] = 0, 0
+        at += lq
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed_attention(*leaves, _offsets(lengths_q), offsets_k=_offsets(lengths_k), backend=backend)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = O.packed(clean[0], k, v, lengths_q, lengths_k, D ** -0.5, True, clean[1])
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)):
+        value, bound = want[name]
+        assert float(((got.double() - value).abs() - U[dtype] * bound).max()) <= 1e-6, name
