@@ -556,15 +556,16 @@ sdpa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_const
     }
     // packed mask words of this owner row
     const uint32_t* mbits = nullptr;
-    // (keys past the end: their rows of K and V are zeros, but P is not, and where a row's scores are far below zero it has no bound)
-    bool key_dropped = kKeyMajor && orow >= a.T;
+    // (keys past the end: their rows of K and V are zeros, but P is not, and where a row's scores are far below zero it has no bound;
+    // only the sums of dq take them in)
+    bool key_dropped = kMerged && orow >= a.T;
     if (a.mask.rows) {
       if (!kKeyMajor) {
         if (!(key_aug && a.mask_key_only))   // a key-only mask was added to the scores as -inf
           mbits = a.mask.rows + b * a.mask.b_stride + h * a.mask.h_stride + int64_t(min(orow, a.S - 1)) * a.mask.row_stride;
       } else if (a.mask_key_only) {
         const uint32_t* krow = a.mask.rows + b * a.mask.b_stride + h * a.mask.h_stride;
-        key_dropped = key_dropped || !((krow[orow >> 5] >> (orow & 31)) & 1u);
+        key_dropped = orow >= a.T || !((krow[orow >> 5] >> (orow & 31)) & 1u);
       } else {
         mbits = a.mask.cols + b * a.mask.tb_stride + h * a.mask.th_stride + int64_t(min(orow, a.T - 1)) * a.mask.tkey_stride;
       }
