@@ -730,7 +730,8 @@ Plan plan(const nb200_decode_params* p) {
   const int group = p->q_heads / c.heads;
   bool q_words = aligned16(p->q);
   for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
-  pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words && p->scale > 0.f;
+  // (with a scale below 1e-30 the MMA loop's threshold, 8 / scale, comes near the end of fp32)
+  pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words && p->scale > 1e-30f;
   int ctas;      // resident per SM: the loops' kMinCtas
   if (pl.mma) {
     pl.heads = group > 8 ? 16 : 8;

@@ -564,3 +564,12 @@ def test_forks_frees_and_compactions_in_a_graph():
         pair.cache = type(pair.cache)(pair.cache.k_pages, pair.cache.v_pages, *(t.clone() for t in result[2:]))
         torch.cuda.synchronize()
         pair.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [1e-20, 1e-34, 2e-38, 1e-38])
+def test_decode_scales_near_the_end_of_fp32(dtype, scale):
+    """The mean of the values."""
+    lengths = [700, 33, 5]
+    cache = _cache_of(lengths, 16, 2, 64, dtype)
+    _check_decode(torch.randn(3, 8, 64, device="cuda").to(dtype), cache, lengths, scale)
