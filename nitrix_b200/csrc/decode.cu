@@ -20,9 +20,10 @@
 //  * anything else: fp32 multiply-adds, two per instruction, lanes along the head dim, a reduce-scatter of the query heads' sums.
 // In both, the next tokens' keys are asked for as soon as the scores have used the last ones, their values after the output.
 //
-// 32 sequences, 410 MB of cache: bf16, head dim 128, 8 key heads with 1 / 4 / 8 query heads each 5.9 / 5.7 / 5.3 TB/s, 4 with 16
-// each 4.3; f32 1 / 4 / 8 5.3 / 4.7 / 3.3 (the last by its instructions).  Four sequences of up to 131072 tokens, f16, 8 x 8 heads
-// of 128: 204 us, 6.6 TB/s.
+// 32 sequences, 400 MB of cache: bf16, head dim 128, 8 key heads with 1 / 4 / 8 query heads each 6.0 / 5.6 / 5.0 TB/s, 4 with 16
+// each 4.3; f32 1 / 4 / 8 5.3 / 4.7 / 3.4.  bf16 of head dim 80, 96 and 256, four query heads per key head: 1.2, 1.4 and 1.9.  One key
+// head with 128 query heads: 0.67.  Four sequences of up to 131072 tokens, f16, 8 x 8 heads of 128: 201 to 208 us, 6.4 to 6.7 TB/s
+// (of reads alone, which may pass a copy's 6.56).
 #include <math.h>
 
 #include "dependent_launch.cuh"

@@ -9,9 +9,9 @@
 // 16-byte reductions, which is the one place where the order of a sum is not fixed.  The scheme of a step -- two issuing
 // warps, two element-wise groups on alternate steps, lse and delta added by a K = 16 MMA step, dQ^T with d on the TMEM lanes --
 // is that of sdpa_tc_bwd_d128.cu, which has the reasons and the measurements.  One thing is different: dS goes to TMEM as well,
-// as the A operand of dK, which takes an eighth off what the MMAs read from shared memory (8192 tokens, 16 heads on 4, causal,
-// head dim 128: 710 -> 682 us).  At head dim 64 the tile of dQ^T has 128 lanes as
-// well, of which the upper 64 (V in place of K: the tiles lie one after the other) are not read.
+// as the A operand of dK, which takes an eighth off what the MMAs read from shared memory (head dim 128: 4 % of the time).  At head
+// dim 64 the tile of dQ^T has 128 lanes as well, of which the upper 64 (V in place of K: the tiles lie one after the other) are not
+// read.
 //
 // P and dS are rounded to the operand type where they become operands (dS from the unrounded P); sums, lse and delta are fp32.
 //
@@ -20,8 +20,9 @@
 // their rows of Q and dO cleared, as have queries that see no key.  Warp 3, which forms the addends of every step before its
 // products may run, does that.
 // Head dim 128: bound by the operands that the MMAs read from shared memory (about 1900 of a step's 2700 cycles) and by the sums
-// of dq in L2 (without them, for timing: 744 -> 551 us when it was 744).  Head dim 64: by the chain of a step; two steps' products
-// in TMEM 522 -> 508 us, two dS tiles as well 551.  All waits bounded.
+// of dq in L2 (without them, for timing: 744 -> 551 us when it was 744); 8192 tokens, 16 heads on 4, causal 720 to 731 us one at a
+// time, 775 in a long loop under the power cap (fp16 743, 815).  Head dim 64: by the chain of a step; 518 to 524 us (fp16 528); two
+// steps' products in TMEM took 522 to 508, two dS tiles as well 551.  All waits bounded.
 #include <math.h>
 
 #include <type_traits>

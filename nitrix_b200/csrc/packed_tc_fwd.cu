@@ -17,8 +17,8 @@
 // 2^8, every third pair of exponentials on the FMA units at head dim 128 -- is that of sdpa_tc_fwd.cu, which has the reasons.
 // Head dim 128: bound by the tensor pipe with its operand fetch (busy 82 % of the time, 63 % of it multiplying: the MMAs of a half
 // read 6 KB of operands for 32 cycles of products) at the clock that the power cap leaves; 8192 tokens, 16 heads on 4, 469 us (1170
-// TFLOP/s), causal 232 (1180).  Key tiles taken whole, with N = 128 and the query tiles in turn, 606 -> 730 us.  Head dim 64: by the
-// exponentials, 398 and 207 us (690 and 660 TFLOP/s).
+// TFLOP/s), causal 232 (1180).  Key tiles taken whole, with N = 128 and the query tiles in turn, 606 -> 730 us.  Head dim 64: 398 and
+// 207 us (690 and 660 TFLOP/s); what bounds it is not known: not the exponentials, of which every fourth on the FMA units changes nothing.
 // All waits on mbarriers are bounded (sdpa_tc_common.cuh).
 #include <type_traits>
 

@@ -6,8 +6,8 @@
 // Bound by HBM: every element is read and written once, and a pair costs three multiply-adds.  The cosines and sines are
 // the same for every head of a token, so a CTA takes all heads of its tokens and forms their table once, in shared memory.  The
 // phase is formed with the rounding errors of its products, so that a position of 2^40 is as good as one of 1: as one product of
-// two fp32 numbers it is off by 0.008 at position 131072.  16384 bf16 tokens, 16 + 16 heads of 128, forward and gradient: 96 us,
-// 5.6 TB/s, with small CTAs and one row per thread in flight; 256 or 512 threads 101 and 108, two or four rows in flight 104 and
+// two fp32 numbers it is off by 0.008 at position 131072.  16384 bf16 tokens, 16 + 16 heads of 128, forward and gradient: 96 to
+// 100 us, 5.4 to 5.6 TB/s, with small CTAs and one row per thread in flight; 256 or 512 threads 101 and 108, two or four rows in flight 104 and
 // 100, cosines and sines in registers of a thread that goes over the heads 115, loads that do not stay in L2 115.
 #include <math.h>
 
