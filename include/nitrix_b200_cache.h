@@ -13,7 +13,10 @@
  *   nb200_cache_fork      row i of the result is row parents[i] (none: empty); full pages are shared, the page that is
  *                         still open is copied for all but the first child
  *   nb200_cache_compact   the live pages move to the pool's front
+ *   nb200_cache_read      tokens of the cache as packed rows
  *   nb200_decode          attention of one query token per sequence over the cache
+ *
+ * nb200_cache_append_quantized and so on do the same for a cache in 4 or 8 bits, see there.
  *
  * Each call reads the cache's small arrays and writes new ones, except for append, which adds entries to `table` behind
  * those in use.  Pages are written in place, but only slots that are free in the state that the call is given; the old
@@ -99,6 +102,67 @@ typedef struct nb200_decode_params {
 
 NB200_API int nb200_decode(const nb200_decode_params* p, void* cuda_stream);
 NB200_API int nb200_decode_workspace_bytes(const nb200_decode_params* p, size_t* bytes);
+
+/*
+ * A cache in few bits.  32 elements of a head's row that follow one another are a group with one fp16 step; with `bits` b,
+ *
+ *   a = max x if max x >= -min x else min x,   step = fp16(-a / 2^(b-1)), cut to +-65504, NaN where an element is not finite
+ *   code = x (1 / step) rounded to even, cut to -2^(b-1) .. 2^(b-1) - 1, plus 2^(b-1);   value = step (code - 2^(b-1))
+ *
+ * in fp32 (a step of zero or NaN has the codes of zero).  A row of codes is (8, head_dim / 32, b / 2) bytes: of every group the
+ * elements 4 j .. 4 j + 3 lie together, the first in the lowest bits.
+ *
+ * In nb200_cache_pages k and v are then the codes, their strides are bytes, dtype is that of the new tokens, of q and out, or of
+ * what is read; head_dim is a multiple of 32.  Rows of codes begin on 16-byte boundaries, those of steps on multiples of their
+ * own size from a 16-byte boundary.
+ */
+typedef struct nb200_cache_steps {
+  void* k;                            /* fp16 (pages, heads, page_size, head_dim / 32), unit stride on the last axis */
+  void* v;
+  int64_t k_stride[3], v_stride[3];   /* elements, over (page, head, slot) */
+  int32_t bits;                       /* 4 or 8 */
+  int32_t reserved;
+} nb200_cache_steps;
+
+typedef struct nb200_cache_quantized_params {
+  size_t struct_size;        /* sizeof(nb200_cache_quantized_params) */
+  nb200_cache_params cache;  /* with its own struct_size; workspace: nb200_cache_workspace_bytes(&cache) */
+  nb200_cache_steps steps;
+} nb200_cache_quantized_params;
+
+NB200_API int nb200_cache_append_quantized(const nb200_cache_quantized_params* p, void* cuda_stream);
+NB200_API int nb200_cache_fork_quantized(const nb200_cache_quantized_params* p, void* cuda_stream);
+NB200_API int nb200_cache_compact_quantized(const nb200_cache_quantized_params* p, void* cuda_stream);
+
+typedef struct nb200_decode_quantized_params {
+  size_t struct_size;        /* sizeof(nb200_decode_quantized_params) */
+  nb200_decode_params decode;
+  nb200_cache_steps steps;
+} nb200_decode_quantized_params;
+
+NB200_API int nb200_decode_quantized(const nb200_decode_quantized_params* p, void* cuda_stream);
+NB200_API int nb200_decode_quantized_workspace_bytes(const nb200_decode_quantized_params* p, size_t* bytes);
+
+/*
+ * Tokens of a cache as packed rows: row t of out_k and out_v, dense (tokens, heads, head_dim) of pages.dtype, is position
+ * starts[i] + t - offsets[i] of the sequence i with offsets[i] <= t < offsets[i + 1]; offsets must not descend.  Rows of no
+ * sequence, and those of positions that the sequence does not hold, are zeros.
+ */
+typedef struct nb200_cache_read_params {
+  size_t struct_size;        /* sizeof(nb200_cache_read_params) */
+  nb200_cache_pages pages;
+  nb200_cache_steps steps;   /* bits 0: the pages hold elements of pages.dtype */
+  const int32_t* table;      /* dense (rows, width) */
+  const int32_t* lengths;    /* (rows) */
+  int32_t rows, width;
+  const int32_t* offsets;    /* (rows + 1) */
+  const int32_t* starts;     /* (rows), or NULL: zeros */
+  void* out_k;
+  void* out_v;
+  int64_t tokens;
+} nb200_cache_read_params;
+
+NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void* cuda_stream);
 
 #ifdef __cplusplus
 }

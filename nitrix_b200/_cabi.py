@@ -110,6 +110,9 @@ EXPORTS = (
     "nb200_layer_norm_fwd",
     "nb200_layer_norm_bwd",
     "nb200_layer_norm_workspace_bytes",
+    "nb200_rms_norm_fwd",
+    "nb200_rms_norm_bwd",
+    "nb200_rms_norm_workspace_bytes",
     "nb200_selective_scan_fwd",
     "nb200_selective_scan_bwd",
     "nb200_selective_scan_workspace_bytes",
@@ -119,9 +122,15 @@ EXPORTS = (
     "nb200_cache_append",
     "nb200_cache_fork",
     "nb200_cache_compact",
+    "nb200_cache_append_quantized",
+    "nb200_cache_fork_quantized",
+    "nb200_cache_compact_quantized",
+    "nb200_cache_read",
     "nb200_cache_workspace_bytes",
     "nb200_decode",
     "nb200_decode_workspace_bytes",
+    "nb200_decode_quantized",
+    "nb200_decode_quantized_workspace_bytes",
     "nb200_packed_fwd",
     "nb200_packed_bwd",
     "nb200_packed_workspace_bytes",

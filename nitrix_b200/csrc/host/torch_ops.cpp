@@ -21,6 +21,7 @@
 #include "nitrix_b200_cache.h"
 #include "nitrix_b200_norm.h"
 #include "nitrix_b200_packed.h"
+#include "nitrix_b200_rms_norm.h"
 #include "nitrix_b200_rotary.h"
 #include "nitrix_b200_scan.h"
 
@@ -38,7 +39,9 @@ using MaybeTensor = std::optional<Tensor>;
   X(nb200_selective_scan_fwd) X(nb200_selective_scan_bwd) X(nb200_selective_scan_checkpoint_bytes)                         \
   X(nb200_selective_scan_workspace_bytes) X(nb200_rotary) X(nb200_cache_append) X(nb200_cache_fork) X(nb200_cache_compact)  \
   X(nb200_cache_workspace_bytes) X(nb200_decode) X(nb200_decode_workspace_bytes) X(nb200_packed_plan) X(nb200_packed_fwd)  \
-  X(nb200_packed_bwd) X(nb200_packed_workspace_bytes)
+  X(nb200_packed_bwd) X(nb200_packed_workspace_bytes) X(nb200_rms_norm_fwd) X(nb200_rms_norm_bwd)                          \
+  X(nb200_rms_norm_workspace_bytes) X(nb200_cache_append_quantized) X(nb200_cache_fork_quantized)                          \
+  X(nb200_cache_compact_quantized) X(nb200_cache_read) X(nb200_decode_quantized) X(nb200_decode_quantized_workspace_bytes)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -581,6 +584,144 @@ Tensor aligned_rows(const Tensor& t) {
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
+// ---- root-mean-square norm ----------------------------------------------------------------------------------------------------
+// (rows, channels), dense; on a 16-byte boundary where the rows are of 16-byte words
+Tensor dense_rows(const Tensor& t, int64_t channels) {
+  const Tensor r = t.reshape({-1, channels}).contiguous();
+  const bool words = channels * int64_t(r.element_size()) % 16 == 0;
+  return words && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ? r.clone() : r;
+}
+
+nb200_rms_norm_params rms_params(const Tensor& x2, const Tensor& weight, double eps) {
+  nb200_rms_norm_params p{};
+  p.struct_size = sizeof(p);
+  p.rows = x2.size(0);
+  p.channels = int32_t(x2.size(1));
+  p.dtype = dtype_code(x2.scalar_type());
+  p.weight_dtype = weight.defined() ? dtype_code(weight.scalar_type()) : p.dtype;
+  p.eps = float(eps);
+  p.x = x2.data_ptr();
+  p.weight = weight.defined() ? weight.data_ptr() : nullptr;
+  return p;
+}
+
+// (y or codes, the sum of the streams, rstd, scales); rstd for a backward pass, scales with codes alone
+struct RmsNorm {
+  Tensor y, sum, rstd, scales;
+};
+RmsNorm rms_norm_forward(const Tensor& x, const MaybeTensor& residual, const Tensor& weight, double eps, bool with_rstd, bool eight, int64_t group) {
+  const int64_t C = x.size(-1);
+  const Tensor x2 = dense_rows(x, C), r2 = residual ? dense_rows(*residual, C) : Tensor();
+  RmsNorm n;
+  n.y = at::empty(x.sizes(), eight ? x.options().dtype(at::kFloat8_e4m3fn) : x.options());
+  if (residual) n.sum = at::empty(x.sizes(), x.options());
+  if (with_rstd) n.rstd = at::empty({x2.size(0)}, x.options().dtype(at::kFloat));
+  if (eight) {
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = group ? C / group : 1;
+    n.scales = at::empty(shape, x.options().dtype(at::kFloat));
+  }
+  nb200_rms_norm_params p = rms_params(x2, weight, eps);
+  p.residual = residual ? r2.data_ptr() : nullptr;
+  p.y = n.y.data_ptr();
+  p.sum = n.sum.defined() ? n.sum.data_ptr() : nullptr;
+  p.rstd = n.rstd.defined() ? n.rstd.data_ptr<float>() : nullptr;
+  p.scales = n.scales.defined() ? n.scales.data_ptr<float>() : nullptr;
+  p.group = int32_t(group);
+  check(lib.nb200_rms_norm_fwd(&p, stream_of(x)), "nb200_rms_norm_fwd");
+  return n;
+}
+
+// Saves (h, weight, rstd), where h is x or the sum, returns (dx, dweight); the gradients of the two streams are one tensor.
+struct RmsNormRule : torch::autograd::Function<RmsNormRule> {
+  static tensor_list forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, double eps) {
+    const Tensor w = weight ? aligned_rows(*weight) : Tensor();
+    const RmsNorm n = rms_norm_forward(x, residual, w, eps, true, false, 0);
+    ctx->save_for_backward({residual ? n.sum : x, w, n.rstd});
+    ctx->saved_data["dw"] = weight && weight->requires_grad();
+    ctx->set_materialize_grads(false);
+    if (residual) return {n.y, n.sum};
+    return {n.y};
+  }
+  static tensor_list backward(AutogradContext* ctx, const tensor_list& grads) {
+    const Tensor gy = grads[0], gs = grads.size() > 1 ? grads[1] : Tensor();
+    tensor_list d(4);
+    if (!gy.defined() && !gs.defined()) return d;
+    const auto s = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    const int64_t C = s[0].size(-1);
+    const Tensor h2 = dense_rows(s[0], C), w = s[1].defined() ? aligned_rows(s[1]) : Tensor(), rstd = s[2].contiguous();
+    const bool want_dw = ctx->saved_data["dw"].toBool();
+    Tensor dx, dw;
+    if (!gy.defined()) {      // (only the sum was used)
+      dx = gs;
+    } else {
+      const Tensor dy = dense_rows(gy.to(h2.scalar_type()), C), ds = gs.defined() ? dense_rows(gs.to(h2.scalar_type()), C) : Tensor();
+      dx = at::empty(s[0].sizes(), h2.options());
+      nb200_rms_norm_params p = rms_params(h2, w, 0.0);
+      p.dy = dy.data_ptr();
+      p.dsum = ds.defined() ? ds.data_ptr() : nullptr;
+      p.dx = dx.data_ptr();
+      p.rstd = rstd.data_ptr<float>();
+      Tensor ws;
+      if (want_dw) {
+        dw = at::empty({C}, w.options());
+        check(lib.nb200_rms_norm_workspace_bytes(&p, &p.workspace_bytes), "nb200_rms_norm_workspace_bytes");
+        ws = scratch(std::max<size_t>(p.workspace_bytes, 16), h2);
+        p.workspace = ws.data_ptr();
+        p.dweight = dw.data_ptr();
+      }
+      check(lib.nb200_rms_norm_bwd(&p, stream_of(h2)), "nb200_rms_norm_bwd");
+    }
+    d[0] = dx;
+    if (grads.size() > 1) d[1] = dx;      // (a residual that is left out has no gradient)
+    d[2] = dw;
+    return d;
+  }
+};
+
+void check_rms_operands(const char* what, const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight) {
+  check_float(what, "x", x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, what, ": x must have a channel at least; got shape ", x.sizes());
+  TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), what, ": ", x.size(-1), " channels do not fit 32 bits");
+  if (residual) {
+    TORCH_CHECK_TYPE(residual->scalar_type() == x.scalar_type() && residual->device() == x.device(), what, ": residual must be ", x.scalar_type(), " on ",
+                     x.device(), "; got ", residual->scalar_type(), " on ", residual->device());
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), what, ": residual must have shape ", x.sizes(), "; got ", residual->sizes());
+  }
+  if (weight) {
+    TORCH_CHECK_TYPE((weight->scalar_type() == x.scalar_type() || weight->scalar_type() == at::kFloat) && weight->device() == x.device(), what,
+                     ": weight must be ", x.scalar_type(), " or Float on ", x.device(), "; got ", weight->scalar_type(), " on ", weight->device());
+    TORCH_CHECK_VALUE(weight->dim() == 1 && weight->size(0) == x.size(-1), what, ": weight must have shape (", x.size(-1), ",); got ", weight->sizes());
+  }
+  refuse_tangents(what, x, residual, weight);
+}
+
+// (y, sum of the streams)
+std::tuple<Tensor, MaybeTensor> rms_norm(const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, double eps) {
+  check_rms_operands("rms_norm", x, residual, weight);
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (c10::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()) || (weight && weight->requires_grad()))) {
+    const tensor_list r = RmsNormRule::apply(x, residual, weight, eps);
+    return {r[0], residual ? MaybeTensor(r[1]) : std::nullopt};
+  }
+  const RmsNorm n = rms_norm_forward(x, residual, weight ? aligned_rows(*weight) : Tensor(), eps, false, false, 0);
+  return {n.y, residual ? MaybeTensor(n.sum) : std::nullopt};
+}
+
+// (codes, scales, sum of the streams); group 0: a scale per row
+std::tuple<Tensor, Tensor, MaybeTensor> rms_norm_quantized(const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, double eps, int64_t group) {
+  const char* what = "rms_norm_quantized";
+  check_rms_operands(what, x, residual, weight);
+  TORCH_CHECK_VALUE(group == 0 || ((group == 32 || group == 64 || group == 128) && x.size(-1) % group == 0), what,
+                    ": group_size must be 32, 64 or 128 and divide the ", x.size(-1), " channels; got ", group);
+  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()) || (weight && weight->requires_grad()))),
+                              what, " is not differentiable; rms_norm is");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const RmsNorm n = rms_norm_forward(x, residual, weight ? aligned_rows(*weight) : Tensor(), eps, false, true, group);
+  return {n.y, n.scales, residual ? MaybeTensor(n.sum) : std::nullopt};
+}
+
 // ---- rotary positions -------------------------------------------------------------------------------------------------------
 // x (..., heads, D) as (B, S, heads, D); the result is dense
 void rotary_operand(nb200_rotary_tensor& t, const Tensor& x4, const Tensor& y) {
@@ -695,26 +836,58 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q, const MaybeTensor& k, co
 }
 
 // ---- paged cache --------------------------------------------------------------------------------------------------------------
-nb200_cache_pages cache_pages(const char* what, const Tensor& k_pages, const Tensor& v_pages) {
-  TORCH_CHECK_TYPE(v_pages.scalar_type() == k_pages.scalar_type() && v_pages.device() == k_pages.device(), what, ": v_pages must be like k_pages");
-  TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), what,
-                    ": k_pages and v_pages must have one shape (pages, heads, page size, head dim); got ", k_pages.sizes(), " and ", v_pages.sizes());
-  TORCH_CHECK_VALUE(k_pages.size(1) > 0 && k_pages.size(2) > 0 && k_pages.size(3) > 0, what, ": a page must hold a token at least; got shape ", k_pages.sizes());
-  check_extents(what, k_pages);
-  nb200_cache_pages c{};
-  const Tensor* t[2] = {&k_pages, &v_pages};
-  for (int i = 0; i < 2; ++i) {
-    // (written in place: a copy in another layout would not do)
-    TORCH_CHECK_VALUE(t[i]->stride(3) == 1 && !has_expanded_axis(*t[i]), what, ": pages must have unit stride along the head dim and no expanded axis");
-    for (int a = 0; a < 3; ++a) (i ? c.v_stride : c.k_stride)[a] = t[i]->stride(a);
-  }
-  c.k = k_pages.data_ptr();
-  c.v = v_pages.data_ptr();
-  c.pages = int32_t(k_pages.size(0)); c.heads = int32_t(k_pages.size(1));
-  c.page_size = int32_t(k_pages.size(2)); c.head_dim = int32_t(k_pages.size(3));
-  c.dtype = dtype_code(k_pages.scalar_type());
-  return c;
+// `k_steps`: those of a cache in few bits, whose pages hold codes
+void check_pool(const char* what, const Tensor& k_pages, const MaybeTensor& k_steps) {
+  if (!k_steps) return check_float(what, "k_pages", k_pages);
+  TORCH_CHECK_TYPE(k_pages.is_cuda() && k_pages.scalar_type() == at::kByte, what, ": k_codes must be a CUDA tensor of uint8; got ", k_pages.scalar_type(), " on ",
+                   k_pages.device());
 }
+
+// The pages of a cache, or its codes and steps.
+struct CachePages {
+  nb200_cache_pages pages{};
+  nb200_cache_steps steps{};
+
+  bool coded() const { return steps.bits != 0; }
+  CachePages(const char* what, const Tensor& k_pages, const Tensor& v_pages, const MaybeTensor& k_steps, const MaybeTensor& v_steps) {
+    const char* names = k_steps ? "k_codes and v_codes" : "k_pages and v_pages";
+    TORCH_CHECK_TYPE(v_pages.scalar_type() == k_pages.scalar_type() && v_pages.device() == k_pages.device(), what,
+                     k_steps ? ": v_codes must be like k_codes" : ": v_pages must be like k_pages");
+    TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), what, ": ", names, " must have one shape (pages, heads, page size, ",
+                      k_steps ? "bytes" : "head dim", "); got ", k_pages.sizes(), " and ", v_pages.sizes());
+    TORCH_CHECK_VALUE(k_pages.size(1) > 0 && k_pages.size(2) > 0 && k_pages.size(3) > 0, what, ": a page must hold a token at least; got shape ", k_pages.sizes());
+    check_extents(what, k_pages);
+    const Tensor* t[2] = {&k_pages, &v_pages};
+    for (int i = 0; i < 2; ++i) {
+      // (written in place: a copy in another layout would not do)
+      TORCH_CHECK_VALUE(t[i]->stride(3) == 1 && !has_expanded_axis(*t[i]), what, ": pages must have unit stride along the ", k_steps ? "bytes of a row" : "head dim",
+                        " and no expanded axis");
+      for (int a = 0; a < 3; ++a) (i ? pages.v_stride : pages.k_stride)[a] = t[i]->stride(a);
+    }
+    pages.k = k_pages.data_ptr();
+    pages.v = v_pages.data_ptr();
+    pages.pages = int32_t(k_pages.size(0)); pages.heads = int32_t(k_pages.size(1));
+    pages.page_size = int32_t(k_pages.size(2)); pages.head_dim = int32_t(k_pages.size(3));
+    pages.dtype = dtype_code(k_pages.scalar_type());
+    if (!k_steps) return;
+    TORCH_CHECK_VALUE(bool(v_steps), what, ": k_steps without v_steps");
+    for (const MaybeTensor* x : {&k_steps, &v_steps}) {
+      TORCH_CHECK_TYPE((*x)->scalar_type() == at::kHalf && (*x)->device() == k_pages.device(), what, ": steps must be float16 on ", k_pages.device(), "; got ",
+                       (*x)->scalar_type(), " on ", (*x)->device());
+      TORCH_CHECK_VALUE((*x)->dim() == 4 && (*x)->sizes() == k_steps->sizes() && (*x)->sizes().slice(0, 3) == k_pages.sizes().slice(0, 3) && (*x)->size(3) > 0, what,
+                        ": k_steps and v_steps must have one shape (", k_pages.size(0), ", ", k_pages.size(1), ", ", k_pages.size(2), ", groups); got ", (*x)->sizes());
+      TORCH_CHECK_VALUE((*x)->stride(3) == 1 || (*x)->size(3) == 1, what, ": steps must have unit stride along the groups");
+      TORCH_CHECK_VALUE(!has_expanded_axis(**x), what, ": steps must have no expanded axis");
+    }
+    const int64_t groups = k_steps->size(3), row = k_pages.size(3);
+    steps.bits = row == 16 * groups ? 4 : row == 32 * groups ? 8 : 0;
+    TORCH_CHECK_VALUE(steps.bits != 0, what, ": ", groups, " groups of 32 elements take ", 16 * groups, " bytes in 4 bits or ", 32 * groups, " in 8; the rows of codes have ", row);
+    pages.head_dim = int32_t(32 * groups);
+    steps.k = k_steps->data_ptr();
+    steps.v = v_steps->data_ptr();
+    for (int a = 0; a < 3; ++a) { steps.k_stride[a] = k_steps->stride(a); steps.v_stride[a] = v_steps->stride(a); }
+  }
+};
 
 // Raises the version of what a call has written in place, by which autograd notices that a saved tensor is no longer what it was.
 // (Inference tensors have none.)
@@ -725,15 +898,20 @@ void written(const T&... tensors) {
 }
 
 struct CacheCall {
-  nb200_cache_params p{};
+  nb200_cache_quantized_params q{};      // p with what a cache in few bits has beside it
+  nb200_cache_params& p = q.cache;
   Tensor lengths, free_pages, free_range;
   const char* what;
 
   CacheCall(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths_in,
-            const Tensor& free_pages_in, const Tensor& free_range_in)
+            const Tensor& free_pages_in, const Tensor& free_range_in, const MaybeTensor& k_steps, const MaybeTensor& v_steps)
       : what(name) {
+    q.struct_size = sizeof(q);
     p.struct_size = sizeof(p);
-    p.pages = cache_pages(what, k_pages, v_pages);
+    const CachePages c(what, k_pages, v_pages, k_steps, v_steps);
+    p.pages = c.pages;
+    if (c.coded()) p.pages.dtype = NB200_F16;      // (of the new tokens: append says which; else of no meaning)
+    q.steps = c.steps;
     check_ints(what, "table", table, k_pages, 2);
     check_ints(what, "lengths", lengths_in, k_pages, 1);
     check_ints(what, "free_pages", free_pages_in, k_pages, 1);
@@ -762,21 +940,30 @@ struct CacheCall {
     p.workspace_bytes = need;
     return ws;
   }
+  void run(int (*plain)(const nb200_cache_params*, void*), int (*quantized)(const nb200_cache_quantized_params*, void*), const Tensor& on) const {
+    const std::string name = std::string("nb200_") + what;
+    if (q.steps.bits) check(quantized(&q, stream_of(on)), (name + "_quantized").c_str());
+    else check(plain(&p, stream_of(on)), name.c_str());
+  }
 };
 
 // (lengths, free_range, shortfall)
 std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
                                                 const Tensor& free_pages, const Tensor& free_range, const Tensor& k, const Tensor& v,
-                                                const Tensor& offsets) {
+                                                const Tensor& offsets, const MaybeTensor& k_steps, const MaybeTensor& v_steps) {
   const char* what = "cache_append";
-  check_float(what, "k_pages", k_pages);
+  check_pool(what, k_pages, k_steps);
   const c10::cuda::CUDAGuard guard(k_pages.device());
-  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
+  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range, k_steps, v_steps);
+  if (k_steps) {      // (quantised from any of the three types)
+    check_float(what, "k", k);
+    c.p.pages.dtype = dtype_code(k.scalar_type());
+  }
+  const at::ScalarType type = k_steps ? k.scalar_type() : k_pages.scalar_type();
   for (const Tensor* t : {&k, &v}) {
-    TORCH_CHECK_TYPE(t->scalar_type() == k_pages.scalar_type() && t->device() == k_pages.device(), what, ": k and v must be ", k_pages.scalar_type(), " on ",
-                     k_pages.device());
-    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) == k.size(0) && t->size(1) == k_pages.size(1) && t->size(2) == k_pages.size(3), what,
-                      ": k and v must be (tokens, ", k_pages.size(1), ", ", k_pages.size(3), "); got ", t->sizes());
+    TORCH_CHECK_TYPE(t->scalar_type() == type && t->device() == k_pages.device(), what, ": k and v must be ", type, " on ", k_pages.device());
+    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) == k.size(0) && t->size(1) == k_pages.size(1) && t->size(2) == c.p.pages.head_dim, what,
+                      ": k and v must be (tokens, ", k_pages.size(1), ", ", c.p.pages.head_dim, "); got ", t->sizes());
   }
   check_ints(what, "offsets", offsets, k_pages, 1);
   TORCH_CHECK_VALUE(table.size(0) > 0 && offsets.size(0) == table.size(0) + 1, what, ": ", table.size(0), " rows, but offsets of shape ", offsets.sizes());
@@ -791,18 +978,22 @@ std::tuple<Tensor, Tensor, Tensor> cache_append(const Tensor& k_pages, const Ten
   c.p.new_lengths = new_lengths.data_ptr<int32_t>();
   c.p.new_free_range = new_range.data_ptr<int32_t>();
   c.p.shortfall = shortfall.data_ptr<int32_t>();
-  check(lib.nb200_cache_append(&c.p, stream_of(k_pages)), "nb200_cache_append");
-  if (k.size(0) > 0) written(k_pages, v_pages, table);
+  c.run(lib.nb200_cache_append, lib.nb200_cache_append_quantized, k_pages);
+  if (k.size(0) > 0) {
+    written(k_pages, v_pages, table);
+    if (k_steps) written(*k_steps, *v_steps);
+  }
   return {new_lengths, new_range, shortfall};
 }
 
 // (table, lengths, free_pages, free_range, shortfall); `rows`: parents (int32), or which rows are finished (bool)
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
-                                                              const Tensor& free_pages, const Tensor& free_range, const Tensor& rows, bool finished) {
+                                                              const Tensor& free_pages, const Tensor& free_range, const Tensor& rows, bool finished,
+                                                              const MaybeTensor& k_steps, const MaybeTensor& v_steps) {
   const char* what = finished ? "cache_free" : "cache_fork";
-  check_float(what, "k_pages", k_pages);
+  check_pool(what, k_pages, k_steps);
   const c10::cuda::CUDAGuard guard(k_pages.device());
-  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range);
+  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range, k_steps, v_steps);
   const Tensor r = rows.contiguous();
   if (finished) {
     TORCH_CHECK_TYPE(r.scalar_type() == at::kBool && r.device() == k_pages.device(), what, ": finished must be bool on ", k_pages.device());
@@ -822,17 +1013,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_pa
   c.p.new_free_range = new_range.data_ptr<int32_t>();
   c.p.shortfall = shortfall.data_ptr<int32_t>();
   const Tensor ws = c.workspace();
-  check(lib.nb200_cache_fork(&c.p, stream_of(k_pages)), "nb200_cache_fork");
-  if (!finished) written(k_pages, v_pages);      // (rows that stay, or become empty, copy nothing)
+  c.run(lib.nb200_cache_fork, lib.nb200_cache_fork_quantized, k_pages);
+  if (!finished) {      // (rows that stay, or become empty, copy nothing)
+    written(k_pages, v_pages);
+    if (k_steps) written(*k_steps, *v_steps);
+  }
   return {new_table, new_lengths, new_free, new_range, shortfall};
 }
 
 // (table, free_pages, free_range, shortfall)
 std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
-                                                         const Tensor& free_pages, const Tensor& free_range) {
-  check_float("cache_compact", "k_pages", k_pages);
+                                                         const Tensor& free_pages, const Tensor& free_range, const MaybeTensor& k_steps,
+                                                         const MaybeTensor& v_steps) {
+  const char* what = "cache_compact";
+  check_pool(what, k_pages, k_steps);
   const c10::cuda::CUDAGuard guard(k_pages.device());
-  CacheCall c("cache_compact", k_pages, v_pages, table, lengths, free_pages, free_range);
+  CacheCall c(what, k_pages, v_pages, table, lengths, free_pages, free_range, k_steps, v_steps);
   const Tensor new_table = at::empty(table.sizes(), table.options()), new_free = c.ints(k_pages.size(0)), new_range = c.ints(2),
                shortfall = c.ints(1);
   c.p.new_table = new_table.data_ptr<int32_t>();
@@ -840,28 +1036,40 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cache_compact(const Tensor& k_pages, 
   c.p.new_free_range = new_range.data_ptr<int32_t>();
   c.p.shortfall = shortfall.data_ptr<int32_t>();
   const Tensor ws = c.workspace();
-  check(lib.nb200_cache_compact(&c.p, stream_of(k_pages)), "nb200_cache_compact");
+  c.run(lib.nb200_cache_compact, lib.nb200_cache_compact_quantized, k_pages);
   written(k_pages, v_pages);
+  if (k_steps) written(*k_steps, *v_steps);
   return {new_table, new_free, new_range, shortfall};
 }
 
-Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, double scale) {
+Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, double scale,
+                        const MaybeTensor& k_steps, const MaybeTensor& v_steps) {
   const char* what = "decode_attention";
-  check_float(what, "k_pages", k_pages);
+  check_pool(what, k_pages, k_steps);
   const c10::cuda::CUDAGuard guard(k_pages.device());
-  nb200_decode_params p{};
+  nb200_decode_quantized_params qp{};
+  nb200_decode_params& p = qp.decode;
+  qp.struct_size = sizeof(qp);
   p.struct_size = sizeof(p);
-  p.pages = cache_pages(what, k_pages, v_pages);
-  TORCH_CHECK_TYPE(q.scalar_type() == k_pages.scalar_type() && q.device() == k_pages.device(), what, ": q must be ", k_pages.scalar_type(), " on ", k_pages.device());
-  TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == table.size(0) && q.size(2) == k_pages.size(3) && q.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, what,
-                    ": q must be (", table.size(0), ", a multiple of ", k_pages.size(1), ", ", k_pages.size(3), "); got ", q.sizes());
+  const CachePages c(what, k_pages, v_pages, k_steps, v_steps);
+  p.pages = c.pages;
+  qp.steps = c.steps;
+  if (c.coded()) {
+    check_float(what, "q", q);
+    p.pages.dtype = dtype_code(q.scalar_type());
+  }
+  const at::ScalarType type = c.coded() ? q.scalar_type() : k_pages.scalar_type();
+  TORCH_CHECK_TYPE(q.scalar_type() == type && q.device() == k_pages.device(), what, ": q must be ", type, " on ", k_pages.device());
+  TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == table.size(0) && q.size(2) == p.pages.head_dim && q.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, what,
+                    ": q must be (", table.size(0), ", a multiple of ", k_pages.size(1), ", ", p.pages.head_dim, "); got ", q.sizes());
   check_extents(what, q);
   check_ints(what, "table", table, k_pages, 2);
   check_ints(what, "lengths", lengths, k_pages, 1);
   TORCH_CHECK_VALUE(lengths.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths.sizes());
-  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad())), what,
-                              " is not differentiable; packed_attention is");
-  refuse_tangents(what, q, k_pages, v_pages);
+  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad() ||
+                                                               (k_steps && (k_steps->requires_grad() || v_steps->requires_grad())))),
+                              what, " is not differentiable; packed_attention is");
+  refuse_tangents(what, q, k_pages, v_pages, k_steps, v_steps);
   const Tensor qr = aligned_rows(q), tab = table.contiguous(), len = lengths.contiguous();
   const Tensor out = at::empty(q.sizes(), q.options());
   p.table = tab.data_ptr<int32_t>();
@@ -875,11 +1083,58 @@ Tensor decode_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
   p.q_heads = int32_t(q.size(1));
   p.scale = float(scale);
   if (p.rows == 0) return out;
-  check(lib.nb200_decode_workspace_bytes(&p, &p.workspace_bytes), "nb200_decode_workspace_bytes");
+  if (c.coded()) check(lib.nb200_decode_quantized_workspace_bytes(&qp, &p.workspace_bytes), "nb200_decode_quantized_workspace_bytes");
+  else check(lib.nb200_decode_workspace_bytes(&p, &p.workspace_bytes), "nb200_decode_workspace_bytes");
   const Tensor ws = scratch(p.workspace_bytes, q);
   p.workspace = ws.data_ptr();
-  check(lib.nb200_decode(&p, stream_of(q)), "nb200_decode");
+  if (c.coded()) check(lib.nb200_decode_quantized(&qp, stream_of(q)), "nb200_decode_quantized");
+  else check(lib.nb200_decode(&p, stream_of(q)), "nb200_decode");
   return out;
+}
+
+// (k, v) of `tokens` packed rows; codes become `type`, elements keep theirs
+std::tuple<Tensor, Tensor> cache_read(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, const Tensor& offsets,
+                                      const MaybeTensor& starts, int64_t tokens, std::optional<at::ScalarType> type, const MaybeTensor& k_steps,
+                                      const MaybeTensor& v_steps) {
+  const char* what = "cache_read";
+  check_pool(what, k_pages, k_steps);
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  nb200_cache_read_params p{};
+  p.struct_size = sizeof(p);
+  const CachePages c(what, k_pages, v_pages, k_steps, v_steps);
+  p.pages = c.pages;
+  p.steps = c.steps;
+  const at::ScalarType out = type ? *type : c.coded() ? at::kBFloat16 : k_pages.scalar_type();
+  TORCH_CHECK_TYPE(dtype_code(out) >= 0 && (c.coded() || out == k_pages.scalar_type()), what, ": dtype must be ",
+                   c.coded() ? "float32, bfloat16 or float16" : "that of the pages", "; got ", out);
+  p.pages.dtype = dtype_code(out);
+  check_ints(what, "table", table, k_pages, 2);
+  check_ints(what, "lengths", lengths, k_pages, 1);
+  check_ints(what, "offsets", offsets, k_pages, 1);
+  TORCH_CHECK_VALUE(lengths.size(0) == table.size(0), what, ": ", table.size(0), " rows, but lengths of shape ", lengths.sizes());
+  TORCH_CHECK_VALUE(offsets.size(0) == table.size(0) + 1, what, ": ", table.size(0), " rows, but offsets of shape ", offsets.sizes());
+  if (starts) {
+    check_ints(what, "starts", *starts, k_pages, 1);
+    TORCH_CHECK_VALUE(starts->size(0) == table.size(0), what, ": ", table.size(0), " rows, but starts of shape ", starts->sizes());
+  }
+  TORCH_CHECK_VALUE(tokens >= 0 && tokens <= std::numeric_limits<int32_t>::max(), what, ": tokens must be a number of rows below 2^31; got ", tokens);
+  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::GradMode::is_enabled() && (k_pages.requires_grad() || v_pages.requires_grad() ||
+                                                               (k_steps && (k_steps->requires_grad() || v_steps->requires_grad())))),
+                              what, " is not differentiable");
+  refuse_tangents(what, k_pages, v_pages, k_steps, v_steps);
+  const Tensor tab = table.contiguous(), len = lengths.contiguous(), off = offsets.contiguous(), first = starts ? starts->contiguous() : Tensor();
+  const Tensor k = at::empty({tokens, p.pages.heads, p.pages.head_dim}, k_pages.options().dtype(out)), v = at::empty(k.sizes(), k.options());
+  p.table = tab.data_ptr<int32_t>();
+  p.lengths = len.data_ptr<int32_t>();
+  p.rows = int32_t(table.size(0));
+  p.width = int32_t(table.size(1));
+  p.offsets = off.data_ptr<int32_t>();
+  p.starts = first.defined() ? first.data_ptr<int32_t>() : nullptr;
+  p.out_k = k.data_ptr();
+  p.out_v = v.data_ptr();
+  p.tokens = tokens;
+  check(lib.nb200_cache_read(&p, stream_of(k_pages)), "nb200_cache_read");
+  return {k, v};
 }
 
 // ---- packed sequences ------------------------------------------------------------------------------------------------------
@@ -1021,5 +1276,8 @@ PYBIND11_MODULE(_torch_ops, m) {
   m.def("cache_fork", torch::wrap_pybind_function_no_gil(cache_fork));
   m.def("cache_compact", torch::wrap_pybind_function_no_gil(cache_compact));
   m.def("decode_attention", torch::wrap_pybind_function_no_gil(decode_attention));
+  m.def("cache_read", torch::wrap_pybind_function_no_gil(cache_read));
+  m.def("rms_norm", torch::wrap_pybind_function_no_gil(rms_norm));
+  m.def("rms_norm_quantized", torch::wrap_pybind_function_no_gil(rms_norm_quantized));
   m.def("packed_attention", torch::wrap_pybind_function_no_gil(packed_attention));
 }

@@ -10,9 +10,8 @@
 // fork is a memset and two launches, compact a memset and three, each set up while the one before runs.  33 k tokens of bf16, 8
 // heads of 128, 50 us (5.5 TB/s); 2100 pages of 64 KB moved among 8300, 60 us (4.5 TB/s), 48 of them the moves; 256 single tokens 7.6 and
 // a fork of 64 rows 10.5 in a captured graph, 15 and 21 where the host makes the calls.
+#include "cache_codes.cuh"
 #include "dependent_launch.cuh"
-#include "nitrix_b200_cache.h"
-#include "sdpa_common.cuh"
 
 namespace nb200 {
 namespace {
@@ -25,6 +24,14 @@ struct Pages {
   uint4* v;
   int64_t ks[3], vs[3];     // words, over (page, head, slot)
   int pages, heads, page_size, words;   // words of a head's row
+};
+
+// The steps of a cache in few bits, as the largest units that their rows are made of.
+struct StepPages {
+  uint16_t* k;
+  uint16_t* v;
+  int64_t ks[3], vs[3];     // elements, over (page, head, slot)
+  int groups;               // elements of a head's row
 };
 
 // ---- append ---------------------------------------------------------------------------------------------------------------
@@ -44,6 +51,7 @@ struct AppendArgs {
   int64_t ks[2], vs[2];     // words, over (token, head)
   int64_t tokens;
   int tokens_per_warp;
+  StepPages steps;
 };
 
 struct RowPlan {
@@ -77,6 +85,40 @@ __device__ __forceinline__ void free_bounds(const int* range, int pages, int* be
   *end = min(max(range[1], *begin), pages);
 }
 
+// Quantises token `t` into slot `slot` of `page`, by a warp.  A lane takes 8 elements, four lanes a group.
+template <int kBits, typename T>
+__device__ __forceinline__ void quantize_token(const AppendArgs& a, int64_t t, int page, int slot) {
+  constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
+  const int lane = threadIdx.x & 31, u = lane & 3;
+  const int units = a.steps.groups * 4, n = a.p.heads * units;      // of 8 elements: of a head's row, of the token
+  uint8_t* kd = reinterpret_cast<uint8_t*>(a.p.k + page * a.p.ks[0] + slot * a.p.ks[2]);
+  uint8_t* vd = reinterpret_cast<uint8_t*>(a.p.v + page * a.p.vs[0] + slot * a.p.vs[2]);
+  uint16_t* kt = a.steps.k + page * a.steps.ks[0] + slot * a.steps.ks[2];
+  uint16_t* vt = a.steps.v + page * a.steps.vs[0] + slot * a.steps.vs[2];
+  const uint4* kx = a.k + t * a.ks[0];
+  const uint4* vx = a.v + t * a.vs[0];
+  // (whole warps go round together: a group's lanes exchange their maxima)
+  for (int w0 = 0; w0 < n; w0 += 32) {
+    const int w = min(w0 + lane, n - 4 + u), h = w / units, c = w - h * units;      // (n is a multiple of 4)
+    uint4 kw[kWords], vw[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      kw[i] = __ldg(kx + h * a.ks[1] + c * kWords + i);
+      vw[i] = __ldg(vx + h * a.vs[1] + c * kWords + i);
+    }
+    const Quantized<kBits> k = quantize<kBits, T>(kw), v = quantize<kBits, T>(vw);
+    if (w0 + lane >= n) continue;
+    store_codes(kd + h * a.p.ks[1] * 16, a.steps.groups, c >> 2, u, k);
+    store_codes(vd + h * a.p.vs[1] * 16, a.steps.groups, c >> 2, u, v);
+    if (u == 0) {
+      kt[h * a.steps.ks[1] + (c >> 2)] = k.step;
+      vt[h * a.steps.vs[1] + (c >> 2)] = v.step;
+    }
+  }
+}
+
+// kBits 0: the tokens' rows are copied; otherwise T is their type.
+template <int kBits, typename T>
 __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int begin, end;
@@ -169,6 +211,10 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
       if (slot == 0 && lane == 0) a.table[int64_t(row) * a.width + column] = page;
     }
     if (page < 0 || page >= a.p.pages) continue;
+    if constexpr (kBits != 0) {
+      quantize_token<kBits, T>(a, t, page, slot);
+      continue;
+    }
     uint4* kd = a.p.k + page * a.p.ks[0] + slot * a.p.ks[2];
     uint4* vd = a.p.v + page * a.p.vs[0] + slot * a.p.vs[2];
     const uint4* kx = a.k + t * a.ks[0];
@@ -216,6 +262,7 @@ Layout layout(int pages) {
 
 struct MoveArgs {
   Pages p;
+  StepPages steps;
   const int* table;
   const int* lengths;
   const int* free_pages;
@@ -248,32 +295,51 @@ __device__ __forceinline__ void mark(const MoveArgs& a, int page) {
   if (page >= 0 && page < a.p.pages) atomicOr(a.bits + (page >> 5), 1u << (page & 31));
 }
 
-// `slots` slots of every head of a page, by the CTAs `part` of `parts`
-__device__ __forceinline__ void copy_page(const Pages& p, int src, int dst, int slots, int part, int parts) {
-  const int per_head = slots * p.words, n = p.heads * per_head, stride = parts * kThreads;
+// `slots` slots of every head of a page, by the CTAs `part` of `parts`: rows of `words` units, strides in units
+template <typename U>
+__device__ __forceinline__ void copy_rows(U* k, U* v, const int64_t (&ks)[3], const int64_t (&vs)[3], int heads, int words, int src, int dst, int slots,
+                                          int part, int parts) {
+  const int per_head = slots * words, n = heads * per_head, stride = parts * kThreads;
   for (int i0 = part * kThreads + int(threadIdx.x); i0 < n; i0 += 4 * stride) {
-    uint4 kw[4], vw[4];
+    U kw[4], vw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * stride, h = i / per_head, rem = i - h * per_head, s = rem / p.words, c = rem - s * p.words;
+      const int i = i0 + j * stride, h = i / per_head, rem = i - h * per_head, s = rem / words, c = rem - s * words;
       if (i < n) {
-        kw[j] = __ldcs(p.k + src * p.ks[0] + h * p.ks[1] + s * p.ks[2] + c);
-        vw[j] = __ldcs(p.v + src * p.vs[0] + h * p.vs[1] + s * p.vs[2] + c);
+        kw[j] = __ldcs(k + src * ks[0] + h * ks[1] + s * ks[2] + c);
+        vw[j] = __ldcs(v + src * vs[0] + h * vs[1] + s * vs[2] + c);
       }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * stride, h = i / per_head, rem = i - h * per_head, s = rem / p.words, c = rem - s * p.words;
+      const int i = i0 + j * stride, h = i / per_head, rem = i - h * per_head, s = rem / words, c = rem - s * words;
       if (i < n) {
-        p.k[dst * p.ks[0] + h * p.ks[1] + s * p.ks[2] + c] = kw[j];
-        p.v[dst * p.vs[0] + h * p.vs[1] + s * p.vs[2] + c] = vw[j];
+        k[dst * ks[0] + h * ks[1] + s * ks[2] + c] = kw[j];
+        v[dst * vs[0] + h * vs[1] + s * vs[2] + c] = vw[j];
       }
     }
+  }
+}
+// (rows of steps begin at multiples of their size: as the largest words that this allows)
+template <typename U>
+__device__ __forceinline__ void copy_steps(const StepPages& p, int heads, int src, int dst, int slots, int part, int parts) {
+  constexpr int n = int(sizeof(U)) / 2;
+  const int64_t ks[3] = {p.ks[0] / n, p.ks[1] / n, p.ks[2] / n}, vs[3] = {p.vs[0] / n, p.vs[1] / n, p.vs[2] / n};
+  copy_rows(reinterpret_cast<U*>(p.k), reinterpret_cast<U*>(p.v), ks, vs, heads, p.groups / n, src, dst, slots, part, parts);
+}
+template <bool kSteps>
+__device__ __forceinline__ void copy_page(const MoveArgs& a, int src, int dst, int slots, int part, int parts) {
+  copy_rows(a.p.k, a.p.v, a.p.ks, a.p.vs, a.p.heads, a.p.words, src, dst, slots, part, parts);
+  if constexpr (kSteps) {
+    if (a.steps.groups % 4 == 0) copy_steps<uint2>(a.steps, a.p.heads, src, dst, slots, part, parts);
+    else if (a.steps.groups % 2 == 0) copy_steps<uint32_t>(a.steps, a.p.heads, src, dst, slots, part, parts);
+    else copy_steps<uint16_t>(a.steps, a.p.heads, src, dst, slots, part, parts);
   }
 }
 
 // One row of the result per blockIdx.x, its page copy in gridDim.y parts.  A row's rank among the rows that copy is the number
 // of rows before it with an open page less the number of their distinct parents, which a bit per parent counts.
+template <bool kSteps>
 __global__ void __launch_bounds__(kThreads) cache_fork_rows_kernel(const MoveArgs a) {
   extern __shared__ unsigned seen[];       // one bit per row of the old table
   allow_dependents();
@@ -333,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) cache_fork_rows_kernel(const MoveArg
   }
   if (served) {
     const int src = from[full];
-    if (src >= 0 && src < a.p.pages && fresh >= 0 && fresh < a.p.pages) copy_page(a.p, src, fresh, part, blockIdx.y, gridDim.y);
+    if (src >= 0 && src < a.p.pages && fresh >= 0 && fresh < a.p.pages) copy_page<kSteps>(a, src, fresh, part, blockIdx.y, gridDim.y);
   }
 }
 
@@ -409,6 +475,7 @@ __global__ void __launch_bounds__(kThreads) cache_list_kernel(const MoveArgs a, 
 
 // Live pages at or behind the number of live pages go to the lowest free ones, in order: free pages are the only ones
 // written, live ones the only ones read, so that moves cannot meet.
+template <bool kSteps>
 __global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a, int parts) {
   wait_for_previous();
   const int n_free = a.new_free_range[1], live = a.p.pages - n_free, kept = live - *a.n_moves;      // kept: live pages that stay
@@ -423,37 +490,49 @@ __global__ void __launch_bounds__(kThreads) cache_move_kernel(const MoveArgs a, 
   }
   // a page in `parts` parts, all parts of all pages dealt to the CTAs in turn
   const int n = *a.n_moves * parts;
-  for (int i = blockIdx.x; i < n; i += gridDim.x) copy_page(a.p, a.moves[i / parts], a.holes[i / parts], a.p.page_size, i % parts, parts);
+  for (int i = blockIdx.x; i < n; i += gridDim.x) copy_page<kSteps>(a, a.moves[i / parts], a.holes[i / parts], a.p.page_size, i % parts, parts);
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.p.pages; i += gridDim.x * kThreads)
     a.new_free_pages[i] = i < n_free ? live + i : -1;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-int check_pages(const nb200_cache_pages& c, const char* what, Pages* out) {
+// `steps`: of a cache in few bits, whose pages hold codes; otherwise NULL
+int check_pages(const nb200_cache_pages& c, const nb200_cache_steps* steps, const char* what, Pages* out) {
   if (c.dtype != NB200_F32 && c.dtype != NB200_BF16 && c.dtype != NB200_F16) { set_error("%s: bad dtype", what); return NB200_ERR_INVALID; }
   if (c.pages < 0 || c.heads <= 0 || c.page_size <= 0 || c.head_dim <= 0 || (c.pages && (!c.k || !c.v))) {
     set_error("%s: bad extents of the pages, or NULL pages", what);
     return NB200_ERR_INVALID;
   }
-  const int vec = c.dtype == NB200_F32 ? 4 : 8;
-  bool ok = c.head_dim % vec == 0 && aligned16(c.k) && aligned16(c.v);
+  if (steps)
+    if (int rc = check_steps(c, *steps, what)) return rc;
+  const int vec = steps ? 16 : c.dtype == NB200_F32 ? 4 : 8;      // elements of a word, bytes of codes
+  const int row = steps ? c.head_dim / 8 * steps->bits : c.head_dim;
+  bool ok = row % vec == 0 && aligned16(c.k) && aligned16(c.v);
   for (int i = 0; i < 3; ++i) ok = ok && c.k_stride[i] % vec == 0 && c.v_stride[i] % vec == 0;
   if (!ok) { set_error("%s: the rows of the pages must begin on 16-byte boundaries", what); return NB200_ERR_ALIGNMENT; }
-  if (int64_t(c.heads) * c.page_size * (c.head_dim / vec) > 0x3fffffff) { set_error("%s: pages too large", what); return NB200_ERR_UNSUPPORTED; }
+  if (int64_t(c.heads) * c.page_size * (row / vec) > 0x3fffffff) { set_error("%s: pages too large", what); return NB200_ERR_UNSUPPORTED; }
   out->k = static_cast<uint4*>(c.k);
   out->v = static_cast<uint4*>(c.v);
   for (int i = 0; i < 3; ++i) {
     out->ks[i] = c.k_stride[i] / vec;
     out->vs[i] = c.v_stride[i] / vec;
   }
-  out->pages = c.pages; out->heads = c.heads; out->page_size = c.page_size; out->words = c.head_dim / vec;
+  out->pages = c.pages; out->heads = c.heads; out->page_size = c.page_size; out->words = row / vec;
   return NB200_OK;
 }
 
-int check_state(const nb200_cache_params* p, const char* what, Pages* pages) {
+StepPages step_pages(const nb200_cache_pages& c, const nb200_cache_steps* s) {
+  StepPages p{};
+  if (!s) return p;
+  p.k = static_cast<uint16_t*>(s->k);
+  p.v = static_cast<uint16_t*>(s->v);
+  for (int i = 0; i < 3; ++i) { p.ks[i] = s->k_stride[i]; p.vs[i] = s->v_stride[i]; }
+  p.groups = c.head_dim / kGroup;
+  return p;
+}
+
+int check_state(const nb200_cache_params* p, const nb200_cache_steps* steps, const char* what, Pages* pages) {
   if (!p || p->struct_size != sizeof(nb200_cache_params)) { set_error("%s: NULL params or wrong struct_size", what); return NB200_ERR_INVALID; }
-  if (int rc = check_pages(p->pages, what, pages)) return rc;
+  if (int rc = check_pages(p->pages, steps, what, pages)) return rc;
   if (p->rows < 0 || p->width <= 0) { set_error("%s: bad extents of the table", what); return NB200_ERR_INVALID; }
   if ((p->rows && (!p->table || !p->lengths)) || !p->free_range || (p->pages.pages && !p->free_pages)) {
     set_error("%s: NULL table, lengths, free_pages or free_range", what);
@@ -462,7 +541,7 @@ int check_state(const nb200_cache_params* p, const char* what, Pages* pages) {
   return NB200_OK;
 }
 
-int move_args(const nb200_cache_params* p, const char* what, const Pages& pages, MoveArgs* a, Layout* l, cudaStream_t st) {
+int move_args(const nb200_cache_params* p, const nb200_cache_steps* steps, const char* what, const Pages& pages, MoveArgs* a, Layout* l, cudaStream_t st) {
   *l = layout(pages.pages);
   if (!p->workspace || p->workspace_bytes < l->total * sizeof(int)) {
     set_error("%s: workspace of %zu bytes needed (nb200_cache_workspace_bytes), %zu given", what, l->total * sizeof(int), p->workspace_bytes);
@@ -471,6 +550,7 @@ int move_args(const nb200_cache_params* p, const char* what, const Pages& pages,
   int* ws = static_cast<int*>(p->workspace);
   *a = MoveArgs{};
   a->p = pages;
+  a->steps = step_pages(p->pages, steps);
   a->table = p->table; a->lengths = p->lengths; a->free_pages = p->free_pages; a->free_range = p->free_range;
   a->rows = p->rows; a->width = p->width; a->new_rows = p->new_rows;
   a->new_table = p->new_table; a->new_lengths = p->new_lengths;
@@ -493,31 +573,19 @@ int page_parts(const Pages& p) {
 
 unsigned list_grid(const Layout& l) { return l.words ? unsigned((l.words + kListWords - 1) / kListWords) : 1u; }
 
-}  // namespace
-}  // namespace nb200
-
-using namespace nb200;
-
-extern "C" NB200_API int nb200_cache_workspace_bytes(const nb200_cache_params* p, size_t* bytes) {
-  if (!p || p->struct_size != sizeof(nb200_cache_params) || !bytes) { set_error("cache_workspace_bytes: NULL or wrong struct_size"); return NB200_ERR_INVALID; }
-  if (p->pages.pages < 0) { set_error("cache_workspace_bytes: bad extents"); return NB200_ERR_INVALID; }
-  *bytes = layout(p->pages.pages).total * sizeof(int);
-  return NB200_OK;
-}
-
-extern "C" NB200_API int nb200_cache_append(const nb200_cache_params* p, void* cuda_stream) {
+int append(const nb200_cache_params* p, const nb200_cache_steps* steps, const char* what, void* cuda_stream) {
   AppendArgs a{};
-  if (int rc = check_state(p, "cache_append", &a.p)) return rc;
-  if (p->rows == 0) { set_error("cache_append: no rows"); return NB200_ERR_INVALID; }
+  if (int rc = check_state(p, steps, what, &a.p)) return rc;
+  if (p->rows == 0) { set_error("%s: no rows", what); return NB200_ERR_INVALID; }
   if (p->tokens < 0 || p->tokens > 0x7fffffff || !p->offsets || !p->new_lengths || !p->new_free_range || !p->shortfall ||
       (p->tokens && (!p->new_k || !p->new_v))) {
-    set_error("cache_append: NULL operand or bad number of tokens");
+    set_error("%s: NULL operand or bad number of tokens", what);
     return NB200_ERR_INVALID;
   }
   const int vec = p->pages.dtype == NB200_F32 ? 4 : 8;
   bool ok = aligned16(p->new_k) && aligned16(p->new_v);
   for (int i = 0; i < 2; ++i) ok = ok && p->new_k_stride[i] % vec == 0 && p->new_v_stride[i] % vec == 0;
-  if (!ok) { set_error("cache_append: the rows of k and v must begin on 16-byte boundaries"); return NB200_ERR_ALIGNMENT; }
+  if (!ok) { set_error("%s: the rows of k and v must begin on 16-byte boundaries", what); return NB200_ERR_ALIGNMENT; }
   a.table = p->table; a.lengths = p->lengths; a.offsets = p->offsets; a.free_pages = p->free_pages; a.free_range = p->free_range;
   a.rows = p->rows; a.width = p->width;
   a.new_lengths = p->new_lengths; a.new_free_range = p->new_free_range; a.shortfall = p->shortfall;
@@ -534,29 +602,37 @@ extern "C" NB200_API int nb200_cache_append(const nb200_cache_params* p, void* c
   const unsigned grid = unsigned((p->tokens + per_cta - 1) / per_cta) + 1u;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  cache_append_kernel<<<grid, kThreads, 0, st>>>(a);
+  a.steps = step_pages(p->pages, steps);
+  void (*kernel)(AppendArgs) = cache_append_kernel<0, uint4>;
+  if (steps) {
+    const bool four = steps->bits == 4;
+    kernel = p->pages.dtype == NB200_F32    ? four ? cache_append_kernel<4, float> : cache_append_kernel<8, float>
+             : p->pages.dtype == NB200_BF16 ? four ? cache_append_kernel<4, __nv_bfloat16> : cache_append_kernel<8, __nv_bfloat16>
+             : four                         ? cache_append_kernel<4, __half> : cache_append_kernel<8, __half>;
+  }
+  kernel<<<grid, kThreads, 0, st>>>(a);
   count_launch();
-  return check_launch("cache_append_kernel");
+  return check_launch(steps ? "cache_append_kernel<quantized>" : "cache_append_kernel");
 }
 
-extern "C" NB200_API int nb200_cache_fork(const nb200_cache_params* p, void* cuda_stream) {
+int fork(const nb200_cache_params* p, const nb200_cache_steps* steps, const char* what, void* cuda_stream) {
   Pages pages;
-  if (int rc = check_state(p, "cache_fork", &pages)) return rc;
+  if (int rc = check_state(p, steps, what, &pages)) return rc;
   if (p->new_rows < 0 || !p->new_free_range || !p->shortfall || (pages.pages && !p->new_free_pages) ||
       (p->new_rows && (!p->new_table || !p->new_lengths || (!p->parents && !p->finished)))) {
-    set_error("cache_fork: NULL operand or bad number of rows");
+    set_error("%s: NULL operand or bad number of rows", what);
     return NB200_ERR_INVALID;
   }
-  if (p->new_rows && !p->parents && p->new_rows != p->rows) { set_error("cache_fork: finished names %d rows of %d", p->new_rows, p->rows); return NB200_ERR_INVALID; }
-  if (p->rows > 262144) { set_error("cache_fork: %d rows, at most 262144", p->rows); return NB200_ERR_UNSUPPORTED; }   // bits in shared memory
+  if (p->new_rows && !p->parents && p->new_rows != p->rows) { set_error("%s: finished names %d rows of %d", what, p->new_rows, p->rows); return NB200_ERR_INVALID; }
+  if (p->rows > 262144) { set_error("%s: %d rows, at most 262144", what, p->rows); return NB200_ERR_UNSUPPORTED; }   // bits in shared memory
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   MoveArgs a;
   Layout l;
-  if (int rc = move_args(p, "cache_fork", pages, &a, &l, st)) return rc;
+  if (int rc = move_args(p, steps, what, pages, &a, &l, st)) return rc;
   a.parents = p->parents; a.finished = p->finished; a.shortfall = p->shortfall;
   if (p->new_rows > 0) {
-    cache_fork_rows_kernel<<<dim3(unsigned(p->new_rows), unsigned(page_parts(pages))), kThreads, size_t((p->rows + 31) / 32) * sizeof(unsigned), st>>>(a);
+    (steps ? cache_fork_rows_kernel<true> : cache_fork_rows_kernel<false>)<<<dim3(unsigned(p->new_rows), unsigned(page_parts(pages))), kThreads, size_t((p->rows + 31) / 32) * sizeof(unsigned), st>>>(a);
     count_launch();
     if (int rc = check_launch("cache_fork_rows_kernel")) return rc;
   }
@@ -566,15 +642,15 @@ extern "C" NB200_API int nb200_cache_fork(const nb200_cache_params* p, void* cud
   return check_launch("cache_list_kernel");
 }
 
-extern "C" NB200_API int nb200_cache_compact(const nb200_cache_params* p, void* cuda_stream) {
+int compact(const nb200_cache_params* p, const nb200_cache_steps* steps, const char* what, void* cuda_stream) {
   Pages pages;
-  if (int rc = check_state(p, "cache_compact", &pages)) return rc;
-  if ((p->rows && !p->new_table) || (pages.pages && !p->new_free_pages) || !p->new_free_range || !p->shortfall) { set_error("cache_compact: NULL operand"); return NB200_ERR_INVALID; }
+  if (int rc = check_state(p, steps, what, &pages)) return rc;
+  if ((p->rows && !p->new_table) || (pages.pages && !p->new_free_pages) || !p->new_free_range || !p->shortfall) { set_error("%s: NULL operand", what); return NB200_ERR_INVALID; }
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   MoveArgs a;
   Layout l;
-  if (int rc = move_args(p, "cache_compact", pages, &a, &l, st)) return rc;
+  if (int rc = move_args(p, steps, what, pages, &a, &l, st)) return rc;
   a.shortfall = p->shortfall;      // (nothing is dropped)
   if (p->rows > 0) {
     cache_mark_kernel<<<unsigned(p->rows), kThreads, 0, st>>>(a);
@@ -590,7 +666,43 @@ extern "C" NB200_API int nb200_cache_compact(const nb200_cache_params* p, void* 
   int64_t grid = int64_t(pages.pages + 1) / 2 * parts;
   if (grid < p->rows) grid = p->rows;
   grid = grid < 1 ? 1 : grid > 65536 ? 65536 : grid;
-  if (launch_dependent(cache_move_kernel, unsigned(grid), kThreads, 0, st, a, parts) != cudaSuccess) return check_launch("cache_move_kernel");
+  if (launch_dependent(steps ? cache_move_kernel<true> : cache_move_kernel<false>, unsigned(grid), kThreads, 0, st, a, parts) != cudaSuccess) return check_launch("cache_move_kernel");
   count_launch();
   return check_launch("cache_move_kernel");
+}
+
+// A parameter block of a cache in few bits is one around the other cache's.
+int check_quantized(const nb200_cache_quantized_params* p, const char* what) {
+  if (p && p->struct_size == sizeof(nb200_cache_quantized_params)) return NB200_OK;
+  set_error("%s: NULL params or wrong struct_size", what);
+  return NB200_ERR_INVALID;
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" NB200_API int nb200_cache_workspace_bytes(const nb200_cache_params* p, size_t* bytes) {
+  if (!p || p->struct_size != sizeof(nb200_cache_params) || !bytes) { set_error("cache_workspace_bytes: NULL or wrong struct_size"); return NB200_ERR_INVALID; }
+  if (p->pages.pages < 0) { set_error("cache_workspace_bytes: bad extents"); return NB200_ERR_INVALID; }
+  *bytes = layout(p->pages.pages).total * sizeof(int);
+  return NB200_OK;
+}
+
+extern "C" NB200_API int nb200_cache_append(const nb200_cache_params* p, void* cuda_stream) { return append(p, nullptr, "cache_append", cuda_stream); }
+extern "C" NB200_API int nb200_cache_fork(const nb200_cache_params* p, void* cuda_stream) { return fork(p, nullptr, "cache_fork", cuda_stream); }
+extern "C" NB200_API int nb200_cache_compact(const nb200_cache_params* p, void* cuda_stream) { return compact(p, nullptr, "cache_compact", cuda_stream); }
+
+extern "C" NB200_API int nb200_cache_append_quantized(const nb200_cache_quantized_params* p, void* cuda_stream) {
+  if (int rc = check_quantized(p, "cache_append_quantized")) return rc;
+  return append(&p->cache, &p->steps, "cache_append_quantized", cuda_stream);
+}
+extern "C" NB200_API int nb200_cache_fork_quantized(const nb200_cache_quantized_params* p, void* cuda_stream) {
+  if (int rc = check_quantized(p, "cache_fork_quantized")) return rc;
+  return fork(&p->cache, &p->steps, "cache_fork_quantized", cuda_stream);
+}
+extern "C" NB200_API int nb200_cache_compact_quantized(const nb200_cache_quantized_params* p, void* cuda_stream) {
+  if (int rc = check_quantized(p, "cache_compact_quantized")) return rc;
+  return compact(&p->cache, &p->steps, "cache_compact_quantized", cuda_stream);
 }

@@ -1,4 +1,5 @@
-"""``nitrix.nn.layer_norm`` on the B200 library: the reference's dispatcher surface over the fused CUDA kernels.
+"""``nitrix.nn.layer_norm`` on the B200 library: the reference's dispatcher surface over the fused CUDA kernels; and the
+root-mean-square norm of decoder layers (``include/nitrix_b200_rms_norm.h``), which the reference does not have.
 
 Mirrors the reference's public function (``src/nitrix/nn/norm/__init__.py:110-176``): same arguments, the same
 ``ValueError`` for a mis-shaped ``weight`` / ``bias`` (``:44-54``), normalisation over the trailing axis with the
@@ -10,14 +11,14 @@ no host path: without a CUDA device or without the built library the call raises
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 
 from .. import _cabi
 from ..backend import resolve_backend
 
-__all__ = ["layer_norm"]
+__all__ = ["layer_norm", "rms_norm", "rms_norm_quantized"]
 
 _DTYPES = {torch.float32: _cabi.F32, torch.bfloat16: _cabi.BF16, torch.float16: _cabi.F16}
 
@@ -90,3 +91,30 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if x.numel() == 0:
         return torch.empty_like(x)
     return _cabi.torch_ops().layer_norm(x, weight, bias, float(eps), float(out_scale))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             backend: str = "auto") -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Root-mean-square norm over the trailing axis, ``x * (mean(x ** 2) + eps) ** -0.5 * weight``.
+
+    With ``residual``, of ``x``'s shape and dtype, the two streams are added first: ``(y, h)`` comes back, where ``h`` is
+    ``x + residual`` in their dtype and ``y`` the norm of ``h``.  ``x`` is a CUDA tensor of fp32, bf16 or fp16, ``weight`` of the
+    same dtype or fp32 with shape ``(c,)``; the arithmetic is fp32, rounded once.  Differentiable in ``x``, ``residual`` and ``weight``."""
+    resolve_backend(backend)   # raises without a Blackwell device: there is no host path
+    y, h = _cabi.torch_ops().rms_norm(x, residual, weight, float(eps))
+    return y if residual is None else (y, h)
+
+
+def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       group_size: Optional[int] = None, backend: str = "auto") -> Tuple[torch.Tensor, ...]:
+    """:func:`rms_norm` with an output in 8 bits: ``(codes, scales)``, with ``residual`` ``(codes, scales, h)``.
+
+    ``codes`` is ``torch.float8_e4m3fn`` of ``x``'s shape, ``scales`` fp32 with a last axis of one element (``group_size=None``) or
+    one for each ``group_size`` channels (32, 64 or 128, which must divide them); ``codes * scales`` stands for the norm.  A scale is
+    the largest magnitude over 448, and what is rounded has not been rounded before.  A row with a NaN or an infinity has NaN codes.
+    Not differentiable."""
+    resolve_backend(backend)
+    if group_size is not None and group_size not in (32, 64, 128):
+        raise ValueError(f"rms_norm_quantized: group_size must be 32, 64 or 128, or None for whole rows; got {group_size}")
+    codes, scales, h = _cabi.torch_ops().rms_norm_quantized(x, residual, weight, float(eps), group_size or 0)
+    return (codes, scales) if residual is None else (codes, scales, h)
