@@ -124,7 +124,267 @@ struct QuantizedFmaLoop {
   }
 };
 
+// 16-bit queries, head dim 64 or 128: warp-level MMAs.  Tokens are the M side of the scores (S^T = K Q^T), elements that of the output
+// (O^T = V^T P^T), as in decode.cu.
+//
+// Codes become operands without a conversion: the bits of a whole number below 1024 in an fp16 are that number times 2^-24, so a
+// mask of a word that holds codes of two operands' halves gives both (in 4 bits every other element's code stands four bits up,
+// which is times 16: the queries have 1/16 there, the output's rows get it at the end).  Queries are fp16, by a power of two per head
+// that brings the largest near 2^10: bf16 has 8 bits, so that nothing is lost above 2^-24 of it.
+// Steps: those of a key's groups multiply the groups' sums, fp32, of which the half of the codes' range has been taken off
+// beforehand (the accumulators begin with it); those of a value's groups multiply its probability before that is rounded to fp16,
+// once, for each group.  The reference maximum is that of score + log2 of the value's largest step, so that no product leaves
+// fp16 and small ones keep their bits whatever the steps are; the sum of the probabilities is fp32.  Values' codes lose the half of
+// their range before the product: a sum of 10^5 tokens would lose more by it than fp32 holds.
+template <typename T, int D, int kBits, int kTiles>
+struct QuantizedMmaLoop {
+  static constexpr const char* kName = "decode_kernel<quantized>";
+  static constexpr int kHeads = 8 * kTiles;
+  static constexpr int kBlock = 16;              // tokens
+  static constexpr int kSlots = 1;
+  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : 4) : D == 64 ? 4 : 2;
+  static constexpr int kG = D / kGroup;          // groups
+  static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
+  static constexpr float kUp = 7.f;              // log2 of what probabilities are kept at: their products are below 2^15
+  float o[kTiles][D / 16][4];
+  float m[kTiles][2], l[kTiles][2];
+
+  template <int n>
+  __device__ __forceinline__ static void load_words(uint32_t (&w)[n], const void* p) {
+    if constexpr (n == 1) {
+      asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    } else if constexpr (n == 2) {
+      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < n / 4; ++i) {
+        const uint4 v = sm100::ldg_no_allocate(static_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    }
+  }
+  // Elements 0 .. 3 of group i of two parts (or of two tokens' same part), as halves of four words.
+  __device__ __forceinline__ static void codes(uint32_t (&e)[4], const uint32_t* a, const uint32_t* b, int i) {
+    if constexpr (kBits == 4) {
+      const uint32_t x = __byte_perm(a[i / 2], b[i / 2], i % 2 ? 0x7632 : 0x5410), y = x >> 8;
+      e[0] = x & 0x000f000fu; e[1] = x & 0x00f000f0u; e[2] = y & 0x000f000fu; e[3] = y & 0x00f000f0u;
+    } else {
+      const uint32_t x = __byte_perm(a[i], b[i], 0x5410), y = __byte_perm(a[i], b[i], 0x7632);
+      e[0] = x & 0x00ff00ffu; e[1] = x >> 8 & 0x00ff00ffu; e[2] = y & 0x00ff00ffu; e[3] = y >> 8 & 0x00ff00ffu;
+    }
+  }
+  // minus the half of the range, for even and odd elements
+  static constexpr uint32_t kEven = kBits == 4 ? 0x80088008u : 0x80808080u, kOdd = 0x80808080u;
+  __device__ __forceinline__ static uint32_t plus(uint32_t a, uint32_t b) {
+    uint32_t c;
+    asm("add.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+  }
+  __device__ __forceinline__ static float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  // step of group i
+  __device__ __forceinline__ static float step(const uint32_t (&w)[kG / 2], int i) { return i % 2 ? halves(w[i / 2]).y : halves(w[i / 2]).x; }
+
+  __device__ __forceinline__ void run(const QuantizedArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0, int t1,
+                                      int wi, int wn) {
+    const T* q = static_cast<const T*>(q_row);
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t qf[kTiles][kG][4];
+    float back[kTiles][2], half[kTiles][kG][2];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      float x[kG][8], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        const uint4 w = n * 8 + g < heads ? *reinterpret_cast<const uint4*>(q + (n * 8 + g) * a.qs[1] + i * kGroup + t * 8) : make_uint4(0, 0, 0, 0);
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[i][j] = to_f32<T>(e[j]);
+          top = fmaxf(top, fabsf(x[i][j]));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int size = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 110);
+      const float up = __uint_as_float(uint32_t(127 + 9 - size) << 23), down = __uint_as_float(uint32_t(127 + 15 + size) << 23);
+      back[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      back[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = kBits == 4 && e % 2 ? up * (1.f / 16.f) : up;
+          qf[n][i][e] = pack2<false>(x[i][e] * f, x[i][4 + e] * f);
+        }
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816<false>(c, kEven, kEven, kOdd, kOdd, qf[n][i][0], qf[n][i][1]);
+        mma16816<false>(c, kEven, kEven, kOdd, kOdd, qf[n][i][2], qf[n][i][3]);
+        half[n][i][0] = c[0];
+        half[n][i][1] = c[1];
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
+    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
+    const int last = t1 - 1;
+    uint32_t kw[2][2 * kW], vw[4][kW], kt[2][kG / 2], vt[2][kG / 2];
+    // (blocks begin at multiples of 16 tokens: in pages of 16, 32, ... slots the page is looked up once, a turn ahead)
+    const bool one_page = a.page_shift >= 4;
+    auto page_of_block = [&](int b) { return one_page && b < t1 ? page_at(a, row_table, b >> a.page_shift) : 0; };
+    // (behind the last token that one's rows are read again, with a probability of zero)
+    auto place = [&](int b, int page, int token) {
+      token = min(token, last);
+      if (one_page) return Where{page, (b & (a.page_size - 1)) + token - b};
+      return where(a, row_table, token);
+    };
+    auto load_k = [&](int b, int page) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const Where at = place(b, page, b + g + 8 * r);
+        load_words(kw[r], reinterpret_cast<const uint32_t*>(row_of(kbase, a.ks, at)) + 2 * kW * t);
+        load_words(kt[r], steps_of(a.k_steps, a.kss, kG, kv_head, at));
+        load_words(vt[r], steps_of(a.v_steps, a.vss, kG, kv_head, at));
+      }
+    };
+    auto load_v = [&](int b, int page) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        load_words(vw[r], reinterpret_cast<const uint32_t*>(row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8))) + kW * g);
+    };
+    int b0 = t0 + wi * kBlock;
+    if (b0 >= t1) return;
+    int next_page = page_of_block(b0);
+    load_k(b0, next_page);
+    load_v(b0, next_page);
+    next_page = page_of_block(b0 + wn * kBlock);
+    for (; b0 < t1; b0 += wn * kBlock) {
+      const int next = b0 + wn * kBlock;
+      float s[kTiles][4];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        uint32_t e0[4], e1[4];
+        codes(e0, kw[0], kw[0] + kW, i);
+        codes(e1, kw[1], kw[1] + kW, i);
+        const float k0 = step(kt[0], i), k1 = step(kt[1], i);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          float c[4] = {half[n][i][0], half[n][i][1], half[n][i][0], half[n][i][1]};
+          mma16816<false>(c, e0[0], e1[0], e0[1], e1[1], qf[n][i][0], qf[n][i][1]);
+          mma16816<false>(c, e0[2], e1[2], e0[3], e1[3], qf[n][i][2], qf[n][i][3]);
+          s[n][0] = fmaf(k0, c[0], s[n][0]);
+          s[n][1] = fmaf(k0, c[1], s[n][1]);
+          s[n][2] = fmaf(k1, c[2], s[n][2]);
+          s[n][3] = fmaf(k1, c[3], s[n][3]);
+        }
+      }
+      float v0[kG], v1[kG], top0 = 0.f, top1 = 0.f;      // steps of the values of tokens g and g + 8
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        v0[i] = step(vt[0], i);
+        v1[i] = step(vt[1], i);
+        top0 = fmaxf(top0, fabsf(v0[i]));
+        top1 = fmaxf(top1, fabsf(v1[i]));
+      }
+      if (next < t1) load_k(next, next_page);
+      const bool in0 = b0 + g < t1, in1 = b0 + g + 8 < t1;
+      const float log0 = in0 ? fmaxf(__log2f(top0), -24.f) : -INFINITY, log1 = in1 ? fmaxf(__log2f(top1), -24.f) : -INFINITY;
+      uint32_t pt[kTiles][kG][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= back[n][j & 1];
+        // The reference maximum moves only when a token passes it by more than 2^8.
+        const float mx0 = fmaxf(fmaf(s[n][0], a.mul, log0), fmaf(s[n][2], a.mul, log1));
+        const float mx1 = fmaxf(fmaf(s[n][1], a.mul, log0), fmaf(s[n][3], a.mul, log1));
+        if (__any_sync(0xffffffffu, mx0 > m[n][0] + 8.f || mx1 > m[n][1] + 8.f)) {
+          float x0 = mx0, x1 = mx1;
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+          }
+          x0 = fmaxf(x0, m[n][0]);
+          x1 = fmaxf(x1, m[n][1]);
+          const float c0 = x0 > m[n][0] ? ex2(m[n][0] - x0) : 1.f, c1 = x1 > m[n][1] ? ex2(m[n][1] - x1) : 1.f;
+          m[n][0] = x0;
+          m[n][1] = x1;
+          l[n][0] *= c0;
+          l[n][1] *= c1;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][0] *= c0; o[n][i][1] *= c1; o[n][i][2] *= c0; o[n][i][3] *= c1;
+          }
+        }
+        const float up0 = m[n][0] == -INFINITY ? kUp : kUp - m[n][0], up1 = m[n][1] == -INFINITY ? kUp : kUp - m[n][1];
+        const float p0 = in0 ? ex2(fmaf(s[n][0], a.mul, up0)) : 0.f, p1 = in0 ? ex2(fmaf(s[n][1], a.mul, up1)) : 0.f;
+        const float p2 = in1 ? ex2(fmaf(s[n][2], a.mul, up0)) : 0.f, p3 = in1 ? ex2(fmaf(s[n][3], a.mul, up1)) : 0.f;
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+          pt[n][i][0] = transpose8x8(pack2<false>(p0 * v0[i], p1 * v0[i]));
+          pt[n][i][1] = transpose8x8(pack2<false>(p2 * v1[i], p3 * v1[i]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        uint32_t e0[4], e1[4];      // of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+        codes(e0, vw[0], vw[1], i);
+        codes(e1, vw[2], vw[3], i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          e0[e] = plus(e0[e], e % 2 ? kOdd : kEven);
+          e1[e] = plus(e1[e], e % 2 ? kOdd : kEven);
+        }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          mma16816<false>(o[n][2 * i], e0[0], e0[1], e1[0], e1[1], pt[n][i][0], pt[n][i][1]);
+          mma16816<false>(o[n][2 * i + 1], e0[2], e0[3], e1[2], e1[3], pt[n][i][0], pt[n][i][1]);
+        }
+      }
+      if (next < t1) load_v(next, next_page);
+      next_page = page_of_block(next + wn * kBlock);
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
+        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
+      }
+  }
+
+  __device__ __forceinline__ void store(const QuantizedArgs& a, float* dst) const {
+    constexpr float kScale = 16777216.f, kOddScale = kBits == 4 ? kScale / 16.f : kScale;      // of codes as fp16
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float* slot = dst + (threadIdx.x >> 5) * kHeads * (D + 2);
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float* row = slot + (n * 8 + 2 * t + hh) * (D + 2);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          *reinterpret_cast<float2*>(row + (i / 2) * kGroup + 4 * g + 2 * (i & 1)) = make_float2(o[n][i][hh] * kScale, o[n][i][2 + hh] * kOddScale);
+        if (g == 0) {
+          row[D] = m[n][hh] == -INFINITY ? -INFINITY : m[n][hh] - kUp;
+          row[D + 1] = l[n][hh];
+        }
+      }
+  }
+};
+
 struct Plan {
+  bool mma;
   int heads, side, chunks;      // query heads of a chunk, chunks side by side, times that a group is taken
   int unit, workers;
   size_t bytes;
@@ -152,8 +412,16 @@ Plan plan(const nb200_decode_params* p) {
   const nb200_cache_pages& c = p->pages;
   Plan pl{};
   const int group = p->q_heads / c.heads;
-  pl.heads = c.head_dim > 128 ? 2 : 4;
-  const int ctas = 2;      // resident per SM: the loops' kMinCtas
+  bool q_words = aligned16(p->q);
+  for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
+  pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words;
+  int ctas = 2;      // resident per SM: the loops' kMinCtas
+  if (pl.mma) {
+    pl.heads = group > 8 ? 16 : 8;
+    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 5 : 4) : c.head_dim == 64 ? 4 : 2;
+  } else {
+    pl.heads = c.head_dim > 128 ? 2 : 4;
+  }
   const int chunks = (group + pl.heads - 1) / pl.heads;
   pl.side = chunks == 1 ? 1 : chunks == 2 ? 2 : 4;
   pl.chunks = (chunks + pl.side - 1) / pl.side;
@@ -170,6 +438,18 @@ int launch_fma(const QuantizedArgs& a, int side, cudaStream_t st) {
   if (a.groups <= 2) return launch<T, QuantizedFmaLoop<T, kBits, 2, 4>, false>(a, side, st);
   if (a.groups <= 4) return launch<T, QuantizedFmaLoop<T, kBits, 4, 4>, false>(a, side, st);
   return launch<T, QuantizedFmaLoop<T, kBits, 8, 2>, false>(a, side, st);
+}
+
+template <typename T, int kBits>
+int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
+  if (a.D == 64) return heads == 8 ? launch<T, QuantizedMmaLoop<T, 64, kBits, 1>, true>(a, side, st) : launch<T, QuantizedMmaLoop<T, 64, kBits, 2>, false>(a, side, st);
+  return heads == 8 ? launch<T, QuantizedMmaLoop<T, 128, kBits, 1>, true>(a, side, st) : launch<T, QuantizedMmaLoop<T, 128, kBits, 2>, false>(a, side, st);
+}
+
+template <typename T>
+int launch_16(const QuantizedArgs& a, const Plan& pl, bool four, cudaStream_t st) {
+  if (pl.mma) return four ? launch_mma<T, 4>(a, pl.heads, pl.side, st) : launch_mma<T, 8>(a, pl.heads, pl.side, st);
+  return four ? launch_fma<T, 4>(a, pl.side, st) : launch_fma<T, 8>(a, pl.side, st);
 }
 
 }  // namespace
@@ -233,6 +513,5 @@ extern "C" NB200_API int nb200_decode_quantized(const nb200_decode_quantized_par
   prof_call_begin(st);
   const bool four = qp->steps.bits == 4;
   if (c.dtype == NB200_F32) return four ? launch_fma<float, 4>(a, pl.side, st) : launch_fma<float, 8>(a, pl.side, st);
-  if (c.dtype == NB200_BF16) return four ? launch_fma<__nv_bfloat16, 4>(a, pl.side, st) : launch_fma<__nv_bfloat16, 8>(a, pl.side, st);
-  return four ? launch_fma<__half, 4>(a, pl.side, st) : launch_fma<__half, 8>(a, pl.side, st);
+  return c.dtype == NB200_BF16 ? launch_16<__nv_bfloat16>(a, pl, four, st) : launch_16<__half>(a, pl, four, st);
 }

@@ -288,16 +288,18 @@ def _filled(lengths, page_size, Hk, dim, bits, seed=0, layout="heads", std=1.0):
     return c
 
 
-def _check_decode(q, cache, lengths, bits, scale=None):
+def _check_decode(q, cache, lengths, bits, scale=None, spoiled=None):
+    """``spoiled``: the elements that have to be NaN; all others must be good."""
     from nitrix_b200.nn import decode_attention
 
     got = decode_attention(q, cache, scale=scale)
     k, v = O.cache_values(cache, bits)
     want, spread, reach = O.decode(q, k, v, cache.table, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
-    assert got.dtype == q.dtype and got.shape == q.shape and not bool(got.isnan().any())
+    assert got.dtype == q.dtype and got.shape == q.shape
+    assert torch.equal(got.isnan(), torch.zeros_like(got, dtype=torch.bool) if spoiled is None else spoiled)
     p_rounding = 0 if q.dtype == torch.float32 else 2.0 ** -11
     bound = HALF[q.dtype] * want.abs() + (p_rounding + 2 * 16 * 2.0 ** -24 * (1 + reach) + 2.0 ** -20) * 2 * spread
-    err = (got.double() - want).abs() - bound - 2.0 ** -25
+    err = ((got.double() - want).abs() - bound - 2.0 ** -25)[~got.isnan()]
     assert float(err.max()) <= 0, float(err.max())
     return got
 
@@ -357,24 +359,21 @@ def test_decode_values_of_very_different_size(bits, dtype, dim):
 
 
 def test_decode_what_is_not_finite_stays_in_its_group():
-    """A step that is NaN or infinite spoils what it stands in, nothing else."""
-    from nitrix_b200.nn import decode_attention
-
+    """A step that is NaN spoils what it stands in, nothing else.  (What the others are rounded at goes by the largest step of a token's
+    values, so that they need not be the same bits as without it.)"""
     lengths = [50, 20]
-    for dtype in DTYPES:
-        cache = _filled(lengths, 16, 2, 64, 4)
-        q = torch.randn(2, 4, 64, device="cuda").to(dtype)
-        clean = decode_attention(q, cache)
-        page, slot = int(cache.table[0, 1]), 3      # token 19 of the first sequence, of key head 1 the second group
-        cache.v_steps[page, 1, slot, 1] = float("nan")
-        got = decode_attention(q, cache)
-        assert bool(got[0, 2:, 32:].isnan().all())
-        keep = torch.ones_like(got, dtype=torch.bool)
-        keep[0, 2:, 32:] = False
-        assert torch.equal(got[keep], clean[keep])
-        cache.k_steps[page, 0, slot, 0] = float("nan")
-        got = decode_attention(q, cache)
-        assert bool(got[0, :2].isnan().all()) and torch.equal(got[1], clean[1])
+    for bits in (4, 8):
+        for dtype in DTYPES:
+            cache = _filled(lengths, 16, 2, 64, bits)
+            q = torch.randn(2, 4, 64, device="cuda").to(dtype)
+            spoiled = torch.zeros(2, 4, 64, dtype=torch.bool, device="cuda")
+            page, slot = int(cache.table[0, 1]), 3      # token 19 of the first sequence, of key head 1 the second group
+            cache.v_steps[page, 1, slot, 1] = float("nan")
+            spoiled[0, 2:, 32:] = True
+            _check_decode(q, cache, lengths, bits, spoiled=spoiled)
+            cache.k_steps[page, 0, slot, 0] = float("nan")
+            spoiled[0, :2] = True
+            _check_decode(q, cache, lengths, bits, spoiled=spoiled)
 
 
 def test_decode_layouts_and_misaligned_queries():
