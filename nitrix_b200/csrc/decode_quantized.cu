@@ -135,8 +135,8 @@ struct QuantizedFmaLoop {
 // beforehand (the accumulators begin with it); those of a value's groups multiply its probability before that is rounded to fp16,
 // once, for each group.  The reference maximum is that of score + log2 of the value's largest step, so that no product leaves
 // fp16 and small ones keep their bits whatever the steps are; the sum of the probabilities is fp32.  Values' codes lose the half of
-// their range before the product: a sum of 10^5 tokens would lose more by it than fp32 holds.
-template <typename T, int D, int kBits, int kTiles>
+// their range before the product, two at a time: taken off the sums instead, by MMAs of their own, it leaves errors of 2^-18 of it.
+template <typename T, int D, int kBits, int kTiles, bool kDense>
 struct QuantizedMmaLoop {
   static constexpr const char* kName = "decode_kernel<quantized>";
   static constexpr int kHeads = 8 * kTiles;
@@ -145,9 +145,11 @@ struct QuantizedMmaLoop {
   static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : 4) : D == 64 ? 4 : 2;
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
+  static constexpr int kRow = D * kBits / 8;     // bytes of a row of codes
   static constexpr float kUp = 7.f;              // log2 of what probabilities are kept at: their products are below 2^15
   float o[kTiles][D / 16][4];
-  float m[kTiles][2], l[kTiles][2];
+  float m[kTiles][2];
+  float2 l[kTiles];
 
   template <int n>
   __device__ __forceinline__ static void load_words(uint32_t (&w)[n], const void* p) {
@@ -180,6 +182,12 @@ struct QuantizedMmaLoop {
     asm("add.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
     return c;
   }
+  // d = c + A B
+  __device__ __forceinline__ static void mma(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  }
   __device__ __forceinline__ static float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
   // step of group i
   __device__ __forceinline__ static float step(const uint32_t (&w)[kG / 2], int i) { return i % 2 ? halves(w[i / 2]).y : halves(w[i / 2]).x; }
@@ -189,7 +197,8 @@ struct QuantizedMmaLoop {
     const T* q = static_cast<const T*>(q_row);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t qf[kTiles][kG][4];
-    float back[kTiles][2], half[kTiles][kG][2];
+    float2 back[kTiles];
+    float half[kTiles][kG][2];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       float x[kG][8], top = 0.f;
@@ -207,8 +216,7 @@ struct QuantizedMmaLoop {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int size = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 110);
       const float up = __uint_as_float(uint32_t(127 + 9 - size) << 23), down = __uint_as_float(uint32_t(127 + 15 + size) << 23);
-      back[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
-      back[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+      back[n] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
 #pragma unroll
       for (int i = 0; i < kG; ++i) {
 #pragma unroll
@@ -227,22 +235,45 @@ struct QuantizedMmaLoop {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
       m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+      l[n] = make_float2(0.f, 0.f);
     }
     const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
     const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
     const int last = t1 - 1;
     uint32_t kw[2][2 * kW], vw[4][kW], kt[2][kG / 2], vt[2][kG / 2];
+    // kDense: pages of 16, 32, ... slots that lie side by side, of one layout for keys and values.  A lane's places in a block are
+    // then constants from the block's.
+    const char *k_lane, *v_lane, *kt_lane, *vt_lane;
+    if constexpr (kDense) {
+      k_lane = reinterpret_cast<const char*>(kbase) + g * kRow + t * 8 * kW;
+      v_lane = reinterpret_cast<const char*>(vbase) + 2 * t * kRow + g * 4 * kW;
+      const int64_t head = int64_t(kv_head) * a.kss[1] * kG + g * kG;
+      kt_lane = reinterpret_cast<const char*>(a.k_steps + head);
+      vt_lane = reinterpret_cast<const char*>(a.v_steps + head);
+    }
+    const int64_t page_bytes = int64_t(a.ks[0]) * 16, page_steps = int64_t(a.kss[0]) * (2 * kG);
     // (blocks begin at multiples of 16 tokens: in pages of 16, 32, ... slots the page is looked up once, a turn ahead)
-    const bool one_page = a.page_shift >= 4;
-    auto page_of_block = [&](int b) { return one_page && b < t1 ? page_at(a, row_table, b >> a.page_shift) : 0; };
-    // (behind the last token that one's rows are read again, with a probability of zero)
+    const bool one_page = kDense || a.page_shift >= 4;
+    auto page_of_block = [&](int b) { return one_page ? page_at(a, row_table, min(b, last) >> a.page_shift) : 0; };
+    // (behind the last token: with kDense what stands in its page, whose steps are set to zero, otherwise that token's rows again; with
+    // a probability of zero)
     auto place = [&](int b, int page, int token) {
       token = min(token, last);
       if (one_page) return Where{page, (b & (a.page_size - 1)) + token - b};
       return where(a, row_table, token);
     };
     auto load_k = [&](int b, int page) {
+      if constexpr (kDense) {
+        const int slot = b & (a.page_size - 1);
+        const int64_t at = page * page_bytes + slot * kRow, steps = page * page_steps + slot * (2 * kG);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          load_words(kw[r], k_lane + at + r * 8 * kRow);
+          load_words(kt[r], kt_lane + steps + r * 16 * kG);
+          load_words(vt[r], vt_lane + steps + r * 16 * kG);
+        }
+        return;
+      }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const Where at = place(b, page, b + g + 8 * r);
@@ -252,6 +283,12 @@ struct QuantizedMmaLoop {
       }
     };
     auto load_v = [&](int b, int page) {
+      if constexpr (kDense) {
+        const int64_t at = page * page_bytes + (b & (a.page_size - 1)) * kRow;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_words(vw[r], v_lane + at + ((r & 1) + (r >> 1) * 8) * kRow);
+        return;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         load_words(vw[r], reinterpret_cast<const uint32_t*>(row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8))) + kW * g);
@@ -263,12 +300,17 @@ struct QuantizedMmaLoop {
     load_v(b0, next_page);
     next_page = page_of_block(b0 + wn * kBlock);
     for (; b0 < t1; b0 += wn * kBlock) {
-      const int next = b0 + wn * kBlock;
-      float s[kTiles][4];
+      const int next = min(b0 + wn * kBlock, last & ~(kBlock - 1));      // (the last block may be asked for again, in vain)
+      if (kDense && b0 + kBlock > t1) {
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n)
+        for (int i = 0; i < kG / 2; ++i) {
+          if (b0 + g >= t1) vt[0][i] = 0;
+          if (b0 + g + 8 >= t1) vt[1][i] = 0;
+        }
+      }
+      float2 s[kTiles][2];      // of tokens g, g + 8: heads 2t, 2t + 1
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+      for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < kG; ++i) {
         uint32_t e0[4], e1[4];
@@ -277,13 +319,11 @@ struct QuantizedMmaLoop {
         const float k0 = step(kt[0], i), k1 = step(kt[1], i);
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-          float c[4] = {half[n][i][0], half[n][i][1], half[n][i][0], half[n][i][1]};
-          mma16816<false>(c, e0[0], e1[0], e0[1], e1[1], qf[n][i][0], qf[n][i][1]);
-          mma16816<false>(c, e0[2], e1[2], e0[3], e1[3], qf[n][i][2], qf[n][i][3]);
-          s[n][0] = fmaf(k0, c[0], s[n][0]);
-          s[n][1] = fmaf(k0, c[1], s[n][1]);
-          s[n][2] = fmaf(k1, c[2], s[n][2]);
-          s[n][3] = fmaf(k1, c[3], s[n][3]);
+          float c[4];
+          mma(c, {half[n][i][0], half[n][i][1], half[n][i][0], half[n][i][1]}, e0[0], e1[0], e0[1], e1[1], qf[n][i][0], qf[n][i][1]);
+          mma(c, c, e0[2], e1[2], e0[3], e1[3], qf[n][i][2], qf[n][i][3]);
+          s[n][0] = __ffma2_rn(make_float2(k0, k0), make_float2(c[0], c[1]), s[n][0]);
+          s[n][1] = __ffma2_rn(make_float2(k1, k1), make_float2(c[2], c[3]), s[n][1]);
         }
       }
       float v0[kG], v1[kG], top0 = 0.f, top1 = 0.f;      // steps of the values of tokens g and g + 8
@@ -294,45 +334,44 @@ struct QuantizedMmaLoop {
         top0 = fmaxf(top0, fabsf(v0[i]));
         top1 = fmaxf(top1, fabsf(v1[i]));
       }
-      if (next < t1) load_k(next, next_page);
+      load_k(next, next_page);
       const bool in0 = b0 + g < t1, in1 = b0 + g + 8 < t1;
       const float log0 = in0 ? fmaxf(__log2f(top0), -24.f) : -INFINITY, log1 = in1 ? fmaxf(__log2f(top1), -24.f) : -INFINITY;
       uint32_t pt[kTiles][kG][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] *= back[n][j & 1];
+        const float2 x0 = __fmul2_rn(s[n][0], back[n]), x1 = __fmul2_rn(s[n][1], back[n]), mul2 = make_float2(a.mul, a.mul);
         // The reference maximum moves only when a token passes it by more than 2^8.
-        const float mx0 = fmaxf(fmaf(s[n][0], a.mul, log0), fmaf(s[n][2], a.mul, log1));
-        const float mx1 = fmaxf(fmaf(s[n][1], a.mul, log0), fmaf(s[n][3], a.mul, log1));
+        const float2 r0 = __ffma2_rn(x0, mul2, make_float2(log0, log0)), r1 = __ffma2_rn(x1, mul2, make_float2(log1, log1));
+        const float mx0 = fmaxf(r0.x, r1.x), mx1 = fmaxf(r0.y, r1.y);
         if (__any_sync(0xffffffffu, mx0 > m[n][0] + 8.f || mx1 > m[n][1] + 8.f)) {
-          float x0 = mx0, x1 = mx1;
+          float y0 = mx0, y1 = mx1;
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+            y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, off));
+            y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, off));
           }
-          x0 = fmaxf(x0, m[n][0]);
-          x1 = fmaxf(x1, m[n][1]);
-          const float c0 = x0 > m[n][0] ? ex2(m[n][0] - x0) : 1.f, c1 = x1 > m[n][1] ? ex2(m[n][1] - x1) : 1.f;
-          m[n][0] = x0;
-          m[n][1] = x1;
-          l[n][0] *= c0;
-          l[n][1] *= c1;
+          y0 = fmaxf(y0, m[n][0]);
+          y1 = fmaxf(y1, m[n][1]);
+          const float c0 = y0 > m[n][0] ? ex2(m[n][0] - y0) : 1.f, c1 = y1 > m[n][1] ? ex2(m[n][1] - y1) : 1.f;
+          m[n][0] = y0;
+          m[n][1] = y1;
+          l[n].x *= c0;
+          l[n].y *= c1;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             o[n][i][0] *= c0; o[n][i][1] *= c1; o[n][i][2] *= c0; o[n][i][3] *= c1;
           }
         }
-        const float up0 = m[n][0] == -INFINITY ? kUp : kUp - m[n][0], up1 = m[n][1] == -INFINITY ? kUp : kUp - m[n][1];
-        const float p0 = in0 ? ex2(fmaf(s[n][0], a.mul, up0)) : 0.f, p1 = in0 ? ex2(fmaf(s[n][1], a.mul, up1)) : 0.f;
-        const float p2 = in1 ? ex2(fmaf(s[n][2], a.mul, up0)) : 0.f, p3 = in1 ? ex2(fmaf(s[n][3], a.mul, up1)) : 0.f;
-        l[n][0] += p0 + p2;
-        l[n][1] += p1 + p3;
+        const float2 up = make_float2(m[n][0] == -INFINITY ? kUp : kUp - m[n][0], m[n][1] == -INFINITY ? kUp : kUp - m[n][1]);
+        const float2 y0 = __ffma2_rn(x0, mul2, up), y1 = __ffma2_rn(x1, mul2, up);
+        const float2 p0 = make_float2(in0 ? ex2(y0.x) : 0.f, in0 ? ex2(y0.y) : 0.f), p1 = make_float2(in1 ? ex2(y1.x) : 0.f, in1 ? ex2(y1.y) : 0.f);
+        l[n] = __fadd2_rn(l[n], __fadd2_rn(p0, p1));
 #pragma unroll
         for (int i = 0; i < kG; ++i) {
-          pt[n][i][0] = transpose8x8(pack2<false>(p0 * v0[i], p1 * v0[i]));
-          pt[n][i][1] = transpose8x8(pack2<false>(p2 * v1[i], p3 * v1[i]));
+          const float2 w0 = __fmul2_rn(p0, make_float2(v0[i], v0[i])), w1 = __fmul2_rn(p1, make_float2(v1[i], v1[i]));
+          pt[n][i][0] = transpose8x8(pack2<false>(w0.x, w0.y));
+          pt[n][i][1] = transpose8x8(pack2<false>(w1.x, w1.y));
         }
       }
 #pragma unroll
@@ -351,15 +390,15 @@ struct QuantizedMmaLoop {
           mma16816<false>(o[n][2 * i + 1], e0[2], e0[3], e1[2], e1[3], pt[n][i][0], pt[n][i][1]);
         }
       }
-      if (next < t1) load_v(next, next_page);
+      load_v(next, next_page);
       next_page = page_of_block(next + wn * kBlock);
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {
-        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
-        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
+        l[n].x += __shfl_xor_sync(0xffffffffu, l[n].x, off);
+        l[n].y += __shfl_xor_sync(0xffffffffu, l[n].y, off);
       }
   }
 
@@ -377,7 +416,7 @@ struct QuantizedMmaLoop {
           *reinterpret_cast<float2*>(row + (i / 2) * kGroup + 4 * g + 2 * (i & 1)) = make_float2(o[n][i][hh] * kScale, o[n][i][2 + hh] * kOddScale);
         if (g == 0) {
           row[D] = m[n][hh] == -INFINITY ? -INFINITY : m[n][hh] - kUp;
-          row[D + 1] = l[n][hh];
+          row[D + 1] = hh ? l[n].y : l[n].x;
         }
       }
   }
@@ -440,10 +479,16 @@ int launch_fma(const QuantizedArgs& a, int side, cudaStream_t st) {
   return launch<T, QuantizedFmaLoop<T, kBits, 8, 2>, false>(a, side, st);
 }
 
+template <typename T, int D, int kBits, bool kDense>
+int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
+  return heads == 8 ? launch<T, QuantizedMmaLoop<T, D, kBits, 1, kDense>, true>(a, side, st) : launch<T, QuantizedMmaLoop<T, D, kBits, 2, kDense>, false>(a, side, st);
+}
 template <typename T, int kBits>
 int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
-  if (a.D == 64) return heads == 8 ? launch<T, QuantizedMmaLoop<T, 64, kBits, 1>, true>(a, side, st) : launch<T, QuantizedMmaLoop<T, 64, kBits, 2>, false>(a, side, st);
-  return heads == 8 ? launch<T, QuantizedMmaLoop<T, 128, kBits, 1>, true>(a, side, st) : launch<T, QuantizedMmaLoop<T, 128, kBits, 2>, false>(a, side, st);
+  bool dense = a.page_shift >= 4 && a.ks[2] * 16 == a.D * kBits / 8 && a.kss[2] == 1;
+  for (int i = 0; i < 3; ++i) dense = dense && a.ks[i] == a.vs[i] && a.kss[i] == a.vss[i];
+  if (a.D == 64) return dense ? launch_mma<T, 64, kBits, true>(a, heads, side, st) : launch_mma<T, 64, kBits, false>(a, heads, side, st);
+  return dense ? launch_mma<T, 128, kBits, true>(a, heads, side, st) : launch_mma<T, 128, kBits, false>(a, heads, side, st);
 }
 
 template <typename T>
