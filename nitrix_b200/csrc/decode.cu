@@ -35,6 +35,7 @@ struct MmaLoop {
   static constexpr int kHeads = 8 * kTiles;      // query heads of a chunk
   static constexpr int kBlock = 16;              // tokens
   static constexpr const char* kName = "decode_kernel";
+  static constexpr int kRing = 0;
   static constexpr int kSlots = 1;               // partial results of a warp
   // (head dim 128, one tile: four CTAs per SM spill, 5280 GB/s of cache, three 5675; 64: four 5510, five 5616)
   static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : 3) : D == 64 ? 4 : 2;
@@ -205,6 +206,7 @@ struct FmaLoop {
   static constexpr int kHeads = kNumHeads;
   static constexpr int kVec = 16 / int(sizeof(T));
   static constexpr const char* kName = "decode_kernel";
+  static constexpr int kRing = 0;
   static constexpr int kSlots = 32 / kLanes;
   static constexpr int kAhead = sizeof(T) == 4 && kPer == 1 ? 4 : 2;
   // (eight heads: two, three, four, five CTAs per SM 2730, 3330, 3030, 2470 GB/s)

@@ -2,6 +2,7 @@
 // work, the kernel around a loop over the tokens, and the joining of pieces.
 //
 // A loop has kName, its name in a profile; kHeads, the query heads that it takes; kSlots, the partial results that a warp leaves; kMinCtas;
+// kRing, bytes of shared memory that a warp has to itself (passed to run where there are any);
 // run(args, row of the table, key head, queries, heads, t0, t1, wi, wn), which takes part `wi` of `wn` of the tokens t0 .. t1 for one
 // warp; and store(args, dst), which leaves output, maximum (base 2) and sum of every head and slot.
 #pragma once
@@ -127,10 +128,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// Shared memory: what the warps leave, then kRing bytes of each warp's own.
+template <typename Loop>
+__host__ __device__ constexpr size_t merge_bytes(int D) { return (size_t(kWarps) * Loop::kSlots * Loop::kHeads * (D + 2) * sizeof(float) + 15) / 16 * 16; }
+
 // kSide chunks of query heads are taken by the warps of a CTA side by side.
 template <typename T, typename Loop, int kSide, typename Args>
 __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const Args a) {
-  extern __shared__ float merge[];      // [slot][head][D + 2]
+  extern __shared__ __align__(16) float merge[];      // [slot][head][D + 2]
   allow_dependents();
   const int lane = threadIdx.x & 31;
   const Share share = share_of(a, lane);
@@ -159,7 +164,12 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
       Loop loop;
       const int t0 = ub * a.unit, t1 = min(length, ue * a.unit);
       const T* q = static_cast<const T*>(a.q) + row * a.qs[0] + (head0 + own * Loop::kHeads) * a.qs[1];
-      loop.run(a, a.table + int64_t(row) * a.width, kv_head, q, min(Loop::kHeads, heads - own * Loop::kHeads), t0, t1, (threadIdx.x >> 5) % wn, wn);
+      const int* row_table = a.table + int64_t(row) * a.width;
+      const int own_heads = min(Loop::kHeads, heads - own * Loop::kHeads), wi = (threadIdx.x >> 5) % wn;
+      if constexpr (Loop::kRing > 0)
+        loop.run(a, row_table, kv_head, q, own_heads, t0, t1, wi, wn, reinterpret_cast<char*>(merge) + merge_bytes<Loop>(a.D) + (threadIdx.x >> 5) * Loop::kRing);
+      else
+        loop.run(a, row_table, kv_head, q, own_heads, t0, t1, wi, wn);
       loop.store(a, merge);
     }
     __syncthreads();
@@ -338,7 +348,9 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
 
 template <typename T, typename Loop, int kSide, typename Args>
 int launch_side(const Args& a, cudaStream_t st) {
-  const size_t smem = size_t(kWarps) * Loop::kSlots * Loop::kHeads * (a.D + 2) * sizeof(float);
+  const size_t smem = merge_bytes<Loop>(a.D) + size_t(kWarps) * Loop::kRing;
+  if (Loop::kRing > 0 && cudaFuncSetAttribute(decode_kernel<T, Loop, kSide, Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    return check_launch(Loop::kName);
   decode_kernel<T, Loop, kSide, Args><<<unsigned(a.workers), kThreads, smem, st>>>(a);
   count_launch();
   if (int rc = check_launch(Loop::kName)) return rc;

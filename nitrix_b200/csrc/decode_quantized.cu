@@ -20,10 +20,15 @@ __device__ __forceinline__ const uint16_t* steps_of(const uint16_t* base, const 
   return base + (int64_t(w.page) * stride[0] + int64_t(kv_head) * stride[1] + int64_t(w.slot) * stride[2]) * groups;
 }
 
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // fp32 multiply-adds.  Eight lanes share a token, a part of its row of codes each; a warp's four groups take tokens of their own.
 template <typename T, int kBits, int kGroups, int kNumHeads>
 struct QuantizedFmaLoop {
   static constexpr const char* kName = "decode_kernel<quantized>";
+  static constexpr int kRing = 0;
   static constexpr int kHeads = kNumHeads;
   static constexpr int kSlots = 4;
   static constexpr int kMinCtas = 2;
@@ -142,10 +147,14 @@ struct QuantizedMmaLoop {
   static constexpr int kHeads = 8 * kTiles;
   static constexpr int kBlock = 16;              // tokens
   static constexpr int kSlots = 1;
-  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : 4) : D == 64 ? 4 : 2;
+  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : kBits == 4 ? 4 : 3) : D == 64 ? 4 : 2;
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
   static constexpr int kRow = D * kBits / 8;     // bytes of a row of codes
+  // kDense: blocks come through a ring in shared memory, [codes of keys, of values, steps of keys, of values][kBlock rows] a stage
+  static constexpr int kStages = kRow > 64 ? 3 : 4;
+  static constexpr int kStepsAt = 2 * kBlock * kRow, kStage = kStepsAt + 4 * kBlock * kG;
+  static constexpr int kRing = kDense ? kStages * kStage : 0;
   static constexpr float kUp = 7.f;              // log2 of what probabilities are kept at: their products are below 2^15
   float o[kTiles][D / 16][4];
   float m[kTiles][2];
@@ -153,7 +162,20 @@ struct QuantizedMmaLoop {
 
   template <int n>
   __device__ __forceinline__ static void load_words(uint32_t (&w)[n], const void* p) {
-    if constexpr (n == 1) {
+    if constexpr (kDense) {      // (in shared memory)
+      if constexpr (n == 1) {
+        w[0] = *static_cast<const uint32_t*>(p);
+      } else if constexpr (n == 2) {
+        const uint2 v = *static_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < n / 4; ++i) {
+          const uint4 v = static_cast<const uint4*>(p)[i];
+          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+      }
+    } else if constexpr (n == 1) {
       asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
     } else if constexpr (n == 2) {
       asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
@@ -193,7 +215,7 @@ struct QuantizedMmaLoop {
   __device__ __forceinline__ static float step(const uint32_t (&w)[kG / 2], int i) { return i % 2 ? halves(w[i / 2]).y : halves(w[i / 2]).x; }
 
   __device__ __forceinline__ void run(const QuantizedArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0, int t1,
-                                      int wi, int wn) {
+                                      int wi, int wn, char* ring = nullptr) {
     const T* q = static_cast<const T*>(q_row);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t qf[kTiles][kG][4];
@@ -241,18 +263,31 @@ struct QuantizedMmaLoop {
     const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
     const int last = t1 - 1;
     uint32_t kw[2][2 * kW], vw[4][kW], kt[2][kG / 2], vt[2][kG / 2];
-    // kDense: pages of 16, 32, ... slots that lie side by side, of one layout for keys and values.  A lane's places in a block are
-    // then constants from the block's.
-    const char *k_lane, *v_lane, *kt_lane, *vt_lane;
+    // Row r of a product's 16 is token `token_of(r)` of the block: with this order the rows that a lane's neighbours read side by side
+    // lie in different banks.
+    auto token_of = [](int r) { return (r & 8) + ((r & 1) ? 4 + ((r >> 1 & 3) ^ 1) : r >> 1 & 3); };
+    const int mine = token_of(g);      // and mine + 8: this lane's tokens of the scores; t, 4 + (t ^ 1) and these + 8 are those of the values
+    // kDense: pages of 16, 32, ... slots that lie side by side, of one layout for keys and values
+    const char *k_from = nullptr, *v_from = nullptr, *steps_from = nullptr;
     if constexpr (kDense) {
-      k_lane = reinterpret_cast<const char*>(kbase) + g * kRow + t * 8 * kW;
-      v_lane = reinterpret_cast<const char*>(vbase) + 2 * t * kRow + g * 4 * kW;
-      const int64_t head = int64_t(kv_head) * a.kss[1] * kG + g * kG;
-      kt_lane = reinterpret_cast<const char*>(a.k_steps + head);
-      vt_lane = reinterpret_cast<const char*>(a.v_steps + head);
+      k_from = reinterpret_cast<const char*>(kbase) + lane * 16;
+      v_from = reinterpret_cast<const char*>(vbase) + lane * 16;
+      steps_from = reinterpret_cast<const char*>((lane < 16 ? a.k_steps : a.v_steps) + int64_t(kv_head) * a.kss[1] * kG) + (lane & 15) * 16;
     }
     const int64_t page_bytes = int64_t(a.ks[0]) * 16, page_steps = int64_t(a.kss[0]) * (2 * kG);
-    // (blocks begin at multiples of 16 tokens: in pages of 16, 32, ... slots the page is looked up once, a turn ahead)
+    auto fetch = [&](int b, int page, int stage) {
+      if (b < t1) {
+        const int slot = b & (a.page_size - 1);
+        const int64_t at = page * page_bytes + slot * kRow;
+        const uint32_t to = uint32_t(__cvta_generic_to_shared(ring)) + stage * kStage + lane * 16;
+#pragma unroll
+        for (int i = 0; i < kRow / 32; ++i) copy_async16(to + i * 512, k_from + at + i * 512);
+#pragma unroll
+        for (int i = 0; i < kRow / 32; ++i) copy_async16(to + kBlock * kRow + i * 512, v_from + at + i * 512);
+        if ((lane & 15) < 2 * kG) copy_async16(to + kStepsAt + (lane < 16 ? 0 : 2 * kBlock * kG - 256), steps_from + page * page_steps + slot * (2 * kG));
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     const bool one_page = kDense || a.page_shift >= 4;
     auto page_of_block = [&](int b) { return one_page ? page_at(a, row_table, min(b, last) >> a.page_shift) : 0; };
     // (behind the last token: with kDense what stands in its page, whose steps are set to zero, otherwise that token's rows again; with
@@ -262,53 +297,64 @@ struct QuantizedMmaLoop {
       if (one_page) return Where{page, (b & (a.page_size - 1)) + token - b};
       return where(a, row_table, token);
     };
-    auto load_k = [&](int b, int page) {
-      if constexpr (kDense) {
-        const int slot = b & (a.page_size - 1);
-        const int64_t at = page * page_bytes + slot * kRow, steps = page * page_steps + slot * (2 * kG);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          load_words(kw[r], k_lane + at + r * 8 * kRow);
-          load_words(kt[r], kt_lane + steps + r * 16 * kG);
-          load_words(vt[r], vt_lane + steps + r * 16 * kG);
-        }
-        return;
-      }
+    // of a block in pages, or of the stage that holds it
+    auto load_k = [&](int b, int page, const char* at) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const Where at = place(b, page, b + g + 8 * r);
-        load_words(kw[r], reinterpret_cast<const uint32_t*>(row_of(kbase, a.ks, at)) + 2 * kW * t);
-        load_words(kt[r], steps_of(a.k_steps, a.kss, kG, kv_head, at));
-        load_words(vt[r], steps_of(a.v_steps, a.vss, kG, kv_head, at));
+        if constexpr (kDense) {
+          const int row = mine + 8 * r;
+          load_words(kw[r], at + row * kRow + t * 8 * kW);
+          load_words(kt[r], at + kStepsAt + row * (2 * kG));
+          load_words(vt[r], at + kStepsAt + 2 * kBlock * kG + row * (2 * kG));
+        } else {
+          const Where w = place(b, page, b + mine + 8 * r);
+          load_words(kw[r], reinterpret_cast<const uint32_t*>(row_of(kbase, a.ks, w)) + 2 * kW * t);
+          load_words(kt[r], steps_of(a.k_steps, a.kss, kG, kv_head, w));
+          load_words(vt[r], steps_of(a.v_steps, a.vss, kG, kv_head, w));
+        }
       }
     };
-    auto load_v = [&](int b, int page) {
-      if constexpr (kDense) {
-        const int64_t at = page * page_bytes + (b & (a.page_size - 1)) * kRow;
+    auto load_v = [&](int b, int page, const char* at) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) load_words(vw[r], v_lane + at + ((r & 1) + (r >> 1) * 8) * kRow);
-        return;
+      for (int r = 0; r < 4; ++r) {
+        const int row = (r & 1 ? 4 + (t ^ 1) : t) + (r >> 1) * 8;
+        if constexpr (kDense) load_words(vw[r], at + (kBlock + row) * kRow + g * 4 * kW);
+        else load_words(vw[r], reinterpret_cast<const uint32_t*>(row_of(vbase, a.vs, place(b, page, b + row))) + kW * g);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        load_words(vw[r], reinterpret_cast<const uint32_t*>(row_of(vbase, a.vs, place(b, page, b + 2 * t + (r & 1) + (r >> 1) * 8))) + kW * g);
     };
     int b0 = t0 + wi * kBlock;
     if (b0 >= t1) return;
-    int next_page = page_of_block(b0);
-    load_k(b0, next_page);
-    load_v(b0, next_page);
-    next_page = page_of_block(b0 + wn * kBlock);
+    int next_page, stage = 0;
+    if constexpr (kDense) {
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) fetch(b0 + i * wn * kBlock, page_of_block(b0 + i * wn * kBlock), i);
+      next_page = page_of_block(b0 + (kStages - 1) * wn * kBlock);
+    } else {
+      next_page = page_of_block(b0);
+      load_k(b0, next_page, nullptr);
+      load_v(b0, next_page, nullptr);
+      next_page = page_of_block(b0 + wn * kBlock);
+    }
     for (; b0 < t1; b0 += wn * kBlock) {
       const int next = min(b0 + wn * kBlock, last & ~(kBlock - 1));      // (the last block may be asked for again, in vain)
-      if (kDense && b0 + kBlock > t1) {
+      const char* at = ring + stage * kStage;
+      if constexpr (kDense) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();      // the block is there, and all have left the one before, whose stage the next copies take
+        const int b = b0 + (kStages - 1) * wn * kBlock;
+        fetch(b, next_page, stage == 0 ? kStages - 1 : stage - 1);
+        next_page = page_of_block(b + wn * kBlock);
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+        load_k(b0, 0, at);
+        if (b0 + kBlock > t1) {
 #pragma unroll
-        for (int i = 0; i < kG / 2; ++i) {
-          if (b0 + g >= t1) vt[0][i] = 0;
-          if (b0 + g + 8 >= t1) vt[1][i] = 0;
+          for (int i = 0; i < kG / 2; ++i) {
+            if (b0 + mine >= t1) vt[0][i] = 0;
+            if (b0 + mine + 8 >= t1) vt[1][i] = 0;
+          }
         }
       }
-      float2 s[kTiles][2];      // of tokens g, g + 8: heads 2t, 2t + 1
+      float2 s[kTiles][2];      // of rows g, g + 8: heads 2t, 2t + 1
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -326,7 +372,7 @@ struct QuantizedMmaLoop {
           s[n][1] = __ffma2_rn(make_float2(k1, k1), make_float2(c[2], c[3]), s[n][1]);
         }
       }
-      float v0[kG], v1[kG], top0 = 0.f, top1 = 0.f;      // steps of the values of tokens g and g + 8
+      float v0[kG], v1[kG], top0 = 0.f, top1 = 0.f;      // steps of the values of rows g and g + 8
 #pragma unroll
       for (int i = 0; i < kG; ++i) {
         v0[i] = step(vt[0], i);
@@ -334,8 +380,9 @@ struct QuantizedMmaLoop {
         top0 = fmaxf(top0, fabsf(v0[i]));
         top1 = fmaxf(top1, fabsf(v1[i]));
       }
-      load_k(next, next_page);
-      const bool in0 = b0 + g < t1, in1 = b0 + g + 8 < t1;
+      if constexpr (kDense) load_v(b0, 0, at);
+      else load_k(next, next_page, nullptr);
+      const bool in0 = b0 + mine < t1, in1 = b0 + mine + 8 < t1;
       const float log0 = in0 ? fmaxf(__log2f(top0), -24.f) : -INFINITY, log1 = in1 ? fmaxf(__log2f(top1), -24.f) : -INFINITY;
       uint32_t pt[kTiles][kG][2];
 #pragma unroll
@@ -376,7 +423,7 @@ struct QuantizedMmaLoop {
       }
 #pragma unroll
       for (int i = 0; i < kG; ++i) {
-        uint32_t e0[4], e1[4];      // of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+        uint32_t e0[4], e1[4];      // of rows 2t, 2t + 1 and 2t + 8, 2t + 9
         codes(e0, vw[0], vw[1], i);
         codes(e1, vw[2], vw[3], i);
 #pragma unroll
@@ -390,8 +437,10 @@ struct QuantizedMmaLoop {
           mma16816<false>(o[n][2 * i + 1], e0[2], e0[3], e1[2], e1[3], pt[n][i][0], pt[n][i][1]);
         }
       }
-      load_v(next, next_page);
-      next_page = page_of_block(next + wn * kBlock);
+      if constexpr (!kDense) {
+        load_v(next, next_page, nullptr);
+        next_page = page_of_block(next + wn * kBlock);
+      }
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
@@ -447,7 +496,7 @@ int check(const nb200_decode_quantized_params* p, const char* what) {
   return check_steps(c, p->steps, what);
 }
 
-Plan plan(const nb200_decode_params* p) {
+Plan plan(const nb200_decode_params* p, int bits) {
   const nb200_cache_pages& c = p->pages;
   Plan pl{};
   const int group = p->q_heads / c.heads;
@@ -457,7 +506,7 @@ Plan plan(const nb200_decode_params* p) {
   int ctas = 2;      // resident per SM: the loops' kMinCtas
   if (pl.mma) {
     pl.heads = group > 8 ? 16 : 8;
-    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 5 : 4) : c.head_dim == 64 ? 4 : 2;
+    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 5 : bits == 4 ? 4 : 3) : c.head_dim == 64 ? 4 : 2;
   } else {
     pl.heads = c.head_dim > 128 ? 2 : 4;
   }
@@ -487,6 +536,7 @@ template <typename T, int kBits>
 int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
   bool dense = a.page_shift >= 4 && a.ks[2] * 16 == a.D * kBits / 8 && a.kss[2] == 1;
   for (int i = 0; i < 3; ++i) dense = dense && a.ks[i] == a.vs[i] && a.kss[i] == a.vss[i];
+  for (int i = 0; i < 2; ++i) dense = dense && int64_t(a.kss[i]) * a.groups % 8 == 0;      // (16-byte copies of steps)
   if (a.D == 64) return dense ? launch_mma<T, 64, kBits, true>(a, heads, side, st) : launch_mma<T, 64, kBits, false>(a, heads, side, st);
   return dense ? launch_mma<T, 128, kBits, true>(a, heads, side, st) : launch_mma<T, 128, kBits, false>(a, heads, side, st);
 }
@@ -505,7 +555,7 @@ using namespace nb200;
 extern "C" NB200_API int nb200_decode_quantized_workspace_bytes(const nb200_decode_quantized_params* p, size_t* bytes) {
   if (!bytes) { set_error("bytes out-pointer is NULL"); return NB200_ERR_INVALID; }
   if (int rc = check(p, "decode_quantized_workspace_bytes")) return rc;
-  *bytes = plan(&p->decode).bytes;
+  *bytes = plan(&p->decode, p->steps.bits).bytes;
   return NB200_OK;
 }
 
@@ -529,7 +579,7 @@ extern "C" NB200_API int nb200_decode_quantized(const nb200_decode_quantized_par
   }
   if (!ok) { set_error("%s: the rows of the pages must begin on 16-byte boundaries", what); return NB200_ERR_ALIGNMENT; }
   if (!near) { set_error("%s: a stride of the pages is 2^31 words of 16 bytes, or rows of steps, or more", what); return NB200_ERR_UNSUPPORTED; }
-  const Plan pl = plan(p);
+  const Plan pl = plan(p, qp->steps.bits);
   if (!p->workspace || p->workspace_bytes < pl.bytes) {
     set_error("%s: workspace of %zu bytes needed (nb200_decode_quantized_workspace_bytes), %zu given", what, pl.bytes, p->workspace_bytes);
     return NB200_ERR_WORKSPACE;
