@@ -2,7 +2,7 @@
 // work, the kernel around a loop over the tokens, and the joining of pieces.
 //
 // A loop has kName, its name in a profile; kHeads, the query heads that it takes; kSlots, the partial results that a warp leaves; kMinCtas;
-// kRing, bytes of shared memory that a warp has to itself (passed to run where there are any);
+// kRing, bytes of shared memory that a warp has to itself, or 0;
 // run(args, row of the table, key head, queries, heads, t0, t1, wi, wn), which takes part `wi` of `wn` of the tokens t0 .. t1 for one
 // warp; and store(args, dst), which leaves output, maximum (base 2) and sum of every head and slot.
 #pragma once
@@ -38,6 +38,7 @@ struct DecodeArgs {
   int chunks;                // times that a key head's group is taken, kSide chunks of query heads side by side each
   float mul;                 // scale * log2 e
   int unit;                  // tokens per unit of work
+  int extra;                 // units that beginning with a (sequence, key head) counts for
   float* part;               // pieces: [2 * CTAs][heads of a chunk][D + 4]: output, maximum (base 2), sum
   int workers;               // most CTAs of the main kernel that get work
 };
@@ -45,7 +46,8 @@ struct DecodeArgs {
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int row) {
   return int(min(int64_t(min(max(a.lengths[row], 0), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.page_size));
 }
-__device__ __forceinline__ int units_of(const DecodeArgs& a, int row) { return (length_of(a, row) + a.unit - 1) / a.unit; }
+__device__ __forceinline__ int units_of_length(const DecodeArgs& a, int length) { return length > 0 ? (length + a.unit - 1) / a.unit + a.extra : 0; }
+__device__ __forceinline__ int units_of(const DecodeArgs& a, int row) { return units_of_length(a, length_of(a, row)); }
 
 // Work position: units of all rows times (key head, chunk), row-major.  All lanes of a warp hold the same values.
 struct Share {
@@ -128,14 +130,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// Shared memory: what the warps leave, then kRing bytes of each warp's own.
+// Floats of shared memory from one slot's results to the next one's; a loop with a ring leaves its results there.
 template <typename Loop>
-__host__ __device__ constexpr size_t merge_bytes(int D) { return (size_t(kWarps) * Loop::kSlots * Loop::kHeads * (D + 2) * sizeof(float) + 15) / 16 * 16; }
+__host__ __device__ constexpr int slot_stride(int D) { return Loop::kRing > 0 ? Loop::kRing / 4 : Loop::kHeads * (D + 2); }
 
 // kSide chunks of query heads are taken by the warps of a CTA side by side.
 template <typename T, typename Loop, int kSide, typename Args>
 __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const Args a) {
-  extern __shared__ __align__(16) float merge[];      // [slot][head][D + 2]
+  extern __shared__ __align__(16) float merge[];      // [slot][head][D + 2], or the warps' rings
   allow_dependents();
   const int lane = threadIdx.x & 31;
   const Share share = share_of(a, lane);
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
   find_row(a, lane, u, &row, &row_begin);
   while (u < u_end) {
     const int length = length_of(a, row);
-    const int units = (length + a.unit - 1) / a.unit;
+    const int units = units_of_length(a, length);
     if (units == 0) { ++row; continue; }
     const int item = int((u - row_begin) / units);
     const int64_t item_begin = row_begin + int64_t(item) * units;
@@ -162,12 +164,12 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
     const int own = (threadIdx.x >> 5) / wn;                            // this warp's chunk
     if (own * Loop::kHeads < heads) {
       Loop loop;
-      const int t0 = ub * a.unit, t1 = min(length, ue * a.unit);
+      const int t0 = max(ub - a.extra, 0) * a.unit, t1 = min(length, max(ue - a.extra, 0) * a.unit);
       const T* q = static_cast<const T*>(a.q) + row * a.qs[0] + (head0 + own * Loop::kHeads) * a.qs[1];
       const int* row_table = a.table + int64_t(row) * a.width;
       const int own_heads = min(Loop::kHeads, heads - own * Loop::kHeads), wi = (threadIdx.x >> 5) % wn;
       if constexpr (Loop::kRing > 0)
-        loop.run(a, row_table, kv_head, q, own_heads, t0, t1, wi, wn, reinterpret_cast<char*>(merge) + merge_bytes<Loop>(a.D) + (threadIdx.x >> 5) * Loop::kRing);
+        loop.run(a, row_table, kv_head, q, own_heads, t0, t1, wi, wn, reinterpret_cast<char*>(merge) + (threadIdx.x >> 5) * Loop::kRing);
       else
         loop.run(a, row_table, kv_head, q, own_heads, t0, t1, wi, wn);
       loop.store(a, merge);
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, Loop::kMinCtas) decode_kernel(const 
     // the CTA's result: sums over the slots of a head's warps, relative to their largest maximum
     float* part = a.part + int64_t(2 * blockIdx.x + (ub == 0 ? 1 : 0)) * kSide * Loop::kHeads * (a.D + 4);
     constexpr int slots = wn * Loop::kSlots;
-    const int step = Loop::kHeads * (a.D + 2);
+    const int step = slot_stride<Loop>(a.D);
     for (int i = threadIdx.x; i < heads * a.D; i += kThreads) {
       const int h = i / a.D, d = i - h * a.D, of = h / Loop::kHeads;
       const float* col = merge + of * slots * step + (h - of * Loop::kHeads) * (a.D + 2);
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
 
 template <typename T, typename Loop, int kSide, typename Args>
 int launch_side(const Args& a, cudaStream_t st) {
-  const size_t smem = merge_bytes<Loop>(a.D) + size_t(kWarps) * Loop::kRing;
+  const size_t smem = size_t(kWarps) * Loop::kSlots * slot_stride<Loop>(a.D) * sizeof(float);
   if (Loop::kRing > 0 && cudaFuncSetAttribute(decode_kernel<T, Loop, kSide, Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
     return check_launch(Loop::kName);
   decode_kernel<T, Loop, kSide, Args><<<unsigned(a.workers), kThreads, smem, st>>>(a);

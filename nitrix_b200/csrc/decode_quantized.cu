@@ -3,6 +3,8 @@
 //   s_t = scale q . k_t,  p = softmax(s),  out = sum_t p_t v_t,     k_t, v_t = step (code - 2^(b-1)) per group of 32 elements
 //
 // Bound by HBM: every code and step is read once, 72 bytes per 128 elements in 4 bits.
+#include <type_traits>
+
 #include "cache_codes.cuh"
 #include "decode.cuh"
 
@@ -20,8 +22,10 @@ __device__ __forceinline__ const uint16_t* steps_of(const uint16_t* base, const 
   return base + (int64_t(w.page) * stride[0] + int64_t(kv_head) * stride[1] + int64_t(w.slot) * stride[2]) * groups;
 }
 
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
 }
 
 // fp32 multiply-adds.  Eight lanes share a token, a part of its row of codes each; a warp's four groups take tokens of their own.
@@ -141,48 +145,41 @@ struct QuantizedFmaLoop {
 // once, for each group.  The reference maximum is that of score + log2 of the value's largest step, so that no product leaves
 // fp16 and small ones keep their bits whatever the steps are; the sum of the probabilities is fp32.  Values' codes lose the half of
 // their range before the product, two at a time: taken off the sums instead, by MMAs of their own, it leaves errors of 2^-18 of it.
+//
+// A warp takes two blocks of 16 tokens at a turn, which come through a ring in shared memory by asynchronous copies, the next turn's
+// while it works on this one: of pages of 16, 32, ... slots that lie side by side (kDense) as they are, of others row by row.
 template <typename T, int D, int kBits, int kTiles, bool kDense>
 struct QuantizedMmaLoop {
   static constexpr const char* kName = "decode_kernel<quantized>";
   static constexpr int kHeads = 8 * kTiles;
-  static constexpr int kBlock = 16;              // tokens
+  static constexpr int kBlock = 16, kTurn = 32;  // tokens
   static constexpr int kSlots = 1;
   static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : kBits == 4 ? 4 : 3) : D == 64 ? 4 : 2;
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
   static constexpr int kRow = D * kBits / 8;     // bytes of a row of codes
-  // kDense: blocks come through a ring in shared memory, [codes of keys, of values, steps of keys, of values][kBlock rows] a stage
-  static constexpr int kStages = kRow > 64 ? 3 : 4;
-  static constexpr int kStepsAt = 2 * kBlock * kRow, kStage = kStepsAt + 4 * kBlock * kG;
-  static constexpr int kRing = kDense ? kStages * kStage : 0;
+  // a stage: rows of codes of keys, of values, rows of steps of keys, of values
+  static constexpr int kStages = 2;
+  static constexpr int kValuesAt = kTurn * kRow, kStepsAt = 2 * kTurn * kRow, kValueStepsAt = kStepsAt + kTurn * 2 * kG;
+  static constexpr int kStage = kStepsAt + kTurn * 4 * kG;
+  static constexpr int kRing = kStages * kStage;
   static constexpr float kUp = 7.f;              // log2 of what probabilities are kept at: their products are below 2^15
+  static constexpr float kLag = 8.f;             // log2 of how far a token may pass the reference
   float o[kTiles][D / 16][4];
-  float m[kTiles][2];
+  float m[kTiles][2];                            // reference maxima, and kLag
   float2 l[kTiles];
 
   template <int n>
-  __device__ __forceinline__ static void load_words(uint32_t (&w)[n], const void* p) {
-    if constexpr (kDense) {      // (in shared memory)
-      if constexpr (n == 1) {
-        w[0] = *static_cast<const uint32_t*>(p);
-      } else if constexpr (n == 2) {
-        const uint2 v = *static_cast<const uint2*>(p);
-        w[0] = v.x; w[1] = v.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < n / 4; ++i) {
-          const uint4 v = static_cast<const uint4*>(p)[i];
-          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
-      }
-    } else if constexpr (n == 1) {
-      asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+  __device__ __forceinline__ static void load_words(uint32_t (&w)[n], const char* p) {
+    if constexpr (n == 1) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else if constexpr (n == 2) {
-      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
     } else {
 #pragma unroll
       for (int i = 0; i < n / 4; ++i) {
-        const uint4 v = sm100::ldg_no_allocate(static_cast<const uint4*>(p) + i);
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
         w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
       }
     }
@@ -206,21 +203,20 @@ struct QuantizedMmaLoop {
   }
   // d = c + A B
   __device__ __forceinline__ static void mma(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
   __device__ __forceinline__ static float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
   // step of group i
   __device__ __forceinline__ static float step(const uint32_t (&w)[kG / 2], int i) { return i % 2 ? halves(w[i / 2]).y : halves(w[i / 2]).x; }
 
   __device__ __forceinline__ void run(const QuantizedArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0, int t1,
-                                      int wi, int wn, char* ring = nullptr) {
+                                      int wi, int wn, char* ring) {
     const T* q = static_cast<const T*>(q_row);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t qf[kTiles][kG][4];
-    float2 back[kTiles];
-    float half[kTiles][kG][2];
+    float mul[kTiles][2], half[kTiles][kG][4];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       float x[kG][8], top = 0.f;
@@ -236,9 +232,10 @@ struct QuantizedMmaLoop {
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int size = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 110);
-      const float up = __uint_as_float(uint32_t(127 + 9 - size) << 23), down = __uint_as_float(uint32_t(127 + 15 + size) << 23);
-      back[n] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
+      const int size = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const float up = __uint_as_float(uint32_t(127 + 9 - size) << 23), down = __uint_as_float(uint32_t(127 + 15 + size) << 23) * a.mul;
+      mul[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      mul[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
 #pragma unroll
       for (int i = 0; i < kG; ++i) {
 #pragma unroll
@@ -246,11 +243,9 @@ struct QuantizedMmaLoop {
           const float f = kBits == 4 && e % 2 ? up * (1.f / 16.f) : up;
           qf[n][i][e] = pack2<false>(x[i][e] * f, x[i][4 + e] * f);
         }
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816<false>(c, kEven, kEven, kOdd, kOdd, qf[n][i][0], qf[n][i][1]);
-        mma16816<false>(c, kEven, kEven, kOdd, kOdd, qf[n][i][2], qf[n][i][3]);
-        half[n][i][0] = c[0];
-        half[n][i][1] = c[1];
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        mma(half[n][i], zero, kEven, kEven, kOdd, kOdd, qf[n][i][0], qf[n][i][1]);
+        mma(half[n][i], half[n][i], kEven, kEven, kOdd, kOdd, qf[n][i][2], qf[n][i][3]);
       }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
@@ -259,188 +254,183 @@ struct QuantizedMmaLoop {
       m[n][0] = m[n][1] = -INFINITY;
       l[n] = make_float2(0.f, 0.f);
     }
-    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
-    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
     const int last = t1 - 1;
-    uint32_t kw[2][2 * kW], vw[4][kW], kt[2][kG / 2], vt[2][kG / 2];
     // Row r of a product's 16 is token `token_of(r)` of the block: with this order the rows that a lane's neighbours read side by side
     // lie in different banks.
     auto token_of = [](int r) { return (r & 8) + ((r & 1) ? 4 + ((r >> 1 & 3) ^ 1) : r >> 1 & 3); };
     const int mine = token_of(g);      // and mine + 8: this lane's tokens of the scores; t, 4 + (t ^ 1) and these + 8 are those of the values
-    // kDense: pages of 16, 32, ... slots that lie side by side, of one layout for keys and values
-    const char *k_from = nullptr, *v_from = nullptr, *steps_from = nullptr;
-    if constexpr (kDense) {
-      k_from = reinterpret_cast<const char*>(kbase) + lane * 16;
-      v_from = reinterpret_cast<const char*>(vbase) + lane * 16;
-      steps_from = reinterpret_cast<const char*>((lane < 16 ? a.k_steps : a.v_steps) + int64_t(kv_head) * a.kss[1] * kG) + (lane & 15) * 16;
-    }
+    const uint32_t to = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16;
+    const char* k_from = reinterpret_cast<const char*>(a.k + int64_t(kv_head) * a.ks[1]) + (kDense ? lane * 16 : 0);
+    const char* v_from = reinterpret_cast<const char*>(a.v + int64_t(kv_head) * a.vs[1]) + (kDense ? lane * 16 : 0);
+    const char* steps_from = reinterpret_cast<const char*>(lane < 16 ? steps_of(a.k_steps, a.kss, kG, kv_head, Where{0, 0})
+                                                                    : steps_of(a.v_steps, a.vss, kG, kv_head, Where{0, 0})) + (kDense ? (lane & 15) * 16 : 0);
     const int64_t page_bytes = int64_t(a.ks[0]) * 16, page_steps = int64_t(a.kss[0]) * (2 * kG);
-    auto fetch = [&](int b, int page, int stage) {
-      if (b < t1) {
+    auto page_of = [&](int b) { return kDense ? page_at(a, row_table, min(b, last) >> a.page_shift) : 0; };
+    // block u of the turn at b; behind the last token what stands in its page, or that token's rows again
+    auto fetch = [&](int b, int u, int page, int stage) {
+      const uint32_t dst = to + stage * kStage;
+      if constexpr (kDense) {
         const int slot = b & (a.page_size - 1);
         const int64_t at = page * page_bytes + slot * kRow;
-        const uint32_t to = uint32_t(__cvta_generic_to_shared(ring)) + stage * kStage + lane * 16;
 #pragma unroll
-        for (int i = 0; i < kRow / 32; ++i) copy_async16(to + i * 512, k_from + at + i * 512);
+        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + at + i * 512);
 #pragma unroll
-        for (int i = 0; i < kRow / 32; ++i) copy_async16(to + kBlock * kRow + i * 512, v_from + at + i * 512);
-        if ((lane & 15) < 2 * kG) copy_async16(to + kStepsAt + (lane < 16 ? 0 : 2 * kBlock * kG - 256), steps_from + page * page_steps + slot * (2 * kG));
+        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + at + i * 512);
+        if ((lane & 15) < 2 * kG)
+          copy_async<16>(dst + kStepsAt + u * kBlock * 2 * kG + (lane < 16 ? 0 : kTurn * 2 * kG - 256), steps_from + page * page_steps + slot * (2 * kG));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRow / 32; ++i) {
+          const int at = lane * 16 + i * 512;
+          const Where w = where(a, row_table, min(b + at / kRow, last));
+          const int64_t k_row = int64_t(w.page) * a.ks[0] + int64_t(w.slot) * a.ks[2], v_row = int64_t(w.page) * a.vs[0] + int64_t(w.slot) * a.vs[2];
+          copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + k_row * 16 + at % kRow);
+          copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + v_row * 16 + at % kRow);
+        }
+        const Where w = where(a, row_table, min(b + (lane & 15), last));
+        const int64_t row = lane < 16 ? int64_t(w.page) * a.kss[0] + int64_t(w.slot) * a.kss[2] : int64_t(w.page) * a.vss[0] + int64_t(w.slot) * a.vss[2];
+        copy_async<2 * kG>(dst - lane * 16 + (lane < 16 ? kStepsAt : kValueStepsAt) + (u * kBlock + (lane & 15)) * 2 * kG, steps_from + row * (2 * kG));
       }
+    };
+    int page[2];
+    auto fetch_turn = [&](int b, int stage) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (b + u * kBlock < t1) fetch(b + u * kBlock, u, page[u], stage);
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const bool one_page = kDense || a.page_shift >= 4;
-    auto page_of_block = [&](int b) { return one_page ? page_at(a, row_table, min(b, last) >> a.page_shift) : 0; };
-    // (behind the last token: with kDense what stands in its page, whose steps are set to zero, otherwise that token's rows again; with
-    // a probability of zero)
-    auto place = [&](int b, int page, int token) {
-      token = min(token, last);
-      if (one_page) return Where{page, (b & (a.page_size - 1)) + token - b};
-      return where(a, row_table, token);
-    };
-    // of a block in pages, or of the stage that holds it
-    auto load_k = [&](int b, int page, const char* at) {
+    // One turn; kTail: the last of the tokens, of which it may hold any number.
+    auto turn = [&](int b0, const char* at, auto tail) {
+      constexpr bool kTail = decltype(tail)::value;
+      float s[2][kTiles][4];      // of rows g, g + 8: heads 2t, 2t + 1
+      uint32_t vt[2][2][kG / 2];
+      float log_step[2][2];       // log2 of the largest step of the values of rows g, g + 8
+      bool in[2][2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if constexpr (kDense) {
-          const int row = mine + 8 * r;
+      for (int u = 0; u < 2; ++u) {
+        uint32_t kw[2][2 * kW], kt[2][kG / 2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = u * kBlock + mine + 8 * r;
           load_words(kw[r], at + row * kRow + t * 8 * kW);
-          load_words(kt[r], at + kStepsAt + row * (2 * kG));
-          load_words(vt[r], at + kStepsAt + 2 * kBlock * kG + row * (2 * kG));
-        } else {
-          const Where w = place(b, page, b + mine + 8 * r);
-          load_words(kw[r], reinterpret_cast<const uint32_t*>(row_of(kbase, a.ks, w)) + 2 * kW * t);
-          load_words(kt[r], steps_of(a.k_steps, a.kss, kG, kv_head, w));
-          load_words(vt[r], steps_of(a.v_steps, a.vss, kG, kv_head, w));
+          load_words(kt[r], at + kStepsAt + row * 2 * kG);
+          load_words(vt[u][r], at + kValueStepsAt + row * 2 * kG);
+          in[u][r] = !kTail || b0 + row < t1;
+          if (kTail && !in[u][r])
+#pragma unroll
+            for (int i = 0; i < kG / 2; ++i) kt[r][i] = vt[u][r][i] = 0;
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < kG; ++i) top = fmaxf(top, fabsf(step(vt[u][r], i)));
+          log_step[u][r] = in[u][r] ? fmaxf(__log2f(top), -24.f) : -INFINITY;
         }
-      }
-    };
-    auto load_v = [&](int b, int page, const char* at) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = (r & 1 ? 4 + (t ^ 1) : t) + (r >> 1) * 8;
-        if constexpr (kDense) load_words(vw[r], at + (kBlock + row) * kRow + g * 4 * kW);
-        else load_words(vw[r], reinterpret_cast<const uint32_t*>(row_of(vbase, a.vs, place(b, page, b + row))) + kW * g);
-      }
-    };
-    int b0 = t0 + wi * kBlock;
-    if (b0 >= t1) return;
-    int next_page, stage = 0;
-    if constexpr (kDense) {
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) fetch(b0 + i * wn * kBlock, page_of_block(b0 + i * wn * kBlock), i);
-      next_page = page_of_block(b0 + (kStages - 1) * wn * kBlock);
-    } else {
-      next_page = page_of_block(b0);
-      load_k(b0, next_page, nullptr);
-      load_v(b0, next_page, nullptr);
-      next_page = page_of_block(b0 + wn * kBlock);
-    }
-    for (; b0 < t1; b0 += wn * kBlock) {
-      const int next = min(b0 + wn * kBlock, last & ~(kBlock - 1));      // (the last block may be asked for again, in vain)
-      const char* at = ring + stage * kStage;
-      if constexpr (kDense) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();      // the block is there, and all have left the one before, whose stage the next copies take
-        const int b = b0 + (kStages - 1) * wn * kBlock;
-        fetch(b, next_page, stage == 0 ? kStages - 1 : stage - 1);
-        next_page = page_of_block(b + wn * kBlock);
-        stage = stage == kStages - 1 ? 0 : stage + 1;
-        load_k(b0, 0, at);
-        if (b0 + kBlock > t1) {
-#pragma unroll
-          for (int i = 0; i < kG / 2; ++i) {
-            if (b0 + mine >= t1) vt[0][i] = 0;
-            if (b0 + mine + 8 >= t1) vt[1][i] = 0;
-          }
-        }
-      }
-      float2 s[kTiles][2];      // of rows g, g + 8: heads 2t, 2t + 1
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < kG; ++i) {
-        uint32_t e0[4], e1[4];
-        codes(e0, kw[0], kw[0] + kW, i);
-        codes(e1, kw[1], kw[1] + kW, i);
-        const float k0 = step(kt[0], i), k1 = step(kt[1], i);
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          float c[4];
-          mma(c, {half[n][i][0], half[n][i][1], half[n][i][0], half[n][i][1]}, e0[0], e1[0], e0[1], e1[1], qf[n][i][0], qf[n][i][1]);
-          mma(c, c, e0[2], e1[2], e0[3], e1[3], qf[n][i][2], qf[n][i][3]);
-          s[n][0] = __ffma2_rn(make_float2(k0, k0), make_float2(c[0], c[1]), s[n][0]);
-          s[n][1] = __ffma2_rn(make_float2(k1, k1), make_float2(c[2], c[3]), s[n][1]);
-        }
-      }
-      float v0[kG], v1[kG], top0 = 0.f, top1 = 0.f;      // steps of the values of rows g and g + 8
-#pragma unroll
-      for (int i = 0; i < kG; ++i) {
-        v0[i] = step(vt[0], i);
-        v1[i] = step(vt[1], i);
-        top0 = fmaxf(top0, fabsf(v0[i]));
-        top1 = fmaxf(top1, fabsf(v1[i]));
-      }
-      if constexpr (kDense) load_v(b0, 0, at);
-      else load_k(next, next_page, nullptr);
-      const bool in0 = b0 + mine < t1, in1 = b0 + mine + 8 < t1;
-      const float log0 = in0 ? fmaxf(__log2f(top0), -24.f) : -INFINITY, log1 = in1 ? fmaxf(__log2f(top1), -24.f) : -INFINITY;
-      uint32_t pt[kTiles][kG][2];
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        const float2 x0 = __fmul2_rn(s[n][0], back[n]), x1 = __fmul2_rn(s[n][1], back[n]), mul2 = make_float2(a.mul, a.mul);
-        // The reference maximum moves only when a token passes it by more than 2^8.
-        const float2 r0 = __ffma2_rn(x0, mul2, make_float2(log0, log0)), r1 = __ffma2_rn(x1, mul2, make_float2(log1, log1));
-        const float mx0 = fmaxf(r0.x, r1.x), mx1 = fmaxf(r0.y, r1.y);
-        if (__any_sync(0xffffffffu, mx0 > m[n][0] + 8.f || mx1 > m[n][1] + 8.f)) {
-          float y0 = mx0, y1 = mx1;
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, off));
-            y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, off));
-          }
-          y0 = fmaxf(y0, m[n][0]);
-          y1 = fmaxf(y1, m[n][1]);
-          const float c0 = y0 > m[n][0] ? ex2(m[n][0] - y0) : 1.f, c1 = y1 > m[n][1] ? ex2(m[n][1] - y1) : 1.f;
-          m[n][0] = y0;
-          m[n][1] = y1;
-          l[n].x *= c0;
-          l[n].y *= c1;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            o[n][i][0] *= c0; o[n][i][1] *= c1; o[n][i][2] *= c0; o[n][i][3] *= c1;
-          }
-        }
-        const float2 up = make_float2(m[n][0] == -INFINITY ? kUp : kUp - m[n][0], m[n][1] == -INFINITY ? kUp : kUp - m[n][1]);
-        const float2 y0 = __ffma2_rn(x0, mul2, up), y1 = __ffma2_rn(x1, mul2, up);
-        const float2 p0 = make_float2(in0 ? ex2(y0.x) : 0.f, in0 ? ex2(y0.y) : 0.f), p1 = make_float2(in1 ? ex2(y1.x) : 0.f, in1 ? ex2(y1.y) : 0.f);
-        l[n] = __fadd2_rn(l[n], __fadd2_rn(p0, p1));
+          for (int j = 0; j < 4; ++j) s[u][n][j] = 0.f;
 #pragma unroll
         for (int i = 0; i < kG; ++i) {
-          const float2 w0 = __fmul2_rn(p0, make_float2(v0[i], v0[i])), w1 = __fmul2_rn(p1, make_float2(v1[i], v1[i]));
-          pt[n][i][0] = transpose8x8(pack2<false>(w0.x, w0.y));
-          pt[n][i][1] = transpose8x8(pack2<false>(w1.x, w1.y));
+          uint32_t e0[4], e1[4];
+          codes(e0, kw[0], kw[0] + kW, i);
+          codes(e1, kw[1], kw[1] + kW, i);
+          const float k0 = step(kt[0], i), k1 = step(kt[1], i);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            float c[4];
+            mma(c, half[n][i], e0[0], e1[0], e0[1], e1[1], qf[n][i][0], qf[n][i][1]);
+            mma(c, c, e0[2], e1[2], e0[3], e1[3], qf[n][i][2], qf[n][i][3]);
+            s[u][n][0] = fmaf(k0, c[0], s[u][n][0]);
+            s[u][n][1] = fmaf(k0, c[1], s[u][n][1]);
+            s[u][n][2] = fmaf(k1, c[2], s[u][n][2]);
+            s[u][n][3] = fmaf(k1, c[3], s[u][n][3]);
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < kG; ++i) {
-        uint32_t e0[4], e1[4];      // of rows 2t, 2t + 1 and 2t + 8, 2t + 9
-        codes(e0, vw[0], vw[1], i);
-        codes(e1, vw[2], vw[3], i);
+      for (int n = 0; n < kTiles; ++n) {
+        // The reference maximum moves only when a token passes it by more than 2^kLag.
+        float most[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          e0[e] = plus(e0[e], e % 2 ? kOdd : kEven);
-          e1[e] = plus(e1[e], e % 2 ? kOdd : kEven);
+        for (int j = 0; j < 2; ++j)
+          most[j] = fmaxf(fmaxf(fmaf(s[0][n][j], mul[n][j], log_step[0][0]), fmaf(s[0][n][2 + j], mul[n][j], log_step[0][1])),
+                          fmaxf(fmaf(s[1][n][j], mul[n][j], log_step[1][0]), fmaf(s[1][n][2 + j], mul[n][j], log_step[1][1])));
+        if (__any_sync(0xffffffffu, most[0] > m[n][0] || most[1] > m[n][1])) {
+          float c[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], off));
+            const float to = fmaxf(most[j] + kLag, m[n][j]);
+            c[j] = to > m[n][j] ? ex2(m[n][j] - to) : 1.f;
+            m[n][j] = to;
+          }
+          l[n].x *= c[0];
+          l[n].y *= c[1];
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][0] *= c[0]; o[n][i][1] *= c[1]; o[n][i][2] *= c[0]; o[n][i][3] *= c[1];
+          }
         }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (kTail && u == 1 && b0 + kBlock >= t1) break;
+        uint32_t vw[4][kW], pt[kTiles][kG][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_words(vw[r], at + kValuesAt + (u * kBlock + (r & 1 ? 4 + (t ^ 1) : t) + (r >> 1) * 8) * kRow + g * 4 * kW);
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-          mma16816<false>(o[n][2 * i], e0[0], e0[1], e1[0], e1[1], pt[n][i][0], pt[n][i][1]);
-          mma16816<false>(o[n][2 * i + 1], e0[2], e0[3], e1[2], e1[3], pt[n][i][0], pt[n][i][1]);
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float up = m[n][j & 1] == -INFINITY ? kUp : kUp + kLag - m[n][j & 1];
+            p[j] = in[u][j >> 1] ? ex2(fmaf(s[u][n][j], mul[n][j & 1], up)) : 0.f;
+          }
+          l[n].x += p[0] + p[2];
+          l[n].y += p[1] + p[3];
+#pragma unroll
+          for (int i = 0; i < kG; ++i) {
+            const float v0 = step(vt[u][0], i), v1 = step(vt[u][1], i);
+            pt[n][i][0] = transpose8x8(pack2<false>(p[0] * v0, p[1] * v0));
+            pt[n][i][1] = transpose8x8(pack2<false>(p[2] * v1, p[3] * v1));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+          uint32_t e0[4], e1[4];      // of rows 2t, 2t + 1 and 2t + 8, 2t + 9
+          codes(e0, vw[0], vw[1], i);
+          codes(e1, vw[2], vw[3], i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            e0[e] = plus(e0[e], e % 2 ? kOdd : kEven);
+            e1[e] = plus(e1[e], e % 2 ? kOdd : kEven);
+          }
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            mma(o[n][2 * i], o[n][2 * i], e0[0], e0[1], e1[0], e1[1], pt[n][i][0], pt[n][i][1]);
+            mma(o[n][2 * i + 1], o[n][2 * i + 1], e0[2], e0[3], e1[2], e1[3], pt[n][i][0], pt[n][i][1]);
+          }
         }
       }
-      if constexpr (!kDense) {
-        load_v(next, next_page, nullptr);
-        next_page = page_of_block(next + wn * kBlock);
-      }
+    };
+    int b0 = t0 + wi * kTurn;
+    if (b0 >= t1) return;
+    const int stride = wn * kTurn;
+    auto pages = [&](int b) { page[0] = page_of(b); page[1] = page_of(b + kBlock); };
+    pages(b0);
+    fetch_turn(b0, 0);
+    pages(b0 + stride);
+    int stage = 0;
+    for (; b0 < t1; b0 += stride) {
+      __syncwarp();      // all have left the turn before, whose stage the next copies take
+      fetch_turn(b0 + stride, stage ^ 1);
+      pages(b0 + 2 * stride);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+      const char* at = ring + stage * kStage;
+      stage ^= 1;
+      if (b0 + kTurn <= t1) turn(b0, at, std::false_type{});
+      else turn(b0, at, std::true_type{});
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
@@ -454,7 +444,9 @@ struct QuantizedMmaLoop {
   __device__ __forceinline__ void store(const QuantizedArgs& a, float* dst) const {
     constexpr float kScale = 16777216.f, kOddScale = kBits == 4 ? kScale / 16.f : kScale;      // of codes as fp16
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float* slot = dst + (threadIdx.x >> 5) * kHeads * (D + 2);
+    static_assert(kRing >= kHeads * (D + 2) * int(sizeof(float)), "a warp's results lie in its ring");
+    float* slot = dst + (threadIdx.x >> 5) * (kRing / 4);
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -464,7 +456,7 @@ struct QuantizedMmaLoop {
         for (int i = 0; i < D / 16; ++i)
           *reinterpret_cast<float2*>(row + (i / 2) * kGroup + 4 * g + 2 * (i & 1)) = make_float2(o[n][i][hh] * kScale, o[n][i][2 + hh] * kOddScale);
         if (g == 0) {
-          row[D] = m[n][hh] == -INFINITY ? -INFINITY : m[n][hh] - kUp;
+          row[D] = m[n][hh] == -INFINITY ? -INFINITY : m[n][hh] - kLag - kUp;
           row[D + 1] = hh ? l[n].y : l[n].x;
         }
       }
@@ -474,7 +466,7 @@ struct QuantizedMmaLoop {
 struct Plan {
   bool mma;
   int heads, side, chunks;      // query heads of a chunk, chunks side by side, times that a group is taken
-  int unit, workers;
+  int unit, extra, workers;
   size_t bytes;
 };
 
@@ -517,6 +509,10 @@ Plan plan(const nb200_decode_params* p, int bits) {
   const int64_t units = (int64_t(p->width) * c.page_size + pl.unit - 1) / pl.unit * p->rows * c.heads * pl.chunks;
   const int64_t most = int64_t(tc::sm_count()) * ctas;
   pl.workers = int(units < most ? (units > 0 ? units : 1) : most);
+  // Beginning with a (sequence, key head) costs a CTA about as much as two units: the queries, the first page, the join of its warps (64
+  // sequences of up to 8192 tokens, 8 heads of 128, 4 bits: none 103 to 107 us, one 93 to 99, two 89 to 94).  Where every unit has a CTA
+  // of its own there is nothing to balance.
+  pl.extra = units < most ? 0 : 2;
   pl.bytes = size_t(pl.workers) * 2 * pl.side * pl.heads * (c.head_dim + 4) * sizeof(float);
   return pl;
 }
@@ -602,6 +598,7 @@ extern "C" NB200_API int nb200_decode_quantized(const nb200_decode_quantized_par
   a.chunks = pl.chunks;
   a.mul = p->scale * kLog2e;
   a.unit = pl.unit;
+  a.extra = pl.extra;
   a.part = static_cast<float*>(p->workspace);
   a.workers = pl.workers;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
