@@ -6,19 +6,23 @@
 //   backward  n = h s,  g = dy w,  dx = dh + s (g - n mean(g n)),  dw = sum_rows dy n
 //
 // Bound by HBM: every stream is read once and written once, so a row is held in registers between its sum and its output: by
-// tpr threads (a power of two, up to the CTA's 256), kPer chunks of kVec elements each.  kVec is a 16-byte word's elements, or
-// one where rows do not begin on 16-byte boundaries.  Rows that are too long for that are read once more (the *_wide kernels).
+// tpr threads (a power of two), kPer chunks of kVec elements each.  kVec is a 16-byte word's elements, or one where rows do not
+// begin on 16-byte boundaries.  CTAs walk the rows with a stride and ask for the next row before they work on the present one.
+// Elements are taken in pairs, two fp32 operations per instruction: with 16-bit storage the conversions and the arithmetic take as
+// many issue slots as the loads leave.  Rows that are too long to be held are read once more (the *_wide kernels).
 #include <cuda_fp8.h>
 #include <math.h>
 
+#include <type_traits>
+
+#include "dependent_launch.cuh"
 #include "nitrix_b200_rms_norm.h"
 #include "sdpa_tc_common.cuh"
 
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxWarps = 16;
 
 struct RmsArgs {
   const void* x;
@@ -38,59 +42,85 @@ struct RmsArgs {
   float eps, inv_c;
 };
 
-// kVec consecutive elements as they lie in memory.
+// kVec consecutive elements as they lie in memory, and as pairs (one element: with a zero behind it).
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return make_float2(0.f, 0.f);
+  else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t word_of(float2 v) {
+  return tc::pack2<!std::is_same<T, __half>::value>(v.x, v.y);
+}
 template <typename T, int kVec>
 struct Chunk {
-  uint4 w;
-  __device__ __forceinline__ static Chunk load(const T* p) { return Chunk{sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(p))}; }
-  __device__ __forceinline__ static Chunk load_cached(const T* p) { return Chunk{*reinterpret_cast<const uint4*>(p)}; }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
-  __device__ __forceinline__ void get(float (&f)[kVec]) const {
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = to_f32<T>(e[i]);
-  }
-  __device__ __forceinline__ static Chunk of(const float (&f)[kVec]) {
+  static constexpr int kPairs = kVec / 2, kWords = kVec * int(sizeof(T)) / 16;
+  uint4 w[kWords];
+  __device__ __forceinline__ static Chunk load(const T* p) {
     Chunk c;
-    T* e = reinterpret_cast<T*>(&c.w);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) e[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < kWords; ++i) c.w[i] = sm100::ldg_no_allocate(reinterpret_cast<const uint4*>(p) + i);
     return c;
   }
-  __device__ __forceinline__ static Chunk zero() { return Chunk{make_uint4(0, 0, 0, 0)}; }
+  __device__ __forceinline__ static Chunk load_cached(const T* p) {
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) c.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return c;
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ void get(float2 (&f)[kPairs]) const {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      f[i] = sizeof(T) == 4 ? make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])) : pair_of<T>(u[i]);
+  }
+  __device__ __forceinline__ static Chunk of(const float2 (&f)[kPairs]) {
+    Chunk c;
+    uint32_t* u = reinterpret_cast<uint32_t*>(c.w);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        u[2 * i] = __float_as_uint(f[i].x);
+        u[2 * i + 1] = __float_as_uint(f[i].y);
+      } else {
+        u[i] = word_of<T>(f[i]);
+      }
+    }
+    return c;
+  }
+  __device__ __forceinline__ static Chunk zero() {
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) c.w[i] = make_uint4(0, 0, 0, 0);
+    return c;
+  }
 };
 template <typename T>
 struct Chunk<T, 1> {
+  static constexpr int kPairs = 1;
   T v;
   __device__ __forceinline__ static Chunk load(const T* p) { return Chunk{__ldg(p)}; }
   __device__ __forceinline__ static Chunk load_cached(const T* p) { return Chunk{*p}; }
   __device__ __forceinline__ void store(T* p) const { *p = v; }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32<T>(v); }
-  __device__ __forceinline__ static Chunk of(const float (&f)[1]) { return Chunk{from_f32<T>(f[0])}; }
+  __device__ __forceinline__ void get(float2 (&f)[1]) const { f[0] = make_float2(to_f32<T>(v), 0.f); }
+  __device__ __forceinline__ static Chunk of(const float2 (&f)[1]) { return Chunk{from_f32<T>(f[0].x)}; }
   __device__ __forceinline__ static Chunk zero() { return Chunk{from_f32<T>(0.f)}; }
 };
 
-// kVec weights of type W (ones without a weight)
+// Weights of a chunk, of their own type; ones without a weight.
 template <typename W, int kVec>
-__device__ __forceinline__ void weights(const void* w, int c, float (&f)[kVec]) {
-  if (!w) {
+__device__ __forceinline__ Chunk<W, kVec> weights(const void* w, int c, bool in) {
+  using C = Chunk<W, kVec>;
+  if (w && in) return C::load_cached(static_cast<const W*>(w) + c);
+  float2 ones[C::kPairs];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = 1.f;
-    return;
-  }
-  const W* p = static_cast<const W*>(w) + c;
-  if constexpr (kVec == 1) {
-    f[0] = to_f32<W>(__ldg(p));
-  } else {
-    constexpr int kWords = kVec * int(sizeof(W)) / 16, kEach = kVec / kWords;
-#pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      const uint4 word = __ldg(reinterpret_cast<const uint4*>(p) + j);
-      const W* e = reinterpret_cast<const W*>(&word);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) f[j * kEach + i] = to_f32<W>(e[i]);
-    }
-  }
+  for (int i = 0; i < C::kPairs; ++i) ones[i] = make_float2(1.f, 1.f);
+  return C::of(ones);
 }
 
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
@@ -100,7 +130,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN on ei
   return m;
 }
 
-// `op` over the tpr threads that share a row.  `red` holds kWarps floats per use; uses that follow one another take other ones, so
+// `op` over the tpr threads that share a row.  `red` holds kMaxWarps floats per use; uses that follow one another take other ones, so
 // that one barrier each is enough.  All threads of the CTA call it.
 template <float (*op)(float, float)>
 __device__ __forceinline__ float over_row(float v, int tpr, float* red) {
@@ -110,171 +140,190 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* red) {
     const int warp = threadIdx.x >> 5, warps = tpr >> 5, first = warp & ~(warps - 1);
     if ((threadIdx.x & 31) == 0) red[warp] = v;
     __syncthreads();
-    v = red[first];
-    for (int i = 1; i < warps; ++i) v = op(v, red[first + i]);
+    const float2* sums = reinterpret_cast<const float2*>(red + first);
+    v = op(sums[0].x, sums[0].y);
+    for (int i = 1; i < warps / 2; ++i) v = op(v, op(sums[i].x, sums[i].y));
   }
   return v;
 }
 
-// codes of kVec values, each times `inv`
-template <int kVec>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[kVec], float inv) {
-  if constexpr (kVec == 1) {
-    *p = __nv_cvt_float_to_fp8(y[0] * inv, __NV_SATFINITE, __NV_E4M3);
-  } else {
-    uint32_t w[kVec / 4];
+// codes of a chunk's values, each times `inv`
+template <int kVec, int kPairs>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float2 (&y)[kPairs], float inv) {
+  uint32_t c[kPairs];
 #pragma unroll
-    for (int i = 0; i < kVec / 4; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * i] * inv, y[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2] * inv, y[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-      w[i] = lo | hi << 16;
-    }
-    if constexpr (kVec == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  }
+  for (int i = 0; i < kPairs; ++i) c[i] = __nv_cvt_float2_to_fp8x2(__fmul2_rn(y[i], make_float2(inv, inv)), __NV_SATFINITE, __NV_E4M3);
+  if constexpr (kVec == 1) *p = uint8_t(c[0]);
+  else if constexpr (kVec == 4) *reinterpret_cast<uint32_t*>(p) = c[0] | c[1] << 16;
+  else *reinterpret_cast<uint2*>(p) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
 constexpr float kLeast = 7.888609052210118e-31f;      // 2^-100
-template <int kVec>
-__device__ __forceinline__ float top_of(const float (&y)[kVec], float top) {
+template <int kPairs>
+__device__ __forceinline__ float top_of(const float2 (&y)[kPairs], float top) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) top = max_nan(top, fabsf(y[i]));
+  for (int i = 0; i < kPairs; ++i) top = max_nan(max_nan(top, fabsf(y[i].x)), fabsf(y[i].y));
   return top;
 }
-// The scale of a group of lanes' values, written by its first lane; what the values are multiplied by.
+// The scale for a largest magnitude, and what the values are multiplied by (the reciprocal of a number of 2^-109 or more, good to 2^-23).
+__device__ __forceinline__ float scale_of(float top) { return top * (1.f / 448.f); }
+__device__ __forceinline__ float inverse_of(float scale) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
+}
+// The same of a group of lanes' values; its first lane writes the scale.
 __device__ __forceinline__ float group_scale(float top, int lanes, float* scale) {
   for (int o = lanes >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & (lanes - 1)) == 0 && scale) *scale = __fdiv_rn(top, 448.f);
-  return __fdiv_rn(448.f, top);
+  const float s = scale_of(top);
+  if ((threadIdx.x & (lanes - 1)) == 0 && scale) *scale = s;
+  return inverse_of(s);
 }
 
-template <typename T, typename W, int kVec, int kPer, bool kEight>
-__global__ void __launch_bounds__(kThreads, kPer <= 2 ? 4 : 2) rms_fwd_kernel(const RmsArgs a, int tpr) {
-  __shared__ float red[2 * kWarps];
+template <typename T, typename W, int kVec, int kPer, int kThreads, bool kEight>
+__global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 : 512) / kThreads) rms_fwd_kernel(const RmsArgs a, int tpr) {
+  __shared__ __align__(16) float red[4 * kMaxWarps];
   using C = Chunk<T, kVec>;
-  const int tin = threadIdx.x & (tpr - 1);
-  const int64_t row = int64_t(blockIdx.x) * (kThreads / tpr) + threadIdx.x / tpr;
-  const bool in_rows = row < a.rows;
-  const int64_t base = in_rows ? row * a.C : 0;
+  constexpr int kPairs = C::kPairs;
+  const int tin = threadIdx.x & (tpr - 1), groups = kThreads / tpr, mine = threadIdx.x / tpr;
+  const int64_t blocks = (a.rows + groups - 1) / groups;
   auto column = [&](int p) { return (p * tpr + tin) * kVec; };
-  C h[kPer];
-#pragma unroll
-  for (int p = 0; p < kPer; ++p) h[p] = in_rows && column(p) < a.C ? C::load(static_cast<const T*>(a.x) + base + column(p)) : C::zero();
-  if (a.r) {
-    C r[kPer];
-#pragma unroll
-    for (int p = 0; p < kPer; ++p) r[p] = in_rows && column(p) < a.C ? C::load(static_cast<const T*>(a.r) + base + column(p)) : C::zero();
+  C nx[kPer], nr[kPer];
+  auto fetch = [&](int64_t block) {
+    const int64_t row = block * groups + mine;
+    const bool in_rows = block < blocks && row < a.rows;
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      float f[kVec], g[kVec];
-      h[p].get(f);
-      r[p].get(g);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) f[i] += g[i];
-      h[p] = C::of(f);
-      if (in_rows && column(p) < a.C) h[p].store(static_cast<T*>(a.sum) + base + column(p));
+      const bool in = in_rows && column(p) < a.C;
+      const int64_t at = in ? row * a.C + column(p) : 0;
+      nx[p] = in ? C::load(static_cast<const T*>(a.x) + at) : C::zero();
+      if (a.r) nr[p] = in ? C::load(static_cast<const T*>(a.r) + at) : C::zero();
     }
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int p = 0; p < kPer; ++p) {
-    float f[kVec];
-    h[p].get(f);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) ss = fmaf(f[i], f[i], ss);
-  }
-  const float s = __frsqrt_rn(fmaf(over_row<add>(ss, tpr, red), a.inv_c, a.eps));
-  if (tin == 0 && in_rows && a.rstd) a.rstd[row] = s;
-  auto output = [&](int p, float (&f)[kVec]) {
-    float w[kVec];
-    h[p].get(f);
-    if (column(p) < a.C) weights<W, kVec>(a.w, column(p), w);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = column(p) < a.C ? f[i] * s * w[i] : 0.f;
   };
-  float inv = 0.f;
-  if constexpr (kEight) {
-    if (a.group == a.C) {
-      float top = kLeast;
+  fetch(blockIdx.x);
+  Chunk<W, kVec> w[kPer];
 #pragma unroll
-      for (int p = 0; p < kPer; ++p) {
-        float f[kVec];
-        output(p, f);
-        top = top_of(f, top);
+  for (int p = 0; p < kPer; ++p) w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
+  int turn = 0;
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    const int64_t row = block * groups + mine, base = row * a.C;
+    const bool in_rows = row < a.rows;
+    C h[kPer];
+    float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      h[p] = nx[p];
+      float2 f[kPairs];
+      h[p].get(f);
+      if (a.r) {
+        float2 g[kPairs];
+        nr[p].get(g);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) f[i] = __fadd2_rn(f[i], g[i]);
+        h[p] = C::of(f);
+        if (in_rows && column(p) < a.C) h[p].store(static_cast<T*>(a.sum) + base + column(p));
+        h[p].get(f);
       }
-      top = over_row<max_nan>(top, tpr, red + kWarps);
-      if (tin == 0 && in_rows) a.scales[row] = __fdiv_rn(top, 448.f);
-      inv = __fdiv_rn(448.f, top);
-    }
-  }
 #pragma unroll
-  for (int p = 0; p < kPer; ++p) {
-    float f[kVec];
-    output(p, f);
-    const bool in = in_rows && column(p) < a.C;
+      for (int i = 0; i < kPairs; ++i) ss = __ffma2_rn(f[i], f[i], ss);
+    }
+    fetch(block + gridDim.x);
+    const float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, tpr, red + turn * kMaxWarps), a.inv_c, a.eps));
+    if (tin == 0 && in_rows && a.rstd) a.rstd[row] = s;
+    auto output = [&](int p, float2 (&f)[kPairs]) {
+      float2 v[kPairs];
+      h[p].get(f);
+      w[p].get(v);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(__fmul2_rn(f[i], make_float2(s, s)), v[i]);
+    };
+    float inv = 0.f;
     if constexpr (kEight) {
-      if (a.group != a.C)
-        inv = group_scale(top_of(f, kLeast), a.group / kVec, in ? a.scales + row * (a.C / a.group) + column(p) / a.group : nullptr);
-      if (in) store_codes<kVec>(static_cast<uint8_t*>(a.y) + base + column(p), f, inv);
-    } else {
-      if (in) C::of(f).store(static_cast<T*>(a.y) + base + column(p));
+      if (a.group == a.C) {
+        float top = kLeast;
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) {
+          float2 f[kPairs];
+          output(p, f);
+          top = top_of(f, top);
+        }
+        const float scale = scale_of(over_row<max_nan>(top, tpr, red + (2 + turn) * kMaxWarps));
+        if (tin == 0 && in_rows) a.scales[row] = scale;
+        inv = inverse_of(scale);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      float2 f[kPairs];
+      output(p, f);
+      const bool in = in_rows && column(p) < a.C;
+      if constexpr (kEight) {
+        if (a.group != a.C)
+          inv = group_scale(top_of(f, kLeast), a.group / kVec, in ? a.scales + row * (a.C / a.group) + column(p) / a.group : nullptr);
+        if (in) store_codes<kVec>(static_cast<uint8_t*>(a.y) + base + column(p), f, inv);
+      } else {
+        if (in) C::of(f).store(static_cast<T*>(a.y) + base + column(p));
+      }
     }
   }
 }
+
+constexpr int kWide = 256;      // threads of a row that is not held
 
 // A row per CTA, read again for its output (and, for one scale of the row, for that).
 template <typename T, typename W, int kVec, bool kEight>
-__global__ void __launch_bounds__(kThreads) rms_fwd_wide_kernel(const RmsArgs a) {
-  __shared__ float red[2 * kWarps];
+__global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
+  __shared__ __align__(16) float red[2 * kMaxWarps];
   using C = Chunk<T, kVec>;
+  constexpr int kPairs = C::kPairs;
   const int64_t row = blockIdx.x, base = row * a.C;
   const T* x = static_cast<const T*>(a.x) + base;
-  float ss = 0.f;
-  for (int c = threadIdx.x * kVec; c < a.C; c += kThreads * kVec) {
+  float2 ss = make_float2(0.f, 0.f);
+  for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
     C h = C::load_cached(x + c);
-    float f[kVec], g[kVec];
+    float2 f[kPairs], g[kPairs];
     h.get(f);
     if (a.r) {
       C::load_cached(static_cast<const T*>(a.r) + base + c).get(g);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) f[i] += g[i];
+      for (int i = 0; i < kPairs; ++i) f[i] = __fadd2_rn(f[i], g[i]);
       h = C::of(f);
       h.store(static_cast<T*>(a.sum) + base + c);
       h.get(f);
     }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) ss = fmaf(f[i], f[i], ss);
+    for (int i = 0; i < kPairs; ++i) ss = __ffma2_rn(f[i], f[i], ss);
   }
-  const float s = __frsqrt_rn(fmaf(over_row<add>(ss, kThreads, red), a.inv_c, a.eps));
+  const float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, kWide, red), a.inv_c, a.eps));
   if (threadIdx.x == 0 && a.rstd) a.rstd[row] = s;
   const T* h = a.r ? static_cast<const T*>(a.sum) + base : x;      // (every thread reads back what it has written itself)
-  auto output = [&](int c, float (&f)[kVec]) {
-    float w[kVec];
+  auto output = [&](int c, float2 (&f)[kPairs]) {
+    float2 v[kPairs];
     C::load_cached(h + c).get(f);
-    weights<W, kVec>(a.w, c, w);
+    weights<W, kVec>(a.w, c, true).get(v);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = f[i] * s * w[i];
+    for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(__fmul2_rn(f[i], make_float2(s, s)), v[i]);
   };
   float inv = 0.f;
   if constexpr (kEight) {
     if (a.group == a.C) {
       float top = kLeast;
-      for (int c = threadIdx.x * kVec; c < a.C; c += kThreads * kVec) {
-        float f[kVec];
+      for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
+        float2 f[kPairs];
         output(c, f);
         top = top_of(f, top);
       }
-      top = over_row<max_nan>(top, kThreads, red + kWarps);
-      if (threadIdx.x == 0) a.scales[row] = __fdiv_rn(top, 448.f);
-      inv = __fdiv_rn(448.f, top);
+      const float scale = scale_of(over_row<max_nan>(top, kWide, red + kMaxWarps));
+      if (threadIdx.x == 0) a.scales[row] = scale;
+      inv = inverse_of(scale);
     }
   }
   // (whole warps go round together: a group's lanes are in one)
-  for (int c0 = (threadIdx.x & ~31) * kVec; c0 < a.C; c0 += kThreads * kVec) {
+  for (int c0 = (threadIdx.x & ~31) * kVec; c0 < a.C; c0 += kWide * kVec) {
     const int c = c0 + (threadIdx.x & 31) * kVec;
     const bool in = c < a.C;
-    float f[kVec];
+    float2 f[kPairs];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = 0.f;
+    for (int i = 0; i < kPairs; ++i) f[i] = make_float2(0.f, 0.f);
     if (in) output(c, f);
     if constexpr (kEight) {
       if (a.group != a.C)
@@ -286,86 +335,118 @@ __global__ void __launch_bounds__(kThreads) rms_fwd_wide_kernel(const RmsArgs a)
   }
 }
 
-// Backward.  CTAs walk the rows with a stride; a thread always has the same columns, whose part of dw stays in its registers, and
-// asks for its chunks of the next row before it works on the present one.
-template <typename T, typename W, int kVec, int kPer>
-__global__ void __launch_bounds__(kThreads, kPer * kVec <= 8 ? 4 : kPer * kVec <= 16 ? 3 : kPer * kVec <= 32 ? 2 : 1)
-rms_bwd_kernel(const RmsArgs a, int tpr) {
-  extern __shared__ float columns[];      // [C], where rows share a CTA
-  __shared__ float red[2][kWarps];
+// Backward.  A thread always has the same columns, whose part of dw stays in its registers; it copies its own chunks of the next
+// kAhead rows into its own places of a ring in shared memory, so that no barrier is needed for them.
+template <int kPer, int kThreads, int kChunkBytes>
+struct Ring {
+  static constexpr int kRow = 3 * kPer * kThreads * kChunkBytes;      // h, dy and dsum of a row (or of as many as share the CTA)
+  static constexpr int kAhead = kRow <= 24576 ? 2 : 1;
+  static constexpr int kBytes = (kAhead + 1) * kRow;
+};
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
+  const uint32_t d = uint32_t(__cvta_generic_to_shared(dst));
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(in ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+
+template <typename T, typename W, int kVec, int kPer, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) rms_bwd_kernel(const RmsArgs a, int tpr) {
   using Ch = Chunk<T, kVec>;
+  constexpr int kPairs = Ch::kPairs, kSize = kVec * int(sizeof(T));
+  using Rg = Ring<kPer, kThreads, kSize>;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ __align__(16) float red[2 * kMaxWarps];
   const int tin = threadIdx.x & (tpr - 1), mine = threadIdx.x / tpr, groups = kThreads / tpr;
   auto column = [&](int p) { return (p * tpr + tin) * kVec; };
-  float dw[kPer][kVec];
+  float2 dw[kPer][kPairs];
+  Chunk<W, kVec> w[kPer];
 #pragma unroll
-  for (int p = 0; p < kPer; ++p)
+  for (int p = 0; p < kPer; ++p) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) dw[p][i] = 0.f;
+    for (int i = 0; i < kPairs; ++i) dw[p][i] = make_float2(0.f, 0.f);
+    w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
+  }
   const int64_t blocks = (a.rows + groups - 1) / groups;
-  Ch h[kPer], dy[kPer], ds[kPer];
-  float s = 0.f;
-  auto fetch = [&](int64_t block) {
+  auto place = [&](int stage, int which, int p) { return ring + stage * Rg::kRow + ((which * kPer + p) * kThreads + threadIdx.x) * kSize; };
+  auto fetch = [&](int64_t block, int stage) {
     const int64_t row = block * groups + mine;
     const bool in_rows = block < blocks && row < a.rows;
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
       const bool in = in_rows && column(p) < a.C;
       const int64_t at = in ? row * a.C + column(p) : 0;
-      h[p] = in ? Ch::load(static_cast<const T*>(a.x) + at) : Ch::zero();
-      dy[p] = in ? Ch::load(static_cast<const T*>(a.dy) + at) : Ch::zero();
-      ds[p] = in && a.dsum ? Ch::load(static_cast<const T*>(a.dsum) + at) : Ch::zero();
-    }
-    s = in_rows ? __ldg(a.rstd + row) : 0.f;
-  };
-  fetch(blockIdx.x);
-  int turn = 0;
-  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
-    const int64_t row = block * groups + mine;
-    Ch hc[kPer], gc[kPer], sc[kPer];
-#pragma unroll
-    for (int p = 0; p < kPer; ++p) { hc[p] = h[p]; gc[p] = dy[p]; sc[p] = ds[p]; }
-    const float rstd = s;
-    fetch(block + gridDim.x);
-    float t = 0.f;
-#pragma unroll
-    for (int p = 0; p < kPer; ++p) {
-      float n[kVec], g[kVec], w[kVec];
-      hc[p].get(n);
-      gc[p].get(g);
-      if (column(p) < a.C) {
-        weights<W, kVec>(a.w, column(p), w);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          n[i] *= rstd;
-          dw[p][i] = fmaf(g[i], n[i], dw[p][i]);
-          t = fmaf(g[i] * w[i], n[i], t);
-        }
+      if constexpr (kSize >= 4) {
+        copy_async<kSize>(place(stage, 0, p), static_cast<const T*>(a.x) + at, in);
+        copy_async<kSize>(place(stage, 1, p), static_cast<const T*>(a.dy) + at, in);
+        if (a.dsum) copy_async<kSize>(place(stage, 2, p), static_cast<const T*>(a.dsum) + at, in);
+      } else {      // (no asynchronous copies of two bytes)
+        (in ? Ch::load(static_cast<const T*>(a.x) + at) : Ch::zero()).store(reinterpret_cast<T*>(place(stage, 0, p)));
+        (in ? Ch::load(static_cast<const T*>(a.dy) + at) : Ch::zero()).store(reinterpret_cast<T*>(place(stage, 1, p)));
+        if (a.dsum) (in ? Ch::load(static_cast<const T*>(a.dsum) + at) : Ch::zero()).store(reinterpret_cast<T*>(place(stage, 2, p)));
       }
     }
-    const float mean = over_row<add>(t, tpr, red[turn]) * a.inv_c;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return in_rows ? __ldg(a.rstd + row) : 0.f;
+  };
+  float rstds[Rg::kAhead];
+#pragma unroll
+  for (int i = 0; i < Rg::kAhead; ++i) rstds[i] = fetch(blockIdx.x + int64_t(i) * gridDim.x, i);
+  int stage = 0, turn = 0;
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    const int64_t row = block * groups + mine;
+    const float rstd = rstds[0];
+    if constexpr (Rg::kAhead == 2) rstds[0] = rstds[1];
+    // (into the stage before this one, which this thread has left)
+    rstds[Rg::kAhead - 1] = fetch(block + int64_t(Rg::kAhead) * gridDim.x, stage == 0 ? Rg::kAhead : stage - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(Rg::kAhead) : "memory");
+    float2 t2 = make_float2(0.f, 0.f), n[kPer][kPairs], g[kPer][kPairs];
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      float2 v[kPairs];
+      Ch::load_cached(reinterpret_cast<const T*>(place(stage, 0, p))).get(n[p]);
+      Ch::load_cached(reinterpret_cast<const T*>(place(stage, 1, p))).get(g[p]);
+      w[p].get(v);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        n[p][i] = __fmul2_rn(n[p][i], make_float2(rstd, rstd));
+        dw[p][i] = __ffma2_rn(g[p][i], n[p][i], dw[p][i]);
+        g[p][i] = __fmul2_rn(g[p][i], v[i]);
+        t2 = __ffma2_rn(g[p][i], n[p][i], t2);
+      }
+    }
+    const float mean = over_row<add>(t2.x + t2.y, tpr, red + turn * kMaxWarps) * a.inv_c;
+    const float2 by = make_float2(-mean, -mean), s2 = make_float2(rstd, rstd);
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
       if (row >= a.rows || column(p) >= a.C) continue;
-      float n[kVec], g[kVec], w[kVec], d[kVec];
-      hc[p].get(n);
-      gc[p].get(g);
-      sc[p].get(d);
-      weights<W, kVec>(a.w, column(p), w);
+      float2 d[kPairs];
+      if (a.dsum) {
+        Ch::load_cached(reinterpret_cast<const T*>(place(stage, 2, p))).get(d);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) d[i] += rstd * (g[i] * w[i] - n[i] * rstd * mean);
+        for (int i = 0; i < kPairs; ++i) d[i] = make_float2(0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) d[i] = __ffma2_rn(s2, __ffma2_rn(n[p][i], by, g[p][i]), d[i]);
       Ch::of(d).store(static_cast<T*>(a.dx) + row * a.C + column(p));
     }
+    stage = stage == Rg::kAhead ? 0 : stage + 1;
   }
   if (!a.part) return;
   if (groups > 1) {      // one group after the other, so that the sums have one order
-    for (int g = 0; g < groups; ++g) {
+    float* columns = reinterpret_cast<float*>(ring);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    for (int k = 0; k < groups; ++k) {
       __syncthreads();
-      if (mine == g) {
+      if (mine == k) {
 #pragma unroll
-        for (int p = 0; p < kPer; ++p)
+        for (int p = 0; p < kPer; ++p) {
+          const float* own = reinterpret_cast<const float*>(dw[p]);
 #pragma unroll
           for (int i = 0; i < kVec; ++i)
-            if (column(p) < a.C) columns[column(p) + i] = dw[p][i] + (g ? columns[column(p) + i] : 0.f);
+            if (column(p) < a.C) columns[column(p) + i] = own[i] + (k ? columns[column(p) + i] : 0.f);
+        }
       }
     }
     __syncthreads();
@@ -373,44 +454,61 @@ rms_bwd_kernel(const RmsArgs a, int tpr) {
     return;
   }
 #pragma unroll
-  for (int p = 0; p < kPer; ++p)
+  for (int p = 0; p < kPer; ++p) {
+    if (column(p) >= a.C) continue;
+    float* to = a.part + int64_t(blockIdx.x) * a.C + column(p);
+    if constexpr (kVec == 1) {
+      *to = dw[p][0].x;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (column(p) < a.C) a.part[int64_t(blockIdx.x) * a.C + column(p) + i] = dw[p][i];
+      for (int i = 0; i < kPairs; i += 2) *reinterpret_cast<float4*>(to + 2 * i) = make_float4(dw[p][i].x, dw[p][i].y, dw[p][i + 1].x, dw[p][i + 1].y);
+    }
+  }
 }
 
 // dx of a row per CTA, read twice.
 template <typename T, typename W, int kVec>
-__global__ void __launch_bounds__(kThreads) rms_bwd_wide_kernel(const RmsArgs a) {
-  __shared__ float red[kWarps];
+__global__ void __launch_bounds__(kWide) rms_bwd_wide_kernel(const RmsArgs a) {
+  __shared__ __align__(16) float red[kMaxWarps];
   using Ch = Chunk<T, kVec>;
+  constexpr int kPairs = Ch::kPairs;
   const int64_t row = blockIdx.x, base = row * a.C;
   const float rstd = a.rstd[row];
-  float t = 0.f;
-  for (int c = threadIdx.x * kVec; c < a.C; c += kThreads * kVec) {
-    float n[kVec], g[kVec], w[kVec];
+  const float2 s2 = make_float2(rstd, rstd);
+  float2 t2 = make_float2(0.f, 0.f);
+  auto operands = [&](int c, float2 (&n)[kPairs], float2 (&g)[kPairs]) {      // n, and dy w
+    float2 v[kPairs];
     Ch::load_cached(static_cast<const T*>(a.x) + base + c).get(n);
     Ch::load_cached(static_cast<const T*>(a.dy) + base + c).get(g);
-    weights<W, kVec>(a.w, c, w);
+    weights<W, kVec>(a.w, c, true).get(v);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) t = fmaf(g[i] * w[i], n[i] * rstd, t);
+    for (int i = 0; i < kPairs; ++i) {
+      n[i] = __fmul2_rn(n[i], s2);
+      g[i] = __fmul2_rn(g[i], v[i]);
+    }
+  };
+  for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
+    float2 n[kPairs], g[kPairs];
+    operands(c, n, g);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) t2 = __ffma2_rn(g[i], n[i], t2);
   }
-  const float mean = over_row<add>(t, kThreads, red) * a.inv_c;
-  for (int c = threadIdx.x * kVec; c < a.C; c += kThreads * kVec) {
-    float n[kVec], g[kVec], w[kVec], d[kVec];
-    Ch::load_cached(static_cast<const T*>(a.x) + base + c).get(n);
-    Ch::load_cached(static_cast<const T*>(a.dy) + base + c).get(g);
-    weights<W, kVec>(a.w, c, w);
+  const float mean = over_row<add>(t2.x + t2.y, kWide, red) * a.inv_c;
+  for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
+    float2 n[kPairs], g[kPairs], d[kPairs];
+    operands(c, n, g);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) d[i] = make_float2(0.f, 0.f);
     if (a.dsum) Ch::load_cached(static_cast<const T*>(a.dsum) + base + c).get(d);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) d[i] = (a.dsum ? d[i] : 0.f) + rstd * (g[i] * w[i] - n[i] * rstd * mean);
+    for (int i = 0; i < kPairs; ++i) d[i] = __ffma2_rn(s2, __ffma2_rn(n[i], make_float2(-mean, -mean), g[i]), d[i]);
     Ch::of(d).store(static_cast<T*>(a.dx) + base + c);
   }
 }
 // dw of wide rows: a thread has a column, a CTA row the rows of its part.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) rms_dweight_wide_kernel(const RmsArgs a) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kWide) rms_dweight_wide_kernel(const RmsArgs a) {
+  const int c = blockIdx.x * kWide + threadIdx.x;
   if (c >= a.C) return;
   const int64_t r0 = a.rows * blockIdx.y / gridDim.y, r1 = a.rows * (blockIdx.y + 1) / gridDim.y;
   float sum = 0.f;
@@ -425,8 +523,11 @@ __global__ void __launch_bounds__(1024) rms_dweight_kernel(const float* part, in
   __shared__ float sums[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float sum = 0.f;
-  if (c < C)
-    for (int r = threadIdx.y; r < rows; r += 32) sum += part[int64_t(r) * C + c];
+  wait_for_previous();
+  if (c < C) {
+#pragma unroll 4
+    for (int r = threadIdx.y; r < rows; r += 32) sum += __ldcg(part + int64_t(r) * C + c);
+  }
   sums[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   float v = sums[threadIdx.x][threadIdx.y];
@@ -441,22 +542,26 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct Shape {
   bool vec;
   int tpr;       // threads of a row
-  int per;       // chunks of a thread; 0: the row is too wide to be held
+  int threads;   // of a CTA: 256, or those of a longer row
+  int per;       // chunks of a thread: least_per, two, four or (forward) eight times that; 0: the row is too wide to be held
 };
-constexpr int kMostVec = 8, kMostScalar = 32;      // chunks of a thread
+constexpr int least_per(bool vec) { return vec ? 1 : 4; }
 
-Shape shape_of(int C, int esz, bool vec) {
-  Shape s{vec, 32, 0};
-  const int chunks = vec ? C * esz / 16 : C, least = vec ? 2 : 4, most = vec ? kMostVec : kMostScalar;
-  while (s.tpr < kThreads && s.tpr * least < chunks) s.tpr *= 2;
-  for (int per = vec ? 1 : 4; per <= most; per *= 2)
+Shape shape_of(int C, int esz, bool vec, int most) {      // most: times least_per
+  Shape s{vec, 32, 256, 0};
+  const int chunks = vec ? C * esz / 16 : C, least = least_per(vec);
+  while (s.tpr < 512 && s.tpr * 2 * least < chunks) s.tpr *= 2;
+  for (int per = least; per <= most * least; per *= 2)
     if (s.tpr * per >= chunks) { s.per = per; break; }
+  s.threads = s.tpr < 256 ? 256 : s.tpr;
   return s;
 }
 
-int bwd_ctas(const Shape& s, int vec_elements) {      // resident per SM, as the launch bounds say
-  const int elements = s.per * vec_elements;
-  return elements <= 8 ? 4 : elements <= 16 ? 3 : elements <= 32 ? 2 : 1;
+// CTAs per SM of the backward, as its launch bounds say: by the registers of its sums and of the row at hand, and the ring.
+constexpr int bwd_ctas(int elements, int threads, int ring) {
+  const int warps = (elements <= 8 ? 32 : elements <= 16 ? 24 : elements <= 32 ? 16 : 8), regs = warps * 32 / threads;
+  const int room = 227 * 1024 / (ring + 1280);
+  return regs < 1 || room < 1 ? 1 : regs < room ? regs : room;
 }
 
 int check(const nb200_rms_norm_params* p, const char* what) {
@@ -476,72 +581,112 @@ bool vectors(const nb200_rms_norm_params* p, bool backward) {
   return aligned16(p->residual) && aligned16(p->sum) && aligned16(p->y);
 }
 
-// The backward's shape and the rows of partial sums that it leaves.
+// Calls f with the kernel's (kVec, kPer, kThreads).
+template <typename T, bool kForward, typename F>
+int with_shape(const Shape& s, F f) {
+  constexpr int kVec = 16 / int(sizeof(T));
+  auto with_per = [&](auto vec, auto threads) {
+    constexpr int kLeast = least_per(decltype(vec)::value > 1);
+    if (s.per == kLeast) return f(vec, std::integral_constant<int, kLeast>{}, threads);
+    if (s.per == 2 * kLeast) return f(vec, std::integral_constant<int, 2 * kLeast>{}, threads);
+    if constexpr (decltype(threads)::value == 512) {      // (smaller CTAs have rows of two chunks a thread at most)
+      if (s.per == 4 * kLeast) return f(vec, std::integral_constant<int, 4 * kLeast>{}, threads);
+      if constexpr (kForward) return f(vec, std::integral_constant<int, 8 * kLeast>{}, threads);
+    }
+    set_error("rms_norm: no kernel for %d chunks a thread", s.per);
+    return int(NB200_ERR_UNSUPPORTED);
+  };
+  auto with_threads = [&](auto vec) {
+    return s.threads == 256 ? with_per(vec, std::integral_constant<int, 256>{}) : with_per(vec, std::integral_constant<int, 512>{});
+  };
+  return s.vec ? with_threads(std::integral_constant<int, kVec>{}) : with_threads(std::integral_constant<int, 1>{});
+}
+
+// The backward's shape, what it takes of an SM, and the rows of partial sums that it leaves.
 struct BwdPlan {
   Shape s;
   int parts;
 };
-BwdPlan bwd_plan(const nb200_rms_norm_params* p, bool vec) {
-  const int esz = dtype_size(p->dtype);
-  BwdPlan pl{shape_of(p->channels, esz, vec), 0};
+template <int kVec, int kPer, int kThreads, int kSize>
+struct BwdShape {
+  static constexpr int kRing = Ring<kPer, kThreads, kSize>::kBytes;
+  static constexpr int kCtas = bwd_ctas(kPer * kVec, kThreads, kRing);
+};
+template <typename T>
+BwdPlan bwd_plan(int C, int64_t rows, bool vec) {
+  BwdPlan pl{shape_of(C, int(sizeof(T)), vec, 4), 0};
   if (pl.s.per == 0) {
-    pl.parts = int(p->rows < 64 ? p->rows : 64);
-  } else {
-    const int64_t blocks = (p->rows + kThreads / pl.s.tpr - 1) / (kThreads / pl.s.tpr);
-    const int64_t most = int64_t(tc::sm_count()) * bwd_ctas(pl.s, vec ? 16 / esz : 1);
-    pl.parts = int(blocks < most ? blocks : most);
+    pl.parts = int(rows < 64 ? rows : 64);
+    return pl;
   }
+  with_shape<T, false>(pl.s, [&](auto kv, auto kp, auto kt) {
+    constexpr int kVec = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
+    const int64_t groups = kThreads / pl.s.tpr, blocks = (rows + groups - 1) / groups;
+    const int64_t most = int64_t(tc::sm_count()) * BwdShape<kVec, kPer, kThreads, kVec * int(sizeof(T))>::kCtas;
+    pl.parts = int(blocks < most ? blocks : most);
+    return int(NB200_OK);
+  });
   return pl;
 }
+BwdPlan bwd_plan(const nb200_rms_norm_params* p) {
+  const bool vec = vectors(p, true);
+  return p->dtype == NB200_F32 ? bwd_plan<float>(p->channels, p->rows, vec) : bwd_plan<__half>(p->channels, p->rows, vec);
+}
 
-template <typename T, typename W, int kVec, bool kEight>
+template <typename T, typename W, bool kEight>
 int launch_fwd(const RmsArgs& a, const Shape& s, cudaStream_t st) {
-  const unsigned grid = unsigned((a.rows + kThreads / s.tpr - 1) / (kThreads / s.tpr));
-  constexpr int k = kVec == 1 ? 4 : 1;
-  if (s.per == 0) rms_fwd_wide_kernel<T, W, kVec, kEight><<<unsigned(a.rows), kThreads, 0, st>>>(a);
-  else if (s.per == k) rms_fwd_kernel<T, W, kVec, k, kEight><<<grid, kThreads, 0, st>>>(a, s.tpr);
-  else if (s.per == 2 * k) rms_fwd_kernel<T, W, kVec, 2 * k, kEight><<<grid, kThreads, 0, st>>>(a, s.tpr);
-  else if (s.per == 4 * k) rms_fwd_kernel<T, W, kVec, 4 * k, kEight><<<grid, kThreads, 0, st>>>(a, s.tpr);
-  else rms_fwd_kernel<T, W, kVec, 8 * k, kEight><<<grid, kThreads, 0, st>>>(a, s.tpr);
-  count_launch();
-  return check_launch("rms_fwd_kernel");
+  constexpr int kVec = 16 / int(sizeof(T));
+  if (s.per == 0) {
+    if (s.vec) rms_fwd_wide_kernel<T, W, kVec, kEight><<<unsigned(a.rows), kWide, 0, st>>>(a);
+    else rms_fwd_wide_kernel<T, W, 1, kEight><<<unsigned(a.rows), kWide, 0, st>>>(a);
+    count_launch();
+    return check_launch("rms_fwd_wide_kernel");
+  }
+  return with_shape<T, true>(s, [&](auto kv, auto kp, auto kt) {
+    constexpr int kV = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
+    constexpr int kCtas = (kPer <= 2 * least_per(kV > 1) ? 1024 : 512) / kThreads;
+    const int64_t groups = kThreads / s.tpr, blocks = (a.rows + groups - 1) / groups, most = int64_t(tc::sm_count()) * kCtas;
+    rms_fwd_kernel<T, W, kV, kPer, kThreads, kEight><<<unsigned(blocks < most ? blocks : most), kThreads, 0, st>>>(a, s.tpr);
+    count_launch();
+    return check_launch("rms_fwd_kernel");
+  });
 }
 template <typename T, typename W>
 int launch_fwd(const RmsArgs& a, const Shape& s, cudaStream_t st) {
-  constexpr int kVec = 16 / int(sizeof(T));
-  if (a.scales) return s.vec ? launch_fwd<T, W, kVec, true>(a, s, st) : launch_fwd<T, W, 1, true>(a, s, st);
-  return s.vec ? launch_fwd<T, W, kVec, false>(a, s, st) : launch_fwd<T, W, 1, false>(a, s, st);
+  return a.scales ? launch_fwd<T, W, true>(a, s, st) : launch_fwd<T, W, false>(a, s, st);
 }
 
-template <typename T, typename W, int kVec>
-int launch_bwd(const RmsArgs& a, const BwdPlan& pl, cudaStream_t st) {
-  const Shape& s = pl.s;
-  constexpr int k = kVec == 1 ? 4 : 1;
-  if (s.per == 0) {
-    rms_bwd_wide_kernel<T, W, kVec><<<unsigned(a.rows), kThreads, 0, st>>>(a);
+template <typename T, typename W>
+int launch_rows(const RmsArgs& a, const BwdPlan& pl, cudaStream_t st) {
+  constexpr int kVec = 16 / int(sizeof(T));
+  if (pl.s.per == 0) {
+    if (pl.s.vec) rms_bwd_wide_kernel<T, W, kVec><<<unsigned(a.rows), kWide, 0, st>>>(a);
+    else rms_bwd_wide_kernel<T, W, 1><<<unsigned(a.rows), kWide, 0, st>>>(a);
     count_launch();
     if (int rc = check_launch("rms_bwd_wide_kernel")) return rc;
-    if (a.part) {
-      rms_dweight_wide_kernel<T><<<dim3(unsigned((a.C + kThreads - 1) / kThreads), unsigned(pl.parts)), kThreads, 0, st>>>(a);
-      count_launch();
-      return check_launch("rms_dweight_wide_kernel");
-    }
-    return NB200_OK;
+    if (!a.part) return NB200_OK;
+    rms_dweight_wide_kernel<T><<<dim3(unsigned((a.C + kWide - 1) / kWide), unsigned(pl.parts)), kWide, 0, st>>>(a);
+    count_launch();
+    return check_launch("rms_dweight_wide_kernel");
   }
-  const size_t smem = s.tpr < kThreads && a.part ? size_t(a.C) * sizeof(float) : 0;
-  if (s.per == k) rms_bwd_kernel<T, W, kVec, k><<<unsigned(pl.parts), kThreads, smem, st>>>(a, s.tpr);
-  else if (s.per == 2 * k) rms_bwd_kernel<T, W, kVec, 2 * k><<<unsigned(pl.parts), kThreads, smem, st>>>(a, s.tpr);
-  else if (s.per == 4 * k) rms_bwd_kernel<T, W, kVec, 4 * k><<<unsigned(pl.parts), kThreads, smem, st>>>(a, s.tpr);
-  else rms_bwd_kernel<T, W, kVec, 8 * k><<<unsigned(pl.parts), kThreads, smem, st>>>(a, s.tpr);
-  count_launch();
-  return check_launch("rms_bwd_kernel");
+  return with_shape<T, false>(pl.s, [&](auto kv, auto kp, auto kt) {
+    constexpr int kV = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
+    using B = BwdShape<kV, kPer, kThreads, kV * int(sizeof(T))>;
+    // (the sums of rows that share a CTA are joined in the ring: 256 threads' columns of fp32)
+    constexpr int smem = B::kRing < kPer * kThreads * kV * 4 ? kPer * kThreads * kV * 4 : B::kRing;
+    auto kernel = rms_bwd_kernel<T, W, kV, kPer, kThreads, B::kCtas>;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return check_launch("rms_bwd_kernel");
+    kernel<<<unsigned(pl.parts), kThreads, smem, st>>>(a, pl.s.tpr);
+    count_launch();
+    return check_launch("rms_bwd_kernel");
+  });
 }
 template <typename T, typename W>
 int launch_bwd(const RmsArgs& a, const BwdPlan& pl, void* dweight, cudaStream_t st) {
-  constexpr int kVec = 16 / int(sizeof(T));
-  if (int rc = pl.s.vec ? launch_bwd<T, W, kVec>(a, pl, st) : launch_bwd<T, W, 1>(a, pl, st)) return rc;
+  if (int rc = launch_rows<T, W>(a, pl, st)) return rc;
   if (!a.part) return NB200_OK;
-  rms_dweight_kernel<W><<<unsigned((a.C + 31) / 32), dim3(32, 32), 0, st>>>(a.part, pl.parts, a.C, static_cast<W*>(dweight));
+  if (launch_dependent(rms_dweight_kernel<W>, dim3(unsigned((a.C + 31) / 32)), dim3(32, 32), 0, st, static_cast<const float*>(a.part), pl.parts, a.C, static_cast<W*>(dweight)) != cudaSuccess)
+    return check_launch("rms_dweight_kernel");
   count_launch();
   return check_launch("rms_dweight_kernel");
 }
@@ -554,7 +699,7 @@ using namespace nb200;
 extern "C" NB200_API int nb200_rms_norm_workspace_bytes(const nb200_rms_norm_params* p, size_t* bytes) {
   if (!bytes) { set_error("bytes out-pointer is NULL"); return NB200_ERR_INVALID; }
   if (int rc = check(p, "rms_norm_workspace_bytes")) return rc;
-  *bytes = size_t(bwd_plan(p, vectors(p, true)).parts) * size_t(p->channels) * sizeof(float);
+  *bytes = size_t(bwd_plan(p).parts) * size_t(p->channels) * sizeof(float);
   return NB200_OK;
 }
 
@@ -576,7 +721,7 @@ extern "C" NB200_API int nb200_rms_norm_fwd(const nb200_rms_norm_params* p, void
   a.group = p->group ? p->group : p->channels;
   a.eps = p->eps;
   a.inv_c = float(1.0 / p->channels);
-  const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec);
+  const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec, 8);
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   const bool wide_weight = p->weight_dtype == NB200_F32;
@@ -593,7 +738,7 @@ extern "C" NB200_API int nb200_rms_norm_bwd(const nb200_rms_norm_params* p, void
     return NB200_OK;
   }
   if (!p->x || !p->dy || !p->dx || !p->rstd) { set_error("rms_norm_bwd: NULL operand"); return NB200_ERR_INVALID; }
-  const BwdPlan pl = bwd_plan(p, vectors(p, true));
+  const BwdPlan pl = bwd_plan(p);
   RmsArgs a{};
   a.x = p->x; a.w = p->weight; a.rstd = p->rstd; a.dy = p->dy; a.dsum = p->dsum; a.dx = p->dx;
   a.rows = p->rows; a.C = p->channels;
