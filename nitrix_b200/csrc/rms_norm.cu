@@ -137,12 +137,13 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr > 32) {
-    const int warp = threadIdx.x >> 5, warps = tpr >> 5, first = warp & ~(warps - 1);
+    const int warp = threadIdx.x >> 5, warps = tpr >> 5, first = tpr == int(blockDim.x) ? 0 : warp & ~(warps - 1);
     if ((threadIdx.x & 31) == 0) red[warp] = v;
     __syncthreads();
     const float2* sums = reinterpret_cast<const float2*>(red + first);
     v = op(sums[0].x, sums[0].y);
     for (int i = 1; i < warps / 2; ++i) v = op(v, op(sums[i].x, sums[i].y));
+    if (warps & 1) v = op(v, red[first + warps - 1]);
   }
   return v;
 }
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
   __shared__ __align__(16) float red[4 * kMaxWarps];
   using C = Chunk<T, kVec>;
   constexpr int kPairs = C::kPairs;
-  const int tin = threadIdx.x & (tpr - 1), groups = kThreads / tpr, mine = threadIdx.x / tpr;
+  const int groups = blockDim.x / tpr, mine = groups == 1 ? 0 : threadIdx.x / tpr, tin = threadIdx.x - mine * tpr;
   const int64_t blocks = (a.rows + groups - 1) / groups;
   auto column = [&](int p) { return (p * tpr + tin) * kVec; };
   C nx[kPer], nr[kPer];
@@ -339,9 +340,9 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
 // kAhead rows into its own places of a ring in shared memory, so that no barrier is needed for them.
 template <int kPer, int kThreads, int kChunkBytes>
 struct Ring {
-  static constexpr int kRow = 3 * kPer * kThreads * kChunkBytes;      // h, dy and dsum of a row (or of as many as share the CTA)
-  static constexpr int kAhead = kRow <= 24576 ? 2 : 1;
-  static constexpr int kBytes = (kAhead + 1) * kRow;
+  static constexpr int kThread = 3 * kPer * kChunkBytes;                        // h, dy and dsum of a row, of a thread
+  static constexpr int kAhead = kThread * kThreads <= 24576 ? 2 : 1;
+  __host__ __device__ static constexpr int bytes(int threads) { return (kAhead + 1) * kThread * threads; }
 };
 template <int kBytes>
 __device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_bwd_kernel(const RmsArgs 
   using Rg = Ring<kPer, kThreads, kSize>;
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float red[2 * kMaxWarps];
-  const int tin = threadIdx.x & (tpr - 1), mine = threadIdx.x / tpr, groups = kThreads / tpr;
+  const int groups = blockDim.x / tpr, mine = groups == 1 ? 0 : threadIdx.x / tpr, tin = threadIdx.x - mine * tpr;
   auto column = [&](int p) { return (p * tpr + tin) * kVec; };
   float2 dw[kPer][kPairs];
   Chunk<W, kVec> w[kPer];
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_bwd_kernel(const RmsArgs 
     w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
   }
   const int64_t blocks = (a.rows + groups - 1) / groups;
-  auto place = [&](int stage, int which, int p) { return ring + stage * Rg::kRow + ((which * kPer + p) * kThreads + threadIdx.x) * kSize; };
+  auto place = [&](int stage, int which, int p) { return ring + (((stage * 3 + which) * kPer + p) * int(blockDim.x) + threadIdx.x) * kSize; };
   auto fetch = [&](int64_t block, int stage) {
     const int64_t row = block * groups + mine;
     const bool in_rows = block < blocks && row < a.rows;
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_bwd_kernel(const RmsArgs 
       }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.C; c += kThreads) a.part[int64_t(blockIdx.x) * a.C + c] = columns[c];
+    for (int c = threadIdx.x; c < a.C; c += blockDim.x) a.part[int64_t(blockIdx.x) * a.C + c] = columns[c];
     return;
   }
 #pragma unroll
@@ -538,31 +539,38 @@ __global__ void __launch_bounds__(1024) rms_dweight_kernel(const float* part, in
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// How a row is divided.
+// How a row is divided: by `tpr` threads, a power of two that shares a CTA of 256 with other rows, or from 160 on a CTA of its own.
 struct Shape {
   bool vec;
-  int tpr;       // threads of a row
-  int threads;   // of a CTA: 256, or those of a longer row
+  int tpr, threads;
   int per;       // chunks of a thread: least_per, two, four or (forward) eight times that; 0: the row is too wide to be held
 };
 constexpr int least_per(bool vec) { return vec ? 1 : 4; }
 
-Shape shape_of(int C, int esz, bool vec, int most) {      // most: times least_per
-  Shape s{vec, 32, 256, 0};
+// The backward takes one chunk a thread as long as 512 threads hold the row (16384 rows of 4096, bf16: two chunks of 256 threads 124 us,
+// one of 512 90; 1024 threads for 8192 channels 89, two chunks of 512 78), the forward two (93 us either way, and fewer shuffles).
+Shape shape_of(int C, int esz, bool vec, bool backward) {
+  Shape s{vec, 0, 0, 0};
   const int chunks = vec ? C * esz / 16 : C, least = least_per(vec);
-  while (s.tpr < 512 && s.tpr * 2 * least < chunks) s.tpr *= 2;
-  for (int per = least; per <= most * least; per *= 2)
-    if (s.tpr * per >= chunks) { s.per = per; break; }
-  s.threads = s.tpr < 256 ? 256 : s.tpr;
+  for (int per = backward ? least : 2 * least; per <= (backward ? 4 : 8) * least; per *= 2) {
+    const int threads = (chunks + per - 1) / per;
+    if (threads > 512) continue;
+    s.per = per;
+    if (threads > 128) {
+      s.tpr = s.threads = (threads + 31) / 32 * 32;
+    } else {
+      s.threads = 256;
+      for (s.tpr = 32; s.tpr < threads;) s.tpr *= 2;
+      if (!backward && s.tpr * least >= chunks) s.per = least;      // (short rows, of a warp)
+    }
+    return s;
+  }
   return s;
 }
-
-// CTAs per SM of the backward, as its launch bounds say: by the registers of its sums and of the row at hand, and the ring.
-constexpr int bwd_ctas(int elements, int threads, int ring) {
-  const int warps = (elements <= 8 ? 32 : elements <= 16 ? 24 : elements <= 32 ? 16 : 8), regs = warps * 32 / threads;
-  const int room = 227 * 1024 / (ring + 1280);
-  return regs < 1 || room < 1 ? 1 : regs < room ? regs : room;
-}
+// Threads of all CTAs of an SM, by the registers that a thread takes (the kernels' launch bounds), and CTAs of `threads`.
+constexpr int fwd_threads(int per, int vec) { return per <= (vec == 1 ? 8 : 2) ? 1024 : 512; }
+constexpr int bwd_threads(int elements) { return elements <= 8 ? 1024 : elements <= 16 ? 768 : 512; }
+constexpr int ctas_of(int all, int threads) { return all < threads ? 1 : all / threads; }
 
 int check(const nb200_rms_norm_params* p, const char* what) {
   if (!p || p->struct_size != sizeof(nb200_rms_norm_params)) { set_error("%s: NULL params or wrong struct_size", what); return NB200_ERR_INVALID; }
@@ -581,7 +589,7 @@ bool vectors(const nb200_rms_norm_params* p, bool backward) {
   return aligned16(p->residual) && aligned16(p->sum) && aligned16(p->y);
 }
 
-// Calls f with the kernel's (kVec, kPer, kThreads).
+// Calls f with the kernel's (kVec, kPer, kThreads: the most threads of a CTA).
 template <typename T, bool kForward, typename F>
 int with_shape(const Shape& s, F f) {
   constexpr int kVec = 16 / int(sizeof(T));
@@ -589,7 +597,7 @@ int with_shape(const Shape& s, F f) {
     constexpr int kLeast = least_per(decltype(vec)::value > 1);
     if (s.per == kLeast) return f(vec, std::integral_constant<int, kLeast>{}, threads);
     if (s.per == 2 * kLeast) return f(vec, std::integral_constant<int, 2 * kLeast>{}, threads);
-    if constexpr (decltype(threads)::value == 512) {      // (smaller CTAs have rows of two chunks a thread at most)
+    if constexpr (decltype(threads)::value == 512) {      // (smaller CTAs have rows of few chunks a thread)
       if (s.per == 4 * kLeast) return f(vec, std::integral_constant<int, 4 * kLeast>{}, threads);
       if constexpr (kForward) return f(vec, std::integral_constant<int, 8 * kLeast>{}, threads);
     }
@@ -597,32 +605,31 @@ int with_shape(const Shape& s, F f) {
     return int(NB200_ERR_UNSUPPORTED);
   };
   auto with_threads = [&](auto vec) {
-    return s.threads == 256 ? with_per(vec, std::integral_constant<int, 256>{}) : with_per(vec, std::integral_constant<int, 512>{});
+    return s.threads <= 256 ? with_per(vec, std::integral_constant<int, 256>{}) : with_per(vec, std::integral_constant<int, 512>{});
   };
   return s.vec ? with_threads(std::integral_constant<int, kVec>{}) : with_threads(std::integral_constant<int, 1>{});
 }
 
-// The backward's shape, what it takes of an SM, and the rows of partial sums that it leaves.
+// The backward's shape, its shared memory, and the rows of partial sums that it leaves, one per CTA.
 struct BwdPlan {
   Shape s;
-  int parts;
-};
-template <int kVec, int kPer, int kThreads, int kSize>
-struct BwdShape {
-  static constexpr int kRing = Ring<kPer, kThreads, kSize>::kBytes;
-  static constexpr int kCtas = bwd_ctas(kPer * kVec, kThreads, kRing);
+  int smem, parts;
 };
 template <typename T>
 BwdPlan bwd_plan(int C, int64_t rows, bool vec) {
-  BwdPlan pl{shape_of(C, int(sizeof(T)), vec, 4), 0};
+  BwdPlan pl{shape_of(C, int(sizeof(T)), vec, true), 0, 0};
   if (pl.s.per == 0) {
     pl.parts = int(rows < 64 ? rows : 64);
     return pl;
   }
   with_shape<T, false>(pl.s, [&](auto kv, auto kp, auto kt) {
     constexpr int kVec = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
-    const int64_t groups = kThreads / pl.s.tpr, blocks = (rows + groups - 1) / groups;
-    const int64_t most = int64_t(tc::sm_count()) * BwdShape<kVec, kPer, kThreads, kVec * int(sizeof(T))>::kCtas;
+    // (the sums of rows that share a CTA are joined in the ring)
+    const int ring = Ring<kPer, kThreads, kVec * int(sizeof(T))>::bytes(pl.s.threads), columns = pl.s.tpr < pl.s.threads ? C * 4 : 0;
+    pl.smem = ring > columns ? ring : columns;
+    const int by_threads = ctas_of(bwd_threads(kPer * kVec), pl.s.threads), by_room = 227 * 1024 / (pl.smem + 2048);
+    const int64_t groups = pl.s.threads / pl.s.tpr, blocks = (rows + groups - 1) / groups;
+    const int64_t most = int64_t(tc::sm_count()) * (by_threads < by_room ? by_threads : by_room);
     pl.parts = int(blocks < most ? blocks : most);
     return int(NB200_OK);
   });
@@ -644,9 +651,9 @@ int launch_fwd(const RmsArgs& a, const Shape& s, cudaStream_t st) {
   }
   return with_shape<T, true>(s, [&](auto kv, auto kp, auto kt) {
     constexpr int kV = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
-    constexpr int kCtas = (kPer <= 2 * least_per(kV > 1) ? 1024 : 512) / kThreads;
-    const int64_t groups = kThreads / s.tpr, blocks = (a.rows + groups - 1) / groups, most = int64_t(tc::sm_count()) * kCtas;
-    rms_fwd_kernel<T, W, kV, kPer, kThreads, kEight><<<unsigned(blocks < most ? blocks : most), kThreads, 0, st>>>(a, s.tpr);
+    const int64_t groups = s.threads / s.tpr, blocks = (a.rows + groups - 1) / groups;
+    const int64_t most = int64_t(tc::sm_count()) * ctas_of(fwd_threads(kPer, kV), s.threads);
+    rms_fwd_kernel<T, W, kV, kPer, kThreads, kEight><<<unsigned(blocks < most ? blocks : most), s.threads, 0, st>>>(a, s.tpr);
     count_launch();
     return check_launch("rms_fwd_kernel");
   });
@@ -671,12 +678,9 @@ int launch_rows(const RmsArgs& a, const BwdPlan& pl, cudaStream_t st) {
   }
   return with_shape<T, false>(pl.s, [&](auto kv, auto kp, auto kt) {
     constexpr int kV = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
-    using B = BwdShape<kV, kPer, kThreads, kV * int(sizeof(T))>;
-    // (the sums of rows that share a CTA are joined in the ring: 256 threads' columns of fp32)
-    constexpr int smem = B::kRing < kPer * kThreads * kV * 4 ? kPer * kThreads * kV * 4 : B::kRing;
-    auto kernel = rms_bwd_kernel<T, W, kV, kPer, kThreads, B::kCtas>;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return check_launch("rms_bwd_kernel");
-    kernel<<<unsigned(pl.parts), kThreads, smem, st>>>(a, pl.s.tpr);
+    auto kernel = rms_bwd_kernel<T, W, kV, kPer, kThreads, ctas_of(bwd_threads(kPer * kV), kThreads)>;
+    if (pl.smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess) return check_launch("rms_bwd_kernel");
+    kernel<<<unsigned(pl.parts), pl.s.threads, pl.smem, st>>>(a, pl.s.tpr);
     count_launch();
     return check_launch("rms_bwd_kernel");
   });
@@ -721,7 +725,7 @@ extern "C" NB200_API int nb200_rms_norm_fwd(const nb200_rms_norm_params* p, void
   a.group = p->group ? p->group : p->channels;
   a.eps = p->eps;
   a.inv_c = float(1.0 / p->channels);
-  const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec, 8);
+  const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec, false);
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   const bool wide_weight = p->weight_dtype == NB200_F32;
