@@ -31,61 +31,115 @@ __device__ __forceinline__ float larger(float a, float b) {      // a NaN on eit
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
   return m;
 }
+__device__ __forceinline__ float smaller(float a, float b) {
+  float m;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 
 // 8 elements of a group whose other elements the lanes beside (of a multiple of four) have.  All lanes of the warp call it.
 template <int kBits, typename T>
 __device__ __forceinline__ Quantized<kBits> quantize(const uint4 (&words)[sizeof(T) / 2]) {
-  constexpr float kHalf = float(1 << (kBits - 1));
+  constexpr int kHalf = 1 << (kBits - 1);
   const T* e = reinterpret_cast<const T*>(words);
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
-  float high = x[0], low = -x[0];      // the largest value, and the smallest one's opposite
+  float high = x[0], low = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
     high = larger(high, x[i]);
-    low = larger(low, -x[i]);
+    low = smaller(low, x[i]);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     high = larger(high, __shfl_xor_sync(0xffffffffu, high, o));
-    low = larger(low, __shfl_xor_sync(0xffffffffu, low, o));
+    low = smaller(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
-  const bool finite = high < INFINITY && low < INFINITY;      // (false for a NaN)
-  const float a = high >= low ? high : -low;
+  const bool finite = high < INFINITY && low > -INFINITY;      // (false for a NaN)
+  const float a = high >= -low ? high : low;
   const __half step = __float2half_rn(fminf(fmaxf(a * (-1.f / kHalf), -65504.f), 65504.f));
   const float s = __half2float(step);
-  const float inverse = finite && s != 0.f ? __frcp_rn(s) : 0.f;
+  const float inverse = s != 0.f ? __frcp_rn(s) : 0.f;
   Quantized<kBits> q;
   q.step = finite ? __half_as_ushort(step) : uint16_t(0x7fff);
-  uint32_t c[8];
-  // (adding 1.5 2^23 + half rounds to whole numbers, halves to even, and leaves the code in the lowest bits)
+  // Adding M = 1.5 2^23 + half rounds to whole numbers, halves to even, and leaves the code in the lowest bits of a number whose
+  // others are known: codes are put side by side by adding these numbers up, shifted, and taking the known bits off at the end.
+  constexpr float kM = 12582912.f + kHalf;
+  constexpr uint32_t kBase = 0x4b400000u, kKnown = kBits == 4 ? kBase * 0x11111111u : kBase * 0x01010101u;
+  uint32_t w[8 * kBits / 32] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float z = finite ? fminf(fmaxf(__fmul_rn(x[i], inverse), -kHalf), kHalf - 1.f) : 0.f;
-    c[i] = __float_as_uint(__fadd_rn(z, 12582912.f + kHalf)) & ((1u << kBits) - 1u);
+    const float z = fminf(fmaxf(__fmul_rn(x[i], inverse), float(-kHalf)), kHalf - 1.f);
+    w[i * kBits / 32] += __float_as_uint(__fadd_rn(z, kM)) << (i * kBits % 32);
   }
-  if constexpr (kBits == 4) {
-    q.lo = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12 | c[4] << 16 | c[5] << 20 | c[6] << 24 | c[7] << 28;
-    q.hi = 0;
-  } else {
-    q.lo = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    q.hi = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-  }
+  // (what is not finite, and a step of zero, has the codes of zero: z is zero in the second case)
+  constexpr uint32_t kZero = kBits == 4 ? 0x88888888u : 0x80808080u;
+  q.lo = finite ? w[0] - kKnown : kZero;
+  q.hi = kBits == 4 ? 0u : finite ? w[8 * kBits / 32 - 1] - kKnown : kZero;
   return q;
 }
 
-// The codes of elements 8 u .. 8 u + 7 of a group: parts 2 u and 2 u + 1 of the row.
+// The codes of elements 8 u .. 8 u + 7 of a group are parts 2 u and 2 u + 1 of the row.  In 4 bits with an even number of groups the
+// lane four further has the same parts of the group beside: the two put their codes together to 32-bit words, a part each.  All lanes
+// of the warp call it; those without `in` store nothing.
 template <int kBits>
-__device__ __forceinline__ void store_codes(uint8_t* row, int groups, int group, int u, const Quantized<kBits>& q) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int groups, int group, int u, const Quantized<kBits>& q, bool in) {
   if constexpr (kBits == 4) {
-    uint16_t* p = reinterpret_cast<uint16_t*>(row) + 2 * u * groups + group;
-    p[0] = uint16_t(q.lo);
-    p[groups] = uint16_t(q.lo >> 16);
-  } else {
+    if (groups % 2 == 0) {
+      const uint32_t beside = __shfl_xor_sync(0xffffffffu, q.lo, 4);
+      const bool odd = group & 1;
+      if (in) reinterpret_cast<uint32_t*>(row)[((2 * u + odd) * groups + group) >> 1] = odd ? __byte_perm(beside, q.lo, 0x7632) : __byte_perm(q.lo, beside, 0x5410);
+    } else if (in) {
+      uint16_t* p = reinterpret_cast<uint16_t*>(row) + 2 * u * groups + group;
+      p[0] = uint16_t(q.lo);
+      p[groups] = uint16_t(q.lo >> 16);
+    }
+  } else if (in) {
     uint32_t* p = reinterpret_cast<uint32_t*>(row) + 2 * u * groups + group;
     p[0] = q.lo;
     p[groups] = q.hi;
+  }
+}
+// The other way: the words that a lane reads (two in 8 bits), then the values of its 8 elements.
+template <int kBits>
+__device__ __forceinline__ uint2 load_words(const uint8_t* row, int groups, int group, int u) {
+  if constexpr (kBits == 4) {
+    if (groups % 2 == 0) return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(row) + (((2 * u + (group & 1)) * groups + group) >> 1)), 0u);
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + 2 * u * groups + group;
+    return make_uint2(__ldg(p) | uint32_t(__ldg(p + groups)) << 16, 0u);
+  } else {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + 2 * u * groups + group;
+    return make_uint2(__ldg(p), __ldg(p + groups));
+  }
+}
+template <int kBits>
+__device__ __forceinline__ void values_of(uint2 w, int groups, int group, float step, float2 (&x)[4]) {
+  if constexpr (kBits == 4) {
+    if (groups % 2 == 0) {
+      const uint32_t beside = __shfl_xor_sync(0xffffffffu, w.x, 4);
+      w.x = group & 1 ? __byte_perm(beside, w.x, 0x7632) : __byte_perm(w.x, beside, 0x5410);
+    }
+  }
+  // A code in the bits from p on of 2^23 is 2^23 + 2^p code: the half of the range and 2^23 come off exactly, the step takes 2^-p.
+  constexpr int kEach = 16 / kBits;      // codes of 16 bits
+#pragma unroll
+  for (int h = 0; h < 8 / kEach; ++h) {
+    const uint32_t part = kBits == 4 ? (h ? w.x >> 16 : w.x) : (h & 1 ? (h & 2 ? w.y : w.x) >> 16 : (h & 2 ? w.y : w.x));
+#pragma unroll
+    for (int i = 0; i < kEach; i += 2) {
+      float2 c;
+      float* e = &c.x;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int p = (i + j) * kBits;
+        e[j] = __uint_as_float(0x4b000000u | (part & (((1u << kBits) - 1u) << p)));
+      }
+      const float p0 = float(1u << (i * kBits)), p1 = float(1u << ((i + 1) * kBits));
+      constexpr float kHalf = float(1 << (kBits - 1));
+      c = __fadd2_rn(c, make_float2(-8388608.f - kHalf * p0, -8388608.f - kHalf * p1));
+      x[(h * kEach + i) / 2] = __fmul2_rn(c, make_float2(step / p0, step / p1));
+    }
   }
 }
 // A part's four codes of a group, less the half of their range.
@@ -94,7 +148,6 @@ __device__ __forceinline__ void load_codes(const uint8_t* row, int groups, int g
   constexpr float kHalf = float(1 << (kBits - 1));
   const uint32_t w = kBits == 4 ? uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + part * groups + group))
                                 : __ldg(reinterpret_cast<const uint32_t*>(row) + part * groups + group);
-  // (a code in the lowest bits of 2^23 is 2^23 + code)
 #pragma unroll
   for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(0x4b000000u | (w >> (kBits * i) & ((1u << kBits) - 1u))) - (8388608.f + kHalf);
 }

@@ -3,7 +3,10 @@
 // Bound by HBM: codes and steps (or elements) read once, the rows written once.  A warp takes a token at a time: its sequence by
 // bisection of the offsets, its page from the table; then a lane eight elements at a time, which are two parts of a row of codes
 // and one or two 16-byte words of the result.
+#include <type_traits>
+
 #include "cache_codes.cuh"
+#include "sdpa_tc_common.cuh"
 
 namespace nb200 {
 namespace {
@@ -19,6 +22,7 @@ struct ReadArgs {
   int64_t kss[3], vss[3];          // elements
   int pages, heads, page_size;
   int row;                         // units of a head's row: of 8 elements, or 16-byte words
+  int unit_shift;                  // log2 of row, or -1
   const int* table;
   const int* lengths;
   int rows, width;
@@ -30,13 +34,14 @@ struct ReadArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void store8(uint4* p, const float (&x)[8]) {
-  uint4 w[sizeof(T) / 2];
-  T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
-#pragma unroll
-  for (int i = 0; i < int(sizeof(T)) / 2; ++i) p[i] = w[i];
+__device__ __forceinline__ void store8(uint4* p, const float2 (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    p[0] = make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
+    p[1] = make_uint4(__float_as_uint(x[2].x), __float_as_uint(x[2].y), __float_as_uint(x[3].x), __float_as_uint(x[3].y));
+  } else {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    p[0] = make_uint4(tc::pack2<kBf16>(x[0].x, x[0].y), tc::pack2<kBf16>(x[1].x, x[1].y), tc::pack2<kBf16>(x[2].x, x[2].y), tc::pack2<kBf16>(x[3].x, x[3].y));
+  }
 }
 
 // kBits 0: words are copied; otherwise T is the type of the result.
@@ -83,22 +88,19 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
     const int groups = a.row / 4;
     const uint16_t* kt = a.k_steps + page * a.kss[0] + slot * a.kss[2];
     const uint16_t* vt = a.v_steps + page * a.vss[0] + slot * a.vss[2];
-    for (int i = lane; i < n; i += 32) {
-      const int h = i / a.row, c = i - h * a.row, group = c >> 2, u = c & 3;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const uint8_t* row = which ? vp + h * a.vs[1] : kp + h * a.ks[1];
-        const float step = __half2float(__ushort_as_half(__ldg(which ? vt + h * a.vss[1] + group : kt + h * a.kss[1] + group)));
-        float first[4], second[4], x[8];
-        load_codes<kBits>(row, groups, group, 2 * u, first);
-        load_codes<kBits>(row, groups, group, 2 * u + 1, second);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = step * first[j];
-          x[4 + j] = step * second[j];
-        }
-        store8<T>((which ? ov : ok) + int64_t(i) * kWords, x);
-      }
+    const int tail = groups % 2 == 0 ? 8 : 4;      // lanes that exchange words; n is a multiple
+    // (whole warps go round together; lanes behind the end repeat its last group's work and store nothing)
+#pragma unroll 2
+    for (int w0 = 0; w0 < n; w0 += 32) {
+      const int i = min(w0 + lane, n - tail + (lane & (tail - 1)));
+      const int h = a.unit_shift >= 0 ? i >> a.unit_shift : i / a.row, c = i - h * a.row, group = c >> 2, u = c & 3;
+      const uint2 kw = load_words<kBits>(kp + h * a.ks[1], groups, group, u), vw = load_words<kBits>(vp + h * a.vs[1], groups, group, u);
+      const float k_step = __half2float(__ushort_as_half(__ldg(kt + h * a.kss[1] + group))), v_step = __half2float(__ushort_as_half(__ldg(vt + h * a.vss[1] + group)));
+      float2 x[4];
+      values_of<kBits>(kw, groups, group, k_step, x);
+      if (w0 + lane < n) store8<T>(ok + int64_t(i) * kWords, x);
+      values_of<kBits>(vw, groups, group, v_step, x);
+      if (w0 + lane < n) store8<T>(ov + int64_t(i) * kWords, x);
     }
   }
 }
@@ -140,6 +142,9 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   }
   a.pages = c.pages; a.heads = c.heads; a.page_size = c.page_size;
   a.row = coded ? c.head_dim / 8 : row / 16;
+  a.unit_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.row == 1 << s) a.unit_shift = s;
   a.table = p->table; a.lengths = p->lengths; a.offsets = p->offsets; a.starts = p->starts;
   a.rows = p->rows; a.width = p->width;
   a.out_k = static_cast<uint4*>(p->out_k); a.out_v = static_cast<uint4*>(p->out_v);

@@ -52,6 +52,7 @@ struct AppendArgs {
   int64_t tokens;
   int tokens_per_warp;
   StepPages steps;
+  int unit_shift;           // log2 of the units of 8 elements of a head's row, or -1
 };
 
 struct RowPlan {
@@ -89,28 +90,38 @@ __device__ __forceinline__ void free_bounds(const int* range, int pages, int* be
 template <int kBits, typename T>
 __device__ __forceinline__ void quantize_token(const AppendArgs& a, int64_t t, int page, int slot) {
   constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
-  const int lane = threadIdx.x & 31, u = lane & 3;
-  const int units = a.steps.groups * 4, n = a.p.heads * units;      // of 8 elements: of a head's row, of the token
+  const int lane = threadIdx.x & 31, u = lane & 3, groups = a.steps.groups;
+  const int units = groups * 4, n = a.p.heads * units;      // of 8 elements: of a head's row, of the token
   uint8_t* kd = reinterpret_cast<uint8_t*>(a.p.k + page * a.p.ks[0] + slot * a.p.ks[2]);
   uint8_t* vd = reinterpret_cast<uint8_t*>(a.p.v + page * a.p.vs[0] + slot * a.p.vs[2]);
   uint16_t* kt = a.steps.k + page * a.steps.ks[0] + slot * a.steps.ks[2];
   uint16_t* vt = a.steps.v + page * a.steps.vs[0] + slot * a.steps.vs[2];
   const uint4* kx = a.k + t * a.ks[0];
   const uint4* vx = a.v + t * a.vs[0];
-  // (whole warps go round together: a group's lanes exchange their maxima)
-  for (int w0 = 0; w0 < n; w0 += 32) {
-    const int w = min(w0 + lane, n - 4 + u), h = w / units, c = w - h * units;      // (n is a multiple of 4)
-    uint4 kw[kWords], vw[kWords];
+  const int tail = groups % 2 == 0 ? 8 : 4;      // lanes that put their codes together; n is a multiple
+  // (whole warps go round together; lanes behind the end repeat its last group's work and store nothing)
+  auto place = [&](int w0) { return min(w0 + lane, n - tail + (lane & (tail - 1))); };
+  auto load = [&](int w, uint4 (&kw)[kWords], uint4 (&vw)[kWords]) {
+    const int h = a.unit_shift >= 0 ? w >> a.unit_shift : w / units, c = w - h * units;
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
       kw[i] = __ldg(kx + h * a.ks[1] + c * kWords + i);
       vw[i] = __ldg(vx + h * a.vs[1] + c * kWords + i);
     }
+  };
+  uint4 kn[kWords], vn[kWords];
+  load(place(0), kn, vn);
+  for (int w0 = 0; w0 < n; w0 += 32) {
+    uint4 kw[kWords], vw[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) { kw[i] = kn[i]; vw[i] = vn[i]; }
+    if (w0 + 32 < n) load(place(w0 + 32), kn, vn);
+    const int w = place(w0), h = a.unit_shift >= 0 ? w >> a.unit_shift : w / units, c = w - h * units;
+    const bool in = w0 + lane < n;
     const Quantized<kBits> k = quantize<kBits, T>(kw), v = quantize<kBits, T>(vw);
-    if (w0 + lane >= n) continue;
-    store_codes(kd + h * a.p.ks[1] * 16, a.steps.groups, c >> 2, u, k);
-    store_codes(vd + h * a.p.vs[1] * 16, a.steps.groups, c >> 2, u, v);
-    if (u == 0) {
+    store_codes(kd + h * a.p.ks[1] * 16, groups, c >> 2, u, k, in);
+    store_codes(vd + h * a.p.vs[1] * 16, groups, c >> 2, u, v, in);
+    if (in && u == 0) {
       kt[h * a.steps.ks[1] + (c >> 2)] = k.step;
       vt[h * a.steps.vs[1] + (c >> 2)] = v.step;
     }
@@ -603,6 +614,9 @@ int append(const nb200_cache_params* p, const nb200_cache_steps* steps, const ch
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   a.steps = step_pages(p->pages, steps);
+  a.unit_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.steps.groups * 4 == 1 << s) a.unit_shift = s;
   void (*kernel)(AppendArgs) = cache_append_kernel<0, uint4>;
   if (steps) {
     const bool four = steps->bits == 4;

@@ -38,7 +38,8 @@ struct RmsArgs {
   float* part;      // [CTA][C]: partial sums of dw
   int64_t rows;
   int C;
-  int group;        // channels of a scale
+  int group;        // channels of a scale; its power of two, where rows have several
+  int group_shift;
   float eps, inv_c;
 };
 
@@ -161,8 +162,10 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float2 (&y)[kPairs
 constexpr float kLeast = 7.888609052210118e-31f;      // 2^-100
 template <int kPairs>
 __device__ __forceinline__ float top_of(const float2 (&y)[kPairs], float top) {
+  // (abs without a flush of small numbers, which is an operand's modifier; fabsf is an instruction here)
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) top = max_nan(max_nan(top, fabsf(y[i].x)), fabsf(y[i].y));
+  for (int i = 0; i < kPairs; ++i)
+    asm("{\n.reg .f32 a, b;\nabs.f32 a, %1;\nabs.f32 b, %2;\nmax.NaN.f32 a, a, b;\nmax.NaN.f32 %0, %0, a;\n}" : "+f"(top) : "f"(y[i].x), "f"(y[i].y));
   return top;
 }
 // The scale for a largest magnitude, and what the values are multiplied by (the reciprocal of a number of 2^-109 or more, good to 2^-23).
@@ -173,10 +176,12 @@ __device__ __forceinline__ float inverse_of(float scale) {
   return r;
 }
 // The same of a group of lanes' values; its first lane writes the scale.
-__device__ __forceinline__ float group_scale(float top, int lanes, float* scale) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+__device__ __forceinline__ float group_scale(float top, int lanes, float* scale, bool write) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float s = scale_of(top);
-  if ((threadIdx.x & (lanes - 1)) == 0 && scale) *scale = s;
+  if (write && (threadIdx.x & (lanes - 1)) == 0) *scale = s;
   return inverse_of(s);
 }
 
@@ -259,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
       const bool in = in_rows && column(p) < a.C;
       if constexpr (kEight) {
         if (a.group != a.C)
-          inv = group_scale(top_of(f, kLeast), a.group / kVec, in ? a.scales + row * (a.C / a.group) + column(p) / a.group : nullptr);
+          inv = group_scale(top_of(f, kLeast), a.group / kVec, a.scales + ((base + column(p)) >> a.group_shift), in);
         if (in) store_codes<kVec>(static_cast<uint8_t*>(a.y) + base + column(p), f, inv);
       } else {
         if (in) C::of(f).store(static_cast<T*>(a.y) + base + column(p));
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
     if (in) output(c, f);
     if constexpr (kEight) {
       if (a.group != a.C)
-        inv = group_scale(top_of(f, kLeast), a.group / kVec, in ? a.scales + row * (a.C / a.group) + c / a.group : nullptr);
+        inv = group_scale(top_of(f, kLeast), a.group / kVec, a.scales + ((base + c) >> a.group_shift), in);
       if (in) store_codes<kVec>(static_cast<uint8_t*>(a.y) + base + c, f, inv);
     } else {
       if (in) C::of(f).store(static_cast<T*>(a.y) + base + c);
@@ -723,6 +728,7 @@ extern "C" NB200_API int nb200_rms_norm_fwd(const nb200_rms_norm_params* p, void
   a.x = p->x; a.r = p->residual; a.w = p->weight; a.y = p->y; a.sum = p->sum; a.rstd = p->rstd; a.scales = p->scales;
   a.rows = p->rows; a.C = p->channels;
   a.group = p->group ? p->group : p->channels;
+  a.group_shift = p->group == 32 ? 5 : p->group == 64 ? 6 : 7;
   a.eps = p->eps;
   a.inv_c = float(1.0 / p->channels);
   const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec, false);
