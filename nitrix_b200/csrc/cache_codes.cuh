@@ -80,65 +80,69 @@ __device__ __forceinline__ Quantized<kBits> quantize(const uint4 (&words)[sizeof
   return q;
 }
 
-// The codes of elements 8 u .. 8 u + 7 of a group are parts 2 u and 2 u + 1 of the row.  In 4 bits with an even number of groups the
-// lane four further has the same parts of the group beside: the two put their codes together to 32-bit words, a part each.  All lanes
-// of the warp call it; those without `in` store nothing.
+// The codes of elements 8 u .. 8 u + 7 of a group are in parts 2 u and 2 u + 1 of the row.
 template <int kBits>
-__device__ __forceinline__ void store_codes(uint8_t* row, int groups, int group, int u, const Quantized<kBits>& q, bool in) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int groups, int group, int u, const Quantized<kBits>& q) {
   if constexpr (kBits == 4) {
-    if (groups % 2 == 0) {
-      const uint32_t beside = __shfl_xor_sync(0xffffffffu, q.lo, 4);
-      const bool odd = group & 1;
-      if (in) reinterpret_cast<uint32_t*>(row)[((2 * u + odd) * groups + group) >> 1] = odd ? __byte_perm(beside, q.lo, 0x7632) : __byte_perm(q.lo, beside, 0x5410);
-    } else if (in) {
-      uint16_t* p = reinterpret_cast<uint16_t*>(row) + 2 * u * groups + group;
-      p[0] = uint16_t(q.lo);
-      p[groups] = uint16_t(q.lo >> 16);
-    }
-  } else if (in) {
+    uint16_t* p = reinterpret_cast<uint16_t*>(row) + 2 * u * groups + group;
+    p[0] = uint16_t(q.lo);
+    p[groups] = uint16_t(q.lo >> 16);
+  } else {
     uint32_t* p = reinterpret_cast<uint32_t*>(row) + 2 * u * groups + group;
     p[0] = q.lo;
     p[groups] = q.hi;
   }
 }
-// The other way: the words that a lane reads (two in 8 bits), then the values of its 8 elements.
-template <int kBits>
-__device__ __forceinline__ uint2 load_words(const uint8_t* row, int groups, int group, int u) {
-  if constexpr (kBits == 4) {
-    if (groups % 2 == 0) return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(row) + (((2 * u + (group & 1)) * groups + group) >> 1)), 0u);
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + 2 * u * groups + group;
-    return make_uint2(__ldg(p) | uint32_t(__ldg(p + groups)) << 16, 0u);
-  } else {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + 2 * u * groups + group;
-    return make_uint2(__ldg(p), __ldg(p + groups));
-  }
+// Those of all groups at once lie side by side, kGroups kBits / 4 words.
+template <int n, typename P>
+__device__ __forceinline__ void store_words(P* to, const uint32_t (&w)[n]) {
+  if constexpr (n == 1) *reinterpret_cast<uint32_t*>(to) = w[0];
+  else if constexpr (n == 2) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < n / 4; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
 }
-template <int kBits>
-__device__ __forceinline__ void values_of(uint2 w, int groups, int group, float step, float2 (&x)[4]) {
-  if constexpr (kBits == 4) {
-    if (groups % 2 == 0) {
-      const uint32_t beside = __shfl_xor_sync(0xffffffffu, w.x, 4);
-      w.x = group & 1 ? __byte_perm(beside, w.x, 0x7632) : __byte_perm(w.x, beside, 0x5410);
+template <int n, typename P>
+__device__ __forceinline__ void load_words(uint32_t (&w)[n], const P* from) {
+  if constexpr (n == 1) {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+  } else if constexpr (n == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(from));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < n / 4; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(from) + i);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
     }
   }
+}
+template <int kBits, int kGroups>
+__device__ __forceinline__ void store_quarter(uint8_t* row, int u, const Quantized<kBits> (&q)[kGroups]) {
+  constexpr int n = kGroups * kBits / 4;
+  uint32_t w[n];
+#pragma unroll
+  for (int i = 0; i < n / 2; ++i) {
+    w[i] = kBits == 4 ? __byte_perm(q[(2 * i) % kGroups].lo, q[(2 * i + 1) % kGroups].lo, 0x5410) : q[i % kGroups].lo;
+    w[n / 2 + i] = kBits == 4 ? __byte_perm(q[(2 * i) % kGroups].lo, q[(2 * i + 1) % kGroups].lo, 0x7632) : q[i % kGroups].hi;
+  }
+  store_words(row + u * n * 4, w);
+}
+// Values of 8 elements, from the words of their codes (one in 4 bits).
+template <int kBits>
+__device__ __forceinline__ void values_of(uint32_t lo, uint32_t hi, float step, float2 (&x)[4]) {
   // A code in the bits from p on of 2^23 is 2^23 + 2^p code: the half of the range and 2^23 come off exactly, the step takes 2^-p.
   constexpr int kEach = 16 / kBits;      // codes of 16 bits
+  constexpr float kHalf = float(1 << (kBits - 1));
 #pragma unroll
   for (int h = 0; h < 8 / kEach; ++h) {
-    const uint32_t part = kBits == 4 ? (h ? w.x >> 16 : w.x) : (h & 1 ? (h & 2 ? w.y : w.x) >> 16 : (h & 2 ? w.y : w.x));
+    const uint32_t word = kBits == 8 && h >= 2 ? hi : lo, part = h & 1 ? word >> 16 : word;
 #pragma unroll
     for (int i = 0; i < kEach; i += 2) {
-      float2 c;
-      float* e = &c.x;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int p = (i + j) * kBits;
-        e[j] = __uint_as_float(0x4b000000u | (part & (((1u << kBits) - 1u) << p)));
-      }
       const float p0 = float(1u << (i * kBits)), p1 = float(1u << ((i + 1) * kBits));
-      constexpr float kHalf = float(1 << (kBits - 1));
-      c = __fadd2_rn(c, make_float2(-8388608.f - kHalf * p0, -8388608.f - kHalf * p1));
-      x[(h * kEach + i) / 2] = __fmul2_rn(c, make_float2(step / p0, step / p1));
+      const uint32_t mask = (1u << kBits) - 1u;
+      const float2 c = make_float2(__uint_as_float(0x4b000000u | (part & mask << (i * kBits))), __uint_as_float(0x4b000000u | (part & mask << ((i + 1) * kBits))));
+      x[(h * kEach + i) / 2] = __fmul2_rn(__fadd2_rn(c, make_float2(-8388608.f - kHalf * p0, -8388608.f - kHalf * p1)), make_float2(step * (1.f / p0), step * (1.f / p1)));
     }
   }
 }

@@ -2,7 +2,7 @@
 //
 // Bound by HBM: codes and steps (or elements) read once, the rows written once.  A warp takes a token at a time: its sequence by
 // bisection of the offsets, its page from the table; then a lane eight elements at a time, which are two parts of a row of codes
-// and one or two 16-byte words of the result.
+// and one or two 16-byte words of the result, of each group of a row of 64 or 128, whose codes lie side by side.
 #include <type_traits>
 
 #include "cache_codes.cuh"
@@ -22,7 +22,6 @@ struct ReadArgs {
   int64_t kss[3], vss[3];          // elements
   int pages, heads, page_size;
   int row;                         // units of a head's row: of 8 elements, or 16-byte words
-  int unit_shift;                  // log2 of row, or -1
   const int* table;
   const int* lengths;
   int rows, width;
@@ -41,6 +40,57 @@ __device__ __forceinline__ void store8(uint4* p, const float2 (&x)[4]) {
   } else {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     p[0] = make_uint4(tc::pack2<kBf16>(x[0].x, x[0].y), tc::pack2<kBf16>(x[1].x, x[1].y), tc::pack2<kBf16>(x[2].x, x[2].y), tc::pack2<kBf16>(x[3].x, x[3].y));
+  }
+}
+
+struct TokenRows {
+  const uint8_t* codes[2];
+  const uint16_t* steps[2];
+  int64_t codes_head[2], steps_head[2];      // from one head to the next
+  uint4* to[2];
+};
+
+// A token's values, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of them, whose codes lie side by
+// side; otherwise, for any number of groups, 8 elements.
+template <int kBits, typename T, int kGroups>
+__device__ __forceinline__ void read_token(const ReadArgs& a, const TokenRows& at) {
+  constexpr int kWords = int(sizeof(T)) / 2, kEach = kGroups ? kGroups : 1;
+  const int units = kGroups ? 4 : a.row, n = a.heads * units;
+  for (int w = threadIdx.x & 31; w < n; w += 32) {
+    const int h = w / units, c = w - h * units;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const uint8_t* row = at.codes[which] + h * at.codes_head[which];
+      const uint16_t* steps = at.steps[which] + h * at.steps_head[which];
+      uint4* to = at.to[which] + (int64_t(h) * a.row + c) * kWords;
+      float2 x[4];
+      if constexpr (kGroups > 0) {
+        constexpr int n = kGroups * kBits / 4;
+        uint32_t codes[n], s[kGroups / 2];
+        load_words(codes, row + c * n * 4);
+        load_words(s, steps);
+#pragma unroll
+        for (int g = 0; g < kEach; ++g) {
+          const float step = __half2float(__ushort_as_half(uint16_t(g % 2 ? s[g / 2] >> 16 : s[g / 2])));
+          if constexpr (kBits == 4) values_of<4>(__byte_perm(codes[g / 2], codes[n / 2 + g / 2], g % 2 ? 0x7632 : 0x5410), 0u, step, x);
+          else values_of<8>(codes[g], codes[n / 2 + g], step, x);
+          store8<T>(to + g * 4 * kWords, x);
+        }
+      } else {
+        const int groups = a.row / 4, g = c >> 2, u = c & 3;
+        uint32_t lo, hi = 0;
+        if constexpr (kBits == 4) {
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + 2 * u * groups + g;
+          lo = __ldg(p) | uint32_t(__ldg(p + groups)) << 16;
+        } else {
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + 2 * u * groups + g;
+          lo = __ldg(p);
+          hi = __ldg(p + groups);
+        }
+        values_of<kBits>(lo, hi, __half2float(__ushort_as_half(__ldg(steps + g))), x);
+        store8<T>(to, x);
+      }
+    }
   }
 }
 
@@ -85,23 +135,11 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
       ov[i] = vw;
     }
   } else {
-    const int groups = a.row / 4;
-    const uint16_t* kt = a.k_steps + page * a.kss[0] + slot * a.kss[2];
-    const uint16_t* vt = a.v_steps + page * a.vss[0] + slot * a.vss[2];
-    const int tail = groups % 2 == 0 ? 8 : 4;      // lanes that exchange words; n is a multiple
-    // (whole warps go round together; lanes behind the end repeat its last group's work and store nothing)
-#pragma unroll 2
-    for (int w0 = 0; w0 < n; w0 += 32) {
-      const int i = min(w0 + lane, n - tail + (lane & (tail - 1)));
-      const int h = a.unit_shift >= 0 ? i >> a.unit_shift : i / a.row, c = i - h * a.row, group = c >> 2, u = c & 3;
-      const uint2 kw = load_words<kBits>(kp + h * a.ks[1], groups, group, u), vw = load_words<kBits>(vp + h * a.vs[1], groups, group, u);
-      const float k_step = __half2float(__ushort_as_half(__ldg(kt + h * a.kss[1] + group))), v_step = __half2float(__ushort_as_half(__ldg(vt + h * a.vss[1] + group)));
-      float2 x[4];
-      values_of<kBits>(kw, groups, group, k_step, x);
-      if (w0 + lane < n) store8<T>(ok + int64_t(i) * kWords, x);
-      values_of<kBits>(vw, groups, group, v_step, x);
-      if (w0 + lane < n) store8<T>(ov + int64_t(i) * kWords, x);
-    }
+    const TokenRows at{{kp, vp}, {a.k_steps + page * a.kss[0] + slot * a.kss[2], a.v_steps + page * a.vss[0] + slot * a.vss[2]},
+                       {a.ks[1], a.vs[1]}, {a.kss[1], a.vss[1]}, {ok, ov}};
+    if (a.row == 16) read_token<kBits, T, 4>(a, at);
+    else if (a.row == 8) read_token<kBits, T, 2>(a, at);
+    else read_token<kBits, T, 0>(a, at);
   }
 }
 
@@ -142,9 +180,6 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   }
   a.pages = c.pages; a.heads = c.heads; a.page_size = c.page_size;
   a.row = coded ? c.head_dim / 8 : row / 16;
-  a.unit_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if (a.row == 1 << s) a.unit_shift = s;
   a.table = p->table; a.lengths = p->lengths; a.offsets = p->offsets; a.starts = p->starts;
   a.rows = p->rows; a.width = p->width;
   a.out_k = static_cast<uint4*>(p->out_k); a.out_v = static_cast<uint4*>(p->out_v);

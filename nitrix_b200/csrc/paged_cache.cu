@@ -12,6 +12,7 @@
 // a fork of 64 rows 10.5 in a captured graph, 15 and 21 where the host makes the calls.
 #include "cache_codes.cuh"
 #include "dependent_launch.cuh"
+#include "sm100_primitives.cuh"
 
 namespace nb200 {
 namespace {
@@ -52,7 +53,6 @@ struct AppendArgs {
   int64_t tokens;
   int tokens_per_warp;
   StepPages steps;
-  int unit_shift;           // log2 of the units of 8 elements of a head's row, or -1
 };
 
 struct RowPlan {
@@ -86,46 +86,69 @@ __device__ __forceinline__ void free_bounds(const int* range, int pages, int* be
   *end = min(max(range[1], *begin), pages);
 }
 
-// Quantises token `t` into slot `slot` of `page`, by a warp.  A lane takes 8 elements, four lanes a group.
-template <int kBits, typename T>
-__device__ __forceinline__ void quantize_token(const AppendArgs& a, int64_t t, int page, int slot) {
-  constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
-  const int lane = threadIdx.x & 31, u = lane & 3, groups = a.steps.groups;
-  const int units = groups * 4, n = a.p.heads * units;      // of 8 elements: of a head's row, of the token
-  uint8_t* kd = reinterpret_cast<uint8_t*>(a.p.k + page * a.p.ks[0] + slot * a.p.ks[2]);
-  uint8_t* vd = reinterpret_cast<uint8_t*>(a.p.v + page * a.p.vs[0] + slot * a.p.vs[2]);
-  uint16_t* kt = a.steps.k + page * a.steps.ks[0] + slot * a.steps.ks[2];
-  uint16_t* vt = a.steps.v + page * a.steps.vs[0] + slot * a.steps.vs[2];
-  const uint4* kx = a.k + t * a.ks[0];
-  const uint4* vx = a.v + t * a.vs[0];
-  const int tail = groups % 2 == 0 ? 8 : 4;      // lanes that put their codes together; n is a multiple
-  // (whole warps go round together; lanes behind the end repeat its last group's work and store nothing)
-  auto place = [&](int w0) { return min(w0 + lane, n - tail + (lane & (tail - 1))); };
-  auto load = [&](int w, uint4 (&kw)[kWords], uint4 (&vw)[kWords]) {
-    const int h = a.unit_shift >= 0 ? w >> a.unit_shift : w / units, c = w - h * units;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      kw[i] = __ldg(kx + h * a.ks[1] + c * kWords + i);
-      vw[i] = __ldg(vx + h * a.vs[1] + c * kWords + i);
-    }
-  };
-  uint4 kn[kWords], vn[kWords];
-  load(place(0), kn, vn);
+// Where a token's codes and steps go, and where it comes from.
+struct TokenPlace {
+  uint8_t* codes[2];
+  uint16_t* steps[2];
+  const uint4* from[2];
+  int64_t codes_head[2], steps_head[2], from_head[2];      // from one head to the next
+};
+__device__ __forceinline__ TokenPlace place_of(const AppendArgs& a, int64_t t, int page, int slot) {
+  return TokenPlace{{reinterpret_cast<uint8_t*>(a.p.k + page * a.p.ks[0] + slot * a.p.ks[2]), reinterpret_cast<uint8_t*>(a.p.v + page * a.p.vs[0] + slot * a.p.vs[2])},
+                    {a.steps.k + page * a.steps.ks[0] + slot * a.steps.ks[2], a.steps.v + page * a.steps.vs[0] + slot * a.steps.vs[2]},
+                    {a.k + t * a.ks[0], a.v + t * a.vs[0]},
+                    {a.p.ks[1] * 16, a.p.vs[1] * 16},
+                    {a.steps.ks[1], a.steps.vs[1]},
+                    {a.ks[1], a.vs[1]}};
+}
+
+// Quantises a token's row into a slot of a page, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of
+// them, so that its codes lie side by side; otherwise, for any number of groups, 8 elements.  Four lanes share a group's elements.
+template <int kBits, typename T, int kGroups>
+__device__ __forceinline__ void quantize_token(const AppendArgs& a, const TokenPlace& at) {
+  constexpr int kWords = sizeof(T) == 4 ? 2 : 1, kEach = kGroups ? kGroups : 1;
+  const int lane = threadIdx.x & 31, u = lane & 3;
+  const int units = kGroups ? 4 : a.steps.groups * 4, n = a.p.heads * units;
+  // (whole warps go round together: a group's lanes exchange their maxima)
   for (int w0 = 0; w0 < n; w0 += 32) {
-    uint4 kw[kWords], vw[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) { kw[i] = kn[i]; vw[i] = vn[i]; }
-    if (w0 + 32 < n) load(place(w0 + 32), kn, vn);
-    const int w = place(w0), h = a.unit_shift >= 0 ? w >> a.unit_shift : w / units, c = w - h * units;
+    const int w = min(w0 + lane, n - 4 + u), h = w / units, c = w - h * units;      // (n is a multiple of 4)
     const bool in = w0 + lane < n;
-    const Quantized<kBits> k = quantize<kBits, T>(kw), v = quantize<kBits, T>(vw);
-    store_codes(kd + h * a.p.ks[1] * 16, groups, c >> 2, u, k, in);
-    store_codes(vd + h * a.p.vs[1] * 16, groups, c >> 2, u, v, in);
-    if (in && u == 0) {
-      kt[h * a.steps.ks[1] + (c >> 2)] = k.step;
-      vt[h * a.steps.vs[1] + (c >> 2)] = v.step;
+    uint4 x[2][kEach][kWords];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int g = 0; g < kEach; ++g)
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) x[which][g][i] = sm100::ldg_no_allocate(at.from[which] + h * at.from_head[which] + (g * 4 + c) * kWords + i);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      Quantized<kBits> q[kEach];
+#pragma unroll
+      for (int g = 0; g < kEach; ++g) q[g] = quantize<kBits, T>(x[which][g]);
+      if (!in) continue;
+      uint8_t* codes = at.codes[which] + h * at.codes_head[which];
+      uint16_t* steps = at.steps[which] + h * at.steps_head[which];
+      if constexpr (kGroups > 0) {
+        store_quarter<kBits, kGroups>(codes, u, q);
+        if (u == 0) {
+          uint32_t s[kGroups / 2];
+#pragma unroll
+          for (int i = 0; i < kGroups / 2; ++i) s[i] = q[2 * i].step | uint32_t(q[2 * i + 1].step) << 16;
+          store_words(steps, s);
+        }
+      } else {
+        store_codes(codes, a.steps.groups, c >> 2, u, q[0]);
+        if (u == 0) steps[c >> 2] = q[0].step;
+      }
     }
   }
+}
+template <int kBits, typename T>
+__device__ __forceinline__ void quantize_token(const AppendArgs& a, int64_t t, int page, int slot) {
+  const TokenPlace at = place_of(a, t, page, slot);
+  if (a.steps.groups == 4) quantize_token<kBits, T, 4>(a, at);
+  else if (a.steps.groups == 2) quantize_token<kBits, T, 2>(a, at);
+  else quantize_token<kBits, T, 0>(a, at);
 }
 
 // kBits 0: the tokens' rows are copied; otherwise T is their type.
@@ -614,9 +637,6 @@ int append(const nb200_cache_params* p, const nb200_cache_steps* steps, const ch
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   a.steps = step_pages(p->pages, steps);
-  a.unit_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if (a.steps.groups * 4 == 1 << s) a.unit_shift = s;
   void (*kernel)(AppendArgs) = cache_append_kernel<0, uint4>;
   if (steps) {
     const bool four = steps->bits == 4;
