@@ -60,19 +60,29 @@ __device__ __forceinline__ Quantized<kBits> quantize(const uint4 (&words)[sizeof
   const float a = high >= -low ? high : low;
   const __half step = __float2half_rn(fminf(fmaxf(a * (-1.f / kHalf), -65504.f), 65504.f));
   const float s = __half2float(step);
-  const float inverse = s != 0.f ? __frcp_rn(s) : 0.f;
+  // (1 / s rounded to nearest: an approximation good to one unit and one step of Newton's method give that for every fp16 number)
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  const float inverse = s != 0.f ? __fmaf_rn(r, __fmaf_rn(-s, r, 1.f), r) : 0.f;
   Quantized<kBits> q;
   q.step = finite ? __half_as_ushort(step) : uint16_t(0x7fff);
   // Adding M = 1.5 2^23 + half rounds to whole numbers, halves to even, and leaves the code in the lowest bits of a number whose
   // others are known: codes are put side by side by adding these numbers up, shifted, and taking the known bits off at the end.
   constexpr float kM = 12582912.f + kHalf;
   constexpr uint32_t kBase = 0x4b400000u, kKnown = kBits == 4 ? kBase * 0x11111111u : kBase * 0x01010101u;
+  // A quotient is at most half (1 + 2^-11) in size, so that only the far end has to be cut, unless the step has been cut itself or has
+  // lost bits as one of fp16's smallest numbers.
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = fminf(__fmul_rn(x[i], inverse), kHalf - 1.f);
+  const float size = fabsf(s);
+  if (__any_sync(0xffffffffu, size < 6.103515625e-05f || size >= 65504.f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = fmaxf(z[i], float(-kHalf));
+  }
   uint32_t w[8 * kBits / 32] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float z = fminf(fmaxf(__fmul_rn(x[i], inverse), float(-kHalf)), kHalf - 1.f);
-    w[i * kBits / 32] += __float_as_uint(__fadd_rn(z, kM)) << (i * kBits % 32);
-  }
+  for (int i = 0; i < 8; ++i) w[i * kBits / 32] += __float_as_uint(__fadd_rn(z[i], kM)) << (i * kBits % 32);
   // (what is not finite, and a step of zero, has the codes of zero: z is zero in the second case)
   constexpr uint32_t kZero = kBits == 4 ? 0x88888888u : 0x80808080u;
   q.lo = finite ? w[0] - kKnown : kZero;

@@ -30,6 +30,7 @@ struct ReadArgs {
   uint4* out_k;
   uint4* out_v;
   int64_t tokens;
+  int tokens_per_warp;
 };
 
 template <typename T>
@@ -58,66 +59,72 @@ __device__ __forceinline__ void read_token(const ReadArgs& a, const TokenRows& a
   const int units = kGroups ? 4 : a.row, n = a.heads * units;
   for (int w = threadIdx.x & 31; w < n; w += 32) {
     const int h = w / units, c = w - h * units;
+    const uint8_t* rows[2] = {at.codes[0] + h * at.codes_head[0], at.codes[1] + h * at.codes_head[1]};
+    const uint16_t* steps[2] = {at.steps[0] + h * at.steps_head[0], at.steps[1] + h * at.steps_head[1]};
+    const int64_t to = (int64_t(h) * a.row + c) * kWords;
+    float2 x[4];
+    if constexpr (kGroups > 0) {
+      constexpr int nw = kGroups * kBits / 4;
+      uint32_t codes[2][nw], s[2][kGroups / 2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint8_t* row = at.codes[which] + h * at.codes_head[which];
-      const uint16_t* steps = at.steps[which] + h * at.steps_head[which];
-      uint4* to = at.to[which] + (int64_t(h) * a.row + c) * kWords;
-      float2 x[4];
-      if constexpr (kGroups > 0) {
-        constexpr int n = kGroups * kBits / 4;
-        uint32_t codes[n], s[kGroups / 2];
-        load_words(codes, row + c * n * 4);
-        load_words(s, steps);
+      for (int which = 0; which < 2; ++which) {
+        load_words(codes[which], rows[which] + c * nw * 4);
+        load_words(s[which], steps[which]);
+      }
+#pragma unroll
+      for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int g = 0; g < kEach; ++g) {
-          const float step = __half2float(__ushort_as_half(uint16_t(g % 2 ? s[g / 2] >> 16 : s[g / 2])));
-          if constexpr (kBits == 4) values_of<4>(__byte_perm(codes[g / 2], codes[n / 2 + g / 2], g % 2 ? 0x7632 : 0x5410), 0u, step, x);
-          else values_of<8>(codes[g], codes[n / 2 + g], step, x);
-          store8<T>(to + g * 4 * kWords, x);
+          const float step = __half2float(__ushort_as_half(uint16_t(g % 2 ? s[which][g / 2] >> 16 : s[which][g / 2])));
+          if constexpr (kBits == 4) values_of<4>(__byte_perm(codes[which][g / 2], codes[which][nw / 2 + g / 2], g % 2 ? 0x7632 : 0x5410), 0u, step, x);
+          else values_of<8>(codes[which][g], codes[which][nw / 2 + g], step, x);
+          store8<T>(at.to[which] + to + g * 4 * kWords, x);
         }
-      } else {
-        const int groups = a.row / 4, g = c >> 2, u = c & 3;
+    } else {
+      const int groups = a.row / 4, g = c >> 2, u = c & 3;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
         uint32_t lo, hi = 0;
         if constexpr (kBits == 4) {
-          const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + 2 * u * groups + g;
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(rows[which]) + 2 * u * groups + g;
           lo = __ldg(p) | uint32_t(__ldg(p + groups)) << 16;
         } else {
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + 2 * u * groups + g;
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(rows[which]) + 2 * u * groups + g;
           lo = __ldg(p);
           hi = __ldg(p + groups);
         }
-        values_of<kBits>(lo, hi, __half2float(__ushort_as_half(__ldg(steps + g))), x);
-        store8<T>(to, x);
+        values_of<kBits>(lo, hi, __half2float(__ushort_as_half(__ldg(steps[which] + g))), x);
+        store8<T>(at.to[which] + to, x);
       }
     }
   }
 }
 
-// kBits 0: words are copied; otherwise T is the type of the result.
-template <int kBits, typename T>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) {
-  constexpr int kWords = kBits == 0 ? 1 : int(sizeof(T)) / 2;      // 16-byte words of a unit of the result
-  const int lane = threadIdx.x & 31;
-  const int64_t t = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  if (t >= a.tokens) return;
-  // the first sequence that ends behind t
-  int lo = 0, hi = a.rows;
+// The first sequence of lo .. hi that ends behind token t.
+__device__ __forceinline__ int row_of(const ReadArgs& a, int64_t t, int lo, int hi) {
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (int64_t(__ldg(a.offsets + mid + 1)) <= t) lo = mid + 1;
     else hi = mid;
   }
-  int page = -1, slot = 0;
-  if (lo < a.rows) {
-    const int64_t first = __ldg(a.offsets + lo), at = t - first + (a.starts ? __ldg(a.starts + lo) : 0);
-    const int64_t held = min(int64_t(min(__ldg(a.lengths + lo), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.page_size);
-    if (t >= first && at >= 0 && at < held) {
-      const int column = int(at / a.page_size);
-      slot = int(at - int64_t(column) * a.page_size);
-      page = __ldg(a.table + int64_t(lo) * a.width + column);
-    }
-  }
+  return lo;
+}
+struct Slot {
+  int page, slot;      // a page outside the pool: there is no such token
+};
+__device__ __forceinline__ Slot slot_of(const ReadArgs& a, int64_t t, int row) {
+  if (row >= a.rows) return Slot{-1, 0};
+  const int64_t first = __ldg(a.offsets + row), at = t - first + (a.starts ? __ldg(a.starts + row) : 0);
+  const int64_t held = min(int64_t(min(__ldg(a.lengths + row), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.page_size);
+  if (t < first || at < 0 || at >= held) return Slot{-1, 0};
+  const int column = int(at) / a.page_size;
+  return Slot{__ldg(a.table + int64_t(row) * a.width + column), int(at) - column * a.page_size};
+}
+
+// A token's rows from a slot of a page, or zeros.
+template <int kBits, typename T>
+__device__ __forceinline__ void read_slot(const ReadArgs& a, int64_t t, int page, int slot, int lane) {
+  constexpr int kWords = kBits == 0 ? 1 : int(sizeof(T)) / 2;
   const int n = a.heads * a.row;
   uint4* ok = a.out_k + t * n * kWords;
   uint4* ov = a.out_v + t * n * kWords;
@@ -140,6 +147,25 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
     if (a.row == 16) read_token<kBits, T, 4>(a, at);
     else if (a.row == 8) read_token<kBits, T, 2>(a, at);
     else read_token<kBits, T, 0>(a, at);
+  }
+}
+
+// kBits 0: words are copied; otherwise T is the type of the result.
+template <int kBits, typename T>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) {
+  const int lane = threadIdx.x & 31;
+  int64_t t = (int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * a.tokens_per_warp;
+  const int64_t t_end = min(t + a.tokens_per_warp, a.tokens);
+  if (t >= t_end) return;
+  int row = row_of(a, t, 0, a.rows);
+  Slot at = slot_of(a, t, row);
+  for (; t < t_end; ++t) {
+    const Slot here = at;
+    if (t + 1 < t_end) {      // (the next token's place is on its way while this one's rows are)
+      while (row < a.rows && int64_t(__ldg(a.offsets + row + 1)) <= t + 1) ++row;
+      at = slot_of(a, t + 1, row);
+    }
+    read_slot<kBits, T>(a, t, here.page, here.slot, lane);
   }
 }
 
@@ -193,7 +219,10 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   }
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  kernel<<<unsigned((p->tokens + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
+  // one token per warp while that does not fill the GPU's warps, then four, which share a search
+  a.tokens_per_warp = p->tokens < 148 * 64 ? 1 : 4;
+  const int64_t per_cta = int64_t(a.tokens_per_warp) * (kThreads / 32);
+  kernel<<<unsigned((p->tokens + per_cta - 1) / per_cta), kThreads, 0, st>>>(a);
   count_launch();
   return check_launch("cache_read_kernel");
 }

@@ -560,3 +560,24 @@ def test_refusals():
     for call in (lambda: decode_attention(dual(q), cache), lambda: cache_append(cache, dual(k), k, offsets), lambda: cache_read(cache._replace(k_steps=dual(cache.k_steps)), offsets, 3)):
         with pytest.raises(NotImplementedError, match="forward-mode"), torch.autograd.forward_ad.dual_level():
             call()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_every_step(bits):
+    """Codes under every fp16 step that there is, of values at, beside and far from the borders between two codes."""
+    from nitrix_b200.nn import cache_append
+
+    half = 1 << (bits - 1)
+    steps = torch.arange(1, 0x7c00, device="cuda").short().view(torch.float16).float()
+    steps = torch.cat([steps, -steps])
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ratio = torch.randint(-half, half, (steps.numel(), 32), generator=g, device="cuda").float() + 0.5
+    ratio[:, 16:] += torch.randn(steps.numel(), 16, generator=g, device="cuda") * 2.0 ** -20
+    x = (ratio * steps[:, None]).clamp(-half * steps.abs()[:, None], half * steps.abs()[:, None])
+    x[:, 0] = -half * steps      # (the largest, which makes the step)
+    x = x[:, None].contiguous()
+    cache = _cache(len(steps) // 64 + 2, 64, 1, 32, bits, 1, len(steps) // 64 + 2)
+    after = cache_append(cache, x, x, _ints([0, len(steps)]))
+    at = _at(after, 0, len(steps))
+    want, want_steps = O.quantize(x, bits)
+    assert torch.equal(after.k_steps[at], want_steps) and torch.equal(after.k_codes[at], O.packed_codes(want, bits))
