@@ -154,7 +154,7 @@ struct QuantizedMmaLoop {
   static constexpr int kHeads = 8 * kTiles;
   static constexpr int kBlock = 16, kTurn = 32;  // tokens
   static constexpr int kSlots = 1;
-  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 5 : kBits == 4 ? 4 : 3) : D == 64 ? 4 : 2;
+  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 4 : kBits == 4 ? 3 : 2) : D == 64 ? 3 : 2;
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
   static constexpr int kRow = D * kBits / 8;     // bytes of a row of codes
@@ -498,7 +498,7 @@ Plan plan(const nb200_decode_params* p, int bits) {
   int ctas = 2;      // resident per SM: the loops' kMinCtas
   if (pl.mma) {
     pl.heads = group > 8 ? 16 : 8;
-    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 5 : bits == 4 ? 4 : 3) : c.head_dim == 64 ? 4 : 2;
+    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 4 : bits == 4 ? 3 : 2) : c.head_dim == 64 ? 3 : 2;
   } else {
     pl.heads = c.head_dim > 128 ? 2 : 4;
   }
