@@ -5,14 +5,16 @@
 Training runs ``rotary_embedding`` and ``packed_attention`` over documents of unequal length that lie one after the other.
 Serving takes prompts in the same way, stores their keys and values with ``cache_append``, and generates a token per sequence and
 step with ``decode_attention``; in between beams are chosen anew (``cache_fork``), finished ones leave (``cache_free``) and the
-pool is packed (``cache_compact``).  No call of it waits for the GPU.
+pool is packed (``cache_compact``).  With ``bits`` the cache holds 4 or 8 bits a value.  Prompts may come in chunks: a chunk's keys
+and values go into the cache, and the whole of them comes back out of it (``cache_read``) for the chunk's queries.  No call of it
+waits for the GPU.
 """
 from __future__ import annotations
 
 import torch
 
-from nitrix_b200.nn import (cache_append, cache_compact, cache_fork, cache_free, decode_attention, packed_attention, paged_cache,
-                            rotary_embedding, rotary_frequencies)
+from nitrix_b200.nn import (cache_append, cache_compact, cache_fork, cache_free, cache_read, decode_attention, packed_attention,
+                            paged_cache, quantized_cache, rms_norm, rotary_embedding, rotary_frequencies)
 
 
 class AttentionLayer:
@@ -40,6 +42,21 @@ class AttentionLayer:
             cache = cache_append(cache, k, v, offsets)
         out = packed_attention(q, k, v, offsets).flatten(1) @ self.w_out.T
         return out if cache is None else (out, cache)
+
+    def chunk(self, x, positions, offsets, cache, tokens):
+        """The next tokens of prompts whose beginnings ``cache`` holds, at most ``tokens`` with them."""
+        q, k, v = self.project(x, positions)
+        cache = cache_append(cache, k, v, offsets)
+        held = torch.nn.functional.pad(cache.lengths.cumsum(0), (1, 0)).int()
+        keys, values = cache_read(cache, held, tokens, dtype=q.dtype)
+        out = packed_attention(q, keys, values, offsets, offsets_k=held)
+        return out.flatten(1) @ self.w_out.T, cache
+
+    def block(self, x, stream, gain, cache):
+        """One new token of every sequence through the norm in front of the layer: the layer's output, and the stream with ``x``."""
+        y, stream = rms_norm(x, gain, residual=stream)
+        out, cache = self.step(y, cache)
+        return out, stream, cache
 
     def step(self, x, cache):
         """One new token of every sequence, ``x`` (sequences, width)."""
@@ -74,13 +91,18 @@ def train(layer, lengths, steps=20, rate=8.0, seed=1):
 
 
 @torch.no_grad()
-def serve(layer, prompts, beams=2, steps=8):
+def serve(layer, prompts, beams=2, steps=8, bits=None):
     """Outputs of the prompts' last tokens and of every generated one, the cache, and the tokens that were fed (for a check).
 
-    ``prompts``: a (length, width) tensor each.  A generated token's output, normalised, is the next token."""
+    ``prompts``: a (length, width) tensor each.  A generated token's output, normalised, is the next token.  ``bits``: 4 or 8 for a
+    cache in few bits."""
     lengths = [p.shape[0] for p in prompts]
     offsets, positions = pack(lengths)
-    cache = paged_cache(256, 16, layer.kv_heads, layer.head_dim, sequences=len(prompts), max_length=512, dtype=prompts[0].dtype)
+    sizes = dict(sequences=len(prompts), max_length=512)
+    if bits is None:
+        cache = paged_cache(256, 16, layer.kv_heads, layer.head_dim, dtype=prompts[0].dtype, **sizes)
+    else:
+        cache = quantized_cache(256, 16, layer.kv_heads, layer.head_dim, bits=bits, **sizes)
     out, cache = layer.packed(torch.cat(prompts), positions, offsets, cache)
     last = out[offsets[1:].long() - 1]
     # every prompt is continued by several beams, which share its pages
@@ -105,4 +127,8 @@ if __name__ == "__main__":
     prompts = [torch.randn(n, 256, device="cuda").bfloat16() for n in (40, 7, 100)]
     outputs, _, packed, before = serve(layer, prompts)
     print("sequences", before.lengths.tolist(), "pages free", int(before.free_range[1] - before.free_range[0]))
+    for bits in (8, 4):
+        few, _, _, _ = serve(layer, prompts, bits=bits)
+        off = (few[-1].float() - outputs[-1].float()).norm() / outputs[-1].float().norm()
+        print(f"the last tokens from a cache of {bits} bits are {float(off):.3f} off")
     print("after three have finished", packed.lengths.tolist(), "pages free", int(packed.free_range[1] - packed.free_range[0]))

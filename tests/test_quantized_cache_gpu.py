@@ -120,15 +120,19 @@ def test_what_is_not_finite_or_beyond_the_steps(bits):
 
 @pytest.mark.parametrize("bits", [0, 4, 8])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_reading_parts_of_sequences(bits, dtype):
+@pytest.mark.parametrize("layout", ["heads", "tokens"])
+def test_reading_parts_of_sequences(bits, dtype, layout):
     """From a position on, past the end, before the start, rows of no sequence; of both kinds of cache."""
     from nitrix_b200.nn import cache_append, cache_read, paged_cache
 
     lengths = [40, 0, 7, 100, 1]
     if bits:
-        cache = _cache(40, 8, 2, 64, bits, 5, 20)
+        cache = _cache(40, 8, 2, 64, bits, 5, 20, layout)
     else:
         cache = paged_cache(40, 8, 2, 64, sequences=5, max_length=160, dtype=dtype)
+        if layout == "tokens":
+            cache = cache._replace(k_pages=torch.empty(40, 8, 2, 64, dtype=dtype, device="cuda").transpose(1, 2),
+                                   v_pages=torch.empty(40, 8, 2, 72, dtype=dtype, device="cuda")[..., :64].transpose(1, 2))
         cache.k_pages.fill_(float("nan")), cache.v_pages.fill_(float("nan"))
     k, v = (_values(148, 2, 64, dtype, seed=s) for s in (2, 3))
     offsets = _offsets(lengths)
@@ -581,3 +585,109 @@ def test_every_step(bits):
     at = _at(after, 0, len(steps))
     want, want_steps = O.quantize(x, bits)
     assert torch.equal(after.k_steps[at], want_steps) and torch.equal(after.k_codes[at], O.packed_codes(want, bits))
+
+
+def test_lengths_at_the_end_of_32_bits():
+    """A table of one page many times over: 2^31 tokens and more.  A sequence counts 2^31 - 256 of them at most."""
+    from nitrix_b200.nn import QuantizedCache, cache_append, cache_read, decode_attention
+
+    page, most = 1 << 16, 2 ** 31 - 256
+    table, z = torch.zeros(1, (1 << 15) + 4, dtype=torch.int32, device="cuda"), _ints([0])
+    for dtype, dim, bits in ((torch.bfloat16, 64, 4), (torch.float16, 128, 8), (torch.float32, 32, 8)):
+        codes = torch.full((1, 1, page, dim * bits // 8), 0x99 if bits == 4 else 0x81, dtype=torch.uint8, device="cuda")
+        steps = torch.zeros(1, 1, page, dim // 32, dtype=torch.float16, device="cuda")
+        for n in (2 ** 31 - 1, most, most - 63):
+            cache = QuantizedCache(codes, codes, steps, torch.full_like(steps, 3.0), table, _ints([n]), z, _ints([0, 0]), z)
+            out = decode_attention(torch.ones(1, 1, dim, dtype=dtype, device="cuda"), cache)
+            assert bool(((out - 3).abs() < 0.02).all()), (dtype, n)
+        got, _ = cache_read(cache._replace(k_steps=cache.v_steps, lengths=_ints([most])), _ints([0, 9]), 9, starts=_ints([most - 5]))
+        assert bool((got[:5] == 3).all()) and not bool(got[5:].any())
+    more = torch.zeros(4, 1, 32, dtype=torch.bfloat16, device="cuda")
+    after = cache_append(cache._replace(lengths=_ints([most - 3])), more, more, _ints([0, 4]))
+    assert after.lengths.tolist() == [most] and after.shortfall.tolist() == [1]
+
+
+def test_two_graphs_and_an_eager_call_with_one_cache():
+    """Workspaces belong to their calls: graphs replayed in any order, with eager calls between, give what each gave alone."""
+    from nitrix_b200.nn import decode_attention
+
+    lengths = [900, 40, 333]
+    cache = _filled(lengths, 16, 2, 128, 4)
+    q = [torch.randn(3, 8, 128, device="cuda").half() for _ in range(3)]
+    want = [decode_attention(x, cache) for x in q]
+    graphs = []
+    for x in q[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = decode_attention(x, cache)
+        graphs.append((graph, out))
+    for order in ((0, 1), (1, 0, 1), (0, 0)):
+        for i in order:
+            graphs[i][0].replay()
+            assert torch.equal(decode_attention(q[2], cache), want[2])
+        for i in set(order):
+            assert torch.equal(graphs[i][1], want[i])
+
+
+def test_forks_and_compactions_in_a_graph():
+    from nitrix_b200.nn import cache_compact, cache_fork
+
+    pair = Pair(64, 4, 6, 8, 2, 64, 4, "heads")
+    pair.append([9, 3, 0, 17, 30, 5])
+    held = type(pair.cache)(*pair.cache[:4], *(t.clone() for t in pair.cache[4:]))
+    parents = torch.arange(6, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache_compact(cache_fork(held, parents))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = cache_compact(cache_fork(held, parents))
+    rng = random.Random(5)
+    for _ in range(10):
+        for mine, theirs in zip(held[4:], pair.cache[4:]):
+            mine.copy_(theirs)
+        chosen = [rng.randint(-1, 5) for _ in range(6)]
+        parents.copy_(_ints(chosen))
+        graph.replay()
+        pair.cache = type(result)(*held[:4], *(t.clone() for t in result[4:]))
+        pair.model.fork(chosen)
+        pair.model.compact()
+        pair.check()
+        pair.append([rng.choice([0, 1, 3]) for _ in range(6)])
+        pair.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_large_groups(dtype, dim):
+    lengths = [100, 3, 700]
+    cache = _filled(lengths, 16, 1, dim, 4)
+    _check_decode(torch.randn(3, 130, dim, device="cuda").to(dtype), cache, lengths, 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_a_query_that_is_not_finite_spoils_its_head(dtype):
+    lengths = [50, 20]
+    for bits in (4, 8):
+        cache = _filled(lengths, 16, 2, 64, bits)
+        q = torch.randn(2, 12, 64, device="cuda").to(dtype)
+        q[0, 3, 5], q[1, 11, 63] = float("nan"), float("nan")
+        spoiled = torch.zeros(2, 12, 64, dtype=torch.bool, device="cuda")
+        spoiled[0, 3] = spoiled[1, 11] = True
+        _check_decode(q, cache, lengths, bits, spoiled=spoiled)
+
+
+def test_decode_on_another_stream():
+    from nitrix_b200.nn import decode_attention
+
+    cache = _filled([900, 40, 0], 16, 2, 64, 4)
+    q = torch.randn(3, 8, 64, device="cuda").half()
+    want = decode_attention(q, cache)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [decode_attention(q, cache) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, want) for x in got)

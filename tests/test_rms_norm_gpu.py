@@ -335,3 +335,28 @@ def test_refusals():
             rms_norm_quantized(x, group_size=group)
     with pytest.raises(ValueError, match="group_size"):
         rms_norm_quantized(x[:, :48].contiguous(), group_size=32)
+
+
+def test_more_than_2_to_the_31_elements():
+    """The last rows of tensors whose offsets leave 32 bits are those of the rows alone."""
+    from nitrix_b200.nn import rms_norm, rms_norm_quantized
+
+    rows, C = 2 ** 31 // 8192 + 40, 8192
+    x = torch.empty(rows, C, dtype=torch.bfloat16, device="cuda")
+    x[-50:].normal_()
+    w = torch.randn(C, device="cuda").bfloat16()
+    few = x[-50:].clone()
+    y = rms_norm(x, w)
+    assert torch.equal(y[-50:], rms_norm(few, w))
+    del y
+    for group in (None, 128):
+        codes, scales = rms_norm_quantized(x, w, group_size=group)
+        want = rms_norm_quantized(few, w, group_size=group)
+        assert torch.equal(codes[-50:].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales[-50:], want[1])
+        del codes, scales
+    x[:-50] = 0
+    a, b = x.requires_grad_(True), few.requires_grad_(True)
+    dy = torch.zeros_like(x)
+    dy[-50:].normal_()
+    (da,), (db,) = torch.autograd.grad(rms_norm(a, w), [a], dy), torch.autograd.grad(rms_norm(b, w), [b], dy[-50:])
+    assert torch.equal(da[-50:], db) and not bool(da[:1000].any())
