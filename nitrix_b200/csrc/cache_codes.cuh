@@ -156,15 +156,6 @@ __device__ __forceinline__ void values_of(uint32_t lo, uint32_t hi, float step, 
     }
   }
 }
-// A part's four codes of a group, less the half of their range.
-template <int kBits>
-__device__ __forceinline__ void load_codes(const uint8_t* row, int groups, int group, int part, float (&c)[4]) {
-  constexpr float kHalf = float(1 << (kBits - 1));
-  const uint32_t w = kBits == 4 ? uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + part * groups + group))
-                                : __ldg(reinterpret_cast<const uint32_t*>(row) + part * groups + group);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = __uint_as_float(0x4b000000u | (w >> (kBits * i) & ((1u << kBits) - 1u))) - (8388608.f + kHalf);
-}
 #endif
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

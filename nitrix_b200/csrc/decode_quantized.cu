@@ -28,107 +28,217 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
 }
 
-// fp32 multiply-adds.  Eight lanes share a token, a part of its row of codes each; a warp's four groups take tokens of their own.
-template <typename T, int kBits, int kGroups, int kNumHeads>
+// fp32 multiply-adds, two per instruction.  Eight lanes share a token, a part of its row of codes each; a warp's four groups take tokens
+// of their own, kAhead at a time: the next ones' codes are on their way while these are worked on.  The query heads' sums are scattered
+// over the lanes as they are reduced, so that a lane has one head's scores.
+//
+// A code in the bits from p on of 2^23 is 2^23 + 2^p code, from which the offset comes off exactly; the queries have 2^-p, the output
+// gets it at the end.
+//
+// kExact: the row has kGroups groups, so that a part's codes of all of them are one load; otherwise at most as many.
+template <typename T, int kBits, int kGroups, bool kExact, int kNumHeads>
 struct QuantizedFmaLoop {
   static constexpr const char* kName = "decode_kernel<quantized>";
   static constexpr int kRing = 0;
   static constexpr int kHeads = kNumHeads;
   static constexpr int kSlots = 4;
-  static constexpr int kMinCtas = 2;
-  float o[kHeads][kGroups][4];
-  float m[kHeads], l[kHeads];
+  static constexpr int kMinCtas = kHeads * kGroups <= 4 ? 4 : kHeads * kGroups <= 8 ? 3 : 2;
+  static constexpr int kAhead = 2;
+  static constexpr int kLanes = 8, kSteps = kHeads == 4 ? 2 : kHeads == 2 ? 1 : 0;      // of the reduce-scatter
+  static constexpr int kWords = (kGroups * kBits + 7) / 8, kStepWords = (kGroups + 1) / 2;
+  static constexpr float kHalf = float(1 << (kBits - 1));
+  float2 o[kHeads][kGroups][2];
+  float m, l;             // of this lane's head
 
-  __device__ __forceinline__ void run(const QuantizedArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0, int t1,
-                                      int wi, int wn) {
-    const T* q = static_cast<const T*>(q_row);
-    const int part = threadIdx.x & 7, first = wi * kSlots, mine = first + ((threadIdx.x & 31) >> 3), step = wn * kSlots;
-    float qf[kHeads][kGroups][4];
+  __device__ __forceinline__ static int my_head(int c) {   // the reduce-scatter's choices, high to low
+    int h = 0;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int s = 0; s < kSteps; ++s) h = 2 * h + ((c & (kLanes >> (s + 1))) ? 1 : 0);
+    return h;
+  }
+  // the first lane (of a group) that holds head h
+  __device__ __forceinline__ static int lane_of(int h) {
+    int c = 0;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g)
+    for (int s = 0; s < kSteps; ++s)
+      if (h & (kHeads >> (s + 1))) c += kLanes >> (s + 1);
+    return c;
+  }
+  // 2^-p of element i of four: with 8 bits the upper two are shifted down
+  __device__ __forceinline__ static float2 unit(int i) {
+    return kBits == 4 ? (i ? make_float2(1.f / 256.f, 1.f / 4096.f) : make_float2(1.f, 1.f / 16.f)) : make_float2(1.f, 1.f / 256.f);
+  }
+  // four codes of group g, each times its 2^p
+  __device__ __forceinline__ static void codes(const uint32_t (&w)[kWords], int g, float2 (&c)[2]) {
+    const uint32_t part = kBits == 4 ? (g % 2 ? w[g / 2] >> 16 : w[g / 2]) : w[g];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[h][g][i] = h < heads && g < a.groups ? to_f32<T>(q[h * a.qs[1] + g * kGroup + part * 4 + i]) : 0.f;
-          o[h][g][i] = 0.f;
-        }
-      m[h] = -INFINITY;
-      l[h] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t x = kBits == 8 && i ? part >> 16 : part;
+      const int p0 = kBits == 4 ? 8 * i : 0, p1 = kBits == 4 ? 8 * i + 4 : 8;
+      constexpr uint32_t mask = (1u << kBits) - 1u;
+      c[i] = __fadd2_rn(make_float2(__uint_as_float(0x4b000000u | (x & mask << p0)), __uint_as_float(0x4b000000u | (x & mask << p1))),
+                        make_float2(-8388608.f - kHalf * float(1 << p0), -8388608.f - kHalf * float(1 << p1)));
     }
-    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
-    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
-    // (all groups of a warp go round together: the shuffles are warp-wide; behind the last token that one's row is read again, with a
-    // probability of zero)
-    for (int b = t0; b + first < t1; b += step) {
-      const Where at = where(a, row_table, min(b + mine, t1 - 1));
-      const uint8_t* kr = reinterpret_cast<const uint8_t*>(row_of(kbase, a.ks, at));
-      const uint8_t* vr = reinterpret_cast<const uint8_t*>(row_of(vbase, a.vs, at));
-      const uint16_t* kt = steps_of(a.k_steps, a.kss, a.groups, kv_head, at);
-      const uint16_t* vt = steps_of(a.v_steps, a.vss, a.groups, kv_head, at);
-      float s[kHeads];
-#pragma unroll
-      for (int h = 0; h < kHeads; ++h) s[h] = 0.f;
+  }
+  __device__ __forceinline__ static float step_of(const uint32_t (&w)[kStepWords], int g) {
+    return __half2float(__ushort_as_half(uint16_t(g % 2 ? w[g / 2] >> 16 : w[g / 2])));
+  }
+  __device__ __forceinline__ static void load(const QuantizedArgs& a, const uint8_t* row, const uint16_t* steps, int part, uint32_t (&w)[kWords], uint32_t (&s)[kStepWords]) {
+    if constexpr (kExact) {
+      load_words(w, row + part * kWords * 4);
+      load_words(s, steps);
+    } else {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        if (g >= a.groups) continue;
-        float c[4];
-        load_codes<kBits>(kr, a.groups, g, part, c);
-        const float size = __half2float(__ushort_as_half(__ldg(kt + g)));
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          float dot = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dot = fmaf(qf[h][g][i], c[i], dot);
-          s[h] = fmaf(dot, size, s[h]);
-        }
-      }
-      float p[kHeads];
-#pragma unroll
-      for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-        for (int off = 4; off > 0; off >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], off);
-        const float x = b + mine < t1 ? s[h] * a.mul : -INFINITY, m_new = fmaxf(m[h], x), shift = m_new == -INFINITY ? 0.f : m_new;
-        const float old = ex2(m[h] - shift);
-        p[h] = ex2(x - shift);
-        l[h] = fmaf(l[h], old, p[h]);
-        m[h] = m_new;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[h][g][i] *= old;
-      }
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        if (g >= a.groups) continue;
-        float c[4];
-        load_codes<kBits>(vr, a.groups, g, part, c);
-        const float size = __half2float(__ushort_as_half(__ldg(vt + g)));
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          const float w = p[h] * size;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[h][g][i] = fmaf(w, c[i], o[h][g][i]);
+        const bool in = g < a.groups;
+        const uint32_t step = in ? __ldg(steps + g) : 0;
+        s[g / 2] = g % 2 ? s[g / 2] | step << 16 : step;
+        if constexpr (kBits == 4) {
+          const uint32_t c = in ? __ldg(reinterpret_cast<const uint16_t*>(row) + part * a.groups + g) : 0;
+          w[g / 2] = g % 2 ? w[g / 2] | c << 16 : c;
+        } else {
+          w[g] = in ? __ldg(reinterpret_cast<const uint32_t*>(row) + part * a.groups + g) : 0;
         }
       }
     }
   }
 
-  __device__ __forceinline__ void store(const QuantizedArgs& a, float* dst) const {
-    const int part = threadIdx.x & 7;
-    float* slot = dst + (threadIdx.x >> 3) * kHeads * (a.D + 2);
+  __device__ __forceinline__ void run(const QuantizedArgs& a, const int* row_table, int kv_head, const void* q_row, int heads, int t0, int t1,
+                                      int wi, int wn) {
+    const T* q = static_cast<const T*>(q_row);
+    const int lane = threadIdx.x & 31, part = lane % kLanes;
+    const int first = wi * kSlots, group = first + lane / kLanes, groups = wn * kSlots;
+    float2 qf[kHeads][kGroups][2];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      float* row = slot + h * (a.D + 2);
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const T* e = q + h * a.qs[1] + g * kGroup + part * 4;
+        const bool in = h < heads && (kExact || g < a.groups);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          qf[h][g][i] = in ? __fmul2_rn(make_float2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1])), unit(i)) : make_float2(0.f, 0.f);
+          o[h][g][i] = make_float2(0.f, 0.f);
+        }
+      }
+    m = -INFINITY;
+    l = 0.f;
+    const uint4* kbase = a.k + int64_t(kv_head) * a.ks[1];
+    const uint4* vbase = a.v + int64_t(kv_head) * a.vs[1];
+    const int last = t1 - 1;
+    uint32_t kw[kAhead][kWords], vw[kAhead][kWords], kt[kAhead][kStepWords], vt[kAhead][kStepWords];
+    Where at[kAhead];       // of the tokens whose keys were asked for last
+    // (behind the last token that one's rows are read again, with a probability of zero)
+    auto load_k = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        at[j] = where(a, row_table, min(b + group + j * groups, last));
+        load(a, reinterpret_cast<const uint8_t*>(row_of(kbase, a.ks, at[j])), steps_of(a.k_steps, a.kss, a.groups, kv_head, at[j]), part, kw[j], kt[j]);
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        load(a, reinterpret_cast<const uint8_t*>(row_of(vbase, a.vs, at[j])), steps_of(a.v_steps, a.vss, a.groups, kv_head, at[j]), part, vw[j], vt[j]);
+    };
+    // (every group of a warp makes as many turns as its first, which has the most: the shuffles below are warp-wide)
+    int b = t0;
+    if (b + first >= t1) return;
+    load_k(b);
+    load_v();
+    for (; b + first < t1; b += groups * kAhead) {
+      const int next = b + groups * kAhead;
+      float x[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        float2 s2[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) s2[h] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float2 c[2];
+          codes(kw[j], g, c);
+          const float step = step_of(kt[j], g);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h)
+            s2[h] = __ffma2_rn(__ffma2_rn(qf[h][g][1], c[1], __fmul2_rn(qf[h][g][0], c[0])), make_float2(step, step), s2[h]);
+        }
+        float s[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) s[h] = s2[h].x + s2[h].y;
+        // reduce-scatter: every step halves the heads that a lane still sums; then what is left of the lanes
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          const int off = kLanes >> (step + 1), n = kHeads >> (step + 1);
+          const bool upper = (part & off) != 0;
+#pragma unroll
+          for (int h = 0; h < kHeads / 2; ++h) {
+            if (h >= n) continue;
+            const float keep = upper ? s[h + n] : s[h], send = upper ? s[h] : s[h + n];
+            s[h] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+          }
+        }
+#pragma unroll
+        for (int off = kLanes >> (kSteps + 1); off > 0; off >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+        x[j] = b + group + j * groups < t1 ? s[0] * a.mul : -INFINITY;
+      }
+      if (next + first < t1) load_k(next);
+      float m_new = m;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) m_new = fmaxf(m_new, x[j]);
+      const float shift = m_new == -INFINITY ? 0.f : m_new;
+      if (__any_sync(0xffffffffu, m_new > m)) {
+        const float alpha = ex2(m - shift);
+        l *= alpha;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const float ah = __shfl_sync(0xffffffffu, alpha, (lane & ~(kLanes - 1)) + lane_of(h));
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[h][g][i] = __fmul2_rn(o[h][g][i], make_float2(ah, ah));
+        }
+      }
+      m = m_new;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float pr = ex2(x[j] - shift);
+        l += pr;
+        float ph[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) ph[h] = __shfl_sync(0xffffffffu, pr, (lane & ~(kLanes - 1)) + lane_of(h));
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float2 c[2];
+          codes(vw[j], g, c);
+          const float step = step_of(vt[j], g);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) {
+            const float w = ph[h] * step;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[h][g][i] = __ffma2_rn(make_float2(w, w), c[i], o[h][g][i]);
+          }
+        }
+      }
+      if (next + first < t1) load_v();
+    }
+  }
+
+  __device__ __forceinline__ void store(const QuantizedArgs& a, float* dst) const {
+    const int part = threadIdx.x % kLanes;
+    float* slot = dst + threadIdx.x / kLanes * kHeads * (a.D + 2);
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        if (g < a.groups)
+        if (kExact || g < a.groups)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) row[g * kGroup + part * 4 + i] = o[h][g][i];
-      if (part == 0) {
-        row[a.D] = m[h];
-        row[a.D + 1] = l[h];
-      }
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<float2*>(slot + h * (a.D + 2) + g * kGroup + part * 4 + 2 * i) = __fmul2_rn(o[h][g][i], unit(i));
+    if ((part & ((kLanes >> kSteps) - 1)) == 0) {
+      float* row = slot + my_head(part) * (a.D + 2);
+      row[a.D] = m;
+      row[a.D + 1] = l;
     }
   }
 };
@@ -488,6 +598,9 @@ int check(const nb200_decode_quantized_params* p, const char* what) {
   return check_steps(c, p->steps, what);
 }
 
+// groups of the fp32 loops that take a head dim
+int groups_of(int head_dim) { return head_dim == 64 ? 2 : head_dim <= 128 ? 4 : 8; }
+
 Plan plan(const nb200_decode_params* p, int bits) {
   const nb200_cache_pages& c = p->pages;
   Plan pl{};
@@ -500,7 +613,10 @@ Plan plan(const nb200_decode_params* p, int bits) {
     pl.heads = group > 8 ? 16 : 8;
     ctas = pl.heads == 8 ? (c.head_dim == 64 ? 4 : bits == 4 ? 3 : 2) : c.head_dim == 64 ? 3 : 2;
   } else {
-    pl.heads = c.head_dim > 128 ? 2 : 4;
+    const int most = c.head_dim > 128 ? 2 : 4;
+    pl.heads = group >= most ? most : group == 3 ? 4 : group;
+    const int size = pl.heads * groups_of(c.head_dim);
+    ctas = size <= 4 ? 4 : size <= 8 ? 3 : 2;
   }
   const int chunks = (group + pl.heads - 1) / pl.heads;
   pl.side = chunks == 1 ? 1 : chunks == 2 ? 2 : 4;
@@ -517,11 +633,23 @@ Plan plan(const nb200_decode_params* p, int bits) {
   return pl;
 }
 
+template <typename T, int kBits, int kGroups, bool kExact>
+int launch_fma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
+  if (heads == 1) return launch<T, QuantizedFmaLoop<T, kBits, kGroups, kExact, 1>, true>(a, side, st);
+  if constexpr (kGroups <= 4) {
+    if (heads == 4) return launch<T, QuantizedFmaLoop<T, kBits, kGroups, kExact, 4>, false>(a, side, st);
+    return launch<T, QuantizedFmaLoop<T, kBits, kGroups, kExact, 2>, true>(a, side, st);
+  } else {
+    return launch<T, QuantizedFmaLoop<T, kBits, kGroups, kExact, 2>, false>(a, side, st);
+  }
+}
 template <typename T, int kBits>
-int launch_fma(const QuantizedArgs& a, int side, cudaStream_t st) {
-  if (a.groups <= 2) return launch<T, QuantizedFmaLoop<T, kBits, 2, 4>, false>(a, side, st);
-  if (a.groups <= 4) return launch<T, QuantizedFmaLoop<T, kBits, 4, 4>, false>(a, side, st);
-  return launch<T, QuantizedFmaLoop<T, kBits, 8, 2>, false>(a, side, st);
+int launch_fma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
+  if (a.groups == 2) return launch_fma<T, kBits, 2, true>(a, heads, side, st);
+  if (a.groups == 4) return launch_fma<T, kBits, 4, true>(a, heads, side, st);
+  if (a.groups < 4) return launch_fma<T, kBits, 4, false>(a, heads, side, st);
+  if (a.groups == 8) return launch_fma<T, kBits, 8, true>(a, heads, side, st);
+  return launch_fma<T, kBits, 8, false>(a, heads, side, st);
 }
 
 template <typename T, int D, int kBits, bool kDense>
@@ -540,7 +668,7 @@ int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
 template <typename T>
 int launch_16(const QuantizedArgs& a, const Plan& pl, bool four, cudaStream_t st) {
   if (pl.mma) return four ? launch_mma<T, 4>(a, pl.heads, pl.side, st) : launch_mma<T, 8>(a, pl.heads, pl.side, st);
-  return four ? launch_fma<T, 4>(a, pl.side, st) : launch_fma<T, 8>(a, pl.side, st);
+  return four ? launch_fma<T, 4>(a, pl.heads, pl.side, st) : launch_fma<T, 8>(a, pl.heads, pl.side, st);
 }
 
 }  // namespace
@@ -604,6 +732,6 @@ extern "C" NB200_API int nb200_decode_quantized(const nb200_decode_quantized_par
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
   const bool four = qp->steps.bits == 4;
-  if (c.dtype == NB200_F32) return four ? launch_fma<float, 4>(a, pl.side, st) : launch_fma<float, 8>(a, pl.side, st);
+  if (c.dtype == NB200_F32) return four ? launch_fma<float, 4>(a, pl.heads, pl.side, st) : launch_fma<float, 8>(a, pl.heads, pl.side, st);
   return c.dtype == NB200_BF16 ? launch_16<__nv_bfloat16>(a, pl, four, st) : launch_16<__half>(a, pl, four, st);
 }
