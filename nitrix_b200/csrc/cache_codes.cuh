@@ -72,17 +72,23 @@ __device__ __forceinline__ Quantized<kBits> quantize(const uint4 (&words)[sizeof
   constexpr uint32_t kBase = 0x4b400000u, kKnown = kBits == 4 ? kBase * 0x11111111u : kBase * 0x01010101u;
   // A quotient is at most half (1 + 2^-11) in size, so that only the far end has to be cut, unless the step has been cut itself or has
   // lost bits as one of fp16's smallest numbers.
-  float z[8];
+  float2 z[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = fminf(__fmul_rn(x[i], inverse), kHalf - 1.f);
+  for (int i = 0; i < 4; ++i) {
+    z[i] = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(inverse, inverse));
+    z[i] = make_float2(fminf(z[i].x, kHalf - 1.f), fminf(z[i].y, kHalf - 1.f));
+  }
   const float size = fabsf(s);
   if (__any_sync(0xffffffffu, size < 6.103515625e-05f || size >= 65504.f)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = fmaxf(z[i], float(-kHalf));
+    for (int i = 0; i < 4; ++i) z[i] = make_float2(fmaxf(z[i].x, float(-kHalf)), fmaxf(z[i].y, float(-kHalf)));
   }
   uint32_t w[8 * kBits / 32] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i * kBits / 32] += __float_as_uint(__fadd_rn(z[i], kM)) << (i * kBits % 32);
+  for (int i = 0; i < 4; ++i) {
+    const float2 c = __fadd2_rn(z[i], make_float2(kM, kM));
+    w[2 * i * kBits / 32] += (__float_as_uint(c.x) << (2 * i * kBits % 32)) + (__float_as_uint(c.y) << ((2 * i + 1) * kBits % 32));
+  }
   // (what is not finite, and a step of zero, has the codes of zero: z is zero in the second case)
   constexpr uint32_t kZero = kBits == 4 ? 0x88888888u : 0x80808080u;
   q.lo = finite ? w[0] - kKnown : kZero;

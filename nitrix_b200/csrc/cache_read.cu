@@ -219,8 +219,8 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   }
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);
-  // one token per warp while that does not fill the GPU's warps, then four, which share a search
-  a.tokens_per_warp = p->tokens < 148 * 64 ? 1 : 4;
+  // One token per warp while that does not fill the GPU's warps a few times over, then more, which share a search.
+  a.tokens_per_warp = p->tokens < 148 * 128 ? 1 : p->tokens < 148 * 512 ? 2 : 4;
   const int64_t per_cta = int64_t(a.tokens_per_warp) * (kThreads / 32);
   kernel<<<unsigned((p->tokens + per_cta - 1) / per_cta), kThreads, 0, st>>>(a);
   count_launch();
