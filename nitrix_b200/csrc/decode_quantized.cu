@@ -370,32 +370,32 @@ struct QuantizedMmaLoop {
     auto token_of = [](int r) { return (r & 8) + ((r & 1) ? 4 + ((r >> 1 & 3) ^ 1) : r >> 1 & 3); };
     const int mine = token_of(g);      // and mine + 8: this lane's tokens of the scores; t, 4 + (t ^ 1) and these + 8 are those of the values
     const uint32_t to = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16;
-    const char* k_from = reinterpret_cast<const char*>(a.k + int64_t(kv_head) * a.ks[1]) + (kDense ? lane * 16 : 0);
-    const char* v_from = reinterpret_cast<const char*>(a.v + int64_t(kv_head) * a.vs[1]) + (kDense ? lane * 16 : 0);
+    const uint4* k_from = a.k + int64_t(kv_head) * a.ks[1] + (kDense ? lane : 0);
+    const uint4* v_from = a.v + int64_t(kv_head) * a.vs[1] + (kDense ? lane : 0);
     const char* steps_from = reinterpret_cast<const char*>(lane < 16 ? steps_of(a.k_steps, a.kss, kG, kv_head, Where{0, 0})
                                                                     : steps_of(a.v_steps, a.vss, kG, kv_head, Where{0, 0})) + (kDense ? (lane & 15) * 16 : 0);
-    const int64_t page_bytes = int64_t(a.ks[0]) * 16, page_steps = int64_t(a.kss[0]) * (2 * kG);
+    // (kDense: a page's steps are whole 16-byte words, as are 16 tokens')
+    const int page_words = a.kss[0] * kG / 8, page_mask = a.page_size - 1;
+    const bool has_steps = (lane & 15) < 2 * kG;
     auto page_of = [&](int b) { return kDense ? page_at(a, row_table, min(b, last) >> a.page_shift) : 0; };
     // block u of the turn at b; behind the last token what stands in its page, or that token's rows again
-    auto fetch = [&](int b, int u, int page, int stage) {
-      const uint32_t dst = to + stage * kStage;
+    auto fetch = [&](int b, int u, int page, uint32_t dst) {
       if constexpr (kDense) {
-        const int slot = b & (a.page_size - 1);
-        const int64_t at = page * page_bytes + slot * kRow;
+        const int slot = b & page_mask;
+        const int64_t at = int64_t(page) * a.ks[0] + slot * (kRow / 16), steps = int64_t(page) * page_words + (slot * kG >> 3);
 #pragma unroll
-        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + at + i * 512);
+        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + at + i * 32);
 #pragma unroll
-        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + at + i * 512);
-        if ((lane & 15) < 2 * kG)
-          copy_async<16>(dst + kStepsAt + u * kBlock * 2 * kG + (lane < 16 ? 0 : kTurn * 2 * kG - 256), steps_from + page * page_steps + slot * (2 * kG));
+        for (int i = 0; i < kRow / 32; ++i) copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + at + i * 32);
+        if (has_steps) copy_async<16>(dst + kStepsAt + u * kBlock * 2 * kG + (lane < 16 ? 0 : kTurn * 2 * kG - 256), reinterpret_cast<const uint4*>(steps_from) + steps);
       } else {
 #pragma unroll
         for (int i = 0; i < kRow / 32; ++i) {
           const int at = lane * 16 + i * 512;
           const Where w = where(a, row_table, min(b + at / kRow, last));
           const int64_t k_row = int64_t(w.page) * a.ks[0] + int64_t(w.slot) * a.ks[2], v_row = int64_t(w.page) * a.vs[0] + int64_t(w.slot) * a.vs[2];
-          copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + k_row * 16 + at % kRow);
-          copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + v_row * 16 + at % kRow);
+          copy_async<16>(dst + u * kBlock * kRow + i * 512, k_from + k_row + at % kRow / 16);
+          copy_async<16>(dst + kValuesAt + u * kBlock * kRow + i * 512, v_from + v_row + at % kRow / 16);
         }
         const Where w = where(a, row_table, min(b + (lane & 15), last));
         const int64_t row = lane < 16 ? int64_t(w.page) * a.kss[0] + int64_t(w.slot) * a.kss[2] : int64_t(w.page) * a.vss[0] + int64_t(w.slot) * a.vss[2];
@@ -404,9 +404,11 @@ struct QuantizedMmaLoop {
     };
     int page[2];
     auto fetch_turn = [&](int b, int stage) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (b + u * kBlock < t1) fetch(b + u * kBlock, u, page[u], stage);
+      const uint32_t dst = to + stage * kStage;
+      if (b < t1) {
+        fetch(b, 0, page[0], dst);
+        fetch(b + kBlock, 1, page[1], dst);      // (of which there may be nothing: then another block's rows, for no one)
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // One turn; kTail: the last of the tokens, of which it may hold any number.
