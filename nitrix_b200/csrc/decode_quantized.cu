@@ -2,7 +2,14 @@
 //
 //   s_t = scale q . k_t,  p = softmax(s),  out = sum_t p_t v_t,     k_t, v_t = step (code - 2^(b-1)) per group of 32 elements
 //
-// Bound by HBM: every code and step is read once, 72 bytes per 128 elements in 4 bits.
+// Every code and step is read once, 72 bytes per 128 elements in 4 bits, which HBM would deliver faster than the codes can be taken
+// apart: 16 tokens of a head of 128 take a warp 322 instructions, 140 of them on the integer pipe at two cycles each, and the
+// schedulers issue 0.6 per cycle with three or four warps each.
+//
+// 64 sequences of up to 8192 tokens (266 k in all), 8 key heads: bf16 4 bits, 4 x 128: 83 us, 3.7 TB/s; 8 bits, 5 x 64: 63, 4.6 TB/s; 4 of
+// up to 131072 tokens, f16 4 bits, 8 x 128: 91, 4.1 TB/s.  32 such sequences in fp32, 4 bits, head dim 128, 1 / 2 / 4 / 8 query heads per
+// key head: 102 / 124 / 183 / 337 us; bf16 52 with 1, 103 with 16.  On the way, for the first of these cases: fp32 units 792 us, MMAs with
+// loads into registers 124, places as constants of a lane 102, the ring 98, two blocks a turn and beginnings counted 89.
 #include <type_traits>
 
 #include "cache_codes.cuh"
@@ -264,6 +271,7 @@ struct QuantizedMmaLoop {
   static constexpr int kHeads = 8 * kTiles;
   static constexpr int kBlock = 16, kTurn = 32;  // tokens
   static constexpr int kSlots = 1;
+  // (head dim 128: three CTAs per SM without spills 97 us over long contexts, four with them 99, five 142)
   static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 4 : kBits == 4 ? 3 : 2) : D == 64 ? 3 : 2;
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes

