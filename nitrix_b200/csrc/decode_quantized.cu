@@ -668,7 +668,9 @@ int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
 }
 template <typename T, int kBits>
 int launch_mma(const QuantizedArgs& a, int heads, int side, cudaStream_t st) {
-  bool dense = a.page_shift >= 4 && a.ks[2] * 16 == a.D * kBits / 8 && a.kss[2] == 1;
+  // (places within a page, and steps' pages, as 32-bit numbers of words)
+  bool dense = a.page_shift >= 4 && a.page_shift <= 24 && a.ks[2] == a.D * kBits / 128 && a.kss[2] == 1;
+  dense = dense && int64_t(a.kss[0]) * a.groups <= 0x7fffffff && int64_t(a.kss[0]) * a.groups >= -0x7fffffff;
   for (int i = 0; i < 3; ++i) dense = dense && a.ks[i] == a.vs[i] && a.kss[i] == a.vss[i];
   for (int i = 0; i < 2; ++i) dense = dense && int64_t(a.kss[i]) * a.groups % 8 == 0;      // (16-byte copies of steps)
   if (a.D == 64) return dense ? launch_mma<T, 64, kBits, true>(a, heads, side, st) : launch_mma<T, 64, kBits, false>(a, heads, side, st);

@@ -31,12 +31,12 @@ struct Pages {
   int pages, heads, page_size, words;   // words of a head's row
 };
 
-// The steps of a cache in few bits, as the largest units that their rows are made of.
+// The steps of a cache in few bits.
 struct StepPages {
   uint16_t* k;
   uint16_t* v;
   int64_t ks[3], vs[3];     // elements, over (page, head, slot)
-  int groups;               // elements of a head's row
+  int groups;               // of a head's row
 };
 
 // ---- append ---------------------------------------------------------------------------------------------------------------

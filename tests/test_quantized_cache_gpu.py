@@ -691,3 +691,40 @@ def test_decode_on_another_stream():
         got = [decode_attention(q, cache) for _ in range(3)]
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_appending_views(bits, dtype):
+    """Slices of one projection's output, misaligned rows, one head's row for all heads."""
+    from nitrix_b200.nn import cache_append, cache_read
+
+    offsets, n = _ints([0, 5, 19]), 19
+    g = torch.Generator(device="cuda").manual_seed(0)
+    wide = torch.randn(n, (6 + 2 * 3) * 64, generator=g, device="cuda").to(dtype)
+    odd = torch.randn(n * 3 * 64 + 1, generator=g, device="cuda").to(dtype)[1:].view(n, 3, 64)
+    heads = wide.unflatten(1, (12, 64))
+    for k, v in ((heads[:, 6:9], heads[:, 9:]), (odd, odd.flip(0)), (heads[:, :1].expand(n, 3, 64), odd), (odd.transpose(0, 1).contiguous().transpose(0, 1), heads[:, ::4])):
+        cache = _cache(12, 4, 3, 64, bits, 2, 8)
+        got = cache_read(cache_append(cache, k, v, offsets), offsets, n, dtype=torch.float32)
+        for x, y in zip((k, v), got):
+            codes, steps = O.quantize(x, bits)
+            assert torch.equal(y, O.values(O.packed_codes(codes, bits), steps, bits).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_steps_in_pages_that_lie_far_apart(dtype):
+    """Strides from one page's steps to the next's of 2^31 elements."""
+    from nitrix_b200.nn import cache_append, cache_read, decode_attention
+
+    small = _cache(2, 16, 2, 128, 4, 1, 2)
+    buffer = torch.empty((1 << 31) + 1024, dtype=torch.float16, device="cuda")
+    far = lambda at: buffer[at:].as_strided((2, 2, 16, 4), (1 << 31, 64, 4, 1))
+    large = small._replace(k_codes=small.k_codes.clone(), v_codes=small.v_codes.clone(), k_steps=far(0), v_steps=far(512), table=small.table.clone())
+    k, v = (torch.randn(30, 2, 128, device="cuda").to(dtype) for _ in range(2))
+    q, offsets = torch.randn(1, 4, 128, device="cuda").to(dtype), _ints([0, 30])
+    small, large = (cache_append(c, k, v, offsets) for c in (small, large))
+    assert torch.equal(small.table, large.table)
+    assert all(torch.equal(a, b) for a, b in zip(cache_read(small, offsets, 30), cache_read(large, offsets, 30)))
+    _check_decode(q, small, [30], 4)
+    _check_decode(q, large, [30], 4)
