@@ -117,7 +117,8 @@ NB200_API int nb200_decode_workspace_bytes(const nb200_decode_params* p, size_t*
  *
  * In nb200_cache_pages k and v are then the codes, their strides are bytes, dtype is that of the new tokens, of q and out, or of
  * what is read; head_dim is a multiple of 32.  Rows of codes begin on 16-byte boundaries, those of steps on multiples of their
- * own size from a 16-byte boundary.
+ * own size from a 16-byte boundary.  Append and decode take strides (append: the new tokens' also) below 2^31 words of 16 bytes or
+ * rows of steps.
  */
 typedef struct nb200_cache_steps {
   void* k;                            /* fp16 (pages, heads, page_size, head_dim / 32), unit stride on the last axis */

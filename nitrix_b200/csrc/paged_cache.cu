@@ -6,14 +6,17 @@
 //
 // Bound by HBM where tokens or pages are moved (each read and written once, in 16-byte words with eight in flight per
 // thread), by launches and latency where a step adds one token per sequence: append is ONE launch, in which every warp finds
-// its token's sequence and the number of pages that the sequences before it take by one pass over `offsets` and `lengths`;
+// its tokens' sequence and the number of pages that the sequences before it take by one pass over `offsets` and `lengths`;
 // fork is a memset and two launches, compact a memset and three, each set up while the one before runs.  33 k tokens of bf16, 8
 // heads of 128, 50 us (5.5 TB/s); 2100 pages of 64 KB moved among 8300, 60 us (4.5 TB/s), 48 of them the moves; 256 single tokens 7.6 and
 // a fork of 64 rows 10.5 in a captured graph, 15 and 21 where the host makes the calls.
 //
-// Tokens for a cache in few bits are quantised on the way (cache_codes.cuh): 35 k tokens of bf16, 8 heads of 128, into 4 bits in 51 us, 3.6
-// TB/s of what is read and written; two thirds of the issue slots are busy, with about a hundred instructions for a lane's 8 elements.
-// One group a lane and 16-bit stores of codes: 78.
+// Tokens for a cache in few bits are quantised on the way (cache_codes.cuh): 34 k tokens of bf16, 8 heads of 128, into 4 bits in 42 us, 4.3
+// TB/s of what is read and written; two thirds of the issue slots are busy, with 47 instructions for a lane's 8 elements and some 300 for
+// a token's place.  On the way: one group a lane and 16-bit stores of codes 78 us, steps worked out by every lane of a group 52, three
+// CTAs per SM without spills 49, places in 64 bits and elements asked for when the place is known 45; four tokens a warp 46.
+#include <algorithm>
+
 #include "cache_codes.cuh"
 #include "dependent_launch.cuh"
 #include "sm100_primitives.cuh"
@@ -54,9 +57,12 @@ struct AppendArgs {
   const uint4* k;
   const uint4* v;
   int64_t ks[2], vs[2];     // words, over (token, head)
-  int64_t tokens;
-  int tokens_per_warp;
+  int tokens, tokens_per_warp;
+  int capacity;             // tokens that a row of the table has places for
   StepPages steps;
+  // Strides where tokens are quantised, of keys and values, so that an offset is one wide multiply-add each: of codes and tokens in
+  // 16-byte words, of steps in rows, over (page, head, slot) and (token, head).
+  int codes_stride[2][3], steps_stride[2][3], from_stride[2][2];
 };
 
 struct RowPlan {
@@ -64,15 +70,15 @@ struct RowPlan {
 };
 
 // Offsets that leave the tokens are cut to them.
-__device__ __forceinline__ int first_of(const AppendArgs& a, int row) { return int(min(int64_t(max(a.offsets[row], 0)), a.tokens)); }
+__device__ __forceinline__ int first_of(const AppendArgs& a, int row) { return min(max(a.offsets[row], 0), a.tokens); }
 
 __device__ __forceinline__ RowPlan plan_row(const AppendArgs& a, int row) {
   RowPlan r;
   const int lo = first_of(a, row), hi = first_of(a, row + 1);
-  r.held = int(min(int64_t(min(max(a.lengths[row], 0), NB200_CACHE_MOST_TOKENS)), int64_t(a.width) * a.p.page_size));
-  r.want = int(min(int64_t(r.held) + max(hi - lo, 0), int64_t(NB200_CACHE_MOST_TOKENS)));
-  r.have = int((int64_t(r.held) + a.p.page_size - 1) / a.p.page_size);
-  const int pages = int((int64_t(r.want) + a.p.page_size - 1) / a.p.page_size);
+  r.held = min(max(a.lengths[row], 0), a.capacity);
+  r.want = int(min(unsigned(r.held) + unsigned(max(hi - lo, 0)), unsigned(NB200_CACHE_MOST_TOKENS)));
+  r.have = int((unsigned(r.held) + unsigned(a.p.page_size - 1)) / unsigned(a.p.page_size));      // (below 2^32)
+  const int pages = int((unsigned(r.want) + unsigned(a.p.page_size - 1)) / unsigned(a.p.page_size));
   r.need = max(min(pages, a.width) - r.have, 0);
   return r;
 }
@@ -90,79 +96,153 @@ __device__ __forceinline__ void free_bounds(const int* range, int pages, int* be
   *end = min(max(range[1], *begin), pages);
 }
 
-// Where a token's codes and steps go, and where it comes from.
-struct TokenPlace {
-  uint8_t* codes[2];
-  uint16_t* steps[2];
-  const uint4* from[2];
-  int64_t codes_head[2], steps_head[2], from_head[2];      // from one head to the next
-};
-__device__ __forceinline__ TokenPlace place_of(const AppendArgs& a, int64_t t, int page, int slot) {
-  return TokenPlace{{reinterpret_cast<uint8_t*>(a.p.k + page * a.p.ks[0] + slot * a.p.ks[2]), reinterpret_cast<uint8_t*>(a.p.v + page * a.p.vs[0] + slot * a.p.vs[2])},
-                    {a.steps.k + page * a.steps.ks[0] + slot * a.steps.ks[2], a.steps.v + page * a.steps.vs[0] + slot * a.steps.vs[2]},
-                    {a.k + t * a.ks[0], a.v + t * a.vs[0]},
-                    {a.p.ks[1] * 16, a.p.vs[1] * 16},
-                    {a.steps.ks[1], a.steps.vs[1]},
-                    {a.ks[1], a.vs[1]}};
-}
-
-// Quantises a token's row into a slot of a page, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of
-// them, so that its codes lie side by side; otherwise, for any number of groups, 8 elements.  Four lanes share a group's elements.
+// A token that is quantised, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of them, so that its
+// codes lie side by side; otherwise, for any number of groups, 8 elements.  Four lanes share a group's elements.
 template <int kBits, typename T, int kGroups>
-__device__ __forceinline__ void quantize_token(const AppendArgs& a, const TokenPlace& at) {
-  constexpr int kWords = sizeof(T) == 4 ? 2 : 1, kEach = kGroups ? kGroups : 1;
-  const int lane = threadIdx.x & 31, u = lane & 3;
-  const int units = kGroups ? 4 : a.steps.groups * 4, n = a.p.heads * units;
-  // (whole warps go round together: a group's lanes exchange their maxima)
-  for (int w0 = 0; w0 < n; w0 += 32) {
-    const int w = min(w0 + lane, n - 4 + u), h = w / units, c = w - h * units;      // (n is a multiple of 4)
-    const bool in = w0 + lane < n;
-    uint4 x[2][kEach][kWords];
+struct Quantizer {
+  static constexpr int kWords = sizeof(T) == 4 ? 2 : 1, kEach = kGroups ? kGroups : 1;
+  uint4 x[2][kEach][kWords];      // of the lane's first elements of the token that comes next
+
+  // the lane's head and place within its row at a turn that begins with w0 (whole warps go round together: a group's lanes exchange
+  // their maxima)
+  struct Turn {
+    int n, h, c;
+    __device__ __forceinline__ Turn(const AppendArgs& a, int w0) {
+      const int lane = threadIdx.x & 31, units = (kGroups ? kGroups : a.steps.groups) * 4 / kEach;
+      n = a.p.heads * units;
+      const int w = min(w0 + lane, n - 4 + (lane & 3));      // (n is a multiple of 4)
+      h = w / units;
+      c = w - h * units;
+    }
+  };
+  __device__ __forceinline__ void load(const AppendArgs& a, int t, const Turn& at) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
+    for (int which = 0; which < 2; ++which) {
+      const uint4* from = (which ? a.v : a.k) + int64_t(t) * a.from_stride[which][0] + int64_t(at.h) * a.from_stride[which][1] + at.c * kWords;
 #pragma unroll
       for (int g = 0; g < kEach; ++g)
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) x[which][g][i] = sm100::ldg_no_allocate(at.from[which] + h * at.from_head[which] + (g * 4 + c) * kWords + i);
+        for (int i = 0; i < kWords; ++i) x[which][g][i] = sm100::ldg_no_allocate(from + g * 4 * kWords + i);
+    }
+  }
+  __device__ __forceinline__ void load(const AppendArgs& a, int t) { load(a, t, Turn(a, 0)); }
+  __device__ __forceinline__ void store(const AppendArgs& a, int t, int page, int slot) {
+    const int lane = threadIdx.x & 31, u = lane & 3, groups = kGroups ? kGroups : a.steps.groups;
+    Turn at(a, 0);
+    for (int w0 = 0;;) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      Quantized<kBits> q[kEach];
-#pragma unroll
-      for (int g = 0; g < kEach; ++g) q[g] = quantize<kBits, T>(x[which][g]);
-      if (!in) continue;
-      uint8_t* codes = at.codes[which] + h * at.codes_head[which];
-      uint16_t* steps = at.steps[which] + h * at.steps_head[which];
-      if constexpr (kGroups > 0) {
-        store_quarter<kBits, kGroups>(codes, u, q);
-        if (u == 0) {
-          uint32_t s[kGroups / 2];
-#pragma unroll
-          for (int i = 0; i < kGroups / 2; ++i) s[i] = q[2 * i].step | uint32_t(q[2 * i + 1].step) << 16;
-          store_words(steps, s);
+      for (int which = 0; which < 2; ++which) {
+        const int (&cs)[3] = a.codes_stride[which], (&ss)[3] = a.steps_stride[which];
+        const Quantized<kBits, kEach> q = quantize<kBits, T, kEach>(x[which]);
+        if (w0 + lane >= at.n) continue;
+        uint8_t* codes = reinterpret_cast<uint8_t*>((which ? a.p.v : a.p.k) + int64_t(page) * cs[0] + int64_t(at.h) * cs[1] + int64_t(slot) * cs[2]);
+        uint16_t* steps = (which ? a.steps.v : a.steps.k) + (int64_t(page) * ss[0] + int64_t(at.h) * ss[1] + int64_t(slot) * ss[2]) * groups;
+        if constexpr (kGroups > 0) {
+          store_quarter<kBits, kGroups>(codes, u, q);
+          const int g = q.step_of(u);
+          if (u == q.first_lane(g)) steps[g] = q.step;
+        } else {
+          store_codes(codes, groups, at.c >> 2, u, q);
+          if (u == 0) steps[at.c >> 2] = q.step;
         }
-      } else {
-        store_codes(codes, a.steps.groups, c >> 2, u, q[0]);
-        if (u == 0) steps[c >> 2] = q[0].step;
+      }
+      w0 += 32;
+      if (w0 >= at.n) return;
+      at = Turn(a, w0);
+      load(a, t, at);
+    }
+  }
+};
+// A token that is copied.
+struct Copier {
+  __device__ __forceinline__ void load(const AppendArgs&, int) {}
+  __device__ __forceinline__ void store(const AppendArgs& a, int t, int page, int slot) {
+    uint4* kd = a.p.k + page * a.p.ks[0] + slot * a.p.ks[2];
+    uint4* vd = a.p.v + page * a.p.vs[0] + slot * a.p.vs[2];
+    const uint4* kx = a.k + int64_t(t) * a.ks[0];
+    const uint4* vx = a.v + int64_t(t) * a.vs[0];
+    const int n = a.p.heads * a.p.words;
+    for (int w0 = threadIdx.x & 31; w0 < n; w0 += 128) {
+      uint4 kw[4], vw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int w = w0 + 32 * i, h = w / a.p.words, c = w - h * a.p.words;
+        if (w < n) {
+          kw[i] = __ldg(kx + h * a.ks[1] + c);
+          vw[i] = __ldg(vx + h * a.vs[1] + c);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int w = w0 + 32 * i, h = w / a.p.words, c = w - h * a.p.words;
+        if (w < n) {
+          kd[h * a.p.ks[1] + c] = kw[i];
+          vd[h * a.p.vs[1] + c] = vw[i];
+        }
       }
     }
   }
-}
-template <int kBits, typename T>
-__device__ __forceinline__ void quantize_token(const AppendArgs& a, int64_t t, int page, int slot) {
-  const TokenPlace at = place_of(a, t, page, slot);
-  if (a.steps.groups == 4) quantize_token<kBits, T, 4>(a, at);
-  else if (a.steps.groups == 2) quantize_token<kBits, T, 2>(a, at);
-  else quantize_token<kBits, T, 0>(a, at);
+};
+
+// Tokens t0 .. t1, by a warp.  Where one comes from does not depend on where it goes: its elements are on their way meanwhile.
+template <typename Token>
+__device__ __forceinline__ void append_tokens(const AppendArgs& a, int begin, int64_t avail, int t0, int t1) {
+  const int lane = threadIdx.x & 31;
+  if (t0 >= t1) return;
+  Token token;
+  token.load(a, t0);
+  int row = -1, next = 0, first = 0, got = 0, before = 0;
+  RowPlan r{0, 0, 0, 0};
+  for (int t = t0;;) {
+    if (row < 0 || t >= next) {
+      // the token's sequence, and the pages that those before it take
+      int count = 0;
+      int64_t need = 0;
+      bool descend = false;
+      for (int i = lane; i < a.rows; i += 32) {
+        descend = descend || a.offsets[i] > a.offsets[i + 1];
+        if (a.offsets[i + 1] <= t) {
+          ++count;
+          need += plan_row(a, i).need;
+        }
+      }
+      // (more than there are free pages is as good as all of them, and fits 32 bits; a sum of 32 such numbers takes two)
+      const unsigned few = unsigned(min(need, avail));
+      need = int64_t(__reduce_add_sync(0xffffffffu, few & 0xffffu)) + (int64_t(__reduce_add_sync(0xffffffffu, few >> 16)) << 16);
+      row = __reduce_add_sync(0xffffffffu, count);
+      if (row >= a.rows || __any_sync(0xffffffffu, descend)) return;     // (tokens behind the last offset)
+      r = plan_row(a, row);
+      first = first_of(a, row);
+      next = a.offsets[row + 1];
+      got = pages_got(r, avail, need);
+      before = int(min(need, avail));
+    }
+    int page = -1, slot = 0;
+    const unsigned pos = unsigned(r.held) + unsigned(t - first);
+    if (t >= first && pos < unsigned(tokens_kept(r, got, a.p.page_size))) {
+      const int column = int(pos / unsigned(a.p.page_size));
+      slot = int(pos) - column * a.p.page_size;
+      if (column >= r.have) {
+        page = a.free_pages[begin + before + column - r.have];
+        if (slot == 0 && lane == 0) a.table[int64_t(row) * a.width + column] = page;
+      } else if (column < a.width) {
+        page = a.table[int64_t(row) * a.width + column];
+      }
+    }
+    if (page >= 0 && page < a.p.pages) token.store(a, t, page, slot);
+    if (++t >= t1) return;
+    token.load(a, t);
+  }
 }
 
 // kBits 0: the tokens' rows are copied; otherwise T is their type.
 template <int kBits, typename T>
-__global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, kBits == 0 || sizeof(T) == 4 ? 1 : 4) cache_append_kernel(const AppendArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int begin, end;
   free_bounds(a.free_range, a.p.pages, &begin, &end);
   const int64_t avail = end - begin;
-  if (blockIdx.x == gridDim.x - 1) {
+  if (blockIdx.x == 0) {
     // the state after the call: one CTA, 256 rows at a time
     __shared__ int64_t part[kThreads / 32];
     __shared__ unsigned long long dropped;
@@ -207,77 +287,12 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendArgs
     }
     return;
   }
-  const int64_t t0 = (int64_t(blockIdx.x) * (kThreads / 32) + warp) * a.tokens_per_warp;
-  const int64_t t1 = min(t0 + a.tokens_per_warp, a.tokens);
-  int row = -1, next = 0, first = 0, got = 0, before = 0;
-  RowPlan r{0, 0, 0, 0};
-  for (int64_t t = t0; t < t1; ++t) {
-    if (row < 0 || t >= next) {
-      // the token's sequence, and the pages that those before it take
-      int count = 0;
-      int64_t need = 0;
-      bool descend = false;
-      for (int i = lane; i < a.rows; i += 32) {
-        descend = descend || a.offsets[i] > a.offsets[i + 1];
-        if (int64_t(a.offsets[i + 1]) <= t) {
-          ++count;
-          need += plan_row(a, i).need;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        count += __shfl_xor_sync(0xffffffffu, count, o);
-        need += __shfl_xor_sync(0xffffffffu, need, o);
-      }
-      row = count;
-      if (row >= a.rows || __any_sync(0xffffffffu, descend)) return;     // (tokens behind the last offset)
-      r = plan_row(a, row);
-      first = first_of(a, row);
-      next = a.offsets[row + 1];
-      got = pages_got(r, avail, need);
-      before = int(min(need, avail));
-    }
-    const int64_t pos = r.held + (t - first);
-    if (t < first || pos >= tokens_kept(r, got, a.p.page_size)) continue;
-    const int column = int(pos / a.p.page_size), slot = int(pos - int64_t(column) * a.p.page_size);
-    int page;
-    if (column < r.have) {
-      if (column >= a.width) continue;
-      page = a.table[int64_t(row) * a.width + column];
-    } else {
-      page = a.free_pages[begin + before + column - r.have];
-      if (slot == 0 && lane == 0) a.table[int64_t(row) * a.width + column] = page;
-    }
-    if (page < 0 || page >= a.p.pages) continue;
-    if constexpr (kBits != 0) {
-      quantize_token<kBits, T>(a, t, page, slot);
-      continue;
-    }
-    uint4* kd = a.p.k + page * a.p.ks[0] + slot * a.p.ks[2];
-    uint4* vd = a.p.v + page * a.p.vs[0] + slot * a.p.vs[2];
-    const uint4* kx = a.k + t * a.ks[0];
-    const uint4* vx = a.v + t * a.vs[0];
-    const int n = a.p.heads * a.p.words;
-    for (int w0 = lane; w0 < n; w0 += 128) {
-      uint4 kw[4], vw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int w = w0 + 32 * i, h = w / a.p.words, c = w - h * a.p.words;
-        if (w < n) {
-          kw[i] = __ldg(kx + h * a.ks[1] + c);
-          vw[i] = __ldg(vx + h * a.vs[1] + c);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int w = w0 + 32 * i, h = w / a.p.words, c = w - h * a.p.words;
-        if (w < n) {
-          kd[h * a.p.ks[1] + c] = kw[i];
-          vd[h * a.p.vs[1] + c] = vw[i];
-        }
-      }
-    }
-  }
+  const int t0 = int(min((int64_t(blockIdx.x - 1) * (kThreads / 32) + warp) * a.tokens_per_warp, int64_t(a.tokens)));
+  const int t1 = t0 + min(a.tokens_per_warp, a.tokens - t0);
+  if constexpr (kBits == 0) append_tokens<Copier>(a, begin, avail, t0, t1);
+  else if (a.steps.groups == 4) append_tokens<Quantizer<kBits, T, 4>>(a, begin, avail, t0, t1);
+  else if (a.steps.groups == 2) append_tokens<Quantizer<kBits, T, 2>>(a, begin, avail, t0, t1);
+  else append_tokens<Quantizer<kBits, T, 0>>(a, begin, avail, t0, t1);
 }
 
 // ---- fork and compact -----------------------------------------------------------------------------------------------------
@@ -632,7 +647,19 @@ int append(const nb200_cache_params* p, const nb200_cache_steps* steps, const ch
     a.ks[i] = p->new_k_stride[i] / vec;
     a.vs[i] = p->new_v_stride[i] / vec;
   }
-  a.tokens = p->tokens;
+  a.tokens = int(p->tokens);
+  a.capacity = int(std::min<int64_t>(int64_t(p->width) * p->pages.page_size, NB200_CACHE_MOST_TOKENS));
+  if (steps) {
+    bool near = true;
+    auto fits = [&](int64_t stride) { near = near && stride <= 0x7fffffff && stride >= -0x7fffffff; return int(stride); };
+    const int groups = p->pages.head_dim / kGroup;
+    for (int i = 0; i < 3; ++i) {
+      a.codes_stride[0][i] = fits(a.p.ks[i]); a.codes_stride[1][i] = fits(a.p.vs[i]);
+      a.steps_stride[0][i] = fits(steps->k_stride[i] / groups); a.steps_stride[1][i] = fits(steps->v_stride[i] / groups);
+    }
+    for (int i = 0; i < 2; ++i) { a.from_stride[0][i] = fits(a.ks[i]); a.from_stride[1][i] = fits(a.vs[i]); }
+    if (!near) { set_error("%s: a stride of the pages or tokens is 2^31 words of 16 bytes, or rows of steps, or more", what); return NB200_ERR_UNSUPPORTED; }
+  }
   // one token per warp while that does not fill the GPU's warps; then two, which share a sequence's search (33 k tokens of bf16,
   // 8 heads of 128: one 55.9 us, two 51.4, four 53.9, eight 60.2)
   a.tokens_per_warp = p->tokens < 148 * 64 ? 1 : 2;

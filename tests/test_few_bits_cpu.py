@@ -53,6 +53,46 @@ def test_the_norm_s_gradient_refuses(change):
     assert _cabi.last_error().startswith("rms_norm_bwd")
 
 
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3)] + \
+        [(n, C.c_int32) for n in ("pages", "heads", "page_size", "head_dim", "dtype", "reserved")]
+
+
+class _Cache(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("pages", _Pages)] + [(n, C.c_void_p) for n in ("table", "lengths", "free_pages", "free_range")] + \
+        [("rows", C.c_int32), ("width", C.c_int32)] + \
+        [(n, C.c_void_p) for n in ("new_table", "new_lengths", "new_free_pages", "new_free_range", "shortfall", "new_k", "new_v")] + \
+        [("new_k_stride", C.c_int64 * 2), ("new_v_stride", C.c_int64 * 2), ("offsets", C.c_void_p), ("tokens", C.c_int64), ("parents", C.c_void_p),
+         ("finished", C.c_void_p), ("new_rows", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class _Steps(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("bits", C.c_int32), ("reserved", C.c_int32)]
+
+
+class _Quantized(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("cache", _Cache), ("steps", _Steps)]
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(bits=5), "INVALID"), (dict(rows=0), "INVALID"), (dict(tokens=-1), "INVALID"), (dict(tokens=1 << 31), "INVALID"), (dict(offsets=None), "INVALID"),
+    (dict(steps=None), "INVALID"), (dict(head_dim=80), "UNSUPPORTED"), (dict(codes=264), "ALIGNMENT"), (dict(steps=260), "ALIGNMENT"), (dict(new_k=264), "ALIGNMENT"),
+    (dict(token_stride=12), "ALIGNMENT"), (dict(slot_stride=40), "ALIGNMENT"), (dict(step_stride=3), "ALIGNMENT"),
+    (dict(token_stride=1 << 34), "UNSUPPORTED"), (dict(slot_stride=1 << 35), "UNSUPPORTED"), (dict(step_stride=1 << 32), "UNSUPPORTED")])
+def test_appending_refuses(change, code):
+    from nitrix_b200 import _cabi
+
+    c = {**dict(bits=4, rows=1, tokens=2, offsets=256, steps=256, head_dim=64, codes=256, new_k=256, token_stride=128, slot_stride=32, step_stride=2), **change}
+    pages = _Pages(k=c["codes"], v=256, k_stride=(512, 256, c["slot_stride"]), v_stride=(512, 256, 32), pages=4, heads=2, page_size=8, head_dim=c["head_dim"], dtype=1)
+    cache = _Cache(struct_size=C.sizeof(_Cache), pages=pages, rows=c["rows"], width=3, new_k_stride=(c["token_stride"], 64), new_v_stride=(128, 64), tokens=c["tokens"],
+                   offsets=c["offsets"], new_k=c["new_k"], new_v=256,
+                   **{n: 256 for n in ("table", "lengths", "free_pages", "free_range", "new_lengths", "new_free_range", "shortfall")})
+    steps = _Steps(k=c["steps"], v=256, k_stride=(32, 16, c["step_stride"]), v_stride=(32, 16, 2), bits=c["bits"])
+    p = _Quantized(struct_size=C.sizeof(_Quantized), cache=cache, steps=steps)
+    assert _cabi.lib().nb200_cache_append_quantized(C.byref(p), None) == getattr(_cabi, "ERR_" + code), _cabi.last_error()
+    assert "cache_append_quantized" in _cabi.last_error()
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="there is a GPU")
 def test_there_is_no_host_path():
     from nitrix_b200 import NitrixBackendError
