@@ -161,7 +161,7 @@ typedef struct nb200_cache_read_params {
   int32_t rows, width;
   const int32_t* offsets;    /* (rows + 1) */
   const int32_t* starts;     /* (rows), or NULL: zeros */
-  void* out_k;
+  void* out_k;               /* on 16-byte boundaries; fp32 from codes: on 32-byte ones */
   void* out_v;
   int64_t tokens;
 } nb200_cache_read_params;

@@ -5,7 +5,7 @@
 // and one or two 16-byte words of the result, of each group of a row of 64 or 128, whose codes lie side by side.
 //
 // 69 k tokens of 8 heads of 128 from 4 bits into bf16, 356 MB in all: 64 us (5.6 TB/s).  By single groups, with two loads of 16 bits for
-// 8 codes, 90.
+// 8 codes, 90.  34 k tokens into fp32, 317 MB: 56 us (5.7 TB/s), of 8 bits 62; with two stores for a lane's 8 elements 96 and 114.
 #include <type_traits>
 
 #include "cache_codes.cuh"
@@ -39,67 +39,13 @@ struct ReadArgs {
 template <typename T>
 __device__ __forceinline__ void store8(uint4* p, const float2 (&x)[4]) {
   if constexpr (sizeof(T) == 4) {
-    p[0] = make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
-    p[1] = make_uint4(__float_as_uint(x[2].x), __float_as_uint(x[2].y), __float_as_uint(x[3].x), __float_as_uint(x[3].y));
+    // (a whole sector at once)
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0].x), "f"(x[0].y), "f"(x[1].x), "f"(x[1].y), "f"(x[2].x), "f"(x[2].y),
+                 "f"(x[3].x), "f"(x[3].y)
+                 : "memory");
   } else {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     p[0] = make_uint4(tc::pack2<kBf16>(x[0].x, x[0].y), tc::pack2<kBf16>(x[1].x, x[1].y), tc::pack2<kBf16>(x[2].x, x[2].y), tc::pack2<kBf16>(x[3].x, x[3].y));
-  }
-}
-
-struct TokenRows {
-  const uint8_t* codes[2];
-  const uint16_t* steps[2];
-  int64_t codes_head[2], steps_head[2];      // from one head to the next
-  uint4* to[2];
-};
-
-// A token's values, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of them, whose codes lie side by
-// side; otherwise, for any number of groups, 8 elements.
-template <int kBits, typename T, int kGroups>
-__device__ __forceinline__ void read_token(const ReadArgs& a, const TokenRows& at) {
-  constexpr int kWords = int(sizeof(T)) / 2, kEach = kGroups ? kGroups : 1;
-  const int units = kGroups ? 4 : a.row, n = a.heads * units;
-  for (int w = threadIdx.x & 31; w < n; w += 32) {
-    const int h = w / units, c = w - h * units;
-    const uint8_t* rows[2] = {at.codes[0] + h * at.codes_head[0], at.codes[1] + h * at.codes_head[1]};
-    const uint16_t* steps[2] = {at.steps[0] + h * at.steps_head[0], at.steps[1] + h * at.steps_head[1]};
-    const int64_t to = (int64_t(h) * a.row + c) * kWords;
-    float2 x[4];
-    if constexpr (kGroups > 0) {
-      constexpr int nw = kGroups * kBits / 4;
-      uint32_t codes[2][nw], s[2][kGroups / 2];
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        load_words(codes[which], rows[which] + c * nw * 4);
-        load_words(s[which], steps[which]);
-      }
-#pragma unroll
-      for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int g = 0; g < kEach; ++g) {
-          const float step = __half2float(__ushort_as_half(uint16_t(g % 2 ? s[which][g / 2] >> 16 : s[which][g / 2])));
-          if constexpr (kBits == 4) values_of<4>(__byte_perm(codes[which][g / 2], codes[which][nw / 2 + g / 2], g % 2 ? 0x7632 : 0x5410), 0u, step, x);
-          else values_of<8>(codes[which][g], codes[which][nw / 2 + g], step, x);
-          store8<T>(at.to[which] + to + g * 4 * kWords, x);
-        }
-    } else {
-      const int groups = a.row / 4, g = c >> 2, u = c & 3;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        uint32_t lo, hi = 0;
-        if constexpr (kBits == 4) {
-          const uint16_t* p = reinterpret_cast<const uint16_t*>(rows[which]) + 2 * u * groups + g;
-          lo = __ldg(p) | uint32_t(__ldg(p + groups)) << 16;
-        } else {
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(rows[which]) + 2 * u * groups + g;
-          lo = __ldg(p);
-          hi = __ldg(p + groups);
-        }
-        values_of<kBits>(lo, hi, __half2float(__ushort_as_half(__ldg(steps[which] + g))), x);
-        store8<T>(at.to[which] + to, x);
-      }
-    }
   }
 }
 
@@ -124,52 +70,115 @@ __device__ __forceinline__ Slot slot_of(const ReadArgs& a, int64_t t, int row) {
   return Slot{__ldg(a.table + int64_t(row) * a.width + column), int(at) - column * a.page_size};
 }
 
-// A token's rows from a slot of a page, or zeros.
-template <int kBits, typename T>
-__device__ __forceinline__ void read_slot(const ReadArgs& a, int64_t t, int page, int slot, int lane) {
-  constexpr int kWords = kBits == 0 ? 1 : int(sizeof(T)) / 2;
-  const int n = a.heads * a.row;
-  uint4* ok = a.out_k + t * n * kWords;
-  uint4* ov = a.out_v + t * n * kWords;
-  if (page < 0 || page >= a.pages) {
-    for (int i = lane; i < n * kWords; i += 32) ok[i] = ov[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const uint8_t* kp = a.k + page * a.ks[0] + slot * a.ks[2];
-  const uint8_t* vp = a.v + page * a.vs[0] + slot * a.vs[2];
-  if constexpr (kBits == 0) {
-    for (int i = lane; i < n; i += 32) {
-      const int h = i / a.row, c = i - h * a.row;
-      const uint4 kw = __ldg(reinterpret_cast<const uint4*>(kp + h * a.ks[1]) + c), vw = __ldg(reinterpret_cast<const uint4*>(vp + h * a.vs[1]) + c);
-      ok[i] = kw;
-      ov[i] = vw;
+// The rows of a token's slot.
+struct Rows {
+  const uint8_t* codes[2];
+  const uint16_t* steps[2];
+  __device__ __forceinline__ Rows(const ReadArgs& a, Slot at)
+      : codes{a.k + at.page * a.ks[0] + at.slot * a.ks[2], a.v + at.page * a.vs[0] + at.slot * a.vs[2]},
+        steps{a.k_steps + at.page * a.kss[0] + at.slot * a.kss[2], a.v_steps + at.page * a.vss[0] + at.slot * a.vss[2]} {}
+};
+
+// A token's values, by a warp.  With kGroups, those of a head's row, a lane takes 8 elements of each of them, whose codes lie side by
+// side; otherwise, for any number of groups, 8 elements.  kBits 0: words are copied.
+template <int kBits, typename T, int kGroups>
+struct Token {
+  static constexpr int kWords = kBits == 0 ? 1 : int(sizeof(T)) / 2, kEach = kGroups ? kGroups : 1;
+  static constexpr int kCodeWords = kBits == 0 ? 4 : kGroups ? kGroups * kBits / 4 : kBits / 4, kStepWords = (kEach + 1) / 2;
+  uint32_t codes[2][kCodeWords], steps[2][kStepWords];      // of the lane's place in a row
+
+  __device__ __forceinline__ static int units(const ReadArgs& a) { return kGroups ? 4 : a.row; }
+  __device__ __forceinline__ void load(const ReadArgs& a, const Rows& rows, int w) {
+    const int h = w / units(a), c = w - h * units(a);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const uint8_t* row = rows.codes[which] + h * (which ? a.vs : a.ks)[1];
+      if constexpr (kBits == 0) {
+        load_words(codes[which], row + c * 16);
+        continue;
+      }
+      const uint16_t* step = rows.steps[which] + h * (which ? a.vss : a.kss)[1];
+      if constexpr (kGroups > 0) {
+        load_words(codes[which], row + c * kCodeWords * 4);
+        load_words(steps[which], step);
+      } else {
+        const int groups = a.row / 4, g = c >> 2, u = c & 3;
+        if constexpr (kBits == 4) {
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + 2 * u * groups + g;
+          codes[which][0] = __ldg(p) | uint32_t(__ldg(p + groups)) << 16;
+        } else {
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + 2 * u * groups + g;
+          codes[which][0] = __ldg(p);
+          codes[which][kCodeWords - 1] = __ldg(p + groups);
+        }
+        steps[which][0] = __ldg(step + g);
+      }
     }
-  } else {
-    const TokenRows at{{kp, vp}, {a.k_steps + page * a.kss[0] + slot * a.kss[2], a.v_steps + page * a.vss[0] + slot * a.vss[2]},
-                       {a.ks[1], a.vs[1]}, {a.kss[1], a.vss[1]}, {ok, ov}};
-    if (a.row == 16) read_token<kBits, T, 4>(a, at);
-    else if (a.row == 8) read_token<kBits, T, 2>(a, at);
-    else read_token<kBits, T, 0>(a, at);
+  }
+  __device__ __forceinline__ void store(const ReadArgs& a, int64_t t, int w) const {
+    const int h = w / units(a), c = w - h * units(a);
+    const int64_t to = ((t * a.heads + h) * a.row + c) * kWords;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      uint4* out = (which ? a.out_v : a.out_k) + to;
+      if constexpr (kBits == 0) {
+        out[0] = make_uint4(codes[which][0], codes[which][1], codes[which][2], codes[which][3]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < kEach; ++g) {
+          constexpr int half = kCodeWords / 2;
+          const float step = __half2float(__ushort_as_half(uint16_t(g % 2 ? steps[which][g / 2] >> 16 : steps[which][g / 2])));
+          float2 x[4];
+          if constexpr (kBits == 8) values_of<8>(codes[which][g], codes[which][half + g], step, x);
+          else if constexpr (kGroups == 0) values_of<4>(codes[which][0], 0u, step, x);
+          else values_of<4>(__byte_perm(codes[which][g / 2], codes[which][half + g / 2], g % 2 ? 0x7632 : 0x5410), 0u, step, x);
+          store8<T>(out + g * 4 * kWords, x);
+        }
+      }
+    }
+  }
+};
+
+// Tokens t .. t_end, by a warp; the next one's place is on its way while this one's rows are.  (The next one's first words as well: 68
+// us instead of 64 for 69 k tokens in 4 bits, bf16, 8 heads of 128.)
+template <typename T>
+__device__ __forceinline__ void read_tokens(const ReadArgs& a, int64_t t, int64_t t_end) {
+  const int lane = threadIdx.x & 31, n = a.heads * T::units(a);
+  int row = row_of(a, t, 0, a.rows);
+  Slot at = slot_of(a, t, row);
+  for (;; ++t) {
+    const Slot here = at;
+    const bool more = t + 1 < t_end;
+    if (more) {
+      while (row < a.rows && int64_t(__ldg(a.offsets + row + 1)) <= t + 1) ++row;
+      at = slot_of(a, t + 1, row);
+    }
+    if (here.page < 0 || here.page >= a.pages) {
+      const int words = a.heads * a.row * T::kWords;
+      for (int i = lane; i < words; i += 32) a.out_k[t * words + i] = a.out_v[t * words + i] = make_uint4(0, 0, 0, 0);
+    } else {
+      const Rows rows(a, here);
+      for (int w = lane; w < n; w += 32) {
+        T token;
+        token.load(a, rows, w);
+        token.store(a, t, w);
+      }
+    }
+    if (!more) return;
   }
 }
 
 // kBits 0: words are copied; otherwise T is the type of the result.
-template <int kBits, typename T>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) {
-  const int lane = threadIdx.x & 31;
-  int64_t t = (int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * a.tokens_per_warp;
+template <int kBits, typename T, int kGroups>
+__global__ void __launch_bounds__(kThreads, kBits && sizeof(T) == 4 ? 3 : 4) cache_read_kernel(const ReadArgs a) {
+  const int64_t t = (int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * a.tokens_per_warp;
   const int64_t t_end = min(t + a.tokens_per_warp, a.tokens);
-  if (t >= t_end) return;
-  int row = row_of(a, t, 0, a.rows);
-  Slot at = slot_of(a, t, row);
-  for (; t < t_end; ++t) {
-    const Slot here = at;
-    if (t + 1 < t_end) {      // (the next token's place is on its way while this one's rows are)
-      while (row < a.rows && int64_t(__ldg(a.offsets + row + 1)) <= t + 1) ++row;
-      at = slot_of(a, t + 1, row);
-    }
-    read_slot<kBits, T>(a, t, here.page, here.slot, lane);
-  }
+  if (t < t_end) read_tokens<Token<kBits, T, kGroups>>(a, t, t_end);
+}
+using Kernel = void (*)(ReadArgs);
+template <int kBits, typename T>
+Kernel kernel_of(int groups) {
+  return groups == 4 ? cache_read_kernel<kBits, T, 4> : groups == 2 ? cache_read_kernel<kBits, T, 2> : cache_read_kernel<kBits, T, 0>;
 }
 
 }  // namespace
@@ -198,7 +207,8 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   const int row = coded ? c.head_dim / 8 * p->steps.bits : c.head_dim * esz;      // bytes
   bool ok = row % 16 == 0 && aligned16(c.k) && aligned16(c.v) && aligned16(p->out_k) && aligned16(p->out_v);
   for (int i = 0; i < 3; ++i) ok = ok && c.k_stride[i] * esz % 16 == 0 && c.v_stride[i] * esz % 16 == 0;
-  if (!ok) { set_error("%s: rows must begin on 16-byte boundaries", what); return NB200_ERR_ALIGNMENT; }
+  if (coded && c.dtype == NB200_F32) ok = ok && (reinterpret_cast<uintptr_t>(p->out_k) | reinterpret_cast<uintptr_t>(p->out_v)) % 32 == 0;
+  if (!ok) { set_error("%s: rows must begin on 16-byte boundaries (fp32 from codes: out_k and out_v on 32-byte ones)", what); return NB200_ERR_ALIGNMENT; }
   if (int64_t(c.heads) * c.head_dim > 0x3fffffff) { set_error("%s: rows too large", what); return NB200_ERR_UNSUPPORTED; }
   ReadArgs a{};
   a.k = static_cast<const uint8_t*>(c.k); a.v = static_cast<const uint8_t*>(c.v);
@@ -213,12 +223,13 @@ extern "C" NB200_API int nb200_cache_read(const nb200_cache_read_params* p, void
   a.rows = p->rows; a.width = p->width;
   a.out_k = static_cast<uint4*>(p->out_k); a.out_v = static_cast<uint4*>(p->out_v);
   a.tokens = p->tokens;
-  void (*kernel)(ReadArgs) = cache_read_kernel<0, uint4>;
+  Kernel kernel = cache_read_kernel<0, uint4, 0>;
   if (coded) {
     const bool four = p->steps.bits == 4;
-    kernel = c.dtype == NB200_F32    ? four ? cache_read_kernel<4, float> : cache_read_kernel<8, float>
-             : c.dtype == NB200_BF16 ? four ? cache_read_kernel<4, __nv_bfloat16> : cache_read_kernel<8, __nv_bfloat16>
-             : four                  ? cache_read_kernel<4, __half> : cache_read_kernel<8, __half>;
+    const int groups = c.head_dim / kGroup;
+    kernel = c.dtype == NB200_F32    ? four ? kernel_of<4, float>(groups) : kernel_of<8, float>(groups)
+             : c.dtype == NB200_BF16 ? four ? kernel_of<4, __nv_bfloat16>(groups) : kernel_of<8, __nv_bfloat16>(groups)
+             : four                  ? kernel_of<4, __half>(groups) : kernel_of<8, __half>(groups);
   }
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   prof_call_begin(st);

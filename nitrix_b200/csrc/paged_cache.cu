@@ -14,7 +14,8 @@
 // Tokens for a cache in few bits are quantised on the way (cache_codes.cuh): 34 k tokens of bf16, 8 heads of 128, into 4 bits in 42 us, 4.3
 // TB/s of what is read and written; two thirds of the issue slots are busy, with 47 instructions for a lane's 8 elements and some 300 for
 // a token's place.  On the way: one group a lane and 16-bit stores of codes 78 us, steps worked out by every lane of a group 52, three
-// CTAs per SM without spills 49, places in 64 bits and elements asked for when the place is known 45; four tokens a warp 46.
+// CTAs per SM without spills 49, places in 64 bits and elements asked for when the place is known 45; four tokens a warp 46.  The same in
+// fp32: 49 (6.4 TB/s); 78 with two CTAs per SM and loads past L1, which holds the other half of a sector until the second load.
 #include <algorithm>
 
 #include "cache_codes.cuh"
@@ -122,7 +123,7 @@ struct Quantizer {
 #pragma unroll
       for (int g = 0; g < kEach; ++g)
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) x[which][g][i] = sm100::ldg_no_allocate(from + g * 4 * kWords + i);
+        for (int i = 0; i < kWords; ++i) x[which][g][i] = kWords == 1 ? sm100::ldg_no_allocate(from + g * 4 * kWords + i) : __ldg(from + g * 4 * kWords + i);
     }
   }
   __device__ __forceinline__ void load(const AppendArgs& a, int t) { load(a, t, Turn(a, 0)); }
@@ -237,7 +238,7 @@ __device__ __forceinline__ void append_tokens(const AppendArgs& a, int begin, in
 
 // kBits 0: the tokens' rows are copied; otherwise T is their type.
 template <int kBits, typename T>
-__global__ void __launch_bounds__(kThreads, kBits == 0 || sizeof(T) == 4 ? 1 : 4) cache_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, kBits == 0 || sizeof(T) == 4 ? 3 : 4) cache_append_kernel(const AppendArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int begin, end;
   free_bounds(a.free_range, a.p.pages, &begin, &end);

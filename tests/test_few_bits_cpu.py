@@ -93,6 +93,27 @@ def test_appending_refuses(change, code):
     assert "cache_append_quantized" in _cabi.last_error()
 
 
+class _Read(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("pages", _Pages), ("steps", _Steps), ("table", C.c_void_p), ("lengths", C.c_void_p), ("rows", C.c_int32),
+                ("width", C.c_int32)] + [(n, C.c_void_p) for n in ("offsets", "starts", "out_k", "out_v")] + [("tokens", C.c_int64)]
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(bits=3), "INVALID"), (dict(dtype=7), "INVALID"), (dict(tokens=1 << 31), "INVALID"), (dict(offsets=None), "INVALID"), (dict(out_v=None), "INVALID"),
+    (dict(head_dim=48), "UNSUPPORTED"), (dict(codes=264), "ALIGNMENT"), (dict(out_v=264), "ALIGNMENT"), (dict(dtype=0, out_v=272), "ALIGNMENT"),
+    (dict(heads=1 << 30), "UNSUPPORTED")])
+def test_reading_refuses(change, code):
+    from nitrix_b200 import _cabi
+
+    c = {**dict(bits=4, dtype=1, tokens=2, offsets=256, head_dim=64, heads=2, codes=256, out_v=256), **change}
+    pages = _Pages(k=c["codes"], v=256, k_stride=(512, 256, 32), v_stride=(512, 256, 32), pages=4, heads=c["heads"], page_size=8, head_dim=c["head_dim"], dtype=c["dtype"])
+    steps = _Steps(k=256, v=256, k_stride=(32, 16, 2), v_stride=(32, 16, 2), bits=c["bits"])
+    p = _Read(struct_size=C.sizeof(_Read), pages=pages, steps=steps, table=256, lengths=256, rows=1, width=3, offsets=c["offsets"], out_k=256, out_v=c["out_v"],
+              tokens=c["tokens"])
+    assert _cabi.lib().nb200_cache_read(C.byref(p), None) == getattr(_cabi, "ERR_" + code), _cabi.last_error()
+    assert "cache_read" in _cabi.last_error()
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="there is a GPU")
 def test_there_is_no_host_path():
     from nitrix_b200 import NitrixBackendError
