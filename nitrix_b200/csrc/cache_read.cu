@@ -4,8 +4,8 @@
 // bisection of the offsets, its page from the table; then a lane eight elements at a time, which are two parts of a row of codes
 // and one or two 16-byte words of the result, of each group of a row of 64 or 128, whose codes lie side by side.
 //
-// 69 k tokens of 8 heads of 128 from 4 bits into bf16, 356 MB in all: 64 us (5.6 TB/s).  By single groups, with two loads of 16 bits for
-// 8 codes, 90.  34 k tokens into fp32, 317 MB: 56 us (5.7 TB/s), of 8 bits 62; with two stores for a lane's 8 elements 96 and 114.
+// 69 k tokens of 8 heads of 128 from 4 bits into bf16, 356 MB in all: 61 us (5.8 TB/s).  By single groups, with two loads of 16 bits for
+// 8 codes, 90.  34 k tokens into fp32, 317 MB: 57 us (5.6 TB/s), of 8 bits 63; with two stores for a lane's 8 elements 96 and 114.
 #include <type_traits>
 
 #include "cache_codes.cuh"
