@@ -45,7 +45,7 @@ typedef struct nb200_rms_norm_params {
   void* workspace;         /* backward with dweight: nb200_rms_norm_workspace_bytes; 16-byte aligned */
   size_t workspace_bytes;
   int64_t rows;
-  int32_t channels;
+  int32_t channels;        /* at most 2^30 */
   int32_t dtype;           /* nb200_dtype of x, residual, y, sum, dy, dsum, dx */
   int32_t weight_dtype;    /* of weight and dweight: dtype or NB200_F32 */
   int32_t group;           /* with scales: 0, 32, 64 or 128 channels; a group divides the channels */

@@ -683,7 +683,7 @@ struct RmsNormRule : torch::autograd::Function<RmsNormRule> {
 void check_rms_operands(const char* what, const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight) {
   check_float(what, "x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, what, ": x must have a channel at least; got shape ", x.sizes());
-  TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), what, ": ", x.size(-1), " channels do not fit 32 bits");
+  TORCH_CHECK_VALUE(x.size(-1) <= int64_t(1) << 30, what, ": ", x.size(-1), " channels, at most 2^30");
   if (residual) {
     TORCH_CHECK_TYPE(residual->scalar_type() == x.scalar_type() && residual->device() == x.device(), what, ": residual must be ", x.scalar_type(), " on ",
                      x.device(), "; got ", residual->scalar_type(), " on ", residual->device());

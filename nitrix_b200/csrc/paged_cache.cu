@@ -12,10 +12,10 @@
 // a fork of 64 rows 10.5 in a captured graph, 15 and 21 where the host makes the calls.
 //
 // Tokens for a cache in few bits are quantised on the way (cache_codes.cuh): 34 k tokens of bf16, 8 heads of 128, into 4 bits in 42 us (39
-// with a cold cache alone), 4.3 TB/s of what is read and written; two thirds of the issue slots are busy, with 47 instructions for a lane's 8 elements and some 300 for
-// a token's place.  On the way: one group a lane and 16-bit stores of codes 78 us, steps worked out by every lane of a group 52, three
-// CTAs per SM without spills 49, places in 64 bits and elements asked for when the place is known 45; four tokens a warp 46.  The same in
-// fp32: 49 (6.4 TB/s); 78 with two CTAs per SM and loads past L1, which holds the other half of a sector until the second load.
+// by itself), 4.3 TB/s of what is read and written; two thirds of the issue slots are busy, with 47 instructions for a lane's 8 elements
+// and some 300 for a token's place.  On the way: one group a lane and 16-bit stores of codes 78 us, steps worked out by every lane of a
+// group 52, three CTAs per SM without spills 49, places in 64 bits and elements asked for when the place is known 45; four tokens a warp
+// 46.  The same in fp32: 49 (6.4 TB/s); 78 with two CTAs per SM and loads past L1, which holds a sector's other half for the second load.
 #include <algorithm>
 
 #include "cache_codes.cuh"

@@ -560,7 +560,7 @@ constexpr int least_per(bool vec) { return vec ? 1 : 4; }
 // one of 512 90; 1024 threads for 8192 channels 89, two chunks of 512 78), the forward two (93 us either way, and fewer shuffles).
 Shape shape_of(int C, int esz, bool vec, bool backward) {
   Shape s{vec, 0, 0, 0};
-  const int chunks = vec ? C * esz / 16 : C, least = least_per(vec);
+  const int chunks = vec ? C / (16 / esz) : C, least = least_per(vec);
   for (int per = backward ? least : 2 * least; per <= (backward ? 4 : 8) * least; per *= 2) {
     const int threads = (chunks + per - 1) / per;
     if (threads > 512) continue;
@@ -586,6 +586,7 @@ int check(const nb200_rms_norm_params* p, const char* what) {
   if (p->dtype != NB200_F32 && p->dtype != NB200_BF16 && p->dtype != NB200_F16) { set_error("%s: bad dtype", what); return NB200_ERR_INVALID; }
   if (p->weight_dtype != p->dtype && p->weight_dtype != NB200_F32) { set_error("%s: the weight must be of the operands' dtype or fp32", what); return NB200_ERR_INVALID; }
   if (p->rows < 0 || p->channels <= 0) { set_error("%s: bad extents", what); return NB200_ERR_INVALID; }
+  if (p->channels > 1 << 30) { set_error("%s: %d channels, at most 2^30", what, p->channels); return NB200_ERR_UNSUPPORTED; }      // (counted in 32 bits)
   if (p->rows > 0x7fffffff) { set_error("%s: %lld rows, at most 2^31 - 1", what, static_cast<long long>(p->rows)); return NB200_ERR_UNSUPPORTED; }
   return NB200_OK;
 }

@@ -36,7 +36,7 @@ def _rms(**kw):
     return p
 
 
-@pytest.mark.parametrize("change", [dict(dtype=7), dict(weight_dtype=2), dict(rows=-1), dict(channels=0), dict(rows=1 << 32), dict(x=None), dict(y=None),
+@pytest.mark.parametrize("change", [dict(dtype=7), dict(weight_dtype=2), dict(rows=-1), dict(channels=0), dict(channels=(1 << 30) + 1), dict(rows=1 << 32), dict(x=None), dict(y=None),
                                     dict(residual=256), dict(scales=256, group=48), dict(scales=256, group=128), dict(scales=256, group=32, x=264)])
 def test_the_norm_refuses(change):
     from nitrix_b200 import _cabi

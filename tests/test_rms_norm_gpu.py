@@ -360,3 +360,24 @@ def test_more_than_2_to_the_31_elements():
     dy[-50:].normal_()
     (da,), (db,) = torch.autograd.grad(rms_norm(a, w), [a], dy), torch.autograd.grad(rms_norm(b, w), [b], dy[-50:])
     assert torch.equal(da[-50:], db) and not bool(da[:1000].any())
+
+
+@pytest.mark.parametrize("dtype,C", [(torch.float32, 1 << 29), (torch.bfloat16, 1 << 30)])
+def test_rows_of_2_to_the_31_bytes(dtype, C):
+    """Of ones of either sign, whose squares' sum is exact: the norm is the row times (1 + eps)^-1/2, within 2^-20."""
+    from nitrix_b200.nn import rms_norm
+
+    x = torch.empty(1, C, dtype=dtype, device="cuda").bernoulli_(0.5).mul_(2).sub_(1)
+    y = rms_norm(x)
+    assert float((y - x).abs().max()) <= 2.0 ** -20 + HALF[dtype]
+    del y
+    with pytest.raises(ValueError, match="2\\^30"):
+        rms_norm(torch.empty(0, (1 << 30) + 1, dtype=dtype, device="cuda"))
+    if dtype == torch.float32:
+        # a gradient in the last 8 columns alone: mean(g n) is 8 / C, which is what the other columns get, against their sign
+        dy = torch.zeros_like(x)
+        dy[:, -8:] = x[:, -8:]
+        x.requires_grad_(True)
+        (dx,) = torch.autograd.grad(rms_norm(x), [x], dy)
+        dx *= x.detach()
+        assert float((dx[:, :-8] * (C / 8) + 1).abs().max()) < 2.0 ** -18 and float((dx[:, -8:] - 1).abs().max()) < 2.0 ** -18
