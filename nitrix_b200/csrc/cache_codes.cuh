@@ -240,6 +240,7 @@ int check_steps(const nb200_cache_pages& c, const nb200_cache_steps& s, const ch
   if (s.bits != 4 && s.bits != 8) { set_error("%s: codes of %d bits, 4 or 8 are possible", what, s.bits); return NB200_ERR_INVALID; }
   if (c.pages && (!s.k || !s.v)) { set_error("%s: NULL steps", what); return NB200_ERR_INVALID; }
   if (c.head_dim % kGroup) { set_error("%s: head dim %d must be a multiple of %d", what, c.head_dim, kGroup); return NB200_ERR_UNSUPPORTED; }
+  if (int64_t(c.heads) * c.head_dim > 0x3fffffff) { set_error("%s: rows too large", what); return NB200_ERR_UNSUPPORTED; }      // (counted in 32 bits)
   const int groups = c.head_dim / kGroup;
   bool ok = aligned16(s.k) && aligned16(s.v);
   for (int i = 0; i < 3; ++i) ok = ok && s.k_stride[i] % groups == 0 && s.v_stride[i] % groups == 0;

@@ -76,14 +76,14 @@ class _Quantized(C.Structure):
 
 @pytest.mark.parametrize("change,code", [
     (dict(bits=5), "INVALID"), (dict(rows=0), "INVALID"), (dict(tokens=-1), "INVALID"), (dict(tokens=1 << 31), "INVALID"), (dict(offsets=None), "INVALID"),
-    (dict(steps=None), "INVALID"), (dict(head_dim=80), "UNSUPPORTED"), (dict(codes=264), "ALIGNMENT"), (dict(steps=260), "ALIGNMENT"), (dict(new_k=264), "ALIGNMENT"),
+    (dict(steps=None), "INVALID"), (dict(head_dim=80), "UNSUPPORTED"), (dict(heads=1 << 25), "UNSUPPORTED"), (dict(codes=264), "ALIGNMENT"), (dict(steps=260), "ALIGNMENT"), (dict(new_k=264), "ALIGNMENT"),
     (dict(token_stride=12), "ALIGNMENT"), (dict(slot_stride=40), "ALIGNMENT"), (dict(step_stride=3), "ALIGNMENT"),
     (dict(token_stride=1 << 34), "UNSUPPORTED"), (dict(slot_stride=1 << 35), "UNSUPPORTED"), (dict(step_stride=1 << 32), "UNSUPPORTED")])
 def test_appending_refuses(change, code):
     from nitrix_b200 import _cabi
 
-    c = {**dict(bits=4, rows=1, tokens=2, offsets=256, steps=256, head_dim=64, codes=256, new_k=256, token_stride=128, slot_stride=32, step_stride=2), **change}
-    pages = _Pages(k=c["codes"], v=256, k_stride=(512, 256, c["slot_stride"]), v_stride=(512, 256, 32), pages=4, heads=2, page_size=8, head_dim=c["head_dim"], dtype=1)
+    c = {**dict(bits=4, heads=2, rows=1, tokens=2, offsets=256, steps=256, head_dim=64, codes=256, new_k=256, token_stride=128, slot_stride=32, step_stride=2), **change}
+    pages = _Pages(k=c["codes"], v=256, k_stride=(512, 256, c["slot_stride"]), v_stride=(512, 256, 32), pages=4, heads=c["heads"], page_size=8, head_dim=c["head_dim"], dtype=1)
     cache = _Cache(struct_size=C.sizeof(_Cache), pages=pages, rows=c["rows"], width=3, new_k_stride=(c["token_stride"], 64), new_v_stride=(128, 64), tokens=c["tokens"],
                    offsets=c["offsets"], new_k=c["new_k"], new_v=256,
                    **{n: 256 for n in ("table", "lengths", "free_pages", "free_range", "new_lengths", "new_free_range", "shortfall")})
