@@ -172,12 +172,14 @@ __device__ __forceinline__ float top_of(const float2 (&y)[kPairs], float top) {
     asm("{\n.reg .f32 a, b;\nabs.f32 a, %1;\nabs.f32 b, %2;\nmax.NaN.f32 a, a, b;\nmax.NaN.f32 %0, %0, a;\n}" : "+f"(top) : "f"(y[i].x), "f"(y[i].y));
   return top;
 }
-// The scale for a largest magnitude, and what the values are multiplied by (the reciprocal of a number of 2^-109 or more, good to 2^-23).
+// The scale for a largest magnitude, and what the values are multiplied by: 448 / top, from the reciprocal of the scale (2^-109 or more),
+// which is good to 2^-22, by one step of Newton's method; an infinity has a factor of zero, a NaN a NaN.
 __device__ __forceinline__ float scale_of(float top) { return top * (1.f / 448.f); }
-__device__ __forceinline__ float inverse_of(float scale) {
+__device__ __forceinline__ float inverse_of(float top, float scale) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
-  return r;
+  const float e = fmaf(-top, r, 448.f);
+  return e == e ? fmaf(r * (1.f / 448.f), e, r) : r;
 }
 // The same of a group of lanes' values; its first lane writes the scale.
 __device__ __forceinline__ float group_scale(float top, int lanes, float* scale, bool write) {
@@ -186,7 +188,7 @@ __device__ __forceinline__ float group_scale(float top, int lanes, float* scale,
     if (o < lanes) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float s = scale_of(top);
   if (write && (threadIdx.x & (lanes - 1)) == 0) *scale = s;
-  return inverse_of(s);
+  return inverse_of(top, s);
 }
 
 template <typename T, typename W, int kVec, int kPer, int kThreads, bool kEight>
@@ -256,9 +258,10 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
           output(p, f);
           top = top_of(f, top);
         }
-        const float scale = scale_of(over_row<max_nan>(top, tpr, red + (2 + turn) * kMaxWarps));
+        top = over_row<max_nan>(top, tpr, red + (2 + turn) * kMaxWarps);
+        const float scale = scale_of(top);
         if (tin == 0 && in_rows) a.scales[row] = scale;
-        inv = inverse_of(scale);
+        inv = inverse_of(top, scale);
       }
     }
 #pragma unroll
@@ -322,9 +325,10 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
         output(c, f);
         top = top_of(f, top);
       }
-      const float scale = scale_of(over_row<max_nan>(top, kWide, red + kMaxWarps));
+      top = over_row<max_nan>(top, kWide, red + kMaxWarps);
+      const float scale = scale_of(top);
       if (threadIdx.x == 0) a.scales[row] = scale;
-      inv = inverse_of(scale);
+      inv = inverse_of(top, scale);
     }
   }
   // (whole warps go round together: a group's lanes are in one)
