@@ -282,6 +282,22 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
 
 constexpr int kWide = 256;      // threads of a row that is not held
 
+// A sum over a thread's chunks of a row of any length, kPairs pairs each: fp32, folded into 64 bits every 64 terms.  (One by one in
+// fp32, 2^16 terms of one size are 2e-4 off.)  term(c, sum) adds the chunk at column c.
+template <int kPairs, int kVec, typename Term>
+__device__ __forceinline__ float long_sum(int C, Term term) {
+  constexpr int kStep = kWide * kVec;
+  double all = 0.0;
+  for (int c = threadIdx.x * kVec; c < C;) {
+    float2 sum = make_float2(0.f, 0.f);
+    const int end = min(C, c + 64 / kPairs * kStep);      // (2^30 + 2^17 at most)
+#pragma unroll 4
+    for (; c < end; c += kStep) term(c, sum);
+    all += double(sum.x) + double(sum.y);
+  }
+  return float(all);
+}
+
 // A row per CTA, read again for its output (and, for one scale of the row, for that).
 template <typename T, typename W, int kVec, bool kEight>
 __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
@@ -290,8 +306,7 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
   constexpr int kPairs = C::kPairs;
   const int64_t row = blockIdx.x, base = row * a.C;
   const T* x = static_cast<const T*>(a.x) + base;
-  float2 ss = make_float2(0.f, 0.f);
-  for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
+  const auto square = [&](int c, float2& sum) {
     C h = C::load_cached(x + c);
     float2 f[kPairs], g[kPairs];
     h.get(f);
@@ -304,9 +319,9 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
       h.get(f);
     }
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) ss = __ffma2_rn(f[i], f[i], ss);
-  }
-  const float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, kWide, red), a.inv_c, a.eps));
+    for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(f[i], f[i], sum);
+  };
+  const float s = rsqrtf(fmaf(over_row<add>(long_sum<kPairs, kVec>(a.C, square), kWide, red), a.inv_c, a.eps));
   if (threadIdx.x == 0 && a.rstd) a.rstd[row] = s;
   const T* h = a.r ? static_cast<const T*>(a.sum) + base : x;      // (every thread reads back what it has written itself)
   auto output = [&](int c, float2 (&f)[kPairs]) {
@@ -489,7 +504,6 @@ __global__ void __launch_bounds__(kWide) rms_bwd_wide_kernel(const RmsArgs a) {
   const int64_t row = blockIdx.x, base = row * a.C;
   const float rstd = a.rstd[row];
   const float2 s2 = make_float2(rstd, rstd);
-  float2 t2 = make_float2(0.f, 0.f);
   auto operands = [&](int c, float2 (&n)[kPairs], float2 (&g)[kPairs]) {      // n, and dy w
     float2 v[kPairs];
     Ch::load_cached(static_cast<const T*>(a.x) + base + c).get(n);
@@ -501,13 +515,13 @@ __global__ void __launch_bounds__(kWide) rms_bwd_wide_kernel(const RmsArgs a) {
       g[i] = __fmul2_rn(g[i], v[i]);
     }
   };
-  for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
+  const auto product = [&](int c, float2& sum) {
     float2 n[kPairs], g[kPairs];
     operands(c, n, g);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) t2 = __ffma2_rn(g[i], n[i], t2);
-  }
-  const float mean = over_row<add>(t2.x + t2.y, kWide, red) * a.inv_c;
+    for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(g[i], n[i], sum);
+  };
+  const float mean = over_row<add>(long_sum<kPairs, kVec>(a.C, product), kWide, red) * a.inv_c;
   for (int c = threadIdx.x * kVec; c < a.C; c += kWide * kVec) {
     float2 n[kPairs], g[kPairs], d[kPairs];
     operands(c, n, g);
