@@ -5,7 +5,7 @@
  *   nb200_rms_norm_fwd   y, or its e4m3 codes and their scales; with a residual also the sum of the two streams
  *   nb200_rms_norm_bwd   dx (the gradient of either stream) and dweight
  *
- * Per row of `channels` elements, in fp32 whatever the storage dtype:
+ * Per row of `channels` elements, in fp32 whatever the storage dtype (rows whose squares leave fp32, above or below, in fp64):
  *
  *   h = x + residual, rounded to the dtype (x without a residual);   rstd = (mean h^2 + eps)^-1/2;   y = h rstd weight
  *

@@ -45,6 +45,7 @@ struct RmsArgs {
   int group;        // channels of a scale; its power of two, where rows have several
   int group_shift;
   float eps, inv_c;
+  double eps64;     // (not flushed where it is one of fp32's smallest numbers)
 };
 
 // kVec consecutive elements as they lie in memory, and as pairs (one element: with a zero behind it).
@@ -128,6 +129,14 @@ __device__ __forceinline__ Chunk<W, kVec> weights(const void* w, int c, bool in)
   return C::of(ones);
 }
 
+// Elements times their row's factor, without a flush of small numbers: of rows of the largest numbers the factor is one of fp32's
+// smallest.
+__device__ __forceinline__ float2 times(float2 a, float factor) {
+  float2 c;
+  asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %4};\nmul.rn.f32x2 c, a, b;\nmov.b64 {%0, %1}, c;\n}" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(factor));
+  return c;
+}
+
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN on either side comes out
   float m;
@@ -151,6 +160,26 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* red) {
     if (warps & 1) v = op(v, red[first + warps - 1]);
   }
   return v;
+}
+
+// A row's factor where its squares leave fp32 or vanish from it: in 64 bits, by every warp of the row for itself.  (Infinities and NaN end
+// up here as well and give 0 and NaN, rows of zeros without an eps infinity.)
+constexpr float kMostFactor = 1125899906842624.f;     // 2^50: squares below 2^-126 are flushed, which a mean of 2^-100 does not feel
+__device__ __forceinline__ bool leaves_fp32(float factor) { return !(factor > 0.f && factor < kMostFactor); }
+template <typename T>
+__device__ __noinline__ float far_factor(const T* x, const T* r, int C, double eps) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int c = threadIdx.x & 31; c < C; c += 32) {
+    float h = to_f32<T>(x[c]);
+    if (r) h = to_f32<T>(from_f32<T>(h + to_f32<T>(r[c])));
+    sum += double(h) * double(h);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float s;      // (down to 2^-128 without a flush)
+  asm("cvt.rn.f32.f64 %0, %1;" : "=f"(s) : "d"(rsqrt(sum / C + eps)));
+  return s;
 }
 
 // codes of a chunk's values, each times `inv`
@@ -191,34 +220,113 @@ __device__ __forceinline__ float group_scale(float top, int lanes, float* scale,
   return inverse_of(top, s);
 }
 
+// The rows of a CTA, from `block` on, whose squares leave fp32: rms_fwd_kernel has left NaN in all that a warp writes of them.  Called behind
+// its loop, with arguments of its own, so that nothing is held for it meanwhile: as a call within the loop 105 us instead of 93 (16384 x 4096
+// bf16 with a residual), 194 instead of 152 (16384 x 8192 to e4m3).
+template <typename T, typename W, int kVec, bool kEight>
+__device__ __noinline__ void far_rows(const RmsArgs* pa, int tpr, int64_t block) {
+  const RmsArgs a = *pa;
+  using C = Chunk<T, kVec>;
+  constexpr int kPairs = C::kPairs;
+  const int groups = blockDim.x / tpr, mine = groups == 1 ? 0 : threadIdx.x / tpr, tin = threadIdx.x - mine * tpr, lane = threadIdx.x & 31;
+  const int step = tpr * kVec, own = tin * kVec;
+#pragma unroll 1
+  for (;; block += gridDim.x) {
+    const int64_t row = block * groups + mine, base = row * a.C;
+    if (row >= a.rows) return;
+    bool good = false;      // (a thread reads back what it has written itself)
+    if (own < a.C) {
+      if constexpr (kEight) good = (static_cast<const uint8_t*>(a.y)[base + own] & 0x7f) != 0x7f;
+      else good = to_f32<T>(static_cast<const T*>(a.y)[base + own]) == to_f32<T>(static_cast<const T*>(a.y)[base + own]);
+    }
+    if (own - lane * kVec >= a.C || __any_sync(0xffffffffu, good)) continue;
+    const T* x = static_cast<const T*>(a.x) + base;
+    const T* r = a.r ? static_cast<const T*>(a.r) + base : nullptr;
+    const float s = far_factor(x, r, a.C, a.eps64);
+    if (tin == 0 && a.rstd) a.rstd[row] = s;
+    auto output = [&](int c, float2 (&f)[kPairs]) {
+      float2 v[kPairs];
+      C::load_cached(x + c).get(f);
+      if (r) {
+        C::load_cached(r + c).get(v);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) f[i] = __fadd2_rn(f[i], v[i]);
+        C::of(f).get(f);
+      }
+      weights<W, kVec>(a.w, c, true).get(v);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(times(f[i], s), v[i]);
+    };
+    float inv = 0.f;
+    if constexpr (kEight) {
+      if (a.group == a.C) {
+        float top = kLeast;
+#pragma unroll 1
+        for (int c = lane * kVec; c < a.C; c += 32 * kVec) {
+          float2 f[kPairs];
+          output(c, f);
+          top = top_of(f, top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float scale = scale_of(top);
+        if (tin == 0) a.scales[row] = scale;
+        inv = inverse_of(top, scale);
+      }
+    }
+#pragma unroll 1
+    for (int c0 = own - lane * kVec; c0 < a.C; c0 += step) {
+      const int c = c0 + lane * kVec;
+      const bool in = c < a.C;
+      float2 f[kPairs];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) f[i] = make_float2(0.f, 0.f);
+      if (in) output(c, f);
+      if constexpr (kEight) {
+        if (a.group != a.C) inv = group_scale(top_of(f, kLeast), a.group / kVec, a.scales + ((base + c) >> a.group_shift), in);
+        if (in) store_codes<kVec>(static_cast<uint8_t*>(a.y) + base + c, f, inv);
+      } else {
+        if (in) C::of(f).store(static_cast<T*>(a.y) + base + c);
+      }
+    }
+  }
+}
+
 template <typename T, typename W, int kVec, int kPer, int kThreads, bool kEight>
-__global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 : 512) / kThreads) rms_fwd_kernel(const RmsArgs a, int tpr) {
+__global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 : 512) / kThreads) rms_fwd_kernel(const __grid_constant__ RmsArgs a, int tpr) {
   __shared__ __align__(16) float red[4 * kMaxWarps];
+  __shared__ uint8_t far[kMaxWarps];
   using C = Chunk<T, kVec>;
   constexpr int kPairs = C::kPairs;
   const int groups = blockDim.x / tpr, mine = groups == 1 ? 0 : threadIdx.x / tpr, tin = threadIdx.x - mine * tpr;
-  const int64_t blocks = (a.rows + groups - 1) / groups;
+  const unsigned rows = unsigned(a.rows), blocks = (rows + groups - 1) / groups;      // (counted in 32 bits: registers are what is short here)
   auto column = [&](int p) { return (p * tpr + tin) * kVec; };
   C nx[kPer], nr[kPer];
-  auto fetch = [&](int64_t block) {
-    const int64_t row = block * groups + mine;
-    const bool in_rows = block < blocks && row < a.rows;
+  auto fetch = [&](unsigned block) {
+    const unsigned row = block * groups + mine;
+    const bool in_rows = block < blocks && row < rows;
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
       const bool in = in_rows && column(p) < a.C;
-      const int64_t at = in ? row * a.C + column(p) : 0;
+      const int64_t at = in ? int64_t(row) * a.C + column(p) : 0;
       nx[p] = in ? C::load(static_cast<const T*>(a.x) + at) : C::zero();
       if (a.r) nr[p] = in ? C::load(static_cast<const T*>(a.r) + at) : C::zero();
     }
   };
   fetch(blockIdx.x);
+  // (fp32 with two chunks a thread has no registers for the weights beside the next row: 121 us held, 94 from L1, 8192 x 4096)
+  constexpr bool kHeld = !(sizeof(T) == 4 && kVec > 1 && kPer == 2);
   Chunk<W, kVec> w[kPer];
 #pragma unroll
-  for (int p = 0; p < kPer; ++p) w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
+  for (int p = 0; p < kPer; ++p)
+    if (kHeld) w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
   int turn = 0;
-  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
-    const int64_t row = block * groups + mine, base = row * a.C;
-    const bool in_rows = row < a.rows;
+  if ((threadIdx.x & 31) == 0) far[threadIdx.x >> 5] = 0;      // (of the warp: a flag in a register is one more than there are)
+  __syncwarp();
+  for (unsigned block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    const unsigned row = block * groups + mine;
+    const int64_t base = int64_t(row) * a.C;
+    const bool in_rows = row < rows;
     C h[kPer];
     float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
@@ -239,14 +347,19 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
       for (int i = 0; i < kPairs; ++i) ss = __ffma2_rn(f[i], f[i], ss);
     }
     fetch(block + gridDim.x);
-    const float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, tpr, red + turn * kMaxWarps), a.inv_c, a.eps));
+    float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, tpr, red + turn * kMaxWarps), a.inv_c, a.eps));
+    if (leaves_fp32(s)) {
+      far[threadIdx.x >> 5] = 1;
+      s = __uint_as_float(0x7fffffffu);
+    }
     if (tin == 0 && in_rows && a.rstd) a.rstd[row] = s;
     auto output = [&](int p, float2 (&f)[kPairs]) {
       float2 v[kPairs];
       h[p].get(f);
-      w[p].get(v);
+      if (kHeld) w[p].get(v);
+      else weights<W, kVec>(a.w, column(p), column(p) < a.C).get(v);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(__fmul2_rn(f[i], make_float2(s, s)), v[i]);
+      for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(times(f[i], s), v[i]);
     };
     float inv = 0.f;
     if constexpr (kEight) {
@@ -277,6 +390,13 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
         if (in) C::of(f).store(static_cast<T*>(a.y) + base + column(p));
       }
     }
+  }
+  __syncwarp();
+  if (far[threadIdx.x >> 5]) {
+    const RmsArgs* args = &a;
+    int threads = tpr;
+    asm volatile("" : "+l"(args), "+r"(threads));      // (not what the loop has worked out of them)
+    far_rows<T, W, kVec, kEight>(args, threads, blockIdx.x);
   }
 }
 
@@ -321,7 +441,8 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(f[i], f[i], sum);
   };
-  const float s = rsqrtf(fmaf(over_row<add>(long_sum<kPairs, kVec>(a.C, square), kWide, red), a.inv_c, a.eps));
+  float s = rsqrtf(fmaf(over_row<add>(long_sum<kPairs, kVec>(a.C, square), kWide, red), a.inv_c, a.eps));
+  if (leaves_fp32(s)) s = far_factor(x, a.r ? static_cast<const T*>(a.r) + base : nullptr, a.C, a.eps64);
   if (threadIdx.x == 0 && a.rstd) a.rstd[row] = s;
   const T* h = a.r ? static_cast<const T*>(a.sum) + base : x;      // (every thread reads back what it has written itself)
   auto output = [&](int c, float2 (&f)[kPairs]) {
@@ -329,7 +450,7 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
     C::load_cached(h + c).get(f);
     weights<W, kVec>(a.w, c, true).get(v);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(__fmul2_rn(f[i], make_float2(s, s)), v[i]);
+    for (int i = 0; i < kPairs; ++i) f[i] = __fmul2_rn(times(f[i], s), v[i]);
   };
   float inv = 0.f;
   if constexpr (kEight) {
@@ -438,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_bwd_kernel(const RmsArgs 
       w[p].get(v);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        n[p][i] = __fmul2_rn(n[p][i], make_float2(rstd, rstd));
+        n[p][i] = times(n[p][i], rstd);
         dw[p][i] = __ffma2_rn(g[p][i], n[p][i], dw[p][i]);
         g[p][i] = __fmul2_rn(g[p][i], v[i]);
         t2 = __ffma2_rn(g[p][i], n[p][i], t2);
@@ -511,7 +632,7 @@ __global__ void __launch_bounds__(kWide) rms_bwd_wide_kernel(const RmsArgs a) {
     weights<W, kVec>(a.w, c, true).get(v);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      n[i] = __fmul2_rn(n[i], s2);
+      n[i] = times(n[i], rstd);
       g[i] = __fmul2_rn(g[i], v[i]);
     }
   };
@@ -541,7 +662,7 @@ __global__ void __launch_bounds__(kWide) rms_dweight_wide_kernel(const RmsArgs a
   const int64_t r0 = a.rows * blockIdx.y / gridDim.y, r1 = a.rows * (blockIdx.y + 1) / gridDim.y;
   float sum = 0.f;
   for (int64_t r = r0; r < r1; ++r)
-    sum = fmaf(to_f32<T>(static_cast<const T*>(a.dy)[r * a.C + c]), to_f32<T>(static_cast<const T*>(a.x)[r * a.C + c]) * a.rstd[r], sum);
+    sum = fmaf(to_f32<T>(static_cast<const T*>(a.dy)[r * a.C + c]), times(make_float2(to_f32<T>(static_cast<const T*>(a.x)[r * a.C + c]), 0.f), a.rstd[r]).x, sum);
   a.part[int64_t(blockIdx.y) * a.C + c] = sum;
 }
 
@@ -753,6 +874,7 @@ extern "C" NB200_API int nb200_rms_norm_fwd(const nb200_rms_norm_params* p, void
   a.group = p->group ? p->group : p->channels;
   a.group_shift = p->group == 32 ? 5 : p->group == 64 ? 6 : 7;
   a.eps = p->eps;
+  a.eps64 = p->eps;
   a.inv_c = float(1.0 / p->channels);
   const Shape s = shape_of(p->channels, dtype_size(p->dtype), vec, false);
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);

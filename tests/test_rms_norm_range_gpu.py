@@ -44,3 +44,124 @@ def test_long_rows(C, dtype):
         (dx,) = torch.autograd.grad(rms_norm(leaf), leaf, cot)
         want_dx, bound, _, _ = O.rms_norm_grads(leaf.detach(), None, 1e-6, cot)
         _close(dx, want_dx, bound, "dx")
+
+
+# ---- numbers whose squares leave fp32 ----------------------------------------------------------------------------------------------
+WIDTHS = [64, 257, 1000, 4096, 8193, 16400, 40000]
+
+
+def _rows(C, dtype, residual):
+    """Rows of one size each, from that whose squares' sum leaves fp32 up to the largest numbers; one that stands alone; a usual one."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    size = torch.tensor([1e18, 1e19, 1.8e19, 1e25, 1e30, 4e37, 1.0], device="cuda")
+    x = (torch.rand(7, C, generator=g, device="cuda") + 0.5) * size[:, None]
+    x[:, ::3] *= -1
+    x = torch.cat([x, torch.randn(2, C, generator=g, device="cuda"), torch.full((1, C), 3.0e38, device="cuda")])
+    x[7, C // 2] = -3e38
+    x = x.to(dtype)
+    r = (x.float() * torch.rand(10, C, generator=g, device="cuda") * 0.1).to(dtype) if residual else None
+    return x, r
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("residual", [False, True])
+def test_squares_that_leave_fp32(C, dtype, residual):
+    from nitrix_b200.nn import rms_norm
+
+    x, r = _rows(C, dtype, residual)
+    w = torch.linspace(0.5, 1.5, C, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, r, w) if t is not None]
+    out = rms_norm(x, w, residual=r)
+    y, h = out if residual else (out, x)
+    h = h.detach()
+    assert torch.equal(h, O.stream_sum(x.detach(), None if r is None else r.detach())) and bool(h.isfinite().all())
+    want, _, _ = O.rms_norm(h, w.detach(), 1e-6)
+    _close(y, want, want.abs(), "y")
+    dy = torch.randn(x.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    grads = torch.autograd.grad(y, leaves, dy)
+    dx, dx_bound, dw, dw_bound = O.rms_norm_grads(h, w.detach(), 1e-6, dy)
+    _close(grads[0], dx, dx_bound, "dx")
+    _close(grads[-1], dw, dw_bound, "dw")
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_squares_that_vanish_from_fp32(C, dtype):
+    """With an eps that leaves them be."""
+    from nitrix_b200.nn import rms_norm
+
+    g = torch.Generator(device="cuda").manual_seed(C)
+    size = torch.tensor([1e-15, 1e-18, 1e-20, 1e-25, 1e-30, 1.0], device="cuda")
+    x = (torch.randn(6, C, generator=g, device="cuda") * size[:, None]).to(dtype)
+    w = torch.linspace(0.5, 1.5, C, device="cuda")
+    dy = torch.randn(x.shape, generator=g, device="cuda").to(dtype)
+    for eps in (0.0, 1e-38):
+        leaves = [x.detach().requires_grad_(True), w.detach().requires_grad_(True)]
+        y = rms_norm(*leaves, eps=eps)
+        eps = float(torch.tensor(eps))
+        want, _, _ = O.rms_norm(x, w, eps)
+        _close(y, want, want.abs(), "y")
+        grads = torch.autograd.grad(y, leaves, dy)
+        dx, dx_bound, dw, dw_bound = O.rms_norm_grads(x, w, eps, dy)
+        _close(grads[0], dx, dx_bound, "dx")
+        _close(grads[1], dw, dw_bound, "dw")
+
+
+@pytest.mark.parametrize("C", [128, 4096, 8192, 40064, 1001, 17001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_eight_bits_of_squares_that_leave_fp32(C, dtype):
+    from nitrix_b200.nn import rms_norm_quantized
+
+    x, r = _rows(C, dtype, True)
+    h = O.stream_sum(x, r)
+    y, _, _ = O.rms_norm(h, None, 1e-6)
+    for group in (None, 32, 128) if C % 128 == 0 else (None,):
+        codes, scales, got = rms_norm_quantized(x, residual=r, group_size=group)
+        assert torch.equal(got, h)
+        want = O.scales_of(y, group)
+        assert float(((scales.double() - want).abs() / want).max()) <= F
+        z = y / want.repeat_interleave(group or C, -1)
+        err = (codes.double() - z).abs() - (2.0 ** -4 * z.abs()).clamp(min=2.0 ** -10) * (1 + 1e-3) - F * z.abs()
+        assert float(err.max()) <= 0, float(err.max())
+
+
+@pytest.mark.parametrize("C", [64, 4096, 20000])
+def test_infinities_and_nan_beside_large_numbers(C):
+    """An infinity has a NaN, the others of its row zeros; a NaN spoils its row; other rows are what they are."""
+    from nitrix_b200.nn import rms_norm
+
+    x = torch.full((6, C), 1e30, device="cuda").bfloat16()
+    x[1, 5], x[3, C - 1], x[4, 0] = float("inf"), -float("inf"), float("nan")
+    y = rms_norm(x).float()
+    for row, at in ((1, 5), (3, C - 1)):
+        spoiled = torch.zeros(C, dtype=torch.bool, device="cuda")
+        spoiled[at] = True
+        assert torch.equal(y[row].isnan(), spoiled) and not bool(y[row][~spoiled].any())
+    assert bool(y[4].isnan().all())
+    assert bool((y[[0, 2, 5]] == 1).all())
+
+
+@pytest.mark.parametrize("C", [40, 520, 1024, 4096, 8192, 1001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_rows_among_many_change_no_other(C, dtype):
+    from nitrix_b200.nn import rms_norm, rms_norm_quantized
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, r = (torch.randn(9001, C, generator=g, device="cuda").to(dtype) for _ in range(2))
+    group = 32 if C % 32 == 0 else None
+    want = [*rms_norm(x, residual=r), *rms_norm_quantized(x, residual=r, group_size=group), *rms_norm_quantized(x)]
+    large = torch.zeros(9001, dtype=torch.bool, device="cuda")
+    large[[0, 7, 600, 4736, 4737, 8999]] = True
+    x2, r2 = x.clone(), r.clone()
+    x2[large] = (x[large].float() * 1e37).to(dtype)
+    got = [*rms_norm(x2, residual=r2), *rms_norm_quantized(x2, residual=r2, group_size=group), *rms_norm_quantized(x2)]
+    for a, b in zip(got, want):
+        assert torch.equal(a[~large].float(), b[~large].float())
+    y, _, _ = O.rms_norm(got[1][large], None, 1e-6)
+    _close(got[0][large], y, y.abs(), "y")
+    for codes, scales, h in ((got[2], got[3], got[1]), (got[5], got[6], x2)):
+        y, _, _ = O.rms_norm(h[large], None, 1e-6)
+        back = codes[large].double() * scales[large].double().repeat_interleave(C // scales.shape[1], -1)
+        top = scales[large].double().repeat_interleave(C // scales.shape[1], -1) * 448
+        assert float(((back - y).abs() - 2.0 ** -4 * y.abs() - 2.0 ** -10 / 448 * top - F * top).max()) <= 0
