@@ -654,15 +654,29 @@ __global__ void __launch_bounds__(kWide) rms_bwd_wide_kernel(const RmsArgs a) {
     Ch::of(d).store(static_cast<T*>(a.dx) + base + c);
   }
 }
+// Sums of dw are fp32 over that many rows of a thread at most (2^14 rows of one size are 1e-4 off); what they come to is added in 64 bits.
+constexpr int kChain = 256;
+
 // dw of wide rows: a thread has a column, a CTA row the rows of its part.
 template <typename T>
 __global__ void __launch_bounds__(kWide) rms_dweight_wide_kernel(const RmsArgs a) {
   const int c = blockIdx.x * kWide + threadIdx.x;
   if (c >= a.C) return;
-  const int64_t r0 = a.rows * blockIdx.y / gridDim.y, r1 = a.rows * (blockIdx.y + 1) / gridDim.y;
-  float sum = 0.f;
-  for (int64_t r = r0; r < r1; ++r)
-    sum = fmaf(to_f32<T>(static_cast<const T*>(a.dy)[r * a.C + c]), times(make_float2(to_f32<T>(static_cast<const T*>(a.x)[r * a.C + c]), 0.f), a.rstd[r]).x, sum);
+  const int64_t r1 = a.rows * (blockIdx.y + 1) / gridDim.y;
+  const auto chain = [&](int64_t r, int64_t end) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (; r < end; ++r)
+      sum = fmaf(to_f32<T>(static_cast<const T*>(a.dy)[r * a.C + c]), times(make_float2(to_f32<T>(static_cast<const T*>(a.x)[r * a.C + c]), 0.f), a.rstd[r]).x, sum);
+    return sum;
+  };
+  int64_t r = a.rows * blockIdx.y / gridDim.y;
+  float sum = chain(r, min(r1, r + kChain));
+  if (r1 - r > kChain) {
+    double all = sum;
+    for (r += kChain; r < r1; r += kChain) all += chain(r, min(r1, r + kChain));
+    sum = float(all);
+  }
   a.part[int64_t(blockIdx.y) * a.C + c] = sum;
 }
 
@@ -674,8 +688,18 @@ __global__ void __launch_bounds__(1024) rms_dweight_kernel(const float* part, in
   float sum = 0.f;
   wait_for_previous();
   if (c < C) {
+    const auto chain = [&](int r, int end) {
+      float part_sum = 0.f;
 #pragma unroll 4
-    for (int r = threadIdx.y; r < rows; r += 32) sum += __ldcg(part + int64_t(r) * C + c);
+      for (; r < end; r += 32) part_sum += __ldcg(part + int64_t(r) * C + c);
+      return part_sum;
+    };
+    sum = chain(threadIdx.y, min(rows, 1024));
+    if (rows > 1024) {
+      double all = sum;
+      for (int r = 1024; r < rows; r += 1024) all += chain(r + threadIdx.y, min(rows, r + 1024));
+      sum = float(all);
+    }
   }
   sums[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
@@ -759,14 +783,17 @@ int with_shape(const Shape& s, F f) {
   return s.vec ? with_threads(std::integral_constant<int, kVec>{}) : with_threads(std::integral_constant<int, 1>{});
 }
 
-// The backward's shape, its shared memory, and the rows of partial sums that it leaves, one per CTA.
+// The backward's shape, its shared memory and CTAs; the rows of a launch, and the rows of partial sums that all launches leave, one per CTA.
 struct BwdPlan {
   Shape s;
-  int smem, parts;
+  int smem, ctas;
+  int64_t launch_rows;
+  int parts;
 };
 template <typename T>
 BwdPlan bwd_plan(int C, int64_t rows, bool vec) {
-  BwdPlan pl{shape_of(C, int(sizeof(T)), vec, true), 0, 0};
+  BwdPlan pl{shape_of(C, int(sizeof(T)), vec, true), 0, 0, rows, 0};
+  if (rows == 0) return pl;
   if (pl.s.per == 0) {
     pl.parts = int(rows < 64 ? rows : 64);
     return pl;
@@ -779,7 +806,11 @@ BwdPlan bwd_plan(int C, int64_t rows, bool vec) {
     const int by_threads = ctas_of(bwd_threads(kPer * kVec), pl.s.threads), by_room = 227 * 1024 / (pl.smem + 2048);
     const int64_t groups = pl.s.threads / pl.s.tpr, blocks = (rows + groups - 1) / groups;
     const int64_t most = int64_t(tc::sm_count()) * (by_threads < by_room ? by_threads : by_room);
-    pl.parts = int(blocks < most ? blocks : most);
+    pl.ctas = int(blocks < most ? blocks : most);
+    // (a launch for each kChain rows of a thread: 0.4 ms of work and more)
+    const int64_t launch_blocks = int64_t(pl.ctas) * kChain, whole = blocks / launch_blocks, rest = blocks % launch_blocks;
+    pl.launch_rows = launch_blocks * groups;
+    pl.parts = int(whole * pl.ctas + (rest < pl.ctas ? rest : pl.ctas));
     return int(NB200_OK);
   });
   return pl;
@@ -829,9 +860,20 @@ int launch_rows(const RmsArgs& a, const BwdPlan& pl, cudaStream_t st) {
     constexpr int kV = decltype(kv)::value, kPer = decltype(kp)::value, kThreads = decltype(kt)::value;
     auto kernel = rms_bwd_kernel<T, W, kV, kPer, kThreads, ctas_of(bwd_threads(kPer * kV), kThreads)>;
     if (pl.smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess) return check_launch("rms_bwd_kernel");
-    kernel<<<unsigned(pl.parts), pl.s.threads, pl.smem, st>>>(a, pl.s.tpr);
-    count_launch();
-    return check_launch("rms_bwd_kernel");
+    for (int64_t r0 = 0; r0 < a.rows; r0 += pl.launch_rows) {
+      const int64_t at = r0 * a.C;
+      RmsArgs b = a;
+      b.x = static_cast<const T*>(a.x) + at; b.dy = static_cast<const T*>(a.dy) + at; b.dx = static_cast<T*>(a.dx) + at;
+      if (a.dsum) b.dsum = static_cast<const T*>(a.dsum) + at;
+      b.rstd = a.rstd + r0;
+      b.rows = a.rows - r0 < pl.launch_rows ? a.rows - r0 : pl.launch_rows;
+      if (a.part) b.part = a.part + r0 / pl.launch_rows * pl.ctas * a.C;
+      const int64_t groups = pl.s.threads / pl.s.tpr, blocks = (b.rows + groups - 1) / groups;
+      kernel<<<unsigned(blocks < pl.ctas ? blocks : pl.ctas), pl.s.threads, pl.smem, st>>>(b, pl.s.tpr);
+      count_launch();
+      if (int rc = check_launch("rms_bwd_kernel")) return rc;
+    }
+    return int(NB200_OK);
   });
 }
 template <typename T, typename W>

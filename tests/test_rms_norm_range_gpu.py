@@ -46,6 +46,25 @@ def test_long_rows(C, dtype):
         _close(dx, want_dx, bound, "dx")
 
 
+# ---- many rows -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,rows,C", [
+    (torch.float32, 1 << 24, 32), (torch.float32, 1 << 24, 7), (torch.bfloat16, 1 << 24, 64), (torch.bfloat16, 1 << 21, 1000),
+    (torch.float16, 1 << 20, 2048), (torch.bfloat16, 1 << 18, 8193), (torch.bfloat16, 1 << 18, 16400)])
+def test_gradients_of_weights_over_many_rows(dtype, rows, C):
+    """Of rows that are all alike: dw is their number times one term, of which 256 at most are added one after the other, 8 groups of rows and
+    32 CTAs' sums in fp32 again, the rest in 64 bits and a tree: 305 roundings."""
+    from nitrix_b200.nn import rms_norm
+
+    x, w = torch.full((rows, C), 1.7, dtype=dtype, device="cuda"), torch.ones(C, device="cuda", requires_grad=True)
+    y = rms_norm(x, w)
+    dy = torch.full_like(x, 0.3)
+    dy[:, 1::2] = -1.1
+    (dw,) = torch.autograd.grad(y, w, dy)
+    n = O.rms_norm(x[:1], None, 1e-6)[0]
+    want = rows * (n * dy[:1].double())[0]
+    assert float(((dw.double() - want).abs() / want.abs()).max()) <= 305 * 2.0 ** -24
+
+
 # ---- numbers whose squares leave fp32 ----------------------------------------------------------------------------------------------
 WIDTHS = [64, 257, 1000, 4096, 8193, 16400, 40000]
 
