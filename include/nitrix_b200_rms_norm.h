@@ -10,8 +10,10 @@
  *   h = x + residual, rounded to the dtype (x without a residual);   rstd = (mean h^2 + eps)^-1/2;   y = h rstd weight
  *
  * With `scales`, y is e4m3: of every `group` channels (0: of the row) a = max(max |y|, 2^-100), scale = a / 448 (fp32,
- * [row][group]), code = y (448 / a) rounded to e4m3, of the y that has not been rounded before.  A NaN or an infinity makes its
- * row's codes NaN.  With g = dy weight and n = h rstd, the backward is
+ * [row][group]), code = y (448 / a) rounded to e4m3, of the y that has not been rounded before.  A NaN makes all of its row NaN.  An
+ * infinity has the mean square infinite and rstd 0: its own y is NaN and the others of its row are 0, so that the codes and the scale
+ * of its group (or row) are NaN, those of the row's other groups zeros under the least scale.  With g = dy weight and n = h rstd, the
+ * backward is
  *
  *   dx = dsum + rstd (g - n mean(g n)),   dweight = sum over rows of dy n
  *

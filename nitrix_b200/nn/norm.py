@@ -99,7 +99,9 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
 
     With ``residual``, of ``x``'s shape and dtype, the two streams are added first: ``(y, h)`` comes back, where ``h`` is
     ``x + residual`` in their dtype and ``y`` the norm of ``h``.  ``x`` is a CUDA tensor of fp32, bf16 or fp16, ``weight`` of the
-    same dtype or fp32 with shape ``(c,)``; the arithmetic is fp32, rounded once.  Differentiable in ``x``, ``residual`` and ``weight``."""
+    same dtype or fp32 with shape ``(c,)``; the arithmetic is fp32, rounded once, and fp64 for the factor of rows whose squares leave
+    fp32.  A row with an infinity has a NaN there and zeros elsewhere, one with a NaN is NaN.  Differentiable in ``x``, ``residual``
+    and ``weight``."""
     resolve_backend(backend)   # raises without a Blackwell device: there is no host path
     y, h = _cabi.torch_ops().rms_norm(x, residual, weight, float(eps))
     return y if residual is None else (y, h)
@@ -111,8 +113,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *
 
     ``codes`` is ``torch.float8_e4m3fn`` of ``x``'s shape, ``scales`` fp32 with a last axis of one element (``group_size=None``) or
     one for each ``group_size`` channels (32, 64 or 128, which must divide them); ``codes * scales`` stands for the norm.  A scale is
-    the largest magnitude over 448, and what is rounded has not been rounded before.  A row with a NaN or an infinity has NaN codes.
-    Not differentiable."""
+    the largest magnitude over 448, and what is rounded has not been rounded before.  A row with a NaN has NaN codes and scales.  With an
+    infinity, codes and scale of its group (``group_size=None``: of the row) are NaN; the row's other groups are zeros.  Not
+    differentiable."""
     resolve_backend(backend)
     if group_size is not None and group_size not in (32, 64, 128):
         raise ValueError(f"rms_norm_quantized: group_size must be 32, 64 or 128, or None for whole rows; got {group_size}")

@@ -184,3 +184,24 @@ def test_large_rows_among_many_change_no_other(C, dtype):
         back = codes[large].double() * scales[large].double().repeat_interleave(C // scales.shape[1], -1)
         top = scales[large].double().repeat_interleave(C // scales.shape[1], -1) * 448
         assert float(((back - y).abs() - 2.0 ** -4 * y.abs() - 2.0 ** -10 / 448 * top - F * top).max()) <= 0
+
+
+@pytest.mark.parametrize("group,C", [(32, 256), (64, 4096), (128, 8192), (32, 40064), (None, 256), (None, 1001), (None, 20000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_eight_bits_of_rows_with_an_infinity_or_a_nan(group, C, dtype):
+    """As documented: codes and scale of an infinity's group are NaN, the others of its row zeros under the least scale; a NaN spoils its row."""
+    from nitrix_b200.nn import rms_norm_quantized
+
+    x = torch.randn(5, C, device="cuda").to(dtype)
+    want = rms_norm_quantized(x, group_size=group)
+    x[1, C // 2 + 3], x[3, 1] = -float("inf"), float("nan")
+    codes, scales = rms_norm_quantized(x, group_size=group)
+    size = group or C
+    spoiled = torch.zeros(5, C // size, dtype=torch.bool, device="cuda")
+    spoiled[1, (C // 2 + 3) // size] = True
+    spoiled[3] = True
+    assert torch.equal(scales.isnan(), spoiled) and torch.equal(codes.float().isnan(), spoiled.repeat_interleave(size, 1))
+    rest = ~spoiled[1]
+    assert not bool(codes[1].float()[rest.repeat_interleave(size)].any()) and bool((scales[1][rest] == 2.0 ** -100 * torch.tensor(1 / 448, device="cuda")).all())
+    for row in (0, 2, 4):
+        assert torch.equal(codes[row].float(), want[0][row].float()) and torch.equal(scales[row], want[1][row])
