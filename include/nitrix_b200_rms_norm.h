@@ -18,8 +18,9 @@
  *   dx = dsum + rstd (g - n mean(g n)),   dweight = sum over rows of dy n
  *
  * Layout.  x, residual, y, sum, dy, dsum, dx are dense [rows][channels]; weight and dweight [channels], of the same dtype or
- * fp32.  Rows of a multiple of 16 bytes and 16-byte aligned pointers take kernels that move 16-byte words, up to 32 KB a row
- * without reading it twice; anything else runs the same kernels element by element.  Sums have one order.  Every pointer is a
+ * fp32.  Rows of a multiple of 16 bytes and 16-byte aligned pointers take kernels that move 16-byte words and read
+ * a row once up to 64 KB (backward: 32 KB); anything else runs the same kernels element by element, up to 16384 (8192) channels at
+ * one reading.  Sums have one order.  Every pointer is a
  * device pointer; all work is enqueued on the caller's stream; nothing is allocated.
  */
 #ifndef NITRIX_B200_RMS_NORM_H_

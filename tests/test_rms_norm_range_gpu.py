@@ -46,6 +46,37 @@ def test_long_rows(C, dtype):
         _close(dx, want_dx, bound, "dx")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C", [32768, 32776, 32896, 65536])
+def test_16_bit_rows_at_and_beyond_what_is_held(C, dtype):
+    """32768 channels are held in the forward, more are read twice, by words; with and without a residual, weights of either type."""
+    from nitrix_b200.nn import rms_norm, rms_norm_quantized
+
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x, r = (torch.randn(5, C, generator=g, device="cuda").to(dtype) for _ in range(2))
+    dy, dh = (torch.randn(5, C, generator=g, device="cuda").to(dtype) for _ in range(2))
+    for residual, w in ((r, torch.randn(C, generator=g, device="cuda")), (None, torch.randn(C, generator=g, device="cuda").to(dtype)), (r, None)):
+        leaves = [t.detach().requires_grad_(True) for t in (x, residual, w) if t is not None]
+        out = rms_norm(leaves[0], None if w is None else leaves[-1], residual=None if residual is None else leaves[1])
+        y, h = (out, x) if residual is None else (out[0], out[1].detach())
+        assert torch.equal(h, O.stream_sum(x, residual))
+        want, _, _ = O.rms_norm(h, w, 1e-6)
+        _close(y, want, want.abs(), "y")
+        grads = torch.autograd.grad(y if residual is None else out, leaves, dy if residual is None else [dy, dh])
+        dx, dx_bound, dw, dw_bound = O.rms_norm_grads(h, w, 1e-6, dy, None if residual is None else dh)
+        _close(grads[0], dx, dx_bound, "dx")
+        if w is not None:
+            _close(grads[-1], dw, dw_bound, "dw")
+        for group in (None, 32, 64, 128) if C % 128 == 0 else (None,):
+            codes, scales, *rest = rms_norm_quantized(x, w, residual=residual, group_size=group)
+            assert not rest or torch.equal(rest[0], h)
+            exact = O.scales_of(want, group)
+            assert float(((scales.double() - exact).abs() / exact).max()) <= F
+            z = want / exact.repeat_interleave(group or C, -1)
+            err = (codes.double() - z).abs() - (2.0 ** -4 * z.abs()).clamp(min=2.0 ** -10) * (1 + 1e-3) - F * z.abs()
+            assert float(err.max()) <= 0, float(err.max())
+
+
 # ---- many rows -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,rows,C", [
     (torch.float32, 1 << 24, 32), (torch.float32, 1 << 24, 7), (torch.bfloat16, 1 << 24, 64), (torch.bfloat16, 1 << 21, 1000),
