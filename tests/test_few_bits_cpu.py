@@ -114,6 +114,41 @@ def test_reading_refuses(change, code):
     assert "cache_read" in _cabi.last_error()
 
 
+class _Decode(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("pages", _Pages), ("table", C.c_void_p), ("lengths", C.c_void_p), ("rows", C.c_int32), ("width", C.c_int32),
+                ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64 * 2), ("q_heads", C.c_int32), ("scale", C.c_float), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class _QuantizedDecode(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("decode", _Decode), ("steps", _Steps)]
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(bits=2), "INVALID"), (dict(dtype=7), "INVALID"), (dict(heads=0), "INVALID"), (dict(page_size=0), "INVALID"), (dict(rows=-1), "INVALID"), (dict(q_heads=3), "INVALID"),
+    (dict(q_heads=0), "INVALID"), (dict(q=None), "INVALID"), (dict(out=None), "INVALID"), (dict(table=None), "INVALID"), (dict(lengths=None), "INVALID"), (dict(codes=None), "INVALID"),
+    (dict(steps=None), "INVALID"), (dict(head_dim=72), "UNSUPPORTED"), (dict(head_dim=288), "UNSUPPORTED"), (dict(rows=65536), "UNSUPPORTED"), (dict(codes=264), "ALIGNMENT"),
+    (dict(slot_stride=40), "ALIGNMENT"), (dict(steps=260), "ALIGNMENT"), (dict(step_stride=3), "ALIGNMENT"), (dict(slot_stride=1 << 35), "UNSUPPORTED"),
+    (dict(step_stride=1 << 32), "UNSUPPORTED"), (dict(workspace=None), "WORKSPACE"), (dict(short=1), "WORKSPACE"), (dict(workspace=264), "ALIGNMENT"), (dict(inner_size=8), "INVALID")])
+def test_attention_over_codes_refuses(change, code):
+    from nitrix_b200 import _cabi
+
+    c = {**dict(bits=4, dtype=1, heads=2, page_size=8, rows=1, q_heads=4, q=256, out=256, table=256, lengths=256, codes=256, steps=256, head_dim=64, slot_stride=32, step_stride=2,
+                workspace=256, short=0, inner_size=C.sizeof(_Decode)), **change}
+    pages = _Pages(k=c["codes"], v=256, k_stride=(512, 256, c["slot_stride"]), v_stride=(512, 256, 32), pages=4, heads=c["heads"], page_size=c["page_size"], head_dim=c["head_dim"],
+                   dtype=c["dtype"])
+    steps = _Steps(k=c["steps"], v=256, k_stride=(32, 16, c["step_stride"]), v_stride=(32, 16, 2), bits=c["bits"])
+    decode = _Decode(struct_size=c["inner_size"], pages=pages, table=c["table"], lengths=c["lengths"], rows=c["rows"], width=3, q=c["q"], out=c["out"], q_stride=(256, 64),
+                     q_heads=c["q_heads"], scale=0.1, workspace=c["workspace"])
+    p = _QuantizedDecode(struct_size=C.sizeof(_QuantizedDecode), decode=decode, steps=steps)
+    need = C.c_size_t(0)
+    if _cabi.lib().nb200_decode_quantized_workspace_bytes(C.byref(p), C.byref(need)) == 0:      # (what it says of the sizes alone is asked first)
+        assert need.value > 0
+    p.decode.workspace_bytes = need.value - c["short"]
+    assert _cabi.lib().nb200_decode_quantized(C.byref(p), None) == getattr(_cabi, "ERR_" + code), _cabi.last_error()
+    assert "decode_quantized" in _cabi.last_error()
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="there is a GPU")
 def test_there_is_no_host_path():
     from nitrix_b200 import NitrixBackendError
