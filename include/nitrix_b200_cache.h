@@ -112,8 +112,9 @@ NB200_API int nb200_decode_workspace_bytes(const nb200_decode_params* p, size_t*
  * in fp32 (a step of zero or NaN has the codes of zero).  A row of codes is (8, head_dim / 32, b / 2) bytes: of every group the
  * elements 4 j .. 4 j + 3 lie together, the first in the lowest bits.
  *
- * nb200_decode_quantized takes 16-bit queries of head dims 64 and 128 as fp16 under a power of two per head; where one of their
- * magnitudes passes 2^100, its head's result may be NaN.
+ * nb200_decode_quantized takes 16-bit queries of head dims 64 and 128, in rows on 16-byte boundaries, as fp16 under a power of two per
+ * head; where one of their magnitudes passes 2^100, its head's result may be NaN.  It rounds a probability times its value's step to
+ * fp16: each token's term is off by 2^-11 of itself, or by 2^(b-1) times 2^-32 of the largest such product of the sequence and head.
  *
  * In nb200_cache_pages k and v are then the codes, their strides are bytes, dtype is that of the new tokens, of q and out, or of
  * what is read; head_dim is a multiple of 32.  Rows of codes begin on 16-byte boundaries, those of steps on multiples of their

@@ -256,11 +256,13 @@ struct QuantizedFmaLoop {
 // Codes become operands without a conversion: the bits of a whole number below 1024 in an fp16 are that number times 2^-24, so a
 // mask of a word that holds codes of two operands' halves gives both (in 4 bits every other element's code stands four bits up,
 // which is times 16: the queries have 1/16 there, the output's rows get it at the end).  Queries are fp16, by a power of two per head
-// that brings the largest near 2^10: bf16 has 8 bits, so that nothing is lost above 2^-24 of it.
+// that brings the largest to 2^9 .. 2^10: fp16's bits are all kept down to 2^-23 of it, bf16's to 2^-26 (with the 1/16 to 2^-19 and 2^-22),
+// and smaller elements are off by 2^-34 (2^-30) of it.
 // Steps: those of a key's groups multiply the groups' sums, fp32, of which the half of the codes' range has been taken off
 // beforehand (the accumulators begin with it); those of a value's groups multiply its probability before that is rounded to fp16,
 // once, for each group.  The reference maximum is that of score + log2 of the value's largest step, so that no product leaves
-// fp16 and small ones keep their bits whatever the steps are; the sum of the probabilities is fp32.  Values' codes lose the half of
+// fp16 and those of small steps keep their bits: a token's largest is at 2^7 .. 2^15 at the reference, so that a rounding is 2^-11 of the
+// product or 2^-32 of the largest one; the sum of the probabilities is fp32.  Values' codes lose the half of
 // their range before the product, two at a time: taken off the sums instead, by MMAs of their own, it leaves errors of 2^-18 of it.
 //
 // A warp takes two blocks of 16 tokens at a turn, which come through a ring in shared memory by asynchronous copies, the next turn's
