@@ -165,7 +165,11 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* red) {
 // A row's factor where its squares leave fp32 or vanish from it: in 64 bits, by every warp of the row for itself.  (Infinities and NaN end
 // up here as well and give 0 and NaN, rows of zeros without an eps infinity.)
 constexpr float kMostFactor = 1125899906842624.f;     // 2^50: squares below 2^-126 are flushed, which a mean of 2^-100 does not feel
-__device__ __forceinline__ bool leaves_fp32(float factor) { return !(factor > 0.f && factor < kMostFactor); }
+// (fp16 has no such numbers: its squares lie between 2^-48 and 2^32; infinities and NaN need nothing else.)
+template <typename T>
+constexpr bool kLeaves = !std::is_same<T, __half>::value;
+template <typename T>
+__device__ __forceinline__ bool leaves_fp32(float factor) { return kLeaves<T> && !(factor > 0.f && factor < kMostFactor); }
 template <typename T>
 __device__ __noinline__ float far_factor(const T* x, const T* r, int C, double eps) {
   double sum = 0.0;
@@ -321,8 +325,10 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
   for (int p = 0; p < kPer; ++p)
     if (kHeld) w[p] = weights<W, kVec>(a.w, column(p), column(p) < a.C);
   int turn = 0;
-  if ((threadIdx.x & 31) == 0) far[threadIdx.x >> 5] = 0;      // (of the warp: a flag in a register is one more than there are)
-  __syncwarp();
+  if constexpr (kLeaves<T>) {
+    if ((threadIdx.x & 31) == 0) far[threadIdx.x >> 5] = 0;      // (of the warp: a flag in a register is one more than there are)
+    __syncwarp();
+  }
   for (unsigned block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
     const unsigned row = block * groups + mine;
     const int64_t base = int64_t(row) * a.C;
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
     }
     fetch(block + gridDim.x);
     float s = rsqrtf(fmaf(over_row<add>(ss.x + ss.y, tpr, red + turn * kMaxWarps), a.inv_c, a.eps));
-    if (leaves_fp32(s)) {
+    if (leaves_fp32<T>(s)) {
       far[threadIdx.x >> 5] = 1;
       s = __uint_as_float(0x7fffffffu);
     }
@@ -391,12 +397,14 @@ __global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 
       }
     }
   }
-  __syncwarp();
-  if (far[threadIdx.x >> 5]) {
-    const RmsArgs* args = &a;
-    int threads = tpr;
-    asm volatile("" : "+l"(args), "+r"(threads));      // (not what the loop has worked out of them)
-    far_rows<T, W, kVec, kEight>(args, threads, blockIdx.x);
+  if constexpr (kLeaves<T>) {
+    __syncwarp();
+    if (far[threadIdx.x >> 5]) {
+      const RmsArgs* args = &a;
+      int threads = tpr;
+      asm volatile("" : "+l"(args), "+r"(threads));      // (not what the loop has worked out of them)
+      far_rows<T, W, kVec, kEight>(args, threads, blockIdx.x);
+    }
   }
 }
 
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(kWide) rms_fwd_wide_kernel(const RmsArgs a) {
     for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(f[i], f[i], sum);
   };
   float s = rsqrtf(fmaf(over_row<add>(long_sum<kPairs, kVec>(a.C, square), kWide, red), a.inv_c, a.eps));
-  if (leaves_fp32(s)) s = far_factor(x, a.r ? static_cast<const T*>(a.r) + base : nullptr, a.C, a.eps64);
+  if (leaves_fp32<T>(s)) s = far_factor(x, a.r ? static_cast<const T*>(a.r) + base : nullptr, a.C, a.eps64);
   if (threadIdx.x == 0 && a.rstd) a.rstd[row] = s;
   const T* h = a.r ? static_cast<const T*>(a.sum) + base : x;      // (every thread reads back what it has written itself)
   auto output = [&](int c, float2 (&f)[kPairs]) {
