@@ -169,3 +169,22 @@ def test_groups_of_values_beyond_fp16_of_each_other(bits, dtype, dim):
             largest = max(largest, float(err[i, h].max()) - n * 2.0 ** -32 * top * half)
     assert largest <= 0, largest
     _check(q.float(), cache, lengths, bits, scale)
+
+
+def test_batched_tensors_are_refused():
+    """The functions have no batching rule: ``vmap`` over them raises, and nothing is written."""
+    from nitrix_b200.nn import cache_append, cache_read, decode_attention, rms_norm, rms_norm_quantized
+
+    cache = _filled([20, 3], 16, 2, 64, 4)
+    before = [t.clone() for t in cache]
+    x, w = torch.randn(3, 5, 64, device="cuda"), torch.ones(64, device="cuda")
+    k, offsets = torch.randn(3, 2, 2, 64, device="cuda"), torch.arange(3, device="cuda").int()
+    q = torch.randn(3, 2, 4, 64, device="cuda")
+    calls = [(lambda t: rms_norm(t, w), x), (lambda t: rms_norm(x[0], t), torch.ones(3, 64, device="cuda")), (lambda t: rms_norm(x[0], w, residual=t), x),
+             (lambda t: rms_norm_quantized(t, w)[0].float(), x), (lambda t: rms_norm(t, w), x.clone().requires_grad_(True)), (lambda t: cache_append(cache, t, t, offsets).lengths, k),
+             (lambda t: cache_read(cache, t, 2)[0], offsets.repeat(3, 1)), (lambda t: decode_attention(t, cache), q)]
+    for call, batched in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(batched)
+    for a, b in zip(cache, before):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
