@@ -6,14 +6,15 @@
 //   backward  n = h s,  g = dy w,  dx = dh + s (g - n mean(g n)),  dw = sum_rows dy n
 //
 // Bound by HBM: every stream is read once and written once, so a row is held in registers between its sum and its output: by
-// tpr threads (a power of two), kPer chunks of kVec elements each.  kVec is a 16-byte word's elements, or one where rows do not
+// tpr threads (whole warps; a power of two where rows share a CTA), kPer chunks of kVec elements each.  kVec is a 16-byte word's elements, or one where rows do not
 // begin on 16-byte boundaries.  CTAs walk the rows with a stride and ask for the next row before they work on the present one.
 // Elements are taken in pairs, two fp32 operations per instruction: with 16-bit storage the conversions and the arithmetic take as
 // many issue slots as the loads leave.  Rows that are too long to be held are read once more (the *_wide kernels).
 //
-// bf16, 16384 x 4096 with a residual: forward 82 us (6.5 TB/s of what has to be moved, the rate of a copy), backward 88 (6.1), of which
-// the sums of dw take 6 more; e4m3 with a scale per 128 channels, 16384 x 8192: 150 us (6.3 TB/s).  fp32, 4099 rows of 1001 channels, by
-// elements: 19 and 22 us.  Scalar arithmetic and conversions, one row at a time: 107, 136 and 279 us.
+// Launches by themselves with cold caches (ncu).  bf16, 16384 x 4096 with a residual: forward 81 us (6.6 TB/s of what has to be moved, the
+// rate of a copy), backward 87 (6.2), and the sums of dw take 6 more; e4m3, 16384 x 8192: with a scale per 128 channels 154 us (149 in a
+// captured graph, 6.3 TB/s), with one per row 5 more.  fp32, 4099 rows of 1001 channels, by elements: 17 and 22 us.  Scalar arithmetic and
+// conversions, one row at a time: 107, 136 and 279 us.
 #include <cuda_fp8.h>
 #include <math.h>
 
