@@ -96,7 +96,7 @@ typedef struct nb200_decode_params {
   int64_t q_stride[2];       /* elements, over (row, head) */
   int32_t q_heads;           /* a multiple of pages.heads: query head h reads key head h / (q_heads / pages.heads) */
   float scale;
-  void* workspace;           /* nb200_decode_workspace_bytes; 16-byte aligned */
+  void* workspace;           /* nb200_decode_workspace_bytes of the same block (q's alignment counts); 16-byte aligned */
   size_t workspace_bytes;
 } nb200_decode_params;
 

@@ -45,7 +45,8 @@ typedef struct nb200_rms_norm_params {
   const void* dsum;        /* backward: the gradient of `sum`, or NULL */
   void* dx;
   void* dweight;           /* backward: NULL: not wanted */
-  void* workspace;         /* backward with dweight: nb200_rms_norm_workspace_bytes; 16-byte aligned */
+  void* workspace;         /* backward with dweight: nb200_rms_norm_workspace_bytes of the same block (the operands' alignment
+                              counts); 16-byte aligned */
   size_t workspace_bytes;
   int64_t rows;
   int32_t channels;        /* at most 2^30 */

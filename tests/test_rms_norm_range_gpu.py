@@ -96,6 +96,33 @@ def test_gradients_of_weights_over_many_rows(dtype, rows, C):
     assert float(((dw.double() - want).abs() / want.abs()).max()) <= 305 * 2.0 ** -24
 
 
+@pytest.mark.parametrize("dtype,C", [(torch.float32, 32), (torch.bfloat16, 2056), (torch.float16, 129)])
+@pytest.mark.parametrize("more", [0, 1, 5003])
+def test_rows_about_a_launch_s_end(dtype, C, more):
+    """The backward takes 256 rows a thread in a launch; every row behind has its gradient, and its part of dw, all the same."""
+    from nitrix_b200.nn import rms_norm
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    rows = 256 * sms * {32: 4 * 8, 2056: 3, 129: 4 * 4}[C] + more      # (CTAs of an SM times rows of a CTA)
+    g = torch.Generator(device="cuda").manual_seed(more)
+    x, r, dy, dh = (torch.randn(rows, C, generator=g, device="cuda").to(dtype) for _ in range(4))
+    w = torch.randn(C, generator=g, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, r, w)]
+    y, h = rms_norm(x, w, residual=r)
+    dx, dr, dw = torch.autograd.grad([y, h], leaves, [dy, dh])
+    again = torch.autograd.grad(rms_norm(x, w, residual=r), leaves, [dy, dh])
+    assert torch.equal(dw, again[2]) and torch.equal(dx, again[0]) and torch.equal(dx, dr)
+    h, w = h.detach(), w.detach()
+    want_dw, bound_dw = torch.zeros(C, dtype=torch.float64, device="cuda"), torch.zeros(C, dtype=torch.float64, device="cuda")
+    for at in range(0, rows, 1 << 18):
+        part = slice(at, at + (1 << 18))
+        want, bound, terms, terms_bound = O.rms_norm_grads(h[part], w, 1e-6, dy[part], dh[part])
+        _close(dx[part], want, bound, "dx")
+        want_dw += terms
+        bound_dw += terms_bound
+    assert float(((dw.double() - want_dw).abs() - 305 * 2.0 ** -24 * bound_dw).max()) <= 0
+
+
 # ---- numbers whose squares leave fp32 ----------------------------------------------------------------------------------------------
 WIDTHS = [64, 257, 1000, 4096, 8193, 16400, 40000]
 
