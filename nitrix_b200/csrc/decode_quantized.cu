@@ -25,6 +25,11 @@ struct QuantizedArgs : DecodeArgs {      // k, v: codes
   int groups;
 };
 
+// CTAs of an SM, which the loops' registers allow and the division of the work counts on.
+constexpr int fma_ctas(int heads_by_groups) { return heads_by_groups <= 4 ? 4 : heads_by_groups <= 8 ? 3 : 2; }
+// (head dim 128: three CTAs per SM without spills 97 us over long contexts, four with them 99, five 142)
+constexpr int mma_ctas(int head_dim, int bits, int heads) { return heads == 8 ? (head_dim == 64 ? 4 : bits == 4 ? 3 : 2) : head_dim == 64 ? 3 : 2; }
+
 __device__ __forceinline__ const uint16_t* steps_of(const uint16_t* base, const int (&stride)[3], int groups, int kv_head, Where w) {
   return base + (int64_t(w.page) * stride[0] + int64_t(kv_head) * stride[1] + int64_t(w.slot) * stride[2]) * groups;
 }
@@ -49,7 +54,7 @@ struct QuantizedFmaLoop {
   static constexpr int kRing = 0;
   static constexpr int kHeads = kNumHeads;
   static constexpr int kSlots = 4;
-  static constexpr int kMinCtas = kHeads * kGroups <= 4 ? 4 : kHeads * kGroups <= 8 ? 3 : 2;
+  static constexpr int kMinCtas = fma_ctas(kHeads * kGroups);
   static constexpr int kAhead = 2;
   static constexpr int kLanes = 8, kSteps = kHeads == 4 ? 2 : kHeads == 2 ? 1 : 0;      // of the reduce-scatter
   static constexpr int kWords = (kGroups * kBits + 7) / 8, kStepWords = (kGroups + 1) / 2;
@@ -273,8 +278,7 @@ struct QuantizedMmaLoop {
   static constexpr int kHeads = 8 * kTiles;
   static constexpr int kBlock = 16, kTurn = 32;  // tokens
   static constexpr int kSlots = 1;
-  // (head dim 128: three CTAs per SM without spills 97 us over long contexts, four with them 99, five 142)
-  static constexpr int kMinCtas = kTiles == 1 ? (D == 64 ? 4 : kBits == 4 ? 3 : 2) : D == 64 ? 3 : 2;
+  static constexpr int kMinCtas = mma_ctas(D, kBits, kHeads);
   static constexpr int kG = D / kGroup;          // groups
   static constexpr int kW = kG * kBits / 8;      // words of a part of a row of codes
   static constexpr int kRow = D * kBits / 8;     // bytes of a row of codes
@@ -620,15 +624,14 @@ Plan plan(const nb200_decode_params* p, int bits) {
   bool q_words = aligned16(p->q);
   for (int i = 0; i < 2; ++i) q_words = q_words && p->q_stride[i] % 8 == 0;
   pl.mma = c.dtype != NB200_F32 && (c.head_dim == 64 || c.head_dim == 128) && q_words;
-  int ctas = 2;      // resident per SM: the loops' kMinCtas
+  int ctas;
   if (pl.mma) {
     pl.heads = group > 8 ? 16 : 8;
-    ctas = pl.heads == 8 ? (c.head_dim == 64 ? 4 : bits == 4 ? 3 : 2) : c.head_dim == 64 ? 3 : 2;
+    ctas = mma_ctas(c.head_dim, bits, pl.heads);
   } else {
     const int most = c.head_dim > 128 ? 2 : 4;
     pl.heads = group >= most ? most : group == 3 ? 4 : group;
-    const int size = pl.heads * groups_of(c.head_dim);
-    ctas = size <= 4 ? 4 : size <= 8 ? 3 : 2;
+    ctas = fma_ctas(pl.heads * groups_of(c.head_dim));
   }
   const int chunks = (group + pl.heads - 1) / pl.heads;
   pl.side = chunks == 1 ? 1 : chunks == 2 ? 2 : 4;

@@ -29,6 +29,11 @@ namespace {
 
 constexpr int kMaxWarps = 16;
 
+// Threads of all CTAs of an SM, by the registers that a thread takes (the kernels' launch bounds), and CTAs of `threads`.
+constexpr int fwd_threads(int per, int vec) { return per <= (vec == 1 ? 8 : 2) ? 1024 : 512; }
+constexpr int bwd_threads(int elements) { return elements <= 8 ? 1024 : elements <= 16 ? 768 : 512; }
+constexpr int ctas_of(int all, int threads) { return all < threads ? 1 : all / threads; }
+
 struct RmsArgs {
   const void* x;
   const void* r;
@@ -298,7 +303,7 @@ __device__ __noinline__ void far_rows(const RmsArgs* pa, int tpr, int64_t block)
 }
 
 template <typename T, typename W, int kVec, int kPer, int kThreads, bool kEight>
-__global__ void __launch_bounds__(kThreads, (kPer <= (kVec == 1 ? 8 : 2) ? 1024 : 512) / kThreads) rms_fwd_kernel(const __grid_constant__ RmsArgs a, int tpr) {
+__global__ void __launch_bounds__(kThreads, ctas_of(fwd_threads(kPer, kVec), kThreads)) rms_fwd_kernel(const __grid_constant__ RmsArgs a, int tpr) {
   __shared__ __align__(16) float red[4 * kMaxWarps];
   __shared__ uint8_t far[kMaxWarps];
   using C = Chunk<T, kVec>;
@@ -748,10 +753,6 @@ Shape shape_of(int C, int esz, bool vec, bool backward) {
   }
   return s;
 }
-// Threads of all CTAs of an SM, by the registers that a thread takes (the kernels' launch bounds), and CTAs of `threads`.
-constexpr int fwd_threads(int per, int vec) { return per <= (vec == 1 ? 8 : 2) ? 1024 : 512; }
-constexpr int bwd_threads(int elements) { return elements <= 8 ? 1024 : elements <= 16 ? 768 : 512; }
-constexpr int ctas_of(int all, int threads) { return all < threads ? 1 : all / threads; }
 
 int check(const nb200_rms_norm_params* p, const char* what) {
   if (!p || p->struct_size != sizeof(nb200_rms_norm_params)) { set_error("%s: NULL params or wrong struct_size", what); return NB200_ERR_INVALID; }
